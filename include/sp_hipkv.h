@@ -218,6 +218,117 @@ int  sp_hipkv_check_model(const void *qm_opaque, long long out[8]);
 /* Bytes of model weights resident in HBM and KV bytes per token per layer. */
 int  sp_hipkv_info(const sp_kvdecode_handle *h, long long out[8]);
 
+/* ---- operators of speculative decoding on device memory ----
+ * For programs that keep K/V in this library's page layout themselves, and run
+ * by sp_hipkv_tree_step, sp_hipkv_tree_keep and sp_hipkv_score on a handle's
+ * own cache.  No counterpart in the reference (its decode takes one token).
+ *
+ * A page holds 64 positions of one layer: K [n_kv_heads][64] rows, then V the
+ * same.  A page table is an array of page addresses, entry p / 64 (of a ring:
+ * p / 64 % ring_pages) for position p.  Rows of head_dim values:
+ *   SP_HIPKV_ROWS_F32     f32
+ *   SP_HIPKV_ROWS_EXACT   int32, k and v as rne(x 2^16), |v| below 2^23
+ *   SP_HIPKV_ROWS_SPINOR  head_dim int8 codes, then one f32 multiplier for each
+ *                         of the ceil(head_dim / 55) chunks, padded to 16 bytes
+ *
+ * Every pointer in an argument block is device memory of the device that
+ * `stream` (a hipStream_t; NULL: the current device's null stream) belongs to;
+ * the current device may be another one.  A call reads the block, enqueues its
+ * kernels on the stream and returns: it allocates nothing, waits for nothing and
+ * can be captured into a graph.  It keeps nothing: `work` is only used between
+ * the call's own kernels, so calls in one stream order may share it, and calls
+ * (or graphs) that may run at the same time need one each.  Arguments outside
+ * the stated limits fail with nothing enqueued.  Limits on what the device arrays
+ * hold are the caller's to keep; an array that breaks them gives wrong values,
+ * and only page addresses can make a kernel read outside the memory it was given. */
+enum { SP_HIPKV_ROWS_F32 = 0, SP_HIPKV_ROWS_EXACT = 1, SP_HIPKV_ROWS_SPINOR = 2 };
+
+/* Attention of drafted tokens (nodes) that follow a sequence's cached positions,
+ * many sequences at once.  Node j of a sequence has its K/V rows at position
+ * cached + j already, and q after norm and rotation.  It attends
+ *   - the cached positions [max(0, cached + depth - window + 1), cached), and
+ *   - the nodes of its sequence whose bit is set in its row of `visible`
+ *     (itself and its ancestors in a tree; the window does not clear bits):
+ *   out = sum_p softmax_p(scale q.k_p) v_p          in f32
+ * or, for exact rows, with the integer arithmetic of exact mode (bit for bit what
+ * a decode step computes on the same rows; |q| below 2^15, |scores| below 2^17).  Nodes that see no position get zeros.  Rows
+ * that a node does not see do not reach it whatever they hold. */
+typedef struct sp_hipkv_tree_args {
+    int32_t n_heads, n_kv_heads;    /* at most 16 q heads for each kv head */
+    int32_t head_dim;               /* 64, 128 or 256 */
+    int32_t rows;                   /* SP_HIPKV_ROWS_* */
+    int32_t n_seqs, n_nodes;        /* sequences (at most 65535), nodes of all of them */
+    int32_t max_nodes;              /* no sequence has more (at most 512) */
+    int32_t max_positions;          /* cached + nodes of no sequence is more (at most 2^20; exact rows 2^18) */
+    int32_t window;                 /* 0: every cached position */
+    int32_t ring_pages;             /* 0: full tables */
+    int32_t mask_words;             /* 64-bit words in a row of visible, at least max_nodes / 64 rounded up */
+    float   scale;                  /* 1 / sqrt(head_dim) in the models served */
+    const int32_t  *node_start;     /* [n_seqs + 1] ascending: nodes node_start[s] .. belong to sequence s */
+    const int32_t  *cached;         /* [n_seqs] positions before the tree */
+    const int32_t  *depth;          /* [n_nodes] a node's position less cached (0 for a root); NULL without a window */
+    const uint64_t *visible;        /* [n_nodes][mask_words], bit j: node j of the same sequence */
+    const void *const *const *tables;   /* [n_seqs] page tables */
+    const float *q;                 /* [n_nodes][q_stride], head h at h * head_dim; 16-byte aligned, stride a multiple of 4 */
+    int64_t q_stride;
+    float *out;                     /* as q */
+    int64_t out_stride;
+    void *work;                     /* sp_hipkv_tree_attention_work bytes, 16-byte aligned */
+    size_t work_bytes;
+} sp_hipkv_tree_args;
+int  sp_hipkv_tree_attention(const sp_hipkv_tree_args *a, void *stream);
+/* Bytes of `work` for these sizes (the pointers are not looked at).  The number
+ * of parts that a long span is cut into, and with it the order of the f32 sums,
+ * goes by the sizes in the block, never by the contents of the arrays. */
+int  sp_hipkv_tree_attention_work(const sp_hipkv_tree_args *a, size_t *bytes);
+
+/* Of each row of logits, with y = scale x and p = softmax(y): log p of given
+ * tokens, the entropy -sum p log p (nats), log sum exp y, and the n_top largest
+ * logits' tokens (ties: the lowest token first) with their log p.  -inf logits
+ * have p = 0.  A given token outside [0, vocab) gets NaN.  A row with a NaN or
+ * +inf logit, or with nothing above -inf, has NaN for every value but lse (NaN, or
+ * +inf, or -inf); its top tokens are still those of the largest logits, a NaN
+ * counting as larger than any number.  f32 sums without the largest term, which is
+ * 1 exactly: entropies near 0 keep their relative precision. */
+typedef struct sp_hipkv_logprob_args {
+    int32_t n_rows, vocab;          /* at most 65535 rows, 2^24 tokens */
+    int32_t n_given, n_top;         /* given tokens of a row (at most 64), alternatives (at most 32 and vocab) */
+    float   scale;                  /* 1 / temperature, positive and finite */
+    const float *logits;            /* [n_rows][stride], any 4-byte alignment */
+    int64_t stride;
+    const int32_t *given;           /* [n_rows][n_given]; NULL if n_given is 0 */
+    float *given_logprob;           /* [n_rows][n_given]; NULL if n_given is 0 */
+    float *entropy, *lse;           /* [n_rows]; NULL: not wanted */
+    int32_t *top_ids;               /* [n_rows][n_top]; NULL if n_top is 0 */
+    float *top_logprob;             /* [n_rows][n_top]; NULL: not wanted */
+    void *work;                     /* sp_hipkv_token_logprobs_work bytes, 16-byte aligned */
+    size_t work_bytes;
+} sp_hipkv_logprob_args;
+int  sp_hipkv_token_logprobs(const sp_hipkv_logprob_args *a, void *stream);
+int  sp_hipkv_token_logprobs_work(const sp_hipkv_logprob_args *a, size_t *bytes);
+
+/* Keep the accepted nodes of drafted trees: in every table of sequence s, the K and
+ * V rows of position cached[s] + keep[i] move to cached[s] + i for the sequence's
+ * list keep[keep_start[s]] .., strictly ascending node numbers.  In place, any
+ * number of layers and sequences in one launch; other rows stay as they are.
+ * Entries that do not ascend, and positions from max_positions on, are left out.
+ * No two tables may hold the same page. */
+typedef struct sp_hipkv_keep_args {
+    int32_t n_kv_heads;
+    int32_t row_bytes;              /* of one stored row, a multiple of 16 */
+    int32_t n_tables;               /* layers x sequences */
+    int32_t n_seqs;
+    int32_t max_keep;               /* no list is longer (at most 512) */
+    int32_t max_positions;          /* every table holds this many positions (a ring: any number) */
+    const void *const *const *tables;   /* [n_tables] page tables; pages 16-byte aligned */
+    const int32_t *seq;             /* [n_tables] the table's sequence; NULL: table i is sequence i % n_seqs */
+    const int32_t *ring_pages;      /* [n_tables] 0: full table; NULL: all full */
+    const int32_t *cached;          /* [n_seqs] */
+    const int32_t *keep_start;      /* [n_seqs + 1] ascending */
+    const int32_t *keep;            /* node numbers */
+} sp_hipkv_keep_args;
+int  sp_hipkv_keep_rows(const sp_hipkv_keep_args *a, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

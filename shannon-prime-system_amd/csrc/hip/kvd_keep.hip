@@ -1,0 +1,82 @@
+// kvd_keep.hip -- keeping the accepted nodes of drafted token trees: rows
+// cached + keep[i] -> cached + i of K and V, in place.
+//
+// The moves of one (table, K or V, kv head) overlap: the place of a later row
+// may hold an earlier one's source.  A thread owns 16 bytes of every row of such a
+// slice and takes the list in order, 8 rows at a time, all loads before the
+// stores; since keep ascends, keep[i] >= i, and a row is read before or with the
+// batch that writes over it.  Threads share nothing, so there is no barrier.
+#include "kvd_op.h"
+
+namespace kvd {
+
+namespace {
+
+constexpr int KEEP_BATCH = 8;
+
+__device__ __forceinline__ uint8_t *keep_row(const sp_hipkv_keep_args &a, const void *const *table, int ring, int pos, size_t slice) {
+    const int lp = pos / PAGE;
+    return (uint8_t *)gmem(table)[ring ? lp % ring : lp] + (slice * PAGE + (pos & (PAGE - 1))) * (size_t)a.row_bytes;
+}
+
+// grid (pieces of a row / 64, K and V slices, tables)
+__global__ __launch_bounds__(64) void k_keep(sp_hipkv_keep_args a) {
+    const int piece = blockIdx.x * 64 + threadIdx.x;
+    if (piece >= a.row_bytes / 16) return;
+    for (int t = blockIdx.z; t < a.n_tables; t += gridDim.z) {
+        const int s = a.seq ? a.seq[t] : t % a.n_seqs;
+        if (s < 0 || s >= a.n_seqs) continue;
+        const int k0 = a.keep_start[s], n = min(a.keep_start[s + 1] - k0, a.max_keep), base = a.cached[s];
+        const int ring = a.ring_pages ? a.ring_pages[t] : 0;
+        if (base < 0 || base >= a.max_positions) continue;
+        const void *const *table = a.tables[t];
+        int last = -1;
+        for (int i0 = 0; i0 < n; i0 += KEEP_BATCH) {
+            uint4 x[KEEP_BATCH];
+            bool ok[KEEP_BATCH];
+            #pragma unroll
+            for (int u = 0; u < KEEP_BATCH; u++) {
+                const int i = i0 + u, k = i < n ? a.keep[k0 + i] : -1;
+                ok[u] = k > last && k >= i && k < a.max_positions - base;
+                if (ok[u]) {
+                    last = k;
+                    ok[u] = k != i;
+                    if (ok[u]) x[u] = gmem((const uint4 *)keep_row(a, table, ring, base + k, blockIdx.y))[piece];
+                }
+            }
+            #pragma unroll
+            for (int u = 0; u < KEEP_BATCH; u++)
+                if (ok[u]) gmem((uint4 *)keep_row(a, table, ring, base + i0 + u, blockIdx.y))[piece] = x[u];
+        }
+    }
+}
+
+int keep_check(const sp_hipkv_keep_args *a) {
+    const char *who = "sp_hipkv_keep_rows";
+    OP_NEED(a, "null arguments");
+    OP_NEED(a->n_kv_heads > 0 && a->n_kv_heads <= 32767, "n_kv_heads outside [1, 32767]");
+    OP_NEED(a->row_bytes > 0 && a->row_bytes % 16 == 0, "row_bytes is not a positive multiple of 16");
+    OP_NEED(a->n_tables >= 0 && a->n_seqs >= 0 && (a->n_seqs > 0 || a->n_tables == 0), "negative n_tables or n_seqs, or tables without a sequence");
+    OP_NEED(a->max_keep >= 0 && a->max_keep <= 512, "max_keep outside [0, 512]");
+    OP_NEED(a->max_positions >= 0, "negative max_positions");
+    OP_NEED(a->n_tables == 0 || a->max_keep == 0 || (a->tables && a->cached && a->keep_start && a->keep), "null array");
+    return 0;
+}
+
+}  // namespace
+
+void launch_keep(const sp_hipkv_keep_args &a, hipStream_t s) {
+    const dim3 grid((a.row_bytes / 16 + 63) / 64, 2 * a.n_kv_heads, a.n_tables < 65535 ? a.n_tables : 65535);
+    hipLaunchKernelGGL(k_keep, grid, dim3(64), 0, s, a);
+}
+
+}  // namespace kvd
+
+extern "C" int sp_hipkv_keep_rows(const sp_hipkv_keep_args *a, void *stream) {
+    using namespace kvd;
+    if (keep_check(a)) return 1;
+    if (!a->n_tables || !a->max_keep) return 0;
+    OpDevice dev((hipStream_t)stream);
+    if (dev.err == hipSuccess) launch_keep(*a, (hipStream_t)stream);
+    return op_done("sp_hipkv_keep_rows", dev);
+}

@@ -44,6 +44,34 @@ class DispatchTable(ctypes.Structure):
                 ("rewind", c_void_p), ("position", c_void_p), ("close", c_void_p)]
 
 
+ROWS_F32, ROWS_EXACT, ROWS_SPINOR = 0, 1, 2     # SP_HIPKV_ROWS_* (include/sp_hipkv.h)
+
+
+class TreeArgs(ctypes.Structure):
+    """sp_hipkv_tree_args (include/sp_hipkv.h); addresses of device memory as int."""
+    _fields_ = [("n_heads", c_int32), ("n_kv_heads", c_int32), ("head_dim", c_int32), ("rows", c_int32),
+                ("n_seqs", c_int32), ("n_nodes", c_int32), ("max_nodes", c_int32), ("max_positions", c_int32),
+                ("window", c_int32), ("ring_pages", c_int32), ("mask_words", c_int32), ("scale", c_float),
+                ("node_start", c_void_p), ("cached", c_void_p), ("depth", c_void_p), ("visible", c_void_p),
+                ("tables", c_void_p), ("q", c_void_p), ("q_stride", ctypes.c_int64), ("out", c_void_p),
+                ("out_stride", ctypes.c_int64), ("work", c_void_p), ("work_bytes", c_size_t)]
+
+
+class LogprobArgs(ctypes.Structure):
+    """sp_hipkv_logprob_args (include/sp_hipkv.h)."""
+    _fields_ = [("n_rows", c_int32), ("vocab", c_int32), ("n_given", c_int32), ("n_top", c_int32), ("scale", c_float),
+                ("logits", c_void_p), ("stride", ctypes.c_int64), ("given", c_void_p), ("given_logprob", c_void_p),
+                ("entropy", c_void_p), ("lse", c_void_p), ("top_ids", c_void_p), ("top_logprob", c_void_p),
+                ("work", c_void_p), ("work_bytes", c_size_t)]
+
+
+class KeepArgs(ctypes.Structure):
+    """sp_hipkv_keep_args (include/sp_hipkv.h)."""
+    _fields_ = [("n_kv_heads", c_int32), ("row_bytes", c_int32), ("n_tables", c_int32), ("n_seqs", c_int32),
+                ("max_keep", c_int32), ("max_positions", c_int32), ("tables", c_void_p), ("seq", c_void_p),
+                ("ring_pages", c_void_p), ("cached", c_void_p), ("keep_start", c_void_p), ("keep", c_void_p)]
+
+
 _l1 = None
 _kv = None
 
@@ -134,6 +162,10 @@ def kv():
         _sig(lib, "sp_hipkv_v_clamps", c_int, [c_void_p, ctypes.POINTER(c_longlong)])
         _sig(lib, "sp_hipkv_set_recall", c_int, [c_void_p, c_int, c_int, c_int, c_int])
         _sig(lib, "sp_hipkv_read_recall_sidecar", c_int, [c_void_p, c_int, c_int, c_int, c_void_p])
+        for op, args in (("tree_attention", TreeArgs), ("token_logprobs", LogprobArgs), ("keep_rows", KeepArgs)):
+            _sig(lib, "sp_hipkv_" + op, c_int, [ctypes.POINTER(args), c_void_p])
+        _sig(lib, "sp_hipkv_tree_attention_work", c_int, [ctypes.POINTER(TreeArgs), ctypes.POINTER(c_size_t)])
+        _sig(lib, "sp_hipkv_token_logprobs_work", c_int, [ctypes.POINTER(LogprobArgs), ctypes.POINTER(c_size_t)])
         _kv = lib
     return _kv
 
@@ -151,6 +183,35 @@ def ptr(a):
 def check(rc, what):
     if rc != 0:
         raise RuntimeError(f"{what} failed ({rc}): {last_error()}")
+
+
+# ---------------------------------------------------------------- operators on device memory
+# (include/sp_hipkv.h; stream: a hipStream_t as int, 0 the null stream)
+def tree_attention(args, stream=0):
+    """Attention of drafted tokens over the paged cache (sp_hipkv_tree_attention)."""
+    check(kv().sp_hipkv_tree_attention(args, stream), "sp_hipkv_tree_attention")
+
+
+def tree_attention_work(args):
+    n = c_size_t()
+    check(kv().sp_hipkv_tree_attention_work(args, ctypes.byref(n)), "sp_hipkv_tree_attention_work")
+    return n.value
+
+
+def token_logprobs(args, stream=0):
+    """Log probabilities of given tokens, entropy, alternatives (sp_hipkv_token_logprobs)."""
+    check(kv().sp_hipkv_token_logprobs(args, stream), "sp_hipkv_token_logprobs")
+
+
+def token_logprobs_work(args):
+    n = c_size_t()
+    check(kv().sp_hipkv_token_logprobs_work(args, ctypes.byref(n)), "sp_hipkv_token_logprobs_work")
+    return n.value
+
+
+def keep_rows(args, stream=0):
+    """Move the accepted nodes' K/V rows into place (sp_hipkv_keep_rows)."""
+    check(kv().sp_hipkv_keep_rows(args, stream), "sp_hipkv_keep_rows")
 
 
 # ---------------------------------------------------------------- synthetic inputs
