@@ -142,6 +142,34 @@ sp_status sp_hipkv_attach(sp_session *s, int pmax, int exact);
 int  sp_hipkv_decode_batch(sp_kvdecode_handle *const *hs, int n, const int32_t *tokens, float *logits,
                            int32_t *next_tokens);
 
+/* ---- speculative decoding (no counterpart in the reference) ----
+ * One step over a tree of n drafted tokens behind the resident position: node i
+ * continues node parents[i] (an earlier node; -1: the resident context).  Each
+ * weight matrix is read once for all nodes; each node attends the context and its
+ * ancestors.  logits: n x vocab rows (may be NULL), row i the distribution after
+ * node i; next_tokens: their greedy tokens (lowest on ties, may be NULL); logprob
+ * (may be NULL): log p of each node's own token after its parent, NaN for roots.
+ * In exact mode every row is bit for bit what decode steps along the node's path
+ * give; in float mode the sums' order differs.  The position stays: the nodes are
+ * pending, until sp_hipkv_tree_keep takes a path of them or any other call writes
+ * or rewinds.  A window ring takes what a prefill pass does; stored nodes count
+ * as written positions for later rewinds.  Fails, with nothing changed, with recall
+ * on, or for model shapes without the batched path. */
+#define SP_HIPKV_TREE_MAX 128
+int  sp_hipkv_tree_step(sp_kvdecode_handle *h, const int32_t *tokens, const int32_t *parents, int n, float *logits,
+                        int32_t *next_tokens, float *logprob);
+/* Keep a path of the pending tree: nodes[0] a root, each further node a child of
+ * the one before.  Their K/V move into place and the position advances by n; the
+ * other nodes are dropped.  n = 0 drops the tree. */
+int  sp_hipkv_tree_keep(sp_kvdecode_handle *h, const int32_t *nodes, int n);
+/* Prefill n tokens (the same K/V as sp_hipkv_prefill in passes of 128) and say of
+ * the distribution after each: log p of given[i] (-1: NaN; given NULL: the next of
+ * the tokens, NaN after the last), its entropy in nats, and the n_top (at most 32)
+ * likeliest tokens with their log p, [n][n_top].  Outputs may be NULL; the logits
+ * stay on the device.  Fails for model shapes without the batched path. */
+int  sp_hipkv_score(sp_kvdecode_handle *h, const int32_t *tokens, const int32_t *given, int n, int n_top, float *logprob,
+                    float *entropy, int32_t *top_tokens, float *top_logprob);
+
 /* ---- device-resident driver entry points (bench / tests) ---- */
 /* n greedy steps entirely on the device (argmax feeds the next token, no host
  * round trip), starting with `first_token` at dpos; writes the n generated

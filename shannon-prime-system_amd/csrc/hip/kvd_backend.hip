@@ -13,6 +13,7 @@
 #include "kvd_internal.h"
 #include "kvd_batch.h"
 #include "kvd_spinor.h"
+#include "kvd_op.h"
 #include <hip/hip_runtime.h>
 #include <algorithm>
 #include <cmath>
@@ -497,6 +498,13 @@ struct StepScratch {
 
 }  // namespace
 
+// The small arrays that the tree operators read (include/sp_hipkv.h).
+constexpr int TREE_MAX = SP_HIPKV_TREE_MAX, TREE_WORDS = TREE_MAX / 64;
+struct TreeBuf {
+    uint64_t visible[2][TREE_MAX][TREE_WORDS];   // full-context layers, window layers
+    int depth[TREE_MAX], keep[TREE_MAX], node_start[2], cached, keep_start[2];
+};
+
 // ------------------------------------------------------------ the handle
 struct sp_kvdecode_handle {
     DevModel *m = nullptr;
@@ -554,6 +562,12 @@ struct sp_kvdecode_handle {
     void *scratch = nullptr;
     int built = 0;                           // tables and scratch allocated (reusable as a shell)
     Batch b;                                 // leased for the duration of a batched call (BatchLease)
+    // a drafted tree behind dpos (sp_hipkv_tree_step): its nodes' parents, until
+    // they are kept or anything else is written or rewound
+    int tree[TREE_MAX], tree_n = 0;
+    struct TreeBuf *d_tree = nullptr, *h_tree = nullptr;   // arrays of the tree operators, and their pinned mirror
+    float *const **d_lists = nullptr, *const **h_lists = nullptr;   // ... the layers' page tables
+    int *d_rings = nullptr, *h_rings = nullptr;            // ... and ring sizes
     // graph cache: key (logits?, argmax?, grid_global, grid_local, chunk_global)
     struct GKey { int lg, am, gg, gl, cg, rt; bool operator<(const GKey &o) const {
         return std::tie(lg, am, gg, gl, cg, rt) < std::tie(o.lg, o.am, o.gg, o.gl, o.cg, o.rt); } };
@@ -601,6 +615,7 @@ std::shared_ptr<KvPool> make_pool(const DevModel *m, int mode, int kvc, int grow
 
 int build_tables(sp_kvdecode_handle *h) {
     const DevModel *m = h->m;
+    h->hwm = 0; h->tree_n = 0;
     h->full_pages = (h->pmax + PAGE - 1) / PAGE;
     h->ring_pages = h->max_rewind > 0 ? std::min(h->full_pages, (m->SW + h->max_rewind + PAGE - 1) / PAGE + 1) : 0;
     h->pt.assign(m->NL, {});
@@ -632,6 +647,7 @@ int build_tables(sp_kvdecode_handle *h) {
 int ensure_pages(sp_kvdecode_handle *h, int p0, int p1, bool may_grow = true) {
     const DevModel *m = h->m;
     if (p1 <= p0) return 0;
+    h->tree_n = 0;                               // a pending tree's places are about to be written
     std::lock_guard<std::mutex> lk(h->pool->mu);
     KvPool &pool = *h->pool;
     const int lp0 = p0 / PAGE, lp1 = (p1 - 1) / PAGE;
@@ -772,7 +788,8 @@ int alloc_scratch(sp_kvdecode_handle *h) {
         {(void **)&h->vacc, (size_t)QD * 8 * VREP}, {(void **)&h->vacc_s, (size_t)m->NH * 8 * VREP},
         {(void **)&h->d_st, sizeof(DState) * 4}, {(void **)&h->vclamp, 64},
         {(void **)&h->stats, (size_t)m->NL * STAT_PER_LAYER * STAT_REP * sizeof(VecStat)},
-        {(void **)&h->ss.wslot, window_slots(m)},
+        {(void **)&h->ss.wslot, window_slots(m)}, {(void **)&h->d_tree, sizeof(TreeBuf)},
+        {(void **)&h->d_lists, (size_t)m->NL * sizeof(void *)}, {(void **)&h->d_rings, (size_t)m->NL * 4},
     };
     size_t tot = 0;
     for (auto &it : items) tot = align_up(tot + it.n, 256);
@@ -788,6 +805,11 @@ int alloc_scratch(sp_kvdecode_handle *h) {
     if (!window_slots(m)) h->ss.wslot = nullptr;
     HIPCHK(hipHostMalloc(&h->h_st, sizeof(DState) * 4, hipHostMallocDefault), "pinned state alloc");
     HIPCHK(hipHostMalloc(&h->h_logits, (size_t)m->V * 4, hipHostMallocDefault), "pinned logits alloc");
+    // the mirror of d_tree, d_lists and d_rings, laid out as they are
+    const size_t span = (size_t)((uint8_t *)(h->d_rings + m->NL) - (uint8_t *)h->d_tree);
+    HIPCHK(hipHostMalloc(&h->h_tree, span, hipHostMallocDefault), "pinned tree arrays alloc");
+    h->h_lists = (float *const **)((uint8_t *)h->h_tree + ((uint8_t *)h->d_lists - (uint8_t *)h->d_tree));
+    h->h_rings = (int *)((uint8_t *)h->h_tree + ((uint8_t *)h->d_rings - (uint8_t *)h->d_tree));
     h->built = 1;
     return 0;
 }
@@ -797,6 +819,7 @@ int alloc_scratch(sp_kvdecode_handle *h) {
 void set_handle_mode(sp_kvdecode_handle *h, int mode) {
     if (h->mode == mode) return;
     h->mode = mode;
+    h->tree_n = 0;
     free_graphs(h);
 }
 
@@ -837,6 +860,7 @@ std::vector<uint32_t> recall_sign_bits(int r, int HD) {
 // set holds at most max(B, W + sink) positions (and at most pmax).
 int alloc_recall(sp_kvdecode_handle *h, int B, int W, int sink, int r) {
     free_recall(h);
+    h->tree_n = 0;
     if (B <= 0) return 0;
     const DevModel *m = h->m;
     auto &R = h->rec;
@@ -918,6 +942,7 @@ void free_handle(sp_kvdecode_handle *h) {
     if (h->scratch) hipFree(h->scratch);
     if (h->h_st) hipHostFree(h->h_st);
     if (h->h_logits) hipHostFree(h->h_logits);
+    if (h->h_tree) hipHostFree(h->h_tree);
     if (h->stream) hipStreamDestroy(h->stream);
     delete h;
 }
@@ -1167,7 +1192,13 @@ int alloc_batch(sp_kvdecode_handle *h) {
 // prefill: positions pos0.., tokens in h->tokbuf, h's page tables.  Several
 // sessions' decode (multi): token t's id, position and page tables come from
 // b.toks / b.tpos / b.tpages; then the LM head writes b.logits and b.next.
-int run_batch(sp_kvdecode_handle *h, int T, int pos0, int pos_hi, bool multi, TimeCb cb = nullptr, void *ctx = nullptr) {
+// TREE: one session's drafted nodes, stored at positions pos0.. and rotated for
+// b.tpos (tokens in b.toks); SCORE: a prefill; both with the LM head's logits.
+enum BatchKind { PREFILL, MULTI, TREE, SCORE };
+bool tree_attention(sp_kvdecode_handle *h, const AttnArgs &a, int layer, hipStream_t s);
+
+int run_batch(sp_kvdecode_handle *h, int T, int pos0, int pos_hi, BatchKind kind, TimeCb cb = nullptr, void *ctx = nullptr) {
+    const bool multi = kind == MULTI, own_pos = multi || kind == TREE;
     const DevModel *m = h->m;
     auto &b = h->b;
     hipStream_t s = h->stream;
@@ -1176,7 +1207,7 @@ int run_batch(sp_kvdecode_handle *h, int T, int pos0, int pos_hi, bool multi, Ti
     auto tp = [&](bool fold) { return fold ? (T + 15) / 16 * 16 : (T + 31) / 32 * 32; };
     auto TM = [&](int cls, bool begin) { if (cb) cb(ctx, cls, begin); };
     TM(8, true);
-    launch_embed_rope_batch(m->embd, h->tokbuf, pos0, multi ? b.toks : nullptr, multi ? b.tpos : nullptr, T, b.x1,
+    launch_embed_rope_batch(m->embd, h->tokbuf, pos0, own_pos ? b.toks : nullptr, own_pos ? b.tpos : nullptr, T, b.x1,
                             m->gemma ? sqrtf((float)m->E) : 0.0f, m->HD, h->mode,
                             m->freq_global, m->gemma ? m->freq_local : m->freq_global, b.rope, s);
     TM(8, false);
@@ -1223,7 +1254,7 @@ int run_batch(sp_kvdecode_handle *h, int T, int pos0, int pos_hi, bool multi, Ti
             a.tpos = b.tpos; a.tpages = b.tpages + (size_t)l * b.TB;
             if (glob || a.win < 0) { a.work = b.work; a.nwork = b.nwork; }
         }
-        else if (h->rec.B > 0 && a.win < 0) {                   // prefill: the sidecar
+        else if (kind != TREE && h->rec.B > 0 && a.win < 0) {   // prefill: the sidecar
             a.rec_R = h->rec.Rb; a.rec_r = h->rec.r; a.rec_side = side_of(h, l);
         }
         // batched decode over sessions: the longest chunks the kernels take,
@@ -1236,7 +1267,9 @@ int run_batch(sp_kvdecode_handle *h, int T, int pos0, int pos_hi, bool multi, Ti
         // by the handle's own pmax, not the leased set's (no smaller): a call's
         // sums must not depend on what other sessions left
         if (!multi) a.part_slots = b.TB * (h->pmax / 64 + 2);
-        if (prefill_attention_float(a)) launch_prefill_float(a, s);
+        if (kind == TREE) {
+            if (!tree_attention(h, a, l, s)) return fail("sp_hipkv_tree_step: the attention's work does not fit the batch buffers%s");
+        } else if (prefill_attention_float(a)) launch_prefill_float(a, s);
         else for (int t = 0; t < T; t += b.TB) {                // one pass for a batched decode
             AttnArgs c = a;
             c.q += (size_t)t * QD; c.k += (size_t)t * KVD; c.v += (size_t)t * KVD; c.qr += (size_t)t * QD; c.ao += (size_t)t * QD;
@@ -1271,14 +1304,14 @@ int run_batch(sp_kvdecode_handle *h, int T, int pos0, int pos_hi, bool multi, Ti
         launch_gemm(dd, m->E, s);
         TM(3, false);
     }
-    if (multi) {
+    if (kind != PREFILL) {
         // LM head over the T rows, then each row's greedy token
         TM(4, true);
         stage(PRO_RESID, b.x0, b.dn, m->gemma ? m->L[m->NL - 1].post_ffw : nullptr, m->out_norm, nullptr, m->E, gemm_folds(m->out));
         GemmArgs lm = gemm(m->E, gemm_folds(m->out));
         lm.nseg = 1; lm.seg[0] = {m->out, b.logits};
         launch_gemm(lm, m->V, s);
-        launch_argmax_rows(b.logits, m->V, T, b.next, s);
+        if (kind != SCORE) launch_argmax_rows(b.logits, m->V, T, b.next, s);
         TM(4, false);
     }
     if (take_launch_error("batched pass")) return 1;
@@ -1286,7 +1319,93 @@ int run_batch(sp_kvdecode_handle *h, int T, int pos0, int pos_hi, bool multi, Ti
     return 0;
 }
 
-int prefill_batch(sp_kvdecode_handle *h, int pos0, int T) { return run_batch(h, T, pos0, pos0 + T - 1, false); }
+int prefill_batch(sp_kvdecode_handle *h, int pos0, int T) { return run_batch(h, T, pos0, pos0 + T - 1, PREFILL); }
+
+// The prefill passes' limit on window layers in a ring: writing position q reuses
+// the page slot of the page ring_pages back, i.e. drops positions up to
+// q - ring*PAGE + PAGE-1; a batch must not drop positions its first token still
+// attends to
+int ring_batch(const sp_kvdecode_handle *h, int most) {
+    if (h->ring_pages > 0) most = std::min(most, h->ring_pages * PAGE - h->m->SW - (PAGE - 1));
+    return std::max(most, 1);
+}
+
+// One layer's attention of a drafted tree: the scratch of the batch's attention as its work.
+bool tree_attention(sp_kvdecode_handle *h, const AttnArgs &a, int layer, hipStream_t s) {
+    const DevModel *m = h->m;
+    const auto &b = h->b;
+    TreeBuf *d = h->d_tree;
+    sp_hipkv_tree_args t{};
+    t.n_heads = a.NH; t.n_kv_heads = a.NKV; t.head_dim = a.HD;
+    t.rows = a.mode == EXACT ? SP_HIPKV_ROWS_EXACT : a.kvc == KVC_SPINOR ? SP_HIPKV_ROWS_SPINOR : SP_HIPKV_ROWS_F32;
+    t.n_seqs = 1; t.n_nodes = t.max_nodes = a.nt; t.max_positions = a.pos0 + a.nt;
+    t.window = a.win >= 0 ? a.win : 0; t.ring_pages = a.ring_pages; t.mask_words = TREE_WORDS; t.scale = a.ascale;
+    t.node_start = d->node_start; t.cached = &d->cached; t.depth = d->depth; t.visible = &d->visible[a.win >= 0][0][0];
+    t.tables = (const void *const *const *)(h->d_lists + layer);
+    t.q = a.qr; t.out = a.ao; t.q_stride = t.out_stride = (int64_t)a.NH * a.HD;
+    size_t need = 0;
+    if (sp_hipkv_tree_attention_work(&t, &need)) return false;
+    t.work = a.mode == EXACT ? (void *)b.zs : (void *)b.part;
+    t.work_bytes = need;
+    const size_t room = a.mode == EXACT ? (size_t)b.TB * m->NH * h->max_chunks * 16 * 4 : (size_t)b.TB * m->NH * (h->pmax / 64 + 2) * m->HD * 4;
+    if (need > room) return false;
+    launch_tree(t, s);
+    return true;
+}
+
+// The batched decode's buffers of the leased set: logits rows, tokens, positions, tables.
+int alloc_decode(sp_kvdecode_handle *h) {
+    const DevModel *m = h->m;
+    auto &b = h->b;
+    const int TB = b.TB;
+    if (b.dbuf) return 0;
+    const size_t lb = (size_t)TB * m->V * 4, nb = (size_t)TB * 4, pb = (size_t)m->NL * TB * sizeof(void *);
+    b.wcap = TB * (b.pmax / ATTN_MAXCH + 2);                 // the set outlives this call: its own pmax
+    const size_t wb = (size_t)b.wcap * sizeof(int2), up = 2 * nb + pb + wb;
+    // pinned staging: the upload block, the tokens, the logits' slots
+    // (allocated before dbuf, which marks both as present)
+    if (!b.hstage) HIPCHK(hipHostMalloc(&b.hstage, align_up(up, 4096) + align_up(nb, 4096) + LOGIT_SLOTS * LOGIT_SLOT_BYTES,
+                                        hipHostMallocDefault), "batch decode staging");
+    b.hnext = (int *)((uint8_t *)b.hstage + align_up(up, 4096));
+    b.hslots = (uint8_t *)b.hnext + align_up(nb, 4096);
+    for (hipEvent_t &e : b.slot_ev) if (!e) HIPCHK(hipEventCreateWithFlags(&e, hipEventDisableTiming), "batch decode event");
+    HIPCHK(dev_malloc(&b.dbuf, align_up(lb, 256) + align_up(nb, 256) + up), "batch decode alloc");
+    uint8_t *p = (uint8_t *)b.dbuf;
+    b.logits = (float *)p; p += align_up(lb, 256);
+    b.next = (int *)p; p += align_up(nb, 256);
+    b.toks = (int *)p; p += nb;
+    b.tpos = (int *)p; p += nb;
+    b.tpages = (float *const **)p; p += pb;
+    b.work = (int2 *)p;
+    return 0;
+}
+
+// Log probabilities of the batch's logits rows: the arrays of the operator on the
+// device, results mirrored in pinned memory by one copy.  Order: what the call
+// reads (given), then what it writes.
+constexpr int SCORE_GIVEN = 64, SCORE_TOP = 32;
+struct Score {
+    int given[PREFILL_TB * SCORE_GIVEN];
+    float lp[PREFILL_TB * SCORE_GIVEN], entropy[PREFILL_TB], top_lp[PREFILL_TB * SCORE_TOP];
+    int top[PREFILL_TB * SCORE_TOP];
+};
+int score_args(sp_kvdecode_handle *h, int T, int n_given, int n_top, sp_hipkv_logprob_args &a) {
+    const DevModel *m = h->m;
+    auto &b = h->b;
+    a = {};
+    a.n_rows = PREFILL_TB; a.vocab = m->V; a.n_given = SCORE_GIVEN; a.n_top = std::min(SCORE_TOP, m->V); a.scale = 1.0f;
+    size_t need = 0;
+    if (sp_hipkv_token_logprobs_work(&a, &need)) return 1;
+    if (!b.hsbuf) HIPCHK(hipHostMalloc(&b.hsbuf, sizeof(Score), hipHostMallocDefault), "score staging");
+    if (!b.sbuf) HIPCHK(dev_malloc(&b.sbuf, align_up(sizeof(Score), 256) + need), "score buffers alloc");
+    Score *d = (Score *)b.sbuf;
+    a.n_rows = T; a.n_given = n_given; a.n_top = n_top;
+    a.logits = b.logits; a.stride = m->V; a.given = d->given; a.given_logprob = d->lp; a.entropy = d->entropy;
+    a.top_ids = d->top; a.top_logprob = d->top_lp;
+    a.work = (uint8_t *)b.sbuf + align_up(sizeof(Score), 256);
+    if (sp_hipkv_token_logprobs_work(&a, &a.work_bytes)) return 1;
+    return 0;
+}
 
 constexpr size_t MAX_GRAPHS = 64;
 
@@ -1471,7 +1590,7 @@ void sp_hipkv_close(sp_kvdecode_handle *h) {
     DevModel *m = h->m;
     if (idle && h->built && m->refs > 1 && m->shells.size() < MAX_SHELLS) {
         // other handles keep the model alive: keep this one as a shell
-        h->dpos = 0; h->hwm = 0;
+        h->dpos = 0; h->hwm = 0; h->tree_n = 0;
         m->shells.push_back(h);
         m->refs--;
         return;
@@ -1493,6 +1612,7 @@ int sp_hipkv_rewind(sp_kvdecode_handle *h, int n) {
         if (h->hwm - (h->dpos - n) > cap)
             return fail("sp_hipkv_rewind: rewinding %s%lld positions leaves the window ring (set a larger max_rewind)", "", (long long)n);
     }
+    h->tree_n = 0;
     h->dpos -= n;          // stale slots past dpos are overwritten by the next steps
     return 0;
 }
@@ -1510,12 +1630,7 @@ int sp_hipkv_prefill(sp_kvdecode_handle *h, const int32_t *tokens, int n_tok) {
     if (h->use_batch && batch_supported(h)) {
         lease.emplace(h);
         if (alloc_batch(h)) return 1;
-        // window layers on a ring: writing position q reuses the page slot of
-        // the page ring_pages back, i.e. drops positions up to q - ring*PAGE + PAGE-1;
-        // a batch must not drop positions its first token still attends to
-        int tb = PREFILL_TG;
-        if (h->ring_pages > 0) tb = std::min(tb, h->ring_pages * PAGE - h->m->SW - (PAGE - 1));
-        if (tb < 1) tb = 1;
+        const int tb = ring_batch(h, PREFILL_TG);
         for (int i = 0; i < n_tok; i += tb)
             if (prefill_batch(h, h->dpos + i, std::min(tb, n_tok - i))) return 1;
     } else {
@@ -1594,29 +1709,9 @@ static int decode_batch_impl(sp_kvdecode_handle *const *hs, int n, const int32_t
     }
     for (int i = 0; i < n; i++) if (ensure_pages(hs[i], hs[i]->dpos, hs[i]->dpos + 1)) return 1;
     BatchLease lease(L);
-    if (alloc_batch(L)) return 1;
+    if (alloc_batch(L) || alloc_decode(L)) return 1;
     auto &b = L->b;
     const int TB = b.TB;
-    if (!b.dbuf) {
-        const size_t lb = (size_t)TB * m->V * 4, nb = (size_t)TB * 4, pb = (size_t)m->NL * TB * sizeof(void *);
-        b.wcap = TB * (b.pmax / ATTN_MAXCH + 2);             // the set outlives this call: its own pmax
-        const size_t wb = (size_t)b.wcap * sizeof(int2), up = 2 * nb + pb + wb;
-        // pinned staging: the upload block, the tokens, the logits' slots
-        // (allocated before dbuf, which marks both as present)
-        if (!b.hstage) HIPCHK(hipHostMalloc(&b.hstage, align_up(up, 4096) + align_up(nb, 4096) + LOGIT_SLOTS * LOGIT_SLOT_BYTES,
-                                            hipHostMallocDefault), "batch decode staging");
-        b.hnext = (int *)((uint8_t *)b.hstage + align_up(up, 4096));
-        b.hslots = (uint8_t *)b.hnext + align_up(nb, 4096);
-        for (hipEvent_t &e : b.slot_ev) if (!e) HIPCHK(hipEventCreateWithFlags(&e, hipEventDisableTiming), "batch decode event");
-        HIPCHK(dev_malloc(&b.dbuf, align_up(lb, 256) + align_up(nb, 256) + up), "batch decode alloc");
-        uint8_t *p = (uint8_t *)b.dbuf;
-        b.logits = (float *)p; p += align_up(lb, 256);
-        b.next = (int *)p; p += align_up(nb, 256);
-        b.toks = (int *)p; p += nb;
-        b.tpos = (int *)p; p += nb;
-        b.tpages = (float *const **)p; p += pb;
-        b.work = (int2 *)p;
-    }
     for (int g0 = 0; g0 < n; g0 += TB) {
         const int T = std::min(TB, n - g0);
         int *htok = (int *)b.hstage, *hpos = htok + TB;
@@ -1638,7 +1733,7 @@ static int decode_batch_impl(sp_kvdecode_handle *const *hs, int n, const int32_t
         // tokens, positions, page tables and work items lie in one block on both sides
         HIPCHK(hipMemcpyAsync(b.toks, htok, (size_t)((uint8_t *)(hwork + b.nwork) - (uint8_t *)htok), hipMemcpyHostToDevice,
                               L->stream), "batch upload");
-        if (run_batch(L, T, 0, pos_hi, true, cb, ctx)) return 1;
+        if (run_batch(L, T, 0, pos_hi, MULTI, cb, ctx)) return 1;
         if (next_tokens) HIPCHK(hipMemcpyAsync(b.hnext, b.next, (size_t)T * 4, hipMemcpyDeviceToHost, L->stream),
                                 "batch tokens download");
         if (logits && logits_to_host(L, logits + (size_t)g0 * m->V, (size_t)T * m->V * 4)) return 1;
@@ -1657,6 +1752,153 @@ static int decode_batch_impl(sp_kvdecode_handle *const *hs, int n, const int32_t
 int sp_hipkv_decode_batch(sp_kvdecode_handle *const *hs, int n, const int32_t *tokens, float *logits,
                           int32_t *next_tokens) {
     return decode_batch_impl(hs, n, tokens, logits, next_tokens, nullptr, nullptr);
+}
+
+// ------------------------------------------------------------ drafted trees, scores
+// (no counterpart in the reference: its decode takes one token per step)
+int sp_hipkv_tree_step(sp_kvdecode_handle *h, const int32_t *tokens, const int32_t *parents, int n, float *logits,
+                       int32_t *next_tokens, float *logprob) {
+    if (!h || !tokens || !parents) return fail("sp_hipkv_tree_step: null argument%s");
+    if (n < 1 || n > TREE_MAX) return fail("sp_hipkv_tree_step: a tree holds 1 to %s%lld nodes", "", (long long)TREE_MAX);
+    if (n > h->pmax - h->dpos) return fail("sp_hipkv_tree_step: context full%s");
+    const DevModel *m = h->m;
+    int depth[TREE_MAX], kids[TREE_MAX] = {}, nth[TREE_MAX] = {}, most = 0;
+    for (int i = 0; i < n; i++) {
+        if (check_tok(h, tokens[i])) return 1;
+        const int p = parents[i];
+        if (p < -1 || p >= i) return fail("sp_hipkv_tree_step: parents come before their children (node %s%lld)", "", (long long)i);
+        depth[i] = p < 0 ? 0 : depth[p] + 1;
+        if (p >= 0) { nth[i] = kids[p]++; most = std::max(most, kids[p]); }
+    }
+    if (logprob && most > SCORE_GIVEN) return fail("sp_hipkv_tree_step: log probabilities of at most %s%lld children of a node", "", (long long)SCORE_GIVEN);
+    if (h->rec.B > 0) return fail("sp_hipkv_tree_step: recall is on (a tree attends every position)%s");
+    if (!batch_supported(h) || !gemm_supported(m->out)) return fail("sp_hipkv_tree_step: no batched path for this model shape%s");
+    if (h->ring_pages > 0 && n > ring_batch(h, TREE_MAX))
+        return fail("sp_hipkv_tree_step: the window ring holds no more than %s%lld nodes (set a larger max_rewind)", "", (long long)ring_batch(h, TREE_MAX));
+    if (ensure_pages(h, h->dpos, h->dpos + n)) return 1;
+    h->hwm = std::max(h->hwm, h->dpos + n);
+    BatchLease lease(h);
+    if (alloc_batch(h) || alloc_decode(h)) return 1;
+    auto &b = h->b;
+    hipStream_t s = h->stream;
+    // what the operators read: a node sees itself and its ancestors, in window layers
+    // those that its window reaches
+    TreeBuf &t = *h->h_tree;
+    int *htok = (int *)b.hstage, *hpos = htok + b.TB;
+    for (int i = 0; i < n; i++) {
+        htok[i] = tokens[i]; hpos[i] = h->dpos + depth[i];
+        t.depth[i] = depth[i];
+        for (int w = 0; w < TREE_WORDS; w++) t.visible[0][i][w] = t.visible[1][i][w] = 0;
+        for (int j = i; j >= 0; j = parents[j]) {
+            t.visible[0][i][j / 64] |= (uint64_t)1 << (j % 64);
+            if (!m->gemma || depth[i] - depth[j] < m->SW) t.visible[1][i][j / 64] |= (uint64_t)1 << (j % 64);
+        }
+    }
+    t.node_start[0] = 0; t.node_start[1] = n; t.cached = h->dpos;
+    for (int l = 0; l < m->NL; l++) h->h_lists[l] = h->d_pt + h->pt_off[l];
+    HIPCHK(hipMemcpyAsync(b.toks, htok, (size_t)2 * b.TB * 4, hipMemcpyHostToDevice, s), "tree upload");
+    HIPCHK(hipMemcpyAsync(h->d_tree, h->h_tree, (size_t)((uint8_t *)(h->d_rings + m->NL) - (uint8_t *)h->d_tree), hipMemcpyHostToDevice, s),
+           "tree upload");
+    if (run_batch(h, n, h->dpos, h->dpos + n - 1, TREE)) return 1;
+    if (logprob && most) {
+        sp_hipkv_logprob_args a;
+        if (score_args(h, n, most, 0, a)) return 1;
+        Score *d = (Score *)b.sbuf, *hs = (Score *)b.hsbuf;
+        std::fill(hs->given, hs->given + n * most, -1);
+        for (int i = 0; i < n; i++) if (parents[i] >= 0) hs->given[parents[i] * most + nth[i]] = tokens[i];
+        HIPCHK(hipMemcpyAsync(d->given, hs->given, (size_t)n * most * 4, hipMemcpyHostToDevice, s), "tree upload");
+        launch_logprob(a, s);
+        HIPCHK(hipGetLastError(), "sp_hipkv_tree_step: launch");
+        HIPCHK(hipMemcpyAsync(hs->lp, d->lp, (size_t)n * most * 4, hipMemcpyDeviceToHost, s), "log probability download");
+    }
+    if (next_tokens) HIPCHK(hipMemcpyAsync(b.hnext, b.next, (size_t)n * 4, hipMemcpyDeviceToHost, s), "tree tokens download");
+    if (logits && logits_to_host(h, logits, (size_t)n * m->V * 4)) return 1;
+    HIPCHK(hipStreamSynchronize(s), "tree step");
+    if (next_tokens) memcpy(next_tokens, b.hnext, (size_t)n * 4);
+    for (int i = 0; logprob && i < n; i++)
+        logprob[i] = parents[i] < 0 ? NAN : ((Score *)b.hsbuf)->lp[parents[i] * most + nth[i]];
+    lease.done();
+    std::copy(parents, parents + n, h->tree);
+    h->tree_n = n;
+    return 0;
+}
+
+int sp_hipkv_tree_keep(sp_kvdecode_handle *h, const int32_t *nodes, int n) {
+    if (!h || n < 0 || (!nodes && n > 0)) return fail("sp_hipkv_tree_keep: bad argument%s");
+    if (!h->tree_n) return fail("sp_hipkv_tree_keep: no tree is pending%s");
+    for (int i = 0; i < n; i++)
+        if (nodes[i] < 0 || nodes[i] >= h->tree_n || h->tree[nodes[i]] != (i ? nodes[i - 1] : -1))
+            return fail("sp_hipkv_tree_keep: the nodes are no path from a root (entry %s%lld)", "", (long long)i);
+    const int pending = h->tree_n;
+    bool moves = false;
+    for (int i = 0; i < n; i++) moves |= nodes[i] != i;
+    if (moves) {
+        const DevModel *m = h->m;
+        if (ensure_pages(h, h->dpos, h->dpos + n)) { h->tree_n = pending; return 1; }       // forked since: the pages written are copied first
+        TreeBuf &t = *h->h_tree;
+        for (int i = 0; i < n; i++) t.keep[i] = nodes[i];
+        t.keep_start[0] = 0; t.keep_start[1] = n; t.cached = h->dpos;
+        for (int l = 0; l < m->NL; l++) {
+            h->h_lists[l] = h->d_pt + h->pt_off[l];
+            h->h_rings[l] = h->slots[l] == h->full_pages ? 0 : h->slots[l];
+        }
+        HIPCHK(hipMemcpyAsync(h->d_tree, h->h_tree, (size_t)((uint8_t *)(h->d_rings + m->NL) - (uint8_t *)h->d_tree), hipMemcpyHostToDevice,
+                              h->stream), "tree upload");
+        sp_hipkv_keep_args a{};
+        a.n_kv_heads = m->NKV; a.row_bytes = (int)kv_row_bytes(m, h->mode, h->kvc); a.n_tables = m->NL; a.n_seqs = 1;
+        a.max_keep = n; a.max_positions = h->dpos + pending;
+        a.tables = (const void *const *const *)h->d_lists; a.ring_pages = h->d_rings;
+        a.cached = &h->d_tree->cached; a.keep_start = h->d_tree->keep_start; a.keep = h->d_tree->keep;
+        launch_keep(a, h->stream);
+        HIPCHK(hipGetLastError(), "sp_hipkv_tree_keep: launch");
+        HIPCHK(hipStreamSynchronize(h->stream), "tree keep");
+    }
+    h->tree_n = 0;
+    h->dpos += n;
+    return 0;
+}
+
+int sp_hipkv_score(sp_kvdecode_handle *h, const int32_t *tokens, const int32_t *given, int n, int n_top, float *logprob, float *entropy,
+                   int32_t *top_tokens, float *top_logprob) {
+    if (!h || (!tokens && n > 0) || n < 0) return fail("sp_hipkv_score: bad argument%s");
+    const DevModel *m = h->m;
+    if (n_top < 0 || n_top > SCORE_TOP || n_top > m->V) return fail("sp_hipkv_score: n_top outside [0, %s%lld]", "", (long long)std::min(SCORE_TOP, m->V));
+    if (n > h->pmax - h->dpos) return fail("sp_hipkv_score: context full%s");
+    for (int i = 0; i < n; i++) {
+        if (check_tok(h, tokens[i])) return 1;
+        if (given && (given[i] < -1 || given[i] >= m->V)) return fail("sp_hipkv_score: given token %s%lld out of vocabulary range", "", (long long)given[i]);
+    }
+    if (!batch_supported(h) || !gemm_supported(m->out)) return fail("sp_hipkv_score: no batched path for this model shape%s");
+    if (n == 0) return 0;
+    if (ensure_pages(h, h->dpos, h->dpos + n)) return 1;
+    HIPCHK(hipStreamSynchronize(h->stream), "score staging");
+    HIPCHK(hipMemcpyAsync(h->tokbuf + h->dpos, tokens, (size_t)n * 4, hipMemcpyHostToDevice, h->stream), "score tokens");
+    BatchLease lease(h);
+    if (alloc_batch(h) || alloc_decode(h)) return 1;
+    auto &b = h->b;
+    hipStream_t s = h->stream;
+    const int tb = ring_batch(h, PREFILL_TB);
+    for (int i = 0; i < n; i += tb) {
+        const int T = std::min(tb, n - i);
+        sp_hipkv_logprob_args a;
+        if (score_args(h, T, 1, n_top, a)) return 1;
+        Score *d = (Score *)b.sbuf, *hs = (Score *)b.hsbuf;
+        for (int t = 0; t < T; t++) hs->given[t] = given ? given[i + t] : i + t + 1 < n ? tokens[i + t + 1] : -1;
+        HIPCHK(hipMemcpyAsync(d->given, hs->given, (size_t)T * 4, hipMemcpyHostToDevice, s), "score tokens");
+        if (run_batch(h, T, h->dpos + i, h->dpos + i + T - 1, SCORE)) return 1;
+        launch_logprob(a, s);
+        HIPCHK(hipGetLastError(), "sp_hipkv_score: launch");
+        HIPCHK(hipMemcpyAsync(hs->lp, d->lp, sizeof(Score) - offsetof(Score, lp), hipMemcpyDeviceToHost, s), "score download");
+        HIPCHK(hipStreamSynchronize(s), "score");
+        if (logprob) memcpy(logprob + i, hs->lp, (size_t)T * 4);
+        if (entropy) memcpy(entropy + i, hs->entropy, (size_t)T * 4);
+        if (top_tokens) memcpy(top_tokens + (size_t)i * n_top, hs->top, (size_t)T * n_top * 4);
+        if (top_logprob) memcpy(top_logprob + (size_t)i * n_top, hs->top_lp, (size_t)T * n_top * 4);
+    }
+    lease.done();
+    h->dpos += n;
+    h->hwm = std::max(h->hwm, h->dpos);
+    return 0;
 }
 
 int sp_hipkv_decode_batch_times(sp_kvdecode_handle *const *hs, int n, const int32_t *tokens, int32_t *next_tokens,
@@ -1789,6 +2031,7 @@ int sp_hipkv_set_kv_codec(sp_kvdecode_handle *h, int codec) {
     if (codec == KVC_SPINOR && h->mode == FLOAT && h->rec.B > 0)
         return fail("sp_hipkv_set_kv_codec: recall in float mode reads plain K/V rows (not Spinor code rows)%s");
     h->kvc = codec;
+    h->tree_n = 0;
     free_graphs(h);
     return repage(h, "sp_hipkv_set_kv_codec");
 }

@@ -38,11 +38,15 @@ struct Batch {
     int *hnext = nullptr;                // the greedy tokens
     uint8_t *hslots = nullptr;           // LOGIT_SLOTS pieces of logits on their way to the caller
     hipEvent_t slot_ev[LOGIT_SLOTS] = {};
+    // log probabilities (allocated on first use): the operator's arrays for TB rows, and their pinned mirror
+    void *sbuf = nullptr, *hsbuf = nullptr;
     bool serves(bool f, int p) const { return (flt || !f) && pmax >= p; }
     void release() {
         if (buf) hipFree(buf);
         if (dbuf) hipFree(dbuf);
         if (hstage) hipHostFree(hstage);
+        if (sbuf) hipFree(sbuf);
+        if (hsbuf) hipHostFree(hsbuf);
         for (hipEvent_t e : slot_ev) if (e) hipEventDestroy(e);
         *this = Batch{};
     }

@@ -43,6 +43,11 @@ inline int op_done(const char *who, const OpDevice &d) {
     return e == hipSuccess ? 0 : op_fail(who, hipGetErrorString(e));
 }
 
+// The operators' launches, for arguments that their entry points accept.
+void launch_tree(const sp_hipkv_tree_args &a, hipStream_t s);
+void launch_logprob(const sp_hipkv_logprob_args &a, hipStream_t s);
+void launch_keep(const sp_hipkv_keep_args &a, hipStream_t s);
+
 __host__ __device__ constexpr int row_bytes_of(int rows, int hd) { return rows == SP_HIPKV_ROWS_SPINOR ? spn_row_bytes(hd) : 4 * hd; }
 
 }  // namespace kvd

@@ -162,6 +162,9 @@ def kv():
         _sig(lib, "sp_hipkv_v_clamps", c_int, [c_void_p, ctypes.POINTER(c_longlong)])
         _sig(lib, "sp_hipkv_set_recall", c_int, [c_void_p, c_int, c_int, c_int, c_int])
         _sig(lib, "sp_hipkv_read_recall_sidecar", c_int, [c_void_p, c_int, c_int, c_int, c_void_p])
+        _sig(lib, "sp_hipkv_tree_step", c_int, [c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_void_p, c_void_p])
+        _sig(lib, "sp_hipkv_tree_keep", c_int, [c_void_p, c_void_p, c_int])
+        _sig(lib, "sp_hipkv_score", c_int, [c_void_p, c_void_p, c_void_p, c_int, c_int, c_void_p, c_void_p, c_void_p, c_void_p])
         for op, args in (("tree_attention", TreeArgs), ("token_logprobs", LogprobArgs), ("keep_rows", KeepArgs)):
             _sig(lib, "sp_hipkv_" + op, c_int, [ctypes.POINTER(args), c_void_p])
         _sig(lib, "sp_hipkv_tree_attention_work", c_int, [ctypes.POINTER(TreeArgs), ctypes.POINTER(c_size_t)])
@@ -411,6 +414,38 @@ class Backend:
         check(kv().sp_hipkv_decode_batch_times(hs, n, ptr(toks), ptr(nxt), ptr(ms), ptr(nl), ptr(by)),
               "sp_hipkv_decode_batch_times")
         return nxt, ms, nl, by
+
+    def tree_step(self, tokens, parents, vocab=0):
+        """A step over a drafted tree (node i continues node parents[i], -1: the
+        context); vocab > 0 asks for the logits.  Returns (logits [n][vocab] or
+        None, greedy next tokens [n], log p of each node's token [n])."""
+        import numpy as np
+        t, p = (np.ascontiguousarray(x, dtype=np.int32) for x in (tokens, parents))
+        assert t.shape == p.shape and t.ndim == 1
+        lg = np.zeros((len(t), vocab), np.float32) if vocab else None
+        nxt, lp = np.zeros(len(t), np.int32), np.zeros(len(t), np.float32)
+        check(kv().sp_hipkv_tree_step(self.h, ptr(t), ptr(p), len(t), ptr(lg) if vocab else None, ptr(nxt), ptr(lp)),
+              "sp_hipkv_tree_step")
+        return lg, nxt, lp
+
+    def tree_keep(self, nodes):
+        """Keep a path of the pending tree (root first); the rest is dropped."""
+        import numpy as np
+        k = np.ascontiguousarray(nodes, dtype=np.int32)
+        check(kv().sp_hipkv_tree_keep(self.h, ptr(k), len(k)), "sp_hipkv_tree_keep")
+
+    def score(self, tokens, given=None, n_top=0):
+        """Prefill `tokens`; returns (log p of given or of the next tokens [n],
+        entropy [n], likeliest tokens [n][n_top], their log p [n][n_top])."""
+        import numpy as np
+        t = np.ascontiguousarray(tokens, dtype=np.int32)
+        g = None if given is None else np.ascontiguousarray(given, dtype=np.int32)
+        assert g is None or g.shape == t.shape
+        lp, ent = np.zeros(len(t), np.float32), np.zeros(len(t), np.float32)
+        ids, tl = np.zeros((len(t), n_top), np.int32), np.zeros((len(t), n_top), np.float32)
+        check(kv().sp_hipkv_score(self.h, ptr(t), None if g is None else ptr(g), len(t), n_top, ptr(lp), ptr(ent), ptr(ids), ptr(tl)),
+              "sp_hipkv_score")
+        return lp, ent, ids, tl
 
     def greedy(self, first_tok, n):
         import numpy as np
