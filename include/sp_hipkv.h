@@ -282,10 +282,10 @@ enum { SP_HIPKV_ROWS_F32 = 0, SP_HIPKV_ROWS_EXACT = 1, SP_HIPKV_ROWS_SPINOR = 2 
  * a decode step computes on the same rows; |q| below 2^15, |scores| below 2^17).  Nodes that see no position get zeros.  Rows
  * that a node does not see do not reach it whatever they hold. */
 typedef struct sp_hipkv_tree_args {
-    int32_t n_heads, n_kv_heads;    /* at most 16 q heads for each kv head */
+    int32_t n_heads, n_kv_heads;    /* at most 4096, and 16 q heads for each kv head */
     int32_t head_dim;               /* 64, 128 or 256 */
     int32_t rows;                   /* SP_HIPKV_ROWS_* */
-    int32_t n_seqs, n_nodes;        /* sequences (at most 65535), nodes of all of them */
+    int32_t n_seqs, n_nodes;        /* sequences (at most 4096), nodes of all of them */
     int32_t max_nodes;              /* no sequence has more (at most 512) */
     int32_t max_positions;          /* cached + nodes of no sequence is more (at most 2^20; exact rows 2^18) */
     int32_t window;                 /* 0: every cached position */

@@ -7,11 +7,12 @@
 //                      w_p = exp_fixed((z_p - M) 2^16) >> 8, out = RNE(sum w vq / (2^16 sum w)),
 // the decode attention's integers (kvd_attn.hip).
 //
-// One workgroup per row: its four waves take the positions in turn, each with a
-// running maximum and sum, and meet in LDS.
+// f32 and Spinor rows run on the f32 matrix cores (k_tree_float below), exact rows
+// one workgroup per row.
 #include "kvd_op.h"
 #include "kvd_exact.h"
 #include "kvd_vec.h"
+#include <algorithm>
 
 namespace kvd {
 
@@ -34,111 +35,536 @@ __device__ __forceinline__ TreeSeq tree_seq(const sp_hipkv_tree_args &a, int s) 
 }
 __device__ __forceinline__ int tree_low(const sp_hipkv_tree_args &a, const TreeSeq &q, int node) {
     if (!a.window) return 0;
-    const int64_t lo = (int64_t)q.cached + a.depth[q.node0 + node] - a.window + 1;
-    return lo < 0 ? 0 : lo > q.cached ? q.cached : (int)lo;
+    const int lo = q.cached + min(max(a.depth[q.node0 + node], 0), 511) - a.window + 1;
+    return min(max(lo, 0), q.cached);
 }
 __device__ __forceinline__ const uint8_t *tree_page(const sp_hipkv_tree_args &a, const TreeSeq &q, int pos) {
     const int lp = pos / PAGE;
     return (const uint8_t *)gmem(q.table)[a.ring_pages ? lp % a.ring_pages : lp];
 }
 
-template <int ROWS, int EPL>
-__global__ __launch_bounds__(64 * TREE_WAVES) void k_tree_row(sp_hipkv_tree_args a) {
-    constexpr int HD = EPL * 64, RB = row_bytes_of(ROWS, HD);
+template <int EPL>
+__global__ __launch_bounds__(64 * TREE_WAVES) void k_tree_exact(sp_hipkv_tree_args a) {
+    constexpr int HD = EPL * 64;
     const int head = blockIdx.x, node = blockIdx.y, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const TreeSeq q = tree_seq(a, blockIdx.z);
     if (node >= q.nodes) return;
     const int h = head / (a.n_heads / a.n_kv_heads), low = tree_low(a, q, node);
     const uint64_t *mask = a.visible + (size_t)(q.node0 + node) * a.mask_words;
     const float *qp = a.q + (size_t)(q.node0 + node) * a.q_stride + head * HD;
-    float qf[EPL];
     int64_t qi[EPL];
     #pragma unroll
-    for (int e = 0; e < EPL; e++) { qf[e] = qp[lane + 64 * e]; qi[e] = (int64_t)rintf(qf[e] * 65536.0f); }
-    auto row_of = [&](int p, int v) { return tree_page(a, q, p) + ((size_t)(v * a.n_kv_heads + h) * PAGE + (p & (PAGE - 1))) * RB; };
-    auto value = [&](const uint8_t *row, int e) {
-        const int d = lane + 64 * e;
-        if constexpr (ROWS == SP_HIPKV_ROWS_SPINOR) return (float)((const int8_t *)row)[d] * ((const float *)(row + HD))[spn_block_of(HD, d)];
-        else return ((const float *)row)[d];
-    };
+    for (int e = 0; e < EPL; e++) qi[e] = (int64_t)rintf(qp[lane + 64 * e] * 65536.0f);
+    auto row_of = [&](int p, int v) { return (const int32_t *)tree_page(a, q, p) + ((size_t)(v * a.n_kv_heads + h) * PAGE + (p & (PAGE - 1))) * HD; };
     auto sees = [&](int p) { return p < q.cached ? p >= low : (mask[(p - q.cached) >> 6] >> ((p - q.cached) & 63) & 1) != 0; };
-    auto grid_score = [&](int p) {                       // exact rows
-        const int32_t *k = (const int32_t *)row_of(p, 0);
+    auto grid_score = [&](int p) {
+        const int32_t *k = row_of(p, 0);
         int64_t ip = 0;
         #pragma unroll
         for (int e = 0; e < EPL; e++) ip += qi[e] * k[lane + 64 * e];
         return (int)llround_pow2<14>((float)((double)wave_allsum(ip) / 4294967296.0) * a.scale);
     };
-    __shared__ float sm[TREE_WAVES], sl[TREE_WAVES], so[TREE_WAVES][HD];
     __shared__ int zm[TREE_WAVES];
     __shared__ int64_t sw[TREE_WAVES], sv[TREE_WAVES][HD];
     const int end = q.cached + q.nodes;
     float *out = a.out + (size_t)(q.node0 + node) * a.out_stride + head * HD;
-    if constexpr (ROWS == SP_HIPKV_ROWS_EXACT) {
-        int M = INT32_MIN;
-        for (int p = low + wave; p < end; p += TREE_WAVES)
-            if (sees(p)) M = max(M, grid_score(p));
-        if (lane == 0) zm[wave] = M;
-        __syncthreads();
-        for (int w = 0; w < TREE_WAVES; w++) M = max(M, zm[w]);
-        int64_t S = 0, o[EPL] = {};
-        for (int p = low + wave; p < end; p += TREE_WAVES)
-            if (sees(p)) {
-                const int64_t w = exp_fixed((((int64_t)grid_score(p) - M) * ONE) >> 14) >> 8;
-                const int32_t *v = (const int32_t *)row_of(p, 1);
-                S += w;
-                #pragma unroll
-                for (int e = 0; e < EPL; e++) o[e] += w * v[lane + 64 * e];
-            }
-        if (lane == 0) sw[wave] = S;
+    int M = INT32_MIN;
+    for (int p = low + wave; p < end; p += TREE_WAVES)
+        if (sees(p)) M = max(M, grid_score(p));
+    if (lane == 0) zm[wave] = M;
+    __syncthreads();
+    for (int w = 0; w < TREE_WAVES; w++) M = max(M, zm[w]);
+    int64_t S = 0, o[EPL] = {};
+    for (int p = low + wave; p < end; p += TREE_WAVES)
+        if (sees(p)) {
+            const int64_t w = exp_fixed((((int64_t)grid_score(p) - M) * ONE) >> 14) >> 8;
+            const int32_t *v = row_of(p, 1);
+            S += w;
+            #pragma unroll
+            for (int e = 0; e < EPL; e++) o[e] += w * v[lane + 64 * e];
+        }
+    if (lane == 0) sw[wave] = S;
+    #pragma unroll
+    for (int e = 0; e < EPL; e++) sv[wave][lane + 64 * e] = o[e];
+    __syncthreads();
+    for (int d = threadIdx.x; d < HD; d += 64 * TREE_WAVES) {
+        int64_t t = 0, den = 0;
+        for (int w = 0; w < TREE_WAVES; w++) { t += sv[w][d]; den += sw[w]; }
+        out[d] = den ? rne_div_to_float((i128)t, den, 16) : 0.0f;
+    }
+}
+
+// ---------------------------------------------------------------- f32 and Spinor rows
+// The q heads of a kv head share its K and V rows: the rows of one kv head are
+// r = node G + q head of the group, 16 to a matrix tile, RT tiles to a workgroup.
+// Its four waves take the 16-position quarters of the pages of a range (a split)
+// in turn, each with all RT tiles, a running maximum, sum and output of its own; they
+// meet in LDS at the end, the splits in k_tree_merge.
+//
+// K and V go from memory into the operands' registers directly, each byte once:
+//   scores, transposed:  S^T = K Q^T, v_mfma_f32_16x16x4_f32, K the A operand (position
+//     lane % 16, 4 consecutive dims of group lane / 16), Q the B operand, from LDS;
+//   then lane l holds row l % 16 and positions 4 (l / 16) + i, as the A operand of
+//     O += P V needs them; V is the B operand, a float4 of a row per lane.
+// Two register buffers alternate, so that a stage (8 KiB a wave) is on its way while
+// the one before is multiplied.  f32 products and sums throughout.
+//
+// The running maximum only moves when a score exceeds it by 2^8 in the exponent (base
+// 2): weights stay below 2^8 and nothing is lost, and a tile needs one ballot instead of
+// a reduction over lanes.  The sums are joined over lanes once at the end.
+//
+// A position that a row does not see has weight 0, which a V row that is not finite
+// would turn into NaN: tiles that some row does not see whole look for such values
+// first and are then put off to a loop behind the main one, which adds positions one
+// by one (inside the main loop that path costs twice the output's registers).
+typedef float v4f __attribute__((ext_vector_type(4)));
+constexpr int TT = 16;                       // positions per tile: a quarter of a page
+constexpr float LOG2E_F = 1.44269504088896341f;
+
+__device__ __forceinline__ bool finite1(float x) { return (__float_as_uint(x) & 0x7F800000u) != 0x7F800000u; }
+
+template <int ROWS, int EPL, int RT>
+__global__ __launch_bounds__(256, 2) void k_tree_float(sp_hipkv_tree_args a, int groups, int nsplit) {
+    constexpr int HD = EPL * 64, CPR = HD / 16, RB = row_bytes_of(ROWS, HD);
+    constexpr bool SPN = ROWS == SP_HIPKV_ROWS_SPINOR;
+    constexpr int NST = !SPN && EPL == 4 ? 2 : 1, NB = 4 * EPL / NST;      // stages of K (and of V) per tile, float4s per stage
+    constexpr int LDS_F = RT * 16 * HD > 4 * 8 * HD ? RT * 16 * HD : 4 * 8 * HD;
+    __shared__ __align__(16) float lds[LDS_F];                             // q rows, then the waves' outputs
+    __shared__ float s_m[4][RT * 16], s_l[4][RT * 16];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), l16 = lane & 15, g = lane >> 4;
+    const int G = a.n_heads / a.n_kv_heads;
+    int id = blockIdx.x;
+    const int h = id % a.n_kv_heads; id /= a.n_kv_heads;
+    const int grp = id % groups; id /= groups;
+    const int split = id % nsplit;
+    const TreeSeq q = tree_seq(a, id / nsplit);
+    const int R = q.nodes * G, r0 = grp * RT * 16;
+    if (r0 >= R) return;
+    const int end = q.cached + q.nodes;
+    // this lane's rows, one of each tile: where it starts to see, its mask
+    int low[RT], nodei[RT], lo_min = INT32_MAX, lo_max = 0;
+    #pragma unroll
+    for (int t = 0; t < RT; t++) {
+        const int r = r0 + t * 16 + l16;
+        nodei[t] = (r < R ? r : R - 1) / G;
+        low[t] = tree_low(a, q, nodei[t]);
+        lo_min = min(lo_min, low[t]); lo_max = max(lo_max, low[t]);
+    }
+    if (a.window) {
         #pragma unroll
-        for (int e = 0; e < EPL; e++) sv[wave][lane + 64 * e] = o[e];
-        __syncthreads();
-        for (int d = threadIdx.x; d < HD; d += 64 * TREE_WAVES) {
-            int64_t t = 0, den = 0;
-            for (int w = 0; w < TREE_WAVES; w++) { t += sv[w][d]; den += sw[w]; }
-            out[d] = den ? rne_div_to_float((i128)t, den, 16) : 0.0f;
+        for (int o = 1; o < 16; o <<= 1) { lo_min = min(lo_min, __shfl_xor(lo_min, o, 64)); lo_max = max(lo_max, __shfl_xor(lo_max, o, 64)); }
+    }
+    lo_min = __builtin_amdgcn_readfirstlane(lo_min); lo_max = __builtin_amdgcn_readfirstlane(lo_max);
+    // this split's pages, and this wave's of them
+    const int pg0 = lo_min / PAGE, pg1 = (end + PAGE - 1) / PAGE, per = (pg1 - pg0 + nsplit - 1) / nsplit;
+    int w0 = pg0 + split * per, w1 = min(w0 + per, pg1);
+    if (w0 < w1 && w0 * PAGE + wave * TT + TT <= lo_min) w0++;
+    if (w0 < w1 && (w1 - 1) * PAGE + wave * TT >= end) w1--;
+    v4f *qs = (v4f *)lds;
+    for (int i = threadIdx.x; i < RT * 16 * (HD / 4); i += 256) {
+        const int r = i / (HD / 4), c = i % (HD / 4), rr = r0 + r < R ? r0 + r : R - 1;
+        qs[r * (HD / 4) + (c ^ (r & 15))] = *(const v4f *)(a.q + (size_t)(q.node0 + rr / G) * a.q_stride + (size_t)(h * G + rr % G) * HD + 4 * c);
+    }
+    v4f O[RT][CPR], S[RT];
+    float m[RT], l[RT];
+    uint32_t see[RT];
+    #pragma unroll
+    for (int t = 0; t < RT; t++) {
+        m[t] = -INFINITY; l[t] = 0.0f; see[t] = 15;
+        #pragma unroll
+        for (int c = 0; c < CPR; c++) O[t][c] = (v4f){0, 0, 0, 0};
+    }
+    __syncthreads();
+    const uint32_t kslice = (uint32_t)h * PAGE * RB, vslice = (uint32_t)(a.n_kv_heads + h) * PAGE * RB;
+    // page addresses are the wave's: rows load as address + 32-bit lane offset
+    auto page = [&](int lp) {
+        const uint64_t p = (uint64_t)tree_page(a, q, lp * PAGE);
+        return (const uint8_t *)((uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(p >> 32)) << 32 |
+                                 (uint32_t)__builtin_amdgcn_readfirstlane((int)p));
+    };
+    // positions past the last one repeat it
+    auto row_off = [&](int lp, int x) { const int p = lp * PAGE + wave * TT + x; return (uint32_t)((p < end ? p : end - 1) & (PAGE - 1)) * RB; };
+    // tiles that some row does not see whole, and those of them put off to the end:
+    // nodes span at most 9 pages, so do the rows' window starts
+    auto ragged = [&](int lp) { const int p0 = lp * PAGE + wave * TT; return p0 < lo_max || p0 + TT > q.cached; };
+    const int tail_pg = q.cached / PAGE;
+    uint32_t later = 0;
+    auto put_off = [&](int lp) { later |= lp >= tail_pg ? 1u << (lp - tail_pg) : 65536u << (lp - pg0); };
+    auto next_off = [&] {
+        const int b = __builtin_ctz(later);
+        later &= later - 1;
+        return b < 16 ? tail_pg + b : pg0 + b - 16;
+    };
+    // scores in base 2, masked; weights into S
+    auto softmax = [&](int lp) {
+        const int p0 = lp * PAGE + wave * TT;
+        const bool whole = !ragged(lp);
+        #pragma unroll
+        for (int t = 0; t < RT; t++) {
+            float mx = -INFINITY;
+            #pragma unroll
+            for (int i = 0; i < 4; i++) S[t][i] *= a.scale * LOG2E_F;
+            if (!whole) {
+                see[t] = 0;
+                #pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    const int p = p0 + 4 * g + i, j = p - q.cached;
+                    bool v = p >= low[t];
+                    if (j >= 0) v = j < q.nodes && (gmem(a.visible)[(size_t)(q.node0 + nodei[t]) * a.mask_words + (j >> 6)] >> (j & 63) & 1);
+                    see[t] |= (uint32_t)v << i;
+                    S[t][i] = v ? S[t][i] : -INFINITY;
+                }
+            }
+            #pragma unroll
+            for (int i = 0; i < 4; i++) mx = fmaxf(mx, S[t][i]);
+            if (__any(mx > m[t] + 8.0f)) {
+                mx = fmaxf(mx, __shfl_xor(mx, 16, 64));
+                mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
+                const float mn = fmaxf(m[t], mx), al = mn == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m[t] - mn);
+                m[t] = mn;
+                l[t] *= al;
+                #pragma unroll
+                for (int i = 0; i < 4; i++) {                              // O's rows are 4 g + i
+                    const float f = __shfl(al, 4 * g + i, 64);
+                    #pragma unroll
+                    for (int c = 0; c < CPR; c++) O[t][c][i] *= f;
+                }
+            }
+            const float ms = m[t] == -INFINITY ? 0.0f : m[t];
+            #pragma unroll
+            for (int i = 0; i < 4; i++) { S[t][i] = __builtin_amdgcn_exp2f(S[t][i] - ms); l[t] += S[t][i]; }
+        }
+    };
+    // O[t][c0 + c] += P x(e, c), positions 4 g + e, N columns
+    auto pv = [&](auto n, int c0, auto &&x) {
+        constexpr int N = decltype(n)::value;
+        #pragma unroll
+        for (int e = 0; e < 4; e++) {
+            #pragma unroll
+            for (int c = 0; c < N; c++) {
+                const float v = x(e, c);
+                #pragma unroll
+                for (int t = 0; t < RT; t++) O[t][c0 + c] = __builtin_amdgcn_mfma_f32_16x16x4f32(S[t][e], v, O[t][c0 + c], 0, 0, 0);
+                if (SPN && c % 4 == 3) __builtin_amdgcn_sched_barrier(0);
+            }
+            __builtin_amdgcn_sched_barrier(0);
+        }
+    };
+    // the same position by position, for the rows that see it; x4(p, k): columns 4 k .. of this lane
+    auto pv_slow = [&](int lp, auto &&x4) {
+        for (int p = 0; p < TT && lp * PAGE + wave * TT + p < end; p++) {
+            const int from = (p >> 2) * 16, pe = p & 3;
+            #pragma unroll
+            for (int t = 0; t < RT; t++) {
+                const float we = pe == 0 ? S[t][0] : pe == 1 ? S[t][1] : pe == 2 ? S[t][2] : S[t][3];
+                float w[4];
+                bool on[4];
+                #pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    w[i] = __shfl(we, from + 4 * g + i, 64);
+                    on[i] = __shfl(see[t], from + 4 * g + i, 64) >> pe & 1;
+                }
+                #pragma unroll
+                for (int k = 0; k < CPR / 4; k++) {
+                    const v4f v = x4(p, k);
+                    #pragma unroll
+                    for (int c = 0; c < 4; c++)
+                        #pragma unroll
+                        for (int i = 0; i < 4; i++) O[t][4 * k + c][i] = on[i] ? O[t][4 * k + c][i] + w[i] * v[c] : O[t][4 * k + c][i];
+                    __builtin_amdgcn_sched_barrier(0);
+                }
+            }
+        }
+    };
+    auto zero_s = [&] {
+        #pragma unroll
+        for (int t = 0; t < RT; t++) S[t] = (v4f){0, 0, 0, 0};
+    };
+    if constexpr (!SPN) {
+        // column of O[t][c], row 4 g + i: 64 (c / 4) + 4 l16 + c % 4
+        auto load_k = [&](v4f (&x)[NB], const uint8_t *pg, int lp, int st) {
+            const uint32_t off = kslice + row_off(lp, l16) + 16 * g + st * NB * 64;
+            #pragma unroll
+            for (int s = 0; s < NB; s++) x[s] = *gmem((const v4f *)(pg + off + 64 * s));
+        };
+        auto load_v = [&](v4f (&x)[NB], const uint8_t *pg, int lp, int st) {
+            #pragma unroll
+            for (int e = 0; e < 4; e++) {
+                const uint32_t off = vslice + row_off(lp, 4 * g + e) + 16 * l16 + st * NB * 64;
+                #pragma unroll
+                for (int u = 0; u < NB / 4; u++) x[e * (NB / 4) + u] = *gmem((const v4f *)(pg + off + 256 * u));
+            }
+        };
+        auto scores = [&](const v4f (&x)[NB], int st) {
+            #pragma unroll
+            for (int s = 0; s < NB; s++) {
+                v4f qv[RT];
+                #pragma unroll
+                for (int t = 0; t < RT; t++) qv[t] = qs[(t * 16 + l16) * (HD / 4) + ((4 * (st * NB + s) + g) ^ l16)];
+                #pragma unroll
+                for (int e = 0; e < 4; e++)
+                    #pragma unroll
+                    for (int t = 0; t < RT; t++) S[t] = __builtin_amdgcn_mfma_f32_16x16x4f32(x[s][e], qv[t][e], S[t], 0, 0, 0);
+                if (s % 2) __builtin_amdgcn_sched_barrier(0);              // few q reads ahead at a time
+            }
+        };
+        auto values = [&](const v4f (&x)[NB], int st) {
+            pv(std::integral_constant<int, NB>{}, st * NB, [&](int e, int c) { return x[e * (NB / 4) + c / 4][c % 4]; });
+        };
+        v4f A[NB], B[NB];
+        const uint8_t *pg = nullptr, *pn = nullptr;
+        if (w0 < w1) {
+            pg = page(w0);
+            load_k(A, pg, w0, 0);
+            if (NST == 2) load_k(B, pg, w0, 1); else load_v(B, pg, w0, 0);
+            pn = page(min(w0 + 1, w1 - 1));
+        }
+        for (int lp = w0; lp < w1; lp++) {
+            const int nx = min(lp + 1, w1 - 1);
+            zero_s();
+            scores(A, 0);
+            __builtin_amdgcn_sched_barrier(0);
+            if constexpr (NST == 2) {
+                load_v(A, pg, lp, 0);
+                __builtin_amdgcn_sched_barrier(0);
+                scores(B, 1);
+                __builtin_amdgcn_sched_barrier(0);
+                load_v(B, pg, lp, 1);
+            } else {
+                load_k(A, pn, nx, 0);
+            }
+            __builtin_amdgcn_sched_barrier(0);
+            bool bad = false;
+            if (ragged(lp)) {
+                #pragma unroll
+                for (int s = 0; s < NB; s++)
+                    #pragma unroll
+                    for (int e = 0; e < 4; e++) bad |= !finite1(B[s][e]) || (NST == 2 && !finite1(A[s][e]));
+            }
+            bad = __any(bad);
+            if (bad) put_off(lp); else softmax(lp);
+            if constexpr (NST == 2) {
+                if (!bad) values(A, 0);
+                __builtin_amdgcn_sched_barrier(0);
+                load_k(A, pn, nx, 0);
+                __builtin_amdgcn_sched_barrier(0);
+                if (!bad) values(B, 1);
+                __builtin_amdgcn_sched_barrier(0);
+                load_k(B, pn, nx, 1);
+            } else {
+                if (!bad) values(B, 0);
+                __builtin_amdgcn_sched_barrier(0);
+                load_v(B, pn, nx, 0);
+            }
+            pg = pn;
+            pn = page(min(lp + 2, w1 - 1));
+            __builtin_amdgcn_sched_barrier(0);
+        }
+        while (later) {
+            const int lp = next_off();
+            pg = page(lp);
+            zero_s();
+            for (int st = 0; st < NST; st++) { load_k(A, pg, lp, st); scores(A, st); }
+            softmax(lp);
+            pv_slow(lp, [&](int p, int k) { return *gmem((const v4f *)(pg + vslice + row_off(lp, p) + 16 * l16 + 256 * k)); });
         }
     } else {
-        float m = -INFINITY, l = 0.0f, o[EPL] = {};
-        for (int p = low + wave; p < end; p += TREE_WAVES)
-            if (sees(p)) {
-                float s = 0.0f;
-                const uint8_t *k = row_of(p, 0), *v = row_of(p, 1);
+        // K: 16 codes of dims 64 i + 16 g.. a load; V: the CPR codes of columns CPR l16..
+        // (O[t][c] is column CPR l16 + c), and the multipliers of the at most two
+        // chunks that they lie in
+        constexpr int NM = spn_blocks(HD);
+        struct KRow { uint4 c[EPL]; float m[NM]; };
+        struct VRow { uint32_t c[EPL]; float m0, m1; };
+        const int d0v = CPR * l16, b0v = spn_block_of(HD, d0v), bnd0 = spn_block_start(HD, b0v + 1), b1v = bnd0 < d0v + CPR ? b0v + 1 : b0v;
+        int bndv = bnd0;
+        auto load_k = [&](KRow &x, const uint8_t *pg, int lp) {
+            const uint8_t *row = pg + kslice + row_off(lp, l16);
+            #pragma unroll
+            for (int i = 0; i < EPL; i++) x.c[i] = *gmem((const uint4 *)(row + 64 * i + 16 * g));
+            #pragma unroll
+            for (int b = 0; b < NM; b++) x.m[b] = *gmem((const float *)(row + HD + 4 * b));
+        };
+        auto load_v = [&](VRow (&x)[4], const uint8_t *pg, int lp) {
+            #pragma unroll
+            for (int e = 0; e < 4; e++) {
+                const uint8_t *row = pg + vslice + row_off(lp, 4 * g + e);
                 #pragma unroll
-                for (int e = 0; e < EPL; e++) s += qf[e] * value(k, e);
-                s = wave_allsum(s) * a.scale;
-                const float mn = fmaxf(m, s), al = mn == -INFINITY ? 0.0f : expf(m - mn), w = mn == -INFINITY ? 0.0f : expf(s - mn);
-                l = l * al + w;
+                for (int i = 0; i < EPL; i++) x[e].c[i] = *gmem((const uint32_t *)(row + d0v + 4 * i));
+                x[e].m0 = *gmem((const float *)(row + HD + 4 * b0v));
+                x[e].m1 = *gmem((const float *)(row + HD + 4 * b1v));
+            }
+        };
+        auto code = [](uint32_t w, int t) { return (float)(int32_t)(int8_t)(w >> (8 * t)); };
+        auto scores = [&](const KRow &x) {
+            #pragma unroll
+            for (int i = 0; i < EPL; i++) {
+                const int d0 = 64 * i + 16 * g, b = spn_block_of(HD, d0);
+                int bnd = spn_block_start(HD, b + 1);
+                asm volatile("" : "+v"(bnd));                              // compared where used: kept masks would fill the scalar registers
+                float m0 = x.m[0], m1 = x.m[0];
                 #pragma unroll
-                for (int e = 0; e < EPL; e++) o[e] = o[e] * al + w * value(v, e);
-                m = mn;
+                for (int bb = 1; bb < NM; bb++) { if (b == bb) m0 = x.m[bb]; if (b + 1 == bb) m1 = x.m[bb]; }
+                const uint32_t w[4] = {x.c[i].x, x.c[i].y, x.c[i].z, x.c[i].w};
+                #pragma unroll
+                for (int k = 0; k < 4; k++) {
+                    v4f qv[RT];
+                    #pragma unroll
+                    for (int t = 0; t < RT; t++) qv[t] = qs[(t * 16 + l16) * (HD / 4) + ((16 * i + 4 * g + k) ^ l16)];
+                    #pragma unroll
+                    for (int e = 0; e < 4; e++) {
+                        const float kv = code(w[k], e) * (d0 + 4 * k + e < bnd ? m0 : m1);
+                        #pragma unroll
+                        for (int t = 0; t < RT; t++) S[t] = __builtin_amdgcn_mfma_f32_16x16x4f32(kv, qv[t][e], S[t], 0, 0, 0);
+                    }
+                    if (k % 2) __builtin_amdgcn_sched_barrier(0);
+                }
             }
-        if (lane == 0) { sm[wave] = m; sl[wave] = l; }
-        #pragma unroll
-        for (int e = 0; e < EPL; e++) so[wave][lane + 64 * e] = o[e];
-        __syncthreads();
-        float M = -INFINITY;
-        for (int w = 0; w < TREE_WAVES; w++) M = fmaxf(M, sm[w]);
-        for (int d = threadIdx.x; d < HD; d += 64 * TREE_WAVES) {
-            float t = 0.0f, den = 0.0f;
-            for (int w = 0; w < TREE_WAVES; w++) {
-                if (sm[w] == -INFINITY) continue;
-                const float f = expf(sm[w] - M);
-                t += f * so[w][d]; den += f * sl[w];
+        };
+        KRow K;
+        VRow V[4];
+        const uint8_t *pg = nullptr, *pn = nullptr;
+        if (w0 < w1) {
+            pg = page(w0);
+            load_k(K, pg, w0);
+            load_v(V, pg, w0);
+            pn = page(min(w0 + 1, w1 - 1));
+        }
+        for (int lp = w0; lp < w1; lp++) {
+            const int nx = min(lp + 1, w1 - 1);
+            zero_s();
+            scores(K);
+            __builtin_amdgcn_sched_barrier(0);
+            load_k(K, pn, nx);
+            __builtin_amdgcn_sched_barrier(0);
+            bool bad = false;
+            if (ragged(lp)) {
+                #pragma unroll
+                for (int e = 0; e < 4; e++) bad |= !finite1(127.0f * V[e].m0) || !finite1(127.0f * V[e].m1);
             }
-            out[d] = den > 0.0f ? t / den : 0.0f;
+            if (__any(bad)) {
+                put_off(lp);
+            } else {
+                softmax(lp);
+                asm volatile("" : "+v"(bndv));
+                pv(std::integral_constant<int, CPR>{}, 0, [&](int e, int c) { return code(V[e].c[c / 4], c % 4) * (d0v + c < bndv ? V[e].m0 : V[e].m1); });
+            }
+            __builtin_amdgcn_sched_barrier(0);
+            load_v(V, pn, nx);
+            pg = pn;
+            pn = page(min(lp + 2, w1 - 1));
+            __builtin_amdgcn_sched_barrier(0);
+        }
+        while (later) {
+            const int lp = next_off();
+            pg = page(lp);
+            zero_s();
+            load_k(K, pg, lp);
+            scores(K);
+            softmax(lp);
+            pv_slow(lp, [&](int p, int k) {
+                const uint8_t *row = pg + vslice + row_off(lp, p);
+                const uint32_t w = *gmem((const uint32_t *)(row + d0v + 4 * k));
+                const float m0 = *gmem((const float *)(row + HD + 4 * b0v)), m1 = *gmem((const float *)(row + HD + 4 * b1v));
+                v4f v;
+                #pragma unroll
+                for (int c = 0; c < 4; c++) v[c] = code(w, c) * (d0v + 4 * k + c < bndv ? m0 : m1);
+                return v;
+            });
         }
     }
+    // the four waves' parts: m and l first
+    #pragma unroll
+    for (int t = 0; t < RT; t++) {
+        l[t] += __shfl_xor(l[t], 16, 64);
+        l[t] += __shfl_xor(l[t], 32, 64);
+        if (g == 0) { s_m[wave][t * 16 + l16] = m[t]; s_l[wave][t * 16 + l16] = l[t]; }
+    }
+    __syncthreads();                                                       // ... and nobody reads q any more
+    float *po = (float *)a.work, *pml = po + (size_t)a.n_nodes * a.n_heads * nsplit * HD;
+    #pragma unroll
+    for (int t = 0; t < RT; t++)
+        #pragma unroll
+        for (int ih = 0; ih < 2; ih++) {                                   // rows 4 g + 2 ih, + 1
+            #pragma unroll
+            for (int i = 2 * ih; i < 2 * ih + 2; i++) {
+                const int r = t * 16 + 4 * g + i;
+                const float M = fmaxf(fmaxf(s_m[0][r], s_m[1][r]), fmaxf(s_m[2][r], s_m[3][r]));
+                const float f = M == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(s_m[wave][r] - M);
+                v4f *dst = (v4f *)lds + ((wave * 8 + 2 * g + (i & 1)) * (HD / 4));
+                #pragma unroll
+                for (int c = 0; c < CPR; c += 4) {
+                    const v4f x = {O[t][c][i], O[t][c + 1][i], O[t][c + 2][i], O[t][c + 3][i]};
+                    dst[SPN ? (CPR / 4) * l16 + c / 4 : 4 * c + l16] = f == 0.0f ? (v4f){0, 0, 0, 0} : x * f;
+                }
+            }
+            __syncthreads();
+            for (int i = threadIdx.x; i < 8 * (HD / 4); i += 256) {
+                const int k = i / (HD / 4), c = i % (HD / 4), rl = t * 16 + 4 * (k >> 1) + 2 * ih + (k & 1), r = r0 + rl;
+                if (r >= R) continue;
+                const v4f *src = (const v4f *)lds + k * (HD / 4) + c;
+                v4f x = (src[0] + src[8 * (HD / 4)]) + (src[16 * (HD / 4)] + src[24 * (HD / 4)]);
+                const float M = fmaxf(fmaxf(s_m[0][rl], s_m[1][rl]), fmaxf(s_m[2][rl], s_m[3][rl]));
+                float L = 0.0f;
+                if (M > -INFINITY)
+                    #pragma unroll
+                    for (int w = 0; w < 4; w++) L += s_l[w][rl] * __builtin_amdgcn_exp2f(s_m[w][rl] - M);
+                const int node = q.node0 + r / G, head = h * G + r % G;
+                if (nsplit == 1) {
+                    *(v4f *)(a.out + (size_t)node * a.out_stride + (size_t)head * HD + 4 * c) = M == -INFINITY ? (v4f){0, 0, 0, 0} : x / L;
+                } else {
+                    const size_t at = ((size_t)node * a.n_heads + head) * nsplit + split;
+                    if (M > -INFINITY) *(v4f *)(po + at * HD + 4 * c) = x;
+                    if (c == 0) { pml[2 * at] = M; pml[2 * at + 1] = L; }
+                }
+            }
+            if (t < RT - 1 || ih == 0) __syncthreads();
+        }
+}
+
+// out = sum_c 2^(m_c - M) O_c / sum_c 2^(m_c - M) l_c; HD / 4 threads a row
+template <int HD>
+__global__ __launch_bounds__(256) void k_tree_merge(sp_hipkv_tree_args a, int nsplit) {
+    const size_t row = (size_t)blockIdx.x * (1024 / HD) + threadIdx.x / (HD / 4);
+    if (row >= (size_t)a.n_nodes * a.n_heads) return;
+    const int c = threadIdx.x % (HD / 4);
+    const v4f *po = (const v4f *)((const float *)a.work + row * nsplit * HD) + c;
+    const float *ml = (const float *)a.work + (size_t)a.n_nodes * a.n_heads * nsplit * HD + 2 * row * nsplit;
+    float M = -INFINITY, L = 0.0f;
+    for (int k = 0; k < nsplit; k++) M = fmaxf(M, ml[2 * k]);
+    v4f x = {0, 0, 0, 0};
+    #pragma unroll 8
+    for (int k = 0; k < nsplit; k++) {
+        const float mk = ml[2 * k];
+        if (!(mk > -INFINITY)) continue;                                   // a part without a position of this row
+        const float f = __builtin_amdgcn_exp2f(mk - M);
+        L += f * ml[2 * k + 1];
+        x += f * po[(size_t)k * (HD / 4)];
+    }
+    *(v4f *)(a.out + (row / a.n_heads) * a.out_stride + (row % a.n_heads) * HD + 4 * c) = M > -INFINITY ? x / L : (v4f){0, 0, 0, 0};
+}
+
+// How a launch is cut: row tiles of a workgroup, workgroups along a sequence's rows,
+// splits of its positions.
+struct TreePlan { int rt, groups, nsplit; };
+TreePlan tree_plan(const sp_hipkv_tree_args &a) {
+    TreePlan p;
+    const int most = a.head_dim == 256 ? 2 : 4, tiles = std::max(1, (a.max_nodes * (a.n_heads / a.n_kv_heads) + 15) / 16);
+    p.groups = (tiles + most - 1) / most;
+    p.rt = (tiles + p.groups - 1) / p.groups;
+    const int span = a.window ? std::min(a.max_positions, a.window + a.max_nodes + PAGE) : a.max_positions;
+    const int64_t base = (int64_t)a.n_kv_heads * p.groups * std::max(a.n_seqs, 1);
+    const int64_t pages = std::max(1, (span + PAGE - 1) / PAGE);
+    p.nsplit = (int)std::max<int64_t>(1, std::min<int64_t>({(512 + base - 1) / base, (pages + 1) / 2, 64}));
+    return p;
 }
 
 int tree_check(const char *who, const sp_hipkv_tree_args *a) {
     OP_NEED(a, "null arguments");
     OP_NEED(a->head_dim == 64 || a->head_dim == 128 || a->head_dim == 256, "head_dim is not 64, 128 or 256");
-    OP_NEED(a->n_kv_heads > 0 && a->n_heads > 0 && a->n_heads % a->n_kv_heads == 0 && a->n_heads / a->n_kv_heads <= 16 && a->n_heads <= 65535,
+    OP_NEED(a->n_kv_heads > 0 && a->n_heads > 0 && a->n_heads % a->n_kv_heads == 0 && a->n_heads / a->n_kv_heads <= 16 && a->n_heads <= 4096,
             "n_heads is not n_kv_heads times 1 to 16");
     OP_NEED(a->rows == SP_HIPKV_ROWS_F32 || a->rows == SP_HIPKV_ROWS_EXACT || a->rows == SP_HIPKV_ROWS_SPINOR, "unknown row format");
-    OP_NEED(a->n_seqs >= 0 && a->n_seqs <= 65535, "n_seqs outside [0, 65535]");
+    OP_NEED(a->n_seqs >= 0 && a->n_seqs <= 4096, "n_seqs outside [0, 4096]");
     OP_NEED(a->n_nodes >= 0, "negative n_nodes");
     OP_NEED(a->max_nodes >= 0 && a->max_nodes <= 512, "max_nodes outside [0, 512]");
     OP_NEED(a->max_positions >= 0 && a->max_positions <= (a->rows == SP_HIPKV_ROWS_EXACT ? 1 << 18 : 1 << 20),
@@ -160,19 +586,36 @@ int tree_check_arrays(const char *who, const sp_hipkv_tree_args *a, size_t need)
     return 0;
 }
 
-template <int ROWS> void tree_go(const sp_hipkv_tree_args &a, hipStream_t s) {
-    const dim3 grid(a.n_heads, a.max_nodes, a.n_seqs);
-    if (a.head_dim == 256) hipLaunchKernelGGL((k_tree_row<ROWS, 4>), grid, dim3(64 * TREE_WAVES), 0, s, a);
-    else if (a.head_dim == 128) hipLaunchKernelGGL((k_tree_row<ROWS, 2>), grid, dim3(64 * TREE_WAVES), 0, s, a);
-    else hipLaunchKernelGGL((k_tree_row<ROWS, 1>), grid, dim3(64 * TREE_WAVES), 0, s, a);
+void tree_exact(const sp_hipkv_tree_args &a, hipStream_t s) {
+    const dim3 grid(a.n_heads, a.max_nodes, a.n_seqs), wg(64 * TREE_WAVES);
+    if (a.head_dim == 256) hipLaunchKernelGGL(k_tree_exact<4>, grid, wg, 0, s, a);
+    else if (a.head_dim == 128) hipLaunchKernelGGL(k_tree_exact<2>, grid, wg, 0, s, a);
+    else hipLaunchKernelGGL(k_tree_exact<1>, grid, wg, 0, s, a);
+}
+int64_t tree_grid(const sp_hipkv_tree_args &a, const TreePlan &p) { return (int64_t)a.n_kv_heads * p.groups * p.nsplit * a.n_seqs; }
+
+template <int ROWS> void tree_float(const sp_hipkv_tree_args &a, hipStream_t s) {
+    const TreePlan p = tree_plan(a);
+    const dim3 grid((uint32_t)tree_grid(a, p)), wg(256);
+#define TREE_RUN(EPL, RT) hipLaunchKernelGGL((k_tree_float<ROWS, EPL, RT>), grid, wg, 0, s, a, p.groups, p.nsplit)
+    if (a.head_dim == 256) { if (p.rt == 1) TREE_RUN(4, 1); else TREE_RUN(4, 2); }
+    else if (a.head_dim == 128) { if (p.rt == 1) TREE_RUN(2, 1); else if (p.rt == 2) TREE_RUN(2, 2); else if (p.rt == 3) TREE_RUN(2, 3); else TREE_RUN(2, 4); }
+    else { if (p.rt == 1) TREE_RUN(1, 1); else if (p.rt == 2) TREE_RUN(1, 2); else if (p.rt == 3) TREE_RUN(1, 3); else TREE_RUN(1, 4); }
+#undef TREE_RUN
+    if (p.nsplit == 1) return;
+    const int64_t rows = (int64_t)a.n_nodes * a.n_heads, per = 1024 / a.head_dim;
+    const dim3 mg((uint32_t)((rows + per - 1) / per));
+    if (a.head_dim == 256) hipLaunchKernelGGL(k_tree_merge<256>, mg, wg, 0, s, a, p.nsplit);
+    else if (a.head_dim == 128) hipLaunchKernelGGL(k_tree_merge<128>, mg, wg, 0, s, a, p.nsplit);
+    else hipLaunchKernelGGL(k_tree_merge<64>, mg, wg, 0, s, a, p.nsplit);
 }
 
 }  // namespace
 
 void launch_tree(const sp_hipkv_tree_args &a, hipStream_t s) {
-    if (a.rows == SP_HIPKV_ROWS_F32) tree_go<SP_HIPKV_ROWS_F32>(a, s);
-    else if (a.rows == SP_HIPKV_ROWS_EXACT) tree_go<SP_HIPKV_ROWS_EXACT>(a, s);
-    else tree_go<SP_HIPKV_ROWS_SPINOR>(a, s);
+    if (a.rows == SP_HIPKV_ROWS_EXACT) tree_exact(a, s);
+    else if (a.rows == SP_HIPKV_ROWS_F32) tree_float<SP_HIPKV_ROWS_F32>(a, s);
+    else tree_float<SP_HIPKV_ROWS_SPINOR>(a, s);
 }
 
 }  // namespace kvd
@@ -183,6 +626,10 @@ extern "C" int sp_hipkv_tree_attention_work(const sp_hipkv_tree_args *a, size_t 
     if (tree_check(who, a)) return 1;
     OP_NEED(bytes, "null bytes");
     *bytes = 0;
+    if (a->rows == SP_HIPKV_ROWS_EXACT) return 0;
+    const TreePlan p = tree_plan(*a);
+    OP_NEED(tree_grid(*a, p) <= 1 << 23, "too many sequences, heads and nodes for one launch");
+    if (p.nsplit > 1) *bytes = (size_t)a->n_nodes * a->n_heads * p.nsplit * (a->head_dim + 2) * 4;
     return 0;
 }
 
