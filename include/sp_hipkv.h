@@ -319,7 +319,7 @@ int  sp_hipkv_tree_attention_work(const sp_hipkv_tree_args *a, size_t *bytes);
  * counting as larger than any number.  f32 sums without the largest term, which is
  * 1 exactly: entropies near 0 keep their relative precision. */
 typedef struct sp_hipkv_logprob_args {
-    int32_t n_rows, vocab;          /* at most 65535 rows, 2^24 tokens */
+    int32_t n_rows, vocab;          /* at most 65535 rows, 2^20 tokens */
     int32_t n_given, n_top;         /* given tokens of a row (at most 64), alternatives (at most 32 and vocab) */
     float   scale;                  /* 1 / temperature, positive and finite */
     const float *logits;            /* [n_rows][stride], any 4-byte alignment */

@@ -8,8 +8,16 @@
 // r is kept without the 1, which f32 sums would round small remainders away on: a
 // row that is sure of its token has an entropy of the remainder's size.
 //
-// One workgroup per row, which it reads once for M, once for the sums and once for
-// each alternative (the largest key below the last one's).
+// k_lp_part reads a row once, a segment of it per workgroup, held in registers: its
+// maximum, its r and sum of e^d d, and its n_top largest as sorted keys.  k_lp_merge
+// joins a row's segments:
+//   r = (segments at M) - 1 + sum_{m_s = M} r_s + sum_{m_s < M} e^(m_s - M) (1 + r_s),
+// and so on.  The floor is the row's bytes.
+//
+// The n_top largest of a workgroup: the n_top-th largest of a wave's 64 lane maxima is
+// a bound from below, found by bisection with ballots; the largest such bound of the
+// waves leaves few candidates (about 100 of 8192 at 20), which are ranked by counting.
+// Rows that leave more than the list holds (many equal logits) are searched by rounds.
 #include "kvd_op.h"
 #include "kvd_vec.h"
 
@@ -17,80 +25,217 @@ namespace kvd {
 
 namespace {
 
-constexpr int LP_THREADS = 256;
+constexpr int LP_THREADS = 256, LP_WAVES = LP_THREADS / 64;
+constexpr int LP_LIST = 1024;                    // candidates of a workgroup
+constexpr int LP_SEGS = 128;                     // segments of a row at most
+constexpr int LP_LONG = 32, LP_SHORT = 8;        // logits per thread
 
-// The order of alternatives as an unsigned key, NaN above all, one zero; the lower
-// token first among equals.
+typedef float v4u __attribute__((ext_vector_type(4), aligned(4)));
+
+// The order of alternatives as an unsigned number, NaN above all, one zero; 0 is below
+// any logit.  The lower token first among equals.
 __device__ __forceinline__ uint32_t lp_order(float x) {
     if (x != x) return 0xFFFFFFFFu;
     const uint32_t b = __float_as_uint(x + 0.0f);
-    return b & 0x80000000u ? ~b : b | 0x80000000u;
+    return b ^ ((uint32_t)((int32_t)b >> 31) | 0x80000000u);
 }
-__device__ __forceinline__ uint64_t lp_key(float x, int t) { return (uint64_t)lp_order(x) << 32 | (uint32_t)~t; }
+__device__ __forceinline__ uint64_t lp_key(uint32_t order, int t) { return order ? (uint64_t)order << 32 | (uint32_t)~t : 0; }
 
-template <typename T, typename Op> __device__ T lp_block(T v, T *red, Op op) {
+template <typename T, typename Op> __device__ __forceinline__ T lp_block(T v, T *red, Op op) {
+    #pragma unroll
     for (int o = 32; o; o >>= 1) v = op(v, (T)__shfl_xor(v, o, 64));
-    __syncthreads();
     if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
     __syncthreads();
     v = red[0];
-    for (int w = 1; w < LP_THREADS / 64; w++) v = op(v, red[w]);
+    #pragma unroll
+    for (int w = 1; w < LP_WAVES; w++) v = op(v, red[w]);
     return v;
 }
 
-__global__ __launch_bounds__(LP_THREADS) void k_logprob_row(sp_hipkv_logprob_args a) {
-    __shared__ uint64_t red8[LP_THREADS / 64];
-    __shared__ float red4[LP_THREADS / 64];
+// The k largest of the workgroup's keys, key(e) of each thread's N, descending, to
+// dst[0..k) (0 where there are fewer).
+struct LpSelect { uint64_t list[LP_LIST], red[LP_WAVES]; uint32_t least[LP_WAVES]; int count; };
+template <int N, typename Key> __device__ __forceinline__ void lp_select(LpSelect &s, int k, Key key, uint64_t *dst) {
+    const int wave = threadIdx.x >> 6;
+    uint32_t mx = 0, T = 0;
+    #pragma unroll
+    for (int e = 0; e < N; e++) mx = max(mx, (uint32_t)(key(e) >> 32));
+    for (int b = 31; b >= 0; b--)
+        if (__popcll(__ballot(mx >= (T | 1u << b))) >= k) T |= 1u << b;
+    if ((threadIdx.x & 63) == 0) s.least[wave] = T;
+    if (threadIdx.x == 0) s.count = 0;
+    __syncthreads();
+    #pragma unroll
+    for (int w = 0; w < LP_WAVES; w++) T = max(T, s.least[w]);
+    T = max(T, 1u);
+    if (__any(mx >= T)) {
+        #pragma unroll
+        for (int e = 0; e < N; e++) {
+            const uint64_t x = key(e);
+            if ((uint32_t)(x >> 32) >= T) {
+                const int at = atomicAdd(&s.count, 1);
+                if (at < LP_LIST) s.list[at] = x;
+            }
+        }
+    }
+    __syncthreads();
+    const int n = s.count;
+    if (n <= LP_LIST) {
+        for (int i = threadIdx.x; i < n; i += LP_THREADS) {
+            const uint64_t x = s.list[i];
+            int rank = 0;
+            for (int j = 0; j < n; j++) rank += s.list[j] > x;
+            if (rank < k) dst[rank] = x;
+        }
+        for (int i = n + threadIdx.x; i < k; i += LP_THREADS) dst[i] = 0;
+        return;
+    }
+    uint64_t last = ~0ull;
+    for (int i = 0; i < k; i++) {
+        uint64_t best = 0;
+        #pragma unroll
+        for (int e = 0; e < N; e++) {
+            const uint64_t x = key(e);
+            if (x < last && x > best) best = x;
+        }
+        __syncthreads();
+        last = lp_block(best, s.red, [](uint64_t p, uint64_t q) { return p > q ? p : q; });
+        if (threadIdx.x == 0) dst[i] = last;
+    }
+}
+
+// A segment's part of its row: M, r, sum of e^d d; nan != 0: it holds a NaN.
+struct LpPart { float m, r, e1, nan; };
+
+// grid (segments, rows); keys [row][segment][n_top]
+template <int N>
+__global__ __launch_bounds__(LP_THREADS) void k_lp_part(sp_hipkv_logprob_args a, LpPart *part, uint64_t *keys) {
+    __shared__ float red[5][LP_WAVES];
+    __shared__ LpSelect sel;
+    const int row = blockIdx.y, t0 = blockIdx.x * N * LP_THREADS + threadIdx.x * 4;
+    const float *x = a.logits + row * a.stride;
+    float v[N];
+    bool in[N / 4];                              // a group of four is whole, or absent but for the vocabulary's end
+    #pragma unroll
+    for (int k = 0; k < N / 4; k++) {
+        const int t = t0 + k * 4 * LP_THREADS;
+        in[k] = t < a.vocab;
+        v4u f = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+        if (t + 4 <= a.vocab) f = *(const v4u *)(x + t);
+        else if (in[k]) {
+            f[0] = x[t];
+            if (t + 1 < a.vocab) f[1] = x[t + 1];
+            if (t + 2 < a.vocab) f[2] = x[t + 2];
+        }
+        #pragma unroll
+        for (int e = 0; e < 4; e++) v[4 * k + e] = f[e];
+    }
+    float m = -INFINITY, nan = 0.0f;
+    #pragma unroll
+    for (int e = 0; e < N; e++) {
+        const float y = v[e] * a.scale;
+        m = fmaxf(m, y);
+        nan = y != y ? 1.0f : nan;
+    }
+    m = lp_block(m, red[0], [](float p, float q) { return fmaxf(p, q); });
+    float r = 0.0f, e1 = 0.0f, same = 0.0f;
+    #pragma unroll
+    for (int e = 0; e < N; e++) {
+        const float d = fmaxf(v[e] * a.scale - m, -200.0f);      // e^-200 is 0
+        const float w = d < 0.0f ? __builtin_amdgcn_exp2f(d * 1.44269504088896341f) : 0.0f;
+        r += w; e1 += w * d;
+        same += d == 0.0f ? 1.0f : 0.0f;
+    }
+    #pragma unroll
+    for (int o = 32; o; o >>= 1) {
+        r += __shfl_xor(r, o, 64); e1 += __shfl_xor(e1, o, 64);
+        same += __shfl_xor(same, o, 64); nan = fmaxf(nan, __shfl_xor(nan, o, 64));
+    }
+    if ((threadIdx.x & 63) == 0) {
+        const int w = threadIdx.x >> 6;
+        red[1][w] = r; red[2][w] = e1; red[3][w] = nan; red[4][w] = same;      // r without the count, which would swallow it
+    }
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        float rs = 0.0f, sm = 0.0f, es = 0.0f, ns = 0.0f;
+        #pragma unroll
+        for (int w = 0; w < LP_WAVES; w++) {
+            rs += red[1][w]; es += red[2][w]; ns = fmaxf(ns, red[3][w]); sm += red[4][w];
+        }
+        part[(size_t)row * gridDim.x + blockIdx.x] = {m, rs + (sm - 1.0f), es, ns};
+    }
+    if (!a.n_top) return;
+    // absent places are below every logit
+    lp_select<N>(sel, a.n_top, [&](int e) {
+        const int t = t0 + (e / 4) * 4 * LP_THREADS + e % 4;
+        return in[e / 4] && t < a.vocab ? lp_key(lp_order(v[e]), t) : 0;
+    }, keys + ((size_t)row * gridDim.x + blockIdx.x) * a.n_top);
+}
+
+// one workgroup per row
+__global__ __launch_bounds__(LP_THREADS) void k_lp_merge(sp_hipkv_logprob_args a, int segs, const LpPart *part, const uint64_t *keys) {
+    __shared__ float redf[LP_WAVES];
+    __shared__ double redd[3][LP_WAVES];
+    __shared__ LpSelect sel;
+    __shared__ uint64_t top[32];
     const int row = blockIdx.x;
     const float *x = a.logits + row * a.stride;
-    float m = -INFINITY, bad = 0.0f;
-    for (int t = threadIdx.x; t < a.vocab; t += LP_THREADS) {
-        const float y = x[t] * a.scale;
-        if (y != y) bad = 1.0f;
-        m = fmaxf(m, y);
-    }
-    m = lp_block(m, red4, [](float p, float q) { return fmaxf(p, q); });
-    bad = lp_block(bad, red4, [](float p, float q) { return fmaxf(p, q); });
-    float r = 0.0f, e1 = 0.0f, same = 0.0f;
-    for (int t = threadIdx.x; t < a.vocab; t += LP_THREADS) {
-        const float d = x[t] * a.scale - m;
-        if (d == 0.0f) same += 1.0f;
-        else if (d > -INFINITY) { const float e = expf(d); r += e; e1 += e * d; }
-    }
-    auto add = [](float p, float q) { return p + q; };
-    same = lp_block(same, red4, add);
-    r = lp_block(r, red4, add) + (same - 1.0f);
-    e1 = lp_block(e1, red4, add);
-    const bool nan = bad != 0.0f, odd = nan || m == INFINITY || m == -INFINITY;
-    const float lr = odd ? NAN : log1pf(r);
+    const bool mine = (int)threadIdx.x < segs;
+    LpPart p = {-INFINITY, 0.0f, 0.0f, 0.0f};
+    if (mine) p = part[(size_t)row * segs + threadIdx.x];
+    const float M = lp_block(p.m, redf, [](float u, float w) { return fmaxf(u, w); });
+    // NaN as a count in the same sum
+    const bool live = mine && p.m > -INFINITY && M < INFINITY;
+    const double f = live ? exp((double)p.m - (double)M) : 0.0;
+    auto add = [](double u, double w) { return u + w; };
+    const bool at = live && p.m == M;
+    double r = live ? (at ? (double)p.r : f * (1.0 + (double)p.r)) : 0.0;
+    double e1 = live ? f * ((double)p.e1 + ((double)p.m - (double)M) * (1.0 + (double)p.r)) : 0.0;
+    r = lp_block(r, redd[0], add);
+    e1 = lp_block(e1, redd[1], add);
+    const double n = lp_block((at ? 1.0 : 0.0) + (p.nan != 0.0f ? 65536.0 : 0.0), redd[2], add);
+    const bool nan = n >= 65536.0, odd = nan || M == INFINITY || M == -INFINITY;
+    r += n - 1.0;
+    const float lr = odd ? NAN : (float)log1p(r);
     if (threadIdx.x == 0) {
-        if (a.lse) a.lse[row] = nan ? NAN : odd ? m : m + lr;
-        if (a.entropy) a.entropy[row] = odd ? NAN : lr - e1 / (1.0f + r);
+        if (a.lse) a.lse[row] = nan ? NAN : odd ? M : (float)((double)M + log1p(r));
+        if (a.entropy) a.entropy[row] = odd ? NAN : (float)(log1p(r) - e1 / (1.0 + r));
     }
     for (int i = threadIdx.x; i < a.n_given; i += LP_THREADS) {
         const int t = a.given[(size_t)row * a.n_given + i];
-        a.given_logprob[(size_t)row * a.n_given + i] = t < 0 || t >= a.vocab ? NAN : x[t] * a.scale - m - lr;
+        a.given_logprob[(size_t)row * a.n_given + i] = t < 0 || t >= a.vocab ? NAN : x[t] * a.scale - M - lr;
     }
-    uint64_t last = ~0ull;
-    for (int i = 0; i < a.n_top; i++) {
-        uint64_t best = 0;
-        for (int t = threadIdx.x; t < a.vocab; t += LP_THREADS) {
-            const uint64_t k = lp_key(x[t], t);
-            if (k < last && k > best) best = k;
-        }
-        last = lp_block(best, red8, [](uint64_t p, uint64_t q) { return p > q ? p : q; });
-        if (threadIdx.x == 0) {
-            const int t = (int)~(uint32_t)last;
-            a.top_ids[(size_t)row * a.n_top + i] = t;
-            if (a.top_logprob) a.top_logprob[(size_t)row * a.n_top + i] = x[t] * a.scale - m - lr;
-        }
+    if (!a.n_top) return;
+    const int have = segs * a.n_top;
+    const uint64_t *kr = keys + (size_t)row * have;
+    constexpr int N = LP_SEGS * 32 / LP_THREADS;
+    uint64_t k[N];
+    #pragma unroll
+    for (int e = 0; e < N; e++) k[e] = e * LP_THREADS + (int)threadIdx.x < have ? kr[e * LP_THREADS + threadIdx.x] : 0;
+    lp_select<N>(sel, a.n_top, [&](int e) { return k[e]; }, top);
+    __syncthreads();
+    if ((int)threadIdx.x < a.n_top) {
+        const int t = (int)~(uint32_t)top[threadIdx.x];
+        a.top_ids[(size_t)row * a.n_top + threadIdx.x] = t;
+        if (a.top_logprob) a.top_logprob[(size_t)row * a.n_top + threadIdx.x] = x[t] * a.scale - M - lr;
     }
 }
+
+// Segments of 2048 logits where that is what it takes to use the device, else of 8192
+// (one row of 151936: 75 workgroups for 19).
+struct LpPlan { int per, segs; };
+LpPlan lp_plan(const sp_hipkv_logprob_args &a) {
+    const int longs = (a.vocab + LP_LONG * LP_THREADS - 1) / (LP_LONG * LP_THREADS);
+    const int shorts = (a.vocab + LP_SHORT * LP_THREADS - 1) / (LP_SHORT * LP_THREADS);
+    if (shorts <= LP_SEGS && (int64_t)a.n_rows * longs < 512) return {LP_SHORT, shorts};
+    return {LP_LONG, longs};
+}
+size_t lp_part_bytes(const sp_hipkv_logprob_args &a, const LpPlan &p) { return (size_t)a.n_rows * p.segs * sizeof(LpPart); }
 
 int logprob_check(const char *who, const sp_hipkv_logprob_args *a) {
     OP_NEED(a, "null arguments");
     OP_NEED(a->n_rows >= 0 && a->n_rows <= 65535, "n_rows outside [0, 65535]");
-    OP_NEED(a->vocab >= 1 && a->vocab <= 1 << 24, "vocab outside [1, 2^24]");
+    OP_NEED(a->vocab >= 1 && a->vocab <= LP_SEGS * LP_LONG * LP_THREADS, "vocab outside [1, 2^20]");
     OP_NEED(a->n_given >= 0 && a->n_given <= 64, "n_given outside [0, 64]");
     OP_NEED(a->n_top >= 0 && a->n_top <= 32 && a->n_top <= a->vocab, "n_top outside [0, 32] or above vocab");
     return 0;
@@ -107,7 +252,13 @@ int logprob_check_arrays(const char *who, const sp_hipkv_logprob_args *a, size_t
 }  // namespace
 
 void launch_logprob(const sp_hipkv_logprob_args &a, hipStream_t s) {
-    hipLaunchKernelGGL(k_logprob_row, dim3(a.n_rows), dim3(LP_THREADS), 0, s, a);
+    const LpPlan p = lp_plan(a);
+    LpPart *part = (LpPart *)a.work;
+    uint64_t *keys = (uint64_t *)((uint8_t *)a.work + lp_part_bytes(a, p));
+    const dim3 grid(p.segs, a.n_rows), wg(LP_THREADS);
+    if (p.per == LP_LONG) hipLaunchKernelGGL(k_lp_part<LP_LONG>, grid, wg, 0, s, a, part, keys);
+    else hipLaunchKernelGGL(k_lp_part<LP_SHORT>, grid, wg, 0, s, a, part, keys);
+    hipLaunchKernelGGL(k_lp_merge, dim3(a.n_rows), wg, 0, s, a, p.segs, part, keys);
 }
 
 }  // namespace kvd
@@ -117,7 +268,8 @@ extern "C" int sp_hipkv_token_logprobs_work(const sp_hipkv_logprob_args *a, size
     const char *who = "sp_hipkv_token_logprobs_work";
     if (logprob_check(who, a)) return 1;
     OP_NEED(bytes, "null bytes");
-    *bytes = 0;
+    const LpPlan p = lp_plan(*a);
+    *bytes = lp_part_bytes(*a, p) + (size_t)a->n_rows * p.segs * a->n_top * sizeof(uint64_t);
     return 0;
 }
 

@@ -59,7 +59,7 @@ def logprob(**kw):
 
 
 @pytest.mark.parametrize("bad", [
-    dict(n_rows=-1), dict(n_rows=65536), dict(vocab=0), dict(vocab=(1 << 24) + 1), dict(n_given=-1), dict(n_given=65), dict(n_top=-1),
+    dict(n_rows=-1), dict(n_rows=65536), dict(vocab=0), dict(vocab=(1 << 20) + 1, stride=1 << 21), dict(n_given=-1), dict(n_given=65), dict(n_top=-1),
     dict(n_top=33), dict(vocab=4, stride=4), dict(scale=0.0), dict(scale=-1.0), dict(scale=float("nan")), dict(scale=float("inf")),
     dict(stride=999), dict(logits=None), dict(logits=P + 2), dict(given=None), dict(given_logprob=None), dict(top_ids=None),
 ])
