@@ -1195,7 +1195,7 @@ int alloc_batch(sp_kvdecode_handle *h) {
 // TREE: one session's drafted nodes, stored at positions pos0.. and rotated for
 // b.tpos (tokens in b.toks); SCORE: a prefill; both with the LM head's logits.
 enum BatchKind { PREFILL, MULTI, TREE, SCORE };
-bool tree_attention(sp_kvdecode_handle *h, const AttnArgs &a, int layer, hipStream_t s);
+int tree_attention(sp_kvdecode_handle *h, const AttnArgs &a, int layer, size_t *need = nullptr);
 
 int run_batch(sp_kvdecode_handle *h, int T, int pos0, int pos_hi, BatchKind kind, TimeCb cb = nullptr, void *ctx = nullptr) {
     const bool multi = kind == MULTI, own_pos = multi || kind == TREE;
@@ -1268,7 +1268,16 @@ int run_batch(sp_kvdecode_handle *h, int T, int pos0, int pos_hi, BatchKind kind
         // sums must not depend on what other sessions left
         if (!multi) a.part_slots = b.TB * (h->pmax / 64 + 2);
         if (kind == TREE) {
-            if (!tree_attention(h, a, l, s)) return fail("sp_hipkv_tree_step: the attention's work does not fit the batch buffers%s");
+            size_t need = 0;
+            if (tree_attention(h, a, l, &need)) return 1;
+            if (need > b.tbytes) {                              // first call, or a longer one
+                HIPCHK(hipStreamSynchronize(s), "tree work");
+                if (b.tbuf) hipFree(b.tbuf);
+                b.tbuf = nullptr; b.tbytes = 0;
+                HIPCHK(dev_malloc(&b.tbuf, need), "tree work alloc");
+                b.tbytes = need;
+            }
+            tree_attention(h, a, l);
         } else if (prefill_attention_float(a)) launch_prefill_float(a, s);
         else for (int t = 0; t < T; t += b.TB) {                // one pass for a batched decode
             AttnArgs c = a;
@@ -1330,10 +1339,9 @@ int ring_batch(const sp_kvdecode_handle *h, int most) {
     return std::max(most, 1);
 }
 
-// One layer's attention of a drafted tree: the scratch of the batch's attention as its work.
-bool tree_attention(sp_kvdecode_handle *h, const AttnArgs &a, int layer, hipStream_t s) {
-    const DevModel *m = h->m;
-    const auto &b = h->b;
+// One layer's attention of a drafted tree, or (need) the bytes of its work.
+int tree_attention(sp_kvdecode_handle *h, const AttnArgs &a, int layer, size_t *need) {
+    hipStream_t s = h->stream;
     TreeBuf *d = h->d_tree;
     sp_hipkv_tree_args t{};
     t.n_heads = a.NH; t.n_kv_heads = a.NKV; t.head_dim = a.HD;
@@ -1343,14 +1351,10 @@ bool tree_attention(sp_kvdecode_handle *h, const AttnArgs &a, int layer, hipStre
     t.node_start = d->node_start; t.cached = &d->cached; t.depth = d->depth; t.visible = &d->visible[a.win >= 0][0][0];
     t.tables = (const void *const *const *)(h->d_lists + layer);
     t.q = a.qr; t.out = a.ao; t.q_stride = t.out_stride = (int64_t)a.NH * a.HD;
-    size_t need = 0;
-    if (sp_hipkv_tree_attention_work(&t, &need)) return false;
-    t.work = a.mode == EXACT ? (void *)b.zs : (void *)b.part;
-    t.work_bytes = need;
-    const size_t room = a.mode == EXACT ? (size_t)b.TB * m->NH * h->max_chunks * 16 * 4 : (size_t)b.TB * m->NH * (h->pmax / 64 + 2) * m->HD * 4;
-    if (need > room) return false;
+    t.work = h->b.tbuf;
+    if (need) return sp_hipkv_tree_attention_work(&t, need);
     launch_tree(t, s);
-    return true;
+    return 0;
 }
 
 // The batched decode's buffers of the leased set: logits rows, tokens, positions, tables.

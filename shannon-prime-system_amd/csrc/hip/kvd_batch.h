@@ -40,6 +40,8 @@ struct Batch {
     hipEvent_t slot_ev[LOGIT_SLOTS] = {};
     // log probabilities (allocated on first use): the operator's arrays for TB rows, and their pinned mirror
     void *sbuf = nullptr, *hsbuf = nullptr;
+    void *tbuf = nullptr;                // work of a drafted tree's attention (grown to what a call needs)
+    size_t tbytes = 0;
     bool serves(bool f, int p) const { return (flt || !f) && pmax >= p; }
     void release() {
         if (buf) hipFree(buf);
@@ -47,6 +49,7 @@ struct Batch {
         if (hstage) hipHostFree(hstage);
         if (sbuf) hipFree(sbuf);
         if (hsbuf) hipHostFree(hsbuf);
+        if (tbuf) hipFree(tbuf);
         for (hipEvent_t e : slot_ev) if (e) hipEventDestroy(e);
         *this = Batch{};
     }

@@ -7,8 +7,8 @@
 //                      w_p = exp_fixed((z_p - M) 2^16) >> 8, out = RNE(sum w vq / (2^16 sum w)),
 // the decode attention's integers (kvd_attn.hip).
 //
-// f32 and Spinor rows run on the f32 matrix cores (k_tree_float below), exact rows
-// one workgroup per row.
+// f32 and Spinor rows run on the f32 matrix cores in one pass over K and V
+// (k_tree_float), exact rows on the int8 matrix cores in two (k_tree_xscore, _xsum).
 #include "kvd_op.h"
 #include "kvd_exact.h"
 #include "kvd_vec.h"
@@ -17,8 +17,6 @@
 namespace kvd {
 
 namespace {
-
-constexpr int TREE_WAVES = 4;
 
 // What a workgroup needs of its sequence.
 struct TreeSeq {
@@ -43,55 +41,9 @@ __device__ __forceinline__ const uint8_t *tree_page(const sp_hipkv_tree_args &a,
     return (const uint8_t *)gmem(q.table)[a.ring_pages ? lp % a.ring_pages : lp];
 }
 
-template <int EPL>
-__global__ __launch_bounds__(64 * TREE_WAVES) void k_tree_exact(sp_hipkv_tree_args a) {
-    constexpr int HD = EPL * 64;
-    const int head = blockIdx.x, node = blockIdx.y, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const TreeSeq q = tree_seq(a, blockIdx.z);
-    if (node >= q.nodes) return;
-    const int h = head / (a.n_heads / a.n_kv_heads), low = tree_low(a, q, node);
-    const uint64_t *mask = a.visible + (size_t)(q.node0 + node) * a.mask_words;
-    const float *qp = a.q + (size_t)(q.node0 + node) * a.q_stride + head * HD;
-    int64_t qi[EPL];
-    #pragma unroll
-    for (int e = 0; e < EPL; e++) qi[e] = (int64_t)rintf(qp[lane + 64 * e] * 65536.0f);
-    auto row_of = [&](int p, int v) { return (const int32_t *)tree_page(a, q, p) + ((size_t)(v * a.n_kv_heads + h) * PAGE + (p & (PAGE - 1))) * HD; };
-    auto sees = [&](int p) { return p < q.cached ? p >= low : (mask[(p - q.cached) >> 6] >> ((p - q.cached) & 63) & 1) != 0; };
-    auto grid_score = [&](int p) {
-        const int32_t *k = row_of(p, 0);
-        int64_t ip = 0;
-        #pragma unroll
-        for (int e = 0; e < EPL; e++) ip += qi[e] * k[lane + 64 * e];
-        return (int)llround_pow2<14>((float)((double)wave_allsum(ip) / 4294967296.0) * a.scale);
-    };
-    __shared__ int zm[TREE_WAVES];
-    __shared__ int64_t sw[TREE_WAVES], sv[TREE_WAVES][HD];
-    const int end = q.cached + q.nodes;
-    float *out = a.out + (size_t)(q.node0 + node) * a.out_stride + head * HD;
-    int M = INT32_MIN;
-    for (int p = low + wave; p < end; p += TREE_WAVES)
-        if (sees(p)) M = max(M, grid_score(p));
-    if (lane == 0) zm[wave] = M;
-    __syncthreads();
-    for (int w = 0; w < TREE_WAVES; w++) M = max(M, zm[w]);
-    int64_t S = 0, o[EPL] = {};
-    for (int p = low + wave; p < end; p += TREE_WAVES)
-        if (sees(p)) {
-            const int64_t w = exp_fixed((((int64_t)grid_score(p) - M) * ONE) >> 14) >> 8;
-            const int32_t *v = row_of(p, 1);
-            S += w;
-            #pragma unroll
-            for (int e = 0; e < EPL; e++) o[e] += w * v[lane + 64 * e];
-        }
-    if (lane == 0) sw[wave] = S;
-    #pragma unroll
-    for (int e = 0; e < EPL; e++) sv[wave][lane + 64 * e] = o[e];
-    __syncthreads();
-    for (int d = threadIdx.x; d < HD; d += 64 * TREE_WAVES) {
-        int64_t t = 0, den = 0;
-        for (int w = 0; w < TREE_WAVES; w++) { t += sv[w][d]; den += sw[w]; }
-        out[d] = den ? rne_div_to_float((i128)t, den, 16) : 0.0f;
-    }
+__device__ __forceinline__ const uint8_t *uniform(const uint8_t *x) {
+    const uint64_t p = (uint64_t)x;
+    return (const uint8_t *)((uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(p >> 32)) << 32 | (uint32_t)__builtin_amdgcn_readfirstlane((int)p));
 }
 
 // ---------------------------------------------------------------- f32 and Spinor rows
@@ -177,11 +129,7 @@ __global__ __launch_bounds__(256, 2) void k_tree_float(sp_hipkv_tree_args a, int
     __syncthreads();
     const uint32_t kslice = (uint32_t)h * PAGE * RB, vslice = (uint32_t)(a.n_kv_heads + h) * PAGE * RB;
     // page addresses are the wave's: rows load as address + 32-bit lane offset
-    auto page = [&](int lp) {
-        const uint64_t p = (uint64_t)tree_page(a, q, lp * PAGE);
-        return (const uint8_t *)((uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(p >> 32)) << 32 |
-                                 (uint32_t)__builtin_amdgcn_readfirstlane((int)p));
-    };
+    auto page = [&](int lp) { return uniform(tree_page(a, q, lp * PAGE)); };
     // positions past the last one repeat it
     auto row_off = [&](int lp, int x) { const int p = lp * PAGE + wave * TT + x; return (uint32_t)((p < end ? p : end - 1) & (PAGE - 1)) * RB; };
     // tiles that some row does not see whole, and those of them put off to the end:
@@ -543,6 +491,402 @@ __global__ __launch_bounds__(256) void k_tree_merge(sp_hipkv_tree_args a, int ns
     *(v4f *)(a.out + (row / a.n_heads) * a.out_stride + (row % a.n_heads) * HD + 4 * c) = M > -INFINITY ? x / L : (v4f){0, 0, 0, 0};
 }
 
+// ---------------------------------------------------------------- exact rows
+// Integer sums are exact in any order, so both products run on the int8 matrix cores
+// (v_mfma_i32_16x16x64_i8) over balanced base-256 digits, three of each number where
+// they fit (|x| <= 127 (1 + 2^8 + 2^16)); products of equal place share an int32 sum.
+//   k_tree_xscore: z of every (row, position) into `work`, and each split's maxima;
+//   k_tree_xsum:   weights (22 bits) from z and M, V sums as int64 of a split;
+//   k_tree_xdiv:   the splits' sums, divided.
+// The weights need M before the first of them, hence z in memory: 4 bytes a row and
+// position, written and read once, against 8 HD bytes of K and V for all G nodes rows.
+//
+// Scores: as in the f32 kernel a wave takes 16 positions straight into registers, here
+// as the B operand (16 dims a lane and step, in an order that q's digits in LDS
+// share), makes their digits once and multiplies them with all row tiles.
+// V sums: a wave owns 32 columns and takes a page a step: lane l 16 positions of two
+// columns, which are the B operand after their digits are formed; no transposition.
+// The weights' digits are made once for all waves and pass through LDS.
+typedef int v4i __attribute__((ext_vector_type(4)));
+constexpr int DIG3 = 127 * (1 + 256 + 65536);                    // largest |x| of three balanced digits
+constexpr int DIG4 = 127 * (1 + 256 + 65536 + 16777216);         // ... of four
+
+// x = d0 + 2^8 d1 + 2^16 d2 + 2^24 d3, d in [-128, 127]; four values' digits, one dword per place
+__device__ __forceinline__ void digits_of(const int32_t x[4], uint32_t w[4]) {
+    uint32_t d[4];
+    #pragma unroll
+    for (int e = 0; e < 4; e++) d[e] = ((uint32_t)x[e] + 0x80808080u) ^ 0x80808080u;
+    const uint32_t ab0 = __builtin_amdgcn_perm(d[1], d[0], 0x05010400u), ab2 = __builtin_amdgcn_perm(d[1], d[0], 0x07030602u);
+    const uint32_t cd0 = __builtin_amdgcn_perm(d[3], d[2], 0x05010400u), cd2 = __builtin_amdgcn_perm(d[3], d[2], 0x07030602u);
+    w[0] = __builtin_amdgcn_perm(cd0, ab0, 0x05040100u); w[1] = __builtin_amdgcn_perm(cd0, ab0, 0x07060302u);
+    w[2] = __builtin_amdgcn_perm(cd2, ab2, 0x05040100u); w[3] = __builtin_amdgcn_perm(cd2, ab2, 0x07060302u);
+}
+// 1: |x| needs a fourth digit, 2: more than four
+__device__ __forceinline__ int level_of(int32_t x) {
+    return ((uint32_t)x + (uint32_t)DIG3 > 2u * DIG3 ? 1 : 0) | ((uint32_t)x + (uint32_t)DIG4 > 2u * DIG4 ? 2 : 0);
+}
+// exp_fixed((z - M) 2^16) >> 8 for z <= M: 2^-g, g = ceil((M - z) log2(e) 2^30 / 2^14) in 30 bits
+__device__ __forceinline__ int32_t weight_of(int32_t z, int32_t M) {
+    const uint64_t g = ((uint64_t)((uint32_t)M - (uint32_t)z) * (uint32_t)LOG2E + 16383) >> 14;
+    const uint32_t n = (uint32_t)(g >> FB), r = (uint32_t)g & (uint32_t)(ONE - 1);
+    if (n >= 23) return 0;
+    return r ? (int32_t)(exp2_frac((uint32_t)ONE - r) >> (n + 9)) : (int32_t)((uint32_t)ONE >> (n + 8));
+}
+
+// Work of exact rows: z [row][zstride], maxima [row][nsplit], V sums [row][vsplit][HD],
+// denominators [row][vsplit]; row = node n_heads + head.
+struct XWork { int32_t *z, *zmax; int64_t *sum, *den; int zstride, nsplit, vsplit; };
+// z is kept by position less the first page's that any node of the sequence sees
+__device__ __forceinline__ int z_first(const sp_hipkv_tree_args &a, const TreeSeq &q) {
+    return a.window ? max(q.cached - a.window + 1, 0) & ~(PAGE - 1) : 0;
+}
+// the span of pages that rows [r0, r1) of a kv head see
+struct Span { int lo_min, lo_max, pg0, pg1; };
+__device__ __forceinline__ Span rows_span(const sp_hipkv_tree_args &a, const TreeSeq &q, int G, int r0, int r1) {
+    Span s = {0, 0, 0, (q.cached + q.nodes + PAGE - 1) / PAGE};
+    if (a.window) {
+        s.lo_min = INT32_MAX;
+        for (int r = r0 + (int)(threadIdx.x & 63); r < r1; r += 64) {
+            const int lo = tree_low(a, q, r / G);
+            s.lo_min = min(s.lo_min, lo); s.lo_max = max(s.lo_max, lo);
+        }
+        s.lo_max = wave_allmax_i(s.lo_max);
+        s.lo_min = -wave_allmax_i(-s.lo_min);
+    }
+    s.pg0 = s.lo_min / PAGE;
+    return s;
+}
+__device__ __forceinline__ bool row_sees(const sp_hipkv_tree_args &a, const TreeSeq &q, int node, int p) {
+    const int j = p - q.cached;
+    if (j < 0) return p >= tree_low(a, q, node);
+    return j < q.nodes && (gmem(a.visible)[(size_t)(q.node0 + node) * a.mask_words + (j >> 6)] >> (j & 63) & 1);
+}
+
+template <int EPL, int RT>
+__global__ __launch_bounds__(256, 2) void k_tree_xscore(sp_hipkv_tree_args a, XWork x, int groups) {
+    constexpr int HD = EPL * 64, KS = EPL, QROW = HD + 16;
+    __shared__ __align__(16) int8_t qd[4][RT * 16][QROW];          // q's digits [place][row][64 ks + 16 g + 4 quarter + e]
+    __shared__ int s_level, s_mx[4][RT * 16];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), l16 = lane & 15, g = lane >> 4;
+    const int G = a.n_heads / a.n_kv_heads;
+    int id = blockIdx.x;
+    const int h = id % a.n_kv_heads; id /= a.n_kv_heads;
+    const int grp = id % groups; id /= groups;
+    const int split = id % x.nsplit;
+    const TreeSeq q = tree_seq(a, id / x.nsplit);
+    const int R = q.nodes * G, r0 = grp * RT * 16;
+    if (r0 >= R) return;
+    if (threadIdx.x == 0) s_level = 0;
+    __syncthreads();
+    const int end = q.cached + q.nodes, z0 = z_first(a, q);
+    int level = 0;
+    for (int i = threadIdx.x; i < RT * 16 * (HD / 4); i += 256) {
+        const int r = i / (HD / 4), c = i % (HD / 4);
+        int32_t v[4] = {0, 0, 0, 0};
+        if (r0 + r < R) {
+            const float4 f = *(const float4 *)(a.q + (size_t)(q.node0 + (r0 + r) / G) * a.q_stride + (size_t)(h * G + (r0 + r) % G) * HD + 4 * c);
+            v[0] = (int32_t)rintf(f.x * 65536.0f); v[1] = (int32_t)rintf(f.y * 65536.0f);
+            v[2] = (int32_t)rintf(f.z * 65536.0f); v[3] = (int32_t)rintf(f.w * 65536.0f);
+        }
+        uint32_t w[4];
+        #pragma unroll
+        for (int e = 0; e < 4; e++) level |= level_of(v[e]);
+        digits_of(v, w);
+        // dims 64 ks + 16 quarter + 4 g + e
+        const int at = (c / 16) * 64 + (c % 4) * 16 + (c / 4 % 4) * 4;
+        #pragma unroll
+        for (int b = 0; b < 4; b++) *(uint32_t *)&qd[b][r][at] = w[b];
+    }
+    level = (__any(level & 1) ? 1 : 0) | (__any(level & 2) ? 2 : 0);
+    if (level && lane == 0) atomicOr(&s_level, level);
+    const Span sp = rows_span(a, q, G, r0, min(r0 + RT * 16, R));
+    const int per = (sp.pg1 - sp.pg0 + x.nsplit - 1) / x.nsplit;
+    int w0 = sp.pg0 + split * per, w1 = min(w0 + per, sp.pg1);
+    if (w0 < w1 && w0 * PAGE + wave * TT + TT <= sp.lo_min) w0++;
+    if (w0 < w1 && (w1 - 1) * PAGE + wave * TT >= end) w1--;
+    // this lane's output rows: 4 g + i of each tile
+    int mx[RT][4], zrow[RT][4];
+    #pragma unroll
+    for (int t = 0; t < RT; t++)
+        #pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const int r = r0 + t * 16 + 4 * g + i;
+            mx[t][i] = INT32_MIN;
+            zrow[t][i] = r < R ? (q.node0 + r / G) * a.n_heads + h * G + r % G : -1;
+        }
+    __syncthreads();
+    const int qlevel = s_level;
+    const uint32_t kslice = (uint32_t)h * PAGE * HD * 4;
+    auto page = [&](int lp) { return uniform(tree_page(a, q, lp * PAGE)); };
+    auto load_k = [&](v4i (&k)[4 * KS], const uint8_t *pg, int lp) {
+        const int p = lp * PAGE + wave * TT + l16;
+        const uint32_t off = kslice + (uint32_t)((p < end ? p : end - 1) & (PAGE - 1)) * (HD * 4) + 16 * g;
+        #pragma unroll
+        for (int s = 0; s < 4 * KS; s++) k[s] = *gmem((const v4i *)(pg + off + 64 * s));
+    };
+    v4i K[4 * KS];
+    const uint8_t *pg = nullptr, *pn = nullptr;
+    if (w0 < w1) {
+        pg = page(w0);
+        load_k(K, pg, w0);
+        pn = page(min(w0 + 1, w1 - 1));
+    }
+    for (int lp = w0; lp < w1; lp++) {
+        const int p0 = lp * PAGE + wave * TT, p = p0 + l16;
+        const bool whole = p0 >= sp.lo_max && p0 + TT <= q.cached;
+        v4i B[4][KS];
+        int lv = 0;
+        #pragma unroll
+        for (int s = 0; s < 4 * KS; s++) {
+            const int32_t v[4] = {K[s][0], K[s][1], K[s][2], K[s][3]};
+            uint32_t w[4];
+            #pragma unroll
+            for (int e = 0; e < 4; e++) lv |= level_of(v[e]);
+            digits_of(v, w);
+            #pragma unroll
+            for (int b = 0; b < 4; b++) B[b][s / 4][s % 4] = (int)w[b];
+        }
+        lv = qlevel | (__any(lv & 1) ? 1 : 0) | (__any(lv & 2) ? 2 : 0);
+        __builtin_amdgcn_sched_barrier(0);
+        load_k(K, pn, min(lp + 1, w1 - 1));
+        __builtin_amdgcn_sched_barrier(0);
+        auto dots = [&](auto nd, int t, int64_t (&ip)[4]) {
+            constexpr int ND = decltype(nd)::value;
+            v4i acc[2 * ND - 1];
+            #pragma unroll
+            for (int k = 0; k < 2 * ND - 1; k++) acc[k] = (v4i){0, 0, 0, 0};
+            #pragma unroll
+            for (int ks = 0; ks < KS; ks++) {
+                v4i A[ND];
+                #pragma unroll
+                for (int b = 0; b < ND; b++) A[b] = *(const v4i *)&qd[b][t * 16 + l16][64 * ks + 16 * g];
+                #pragma unroll
+                for (int u = 0; u < ND; u++)
+                    #pragma unroll
+                    for (int b = 0; b < ND; b++) acc[u + b] = __builtin_amdgcn_mfma_i32_16x16x64_i8(A[u], B[b][ks], acc[u + b], 0, 0, 0);
+            }
+            #pragma unroll
+            for (int i = 0; i < 4; i++) {
+                ip[i] = acc[2 * ND - 2][i];
+                #pragma unroll
+                for (int k = 2 * ND - 3; k >= 0; k--) ip[i] = ip[i] * 256 + acc[k][i];
+            }
+        };
+        #pragma unroll
+        for (int t = 0; t < RT; t++) {
+            int64_t ip[4];
+            if (lv == 0) dots(std::integral_constant<int, 3>{}, t, ip);
+            else if (lv == 1) dots(std::integral_constant<int, 4>{}, t, ip);
+            else {                                                         // more than four digits: from the numbers
+                const int32_t *kr = (const int32_t *)(pg + kslice) + (size_t)((p < end ? p : end - 1) & (PAGE - 1)) * HD;
+                for (int i = 0; i < 4; i++) {
+                    const int r = min(r0 + t * 16 + 4 * g + i, R - 1);
+                    const float *qr = a.q + (size_t)(q.node0 + r / G) * a.q_stride + (size_t)(h * G + r % G) * HD;
+                    int64_t s = 0;
+                    for (int d = 0; d < HD; d++) s += (int64_t)(int32_t)rintf(qr[d] * 65536.0f) * gmem(kr)[d];
+                    ip[i] = s;
+                }
+            }
+            #pragma unroll
+            for (int i = 0; i < 4; i++) {
+                const float sc = (float)((double)ip[i] / 4294967296.0) * a.scale;
+                const int32_t z = (int32_t)llround_pow2<14>(sc);
+                if (zrow[t][i] >= 0 && p < end) {
+                    x.z[(size_t)zrow[t][i] * x.zstride + (p - z0)] = z;
+                    if (whole || row_sees(a, q, zrow[t][i] / a.n_heads - q.node0, p)) mx[t][i] = max(mx[t][i], z);
+                }
+            }
+        }
+        pg = pn;
+        pn = page(min(lp + 2, w1 - 1));
+    }
+    #pragma unroll
+    for (int t = 0; t < RT; t++)
+        #pragma unroll
+        for (int i = 0; i < 4; i++) {
+            #pragma unroll
+            for (int o = 1; o < 16; o <<= 1) mx[t][i] = max(mx[t][i], __shfl_xor(mx[t][i], o, 64));
+            if (l16 == 0) s_mx[wave][t * 16 + 4 * g + i] = mx[t][i];
+        }
+    __syncthreads();
+    if (threadIdx.x < RT * 16 && r0 + (int)threadIdx.x < R) {
+        const int r = r0 + threadIdx.x, k = threadIdx.x;
+        x.zmax[((size_t)(q.node0 + r / G) * a.n_heads + h * G + r % G) * x.nsplit + split] = max(max(s_mx[0][k], s_mx[1][k]), max(s_mx[2][k], s_mx[3][k]));
+    }
+}
+
+// waves: HD / 32; one page a step
+template <int EPL, int RT>
+__global__ __launch_bounds__(EPL * 128, 2) void k_tree_xsum(sp_hipkv_tree_args a, XWork x, int groups) {
+    constexpr int HD = EPL * 64, NT = EPL * 128, ROWS = RT * 16, WROW = PAGE + 16;
+    constexpr int QUADS = (ROWS * 16 + NT - 1) / NT;                           // position quads of a thread and step
+    __shared__ __align__(16) int8_t wd[2][3][ROWS][WROW];                      // weights' digits [step parity][place][row][position]
+    __shared__ int s_M[ROWS];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), l16 = lane & 15, g = lane >> 4;
+    const int G = a.n_heads / a.n_kv_heads;
+    int id = blockIdx.x;
+    const int h = id % a.n_kv_heads; id /= a.n_kv_heads;
+    const int grp = id % groups; id /= groups;
+    const int split = id % x.vsplit;
+    const TreeSeq q = tree_seq(a, id / x.vsplit);
+    const int R = q.nodes * G, r0 = grp * ROWS;
+    if (r0 >= R) return;
+    const int end = q.cached + q.nodes, z0 = z_first(a, q);
+    const Span sp = rows_span(a, q, G, r0, min(r0 + ROWS, R));
+    const int per = (sp.pg1 - sp.pg0 + x.vsplit - 1) / x.vsplit, b0 = sp.pg0 + split * per, b1 = min(b0 + per, sp.pg1);
+    for (int k = threadIdx.x; k < ROWS; k += NT) {
+        int M = INT32_MIN;
+        if (r0 + k < R) {
+            const int32_t *m = x.zmax + ((size_t)(q.node0 + (r0 + k) / G) * a.n_heads + h * G + (r0 + k) % G) * x.nsplit;
+            for (int c = 0; c < x.nsplit; c++) M = max(M, m[c]);
+        }
+        s_M[k] = M;
+    }
+    __syncthreads();
+    // this thread's weights: positions 4 (tid % 16) .. of rows tid / 16 + k NT / 16
+    const int quad = threadIdx.x & 15;
+    int64_t den[QUADS];
+    int zrow[QUADS], M[QUADS], node[QUADS];
+    #pragma unroll
+    for (int k = 0; k < QUADS; k++) {
+        const int rl = threadIdx.x / 16 + k * (NT / 16), r = r0 + rl;
+        den[k] = 0;
+        const bool live = rl < ROWS && r < R && s_M[rl < ROWS ? rl : 0] > INT32_MIN;   // (no position seen: weights stay 0)
+        node[k] = live ? r / G : -1;
+        zrow[k] = live ? (q.node0 + r / G) * a.n_heads + h * G + r % G : 0;
+        M[k] = s_M[rl < ROWS ? rl : 0];
+    }
+    int4 z[QUADS];
+    auto load_z = [&](int lp) {
+        #pragma unroll
+        for (int k = 0; k < QUADS; k++)
+            if (node[k] >= 0) z[k] = *(const int4 *)(x.z + (size_t)zrow[k] * x.zstride + (lp * PAGE - z0 + 4 * quad));
+    };
+    auto weights = [&](int lp, int par) {
+        const int p0 = lp * PAGE;
+        const bool whole = p0 >= sp.lo_max && p0 + PAGE <= q.cached;
+        #pragma unroll
+        for (int k = 0; k < QUADS; k++) {
+            if ((int)threadIdx.x / 16 + k * (NT / 16) >= ROWS) break;
+            int32_t w[4] = {0, 0, 0, 0};
+            if (node[k] >= 0) {
+                const int32_t zz[4] = {z[k].x, z[k].y, z[k].z, z[k].w};
+                #pragma unroll
+                for (int e = 0; e < 4; e++)
+                    if (whole || row_sees(a, q, node[k], p0 + 4 * quad + e)) w[e] = weight_of(zz[e], M[k]);
+            }
+            den[k] += (int64_t)w[0] + w[1] + w[2] + w[3];
+            uint32_t d[4];
+            digits_of(w, d);
+            #pragma unroll
+            for (int b = 0; b < 3; b++) *(uint32_t *)&wd[par][b][threadIdx.x / 16 + k * (NT / 16)][4 * quad] = d[b];
+        }
+    };
+    const uint32_t vslice = (uint32_t)(a.n_kv_heads + h) * PAGE * HD * 4;
+    typedef int v2i __attribute__((ext_vector_type(2)));
+    v2i V[16];
+    // lane: positions 16 g + j of columns 32 wave + 2 l16, + 1
+    auto load_v = [&](const uint8_t *pg, int lp) {
+        const uint32_t col = vslice + (32 * wave + 2 * l16) * 4;
+        #pragma unroll
+        for (int j = 0; j < 16; j++) {
+            const int p = lp * PAGE + 16 * g + j;
+            V[j] = *gmem((const v2i *)(pg + col + (uint32_t)((p < end ? p : end - 1) & (PAGE - 1)) * (HD * 4)));
+        }
+    };
+    v4i acc[RT][2][5];
+    #pragma unroll
+    for (int t = 0; t < RT; t++)
+        #pragma unroll
+        for (int c = 0; c < 2; c++)
+            #pragma unroll
+            for (int k = 0; k < 5; k++) acc[t][c][k] = (v4i){0, 0, 0, 0};
+    auto page = [&](int lp) { return uniform(tree_page(a, q, lp * PAGE)); };
+    if (b0 < b1) { load_z(b0); load_v(page(b0), b0); }
+    for (int lp = b0; lp < b1; lp++) {
+        const int par = (lp - b0) & 1, nx = min(lp + 1, b1 - 1);
+        const uint8_t *pn = page(nx);
+        weights(lp, par);
+        load_z(nx);
+        __syncthreads();                                                   // (the other parity's readers are past it too)
+        // |v| may exceed three digits by little: what is left goes through once more
+        for (bool more = true; more;) {
+            v4i B[2][3];
+            int left = 0;
+            #pragma unroll
+            for (int c = 0; c < 2; c++)
+                #pragma unroll
+                for (int j = 0; j < 4; j++) {
+                    int32_t v[4];
+                    uint32_t d[4];
+                    #pragma unroll
+                    for (int e = 0; e < 4; e++) {
+                        v[e] = min(max(V[4 * j + e][c], -DIG3), DIG3);
+                        V[4 * j + e][c] -= v[e];
+                        left |= V[4 * j + e][c];
+                    }
+                    digits_of(v, d);
+                    #pragma unroll
+                    for (int b = 0; b < 3; b++) B[c][b][j] = (int)d[b];
+                }
+            more = __any(left != 0);
+            if (!more) {
+                __builtin_amdgcn_sched_barrier(0);
+                load_v(pn, nx);
+                __builtin_amdgcn_sched_barrier(0);
+            }
+            #pragma unroll
+            for (int t = 0; t < RT; t++)
+                #pragma unroll
+                for (int u = 0; u < 3; u++) {
+                    const v4i A = *(const v4i *)&wd[par][u][t * 16 + l16][16 * g];
+                    #pragma unroll
+                    for (int b = 0; b < 3; b++)
+                        #pragma unroll
+                        for (int c = 0; c < 2; c++) acc[t][c][u + b] = __builtin_amdgcn_mfma_i32_16x16x64_i8(A, B[c][b], acc[t][c][u + b], 0, 0, 0);
+                }
+        }
+    }
+    // denominators: over a row's 16 threads
+    #pragma unroll
+    for (int k = 0; k < QUADS; k++) {
+        #pragma unroll
+        for (int o = 1; o < 16; o <<= 1) den[k] += __shfl_xor(den[k], o, 64);
+        const int rl = threadIdx.x / 16 + k * (NT / 16), r = r0 + rl;
+        if (rl < ROWS && quad == 0 && r < R) x.den[((size_t)(q.node0 + r / G) * a.n_heads + h * G + r % G) * x.vsplit + split] = den[k];
+    }
+    #pragma unroll
+    for (int t = 0; t < RT; t++)
+        #pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const int r = r0 + t * 16 + 4 * g + i;
+            int64_t s[2];
+            #pragma unroll
+            for (int c = 0; c < 2; c++) {
+                s[c] = acc[t][c][4][i];
+                #pragma unroll
+                for (int k = 3; k >= 0; k--) s[c] = s[c] * 256 + acc[t][c][k][i];
+            }
+            if (r < R) {
+                int64_t *dst = x.sum + (((size_t)(q.node0 + r / G) * a.n_heads + h * G + r % G) * x.vsplit + split) * HD + 32 * wave + 2 * l16;
+                dst[0] = s[0]; dst[1] = s[1];
+            }
+        }
+}
+
+// one output element per thread
+template <int HD>
+__global__ __launch_bounds__(256) void k_tree_xdiv(sp_hipkv_tree_args a, XWork x) {
+    const size_t row = (size_t)blockIdx.x * (256 / HD) + threadIdx.x / HD;
+    const int d = threadIdx.x % HD;
+    if (row >= (size_t)a.n_nodes * a.n_heads) return;
+    const int64_t *s = x.sum + row * x.vsplit * HD + d, *dn = x.den + row * x.vsplit;
+    int64_t t = 0, den = 0;
+    #pragma unroll 8
+    for (int k = 0; k < x.vsplit; k++) { t += s[(size_t)k * HD]; den += dn[k]; }
+    a.out[(row / a.n_heads) * a.out_stride + (row % a.n_heads) * HD + d] = den > 0 ? rne_div_to_float((i128)t, den, 16) : 0.0f;
+}
+
 // How a launch is cut: row tiles of a workgroup, workgroups along a sequence's rows,
 // splits of its positions.
 struct TreePlan { int rt, groups, nsplit; };
@@ -570,6 +914,7 @@ int tree_check(const char *who, const sp_hipkv_tree_args *a) {
     OP_NEED(a->max_positions >= 0 && a->max_positions <= (a->rows == SP_HIPKV_ROWS_EXACT ? 1 << 18 : 1 << 20),
             "max_positions outside [0, 2^20] (exact rows: 2^18)");
     OP_NEED(a->n_nodes <= (int64_t)a->n_seqs * a->max_nodes, "n_nodes is more than n_seqs times max_nodes");
+    OP_NEED((int64_t)a->n_nodes * a->n_heads <= 1 << 28, "more than 2^28 rows (n_nodes x n_heads)");
     OP_NEED(a->window >= 0 && a->ring_pages >= 0, "negative window or ring_pages");
     return 0;
 }
@@ -586,12 +931,6 @@ int tree_check_arrays(const char *who, const sp_hipkv_tree_args *a, size_t need)
     return 0;
 }
 
-void tree_exact(const sp_hipkv_tree_args &a, hipStream_t s) {
-    const dim3 grid(a.n_heads, a.max_nodes, a.n_seqs), wg(64 * TREE_WAVES);
-    if (a.head_dim == 256) hipLaunchKernelGGL(k_tree_exact<4>, grid, wg, 0, s, a);
-    else if (a.head_dim == 128) hipLaunchKernelGGL(k_tree_exact<2>, grid, wg, 0, s, a);
-    else hipLaunchKernelGGL(k_tree_exact<1>, grid, wg, 0, s, a);
-}
 int64_t tree_grid(const sp_hipkv_tree_args &a, const TreePlan &p) { return (int64_t)a.n_kv_heads * p.groups * p.nsplit * a.n_seqs; }
 
 template <int ROWS> void tree_float(const sp_hipkv_tree_args &a, hipStream_t s) {
@@ -610,6 +949,46 @@ template <int ROWS> void tree_float(const sp_hipkv_tree_args &a, hipStream_t s) 
     else hipLaunchKernelGGL(k_tree_merge<64>, mg, wg, 0, s, a, p.nsplit);
 }
 
+// Exact rows: both passes take up to 48 rows a workgroup; a V split's int32 sums hold
+// 2 x 3 x 2^14 a position (values that need a second round of digits), so at most 2^14 positions.
+struct XPlan { int rt, groups; XWork w; size_t bytes; };
+XPlan tree_xplan(const sp_hipkv_tree_args &a) {
+    XPlan p{};
+    const int tiles = std::max(1, (a.max_nodes * (a.n_heads / a.n_kv_heads) + 15) / 16);
+    const int most = a.head_dim == 64 ? 2 : 3;                   // row tiles whose sums a wave's registers hold
+    p.groups = (tiles + most - 1) / most;
+    p.rt = (tiles + p.groups - 1) / p.groups;
+    const int span = a.window ? (int)std::min<int64_t>(a.max_positions, (int64_t)a.window + a.max_nodes + PAGE) : a.max_positions;
+    const int64_t base = (int64_t)a.n_kv_heads * p.groups * std::max(a.n_seqs, 1), pages = std::max(1, (span + PAGE - 1) / PAGE + 1);
+    p.w.zstride = (int)pages * PAGE;
+    p.w.nsplit = (int)std::max<int64_t>(1, std::min<int64_t>({(512 + base - 1) / base, (pages + 1) / 2, 64}));
+    p.w.vsplit = (int)std::max<int64_t>((pages * PAGE + 16383) >> 14, p.w.nsplit);
+    const size_t rows = (size_t)a.n_nodes * a.n_heads;
+    auto up = [](size_t n) { return (n + 15) / 16 * 16; };
+    const size_t zb = up(rows * p.w.zstride * 4), mb = up(rows * p.w.nsplit * 4), sb = rows * p.w.vsplit * a.head_dim * 8;
+    uint8_t *at = (uint8_t *)a.work;
+    p.w.z = (int32_t *)at; p.w.zmax = (int32_t *)(at + zb); p.w.sum = (int64_t *)(at + zb + mb); p.w.den = (int64_t *)(at + zb + mb + sb);
+    p.bytes = zb + mb + sb + up(rows * p.w.vsplit * 8);
+    return p;
+}
+template <int EPL, int RT> void tree_xgo(const sp_hipkv_tree_args &a, const XPlan &p, hipStream_t s) {
+    const int64_t one = (int64_t)a.n_kv_heads * p.groups * a.n_seqs, rows = (int64_t)a.n_nodes * a.n_heads, per = 256 / (EPL * 64);
+    hipLaunchKernelGGL((k_tree_xscore<EPL, RT>), dim3((uint32_t)(one * p.w.nsplit)), dim3(256), 0, s, a, p.w, p.groups);
+    hipLaunchKernelGGL((k_tree_xsum<EPL, RT>), dim3((uint32_t)(one * p.w.vsplit)), dim3(EPL * 128), 0, s, a, p.w, p.groups);
+    hipLaunchKernelGGL(k_tree_xdiv<EPL * 64>, dim3((uint32_t)((rows + per - 1) / per)), dim3(256), 0, s, a, p.w);
+}
+template <int EPL> void tree_xgo(const sp_hipkv_tree_args &a, const XPlan &p, hipStream_t s) {
+    if (p.rt == 1) tree_xgo<EPL, 1>(a, p, s);
+    else if (EPL == 1 || p.rt == 2) tree_xgo<EPL, 2>(a, p, s);
+    else if constexpr (EPL > 1) tree_xgo<EPL, 3>(a, p, s);
+}
+void tree_exact(const sp_hipkv_tree_args &a, hipStream_t s) {
+    const XPlan p = tree_xplan(a);
+    if (a.head_dim == 256) tree_xgo<4>(a, p, s);
+    else if (a.head_dim == 128) tree_xgo<2>(a, p, s);
+    else tree_xgo<1>(a, p, s);
+}
+
 }  // namespace
 
 void launch_tree(const sp_hipkv_tree_args &a, hipStream_t s) {
@@ -626,7 +1005,14 @@ extern "C" int sp_hipkv_tree_attention_work(const sp_hipkv_tree_args *a, size_t 
     if (tree_check(who, a)) return 1;
     OP_NEED(bytes, "null bytes");
     *bytes = 0;
-    if (a->rows == SP_HIPKV_ROWS_EXACT) return 0;
+    if (a->rows == SP_HIPKV_ROWS_EXACT) {
+        sp_hipkv_tree_args b = *a;
+        b.work = nullptr;
+        const XPlan p = tree_xplan(b);
+        OP_NEED((int64_t)a->n_kv_heads * p.groups * a->n_seqs * p.w.vsplit <= 1 << 22, "too many sequences, heads and nodes for one launch");
+        *bytes = p.bytes;
+        return 0;
+    }
     const TreePlan p = tree_plan(*a);
     OP_NEED(tree_grid(*a, p) <= 1 << 23, "too many sequences, heads and nodes for one launch");
     if (p.nsplit > 1) *bytes = (size_t)a->n_nodes * a->n_heads * p.nsplit * (a->head_dim + 2) * 4;
