@@ -7,11 +7,13 @@
 //                      w_p = exp_fixed((z_p - M) 2^16) >> 8, out = RNE(sum w vq / (2^16 sum w)),
 // the decode attention's integers (kvd_attn.hip).
 //
-// f32 and Spinor rows run on the f32 matrix cores in one pass over K and V
-// (k_tree_float), exact rows on the int8 matrix cores in two (k_tree_xscore, _xsum).
+// f32 and Spinor rows run in one pass over K and V (k_tree_float), f32 rows on the bf16
+// matrix cores in exact pieces, Spinor rows on the f32 ones; exact rows on the int8 matrix
+// cores in two passes (k_tree_xscore, _xsum).
 #include "kvd_op.h"
 #include "kvd_exact.h"
 #include "kvd_vec.h"
+#include "kvd_pass.h"
 #include <algorithm>
 
 namespace kvd {
@@ -31,6 +33,15 @@ __device__ __forceinline__ TreeSeq tree_seq(const sp_hipkv_tree_args &a, int s) 
     q.table = gmem(a.tables)[s];
     return q;
 }
+// whether some sequence has the node, for this thread's share t, t + n, .. of the sequences
+__device__ __forceinline__ bool tree_has(const sp_hipkv_tree_args &a, int node, int t, int n) {
+    bool has = false;
+    for (int s = t; s < a.n_seqs; s += n) {
+        const TreeSeq q = tree_seq(a, s);
+        has |= node >= q.node0 && node - q.node0 < q.nodes;
+    }
+    return has;
+}
 __device__ __forceinline__ int tree_low(const sp_hipkv_tree_args &a, const TreeSeq &q, int node) {
     if (!a.window) return 0;
     const int lo = q.cached + min(max(a.depth[q.node0 + node], 0), 511) - a.window + 1;
@@ -49,17 +60,29 @@ __device__ __forceinline__ const uint8_t *uniform(const uint8_t *x) {
 // ---------------------------------------------------------------- f32 and Spinor rows
 // The q heads of a kv head share its K and V rows: the rows of one kv head are
 // r = node G + q head of the group, 16 to a matrix tile, RT tiles to a workgroup.
-// Its four waves take the 16-position quarters of the pages of a range (a split)
-// in turn, each with all RT tiles, a running maximum, sum and output of its own; they
-// meet in LDS at the end, the splits in k_tree_merge.
+// Its waves take the tiles of a range of pages (a split) in turn, each with all RT row
+// tiles, a running maximum, sum and output of its own; they meet in LDS at the end, the
+// splits in k_tree_merge.  K and V are read once for all nodes and q heads of a workgroup.
 //
-// K and V go from memory into the operands' registers directly, each byte once:
-//   scores, transposed:  S^T = K Q^T, v_mfma_f32_16x16x4_f32, K the A operand (position
-//     lane % 16, 4 consecutive dims of group lane / 16), Q the B operand, from LDS;
-//   then lane l holds row l % 16 and positions 4 (l / 16) + i, as the A operand of
-//     O += P V needs them; V is the B operand, a float4 of a row per lane.
-// Two register buffers alternate, so that a stage (8 KiB a wave) is on its way while
-// the one before is multiplied.  f32 products and sums throughout.
+// Scores are made transposed, S^T = K Q^T (K the A operand, Q the B operand, from LDS): a
+// lane then holds a row's scores of the positions that O += P V needs from it as its A
+// operand, so weights stay in registers between the two products.
+//
+// f32 rows (8 waves, 32 positions a tile).  The f32 matrix cores bound the first form of
+// this kernel: 16x16x4 takes 32 cycles, 154 TF, 223 us of the 322 that 64 nodes of 16
+// heads at 32k took (2 kv heads of 256 dims).  A product of two f32 as six products
+// of bf16 pieces (below) costs 2.7 times fewer cycles and errs by 2^-26 of it, less than
+// f32 accumulation does: 235 us.  What bounds it now is a sum, as variants with one part
+// taken out showed: forming the pieces (3 roundings and 2 subtractions for each element) a third, the
+// matrix products a third, the wait for memory and for the slowest wave the rest; in a
+// wave they hardly overlap, and the registers (O: 16 RT x HD f32 a wave) allow 2 waves
+// a SIMD.  Memory comes through LDS by direct loads: held in registers on
+// the way, a tile cost 64 more of them (250 us).
+//
+// Spinor rows (4 waves, 16 positions a tile) keep the f32 matrix cores: codes and
+// multipliers go from memory into registers, are multiplied out there, and are the
+// operands.  36 us for 16 nodes at 6k of 2 kv heads of 256 dims; the f32
+// products are 10 of these, the multiplying-out as many, the rest is fixed (as above).
 //
 // The running maximum only moves when a score exceeds it by 2^8 in the exponent (base
 // 2): weights stay below 2^8 and nothing is lost, and a tile needs one ballot instead of
@@ -70,19 +93,53 @@ __device__ __forceinline__ const uint8_t *uniform(const uint8_t *x) {
 // first and are then put off to a loop behind the main one, which adds positions one
 // by one (inside the main loop that path costs twice the output's registers).
 typedef float v4f __attribute__((ext_vector_type(4)));
-constexpr int TT = 16;                       // positions per tile: a quarter of a page
 constexpr float LOG2E_F = 1.44269504088896341f;
+constexpr int TREE_PAGES = 256;              // pages of a split at most
+constexpr int tree_waves(int rows) { return rows == SP_HIPKV_ROWS_SPINOR ? 4 : 8; }
 
 __device__ __forceinline__ bool finite1(float x) { return (__float_as_uint(x) & 0x7F800000u) != 0x7F800000u; }
 
+// Of an f32 its three bf16 pieces, which sum to it exactly: x = h + m + l, |m| <= 2^-9 |x|,
+// |l| <= 2^-18 |x| (magnitudes from 2^127 on round up to infinity and make NaN).
+typedef __bf16 bf8 __attribute__((ext_vector_type(8)));
+typedef __bf16 bf2 __attribute__((ext_vector_type(2)));
+typedef float v2f __attribute__((ext_vector_type(2)));
+typedef uint32_t v4u32 __attribute__((ext_vector_type(4)));
+struct Pieces { bf8 p[3]; };
+template <typename X> __device__ __forceinline__ Pieces pieces_of(X &&x) {                 // of x(0) .. x(7)
+    v4u32 w[3];
+    #pragma unroll
+    for (int k = 0; k < 4; k++) {
+        float a = x(2 * k), b = x(2 * k + 1);
+        #pragma unroll
+        for (int n = 0; n < 3; n++) {
+            const uint32_t u = __builtin_bit_cast(uint32_t, __builtin_convertvector((v2f){a, b}, bf2));
+            w[n][k] = u;
+            if (n < 2) { a -= __uint_as_float(u << 16); b -= __uint_as_float(u & 0xFFFF0000u); }
+        }
+    }
+    return {{__builtin_bit_cast(bf8, w[0]), __builtin_bit_cast(bf8, w[1]), __builtin_bit_cast(bf8, w[2])}};
+}
+// The products of a's pieces with b's that make up a b to 2^-26, smallest first
+__device__ constexpr int MUL_A[6] = {2, 1, 0, 1, 0, 0}, MUL_B[6] = {0, 1, 2, 0, 1, 0};
+__device__ __forceinline__ v4f mfma_piece(const Pieces &a, const Pieces &b, int n, v4f c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a.p[MUL_A[n]], b.p[MUL_B[n]], c, 0, 0, 0);
+}
+
 template <int ROWS, int EPL, int RT>
-__global__ __launch_bounds__(256, 2) void k_tree_float(sp_hipkv_tree_args a, int groups, int nsplit) {
+__global__ __launch_bounds__(64 * tree_waves(ROWS), 2) void k_tree_float(sp_hipkv_tree_args a, int groups, int nsplit, int pages) {
     constexpr int HD = EPL * 64, CPR = HD / 16, RB = row_bytes_of(ROWS, HD);
     constexpr bool SPN = ROWS == SP_HIPKV_ROWS_SPINOR;
-    constexpr int NST = !SPN && EPL == 4 ? 2 : 1, NB = 4 * EPL / NST;      // stages of K (and of V) per tile, float4s per stage
-    constexpr int LDS_F = RT * 16 * HD > 4 * 8 * HD ? RT * 16 * HD : 4 * 8 * HD;
-    __shared__ __align__(16) float lds[LDS_F];                             // q rows, then the waves' outputs
-    __shared__ float s_m[4][RT * 16], s_l[4][RT * 16];
+    constexpr int NS = SPN ? 1 : 2, TP = 16 * NS;                          // 16-position tiles a wave takes at a time
+    constexpr int NW = tree_waves(ROWS), NT = 64 * NW;
+    // q (f32; or [piece][row][dim] bf16) and the waves' rings, then the waves' outputs
+    constexpr int Q_B = RT * 16 * HD * (SPN ? 4 : 6), UNIT = 4096, OUT_B = NW * 16 * HD * 4;
+    constexpr int RING = SPN ? 0 : 152 * 1024 - Q_B >= 4 * NW * UNIT ? 4 : 3;
+    constexpr int LDS_B = Q_B + NW * RING * UNIT > OUT_B ? Q_B + NW * RING * UNIT : OUT_B;
+    __shared__ __align__(1024) uint8_t lds[LDS_B];
+    __shared__ float s_m[NW][RT * 16], s_l[NW][RT * 16], s_M[RT * 16], s_L[RT * 16];
+    __shared__ int s_node[RT * 16], s_low[RT * 16];
+    __shared__ const uint8_t *s_page[SPN ? 1 : TREE_PAGES];               // this split's
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), l16 = lane & 15, g = lane >> 4;
     const int G = a.n_heads / a.n_kv_heads;
     int id = blockIdx.x;
@@ -93,78 +150,94 @@ __global__ __launch_bounds__(256, 2) void k_tree_float(sp_hipkv_tree_args a, int
     const int R = q.nodes * G, r0 = grp * RT * 16;
     if (r0 >= R) return;
     const int end = q.cached + q.nodes;
-    // this lane's rows, one of each tile: where it starts to see, its mask
-    int low[RT], nodei[RT], lo_min = INT32_MAX, lo_max = 0;
+    // each row's node and where it starts to see (rows past the last repeat it)
+    int lo_min = INT32_MAX, lo_max = 0;
     #pragma unroll
     for (int t = 0; t < RT; t++) {
-        const int r = r0 + t * 16 + l16;
-        nodei[t] = (r < R ? r : R - 1) / G;
-        low[t] = tree_low(a, q, nodei[t]);
-        lo_min = min(lo_min, low[t]); lo_max = max(lo_max, low[t]);
+        const int r = r0 + t * 16 + l16, node = (r < R ? r : R - 1) / G, lo = tree_low(a, q, node);
+        lo_min = min(lo_min, lo); lo_max = max(lo_max, lo);
+        if (threadIdx.x < 16) { s_node[t * 16 + l16] = q.node0 + node; s_low[t * 16 + l16] = lo; }
     }
     if (a.window) {
         #pragma unroll
         for (int o = 1; o < 16; o <<= 1) { lo_min = min(lo_min, __shfl_xor(lo_min, o, 64)); lo_max = max(lo_max, __shfl_xor(lo_max, o, 64)); }
     }
     lo_min = __builtin_amdgcn_readfirstlane(lo_min); lo_max = __builtin_amdgcn_readfirstlane(lo_max);
-    // this split's pages, and this wave's of them
-    const int pg0 = lo_min / PAGE, pg1 = (end + PAGE - 1) / PAGE, per = (pg1 - pg0 + nsplit - 1) / nsplit;
-    int w0 = pg0 + split * per, w1 = min(w0 + per, pg1);
-    if (w0 < w1 && w0 * PAGE + wave * TT + TT <= lo_min) w0++;
-    if (w0 < w1 && (w1 - 1) * PAGE + wave * TT >= end) w1--;
-    v4f *qs = (v4f *)lds;
-    for (int i = threadIdx.x; i < RT * 16 * (HD / 4); i += 256) {
-        const int r = i / (HD / 4), c = i % (HD / 4), rr = r0 + r < R ? r0 + r : R - 1;
-        qs[r * (HD / 4) + (c ^ (r & 15))] = *(const v4f *)(a.q + (size_t)(q.node0 + rr / G) * a.q_stride + (size_t)(h * G + rr % G) * HD + 4 * c);
+    // this split's tiles with a position that is seen, and this wave's: w0, w0 + NW, .. below w1
+    // (a sequence shorter than the longest has proportionally fewer parts)
+    const int pg0 = lo_min / PAGE, np = (end + PAGE - 1) / PAGE - pg0;
+    const int parts = max((int)(((int64_t)np * nsplit + pages - 1) / pages), (np + TREE_PAGES - 1) / TREE_PAGES);
+    const int b0 = pg0 + (int)((int64_t)np * min(split, parts) / parts), b1 = pg0 + (int)((int64_t)np * min(split + 1, parts) / parts);
+    const int t0 = max(b0 * (PAGE / TP), lo_min / TP), w1 = min(b1 * (PAGE / TP), (end + TP - 1) / TP), w0 = t0 + wave;
+    auto row_q = [&](int r) {
+        const int rr = r0 + r < R ? r0 + r : R - 1;
+        return a.q + (size_t)(q.node0 + rr / G) * a.q_stride + (size_t)(h * G + rr % G) * HD;
+    };
+    // 16-byte pieces of a row in an order that spreads a column over the banks
+    if constexpr (SPN) {
+        for (int i = threadIdx.x; i < RT * 16 * (HD / 4); i += NT) {
+            const int r = i / (HD / 4), c = i % (HD / 4);
+            ((v4f *)lds)[r * (HD / 4) + (c ^ (r & 15))] = *(const v4f *)(row_q(r) + 4 * c);
+        }
+    } else {
+        for (int i = threadIdx.x; i < b1 - b0 && i < TREE_PAGES; i += NT) s_page[i] = tree_page(a, q, (b0 + i) * PAGE);
+        for (int i = threadIdx.x; i < RT * 16 * (HD / 8); i += NT) {
+            const int r = i / (HD / 8), c = i % (HD / 8);
+            const v4f x = *(const v4f *)(row_q(r) + 8 * c), y = *(const v4f *)(row_q(r) + 8 * c + 4);
+            const Pieces p = pieces_of([&](int k) { return k < 4 ? x[k] : y[k - 4]; });
+            #pragma unroll
+            for (int n = 0; n < 3; n++) ((bf8 *)lds)[(n * RT * 16 + r) * (HD / 8) + (c ^ (r & 7))] = p.p[n];
+        }
     }
-    v4f O[RT][CPR], S[RT];
+    v4f O[RT][CPR], S[RT][NS];
     float m[RT], l[RT];
-    uint32_t see[RT];
     #pragma unroll
     for (int t = 0; t < RT; t++) {
-        m[t] = -INFINITY; l[t] = 0.0f; see[t] = 15;
+        m[t] = -INFINITY; l[t] = 0.0f;
         #pragma unroll
         for (int c = 0; c < CPR; c++) O[t][c] = (v4f){0, 0, 0, 0};
     }
     __syncthreads();
     const uint32_t kslice = (uint32_t)h * PAGE * RB, vslice = (uint32_t)(a.n_kv_heads + h) * PAGE * RB;
     // page addresses are the wave's: rows load as address + 32-bit lane offset
-    auto page = [&](int lp) { return uniform(tree_page(a, q, lp * PAGE)); };
-    // positions past the last one repeat it
-    auto row_off = [&](int lp, int x) { const int p = lp * PAGE + wave * TT + x; return (uint32_t)((p < end ? p : end - 1) & (PAGE - 1)) * RB; };
-    // tiles that some row does not see whole, and those of them put off to the end:
-    // nodes span at most 9 pages, so do the rows' window starts
-    auto ragged = [&](int lp) { const int p0 = lp * PAGE + wave * TT; return p0 < lo_max || p0 + TT > q.cached; };
-    const int tail_pg = q.cached / PAGE;
-    uint32_t later = 0;
-    auto put_off = [&](int lp) { later |= lp >= tail_pg ? 1u << (lp - tail_pg) : 65536u << (lp - pg0); };
-    auto next_off = [&] {
-        const int b = __builtin_ctz(later);
-        later &= later - 1;
-        return b < 16 ? tail_pg + b : pg0 + b - 16;
+    auto page = [&](int tile) { return uniform(tree_page(a, q, tile * TP)); };
+    // tiles that some row does not see whole, and those of them with a V value that is
+    // not finite: nodes span at most 10 pages, so do the rows' window starts
+    auto ragged = [&](int tile) { return tile * TP < lo_max || tile * TP + TP > q.cached; };
+    const int tail = q.cached / TP, head = lo_min / TP;
+    uint64_t later = 0;
+    auto put_off = [&](int tile) { later |= tile >= tail ? 1ull << (tile - tail) : 1ull << (32 + tile - head); };
+    // whether this lane's row of tile t sees positions p0 + 4 g + i, as bits
+    auto seen4 = [&](int t, int p0) {
+        uint32_t see = 0;
+        const int lo = s_low[t * 16 + l16];
+        const uint64_t *mask = a.visible + (size_t)s_node[t * 16 + l16] * a.mask_words;
+        #pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const int p = p0 + 4 * g + i, j = p - q.cached;
+            bool v = p >= lo;
+            if (j >= 0) v = j < q.nodes && (gmem(mask)[j >> 6] >> (j & 63) & 1);
+            see |= (uint32_t)v << i;
+        }
+        return see;
     };
     // scores in base 2, masked; weights into S
-    auto softmax = [&](int lp) {
-        const int p0 = lp * PAGE + wave * TT;
-        const bool whole = !ragged(lp);
+    auto softmax = [&](int tile, bool rag) {
         #pragma unroll
         for (int t = 0; t < RT; t++) {
             float mx = -INFINITY;
             #pragma unroll
-            for (int i = 0; i < 4; i++) S[t][i] *= a.scale * LOG2E_F;
-            if (!whole) {
-                see[t] = 0;
+            for (int u = 0; u < NS; u++) {
                 #pragma unroll
-                for (int i = 0; i < 4; i++) {
-                    const int p = p0 + 4 * g + i, j = p - q.cached;
-                    bool v = p >= low[t];
-                    if (j >= 0) v = j < q.nodes && (gmem(a.visible)[(size_t)(q.node0 + nodei[t]) * a.mask_words + (j >> 6)] >> (j & 63) & 1);
-                    see[t] |= (uint32_t)v << i;
-                    S[t][i] = v ? S[t][i] : -INFINITY;
+                for (int i = 0; i < 4; i++) S[t][u][i] *= a.scale * LOG2E_F;
+                if (rag) {
+                    const uint32_t see = seen4(t, tile * TP + 16 * u);
+                    #pragma unroll
+                    for (int i = 0; i < 4; i++) S[t][u][i] = see >> i & 1 ? S[t][u][i] : -INFINITY;
                 }
+                #pragma unroll
+                for (int i = 0; i < 4; i++) mx = fmaxf(mx, S[t][u][i]);
             }
-            #pragma unroll
-            for (int i = 0; i < 4; i++) mx = fmaxf(mx, S[t][i]);
             if (__any(mx > m[t] + 8.0f)) {
                 mx = fmaxf(mx, __shfl_xor(mx, 16, 64));
                 mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
@@ -180,162 +253,195 @@ __global__ __launch_bounds__(256, 2) void k_tree_float(sp_hipkv_tree_args a, int
             }
             const float ms = m[t] == -INFINITY ? 0.0f : m[t];
             #pragma unroll
-            for (int i = 0; i < 4; i++) { S[t][i] = __builtin_amdgcn_exp2f(S[t][i] - ms); l[t] += S[t][i]; }
+            for (int u = 0; u < NS; u++)
+                #pragma unroll
+                for (int i = 0; i < 4; i++) { S[t][u][i] = __builtin_amdgcn_exp2f(S[t][u][i] - ms); l[t] += S[t][u][i]; }
         }
     };
-    // O[t][c0 + c] += P x(e, c), positions 4 g + e, N columns
-    auto pv = [&](auto n, int c0, auto &&x) {
-        constexpr int N = decltype(n)::value;
-        #pragma unroll
-        for (int e = 0; e < 4; e++) {
-            #pragma unroll
-            for (int c = 0; c < N; c++) {
-                const float v = x(e, c);
+    // V values that are not finite, for the rows that see them; x4(page, row offset, k): columns 4 k .. of this lane
+    auto add_later = [&](auto &&x4) {
+        while (later) {
+            const int b = __builtin_ctzll(later), tile = b < 32 ? tail + b : head + b - 32;
+            later &= later - 1;
+            const uint8_t *pg = page(tile);
+            for (int p = tile * TP; p < tile * TP + TP && p < end; p++) {
                 #pragma unroll
-                for (int t = 0; t < RT; t++) O[t][c0 + c] = __builtin_amdgcn_mfma_f32_16x16x4f32(S[t][e], v, O[t][c0 + c], 0, 0, 0);
-                if (SPN && c % 4 == 3) __builtin_amdgcn_sched_barrier(0);
-            }
-            __builtin_amdgcn_sched_barrier(0);
-        }
-    };
-    // the same position by position, for the rows that see it; x4(p, k): columns 4 k .. of this lane
-    auto pv_slow = [&](int lp, auto &&x4) {
-        for (int p = 0; p < TT && lp * PAGE + wave * TT + p < end; p++) {
-            const int from = (p >> 2) * 16, pe = p & 3;
-            #pragma unroll
-            for (int t = 0; t < RT; t++) {
-                const float we = pe == 0 ? S[t][0] : pe == 1 ? S[t][1] : pe == 2 ? S[t][2] : S[t][3];
-                float w[4];
-                bool on[4];
-                #pragma unroll
-                for (int i = 0; i < 4; i++) {
-                    w[i] = __shfl(we, from + 4 * g + i, 64);
-                    on[i] = __shfl(see[t], from + 4 * g + i, 64) >> pe & 1;
-                }
-                #pragma unroll
-                for (int k = 0; k < CPR / 4; k++) {
-                    const v4f v = x4(p, k);
+                for (int t = 0; t < RT; t++) {
+                    bool on[4];
                     #pragma unroll
-                    for (int c = 0; c < 4; c++)
+                    for (int i = 0; i < 4; i++) {
+                        const int k = t * 16 + 4 * g + i, j = p - q.cached;
+                        on[i] = j < 0 ? p >= s_low[k] : (gmem(a.visible)[(size_t)s_node[k] * a.mask_words + (j >> 6)] >> (j & 63) & 1);
+                    }
+                    #pragma unroll
+                    for (int k = 0; k < CPR / 4; k++) {
+                        const v4f v = x4(pg + vslice + (uint32_t)(p & (PAGE - 1)) * RB, k);
                         #pragma unroll
-                        for (int i = 0; i < 4; i++) O[t][4 * k + c][i] = on[i] ? O[t][4 * k + c][i] + w[i] * v[c] : O[t][4 * k + c][i];
-                    __builtin_amdgcn_sched_barrier(0);
+                        for (int c = 0; c < 4; c++)
+                            #pragma unroll
+                            for (int i = 0; i < 4; i++) O[t][4 * k + c][i] += on[i] && !finite1(v[c]) ? v[c] : 0.0f;
+                        __builtin_amdgcn_sched_barrier(0);
+                    }
                 }
             }
         }
     };
     auto zero_s = [&] {
         #pragma unroll
-        for (int t = 0; t < RT; t++) S[t] = (v4f){0, 0, 0, 0};
+        for (int t = 0; t < RT; t++)
+            #pragma unroll
+            for (int u = 0; u < NS; u++) S[t][u] = (v4f){0, 0, 0, 0};
     };
     if constexpr (!SPN) {
-        // column of O[t][c], row 4 g + i: 64 (c / 4) + 4 l16 + c % 4
-        auto load_k = [&](v4f (&x)[NB], const uint8_t *pg, int lp, int st) {
-            const uint32_t off = kslice + row_off(lp, l16) + 16 * g + st * NB * 64;
+        // A tile's memory comes in units of 32 rows x 128 bytes, straight into a ring of the
+        // wave's own in LDS (no registers, no barrier: the wave waits for its own loads):
+        // K steps of 32 dims, then V as 32 columns.  16-byte piece c of a row lies at place
+        // c ^ (slot % 8) of its slot; rows are in order for K, by (row % 4, row / 4) for V,
+        // which is how the operands' reads meet no bank twice.
+        constexpr int NK = HD / 32, NU = 2 * NK;
+        const uint32_t ring = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t *)(lds + Q_B + wave * RING * UNIT);
+        const uint8_t *ringp = lds + Q_B + wave * RING * UNIT;
+        const int rj = lane >> 3, vo_k = rj * RB + ((lane & 7) ^ rj) * 16, vo_v = (16 * (rj >> 2) + 4 * (rj & 3)) * RB + ((lane & 7) ^ rj) * 16;
+        auto page_at = [&](int tile) { return uniform(s_page[tile / (PAGE / TP) - b0]); };
+        auto load = [&](const uint8_t *pg, int tile, int n, uint32_t slot) {
+            const int row = tile * TP & (PAGE - 1);
+            const bool v = n >= NK;
+            const v4i rs = rsrc_of(pg + (v ? vslice : kslice) + row * RB + (n - (v ? NK : 0)) * 128, (TP - 1) * RB + 128);
             #pragma unroll
-            for (int s = 0; s < NB; s++) x[s] = *gmem((const v4f *)(pg + off + 64 * s));
+            for (int k = 0; k < 4; k++) dma16(ring + slot * UNIT + k * 1024, v ? vo_v : vo_k, rs, (v ? k : 8 * k) * RB);
         };
-        auto load_v = [&](v4f (&x)[NB], const uint8_t *pg, int lp, int st) {
-            #pragma unroll
-            for (int e = 0; e < 4; e++) {
-                const uint32_t off = vslice + row_off(lp, 4 * g + e) + 16 * l16 + st * NB * 64;
+        int kb[2];
+        #pragma unroll
+        for (int e = 0; e < 2; e++) kb[e] = l16 * (HD / 8) + ((4 * e + g) ^ (l16 & 7));
+        const bf8 *qs = (const bf8 *)lds;
+        // this lane's places in a unit: K piece 2 g (and ^ 1) of row l16 (+ 16), V columns 2 l16, + 1 of row 4 g + e (slot 8 e + g)
+        const int kp = l16 * 128 + ((2 * g) ^ (l16 & 7)) * 16;
+        int vp[2];
+        #pragma unroll
+        for (int u = 0; u < 2; u++) vp[u] = (4 * u + g) * 128 + (((l16 >> 1) ^ (4 * u + g)) * 16) + 8 * (l16 & 1);
+        // Unit n is read from the ring into x while unit n - 1 is multiplied, q's pieces while
+        // the operand's are formed.
+        uint32_t slot = 0;                                                 // of the unit after the one in x
+        float x[16];
+        auto arrive = [&] { asm volatile("s_waitcnt vmcnt(%0)" : : "n"(4 * (RING - 1)) : "memory"); };
+        auto read = [&](int n) {
+            const uint8_t *un = ringp + slot * UNIT;
+            if (n < NK) {
                 #pragma unroll
-                for (int u = 0; u < NB / 4; u++) x[e * (NB / 4) + u] = *gmem((const v4f *)(pg + off + 256 * u));
+                for (int u = 0; u < 2; u++) {
+                    *(v4f *)(x + 8 * u) = *(const v4f *)(un + kp + 2048 * u);
+                    *(v4f *)(x + 8 * u + 4) = *(const v4f *)(un + (kp ^ 16) + 2048 * u);
+                }
+            } else {
+                #pragma unroll
+                for (int k = 0; k < 8; k++) *(v2f *)(x + 2 * k) = *(const v2f *)(un + vp[k >> 2] + 1024 * (k & 3));
             }
+            __builtin_amdgcn_sched_barrier(0);
         };
-        auto scores = [&](const v4f (&x)[NB], int st) {
-            #pragma unroll
-            for (int s = 0; s < NB; s++) {
-                v4f qv[RT];
-                #pragma unroll
-                for (int t = 0; t < RT; t++) qv[t] = qs[(t * 16 + l16) * (HD / 4) + ((4 * (st * NB + s) + g) ^ l16)];
-                #pragma unroll
-                for (int e = 0; e < 4; e++)
-                    #pragma unroll
-                    for (int t = 0; t < RT; t++) S[t] = __builtin_amdgcn_mfma_f32_16x16x4f32(x[s][e], qv[t][e], S[t], 0, 0, 0);
-                if (s % 2) __builtin_amdgcn_sched_barrier(0);              // few q reads ahead at a time
-            }
-        };
-        auto values = [&](const v4f (&x)[NB], int st) {
-            pv(std::integral_constant<int, NB>{}, st * NB, [&](int e, int c) { return x[e * (NB / 4) + c / 4][c % 4]; });
-        };
-        v4f A[NB], B[NB];
         const uint8_t *pg = nullptr, *pn = nullptr;
         if (w0 < w1) {
-            pg = page(w0);
-            load_k(A, pg, w0, 0);
-            if (NST == 2) load_k(B, pg, w0, 1); else load_v(B, pg, w0, 0);
-            pn = page(min(w0 + 1, w1 - 1));
+            pg = page_at(w0);
+            #pragma unroll
+            for (int n = 0; n < RING; n++) load(pg, w0, n, n);
+            arrive();
+            read(0);
         }
-        for (int lp = w0; lp < w1; lp++) {
-            const int nx = min(lp + 1, w1 - 1);
+        for (int tile = w0; tile < w1; tile += NW) {
+            const int nx = tile + NW < w1 ? tile + NW : tile;
+            const bool rag = ragged(tile);
+            pn = page_at(nx);
+            // x is read: unit n's slot takes the unit RING later
+            auto refill = [&](int n) {
+                asm volatile("s_waitcnt lgkmcnt(0)" : : : "memory");
+                if (n + RING < NU) load(pg, tile, n + RING, slot); else load(pn, nx, n + RING - NU, slot);
+                slot = slot == RING - 1 ? 0 : slot + 1;
+            };
             zero_s();
-            scores(A, 0);
-            __builtin_amdgcn_sched_barrier(0);
-            if constexpr (NST == 2) {
-                load_v(A, pg, lp, 0);
-                __builtin_amdgcn_sched_barrier(0);
-                scores(B, 1);
-                __builtin_amdgcn_sched_barrier(0);
-                load_v(B, pg, lp, 1);
-            } else {
-                load_k(A, pn, nx, 0);
-            }
-            __builtin_amdgcn_sched_barrier(0);
-            bool bad = false;
-            if (ragged(lp)) {
-                #pragma unroll
-                for (int s = 0; s < NB; s++)
+            #pragma unroll
+            for (int n = 0; n < NK; n++) {
+                Pieces K[2], Q[2];
+                auto load_q = [&](int t) {
                     #pragma unroll
-                    for (int e = 0; e < 4; e++) bad |= !finite1(B[s][e]) || (NST == 2 && !finite1(A[s][e]));
+                    for (int k = 0; k < 3; k++) Q[t & 1].p[k] = qs[kb[n & 1] + (k * RT + t) * 2 * HD + 8 * (n >> 1)];
+                    __builtin_amdgcn_sched_barrier(0);
+                };
+                load_q(0);
+                #pragma unroll
+                for (int u = 0; u < 2; u++) K[u] = pieces_of([&](int k) { return x[8 * u + k]; });
+                refill(n);
+                #pragma unroll
+                for (int t = 0; t < RT; t++) {
+                    if (t + 1 < RT) load_q(t + 1);
+                    #pragma unroll
+                    for (int k = 0; k < 6; k++)
+                        #pragma unroll
+                        for (int u = 0; u < 2; u++) S[t][u] = mfma_piece(K[u], Q[t & 1], k, S[t][u]);
+                    if (t == 0) { arrive(); read(n + 1); }
+                }
             }
-            bad = __any(bad);
-            if (bad) put_off(lp); else softmax(lp);
-            if constexpr (NST == 2) {
-                if (!bad) values(A, 0);
-                __builtin_amdgcn_sched_barrier(0);
-                load_k(A, pn, nx, 0);
-                __builtin_amdgcn_sched_barrier(0);
-                if (!bad) values(B, 1);
-                __builtin_amdgcn_sched_barrier(0);
-                load_k(B, pn, nx, 1);
-            } else {
-                if (!bad) values(B, 0);
-                __builtin_amdgcn_sched_barrier(0);
-                load_v(B, pn, nx, 0);
+            softmax(tile, rag);
+            Pieces P[RT];
+            #pragma unroll
+            for (int t = 0; t < RT; t++) P[t] = pieces_of([&](int k) { return S[t][k >> 2][k & 3]; });
+            uint32_t bad = 0;                                              // largest exponent field of a row before the end
+            #pragma unroll
+            for (int n = NK; n < NU; n++) {
+                if (rag) {
+                    #pragma unroll
+                    for (int k = 0; k < 16; k++) {
+                        const uint32_t f = __float_as_uint(x[k]) & 0x7F800000u;
+                        bad = max(bad, tile * TP + 16 * (k >> 3) + 4 * g + (k >> 1 & 3) < end ? f : 0u);
+                        x[k] = f == 0x7F800000u ? 0.0f : x[k];
+                        if (k % 4 == 3) __builtin_amdgcn_sched_barrier(0);
+                    }
+                }
+                Pieces V[2];
+                #pragma unroll
+                for (int c = 0; c < 2; c++) V[c] = pieces_of([&](int k) { return x[2 * k + c]; });
+                refill(n);
+                #pragma unroll
+                for (int t = 0; t < RT; t++) {
+                    #pragma unroll
+                    for (int k = 0; k < 6; k++)
+                        #pragma unroll
+                        for (int c = 0; c < 2; c++) O[t][2 * (n - NK) + c] = mfma_piece(P[t], V[c], k, O[t][2 * (n - NK) + c]);
+                    if (t == 0) { arrive(); read(n + 1 < NU ? n + 1 : 0); }
+                }
             }
+            if (__any(bad == 0x7F800000u)) put_off(tile);
             pg = pn;
-            pn = page(min(lp + 2, w1 - 1));
-            __builtin_amdgcn_sched_barrier(0);
         }
-        while (later) {
-            const int lp = next_off();
-            pg = page(lp);
-            zero_s();
-            for (int st = 0; st < NST; st++) { load_k(A, pg, lp, st); scores(A, st); }
-            softmax(lp);
-            pv_slow(lp, [&](int p, int k) { return *gmem((const v4f *)(pg + vslice + row_off(lp, p) + 16 * l16 + 256 * k)); });
-        }
+        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" : : : "memory");                 // nothing lands in LDS after this
+        add_later([&](const uint8_t *row, int k) {
+            const v2f x = *gmem((const v2f *)(row + 8 * l16 + 256 * k)), y = *gmem((const v2f *)(row + 8 * l16 + 256 * k + 128));
+            return (v4f){x[0], x[1], y[0], y[1]};
+        });
     } else {
         // K: 16 codes of dims 64 i + 16 g.. a load; V: the CPR codes of columns CPR l16..
         // (O[t][c] is column CPR l16 + c), and the multipliers of the at most two
         // chunks that they lie in
         constexpr int NM = spn_blocks(HD);
+        const v4f *qs = (const v4f *)lds;
+        int kb[4];
+        #pragma unroll
+        for (int e = 0; e < 4; e++) kb[e] = l16 * (HD / 4) + ((4 * g + e) ^ l16);
+        // positions past the last one repeat it
+        auto row_off = [&](int tile, int x) { const int p = tile * TP + x; return (uint32_t)((p < end ? p : end - 1) & (PAGE - 1)) * RB; };
         struct KRow { uint4 c[EPL]; float m[NM]; };
         struct VRow { uint32_t c[EPL]; float m0, m1; };
         const int d0v = CPR * l16, b0v = spn_block_of(HD, d0v), bnd0 = spn_block_start(HD, b0v + 1), b1v = bnd0 < d0v + CPR ? b0v + 1 : b0v;
         int bndv = bnd0;
-        auto load_k = [&](KRow &x, const uint8_t *pg, int lp) {
-            const uint8_t *row = pg + kslice + row_off(lp, l16);
+        auto load_k = [&](KRow &x, const uint8_t *pg, int tile) {
+            const uint8_t *row = pg + kslice + row_off(tile, l16);
             #pragma unroll
             for (int i = 0; i < EPL; i++) x.c[i] = *gmem((const uint4 *)(row + 64 * i + 16 * g));
             #pragma unroll
             for (int b = 0; b < NM; b++) x.m[b] = *gmem((const float *)(row + HD + 4 * b));
         };
-        auto load_v = [&](VRow (&x)[4], const uint8_t *pg, int lp) {
+        auto load_v = [&](VRow (&x)[4], const uint8_t *pg, int tile) {
             #pragma unroll
             for (int e = 0; e < 4; e++) {
-                const uint8_t *row = pg + vslice + row_off(lp, 4 * g + e);
+                const uint8_t *row = pg + vslice + row_off(tile, 4 * g + e);
                 #pragma unroll
                 for (int i = 0; i < EPL; i++) x[e].c[i] = *gmem((const uint32_t *)(row + d0v + 4 * i));
                 x[e].m0 = *gmem((const float *)(row + HD + 4 * b0v));
@@ -343,31 +449,6 @@ __global__ __launch_bounds__(256, 2) void k_tree_float(sp_hipkv_tree_args a, int
             }
         };
         auto code = [](uint32_t w, int t) { return (float)(int32_t)(int8_t)(w >> (8 * t)); };
-        auto scores = [&](const KRow &x) {
-            #pragma unroll
-            for (int i = 0; i < EPL; i++) {
-                const int d0 = 64 * i + 16 * g, b = spn_block_of(HD, d0);
-                int bnd = spn_block_start(HD, b + 1);
-                asm volatile("" : "+v"(bnd));                              // compared where used: kept masks would fill the scalar registers
-                float m0 = x.m[0], m1 = x.m[0];
-                #pragma unroll
-                for (int bb = 1; bb < NM; bb++) { if (b == bb) m0 = x.m[bb]; if (b + 1 == bb) m1 = x.m[bb]; }
-                const uint32_t w[4] = {x.c[i].x, x.c[i].y, x.c[i].z, x.c[i].w};
-                #pragma unroll
-                for (int k = 0; k < 4; k++) {
-                    v4f qv[RT];
-                    #pragma unroll
-                    for (int t = 0; t < RT; t++) qv[t] = qs[(t * 16 + l16) * (HD / 4) + ((16 * i + 4 * g + k) ^ l16)];
-                    #pragma unroll
-                    for (int e = 0; e < 4; e++) {
-                        const float kv = code(w[k], e) * (d0 + 4 * k + e < bnd ? m0 : m1);
-                        #pragma unroll
-                        for (int t = 0; t < RT; t++) S[t] = __builtin_amdgcn_mfma_f32_16x16x4f32(kv, qv[t][e], S[t], 0, 0, 0);
-                    }
-                    if (k % 2) __builtin_amdgcn_sched_barrier(0);
-                }
-            }
-        };
         KRow K;
         VRow V[4];
         const uint8_t *pg = nullptr, *pn = nullptr;
@@ -375,52 +456,76 @@ __global__ __launch_bounds__(256, 2) void k_tree_float(sp_hipkv_tree_args a, int
             pg = page(w0);
             load_k(K, pg, w0);
             load_v(V, pg, w0);
-            pn = page(min(w0 + 1, w1 - 1));
+            pn = page(w0 + NW < w1 ? w0 + NW : w0);
         }
-        for (int lp = w0; lp < w1; lp++) {
-            const int nx = min(lp + 1, w1 - 1);
+        for (int tile = w0; tile < w1; tile += NW) {
+            const int nx = tile + NW < w1 ? tile + NW : tile;
+            const bool rag = ragged(tile);
             zero_s();
-            scores(K);
+            #pragma unroll
+            for (int i = 0; i < EPL; i++) {
+                const int d0 = 64 * i + 16 * g, b = spn_block_of(HD, d0);
+                int bnd = spn_block_start(HD, b + 1);
+                asm volatile("" : "+v"(bnd));                              // compared where used: kept masks would fill the scalar registers
+                float m0 = K.m[0], m1 = K.m[0];
+                #pragma unroll
+                for (int bb = 1; bb < NM; bb++) { if (b == bb) m0 = K.m[bb]; if (b + 1 == bb) m1 = K.m[bb]; }
+                const uint32_t w[4] = {K.c[i].x, K.c[i].y, K.c[i].z, K.c[i].w};
+                #pragma unroll
+                for (int k = 0; k < 4; k++) {
+                    v4f qv[RT];
+                    #pragma unroll
+                    for (int t = 0; t < RT; t++) qv[t] = qs[kb[k] + t * 4 * HD + 16 * i];
+                    float kv[4];
+                    #pragma unroll
+                    for (int e = 0; e < 4; e++) kv[e] = code(w[k], e) * (d0 + 4 * k + e < bnd ? m0 : m1);
+                    #pragma unroll
+                    for (int e = 0; e < 4; e++)
+                        #pragma unroll
+                        for (int t = 0; t < RT; t++) S[t][0] = __builtin_amdgcn_mfma_f32_16x16x4f32(kv[e], qv[t][e], S[t][0], 0, 0, 0);
+                    if (k % 2) __builtin_amdgcn_sched_barrier(0);
+                }
+            }
             __builtin_amdgcn_sched_barrier(0);
             load_k(K, pn, nx);
             __builtin_amdgcn_sched_barrier(0);
-            bool bad = false;
-            if (ragged(lp)) {
+            softmax(tile, rag);
+            if (rag) {
+                bool bad = false;
                 #pragma unroll
-                for (int e = 0; e < 4; e++) bad |= !finite1(127.0f * V[e].m0) || !finite1(127.0f * V[e].m1);
+                for (int e = 0; e < 4; e++) {
+                    const bool f0 = finite1(127.0f * V[e].m0), f1 = finite1(127.0f * V[e].m1);
+                    bad |= !f0 || !f1;
+                    V[e].m0 = f0 ? V[e].m0 : 0.0f; V[e].m1 = f1 ? V[e].m1 : 0.0f;
+                }
+                if (__any(bad)) put_off(tile);
             }
-            if (__any(bad)) {
-                put_off(lp);
-            } else {
-                softmax(lp);
-                asm volatile("" : "+v"(bndv));
-                pv(std::integral_constant<int, CPR>{}, 0, [&](int e, int c) { return code(V[e].c[c / 4], c % 4) * (d0v + c < bndv ? V[e].m0 : V[e].m1); });
+            asm volatile("" : "+v"(bndv));
+            #pragma unroll
+            for (int e = 0; e < 4; e++) {
+                #pragma unroll
+                for (int c = 0; c < CPR; c++) {
+                    const float v = code(V[e].c[c / 4], c % 4) * (d0v + c < bndv ? V[e].m0 : V[e].m1);
+                    #pragma unroll
+                    for (int t = 0; t < RT; t++) O[t][c] = __builtin_amdgcn_mfma_f32_16x16x4f32(S[t][0][e], v, O[t][c], 0, 0, 0);
+                    if (c % 4 == 3) __builtin_amdgcn_sched_barrier(0);
+                }
             }
             __builtin_amdgcn_sched_barrier(0);
             load_v(V, pn, nx);
             pg = pn;
-            pn = page(min(lp + 2, w1 - 1));
+            pn = page(tile + 2 * NW < w1 ? tile + 2 * NW : nx);
             __builtin_amdgcn_sched_barrier(0);
         }
-        while (later) {
-            const int lp = next_off();
-            pg = page(lp);
-            zero_s();
-            load_k(K, pg, lp);
-            scores(K);
-            softmax(lp);
-            pv_slow(lp, [&](int p, int k) {
-                const uint8_t *row = pg + vslice + row_off(lp, p);
-                const uint32_t w = *gmem((const uint32_t *)(row + d0v + 4 * k));
-                const float m0 = *gmem((const float *)(row + HD + 4 * b0v)), m1 = *gmem((const float *)(row + HD + 4 * b1v));
-                v4f v;
-                #pragma unroll
-                for (int c = 0; c < 4; c++) v[c] = code(w, c) * (d0v + 4 * k + c < bndv ? m0 : m1);
-                return v;
-            });
-        }
+        add_later([&](const uint8_t *row, int k) {                         // multipliers that are not finite
+            const float m0 = *gmem((const float *)(row + HD + 4 * b0v)), m1 = *gmem((const float *)(row + HD + 4 * b1v));
+            v4f v;
+            #pragma unroll
+            for (int c = 0; c < 4; c++) v[c] = finite1(127.0f * (d0v + 4 * k + c < bnd0 ? m0 : m1)) ? 0.0f : NAN;
+            return v;
+        });
     }
-    // the four waves' parts: m and l first
+    // the waves' parts: m and l first, then the outputs, 16 rows at a time
     #pragma unroll
     for (int t = 0; t < RT; t++) {
         l[t] += __shfl_xor(l[t], 16, 64);
@@ -428,67 +533,90 @@ __global__ __launch_bounds__(256, 2) void k_tree_float(sp_hipkv_tree_args a, int
         if (g == 0) { s_m[wave][t * 16 + l16] = m[t]; s_l[wave][t * 16 + l16] = l[t]; }
     }
     __syncthreads();                                                       // ... and nobody reads q any more
+    if (threadIdx.x < RT * 16) {
+        const int k = threadIdx.x;
+        float M = -INFINITY, L = 0.0f, f[NW];
+        #pragma unroll
+        for (int w = 0; w < NW; w++) M = fmaxf(M, s_m[w][k]);
+        #pragma unroll
+        for (int w = 0; w < NW; w++) {
+            f[w] = M == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(s_m[w][k] - M);
+            L += f[w] * s_l[w][k];
+        }
+        #pragma unroll
+        for (int w = 0; w < NW; w++) s_m[w][k] = f[w];
+        s_M[k] = M; s_L[k] = L;
+    }
+    __syncthreads();
     float *po = (float *)a.work, *pml = po + (size_t)a.n_nodes * a.n_heads * nsplit * HD;
     #pragma unroll
-    for (int t = 0; t < RT; t++)
+    for (int t = 0; t < RT; t++) {
         #pragma unroll
-        for (int ih = 0; ih < 2; ih++) {                                   // rows 4 g + 2 ih, + 1
+        for (int i = 0; i < 4; i++) {
+            const float f = s_m[wave][t * 16 + 4 * g + i];
+            v2f *dst = (v2f *)lds + (wave * 16 + 4 * g + i) * (HD / 2);
             #pragma unroll
-            for (int i = 2 * ih; i < 2 * ih + 2; i++) {
-                const int r = t * 16 + 4 * g + i;
-                const float M = fmaxf(fmaxf(s_m[0][r], s_m[1][r]), fmaxf(s_m[2][r], s_m[3][r]));
-                const float f = M == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(s_m[wave][r] - M);
-                v4f *dst = (v4f *)lds + ((wave * 8 + 2 * g + (i & 1)) * (HD / 4));
-                #pragma unroll
-                for (int c = 0; c < CPR; c += 4) {
-                    const v4f x = {O[t][c][i], O[t][c + 1][i], O[t][c + 2][i], O[t][c + 3][i]};
-                    dst[SPN ? (CPR / 4) * l16 + c / 4 : 4 * c + l16] = f == 0.0f ? (v4f){0, 0, 0, 0} : x * f;
-                }
+            for (int c = 0; c < CPR; c += 2) {
+                const v2f x = {O[t][c][i], O[t][c + 1][i]};
+                dst[SPN ? (CPR / 2) * l16 + c / 2 : 8 * c + l16] = f == 0.0f ? (v2f){0, 0} : x * f;
             }
-            __syncthreads();
-            for (int i = threadIdx.x; i < 8 * (HD / 4); i += 256) {
-                const int k = i / (HD / 4), c = i % (HD / 4), rl = t * 16 + 4 * (k >> 1) + 2 * ih + (k & 1), r = r0 + rl;
-                if (r >= R) continue;
-                const v4f *src = (const v4f *)lds + k * (HD / 4) + c;
-                v4f x = (src[0] + src[8 * (HD / 4)]) + (src[16 * (HD / 4)] + src[24 * (HD / 4)]);
-                const float M = fmaxf(fmaxf(s_m[0][rl], s_m[1][rl]), fmaxf(s_m[2][rl], s_m[3][rl]));
-                float L = 0.0f;
-                if (M > -INFINITY)
-                    #pragma unroll
-                    for (int w = 0; w < 4; w++) L += s_l[w][rl] * __builtin_amdgcn_exp2f(s_m[w][rl] - M);
-                const int node = q.node0 + r / G, head = h * G + r % G;
-                if (nsplit == 1) {
-                    *(v4f *)(a.out + (size_t)node * a.out_stride + (size_t)head * HD + 4 * c) = M == -INFINITY ? (v4f){0, 0, 0, 0} : x / L;
-                } else {
-                    const size_t at = ((size_t)node * a.n_heads + head) * nsplit + split;
-                    if (M > -INFINITY) *(v4f *)(po + at * HD + 4 * c) = x;
-                    if (c == 0) { pml[2 * at] = M; pml[2 * at + 1] = L; }
-                }
-            }
-            if (t < RT - 1 || ih == 0) __syncthreads();
         }
+        __syncthreads();
+        for (int i = threadIdx.x; i < 4 * HD; i += NT) {                   // 16 rows of HD / 4 pieces
+            const int k = i / (HD / 4), c = i % (HD / 4), rl = t * 16 + k, r = r0 + rl;
+            if (r >= R) continue;
+            const v4f *src = (const v4f *)lds + i;
+            v4f x = (src[0] + src[4 * HD]) + (src[8 * HD] + src[12 * HD]);
+            if constexpr (NW == 8) x += (src[16 * HD] + src[20 * HD]) + (src[24 * HD] + src[28 * HD]);
+            const float M = s_M[rl], L = s_L[rl];
+            const int node = q.node0 + r / G, head = h * G + r % G;
+            if (nsplit == 1) {
+                *(v4f *)(a.out + (size_t)node * a.out_stride + (size_t)head * HD + 4 * c) = L == 0.0f ? (v4f){0, 0, 0, 0} : x / L;
+            } else {
+                const size_t at = ((size_t)node * a.n_heads + head) * nsplit + split;
+                if (M > -INFINITY) *(v4f *)(po + at * HD + 4 * c) = x;
+                if (c == 0) { pml[2 * at] = M; pml[2 * at + 1] = L; }
+            }
+        }
+        if (t < RT - 1) __syncthreads();
+    }
 }
 
-// out = sum_c 2^(m_c - M) O_c / sum_c 2^(m_c - M) l_c; HD / 4 threads a row
+// out = sum_c 2^(m_c - M) O_c / sum_c 2^(m_c - M) l_c: a workgroup per row, HD / 4
+// threads along it, the others share the (at most 64) parts.  Rows of no sequence stay
+// as they were.
 template <int HD>
 __global__ __launch_bounds__(256) void k_tree_merge(sp_hipkv_tree_args a, int nsplit) {
-    const size_t row = (size_t)blockIdx.x * (1024 / HD) + threadIdx.x / (HD / 4);
-    if (row >= (size_t)a.n_nodes * a.n_heads) return;
-    const int c = threadIdx.x % (HD / 4);
-    const v4f *po = (const v4f *)((const float *)a.work + row * nsplit * HD) + c;
+    constexpr int NG = 1024 / HD;
+    __shared__ float s_f[64], s_L;
+    __shared__ v4f s_x[256];
+    const size_t row = blockIdx.x;
+    const int c = threadIdx.x % (HD / 4), grp = threadIdx.x / (HD / 4);
     const float *ml = (const float *)a.work + (size_t)a.n_nodes * a.n_heads * nsplit * HD + 2 * row * nsplit;
-    float M = -INFINITY, L = 0.0f;
-    for (int k = 0; k < nsplit; k++) M = fmaxf(M, ml[2 * k]);
-    v4f x = {0, 0, 0, 0};
-    #pragma unroll 8
-    for (int k = 0; k < nsplit; k++) {
-        const float mk = ml[2 * k];
-        if (!(mk > -INFINITY)) continue;                                   // a part without a position of this row
-        const float f = __builtin_amdgcn_exp2f(mk - M);
-        L += f * ml[2 * k + 1];
-        x += f * po[(size_t)k * (HD / 4)];
+    if (threadIdx.x < 64) {
+        const bool in = (int)threadIdx.x < nsplit;
+        const float m = in ? ml[2 * threadIdx.x] : -INFINITY, l = in ? ml[2 * threadIdx.x + 1] : 0.0f, M = wave_allmax(m);
+        const float f = m > -INFINITY ? __builtin_amdgcn_exp2f(m - M) : 0.0f;        // 0: a part without a position of this row
+        s_f[threadIdx.x] = f;
+        const float L = wave_allsum(f * l);                               // NaN scores: l is NaN also where m is -inf
+        if (threadIdx.x == 0) s_L = L;
     }
-    *(v4f *)(a.out + (row / a.n_heads) * a.out_stride + (row % a.n_heads) * HD + 4 * c) = M > -INFINITY ? x / L : (v4f){0, 0, 0, 0};
+    if (!__syncthreads_or(tree_has(a, (int)(row / a.n_heads), threadIdx.x, 256))) return;
+    const v4f *po = (const v4f *)((const float *)a.work + row * nsplit * HD) + c;
+    v4f x = {0, 0, 0, 0};
+    #pragma unroll 4
+    for (int k = grp; k < nsplit; k += NG) {
+        const v4f v = po[(size_t)k * (HD / 4)];
+        const float f = s_f[k];
+        x += f == 0.0f ? (v4f){0, 0, 0, 0} : f * v;
+    }
+    s_x[threadIdx.x] = x;
+    __syncthreads();
+    if (grp) return;
+    #pragma unroll
+    for (int k = 1; k < NG; k++) x += s_x[k * (HD / 4) + c];
+    const float L = s_L;
+    *(v4f *)(a.out + (row / a.n_heads) * a.out_stride + (row % a.n_heads) * HD + 4 * c) = L == 0.0f ? (v4f){0, 0, 0, 0} : x / L;
 }
 
 // ---------------------------------------------------------------- exact rows
@@ -507,7 +635,6 @@ __global__ __launch_bounds__(256) void k_tree_merge(sp_hipkv_tree_args a, int ns
 // V sums: a wave owns 32 columns and takes a page a step: lane l 16 positions of two
 // columns, which are the B operand after their digits are formed; no transposition.
 // The weights' digits are made once for all waves and pass through LDS.
-typedef int v4i __attribute__((ext_vector_type(4)));
 constexpr int DIG3 = 127 * (1 + 256 + 65536);                    // largest |x| of three balanced digits
 constexpr int DIG4 = 127 * (1 + 256 + 65536 + 16777216);         // ... of four
 
@@ -602,8 +729,8 @@ __global__ __launch_bounds__(256, 2) void k_tree_xscore(sp_hipkv_tree_args a, XW
     const Span sp = rows_span(a, q, G, r0, min(r0 + RT * 16, R));
     const int per = (sp.pg1 - sp.pg0 + x.nsplit - 1) / x.nsplit;
     int w0 = sp.pg0 + split * per, w1 = min(w0 + per, sp.pg1);
-    if (w0 < w1 && w0 * PAGE + wave * TT + TT <= sp.lo_min) w0++;
-    if (w0 < w1 && (w1 - 1) * PAGE + wave * TT >= end) w1--;
+    if (w0 < w1 && w0 * PAGE + wave * 16 + 16 <= sp.lo_min) w0++;
+    if (w0 < w1 && (w1 - 1) * PAGE + wave * 16 >= end) w1--;
     // this lane's output rows: 4 g + i of each tile
     int mx[RT][4], zrow[RT][4];
     #pragma unroll
@@ -619,7 +746,7 @@ __global__ __launch_bounds__(256, 2) void k_tree_xscore(sp_hipkv_tree_args a, XW
     const uint32_t kslice = (uint32_t)h * PAGE * HD * 4;
     auto page = [&](int lp) { return uniform(tree_page(a, q, lp * PAGE)); };
     auto load_k = [&](v4i (&k)[4 * KS], const uint8_t *pg, int lp) {
-        const int p = lp * PAGE + wave * TT + l16;
+        const int p = lp * PAGE + wave * 16 + l16;
         const uint32_t off = kslice + (uint32_t)((p < end ? p : end - 1) & (PAGE - 1)) * (HD * 4) + 16 * g;
         #pragma unroll
         for (int s = 0; s < 4 * KS; s++) k[s] = *gmem((const v4i *)(pg + off + 64 * s));
@@ -632,8 +759,8 @@ __global__ __launch_bounds__(256, 2) void k_tree_xscore(sp_hipkv_tree_args a, XW
         pn = page(min(w0 + 1, w1 - 1));
     }
     for (int lp = w0; lp < w1; lp++) {
-        const int p0 = lp * PAGE + wave * TT, p = p0 + l16;
-        const bool whole = p0 >= sp.lo_max && p0 + TT <= q.cached;
+        const int p0 = lp * PAGE + wave * 16, p = p0 + l16;
+        const bool whole = p0 >= sp.lo_max && p0 + 16 <= q.cached;
         v4i B[4][KS];
         int lv = 0;
         #pragma unroll
@@ -879,7 +1006,12 @@ template <int HD>
 __global__ __launch_bounds__(256) void k_tree_xdiv(sp_hipkv_tree_args a, XWork x) {
     const size_t row = (size_t)blockIdx.x * (256 / HD) + threadIdx.x / HD;
     const int d = threadIdx.x % HD;
-    if (row >= (size_t)a.n_nodes * a.n_heads) return;
+    __shared__ int s_has[256 / HD];
+    if (d == 0) s_has[threadIdx.x / HD] = 0;
+    __syncthreads();
+    if (row < (size_t)a.n_nodes * a.n_heads && tree_has(a, (int)(row / a.n_heads), d, HD)) s_has[threadIdx.x / HD] = 1;
+    __syncthreads();
+    if (!s_has[threadIdx.x / HD]) return;                                  // a row of no sequence stays as it was
     const int64_t *s = x.sum + row * x.vsplit * HD + d, *dn = x.den + row * x.vsplit;
     int64_t t = 0, den = 0;
     #pragma unroll 8
@@ -889,16 +1021,37 @@ __global__ __launch_bounds__(256) void k_tree_xdiv(sp_hipkv_tree_args a, XWork x
 
 // How a launch is cut: row tiles of a workgroup, workgroups along a sequence's rows,
 // splits of its positions.
-struct TreePlan { int rt, groups, nsplit; };
+// The parts of a span are chosen by estimated time: a workgroup's fixed part (set-up, q,
+// first loads, joining its waves: 6 us, Spinor 8), its rounds of tiles and, if there are
+// several, joining the parts.  A round takes about 1.1 us for each row tile and 64 dims
+// and one more (f32; 0.6 of it where one wave of a SIMD has a tile), Spinor's
+// 0.55 us, from stamps of workgroups.  Measured against parts for a fixed 256
+// workgroups: 24 nodes at 4k 28.5 -> 26.9 us, one node at 100 12.2 -> 8.9 us (one
+// part for two), the others alike.
+struct TreePlan { int rt, groups, nsplit, pages; };
 TreePlan tree_plan(const sp_hipkv_tree_args &a) {
     TreePlan p;
-    const int most = a.head_dim == 256 ? 2 : 4, tiles = std::max(1, (a.max_nodes * (a.n_heads / a.n_kv_heads) + 15) / 16);
+    const bool spn = a.rows == SP_HIPKV_ROWS_SPINOR;
+    // row tiles whose outputs a wave's registers hold (with one more they spill, and loads from scratch wait behind
+    // the prefetched tiles: 10 us a page for 3)
+    const int most = a.head_dim == 256 ? (spn ? 1 : 2) : a.head_dim == 128 ? 3 : 4;
+    const int tiles = std::max(1, (a.max_nodes * (a.n_heads / a.n_kv_heads) + 15) / 16);
     p.groups = (tiles + most - 1) / most;
     p.rt = (tiles + p.groups - 1) / p.groups;
-    const int span = a.window ? std::min(a.max_positions, a.window + a.max_nodes + PAGE) : a.max_positions;
+    const int64_t span = a.window ? std::min<int64_t>(a.max_positions, (int64_t)a.window + a.max_nodes + PAGE) : a.max_positions;
     const int64_t base = (int64_t)a.n_kv_heads * p.groups * std::max(a.n_seqs, 1);
-    const int64_t pages = std::max(1, (span + PAGE - 1) / PAGE);
-    p.nsplit = (int)std::max<int64_t>(1, std::min<int64_t>({(512 + base - 1) / base, (pages + 1) / 2, 64}));
+    p.pages = (int)std::max<int64_t>(1, (span + PAGE - 1) / PAGE);
+    const int waves = tree_waves(a.rows), per_page = PAGE / (spn ? 16 : 32);
+    const double round = (spn ? 0.55 : 1.1) * p.rt * (a.head_dim / 64) + (spn ? 0.0 : 1.0);
+    double best = 0;
+    p.nsplit = 0;
+    for (int n = (p.pages + TREE_PAGES - 1) / TREE_PAGES; n <= 64 && n <= p.pages; n++) {
+        const int t = (per_page * p.pages + n - 1) / n, last = (t - 1) % waves + 1;            // tiles of a workgroup
+        const double work = round * ((t - 1) / waves + (!spn && last <= waves / 2 ? 0.6 : 1.0));
+        const int64_t wgs = base * n, lots = (wgs + 255) / 256;                                 // a Spinor workgroup is half a unit's
+        const double us = (spn ? (lots + 1) / 2 * 8.0 + lots * work : lots * (6.0 + work)) + (n > 1 ? 4.0 + 0.05 * n : 0.0);
+        if (!p.nsplit || us < best) { best = us; p.nsplit = n; }
+    }
     return p;
 }
 
@@ -936,14 +1089,15 @@ int64_t tree_grid(const sp_hipkv_tree_args &a, const TreePlan &p) { return (int6
 template <int ROWS> void tree_float(const sp_hipkv_tree_args &a, hipStream_t s) {
     const TreePlan p = tree_plan(a);
     const dim3 grid((uint32_t)tree_grid(a, p)), wg(256);
-#define TREE_RUN(EPL, RT) hipLaunchKernelGGL((k_tree_float<ROWS, EPL, RT>), grid, wg, 0, s, a, p.groups, p.nsplit)
-    if (a.head_dim == 256) { if (p.rt == 1) TREE_RUN(4, 1); else TREE_RUN(4, 2); }
-    else if (a.head_dim == 128) { if (p.rt == 1) TREE_RUN(2, 1); else if (p.rt == 2) TREE_RUN(2, 2); else if (p.rt == 3) TREE_RUN(2, 3); else TREE_RUN(2, 4); }
+#define TREE_RUN(EPL, RT) hipLaunchKernelGGL((k_tree_float<ROWS, EPL, RT>), grid, dim3(64 * tree_waves(ROWS)), 0, s, a, p.groups, p.nsplit, p.pages)
+    if (a.head_dim == 256) {
+        if constexpr (ROWS == SP_HIPKV_ROWS_F32) { if (p.rt == 2) TREE_RUN(4, 2); else TREE_RUN(4, 1); }
+        else TREE_RUN(4, 1);
+    } else if (a.head_dim == 128) { if (p.rt == 1) TREE_RUN(2, 1); else if (p.rt == 2) TREE_RUN(2, 2); else TREE_RUN(2, 3); }
     else { if (p.rt == 1) TREE_RUN(1, 1); else if (p.rt == 2) TREE_RUN(1, 2); else if (p.rt == 3) TREE_RUN(1, 3); else TREE_RUN(1, 4); }
 #undef TREE_RUN
     if (p.nsplit == 1) return;
-    const int64_t rows = (int64_t)a.n_nodes * a.n_heads, per = 1024 / a.head_dim;
-    const dim3 mg((uint32_t)((rows + per - 1) / per));
+    const dim3 mg((uint32_t)((int64_t)a.n_nodes * a.n_heads));
     if (a.head_dim == 256) hipLaunchKernelGGL(k_tree_merge<256>, mg, wg, 0, s, a, p.nsplit);
     else if (a.head_dim == 128) hipLaunchKernelGGL(k_tree_merge<128>, mg, wg, 0, s, a, p.nsplit);
     else hipLaunchKernelGGL(k_tree_merge<64>, mg, wg, 0, s, a, p.nsplit);

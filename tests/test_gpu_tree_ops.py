@@ -159,6 +159,83 @@ def test_one_sided_rows():
     t.ready().check()
 
 
+@pytest.mark.parametrize("rows", [F32, SPINOR])
+def test_seen_rows_that_are_not_finite(rows):
+    """A node that sees NaN in K or V has no number for an answer, also where it sees
+    nothing else; the nodes beside it keep theirs."""
+    t = Tree(rows, 128, 2, [0, 500], [6, 20], kind="chain", seed=15)
+    t.trees[0] = ([{j} for j in range(6)], list(range(6)))
+    vis = t.dv.get()
+    vis[:6, 0] = [1 << j for j in range(6)]
+    t.dv.put(vis)
+    t.cache.set(0, 3, np.nan)                           # node 3 of the first, alone in its sight
+    t.cache.set(1, 500 + 12, np.nan)                    # nodes 12.. of the second
+    t.ready()
+    got, (want, tol) = t.run(), t.want()
+    hit = np.array([3] + list(range(6 + 12, 26)))
+    rest = np.setdiff1d(np.arange(26), hit)
+    assert not np.isfinite(got[hit]).any()
+    assert np.isfinite(got[rest]).all() and (np.abs(got[rest] - want[rest]) <= tol[rest]).all()
+
+
+@pytest.mark.parametrize("rows", ALL)
+def test_sequences_without_nodes(rows):
+    """Empty places in a batch, and rows behind the last sequence."""
+    t = Tree(rows, 128, 2, [40, 300, 0, 9, 1000], [3, 0, 2, 0, 4], seed=16).ready()
+    t.check()
+    before = t.result()
+    t.dstart.put(np.array([0, 3, 3, 5, 5, 5], np.int32))                    # the last sequence's four are nobody's now
+    t.dout.put(np.full_like(t.dout.a, t.MARK))
+    got = t.run()
+    assert np.array_equal(got[:5].view(np.uint32), before[:5].view(np.uint32))
+    assert (got[5:] == t.MARK).all()
+
+
+class Repeated(tree_ref.Cache):
+    """A long span whose table names a few pages again and again."""
+
+    def repeat(self, n):
+        self.page[0] = np.resize(self.page[0], -(-n // 64))
+
+    def values(self, s, positions, v):
+        p = np.asarray(positions)
+        return self.pool[self.page[0][p // 64], v, :, p % 64]
+
+
+@pytest.mark.parametrize("rows,n,hd", [(F32, 1 << 20, 64), (F32, 100003, 256), (EXACT, 1 << 18, 64), (EXACT, 70001, 128)])
+def test_longest_spans(rows, n, hd):
+    """The largest position counts: more pages than one part of a span holds."""
+    t = Tree(rows, hd, 2, [37 * 64 - 3], [3], kind="chain", seed=17, nkv=1)
+    t.cache.__class__ = Repeated
+    t.cache.repeat(n)
+    t.cached = [n - 3]
+    t.dcached.put(np.array(t.cached, np.int32))
+    t.args.max_positions = n
+    t.ready()
+    if rows == EXACT:
+        t.check()
+        return
+    # no sum runs over all n: a wave of eight in a part has n / (8 parts) + 32 positions
+    # at most, parts are of 256 pages at most; then 8 waves and 64 parts are added
+    got, (want, tol) = t.run(), t.want()
+    u, terms = 2.0 ** -24, n / (8 * -(-n // 16384)) + 32 + 8 + 64
+    tol -= (2 * n - 2 * terms) * u * tree_abs(t)
+    assert (tol > 0).all() and tol.max() < 1e-2 and (np.abs(got - want) <= tol).all(), np.abs(got - want).max()
+
+
+def tree_abs(t):
+    """sum p |v| of every node and head."""
+    out = np.zeros((3, t.NH, t.hd))
+    for j in range(3):
+        pos = np.concatenate([np.arange(t.cached[0]), t.cached[0] + np.arange(j + 1)])
+        K, V = t.cache.values(0, pos, 0)[:, 0].astype(np.float64), t.cache.values(0, pos, 1)[:, 0].astype(np.float64)
+        for h in range(t.NH):
+            z = K @ t.q[j, h * t.hd:(h + 1) * t.hd].astype(np.float64) * t.scale
+            w = np.exp(z - z.max())
+            out[j, h] = w / w.sum() @ np.abs(V)
+    return out
+
+
 @pytest.mark.parametrize("rows", ALL)
 def test_strides_and_neighbours(rows):
     Tree(rows, 64, 2, [100, 3], [7, 2], seed=9, pad=12).ready().check()
