@@ -343,7 +343,7 @@ int  sp_hipkv_token_logprobs_work(const sp_hipkv_logprob_args *a, size_t *bytes)
  * No two tables may hold the same page. */
 typedef struct sp_hipkv_keep_args {
     int32_t n_kv_heads;
-    int32_t row_bytes;              /* of one stored row, a multiple of 16 */
+    int32_t row_bytes;              /* of one stored row, a multiple of 16, at most 65536 */
     int32_t n_tables;               /* layers x sequences */
     int32_t n_seqs;
     int32_t max_keep;               /* no list is longer (at most 512) */

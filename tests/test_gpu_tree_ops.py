@@ -381,6 +381,20 @@ def test_logprobs_sure_and_masked_rows():
     assert list(o["ids"][4]) == list(range(20))
 
 
+@pytest.mark.parametrize("V,left", [(9001, 3), (262144, 40), (8192, 31), (1024, 19), (8200, 12)])
+def test_logprobs_masked_vocabularies(V, left):
+    """Few logits above -infinity, some early: the alternatives go on with the
+    lowest masked tokens."""
+    g = np.random.default_rng([V, left])
+    x = np.full((9, V), -np.inf, np.float32)
+    for r in range(9):
+        at = g.permutation(V if r % 3 else min(V, 200))[:left]
+        x[r, at] = g.standard_normal(left)
+    o, _ = logprob(x, 1.0, None, 20)
+    check_logprobs(x, 1.0, None, 20, o)
+    assert np.array_equal(o["ids"], np.argsort(-x, axis=1, kind="stable")[:, :20])
+
+
 def test_logprobs_ties_go_to_the_lowest_token():
     x = np.zeros((3, 20000), np.float32)
     x[0, 1::2] = -0.0                                   # one zero
