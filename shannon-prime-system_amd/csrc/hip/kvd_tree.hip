@@ -70,7 +70,7 @@ __device__ __forceinline__ const uint8_t *uniform(const uint8_t *x) {
 //
 // f32 rows (8 waves, 32 positions a tile).  The f32 matrix cores bound the first form of
 // this kernel: 16x16x4 takes 32 cycles, 154 TF, 223 us of the 322 that 64 nodes of 16
-// heads at 32k took (2 kv heads of 256 dims).  A product of two f32 as six products
+// heads at 32k took (8 kv heads of 256 dims).  A product of two f32 as six products
 // of bf16 pieces (below) costs 2.7 times fewer cycles and errs by 2^-26 of it, less than
 // f32 accumulation does: 235 us.  What bounds it now is a sum, as variants with one part
 // taken out showed: forming the pieces (3 roundings and 2 subtractions for each element) a third, the
@@ -81,7 +81,7 @@ __device__ __forceinline__ const uint8_t *uniform(const uint8_t *x) {
 //
 // Spinor rows (4 waves, 16 positions a tile) keep the f32 matrix cores: codes and
 // multipliers go from memory into registers, are multiplied out there, and are the
-// operands.  36 us for 16 nodes at 6k of 2 kv heads of 256 dims; the f32
+// operands.  36 us for 16 nodes at 6k of 16 heads, 8 kv heads of 256 dims; the f32
 // products are 10 of these, the multiplying-out as many, the rest is fixed (as above).
 //
 // The running maximum only moves when a score exceeds it by 2^8 in the exponent (base
@@ -636,9 +636,9 @@ __global__ __launch_bounds__(256) void k_tree_merge(sp_hipkv_tree_args a, int ns
 // columns, which are the B operand after their digits are formed; no transposition.
 // The weights' digits are made once for all waves and pass through LDS.
 constexpr int DIG3 = 127 * (1 + 256 + 65536);                    // largest |x| of three balanced digits
-constexpr int DIG4 = 127 * (1 + 256 + 65536 + 16777216);         // ... of four
 
-// x = d0 + 2^8 d1 + 2^16 d2 + 2^24 d3, d in [-128, 127]; four values' digits, one dword per place
+// x = d0 + 2^8 d1 + 2^16 d2 + 2^24 d3, d in [-128, 127]; four values' digits, one dword per
+// place.  w[3] == 0: three digits hold them all; a digit of -128 there: perhaps not even four.
 __device__ __forceinline__ void digits_of(const int32_t x[4], uint32_t w[4]) {
     uint32_t d[4];
     #pragma unroll
@@ -648,16 +648,34 @@ __device__ __forceinline__ void digits_of(const int32_t x[4], uint32_t w[4]) {
     w[0] = __builtin_amdgcn_perm(cd0, ab0, 0x05040100u); w[1] = __builtin_amdgcn_perm(cd0, ab0, 0x07060302u);
     w[2] = __builtin_amdgcn_perm(cd2, ab2, 0x05040100u); w[3] = __builtin_amdgcn_perm(cd2, ab2, 0x07060302u);
 }
-// 1: |x| needs a fourth digit, 2: more than four
-__device__ __forceinline__ int level_of(int32_t x) {
-    return ((uint32_t)x + (uint32_t)DIG3 > 2u * DIG3 ? 1 : 0) | ((uint32_t)x + (uint32_t)DIG4 > 2u * DIG4 ? 2 : 0);
+__device__ __forceinline__ bool four_fail(uint32_t w3) { return (w3 & 0x80808080u & ~((w3 & 0x7F7F7F7Fu) + 0x7F7F7F7Fu)) != 0; }
+// sum_k 2^(8 k) a[k]
+template <int N> __device__ __forceinline__ int64_t places(const int32_t (&a)[N]) {
+    static_assert(N == 5 || N == 7, "");
+    int64_t s = (int64_t)a[1] * 256 + a[0];
+    s += (int64_t)a[2] * 65536;
+    s += (int64_t)a[3] * 16777216;
+    int64_t hi = a[4];
+    if constexpr (N == 7) hi += (int64_t)a[5] * 256 + (int64_t)a[6] * 65536;
+    return s + (int64_t)((uint64_t)hi << 32);
 }
-// exp_fixed((z - M) 2^16) >> 8 for z <= M: 2^-g, g = ceil((M - z) log2(e) 2^30 / 2^14) in 30 bits
+// f32(ip / 2^32): one rounding to double, one to f32
+__device__ __forceinline__ float ip_float(int64_t ip) {
+    return (float)fma((double)(uint32_t)ip, 0x1p-32, (double)(int32_t)(ip >> 32));
+}
+// exp_fixed((z - M) 2^16) >> 8 for z <= M: 2^-g, g = ceil((M - z) log2(e) 2^30 / 2^14) in
+// 30 bits; exp2_frac without a branch, each step one 32 x 32 + 64 bit product
 __device__ __forceinline__ int32_t weight_of(int32_t z, int32_t M) {
     const uint64_t g = ((uint64_t)((uint32_t)M - (uint32_t)z) * (uint32_t)LOG2E + 16383) >> 14;
-    const uint32_t n = (uint32_t)(g >> FB), r = (uint32_t)g & (uint32_t)(ONE - 1);
-    if (n >= 23) return 0;
-    return r ? (int32_t)(exp2_frac((uint32_t)ONE - r) >> (n + 9)) : (int32_t)((uint32_t)ONE >> (n + 8));
+    const uint32_t n = (uint32_t)(g >> FB), r = (uint32_t)g & (uint32_t)(ONE - 1), f = (uint32_t)ONE - r;
+    uint32_t e = (uint32_t)EXPC[6];
+    #pragma unroll
+    for (int k = 5; k >= 0; k--) {
+        const uint64_t t = (uint64_t)e * f + ((uint64_t)EXPC[k] << FB);
+        e = __builtin_amdgcn_alignbit((uint32_t)(t >> 32), (uint32_t)t, FB);
+    }
+    e = r ? e : 0x80000000u;
+    return n < 23 ? (int32_t)(e >> ((n + 9) & 31)) : 0;
 }
 
 // Work of exact rows: z [row][zstride], maxima [row][nsplit], V sums [row][vsplit][HD],
@@ -692,8 +710,9 @@ __device__ __forceinline__ bool row_sees(const sp_hipkv_tree_args &a, const Tree
 template <int EPL, int RT>
 __global__ __launch_bounds__(256, 2) void k_tree_xscore(sp_hipkv_tree_args a, XWork x, int groups) {
     constexpr int HD = EPL * 64, KS = EPL, QROW = HD + 16;
-    __shared__ __align__(16) int8_t qd[4][RT * 16][QROW];          // q's digits [place][row][64 ks + 16 g + 4 quarter + e]
+    __shared__ __align__(16) int8_t qd[3][RT * 16][QROW];          // q's digits [place][row][64 ks + 16 g + 4 quarter + e]
     __shared__ int s_level, s_mx[4][RT * 16];
+    __shared__ __align__(16) int s_row[RT * 16];                   // node n_heads + head; past the last row again the last
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), l16 = lane & 15, g = lane >> 4;
     const int G = a.n_heads / a.n_kv_heads;
     int id = blockIdx.x;
@@ -703,129 +722,194 @@ __global__ __launch_bounds__(256, 2) void k_tree_xscore(sp_hipkv_tree_args a, XW
     const TreeSeq q = tree_seq(a, id / x.nsplit);
     const int R = q.nodes * G, r0 = grp * RT * 16;
     if (r0 >= R) return;
-    if (threadIdx.x == 0) s_level = 0;
-    __syncthreads();
     const int end = q.cached + q.nodes, z0 = z_first(a, q);
-    int level = 0;
-    for (int i = threadIdx.x; i < RT * 16 * (HD / 4); i += 256) {
-        const int r = i / (HD / 4), c = i % (HD / 4);
-        int32_t v[4] = {0, 0, 0, 0};
-        if (r0 + r < R) {
-            const float4 f = *(const float4 *)(a.q + (size_t)(q.node0 + (r0 + r) / G) * a.q_stride + (size_t)(h * G + (r0 + r) % G) * HD + 4 * c);
-            v[0] = (int32_t)rintf(f.x * 65536.0f); v[1] = (int32_t)rintf(f.y * 65536.0f);
-            v[2] = (int32_t)rintf(f.z * 65536.0f); v[3] = (int32_t)rintf(f.w * 65536.0f);
-        }
-        uint32_t w[4];
-        #pragma unroll
-        for (int e = 0; e < 4; e++) level |= level_of(v[e]);
-        digits_of(v, w);
-        // dims 64 ks + 16 quarter + 4 g + e
-        const int at = (c / 16) * 64 + (c % 4) * 16 + (c / 4 % 4) * 4;
-        #pragma unroll
-        for (int b = 0; b < 4; b++) *(uint32_t *)&qd[b][r][at] = w[b];
-    }
-    level = (__any(level & 1) ? 1 : 0) | (__any(level & 2) ? 2 : 0);
-    if (level && lane == 0) atomicOr(&s_level, level);
     const Span sp = rows_span(a, q, G, r0, min(r0 + RT * 16, R));
     const int per = (sp.pg1 - sp.pg0 + x.nsplit - 1) / x.nsplit;
     int w0 = sp.pg0 + split * per, w1 = min(w0 + per, sp.pg1);
     if (w0 < w1 && w0 * PAGE + wave * 16 + 16 <= sp.lo_min) w0++;
     if (w0 < w1 && (w1 - 1) * PAGE + wave * 16 >= end) w1--;
-    // this lane's output rows: 4 g + i of each tile
-    int mx[RT][4], zrow[RT][4];
-    #pragma unroll
-    for (int t = 0; t < RT; t++)
-        #pragma unroll
-        for (int i = 0; i < 4; i++) {
-            const int r = r0 + t * 16 + 4 * g + i;
-            mx[t][i] = INT32_MIN;
-            zrow[t][i] = r < R ? (q.node0 + r / G) * a.n_heads + h * G + r % G : -1;
-        }
-    __syncthreads();
-    const int qlevel = s_level;
     const uint32_t kslice = (uint32_t)h * PAGE * HD * 4;
     auto page = [&](int lp) { return uniform(tree_page(a, q, lp * PAGE)); };
-    auto load_k = [&](v4i (&k)[4 * KS], const uint8_t *pg, int lp) {
+    // positions past the last one repeat it
+    auto row_at = [&](int lp) {
         const int p = lp * PAGE + wave * 16 + l16;
-        const uint32_t off = kslice + (uint32_t)((p < end ? p : end - 1) & (PAGE - 1)) * (HD * 4) + 16 * g;
+        return kslice + (uint32_t)((p < end ? p : end - 1) & (PAGE - 1)) * (HD * 4) + 16 * g;
+    };
+    auto load_k = [&](v4i (&k)[4 * KS], const uint8_t *pg, int lp) {
+        const uint32_t off = row_at(lp);
         #pragma unroll
         for (int s = 0; s < 4 * KS; s++) k[s] = *gmem((const v4i *)(pg + off + 64 * s));
     };
+    auto row_q = [&](int r) {
+        const int rr = r0 + r < R ? r0 + r : R - 1;
+        return a.q + (size_t)(q.node0 + rr / G) * a.q_stride + (size_t)(h * G + rr % G) * HD;
+    };
+    auto grid_of = [](float4 f, int32_t (&v)[4]) {
+        v[0] = (int32_t)rintf(f.x * 65536.0f); v[1] = (int32_t)rintf(f.y * 65536.0f);
+        v[2] = (int32_t)rintf(f.z * 65536.0f); v[3] = (int32_t)rintf(f.w * 65536.0f);
+    };
     v4i K[4 * KS];
-    const uint8_t *pg = nullptr, *pn = nullptr;
-    if (w0 < w1) {
-        pg = page(w0);
-        load_k(K, pg, w0);
+    const uint8_t *pn = nullptr;
+    if (w0 < w1) {                                                         // K first: q's digits are made while it comes
+        load_k(K, page(w0), w0);
         pn = page(min(w0 + 1, w1 - 1));
     }
-    for (int lp = w0; lp < w1; lp++) {
+    if (threadIdx.x == 0) s_level = 0;
+    if (threadIdx.x < RT * 16) {
+        const int r = min(r0 + (int)threadIdx.x, R - 1);
+        s_row[threadIdx.x] = (q.node0 + r / G) * a.n_heads + h * G + r % G;
+    }
+    __syncthreads();
+    uint32_t over = 0;
+    #pragma unroll 4
+    for (int i = threadIdx.x; i < RT * 16 * (HD / 4); i += 256) {
+        const int r = i / (HD / 4), c = i % (HD / 4);
+        int32_t v[4];
+        uint32_t w[4];
+        grid_of(*(const float4 *)(row_q(r) + 4 * c), v);
+        digits_of(v, w);
+        over |= w[3];
+        // dims 64 ks + 16 quarter + 4 g + e
+        const int at = (c / 16) * 64 + (c % 4) * 16 + (c / 4 % 4) * 4;
+        #pragma unroll
+        for (int b = 0; b < 3; b++) *(uint32_t *)&qd[b][r][at] = w[b];
+    }
+    if (__any(over != 0) && lane == 0) atomicOr(&s_level, 1);
+    int mx[RT][4];                                                         // of rows 4 g + i of each tile
+    #pragma unroll
+    for (int t = 0; t < RT; t++)
+        #pragma unroll
+        for (int i = 0; i < 4; i++) mx[t][i] = INT32_MIN;
+    __syncthreads();
+    const bool qbig = s_level != 0;
+    const float zscale = a.scale * 16384.0f;
+    // scores into z and the maxima
+    auto finish = [&](int lp, int t, int rowg, const int64_t (&ip)[4]) {
         const int p0 = lp * PAGE + wave * 16, p = p0 + l16;
-        const bool whole = p0 >= sp.lo_max && p0 + 16 <= q.cached;
-        v4i B[4][KS];
-        int lv = 0;
+        const int4 rows = *(const int4 *)&s_row[t * 16 + rowg];
+        const int row[4] = {rows.x, rows.y, rows.z, rows.w};
+        int32_t z[4];
+        #pragma unroll
+        for (int i = 0; i < 4; i++) z[i] = (int32_t)round_away(ip_float(ip[i]) * zscale);   // scale 2^14 is exact: the same product
+        if (p0 >= sp.lo_max && p0 + 16 <= q.cached) {
+            #pragma unroll
+            for (int i = 0; i < 4; i++) {
+                x.z[(size_t)row[i] * x.zstride + (p - z0)] = z[i];
+                mx[t][i] = max(mx[t][i], z[i]);
+            }
+        } else if (p < end) {
+            #pragma unroll
+            for (int i = 0; i < 4; i++) {
+                x.z[(size_t)row[i] * x.zstride + (p - z0)] = z[i];
+                mx[t][i] = row_sees(a, q, row[i] / a.n_heads - q.node0, p) ? max(mx[t][i], z[i]) : mx[t][i];
+            }
+        }
+    };
+    bool later = qbig;
+    for (int lp = qbig ? w1 : w0; lp < w1; lp++) {
+        v4i B[3][KS];
+        uint32_t over = 0;
         #pragma unroll
         for (int s = 0; s < 4 * KS; s++) {
             const int32_t v[4] = {K[s][0], K[s][1], K[s][2], K[s][3]};
             uint32_t w[4];
-            #pragma unroll
-            for (int e = 0; e < 4; e++) lv |= level_of(v[e]);
             digits_of(v, w);
+            over |= w[3];
             #pragma unroll
-            for (int b = 0; b < 4; b++) B[b][s / 4][s % 4] = (int)w[b];
+            for (int b = 0; b < 3; b++) B[b][s / 4][s % 4] = (int)w[b];
         }
-        lv = qlevel | (__any(lv & 1) ? 1 : 0) | (__any(lv & 2) ? 2 : 0);
         __builtin_amdgcn_sched_barrier(0);
         load_k(K, pn, min(lp + 1, w1 - 1));
+        pn = page(min(lp + 2, w1 - 1));
         __builtin_amdgcn_sched_barrier(0);
-        auto dots = [&](auto nd, int t, int64_t (&ip)[4]) {
-            constexpr int ND = decltype(nd)::value;
-            v4i acc[2 * ND - 1];
-            #pragma unroll
-            for (int k = 0; k < 2 * ND - 1; k++) acc[k] = (v4i){0, 0, 0, 0};
-            #pragma unroll
-            for (int ks = 0; ks < KS; ks++) {
-                v4i A[ND];
-                #pragma unroll
-                for (int b = 0; b < ND; b++) A[b] = *(const v4i *)&qd[b][t * 16 + l16][64 * ks + 16 * g];
-                #pragma unroll
-                for (int u = 0; u < ND; u++)
-                    #pragma unroll
-                    for (int b = 0; b < ND; b++) acc[u + b] = __builtin_amdgcn_mfma_i32_16x16x64_i8(A[u], B[b][ks], acc[u + b], 0, 0, 0);
-            }
-            #pragma unroll
-            for (int i = 0; i < 4; i++) {
-                ip[i] = acc[2 * ND - 2][i];
-                #pragma unroll
-                for (int k = 2 * ND - 3; k >= 0; k--) ip[i] = ip[i] * 256 + acc[k][i];
-            }
-        };
+        if (__any(over != 0)) { later = true; continue; }
+        int rowg = 4 * g;
+        asm volatile("" : "+v"(rowg));                                     // rows' numbers read where used, not kept
         #pragma unroll
         for (int t = 0; t < RT; t++) {
+            v4i acc[5];
+            #pragma unroll
+            for (int k = 0; k < 5; k++) acc[k] = (v4i){0, 0, 0, 0};
+            #pragma unroll
+            for (int ks = 0; ks < KS; ks++) {
+                v4i A[3];
+                #pragma unroll
+                for (int b = 0; b < 3; b++) A[b] = *(const v4i *)&qd[b][t * 16 + l16][64 * ks + 16 * g];
+                #pragma unroll
+                for (int u = 0; u < 3; u++)
+                    #pragma unroll
+                    for (int b = 0; b < 3; b++) acc[u + b] = __builtin_amdgcn_mfma_i32_16x16x64_i8(A[u], B[b][ks], acc[u + b], 0, 0, 0);
+            }
             int64_t ip[4];
-            if (lv == 0) dots(std::integral_constant<int, 3>{}, t, ip);
-            else if (lv == 1) dots(std::integral_constant<int, 4>{}, t, ip);
-            else {                                                         // more than four digits: from the numbers
-                const int32_t *kr = (const int32_t *)(pg + kslice) + (size_t)((p < end ? p : end - 1) & (PAGE - 1)) * HD;
+            #pragma unroll
+            for (int i = 0; i < 4; i++) {
+                const int32_t c[5] = {acc[0][i], acc[1][i], acc[2][i], acc[3][i], acc[4][i]};
+                ip[i] = places(c);
+            }
+            finish(lp, t, rowg, ip);
+            __builtin_amdgcn_sched_barrier(0);
+        }
+    }
+    // tiles put off, with four digits, q and K read again
+    for (int lp = later ? w0 : w1; lp < w1; lp++) {
+        const uint8_t *kr = page(lp) + row_at(lp);
+        uint32_t over = qbig ? 1 : 0;
+        for (int s = 0; s < 4 * KS; s++) {
+            const v4i k = *gmem((const v4i *)(kr + 64 * s));
+            const int32_t v[4] = {k[0], k[1], k[2], k[3]};
+            uint32_t w[4];
+            digits_of(v, w);
+            over |= w[3];
+        }
+        if (!__any(over != 0)) continue;
+        #pragma unroll
+        for (int t = 0; t < RT; t++) {
+            v4i acc[7];
+            bool fail = false;
+            #pragma unroll
+            for (int k = 0; k < 7; k++) acc[k] = (v4i){0, 0, 0, 0};
+            const float *qr = row_q(t * 16 + l16) + 4 * g;
+            #pragma unroll 1
+            for (int ks = 0; ks < KS; ks++) {
+                v4i A[4], C[4];
+                #pragma unroll
+                for (int s = 0; s < 4; s++) {
+                    int32_t v[4];
+                    uint32_t w[4];
+                    grid_of(*(const float4 *)(qr + 64 * ks + 16 * s), v);
+                    digits_of(v, w);
+                    fail |= four_fail(w[3]);
+                    #pragma unroll
+                    for (int b = 0; b < 4; b++) A[b][s] = (int)w[b];
+                    const v4i k = *gmem((const v4i *)(kr + 256 * ks + 64 * s));
+                    const int32_t vk[4] = {k[0], k[1], k[2], k[3]};
+                    digits_of(vk, w);
+                    fail |= four_fail(w[3]);
+                    #pragma unroll
+                    for (int b = 0; b < 4; b++) C[b][s] = (int)w[b];
+                }
+                #pragma unroll
+                for (int u = 0; u < 4; u++)
+                    #pragma unroll
+                    for (int b = 0; b < 4; b++) acc[u + b] = __builtin_amdgcn_mfma_i32_16x16x64_i8(A[u], C[b], acc[u + b], 0, 0, 0);
+            }
+            int64_t ip[4];
+            #pragma unroll
+            for (int i = 0; i < 4; i++) {
+                const int32_t c[7] = {acc[0][i], acc[1][i], acc[2][i], acc[3][i], acc[4][i], acc[5][i], acc[6][i]};
+                ip[i] = places(c);
+            }
+            if (__any(fail)) {                                             // more than four: from the numbers
+                const int32_t *kn = (const int32_t *)(kr - 16 * g);
                 for (int i = 0; i < 4; i++) {
-                    const int r = min(r0 + t * 16 + 4 * g + i, R - 1);
-                    const float *qr = a.q + (size_t)(q.node0 + r / G) * a.q_stride + (size_t)(h * G + r % G) * HD;
+                    const float *qn = row_q(t * 16 + 4 * g + i);
                     int64_t s = 0;
-                    for (int d = 0; d < HD; d++) s += (int64_t)(int32_t)rintf(qr[d] * 65536.0f) * gmem(kr)[d];
+                    for (int d = 0; d < HD; d++) s += (int64_t)(int32_t)rintf(qn[d] * 65536.0f) * gmem(kn)[d];
                     ip[i] = s;
                 }
             }
-            #pragma unroll
-            for (int i = 0; i < 4; i++) {
-                const float sc = (float)((double)ip[i] / 4294967296.0) * a.scale;
-                const int32_t z = (int32_t)llround_pow2<14>(sc);
-                if (zrow[t][i] >= 0 && p < end) {
-                    x.z[(size_t)zrow[t][i] * x.zstride + (p - z0)] = z;
-                    if (whole || row_sees(a, q, zrow[t][i] / a.n_heads - q.node0, p)) mx[t][i] = max(mx[t][i], z);
-                }
-            }
+            finish(lp, t, 4 * g, ip);
         }
-        pg = pn;
-        pn = page(min(lp + 2, w1 - 1));
     }
     #pragma unroll
     for (int t = 0; t < RT; t++)
@@ -836,9 +920,9 @@ __global__ __launch_bounds__(256, 2) void k_tree_xscore(sp_hipkv_tree_args a, XW
             if (l16 == 0) s_mx[wave][t * 16 + 4 * g + i] = mx[t][i];
         }
     __syncthreads();
-    if (threadIdx.x < RT * 16 && r0 + (int)threadIdx.x < R) {
-        const int r = r0 + threadIdx.x, k = threadIdx.x;
-        x.zmax[((size_t)(q.node0 + r / G) * a.n_heads + h * G + r % G) * x.nsplit + split] = max(max(s_mx[0][k], s_mx[1][k]), max(s_mx[2][k], s_mx[3][k]));
+    if (threadIdx.x < RT * 16) {
+        const int k = threadIdx.x;
+        x.zmax[(size_t)s_row[k] * x.nsplit + split] = max(max(s_mx[0][k], s_mx[1][k]), max(s_mx[2][k], s_mx[3][k]));
     }
 }
 
@@ -846,9 +930,10 @@ __global__ __launch_bounds__(256, 2) void k_tree_xscore(sp_hipkv_tree_args a, XW
 template <int EPL, int RT>
 __global__ __launch_bounds__(EPL * 128, 2) void k_tree_xsum(sp_hipkv_tree_args a, XWork x, int groups) {
     constexpr int HD = EPL * 64, NT = EPL * 128, ROWS = RT * 16, WROW = PAGE + 16;
-    constexpr int QUADS = (ROWS * 16 + NT - 1) / NT;                           // position quads of a thread and step
+    constexpr int PAIRS = ROWS * 32 / NT, RSTEP = NT / 32;                     // position pairs of a thread and step, rows apart
     __shared__ __align__(16) int8_t wd[2][3][ROWS][WROW];                      // weights' digits [step parity][place][row][position]
-    __shared__ int s_M[ROWS];
+    __shared__ int s_M[ROWS], s_row[ROWS];
+    __shared__ const uint8_t *s_page[TREE_PAGES];                              // this split's (at most 2^14 positions)
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), l16 = lane & 15, g = lane >> 4;
     const int G = a.n_heads / a.n_kv_heads;
     int id = blockIdx.x;
@@ -861,64 +946,64 @@ __global__ __launch_bounds__(EPL * 128, 2) void k_tree_xsum(sp_hipkv_tree_args a
     const int end = q.cached + q.nodes, z0 = z_first(a, q);
     const Span sp = rows_span(a, q, G, r0, min(r0 + ROWS, R));
     const int per = (sp.pg1 - sp.pg0 + x.vsplit - 1) / x.vsplit, b0 = sp.pg0 + split * per, b1 = min(b0 + per, sp.pg1);
-    for (int k = threadIdx.x; k < ROWS; k += NT) {
+    const uint32_t vslice = (uint32_t)(a.n_kv_heads + h) * PAGE * HD * 4;
+    typedef int v2i __attribute__((ext_vector_type(2)));
+    v2i V[16];
+    auto page = [&](int lp) { return uniform(s_page[lp - b0]); };
+    // lane: positions 16 g + j of columns 32 wave + 2 l16, + 1
+    const uint32_t vo = (16 * g * HD + 32 * wave + 2 * l16) * 4;
+    auto load_v = [&](const uint8_t *pg) {
+        #pragma unroll
+        for (int j = 0; j < 16; j++) V[j] = *gmem((const v2i *)(pg + vslice + j * (HD * 4) + vo));
+    };
+    for (int i = threadIdx.x; i < b1 - b0; i += NT) s_page[i] = tree_page(a, q, (b0 + i) * PAGE);
+    if (b0 < b1) load_v(uniform(tree_page(a, q, b0 * PAGE)));
+    // rows' maxima, 8 threads a row; rows without a position or past the last: no row, the least number
+    for (int k = threadIdx.x / 8; k < ROWS; k += NT / 8) {
         int M = INT32_MIN;
-        if (r0 + k < R) {
-            const int32_t *m = x.zmax + ((size_t)(q.node0 + (r0 + k) / G) * a.n_heads + h * G + (r0 + k) % G) * x.nsplit;
-            for (int c = 0; c < x.nsplit; c++) M = max(M, m[c]);
-        }
+        const int r = r0 + k, row = (q.node0 + r / G) * a.n_heads + h * G + r % G;
+        if (r < R)
+            for (int c = threadIdx.x & 7; c < x.nsplit; c += 8) M = max(M, x.zmax[(size_t)row * x.nsplit + c]);
+        #pragma unroll
+        for (int o = 1; o < 8; o <<= 1) M = max(M, __shfl_xor(M, o, 64));
         s_M[k] = M;
+        s_row[k] = r < R && M > INT32_MIN ? row : -1;
     }
     __syncthreads();
-    // this thread's weights: positions 4 (tid % 16) .. of rows tid / 16 + k NT / 16
-    const int quad = threadIdx.x & 15;
-    int64_t den[QUADS];
-    int zrow[QUADS], M[QUADS], node[QUADS];
+    // this thread's weights: positions 2 (tid % 32), + 1 of rows tid / 32 + k RSTEP
+    const int pair = threadIdx.x & 31;
+    int64_t den[PAIRS];
+    int2 z[PAIRS];
     #pragma unroll
-    for (int k = 0; k < QUADS; k++) {
-        const int rl = threadIdx.x / 16 + k * (NT / 16), r = r0 + rl;
-        den[k] = 0;
-        const bool live = rl < ROWS && r < R && s_M[rl < ROWS ? rl : 0] > INT32_MIN;   // (no position seen: weights stay 0)
-        node[k] = live ? r / G : -1;
-        zrow[k] = live ? (q.node0 + r / G) * a.n_heads + h * G + r % G : 0;
-        M[k] = s_M[rl < ROWS ? rl : 0];
-    }
-    int4 z[QUADS];
+    for (int k = 0; k < PAIRS; k++) { den[k] = 0; z[k] = make_int2(0, 0); }
     auto load_z = [&](int lp) {
         #pragma unroll
-        for (int k = 0; k < QUADS; k++)
-            if (node[k] >= 0) z[k] = *(const int4 *)(x.z + (size_t)zrow[k] * x.zstride + (lp * PAGE - z0 + 4 * quad));
+        for (int k = 0; k < PAIRS; k++) {
+            const int row = s_row[threadIdx.x / 32 + k * RSTEP];
+            if (row >= 0) z[k] = *(const int2 *)(x.z + (size_t)row * x.zstride + (lp * PAGE - z0 + 2 * pair));
+        }
     };
     auto weights = [&](int lp, int par) {
         const int p0 = lp * PAGE;
         const bool whole = p0 >= sp.lo_max && p0 + PAGE <= q.cached;
         #pragma unroll
-        for (int k = 0; k < QUADS; k++) {
-            if ((int)threadIdx.x / 16 + k * (NT / 16) >= ROWS) break;
-            int32_t w[4] = {0, 0, 0, 0};
-            if (node[k] >= 0) {
-                const int32_t zz[4] = {z[k].x, z[k].y, z[k].z, z[k].w};
+        for (int k = 0; k < PAIRS; k++) {
+            int rl = threadIdx.x / 32 + k * RSTEP;
+            asm volatile("" : "+v"(rl));                                   // what follows from it is made here, not kept
+            const int M = s_M[rl];
+            int32_t w[2] = {weight_of(z[k].x, M), weight_of(z[k].y, M)};   // (of no row: z = 0 below the least M)
+            if (!whole) {
+                const int node = min(r0 + rl, R - 1) / G;
                 #pragma unroll
-                for (int e = 0; e < 4; e++)
-                    if (whole || row_sees(a, q, node[k], p0 + 4 * quad + e)) w[e] = weight_of(zz[e], M[k]);
+                for (int e = 0; e < 2; e++) w[e] = row_sees(a, q, node, p0 + 2 * pair + e) ? w[e] : 0;
             }
-            den[k] += (int64_t)w[0] + w[1] + w[2] + w[3];
-            uint32_t d[4];
-            digits_of(w, d);
-            #pragma unroll
-            for (int b = 0; b < 3; b++) *(uint32_t *)&wd[par][b][threadIdx.x / 16 + k * (NT / 16)][4 * quad] = d[b];
-        }
-    };
-    const uint32_t vslice = (uint32_t)(a.n_kv_heads + h) * PAGE * HD * 4;
-    typedef int v2i __attribute__((ext_vector_type(2)));
-    v2i V[16];
-    // lane: positions 16 g + j of columns 32 wave + 2 l16, + 1
-    auto load_v = [&](const uint8_t *pg, int lp) {
-        const uint32_t col = vslice + (32 * wave + 2 * l16) * 4;
-        #pragma unroll
-        for (int j = 0; j < 16; j++) {
-            const int p = lp * PAGE + 16 * g + j;
-            V[j] = *gmem((const v2i *)(pg + col + (uint32_t)((p < end ? p : end - 1) & (PAGE - 1)) * (HD * 4)));
+            den[k] += (int64_t)w[0] + w[1];
+            const uint32_t d0 = ((uint32_t)w[0] + 0x808080u) ^ 0x808080u, d1 = ((uint32_t)w[1] + 0x808080u) ^ 0x808080u;
+            const uint32_t lo = __builtin_amdgcn_perm(d1, d0, 0x05010400u), hi = __builtin_amdgcn_perm(d1, d0, 0x0C0C0602u);
+            *(uint16_t *)&wd[par][0][rl][2 * pair] = (uint16_t)lo;
+            *(uint16_t *)&wd[par][1][rl][2 * pair] = (uint16_t)(lo >> 16);
+            *(uint16_t *)&wd[par][2][rl][2 * pair] = (uint16_t)hi;
+            __builtin_amdgcn_sched_barrier(0);
         }
     };
     v4i acc[RT][2][5];
@@ -928,38 +1013,69 @@ __global__ __launch_bounds__(EPL * 128, 2) void k_tree_xsum(sp_hipkv_tree_args a
         for (int c = 0; c < 2; c++)
             #pragma unroll
             for (int k = 0; k < 5; k++) acc[t][c][k] = (v4i){0, 0, 0, 0};
-    auto page = [&](int lp) { return uniform(tree_page(a, q, lp * PAGE)); };
-    if (b0 < b1) { load_z(b0); load_v(page(b0), b0); }
+    // Two waves share a SIMD: half of the waves make their weights of the next page before
+    // the products, half after, so that the vector and the matrix units both have work.
+    const bool first = wave < NT / 128;
+    if (b0 < b1) {
+        load_z(b0);
+        weights(b0, 0);
+        load_z(min(b0 + 1, b1 - 1));
+    }
     for (int lp = b0; lp < b1; lp++) {
         const int par = (lp - b0) & 1, nx = min(lp + 1, b1 - 1);
         const uint8_t *pn = page(nx);
-        weights(lp, par);
-        load_z(nx);
-        __syncthreads();                                                   // (the other parity's readers are past it too)
+        auto next_weights = [&] {
+            if (lp + 1 < b1) {
+                weights(lp + 1, par ^ 1);
+                load_z(min(lp + 2, b1 - 1));
+            }
+        };
+        __syncthreads();                                                   // this page's weights are there, the last one's are read
+        if (first) next_weights();
+        if (lp * PAGE + PAGE > end) {                                      // places behind the last position
+            #pragma unroll
+            for (int j = 0; j < 16; j++)
+                if (lp * PAGE + 16 * g + j >= end) V[j] = (v2i){0, 0};
+        }
         // |v| may exceed three digits by little: what is left goes through once more
         for (bool more = true; more;) {
             v4i B[2][3];
-            int left = 0;
+            uint32_t over = 0;
             #pragma unroll
             for (int c = 0; c < 2; c++)
                 #pragma unroll
                 for (int j = 0; j < 4; j++) {
-                    int32_t v[4];
+                    const int32_t v[4] = {V[4 * j][c], V[4 * j + 1][c], V[4 * j + 2][c], V[4 * j + 3][c]};
                     uint32_t d[4];
-                    #pragma unroll
-                    for (int e = 0; e < 4; e++) {
-                        v[e] = min(max(V[4 * j + e][c], -DIG3), DIG3);
-                        V[4 * j + e][c] -= v[e];
-                        left |= V[4 * j + e][c];
-                    }
                     digits_of(v, d);
+                    over |= d[3];
                     #pragma unroll
                     for (int b = 0; b < 3; b++) B[c][b][j] = (int)d[b];
                 }
-            more = __any(left != 0);
+            more = __any(over != 0);
+            if (more) {
+                int left = 0;
+                #pragma unroll
+                for (int c = 0; c < 2; c++)
+                    #pragma unroll
+                    for (int j = 0; j < 4; j++) {
+                        int32_t v[4];
+                        uint32_t d[4];
+                        #pragma unroll
+                        for (int e = 0; e < 4; e++) {
+                            v[e] = min(max(V[4 * j + e][c], -DIG3), DIG3);
+                            V[4 * j + e][c] -= v[e];
+                            left |= V[4 * j + e][c];
+                        }
+                        digits_of(v, d);
+                        #pragma unroll
+                        for (int b = 0; b < 3; b++) B[c][b][j] = (int)d[b];
+                    }
+                more = __any(left != 0);
+            }
             if (!more) {
                 __builtin_amdgcn_sched_barrier(0);
-                load_v(pn, nx);
+                load_v(pn);
                 __builtin_amdgcn_sched_barrier(0);
             }
             #pragma unroll
@@ -973,14 +1089,15 @@ __global__ __launch_bounds__(EPL * 128, 2) void k_tree_xsum(sp_hipkv_tree_args a
                         for (int c = 0; c < 2; c++) acc[t][c][u + b] = __builtin_amdgcn_mfma_i32_16x16x64_i8(A, B[c][b], acc[t][c][u + b], 0, 0, 0);
                 }
         }
+        if (!first) next_weights();
     }
-    // denominators: over a row's 16 threads
+    // denominators: over a row's 32 threads
     #pragma unroll
-    for (int k = 0; k < QUADS; k++) {
+    for (int k = 0; k < PAIRS; k++) {
         #pragma unroll
-        for (int o = 1; o < 16; o <<= 1) den[k] += __shfl_xor(den[k], o, 64);
-        const int rl = threadIdx.x / 16 + k * (NT / 16), r = r0 + rl;
-        if (rl < ROWS && quad == 0 && r < R) x.den[((size_t)(q.node0 + r / G) * a.n_heads + h * G + r % G) * x.vsplit + split] = den[k];
+        for (int o = 1; o < 32; o <<= 1) den[k] += __shfl_xor(den[k], o, 64);
+        const int r = r0 + threadIdx.x / 32 + k * RSTEP;
+        if (pair == 0 && r < R) x.den[((size_t)(q.node0 + r / G) * a.n_heads + h * G + r % G) * x.vsplit + split] = den[k];
     }
     #pragma unroll
     for (int t = 0; t < RT; t++)
@@ -990,9 +1107,8 @@ __global__ __launch_bounds__(EPL * 128, 2) void k_tree_xsum(sp_hipkv_tree_args a
             int64_t s[2];
             #pragma unroll
             for (int c = 0; c < 2; c++) {
-                s[c] = acc[t][c][4][i];
-                #pragma unroll
-                for (int k = 3; k >= 0; k--) s[c] = s[c] * 256 + acc[t][c][k][i];
+                const int32_t k[5] = {acc[t][c][0][i], acc[t][c][1][i], acc[t][c][2][i], acc[t][c][3][i], acc[t][c][4][i]};
+                s[c] = places(k);
             }
             if (r < R) {
                 int64_t *dst = x.sum + (((size_t)(q.node0 + r / G) * a.n_heads + h * G + r % G) * x.vsplit + split) * HD + 32 * wave + 2 * l16;
@@ -1001,21 +1117,23 @@ __global__ __launch_bounds__(EPL * 128, 2) void k_tree_xsum(sp_hipkv_tree_args a
         }
 }
 
-// one output element per thread
+// a workgroup per row, its parts shared by NG groups of threads
 template <int HD>
-__global__ __launch_bounds__(256) void k_tree_xdiv(sp_hipkv_tree_args a, XWork x) {
-    const size_t row = (size_t)blockIdx.x * (256 / HD) + threadIdx.x / HD;
-    const int d = threadIdx.x % HD;
-    __shared__ int s_has[256 / HD];
-    if (d == 0) s_has[threadIdx.x / HD] = 0;
-    __syncthreads();
-    if (row < (size_t)a.n_nodes * a.n_heads && tree_has(a, (int)(row / a.n_heads), d, HD)) s_has[threadIdx.x / HD] = 1;
-    __syncthreads();
-    if (!s_has[threadIdx.x / HD]) return;                                  // a row of no sequence stays as it was
+__global__ __launch_bounds__(512) void k_tree_xdiv(sp_hipkv_tree_args a, XWork x) {
+    constexpr int NG = 512 / HD;
+    __shared__ int64_t s_t[512], s_d[NG];
+    const size_t row = blockIdx.x;
+    const int d = threadIdx.x % HD, grp = threadIdx.x / HD;
     const int64_t *s = x.sum + row * x.vsplit * HD + d, *dn = x.den + row * x.vsplit;
     int64_t t = 0, den = 0;
     #pragma unroll 8
-    for (int k = 0; k < x.vsplit; k++) { t += s[(size_t)k * HD]; den += dn[k]; }
+    for (int k = grp; k < x.vsplit; k += NG) { t += s[(size_t)k * HD]; den += dn[k]; }
+    s_t[threadIdx.x] = t;
+    if (d == 0) s_d[grp] = den;
+    // a row of no sequence stays as it was
+    if (!__syncthreads_or(tree_has(a, (int)(row / a.n_heads), threadIdx.x, 512)) || grp) return;
+    #pragma unroll
+    for (int k = 1; k < NG; k++) { t += s_t[k * HD + d]; den += s_d[k]; }
     a.out[(row / a.n_heads) * a.out_stride + (row % a.n_heads) * HD + d] = den > 0 ? rne_div_to_float((i128)t, den, 16) : 0.0f;
 }
 
@@ -1103,20 +1221,25 @@ template <int ROWS> void tree_float(const sp_hipkv_tree_args &a, hipStream_t s) 
     else hipLaunchKernelGGL(k_tree_merge<64>, mg, wg, 0, s, a, p.nsplit);
 }
 
-// Exact rows: both passes take up to 48 rows a workgroup; a V split's int32 sums hold
+// Exact rows: a workgroup's row tiles for the scores, whose q digits two workgroups' LDS
+// holds, and for the sums, whose registers hold their accumulators; splits for 512
+// workgroups, for as many as can run at once.  A V split's int32 sums hold
 // 2 x 3 x 2^14 a position (values that need a second round of digits), so at most 2^14 positions.
-struct XPlan { int rt, groups; XWork w; size_t bytes; };
+struct XPlan { int rt, groups, srt, sgroups; XWork w; size_t bytes; };
 XPlan tree_xplan(const sp_hipkv_tree_args &a) {
     XPlan p{};
     const int tiles = std::max(1, (a.max_nodes * (a.n_heads / a.n_kv_heads) + 15) / 16);
-    const int most = a.head_dim == 64 ? 2 : 3;                   // row tiles whose sums a wave's registers hold
+    const int most = a.head_dim == 64 ? 2 : 3;
     p.groups = (tiles + most - 1) / most;
     p.rt = (tiles + p.groups - 1) / p.groups;
+    p.sgroups = (tiles + 5) / 6;
+    p.srt = (tiles + p.sgroups - 1) / p.sgroups;
     const int span = a.window ? (int)std::min<int64_t>(a.max_positions, (int64_t)a.window + a.max_nodes + PAGE) : a.max_positions;
-    const int64_t base = (int64_t)a.n_kv_heads * p.groups * std::max(a.n_seqs, 1), pages = std::max(1, (span + PAGE - 1) / PAGE + 1);
+    const int64_t base = (int64_t)a.n_kv_heads * std::max(a.n_seqs, 1), pages = std::max(1, (span + PAGE - 1) / PAGE + 1);
+    auto splits = [&](int64_t wgs, int64_t each) { return (int)std::max<int64_t>(1, std::min<int64_t>({(wgs + each - 1) / each, (pages + 1) / 2, 64})); };
     p.w.zstride = (int)pages * PAGE;
-    p.w.nsplit = (int)std::max<int64_t>(1, std::min<int64_t>({(512 + base - 1) / base, (pages + 1) / 2, 64}));
-    p.w.vsplit = (int)std::max<int64_t>((pages * PAGE + 16383) >> 14, p.w.nsplit);
+    p.w.nsplit = splits(512, base * p.sgroups);
+    p.w.vsplit = std::max((int)((pages * PAGE + 16383) >> 14), splits(65536 / a.head_dim, base * p.groups));
     const size_t rows = (size_t)a.n_nodes * a.n_heads;
     auto up = [](size_t n) { return (n + 15) / 16 * 16; };
     const size_t zb = up(rows * p.w.zstride * 4), mb = up(rows * p.w.nsplit * 4), sb = rows * p.w.vsplit * a.head_dim * 8;
@@ -1125,16 +1248,17 @@ XPlan tree_xplan(const sp_hipkv_tree_args &a) {
     p.bytes = zb + mb + sb + up(rows * p.w.vsplit * 8);
     return p;
 }
-template <int EPL, int RT> void tree_xgo(const sp_hipkv_tree_args &a, const XPlan &p, hipStream_t s) {
-    const int64_t one = (int64_t)a.n_kv_heads * p.groups * a.n_seqs, rows = (int64_t)a.n_nodes * a.n_heads, per = 256 / (EPL * 64);
-    hipLaunchKernelGGL((k_tree_xscore<EPL, RT>), dim3((uint32_t)(one * p.w.nsplit)), dim3(256), 0, s, a, p.w, p.groups);
-    hipLaunchKernelGGL((k_tree_xsum<EPL, RT>), dim3((uint32_t)(one * p.w.vsplit)), dim3(EPL * 128), 0, s, a, p.w, p.groups);
-    hipLaunchKernelGGL(k_tree_xdiv<EPL * 64>, dim3((uint32_t)((rows + per - 1) / per)), dim3(256), 0, s, a, p.w);
-}
 template <int EPL> void tree_xgo(const sp_hipkv_tree_args &a, const XPlan &p, hipStream_t s) {
-    if (p.rt == 1) tree_xgo<EPL, 1>(a, p, s);
-    else if (EPL == 1 || p.rt == 2) tree_xgo<EPL, 2>(a, p, s);
-    else if constexpr (EPL > 1) tree_xgo<EPL, 3>(a, p, s);
+    const int64_t base = (int64_t)a.n_kv_heads * a.n_seqs;
+#define TREE_SCORE(RT) hipLaunchKernelGGL((k_tree_xscore<EPL, RT>), dim3((uint32_t)(base * p.sgroups * p.w.nsplit)), dim3(256), 0, s, a, p.w, p.sgroups)
+#define TREE_SUM(RT) hipLaunchKernelGGL((k_tree_xsum<EPL, RT>), dim3((uint32_t)(base * p.groups * p.w.vsplit)), dim3(EPL * 128), 0, s, a, p.w, p.groups)
+    if (p.srt == 1) TREE_SCORE(1); else if (p.srt == 2) TREE_SCORE(2); else if (p.srt == 3) TREE_SCORE(3); else if (p.srt == 4) TREE_SCORE(4); else TREE_SCORE(6);
+    if (p.rt == 1) TREE_SUM(1);
+    else if (EPL == 1 || p.rt == 2) TREE_SUM(2);
+    else if constexpr (EPL > 1) TREE_SUM(3);
+    hipLaunchKernelGGL(k_tree_xdiv<EPL * 64>, dim3((uint32_t)((int64_t)a.n_nodes * a.n_heads)), dim3(512), 0, s, a, p.w);
+#undef TREE_SCORE
+#undef TREE_SUM
 }
 void tree_exact(const sp_hipkv_tree_args &a, hipStream_t s) {
     const XPlan p = tree_xplan(a);
@@ -1163,7 +1287,7 @@ extern "C" int sp_hipkv_tree_attention_work(const sp_hipkv_tree_args *a, size_t 
         sp_hipkv_tree_args b = *a;
         b.work = nullptr;
         const XPlan p = tree_xplan(b);
-        OP_NEED((int64_t)a->n_kv_heads * p.groups * a->n_seqs * p.w.vsplit <= 1 << 22, "too many sequences, heads and nodes for one launch");
+        OP_NEED((int64_t)a->n_kv_heads * a->n_seqs * std::max(p.groups * p.w.vsplit, p.sgroups * p.w.nsplit) <= 1 << 22, "too many sequences, heads and nodes for one launch");
         *bytes = p.bytes;
         return 0;
     }
