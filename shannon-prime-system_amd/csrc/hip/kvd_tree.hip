@@ -1137,38 +1137,41 @@ __global__ __launch_bounds__(512) void k_tree_xdiv(sp_hipkv_tree_args a, XWork x
     a.out[(row / a.n_heads) * a.out_stride + (row % a.n_heads) * HD + d] = den > 0 ? rne_div_to_float((i128)t, den, 16) : 0.0f;
 }
 
-// How a launch is cut: row tiles of a workgroup, workgroups along a sequence's rows,
-// splits of its positions.
-// The parts of a span are chosen by estimated time: a workgroup's fixed part (set-up, q,
-// first loads, joining its waves: 6 us, Spinor 8), its rounds of tiles and, if there are
-// several, joining the parts.  A round takes about 1.1 us for each row tile and 64 dims
-// and one more (f32; 0.6 of it where one wave of a SIMD has a tile), Spinor's
-// 0.55 us, from stamps of workgroups.  Measured against parts for a fixed 256
-// workgroups: 24 nodes at 4k 28.5 -> 26.9 us, one node at 100 12.2 -> 8.9 us (one
-// part for two), the others alike.
+// How a launch is cut: row tiles of a workgroup (rt), workgroups along a sequence's rows
+// (groups), parts of its positions (nsplit): whatever the least time is estimated for.
+//   A round of tiles, one a wave: 1.1 us for each row tile and 64 dims, and one more (f32;
+//   0.6 of it where one wave of a SIMD has a tile); Spinor 0.55 us.
+//   A workgroup besides: 4.5 us and 1.5 for each row tile (set-up, q, joining its waves); Spinor 8.
+//   The groups read K and V again from L2: 25 TB/s.  Joining parts: 4 us.
+// From stamps of workgroups, and sweeps of both numbers.  Against one fixed choice (most row
+// tiles, 256 workgroups): one node at 100 12.2 -> 9.0 us (one part for two), 8 nodes at 600
+// 15.5 -> 12.4 (two groups for one), 24 nodes at 4k 28.5 -> 26.9 (11 parts for 16).
 struct TreePlan { int rt, groups, nsplit, pages; };
 TreePlan tree_plan(const sp_hipkv_tree_args &a) {
-    TreePlan p;
+    TreePlan p{};
     const bool spn = a.rows == SP_HIPKV_ROWS_SPINOR;
     // row tiles whose outputs a wave's registers hold (with one more they spill, and loads from scratch wait behind
     // the prefetched tiles: 10 us a page for 3)
     const int most = a.head_dim == 256 ? (spn ? 1 : 2) : a.head_dim == 128 ? 3 : 4;
     const int tiles = std::max(1, (a.max_nodes * (a.n_heads / a.n_kv_heads) + 15) / 16);
-    p.groups = (tiles + most - 1) / most;
-    p.rt = (tiles + p.groups - 1) / p.groups;
     const int64_t span = a.window ? std::min<int64_t>(a.max_positions, (int64_t)a.window + a.max_nodes + PAGE) : a.max_positions;
-    const int64_t base = (int64_t)a.n_kv_heads * p.groups * std::max(a.n_seqs, 1);
     p.pages = (int)std::max<int64_t>(1, (span + PAGE - 1) / PAGE);
     const int waves = tree_waves(a.rows), per_page = PAGE / (spn ? 16 : 32);
-    const double round = (spn ? 0.55 : 1.1) * p.rt * (a.head_dim / 64) + (spn ? 0.0 : 1.0);
+    const double seqs = (double)a.n_kv_heads * std::max(a.n_seqs, 1);
+    const double mb = seqs * p.pages * PAGE * 2 * row_bytes_of(a.rows, a.head_dim) * 1e-6;
     double best = 0;
-    p.nsplit = 0;
-    for (int n = (p.pages + TREE_PAGES - 1) / TREE_PAGES; n <= 64 && n <= p.pages; n++) {
-        const int t = (per_page * p.pages + n - 1) / n, last = (t - 1) % waves + 1;            // tiles of a workgroup
-        const double work = round * ((t - 1) / waves + (!spn && last <= waves / 2 ? 0.6 : 1.0));
-        const int64_t wgs = base * n, lots = (wgs + 255) / 256;                                 // a Spinor workgroup is half a unit's
-        const double us = (spn ? (lots + 1) / 2 * 8.0 + lots * work : lots * (6.0 + work)) + (n > 1 ? 4.0 + 0.05 * n : 0.0);
-        if (!p.nsplit || us < best) { best = us; p.nsplit = n; }
+    for (int m = most; m >= 1; m--) {
+        const int groups = (tiles + m - 1) / m, rt = (tiles + groups - 1) / groups;
+        if (rt < m) continue;                                                                   // the same as a smaller m
+        const double round = (spn ? 0.55 : 1.1) * rt * (a.head_dim / 64) + (spn ? 0.0 : 1.0);
+        for (int n = (p.pages + TREE_PAGES - 1) / TREE_PAGES; n <= 64 && n <= p.pages; n++) {
+            const int t = (per_page * p.pages + n - 1) / n, last = (t - 1) % waves + 1;        // tiles of a workgroup
+            const double work = round * ((t - 1) / waves + (!spn && last <= waves / 2 ? 0.6 : 1.0));
+            const double lots = std::ceil(seqs * groups * n / 256);                             // a Spinor workgroup is half a unit's
+            const double us = (spn ? std::ceil(lots / 2) * 8.0 + lots * work : lots * (4.5 + 1.5 * rt + work))
+                            + 0.04 * mb * groups + (n > 1 ? 4.0 + 0.05 * n : 0.0);
+            if (!p.nsplit || us < best) { best = us; p.nsplit = n; p.rt = rt; p.groups = groups; }
+        }
     }
     return p;
 }
