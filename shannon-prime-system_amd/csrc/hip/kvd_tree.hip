@@ -7,9 +7,9 @@
 //                      w_p = exp_fixed((z_p - M) 2^16) >> 8, out = RNE(sum w vq / (2^16 sum w)),
 // the decode attention's integers (kvd_attn.hip).
 //
-// f32 and Spinor rows run in one pass over K and V (k_tree_float), f32 rows on the bf16
-// matrix cores in exact pieces, Spinor rows on the f32 ones; exact rows on the int8 matrix
-// cores in two passes (k_tree_xscore, _xsum).
+// f32 and Spinor rows run in one pass over K and V (k_tree_float), on the bf16 matrix
+// cores in exact pieces; exact rows on the int8 matrix cores in two passes (k_tree_xscore,
+// _xsum).
 #include "kvd_op.h"
 #include "kvd_exact.h"
 #include "kvd_vec.h"
@@ -79,10 +79,14 @@ __device__ __forceinline__ const uint8_t *uniform(const uint8_t *x) {
 // a SIMD.  Memory comes through LDS by direct loads: held in registers on
 // the way, a tile cost 64 more of them (250 us).
 //
-// Spinor rows (4 waves, 16 positions a tile) keep the f32 matrix cores: codes and
-// multipliers go from memory into registers, are multiplied out there, and are the
-// operands.  36 us for 16 nodes at 6k of 16 heads, 8 kv heads of 256 dims; the f32
-// products are 10 of these, the multiplying-out as many, the rest is fixed (as above).
+// Spinor rows (4 waves, 32 positions a tile): a code is a bf16 number as it is, so three
+// products with q's or the weights' pieces are exact, and a chunk's multiplier (one number for a
+// position) joins outside the product: on the scores of the chunk's dims, and on the weights
+// before they are taken apart.  Dims and columns are therefore dealt to steps and tiles by
+// chunk, as windows of 64 dims of which 51 (43, 32) count.  16 nodes at 6k of 16 heads (8 kv
+// heads of 256 dims) take 26.5 us; as f32 products of codes times multipliers, which was the first form,
+// 36.5, and 30 nodes of 32 heads at 12k 50 for 82 us.  The codes' conversion bounds it now, 1.5
+// instructions a code, and below 20 us what is fixed.
 //
 // The running maximum only moves when a score exceeds it by 2^8 in the exponent (base
 // 2): weights stay below 2^8 and nothing is lost, and a tile needs one ballot instead of
@@ -105,6 +109,7 @@ typedef __bf16 bf8 __attribute__((ext_vector_type(8)));
 typedef __bf16 bf2 __attribute__((ext_vector_type(2)));
 typedef float v2f __attribute__((ext_vector_type(2)));
 typedef uint32_t v4u32 __attribute__((ext_vector_type(4)));
+typedef uint32_t v2u32 __attribute__((ext_vector_type(2), aligned(4)));
 struct Pieces { bf8 p[3]; };
 template <typename X> __device__ __forceinline__ Pieces pieces_of(X &&x) {                 // of x(0) .. x(7)
     v4u32 w[3];
@@ -126,20 +131,29 @@ __device__ __forceinline__ v4f mfma_piece(const Pieces &a, const Pieces &b, int 
     return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a.p[MUL_A[n]], b.p[MUL_B[n]], c, 0, 0, 0);
 }
 
+// The first dword of a window of `win` bytes of a Spinor row that holds chunk b's codes and ends inside the row
+__device__ constexpr int spn_window(int hd, int b, int win) {
+    const int d = spn_block_start(hd, b) / 4, most = (row_bytes_of(SP_HIPKV_ROWS_SPINOR, hd) - win) / 4;
+    return d < most ? d : most;
+}
+
 template <int ROWS, int EPL, int RT>
 __global__ __launch_bounds__(64 * tree_waves(ROWS), 2) void k_tree_float(sp_hipkv_tree_args a, int groups, int nsplit, int pages) {
-    constexpr int HD = EPL * 64, CPR = HD / 16, RB = row_bytes_of(ROWS, HD);
+    constexpr int HD = EPL * 64, RB = row_bytes_of(ROWS, HD);
     constexpr bool SPN = ROWS == SP_HIPKV_ROWS_SPINOR;
-    constexpr int NS = SPN ? 1 : 2, TP = 16 * NS;                          // 16-position tiles a wave takes at a time
+    constexpr int TP = 32;                                                 // positions a wave takes at a time
     constexpr int NW = tree_waves(ROWS), NT = 64 * NW;
-    // q (f32; or [piece][row][dim] bf16) and the waves' rings, then the waves' outputs
-    constexpr int Q_B = RT * 16 * HD * (SPN ? 4 : 6), UNIT = 4096, OUT_B = NW * 16 * HD * 4;
-    constexpr int RING = SPN ? 0 : 152 * 1024 - Q_B >= 4 * NW * UNIT ? 4 : 3;
+    // Spinor: a chunk's dims as a window of WIN from a multiple of 4 on; its columns as four tiles
+    constexpr int NB = SPN ? spn_blocks(HD) : 0, WIN = HD == 64 ? 32 : 64, QD = SPN ? NB * WIN : HD;
+    constexpr int CPR = SPN ? 4 * NB : HD / 16;                            // column tiles
+    // q, [piece][row][dim] bf16, and the waves' rings or multipliers; then the waves' outputs
+    constexpr int Q_B = RT * 16 * QD * 6, UNIT = SPN ? 2048 : 4096, OUT_B = NW * 16 * HD * 4;
+    constexpr int RING = SPN ? 1 : 152 * 1024 - Q_B >= 4 * NW * UNIT ? 4 : 3;
     constexpr int LDS_B = Q_B + NW * RING * UNIT > OUT_B ? Q_B + NW * RING * UNIT : OUT_B;
     __shared__ __align__(1024) uint8_t lds[LDS_B];
     __shared__ float s_m[NW][RT * 16], s_l[NW][RT * 16], s_M[RT * 16], s_L[RT * 16];
     __shared__ int s_node[RT * 16], s_low[RT * 16];
-    __shared__ const uint8_t *s_page[SPN ? 1 : TREE_PAGES];               // this split's
+    __shared__ const uint8_t *s_page[TREE_PAGES];                         // this split's
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), l16 = lane & 15, g = lane >> 4;
     const int G = a.n_heads / a.n_kv_heads;
     int id = blockIdx.x;
@@ -174,22 +188,22 @@ __global__ __launch_bounds__(64 * tree_waves(ROWS), 2) void k_tree_float(sp_hipk
         return a.q + (size_t)(q.node0 + rr / G) * a.q_stride + (size_t)(h * G + rr % G) * HD;
     };
     // 16-byte pieces of a row in an order that spreads a column over the banks
-    if constexpr (SPN) {
-        for (int i = threadIdx.x; i < RT * 16 * (HD / 4); i += NT) {
-            const int r = i / (HD / 4), c = i % (HD / 4);
-            ((v4f *)lds)[r * (HD / 4) + (c ^ (r & 15))] = *(const v4f *)(row_q(r) + 4 * c);
-        }
-    } else {
-        for (int i = threadIdx.x; i < b1 - b0 && i < TREE_PAGES; i += NT) s_page[i] = tree_page(a, q, (b0 + i) * PAGE);
-        for (int i = threadIdx.x; i < RT * 16 * (HD / 8); i += NT) {
-            const int r = i / (HD / 8), c = i % (HD / 8);
+    for (int i = threadIdx.x; i < b1 - b0 && i < TREE_PAGES; i += NT) s_page[i] = tree_page(a, q, (b0 + i) * PAGE);
+    for (int i = threadIdx.x; i < RT * 16 * (QD / 8); i += NT) {
+        const int r = i / (QD / 8), c = i % (QD / 8);
+        Pieces p;
+        if constexpr (SPN) {                                               // zeros beside the chunk's dims
+            const int b = c / (WIN / 8), d0 = 4 * spn_window(HD, b, WIN) + 8 * (c % (WIN / 8));
+            const float *x = row_q(r);
+            p = pieces_of([&](int k) { return d0 + k < HD && spn_block_of(HD, d0 + k) == b ? x[d0 + k] : 0.0f; });
+        } else {
             const v4f x = *(const v4f *)(row_q(r) + 8 * c), y = *(const v4f *)(row_q(r) + 8 * c + 4);
-            const Pieces p = pieces_of([&](int k) { return k < 4 ? x[k] : y[k - 4]; });
-            #pragma unroll
-            for (int n = 0; n < 3; n++) ((bf8 *)lds)[(n * RT * 16 + r) * (HD / 8) + (c ^ (r & 7))] = p.p[n];
+            p = pieces_of([&](int k) { return k < 4 ? x[k] : y[k - 4]; });
         }
+        #pragma unroll
+        for (int n = 0; n < 3; n++) ((bf8 *)lds)[(n * RT * 16 + r) * (QD / 8) + (c ^ (r & (WIN == 32 && SPN ? 3 : 7)))] = p.p[n];
     }
-    v4f O[RT][CPR], S[RT][NS];
+    v4f O[RT][CPR], S[RT][2];
     float m[RT], l[RT];
     #pragma unroll
     for (int t = 0; t < RT; t++) {
@@ -200,7 +214,7 @@ __global__ __launch_bounds__(64 * tree_waves(ROWS), 2) void k_tree_float(sp_hipk
     __syncthreads();
     const uint32_t kslice = (uint32_t)h * PAGE * RB, vslice = (uint32_t)(a.n_kv_heads + h) * PAGE * RB;
     // page addresses are the wave's: rows load as address + 32-bit lane offset
-    auto page = [&](int tile) { return uniform(tree_page(a, q, tile * TP)); };
+    auto page_at = [&](int tile) { return uniform(s_page[tile / (PAGE / TP) - b0]); };
     // tiles that some row does not see whole, and those of them with a V value that is
     // not finite: nodes span at most 10 pages, so do the rows' window starts
     auto ragged = [&](int tile) { return tile * TP < lo_max || tile * TP + TP > q.cached; };
@@ -227,7 +241,7 @@ __global__ __launch_bounds__(64 * tree_waves(ROWS), 2) void k_tree_float(sp_hipk
         for (int t = 0; t < RT; t++) {
             float mx = -INFINITY;
             #pragma unroll
-            for (int u = 0; u < NS; u++) {
+            for (int u = 0; u < 2; u++) {
                 #pragma unroll
                 for (int i = 0; i < 4; i++) S[t][u][i] *= a.scale * LOG2E_F;
                 if (rag) {
@@ -253,7 +267,7 @@ __global__ __launch_bounds__(64 * tree_waves(ROWS), 2) void k_tree_float(sp_hipk
             }
             const float ms = m[t] == -INFINITY ? 0.0f : m[t];
             #pragma unroll
-            for (int u = 0; u < NS; u++)
+            for (int u = 0; u < 2; u++)
                 #pragma unroll
                 for (int i = 0; i < 4; i++) { S[t][u][i] = __builtin_amdgcn_exp2f(S[t][u][i] - ms); l[t] += S[t][u][i]; }
         }
@@ -263,7 +277,7 @@ __global__ __launch_bounds__(64 * tree_waves(ROWS), 2) void k_tree_float(sp_hipk
         while (later) {
             const int b = __builtin_ctzll(later), tile = b < 32 ? tail + b : head + b - 32;
             later &= later - 1;
-            const uint8_t *pg = page(tile);
+            const uint8_t *pg = page_at(tile);
             for (int p = tile * TP; p < tile * TP + TP && p < end; p++) {
                 #pragma unroll
                 for (int t = 0; t < RT; t++) {
@@ -290,7 +304,7 @@ __global__ __launch_bounds__(64 * tree_waves(ROWS), 2) void k_tree_float(sp_hipk
         #pragma unroll
         for (int t = 0; t < RT; t++)
             #pragma unroll
-            for (int u = 0; u < NS; u++) S[t][u] = (v4f){0, 0, 0, 0};
+            for (int u = 0; u < 2; u++) S[t][u] = (v4f){0, 0, 0, 0};
     };
     if constexpr (!SPN) {
         // A tile's memory comes in units of 32 rows x 128 bytes, straight into a ring of the
@@ -302,7 +316,6 @@ __global__ __launch_bounds__(64 * tree_waves(ROWS), 2) void k_tree_float(sp_hipk
         const uint32_t ring = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t *)(lds + Q_B + wave * RING * UNIT);
         const uint8_t *ringp = lds + Q_B + wave * RING * UNIT;
         const int rj = lane >> 3, vo_k = rj * RB + ((lane & 7) ^ rj) * 16, vo_v = (16 * (rj >> 2) + 4 * (rj & 3)) * RB + ((lane & 7) ^ rj) * 16;
-        auto page_at = [&](int tile) { return uniform(s_page[tile / (PAGE / TP) - b0]); };
         auto load = [&](const uint8_t *pg, int tile, int n, uint32_t slot) {
             const int row = tile * TP & (PAGE - 1);
             const bool v = n >= NK;
@@ -417,112 +430,138 @@ __global__ __launch_bounds__(64 * tree_waves(ROWS), 2) void k_tree_float(sp_hipk
             return (v4f){x[0], x[1], y[0], y[1]};
         });
     } else {
-        // K: 16 codes of dims 64 i + 16 g.. a load; V: the CPR codes of columns CPR l16..
-        // (O[t][c] is column CPR l16 + c), and the multipliers of the at most two
-        // chunks that they lie in
-        constexpr int NM = spn_blocks(HD);
-        const v4f *qs = (const v4f *)lds;
-        int kb[4];
-        #pragma unroll
-        for (int e = 0; e < 4; e++) kb[e] = l16 * (HD / 4) + ((4 * g + e) ^ l16);
+        // Codes are bf16 numbers as they are.  A chunk's multiplier is one number for a position:
+        // scores of a chunk's dims are multiplied by it when they are summed, and for a chunk's
+        // columns the weights are, before their pieces are taken.  Multipliers go through
+        // LDS, [K, V][chunk][position], from the rows' lanes to those of the scores.
+        constexpr int KD = WIN / 16;                                       // dwords of a lane in a window
+        float (*mul)[8][32] = (float (*)[8][32])(lds + Q_B + wave * UNIT);
+        const bf8 *qs = (const bf8 *)lds;
+        struct Row { uint32_t c[KD]; };
+        Row K[NB][2];
+        uint32_t V[NB][8];
+        v4f km, vm;
         // positions past the last one repeat it
         auto row_off = [&](int tile, int x) { const int p = tile * TP + x; return (uint32_t)((p < end ? p : end - 1) & (PAGE - 1)) * RB; };
-        struct KRow { uint4 c[EPL]; float m[NM]; };
-        struct VRow { uint32_t c[EPL]; float m0, m1; };
-        const int d0v = CPR * l16, b0v = spn_block_of(HD, d0v), bnd0 = spn_block_start(HD, b0v + 1), b1v = bnd0 < d0v + CPR ? b0v + 1 : b0v;
-        int bndv = bnd0;
-        auto load_k = [&](KRow &x, const uint8_t *pg, int tile) {
-            const uint8_t *row = pg + kslice + row_off(tile, l16);
+        const int part = NB > 4 ? lane >> 5 : 0;                           // chunks 4 part .. of row lane % 32
+        auto load_k = [&](const uint8_t *pg, int tile) {
             #pragma unroll
-            for (int i = 0; i < EPL; i++) x.c[i] = *gmem((const uint4 *)(row + 64 * i + 16 * g));
-            #pragma unroll
-            for (int b = 0; b < NM; b++) x.m[b] = *gmem((const float *)(row + HD + 4 * b));
-        };
-        auto load_v = [&](VRow (&x)[4], const uint8_t *pg, int tile) {
-            #pragma unroll
-            for (int e = 0; e < 4; e++) {
-                const uint8_t *row = pg + vslice + row_off(tile, 4 * g + e);
+            for (int u = 0; u < 2; u++) {
+                const uint8_t *row = pg + kslice + row_off(tile, 16 * u + l16) + 4 * KD * g;
                 #pragma unroll
-                for (int i = 0; i < EPL; i++) x[e].c[i] = *gmem((const uint32_t *)(row + d0v + 4 * i));
-                x[e].m0 = *gmem((const float *)(row + HD + 4 * b0v));
-                x[e].m1 = *gmem((const float *)(row + HD + 4 * b1v));
+                for (int b = 0; b < NB; b++)
+                    #pragma unroll
+                    for (int d = 0; d < KD; d += 2) {
+                        const v2u32 w = *gmem((const v2u32 *)(row + 4 * spn_window(HD, b, WIN) + 4 * d));
+                        K[b][u].c[d] = w[0]; K[b][u].c[d + 1] = w[1];
+                    }
             }
+            km = *gmem((const v4f *)(pg + kslice + row_off(tile, lane & 31) + HD + 16 * part));
+        };
+        auto load_v = [&](const uint8_t *pg, int tile) {
+            #pragma unroll
+            for (int j = 0; j < 8; j++) {
+                const uint8_t *row = pg + vslice + row_off(tile, 16 * (j >> 2) + 4 * g + (j & 3)) + 4 * l16;
+                #pragma unroll
+                for (int b = 0; b < NB; b++) V[b][j] = *gmem((const uint32_t *)(row + 4 * spn_window(HD, b, 64)));
+            }
+            vm = *gmem((const v4f *)(pg + vslice + row_off(tile, lane & 31) + HD + 16 * part));
+        };
+        auto put_mul = [&](int kv, v4f x) {
+            #pragma unroll
+            for (int i = 0; i < 4; i++) mul[kv][4 * part + i][lane & 31] = x[i];
+            __builtin_amdgcn_wave_barrier();
         };
         auto code = [](uint32_t w, int t) { return (float)(int32_t)(int8_t)(w >> (8 * t)); };
-        KRow K;
-        VRow V[4];
+        auto codes = [&](auto &&x) {                                       // of x(0) .. x(7), exactly
+            v4u32 w;
+            #pragma unroll
+            for (int k = 0; k < 4; k++) w[k] = __builtin_bit_cast(uint32_t, __builtin_convertvector((v2f){x(2 * k), x(2 * k + 1)}, bf2));
+            return __builtin_bit_cast(bf8, w);
+        };
         const uint8_t *pg = nullptr, *pn = nullptr;
         if (w0 < w1) {
-            pg = page(w0);
-            load_k(K, pg, w0);
-            load_v(V, pg, w0);
-            pn = page(w0 + NW < w1 ? w0 + NW : w0);
+            pg = page_at(w0);
+            load_k(pg, w0);
+            load_v(pg, w0);
         }
         for (int tile = w0; tile < w1; tile += NW) {
             const int nx = tile + NW < w1 ? tile + NW : tile;
             const bool rag = ragged(tile);
+            pn = page_at(nx);
             zero_s();
+            put_mul(0, km);
             #pragma unroll
-            for (int i = 0; i < EPL; i++) {
-                const int d0 = 64 * i + 16 * g, b = spn_block_of(HD, d0);
-                int bnd = spn_block_start(HD, b + 1);
-                asm volatile("" : "+v"(bnd));                              // compared where used: kept masks would fill the scalar registers
-                float m0 = K.m[0], m1 = K.m[0];
+            for (int b = 0; b < NB; b++) {
+                v4f C[RT][2];
                 #pragma unroll
-                for (int bb = 1; bb < NM; bb++) { if (b == bb) m0 = K.m[bb]; if (b + 1 == bb) m1 = K.m[bb]; }
-                const uint32_t w[4] = {K.c[i].x, K.c[i].y, K.c[i].z, K.c[i].w};
+                for (int t = 0; t < RT; t++)
+                    #pragma unroll
+                    for (int u = 0; u < 2; u++) C[t][u] = (v4f){0, 0, 0, 0};
                 #pragma unroll
-                for (int k = 0; k < 4; k++) {
-                    v4f qv[RT];
+                for (int ks = 0; ks < KD / 2; ks++) {
+                    bf8 A[2];
                     #pragma unroll
-                    for (int t = 0; t < RT; t++) qv[t] = qs[kb[k] + t * 4 * HD + 16 * i];
-                    float kv[4];
+                    for (int u = 0; u < 2; u++) A[u] = codes([&](int k) { return code(K[b][u].c[2 * ks + k / 4], k % 4); });
                     #pragma unroll
-                    for (int e = 0; e < 4; e++) kv[e] = code(w[k], e) * (d0 + 4 * k + e < bnd ? m0 : m1);
-                    #pragma unroll
-                    for (int e = 0; e < 4; e++)
+                    for (int t = 0; t < RT; t++) {
+                        bf8 Q[3];
+                        const int c = b * (WIN / 8) + KD / 2 * g + ks;
                         #pragma unroll
-                        for (int t = 0; t < RT; t++) S[t][0] = __builtin_amdgcn_mfma_f32_16x16x4f32(kv[e], qv[t][e], S[t][0], 0, 0, 0);
-                    if (k % 2) __builtin_amdgcn_sched_barrier(0);
+                        for (int n = 0; n < 3; n++) Q[n] = qs[(n * RT * 16 + t * 16 + l16) * (QD / 8) + (c ^ (l16 & (WIN == 32 ? 3 : 7)))];
+                        #pragma unroll
+                        for (int n = 2; n >= 0; n--)
+                            #pragma unroll
+                            for (int u = 0; u < 2; u++) C[t][u] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(A[u], Q[n], C[t][u], 0, 0, 0);
+                    }
                 }
+                #pragma unroll
+                for (int u = 0; u < 2; u++) {
+                    const v4f mk = *(const v4f *)&mul[0][b][16 * u + 4 * g];
+                    #pragma unroll
+                    for (int t = 0; t < RT; t++)
+                        #pragma unroll
+                        for (int i = 0; i < 4; i++) S[t][u][i] = fmaf(mk[i], C[t][u][i], S[t][u][i]);
+                }
+                __builtin_amdgcn_sched_barrier(0);
             }
-            __builtin_amdgcn_sched_barrier(0);
-            load_k(K, pn, nx);
+            load_k(pn, nx);
             __builtin_amdgcn_sched_barrier(0);
             softmax(tile, rag);
             if (rag) {
                 bool bad = false;
                 #pragma unroll
-                for (int e = 0; e < 4; e++) {
-                    const bool f0 = finite1(127.0f * V[e].m0), f1 = finite1(127.0f * V[e].m1);
-                    bad |= !f0 || !f1;
-                    V[e].m0 = f0 ? V[e].m0 : 0.0f; V[e].m1 = f1 ? V[e].m1 : 0.0f;
+                for (int i = 0; i < 4; i++) {
+                    const bool f = finite1(127.0f * vm[i]) || 4 * part + i >= NB;
+                    bad |= !f;
+                    vm[i] = f ? vm[i] : 0.0f;
                 }
                 if (__any(bad)) put_off(tile);
             }
-            asm volatile("" : "+v"(bndv));
+            put_mul(1, vm);
             #pragma unroll
-            for (int e = 0; e < 4; e++) {
+            for (int b = 0; b < NB; b++) {
+                const v4f m0 = *(const v4f *)&mul[1][b][4 * g], m1 = *(const v4f *)&mul[1][b][16 + 4 * g];
+                Pieces P[RT];
                 #pragma unroll
-                for (int c = 0; c < CPR; c++) {
-                    const float v = code(V[e].c[c / 4], c % 4) * (d0v + c < bndv ? V[e].m0 : V[e].m1);
+                for (int t = 0; t < RT; t++) P[t] = pieces_of([&](int k) { return S[t][k >> 2][k & 3] * (k < 4 ? m0[k & 3] : m1[k & 3]); });
+                #pragma unroll
+                for (int c = 0; c < 4; c++) {
+                    const bf8 B = codes([&](int k) { return code(V[b][k], c); });
                     #pragma unroll
-                    for (int t = 0; t < RT; t++) O[t][c] = __builtin_amdgcn_mfma_f32_16x16x4f32(S[t][0][e], v, O[t][c], 0, 0, 0);
-                    if (c % 4 == 3) __builtin_amdgcn_sched_barrier(0);
+                    for (int t = 0; t < RT; t++)
+                        #pragma unroll
+                        for (int n = 2; n >= 0; n--) O[t][4 * b + c] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(P[t].p[n], B, O[t][4 * b + c], 0, 0, 0);
                 }
+                __builtin_amdgcn_sched_barrier(0);
             }
+            load_v(pn, nx);
             __builtin_amdgcn_sched_barrier(0);
-            load_v(V, pn, nx);
             pg = pn;
-            pn = page(tile + 2 * NW < w1 ? tile + 2 * NW : nx);
-            __builtin_amdgcn_sched_barrier(0);
         }
-        add_later([&](const uint8_t *row, int k) {                         // multipliers that are not finite
-            const float m0 = *gmem((const float *)(row + HD + 4 * b0v)), m1 = *gmem((const float *)(row + HD + 4 * b1v));
-            v4f v;
-            #pragma unroll
-            for (int c = 0; c < 4; c++) v[c] = finite1(127.0f * (d0v + 4 * k + c < bnd0 ? m0 : m1)) ? 0.0f : NAN;
-            return v;
+        add_later([&](const uint8_t *row, int b) {                         // multipliers that are not finite
+            const float m = *gmem((const float *)(row + HD + 4 * b));
+            return finite1(127.0f * m) ? (v4f){0, 0, 0, 0} : (v4f){NAN, NAN, NAN, NAN};
         });
     }
     // the waves' parts: m and l first, then the outputs, 16 rows at a time
@@ -554,11 +593,21 @@ __global__ __launch_bounds__(64 * tree_waves(ROWS), 2) void k_tree_float(sp_hipk
         #pragma unroll
         for (int i = 0; i < 4; i++) {
             const float f = s_m[wave][t * 16 + 4 * g + i];
-            v2f *dst = (v2f *)lds + (wave * 16 + 4 * g + i) * (HD / 2);
-            #pragma unroll
-            for (int c = 0; c < CPR; c += 2) {
-                const v2f x = {O[t][c][i], O[t][c + 1][i]};
-                dst[SPN ? (CPR / 2) * l16 + c / 2 : 8 * c + l16] = f == 0.0f ? (v2f){0, 0} : x * f;
+            float *dst = (float *)lds + (wave * 16 + 4 * g + i) * HD;
+            if constexpr (SPN) {                                           // tile 4 b + c: columns 4 (window + lane) + c of chunk b
+                #pragma unroll
+                for (int b = 0; b < NB; b++) {
+                    const int d0 = 4 * (spn_window(HD, b, 64) + l16);
+                    #pragma unroll
+                    for (int c = 0; c < 4; c++)
+                        if (d0 + c >= spn_block_start(HD, b) && d0 + c < spn_block_start(HD, b + 1)) dst[d0 + c] = f == 0.0f ? 0.0f : O[t][4 * b + c][i] * f;
+                }
+            } else {
+                #pragma unroll
+                for (int c = 0; c < CPR; c += 2) {
+                    const v2f x = {O[t][c][i], O[t][c + 1][i]};
+                    ((v2f *)dst)[8 * c + l16] = f == 0.0f ? (v2f){0, 0} : x * f;
+                }
             }
         }
         __syncthreads();
@@ -1139,37 +1188,41 @@ __global__ __launch_bounds__(512) void k_tree_xdiv(sp_hipkv_tree_args a, XWork x
 
 // How a launch is cut: row tiles of a workgroup (rt), workgroups along a sequence's rows
 // (groups), parts of its positions (nsplit): whatever the least time is estimated for.
-//   A round of tiles, one a wave: 1.1 us for each row tile and 64 dims, and one more (f32;
-//   0.6 of it where one wave of a SIMD has a tile); Spinor 0.55 us.
-//   A workgroup besides: 4.5 us and 1.5 for each row tile (set-up, q, joining its waves); Spinor 8.
+//   f32: a round of tiles, one a wave, 1.1 us for each row tile and 64 dims, and one more
+//   (0.6 of it where one wave of a SIMD has a tile); a workgroup 4.5 us and 1.5 for each row
+//   tile (set-up, q, joining its waves).
+//   Spinor: a round 0.7 us, and for each 128 dims 0.45 and 0.9 for each row tile (1.7 times it
+//   where two workgroups share a unit); a workgroup 4 us for each row tile and 1 for each 32
+//   dims.  Several sequences are taken to be 0.6 of the longest (8 of 300 to 4000: 39 us for 55;
+//   for f32's one workgroup a unit that misleads: 16 sessions 112 us for 99).
 //   The groups read K and V again from L2: 25 TB/s.  Joining parts: 4 us.
 // From stamps of workgroups, and sweeps of both numbers.  Against one fixed choice (most row
 // tiles, 256 workgroups): one node at 100 12.2 -> 9.0 us (one part for two), 8 nodes at 600
-// 15.5 -> 12.4 (two groups for one), 24 nodes at 4k 28.5 -> 26.9 (11 parts for 16).
+// 15.5 -> 12.4 (two groups for one), 24 nodes at 4k 28.5 -> 25.9 (8 parts for 16).
 struct TreePlan { int rt, groups, nsplit, pages; };
 TreePlan tree_plan(const sp_hipkv_tree_args &a) {
     TreePlan p{};
     const bool spn = a.rows == SP_HIPKV_ROWS_SPINOR;
     // row tiles whose outputs a wave's registers hold (with one more they spill, and loads from scratch wait behind
     // the prefetched tiles: 10 us a page for 3)
-    const int most = a.head_dim == 256 ? (spn ? 1 : 2) : a.head_dim == 128 ? 3 : 4;
+    const int most = (a.head_dim == 256 ? 2 : a.head_dim == 128 ? 3 : 4) - (spn ? 1 : 0);
     const int tiles = std::max(1, (a.max_nodes * (a.n_heads / a.n_kv_heads) + 15) / 16);
     const int64_t span = a.window ? std::min<int64_t>(a.max_positions, (int64_t)a.window + a.max_nodes + PAGE) : a.max_positions;
     p.pages = (int)std::max<int64_t>(1, (span + PAGE - 1) / PAGE);
-    const int waves = tree_waves(a.rows), per_page = PAGE / (spn ? 16 : 32);
-    const double seqs = (double)a.n_kv_heads * std::max(a.n_seqs, 1);
+    const int waves = tree_waves(a.rows);
+    const double seqs = (double)a.n_kv_heads * (spn && a.n_seqs > 1 ? 0.6 * a.n_seqs : std::max(a.n_seqs, 1));
     const double mb = seqs * p.pages * PAGE * 2 * row_bytes_of(a.rows, a.head_dim) * 1e-6;
     double best = 0;
     for (int m = most; m >= 1; m--) {
         const int groups = (tiles + m - 1) / m, rt = (tiles + groups - 1) / groups;
         if (rt < m) continue;                                                                   // the same as a smaller m
-        const double round = (spn ? 0.55 : 1.1) * rt * (a.head_dim / 64) + (spn ? 0.0 : 1.0);
+        const double round = spn ? 0.7 + a.head_dim / 128.0 * (0.45 + 0.9 * rt) : 1.0 + 1.1 * rt * (a.head_dim / 64);
         for (int n = (p.pages + TREE_PAGES - 1) / TREE_PAGES; n <= 64 && n <= p.pages; n++) {
-            const int t = (per_page * p.pages + n - 1) / n, last = (t - 1) % waves + 1;        // tiles of a workgroup
-            const double work = round * ((t - 1) / waves + (!spn && last <= waves / 2 ? 0.6 : 1.0));
-            const double lots = std::ceil(seqs * groups * n / 256);                             // a Spinor workgroup is half a unit's
-            const double us = (spn ? std::ceil(lots / 2) * 8.0 + lots * work : lots * (4.5 + 1.5 * rt + work))
-                            + 0.04 * mb * groups + (n > 1 ? 4.0 + 0.05 * n : 0.0);
+            const int t = (PAGE / 32 * p.pages + n - 1) / n, lots = (int)std::ceil(seqs * groups * n / 256);   // tiles of a workgroup; workgroups of a unit
+            const int rounds = (t + waves - 1) / waves;
+            double us = 0.04 * mb * groups + (n > 1 ? 4.0 + 0.05 * n : 0.0);
+            if (spn) us += (lots + 1) / 2 * (a.head_dim / 32 + 4.0 * rt) + round * rounds * (lots / 2 * 1.7 + lots % 2);
+            else us += lots * (4.5 + 1.5 * rt + round * (rounds - ((t - 1) % waves < waves / 2 ? 0.4 : 0.0)));
             if (!p.nsplit || us < best) { best = us; p.nsplit = n; p.rt = rt; p.groups = groups; }
         }
     }
@@ -1214,8 +1267,8 @@ template <int ROWS> void tree_float(const sp_hipkv_tree_args &a, hipStream_t s) 
     if (a.head_dim == 256) {
         if constexpr (ROWS == SP_HIPKV_ROWS_F32) { if (p.rt == 2) TREE_RUN(4, 2); else TREE_RUN(4, 1); }
         else TREE_RUN(4, 1);
-    } else if (a.head_dim == 128) { if (p.rt == 1) TREE_RUN(2, 1); else if (p.rt == 2) TREE_RUN(2, 2); else TREE_RUN(2, 3); }
-    else { if (p.rt == 1) TREE_RUN(1, 1); else if (p.rt == 2) TREE_RUN(1, 2); else if (p.rt == 3) TREE_RUN(1, 3); else TREE_RUN(1, 4); }
+    } else if (a.head_dim == 128) { if (p.rt == 1) TREE_RUN(2, 1); else if (p.rt == 2) TREE_RUN(2, 2); else if constexpr (ROWS == SP_HIPKV_ROWS_F32) TREE_RUN(2, 3); }
+    else { if (p.rt == 1) TREE_RUN(1, 1); else if (p.rt == 2) TREE_RUN(1, 2); else if (p.rt == 3) TREE_RUN(1, 3); else if constexpr (ROWS == SP_HIPKV_ROWS_F32) TREE_RUN(1, 4); }
 #undef TREE_RUN
     if (p.nsplit == 1) return;
     const dim3 mg((uint32_t)((int64_t)a.n_nodes * a.n_heads));
