@@ -279,13 +279,17 @@ enum { SP_HIPKV_ROWS_F32 = 0, SP_HIPKV_ROWS_EXACT = 1, SP_HIPKV_ROWS_SPINOR = 2 
  *     (itself and its ancestors in a tree; the window does not clear bits):
  *   out = sum_p softmax_p(scale q.k_p) v_p          in f32
  * or, for exact rows, with the integer arithmetic of exact mode (bit for bit what
- * a decode step computes on the same rows; |q| below 2^15, |scores| below 2^17).  Nodes that see no position get zeros.  Rows
- * that a node does not see do not reach it whatever they hold. */
+ * a decode step computes on the same rows; |q| below 2^15, |scores| below 2^17).
+ * Nodes that see no position get zeros.  Rows that a node does not see do not
+ * reach it whatever they hold; one that it sees with a value that is not finite
+ * leaves it without a finite value (magnitudes from 2^127 on may count as that, of
+ * Spinor rows a multiplier's times 127).  Rows of `out` behind the last sequence's
+ * nodes stay as they are. */
 typedef struct sp_hipkv_tree_args {
     int32_t n_heads, n_kv_heads;    /* at most 4096, and 16 q heads for each kv head */
     int32_t head_dim;               /* 64, 128 or 256 */
     int32_t rows;                   /* SP_HIPKV_ROWS_* */
-    int32_t n_seqs, n_nodes;        /* sequences (at most 4096), nodes of all of them */
+    int32_t n_seqs, n_nodes;        /* sequences (at most 4096), nodes of all of them (times n_heads at most 2^22) */
     int32_t max_nodes;              /* no sequence has more (at most 512) */
     int32_t max_positions;          /* cached + nodes of no sequence is more (at most 2^20; exact rows 2^18) */
     int32_t window;                 /* 0: every cached position */
@@ -306,8 +310,8 @@ typedef struct sp_hipkv_tree_args {
 } sp_hipkv_tree_args;
 int  sp_hipkv_tree_attention(const sp_hipkv_tree_args *a, void *stream);
 /* Bytes of `work` for these sizes (the pointers are not looked at).  The number
- * of parts that a long span is cut into, and with it the order of the f32 sums,
- * goes by the sizes in the block, never by the contents of the arrays. */
+ * of parts that a span is cut into, and with it the order of the f32 sums, goes by
+ * the sizes in the block and the sequence's own lengths, not by other sequences'. */
 int  sp_hipkv_tree_attention_work(const sp_hipkv_tree_args *a, size_t *bytes);
 
 /* Of each row of logits, with y = scale x and p = softmax(y): log p of given

@@ -183,6 +183,13 @@ __global__ __launch_bounds__(64 * tree_waves(ROWS), 2) void k_tree_float(sp_hipk
     const int parts = max((int)(((int64_t)np * nsplit + pages - 1) / pages), (np + TREE_PAGES - 1) / TREE_PAGES);
     const int b0 = pg0 + (int)((int64_t)np * min(split, parts) / parts), b1 = pg0 + (int)((int64_t)np * min(split + 1, parts) / parts);
     const int t0 = max(b0 * (PAGE / TP), lo_min / TP), w1 = min(b1 * (PAGE / TP), (end + TP - 1) / TP), w0 = t0 + wave;
+    float *po = (float *)a.work, *pml = po + (size_t)a.n_nodes * a.n_heads * nsplit * HD;
+    if (nsplit > 1 && t0 >= w1) {                                          // nothing here (splits past this sequence's parts)
+        const int r = r0 + threadIdx.x;
+        if (threadIdx.x < RT * 16 && r < R)
+            *(v2f *)(pml + 2 * (((size_t)(q.node0 + r / G) * a.n_heads + h * G + r % G) * nsplit + split)) = (v2f){-INFINITY, 0.0f};
+        return;
+    }
     auto row_q = [&](int r) {
         const int rr = r0 + r < R ? r0 + r : R - 1;
         return a.q + (size_t)(q.node0 + rr / G) * a.q_stride + (size_t)(h * G + rr % G) * HD;
@@ -587,7 +594,6 @@ __global__ __launch_bounds__(64 * tree_waves(ROWS), 2) void k_tree_float(sp_hipk
         s_M[k] = M; s_L[k] = L;
     }
     __syncthreads();
-    float *po = (float *)a.work, *pml = po + (size_t)a.n_nodes * a.n_heads * nsplit * HD;
     #pragma unroll
     for (int t = 0; t < RT; t++) {
         #pragma unroll
@@ -678,12 +684,21 @@ __global__ __launch_bounds__(256) void k_tree_merge(sp_hipkv_tree_args a, int ns
 // The weights need M before the first of them, hence z in memory: 4 bytes a row and
 // position, written and read once, against 8 HD bytes of K and V for all G nodes rows.
 //
-// Scores: as in the f32 kernel a wave takes 16 positions straight into registers, here
-// as the B operand (16 dims a lane and step, in an order that q's digits in LDS
-// share), makes their digits once and multiplies them with all row tiles.
+// Scores: a wave takes 16 positions straight into registers as the B operand (16 dims a
+// lane and step, in an order that q's digits in LDS share), makes their digits once and
+// multiplies them with all row tiles, up to 6 (96 rows), so that K is read and taken
+// apart once for that many.  Tiles whose numbers, or whose q, need a fourth digit are put off to a
+// loop behind: in the main one its registers spilled, which cost 30 us of 150.
 // V sums: a wave owns 32 columns and takes a page a step: lane l 16 positions of two
 // columns, which are the B operand after their digits are formed; no transposition.
-// The weights' digits are made once for all waves and pass through LDS.
+// The weights' digits are made once for all waves and pass through LDS; half of the waves
+// make the next page's before the products, half after.
+//
+// 48 nodes of 16 heads at 32k (8 kv heads of 256 dims): scores 105 us, sums 120, division
+// 6; reading K and V once is 113 us, and variants with one part taken out name none
+// that would give more than 40 (memory's wait; the int8 products, digits, weights and
+// epilogues 10 each).  7 nodes at 4k: 9.7 + 11 + 3.4 us, where no part but the first loads (3 us)
+// shows: launches and dependent loads.
 constexpr int DIG3 = 127 * (1 + 256 + 65536);                    // largest |x| of three balanced digits
 
 // x = d0 + 2^8 d1 + 2^16 d2 + 2^24 d3, d in [-128, 127]; four values' digits, one dword per
@@ -1241,7 +1256,7 @@ int tree_check(const char *who, const sp_hipkv_tree_args *a) {
     OP_NEED(a->max_positions >= 0 && a->max_positions <= (a->rows == SP_HIPKV_ROWS_EXACT ? 1 << 18 : 1 << 20),
             "max_positions outside [0, 2^20] (exact rows: 2^18)");
     OP_NEED(a->n_nodes <= (int64_t)a->n_seqs * a->max_nodes, "n_nodes is more than n_seqs times max_nodes");
-    OP_NEED((int64_t)a->n_nodes * a->n_heads <= 1 << 28, "more than 2^28 rows (n_nodes x n_heads)");
+    OP_NEED((int64_t)a->n_nodes * a->n_heads <= 1 << 22, "more than 2^22 rows (n_nodes x n_heads)");
     OP_NEED(a->window >= 0 && a->ring_pages >= 0, "negative window or ring_pages");
     return 0;
 }
@@ -1348,7 +1363,7 @@ extern "C" int sp_hipkv_tree_attention_work(const sp_hipkv_tree_args *a, size_t 
         return 0;
     }
     const TreePlan p = tree_plan(*a);
-    OP_NEED(tree_grid(*a, p) <= 1 << 23, "too many sequences, heads and nodes for one launch");
+    OP_NEED(tree_grid(*a, p) <= 1 << 22, "too many sequences, heads and nodes for one launch");
     if (p.nsplit > 1) *bytes = (size_t)a->n_nodes * a->n_heads * p.nsplit * (a->head_dim + 2) * 4;
     return 0;
 }

@@ -20,7 +20,7 @@ def tree(**kw):
 @pytest.mark.parametrize("bad", [
     dict(head_dim=96), dict(head_dim=0), dict(n_kv_heads=0), dict(n_heads=12), dict(n_heads=0), dict(n_heads=136, n_kv_heads=8),
     dict(rows=3), dict(rows=-1), dict(n_seqs=-1), dict(n_seqs=4097), dict(n_heads=4104, n_kv_heads=1026), dict(n_nodes=-1), dict(n_nodes=33), dict(max_nodes=513, mask_words=9),
-    dict(max_positions=(1 << 20) + 1), dict(rows=spkv.ROWS_EXACT, max_positions=(1 << 18) + 1), dict(max_positions=-1),
+    dict(n_seqs=4096, n_nodes=(1 << 18) + 1, max_nodes=512, mask_words=8), dict(max_positions=(1 << 20) + 1), dict(rows=spkv.ROWS_EXACT, max_positions=(1 << 18) + 1), dict(max_positions=-1),
     dict(window=-1), dict(ring_pages=-1), dict(max_nodes=65, mask_words=1), dict(scale=float("nan")), dict(scale=float("inf")),
     dict(node_start=None), dict(cached=None), dict(visible=None), dict(tables=None), dict(q=None), dict(out=None),
     dict(window=5, depth=None), dict(q_stride=2047), dict(q_stride=2050), dict(out_stride=100), dict(q=P + 4), dict(out=P + 8),
