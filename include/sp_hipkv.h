@@ -252,8 +252,9 @@ int  sp_hipkv_info(const sp_kvdecode_handle *h, long long out[8]);
  * own cache.  No counterpart in the reference (its decode takes one token).
  *
  * A page holds 64 positions of one layer: K [n_kv_heads][64] rows, then V the
- * same.  A page table is an array of page addresses, entry p / 64 (of a ring:
- * p / 64 % ring_pages) for position p.  Rows of head_dim values:
+ * same; it starts 16-byte aligned.  A page table is an array of page addresses,
+ * entry p / 64 (of a ring: p / 64 % ring_pages) for position p.  Rows of head_dim
+ * values:
  *   SP_HIPKV_ROWS_F32     f32
  *   SP_HIPKV_ROWS_EXACT   int32, k and v as rne(x 2^16), |v| below 2^23
  *   SP_HIPKV_ROWS_SPINOR  head_dim int8 codes, then one f32 multiplier for each
