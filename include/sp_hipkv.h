@@ -312,7 +312,8 @@ typedef struct sp_hipkv_tree_args {
 int  sp_hipkv_tree_attention(const sp_hipkv_tree_args *a, void *stream);
 /* Bytes of `work` for these sizes (the pointers are not looked at).  The number
  * of parts that a span is cut into, and with it the order of the f32 sums, goes by
- * the sizes in the block and the sequence's own lengths, not by other sequences'. */
+ * the sizes in the block and the sequence's own lengths, not by other sequences'.
+ * Ask again when a size changes: a smaller call may need more parts. */
 int  sp_hipkv_tree_attention_work(const sp_hipkv_tree_args *a, size_t *bytes);
 
 /* Of each row of logits, with y = scale x and p = softmax(y): log p of given
@@ -338,6 +339,7 @@ typedef struct sp_hipkv_logprob_args {
     size_t work_bytes;
 } sp_hipkv_logprob_args;
 int  sp_hipkv_token_logprobs(const sp_hipkv_logprob_args *a, void *stream);
+/* Bytes of `work`; what a call needs is enough for fewer rows and alternatives too. */
 int  sp_hipkv_token_logprobs_work(const sp_hipkv_logprob_args *a, size_t *bytes);
 
 /* Keep the accepted nodes of drafted trees: in every table of sequence s, the K and

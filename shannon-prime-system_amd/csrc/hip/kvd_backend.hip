@@ -1775,6 +1775,11 @@ int sp_hipkv_tree_step(sp_kvdecode_handle *h, const int32_t *tokens, const int32
         if (p >= 0) { nth[i] = kids[p]++; most = std::max(most, kids[p]); }
     }
     if (logprob && most > SCORE_GIVEN) return fail("sp_hipkv_tree_step: log probabilities of at most %s%lld children of a node", "", (long long)SCORE_GIVEN);
+    sp_hipkv_tree_args limits{};
+    limits.n_heads = m->NH; limits.n_kv_heads = m->NKV; limits.head_dim = m->HD; limits.n_seqs = 1; limits.n_nodes = limits.max_nodes = n;
+    limits.rows = h->mode == EXACT ? SP_HIPKV_ROWS_EXACT : SP_HIPKV_ROWS_F32; limits.max_positions = h->dpos + n;
+    size_t unused;
+    if (sp_hipkv_tree_attention_work(&limits, &unused)) return 1;          // head layouts and contexts beyond the operator's
     if (h->rec.B > 0) return fail("sp_hipkv_tree_step: recall is on (a tree attends every position)%s");
     if (!batch_supported(h) || !gemm_supported(m->out)) return fail("sp_hipkv_tree_step: no batched path for this model shape%s");
     if (h->ring_pages > 0 && n > ring_batch(h, TREE_MAX))

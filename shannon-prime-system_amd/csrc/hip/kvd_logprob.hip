@@ -25,6 +25,7 @@
 // ranking's latency, once for each workgroup.
 #include "kvd_op.h"
 #include "kvd_vec.h"
+#include <algorithm>
 
 namespace kvd {
 
@@ -281,14 +282,15 @@ __global__ __launch_bounds__(LP_THREADS) void k_lp_merge(sp_hipkv_logprob_args a
 
 // Segments of 2048 logits where that is what it takes to use the device, else of 8192
 // (one row of 151936: 75 workgroups for 19).
-struct LpPlan { int per, segs; };
+struct LpPlan { int per, segs; int64_t parts; };       // parts: room for this many rows or fewer
 LpPlan lp_plan(const sp_hipkv_logprob_args &a) {
     const int longs = (a.vocab + LP_LONG * LP_THREADS - 1) / (LP_LONG * LP_THREADS);
     const int shorts = (a.vocab + LP_SHORT * LP_THREADS - 1) / (LP_SHORT * LP_THREADS);
-    if (shorts <= LP_SEGS && (int64_t)a.n_rows * longs < 512) return {LP_SHORT, shorts};
-    return {LP_LONG, longs};
+    const int64_t few = shorts <= LP_SEGS ? std::min(a.n_rows, 511 / longs) * (int64_t)shorts : 0, many = (int64_t)a.n_rows * longs;
+    if (shorts <= LP_SEGS && many < 512) return {LP_SHORT, shorts, few};
+    return {LP_LONG, longs, std::max(few, many)};
 }
-size_t lp_part_bytes(const sp_hipkv_logprob_args &a, const LpPlan &p) { return (size_t)a.n_rows * p.segs * sizeof(LpPart); }
+size_t lp_part_bytes(const LpPlan &p) { return (size_t)p.parts * sizeof(LpPart); }
 
 int logprob_check(const char *who, const sp_hipkv_logprob_args *a) {
     OP_NEED(a, "null arguments");
@@ -312,7 +314,7 @@ int logprob_check_arrays(const char *who, const sp_hipkv_logprob_args *a, size_t
 void launch_logprob(const sp_hipkv_logprob_args &a, hipStream_t s) {
     const LpPlan p = lp_plan(a);
     LpPart *part = (LpPart *)a.work;
-    uint64_t *keys = (uint64_t *)((uint8_t *)a.work + lp_part_bytes(a, p));
+    uint64_t *keys = (uint64_t *)((uint8_t *)a.work + lp_part_bytes(p));
     const dim3 grid(p.segs, a.n_rows), wg(LP_THREADS);
     if (p.per == LP_LONG) hipLaunchKernelGGL(k_lp_part<LP_LONG>, grid, wg, 0, s, a, part, keys);
     else hipLaunchKernelGGL(k_lp_part<LP_SHORT>, grid, wg, 0, s, a, part, keys);
@@ -327,7 +329,7 @@ extern "C" int sp_hipkv_token_logprobs_work(const sp_hipkv_logprob_args *a, size
     if (logprob_check(who, a)) return 1;
     OP_NEED(bytes, "null bytes");
     const LpPlan p = lp_plan(*a);
-    *bytes = lp_part_bytes(*a, p) + (size_t)a->n_rows * p.segs * a->n_top * sizeof(uint64_t);
+    *bytes = lp_part_bytes(p) + (size_t)p.parts * a->n_top * sizeof(uint64_t);
     return 0;
 }
 

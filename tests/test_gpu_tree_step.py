@@ -314,6 +314,29 @@ def test_score_equals_decode_steps(tmpdir_models, shape, exact):
     b.close(); one.close(); r.close()
 
 
+def test_score_takes_any_number_of_tokens_in_any_order(tmpdir_models):
+    """A vocabulary where 127 rows take more work than 128 do: long, short and long
+    calls on one handle, and a handle beside it."""
+    r, beside = Rig(tmpdir_models, "qwen3-tiny", vocab=32768), Rig(tmpdir_models, "qwen3-tiny", vocab=32768)
+    g = np.random.default_rng(41)
+    toks = g.integers(0, r.V, 255).astype(np.int32)
+    h, other = r.backend(True), beside.backend(True)
+    other.prefill(toks[:40])
+    want, again = np.zeros(r.V, np.float32), np.zeros(r.V, np.float32)
+    other.decode(int(toks[40]), want)
+    other.rewind(1)
+    parts = [h.score(toks[a:b], given=toks[a + 1:b + 1], n_top=32) for a, b in ((0, 128), (128, 254))]
+    h.rewind(254)
+    pieces = [h.score(toks[a:b], given=toks[a + 1:b + 1], n_top=32) for a, b in ((0, 1), (1, 128), (128, 190), (190, 254))]
+    for k in range(4):
+        x, y = (np.concatenate([p[k] for p in q]) for q in (parts, pieces))
+        # the same logits, the operator's sums in another order: 1e-5 each (its own tests)
+        assert np.array_equal(x, y) if x.dtype == np.int32 else np.abs(x - y).max() <= 2e-5
+    other.decode(int(toks[40]), again)
+    assert same_bits(again, want)
+    h.close(); other.close(); r.close(); beside.close()
+
+
 def test_speculative_decoding_gives_the_greedy_tokens(tmpdir_models):
     """Exact mode: drafts from a table of what followed a token before, verified as
     a tree with wrong guesses beside them; the tokens are the greedy loop's."""

@@ -43,6 +43,15 @@ def test_tree_work_is_required():
     assert spkv.kv().sp_hipkv_tree_attention_work(ctypes.byref(tree()), None) != 0
 
 
+@pytest.mark.parametrize("vocab", [1, 2048, 2049, 8192, 20000, 32768, 100000, 151936, 262144, 262145, 1 << 20])
+def test_logprob_work_of_a_call_is_enough_for_a_smaller_one(vocab):
+    for top in (0, 1, min(vocab, 32)):
+        need = [spkv.token_logprobs_work(logprob(n_rows=r, vocab=vocab, stride=vocab, n_top=top)) for r in range(1, 600)]
+        assert need == sorted(need)
+    assert spkv.token_logprobs_work(logprob(n_rows=7, vocab=vocab, stride=vocab, n_top=0)) <= \
+        spkv.token_logprobs_work(logprob(n_rows=7, vocab=vocab, stride=vocab, n_top=1))
+
+
 def test_nothing_to_do_touches_no_device():
     spkv.tree_attention(tree(n_nodes=0, q=None))
     spkv.tree_attention(tree(n_nodes=0, n_seqs=0))
