@@ -104,7 +104,9 @@ constexpr int tree_waves(int rows) { return rows == SP_HIPKV_ROWS_SPINOR ? 4 : 8
 __device__ __forceinline__ bool finite1(float x) { return (__float_as_uint(x) & 0x7F800000u) != 0x7F800000u; }
 
 // Of an f32 its three bf16 pieces, which sum to it exactly: x = h + m + l, |m| <= 2^-9 |x|,
-// |l| <= 2^-18 |x| (magnitudes from 2^127 on round up to infinity and make NaN).
+// |l| <= 2^-18 |x| (magnitudes from 2^127 on round up to infinity and make NaN; below 2^-110 l
+// is lost to denormals bit by bit).  Cutting bits off instead of rounding saves 4% of a call, and
+// 2^-21 of a product would be missing for 2^-26.
 typedef __bf16 bf8 __attribute__((ext_vector_type(8)));
 typedef __bf16 bf2 __attribute__((ext_vector_type(2)));
 typedef float v2f __attribute__((ext_vector_type(2)));
