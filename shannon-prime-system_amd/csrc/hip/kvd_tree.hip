@@ -84,7 +84,7 @@ __device__ __forceinline__ const uint8_t *uniform(const uint8_t *x) {
 // position) joins outside the product: on the scores of the chunk's dims, and on the weights
 // before they are taken apart.  Dims and columns are therefore dealt to steps and tiles by
 // chunk, as windows of 64 dims of which 51 (43, 32) count.  16 nodes at 6k of 16 heads (8 kv
-// heads of 256 dims) take 26.5 us; as f32 products of codes times multipliers, which was the first form,
+// heads of 256 dims) take 25.9 us; as f32 products of codes times multipliers, which was the first form,
 // 36.5, and 30 nodes of 32 heads at 12k 50 for 82 us.  The codes' conversion bounds it now, 1.5
 // instructions a code, and below 20 us what is fixed.
 //
@@ -203,8 +203,10 @@ __global__ __launch_bounds__(64 * tree_waves(ROWS), 2) void k_tree_float(sp_hipk
         Pieces p;
         if constexpr (SPN) {                                               // zeros beside the chunk's dims
             const int b = c / (WIN / 8), d0 = 4 * spn_window(HD, b, WIN) + 8 * (c % (WIN / 8));
-            const float *x = row_q(r);
-            p = pieces_of([&](int k) { return d0 + k < HD && spn_block_of(HD, d0 + k) == b ? x[d0 + k] : 0.0f; });
+            const int lo = spn_block_start(HD, b) - d0, hi = spn_block_start(HD, b + 1) - d0;
+            const float *x = row_q(r) + d0;
+            const v4f zero = {0, 0, 0, 0}, y0 = d0 < HD ? *(const v4f *)x : zero, y1 = d0 + 4 < HD ? *(const v4f *)(x + 4) : zero;
+            p = pieces_of([&](int k) { return k >= lo && k < hi ? (k < 4 ? y0[k & 3] : y1[k & 3]) : 0.0f; });
         } else {
             const v4f x = *(const v4f *)(row_q(r) + 8 * c), y = *(const v4f *)(row_q(r) + 8 * c + 4);
             p = pieces_of([&](int k) { return k < 4 ? x[k] : y[k - 4]; });
