@@ -92,8 +92,8 @@ __device__ __forceinline__ const uint8_t *uniform(const uint8_t *x) {
 // 2): weights stay below 2^8 and nothing is lost, and a tile needs one ballot instead of
 // a reduction over lanes.  The sums are joined over lanes once at the end.
 //
-// A position that a row does not see has weight 0, which a V row that is not finite
-// would turn into NaN: tiles that some row does not see whole look for such values
+// A position that a row does not see has weight 0, which a V value whose pieces are not
+// finite would turn into NaN: tiles that some row does not see whole look for such values
 // first and are then put off to a loop behind the main one, which adds positions one
 // by one (inside the main loop that path costs twice the output's registers).
 typedef float v4f __attribute__((ext_vector_type(4)));
@@ -102,10 +102,14 @@ constexpr int TREE_PAGES = 256;              // pages of a split at most
 constexpr int tree_waves(int rows) { return rows == SP_HIPKV_ROWS_SPINOR ? 4 : 8; }
 
 __device__ __forceinline__ bool finite1(float x) { return (__float_as_uint(x) & 0x7F800000u) != 0x7F800000u; }
+// whether bf16 pieces hold x: not infinities, NaN, nor the magnitudes above the midpoint of the
+// largest bf16 number and the next power of two, which round up to an infinite first piece
+constexpr uint32_t PIECES_END = 0x7F7F8000u;
+__device__ __forceinline__ bool pieces_hold(float x) { return (__float_as_uint(x) & 0x7FFFFFFFu) < PIECES_END; }
 
 // Of an f32 its three bf16 pieces, which sum to it exactly: x = h + m + l, |m| <= 2^-9 |x|,
-// |l| <= 2^-18 |x| (magnitudes from 2^127 on round up to infinity and make NaN; below 2^-110 l
-// is lost to denormals bit by bit).  Cutting bits off instead of rounding saves 4% of a call, and
+// |l| <= 2^-18 |x| (magnitudes from PIECES_END on round up to infinity and make NaN, with a weight of 0
+// too; below 2^-110 l is lost to denormals bit by bit).  Cutting bits off instead of rounding saves 4% of a call, and
 // 2^-21 of a product would be missing for 2^-26.
 typedef __bf16 bf8 __attribute__((ext_vector_type(8)));
 typedef __bf16 bf2 __attribute__((ext_vector_type(2)));
@@ -226,8 +230,8 @@ __global__ __launch_bounds__(64 * tree_waves(ROWS), 2) void k_tree_float(sp_hipk
     const uint32_t kslice = (uint32_t)h * PAGE * RB, vslice = (uint32_t)(a.n_kv_heads + h) * PAGE * RB;
     // page addresses are the wave's: rows load as address + 32-bit lane offset
     auto page_at = [&](int tile) { return uniform(s_page[tile / (PAGE / TP) - b0]); };
-    // tiles that some row does not see whole, and those of them with a V value that is
-    // not finite: nodes span at most 10 pages, so do the rows' window starts
+    // tiles that some row does not see whole, and those of them with a V value that
+    // pieces do not hold: nodes span at most 10 pages, so do the rows' window starts
     auto ragged = [&](int tile) { return tile * TP < lo_max || tile * TP + TP > q.cached; };
     const int tail = q.cached / TP, head = lo_min / TP;
     uint64_t later = 0;
@@ -283,7 +287,7 @@ __global__ __launch_bounds__(64 * tree_waves(ROWS), 2) void k_tree_float(sp_hipk
                 for (int i = 0; i < 4; i++) { S[t][u][i] = __builtin_amdgcn_exp2f(S[t][u][i] - ms); l[t] += S[t][u][i]; }
         }
     };
-    // V values that are not finite, for the rows that see them; x4(page, row offset, k): columns 4 k .. of this lane
+    // V values that pieces do not hold, as infinities and NaN for the rows that see them; x4(page, row offset, k): columns 4 k .. of this lane
     auto add_later = [&](auto &&x4) {
         while (later) {
             const int b = __builtin_ctzll(later), tile = b < 32 ? tail + b : head + b - 32;
@@ -304,7 +308,7 @@ __global__ __launch_bounds__(64 * tree_waves(ROWS), 2) void k_tree_float(sp_hipk
                         #pragma unroll
                         for (int c = 0; c < 4; c++)
                             #pragma unroll
-                            for (int i = 0; i < 4; i++) O[t][4 * k + c][i] += on[i] && !finite1(v[c]) ? v[c] : 0.0f;
+                            for (int i = 0; i < 4; i++) O[t][4 * k + c][i] += on[i] && !pieces_hold(v[c]) ? v[c] * INFINITY : 0.0f;
                         __builtin_amdgcn_sched_barrier(0);
                     }
                 }
@@ -407,15 +411,15 @@ __global__ __launch_bounds__(64 * tree_waves(ROWS), 2) void k_tree_float(sp_hipk
             Pieces P[RT];
             #pragma unroll
             for (int t = 0; t < RT; t++) P[t] = pieces_of([&](int k) { return S[t][k >> 2][k & 3]; });
-            uint32_t bad = 0;                                              // largest exponent field of a row before the end
+            uint32_t bad = 0;                                              // largest magnitude of a row before the end
             #pragma unroll
             for (int n = NK; n < NU; n++) {
                 if (rag) {
                     #pragma unroll
                     for (int k = 0; k < 16; k++) {
-                        const uint32_t f = __float_as_uint(x[k]) & 0x7F800000u;
+                        const uint32_t f = __float_as_uint(x[k]) & 0x7FFFFFFFu;
                         bad = max(bad, tile * TP + 16 * (k >> 3) + 4 * g + (k >> 1 & 3) < end ? f : 0u);
-                        x[k] = f == 0x7F800000u ? 0.0f : x[k];
+                        x[k] = f >= PIECES_END ? 0.0f : x[k];
                         if (k % 4 == 3) __builtin_amdgcn_sched_barrier(0);
                     }
                 }
@@ -432,7 +436,7 @@ __global__ __launch_bounds__(64 * tree_waves(ROWS), 2) void k_tree_float(sp_hipk
                     if (t == 0) { arrive(); read(n + 1 < NU ? n + 1 : 0); }
                 }
             }
-            if (__any(bad == 0x7F800000u)) put_off(tile);
+            if (__any(bad >= PIECES_END)) put_off(tile);
             pg = pn;
         }
         asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" : : : "memory");                 // nothing lands in LDS after this

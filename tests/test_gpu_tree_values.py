@@ -1,0 +1,125 @@
+"""Tree attention of rows that hold extreme values: what a node does not see never
+reaches it, what it sees and is not finite always does.  Tolerances: tree_ref."""
+import numpy as np
+import pytest
+
+import tree_ref
+from helpers import prompt
+from test_gpu_tree_ops import EXACT, F32, SPINOR, Tree
+from test_gpu_tree_step import Rig, close, path, tree
+
+pytestmark = pytest.mark.gpu
+
+
+def f32(bits):
+    return np.array([bits], np.uint32).view(np.float32)[0]
+
+
+# 0x7F7F8000 is the least magnitude that rounds to an infinite bf16, 0x7F7F7FFF the largest that does not
+HUGE = [0x7F7FFFFF, 0xFF7FFFFF, 0x7F7F8000, 0xFF7F8000, 0x7F7F7FFF, 0xFF7F7FFF, 0x7F800000, 0xFF800000, 0x7FC00000, 0x7F800001]
+
+
+def fill_unused(t, value):
+    """Places of the pool that no position maps to (Cache marks them with NaN)."""
+    if t.cache.rows == SPINOR:
+        chunk, nb, rb = tree_ref.spinor_chunks(t.hd)
+        mul = np.ascontiguousarray(t.cache.pool[..., t.hd:t.hd + 4 * nb]).view(np.float32)
+        mul[np.isnan(mul)] = value
+        t.cache.pool[..., t.hd:t.hd + 4 * nb] = mul.view(np.uint8)
+    elif t.cache.rows == F32:
+        t.cache.pool[np.isnan(t.cache.pool)] = value
+    else:
+        t.cache.pool[t.cache.pool == 0x7FFFFF] = value
+
+
+def hidden(rows, hd, value, cached=300, nodes=40, window=64):
+    """A tree whose hidden positions and unused places all hold a value: below every
+    window, and a last node that only it sees itself."""
+    t = Tree(rows, hd, 2, [cached], [nodes], window=window, seed=31)
+    with np.errstate(all="ignore"):
+        fill_unused(t, value)
+        for p in range(cached - window - 20 if window else 0):
+            t.cache.set(0, p, value)
+        t.cache.set(0, cached + nodes - 1, value)
+    assert all(nodes - 1 not in see for see in t.trees[0][0][:-1])
+    return t.ready()
+
+
+def same_but_the_last(t):
+    with np.errstate(all="ignore"):
+        got, (want, tol) = t.run(), t.want()
+    n = len(got) - 1
+    assert np.isfinite(got[:n]).all()
+    assert (np.abs(got[:n] - want[:n]) <= tol[:n]).all()
+    return got
+
+
+@pytest.mark.parametrize("hd", [64, 128, 256])
+@pytest.mark.parametrize("rows", [F32, SPINOR])
+def test_unseen_values_of_any_size(rows, hd):
+    """Largest numbers beside infinities and NaN, with a window and without."""
+    for bits in HUGE:
+        same_but_the_last(hidden(rows, hd, f32(bits)))
+    same_but_the_last(hidden(rows, hd, f32(0x7F7FFFFF), cached=2900, nodes=9, window=0))
+
+
+@pytest.mark.parametrize("hd", [64, 128, 256])
+def test_unseen_values_of_exact_rows(hd):
+    """... and the largest integers: the bits of a cache without them."""
+    clean = hidden(EXACT, hd, 0).run()
+    for value in (0x7FFFFFFF, -0x80000000, 0x7FFFFF, -1):
+        assert np.array_equal(hidden(EXACT, hd, value).run()[:-1].view(np.uint32), clean[:-1].view(np.uint32))
+
+
+def test_unseen_words_of_any_bits():
+    """Whatever memory held before: random words in every hidden and unused place."""
+    g = np.random.default_rng(5)
+    t = Tree(F32, 128, 2, [300], [40], window=64, seed=32)
+    bits = g.integers(0, 1 << 32, t.cache.pool.shape, np.uint64).astype(np.uint32)
+    some = g.random(bits.shape) < 0.5                     # half of them among the values that round up to infinity
+    bits[some] = 0x7F7F8000 | (bits[some] & 0x80007FFF)
+    unused = np.isnan(t.cache.pool)
+    t.cache.pool.view(np.uint32)[unused] = bits[unused]
+    for p in list(range(200)) + [339]:
+        a, b = t.cache._at(0, p)
+        t.cache.pool.view(np.uint32)[a, :, :, b] = bits[a, :, :, b]
+    same_but_the_last(t.ready())
+
+
+def test_seen_values_that_pieces_do_not_hold():
+    """The header counts magnitudes from 2^127 on as not finite: a node that sees one is
+    without a finite value in its column, in whole tiles and in others."""
+    for p in (5, 200, 339):
+        t = Tree(F32, 128, 2, [300], [40], kind="chain", seed=33)
+        a, b = t.cache._at(0, p)
+        t.cache.pool[a, 1, :, b, 17] = f32(0x7F7F9000)
+        t.ready()
+        got, (want, tol) = t.run(), t.want()
+        hit = np.arange(40) >= p - 300
+        assert not np.isfinite(got[hit][..., 17]).any()
+        got[hit, :, 17], want[hit, :, 17] = 0, 0
+        assert (np.abs(got - want) <= tol).all()
+
+
+@pytest.mark.parametrize("shape", ["qwen3-tiny", "qwen3-hd128", "gemma3-hd256"])
+def test_steps_over_pages_that_held_large_values(tmpdir_models, shape):
+    """A handle's pages keep what was written and rewound: decode steps, which read no
+    unused place, say what a tree step gives on them."""
+    r = Rig(tmpdir_models, shape)
+    b = r.backend(False)
+    big = np.full((128, r.kvd), f32(0x7F7F8000), np.float32)
+    big[::2] = f32(0xFF7FFFFF)
+    for l in range(r.d["n_layers"]):
+        b.write_kv(l, 0, big, big)
+    assert b.rewind(128) == 0
+    b.prefill(prompt(37, r.V, seed=3))
+    parents, toks = tree(9, 4), prompt(9, r.V, seed=8)
+    lg, nxt, _ = b.tree_step(toks, parents, r.V)
+    ref = np.zeros(r.V, np.float32)
+    for leaf in [i for i in range(9) if i not in parents]:
+        f = b.fork()
+        for i in path(parents, leaf):
+            f.decode(int(toks[i]), ref)
+            assert close(lg[i], ref), i
+        f.close()
+    b.close(); r.close()
