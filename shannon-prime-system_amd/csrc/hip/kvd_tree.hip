@@ -606,7 +606,7 @@ __global__ __launch_bounds__(64 * tree_waves(ROWS), 2) void k_tree_float(sp_hipk
     for (int t = 0; t < RT; t++) {
         #pragma unroll
         for (int i = 0; i < 4; i++) {
-            const float f = s_m[wave][t * 16 + 4 * g + i];
+            const float f = s_m[wave][t * 16 + 4 * g + i];                 // 0 times NaN is NaN: what a row sees reaches it
             float *dst = (float *)lds + (wave * 16 + 4 * g + i) * HD;
             if constexpr (SPN) {                                           // tile 4 b + c: columns 4 (window + lane) + c of chunk b
                 #pragma unroll
@@ -614,13 +614,13 @@ __global__ __launch_bounds__(64 * tree_waves(ROWS), 2) void k_tree_float(sp_hipk
                     const int d0 = 4 * (spn_window(HD, b, 64) + l16);
                     #pragma unroll
                     for (int c = 0; c < 4; c++)
-                        if (d0 + c >= spn_block_start(HD, b) && d0 + c < spn_block_start(HD, b + 1)) dst[d0 + c] = f == 0.0f ? 0.0f : O[t][4 * b + c][i] * f;
+                        if (d0 + c >= spn_block_start(HD, b) && d0 + c < spn_block_start(HD, b + 1)) dst[d0 + c] = O[t][4 * b + c][i] * f;
                 }
             } else {
                 #pragma unroll
                 for (int c = 0; c < CPR; c += 2) {
                     const v2f x = {O[t][c][i], O[t][c + 1][i]};
-                    ((v2f *)dst)[8 * c + l16] = f == 0.0f ? (v2f){0, 0} : x * f;
+                    ((v2f *)dst)[8 * c + l16] = x * f;
                 }
             }
         }
@@ -659,8 +659,9 @@ __global__ __launch_bounds__(256) void k_tree_merge(sp_hipkv_tree_args a, int ns
     if (threadIdx.x < 64) {
         const bool in = (int)threadIdx.x < nsplit;
         const float m = in ? ml[2 * threadIdx.x] : -INFINITY, l = in ? ml[2 * threadIdx.x + 1] : 0.0f, M = wave_allmax(m);
-        const float f = m > -INFINITY ? __builtin_amdgcn_exp2f(m - M) : 0.0f;        // 0: a part without a position of this row
-        s_f[threadIdx.x] = f;
+        const bool none = m == -INFINITY;                                 // a part without a position of this row, or without a score
+        const float f = none ? 0.0f : __builtin_amdgcn_exp2f(m - M);
+        s_f[threadIdx.x] = none ? -1.0f : f;
         const float L = wave_allsum(f * l);                               // NaN scores: l is NaN also where m is -inf
         if (threadIdx.x == 0) s_L = L;
     }
@@ -671,7 +672,7 @@ __global__ __launch_bounds__(256) void k_tree_merge(sp_hipkv_tree_args a, int ns
     for (int k = grp; k < nsplit; k += NG) {
         const v4f v = po[(size_t)k * (HD / 4)];
         const float f = s_f[k];
-        x += f == 0.0f ? (v4f){0, 0, 0, 0} : f * v;
+        x += f < 0.0f ? (v4f){0, 0, 0, 0} : f * v;                        // ... whose output was not written
     }
     s_x[threadIdx.x] = x;
     __syncthreads();

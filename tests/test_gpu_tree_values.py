@@ -123,3 +123,54 @@ def test_steps_over_pages_that_held_large_values(tmpdir_models, shape):
             assert close(lg[i], ref), i
         f.close()
     b.close(); r.close()
+
+
+def lifted(rows, cached, nodes, p0, hd=128):
+    """Position p0 scores far above all others, 2^-300 or less of whose weight is left."""
+    t = Tree(rows, hd, 2, [cached], [nodes], kind="chain", seed=34)
+    t.q[:] = 1.0
+    t.dq.put(t.q)
+    a, b = t.cache._at(0, p0)
+    k = np.float32(600 * np.sqrt(hd) / hd * np.log(2))
+    if rows == F32:
+        t.cache.pool[a, 0, :, b] = k
+    else:
+        chunk, nb, rb = tree_ref.spinor_chunks(hd)
+        t.cache.pool[a, 0, :, b, :hd] = 100
+        t.cache.pool[a, 0, :, b, hd:hd + 4 * nb] = np.full(nb, k / 100, np.float32).view(np.uint8)
+    return t
+
+
+def spoil(t, p, kv, value, column=0):
+    """One V (1) or K (0) column of position p, of Spinor rows its chunk; the columns hit."""
+    a, b = t.cache._at(0, p)
+    if t.cache.rows == F32:
+        t.cache.pool[a, kv, :, b, column] = value
+        return np.arange(t.hd) == column
+    chunk, nb, rb = tree_ref.spinor_chunks(t.hd)
+    at = t.hd + 4 * chunk[column]
+    t.cache.pool[a, kv, :, b, at:at + 4] = np.array([value], np.float32).view(np.uint8)
+    return chunk == chunk[column]
+
+
+@pytest.mark.parametrize("value", [np.nan, np.inf, -np.inf])
+@pytest.mark.parametrize("rows", [F32, SPINOR])
+@pytest.mark.parametrize("cached,p0,p1", [(300, 10, 12), (300, 10, 40), (300, 200, 5), (300, 10, 299), (300, 10, 302), (300, 302, 33), (5000, 100, 4000),
+                                          (5000, 4000, 100), (5000, 100, 5001), (5000, 5000, 100)])
+def test_seen_values_of_no_weight(rows, cached, p0, p1, value):
+    """0 times NaN or infinity is NaN also where the weight is 0 by rounding: a V value that is
+    seen spoils its column, in whatever tile, wave or part it lies beside the largest score."""
+    t = lifted(rows, cached, 6, p0)
+    hit = spoil(t, p1, 1, value, 70)
+    t.ready()
+    with np.errstate(all="ignore"):
+        got, (want, tol) = t.run(), t.want()
+    # node j sees the nodes up to itself; before the lifted one is seen the others share the weight
+    sees = np.arange(6) >= p1 - cached
+    assert not np.isfinite(got[sees][..., hit]).any()
+    spoiled = sees[:, None, None] & hit
+    got, want, tol = (np.where(spoiled, 0, x) for x in (got, want, tol))
+    # the bounds are relative to sum p |v|; beside them a weight (at most 1 after its part's factor) below the
+    # least normal number may be 0: (cached + 6) 2^-126 |v|, where nothing of weight has a value but 0
+    v = 6.0 if rows == F32 else 127 * 0.03
+    assert (np.abs(got - want) <= tol + (cached + 6) * 2.0 ** -126 * v).all()
