@@ -505,6 +505,9 @@ __global__ __launch_bounds__(64 * tree_waves(ROWS), 2) void k_tree_float(sp_hipk
             const bool rag = ragged(tile);
             pn = page_at(nx);
             zero_s();
+            // infinities become NaN: scores of -infinity would count as positions that nobody sees
+            #pragma unroll
+            for (int i = 0; i < 4; i++) km[i] = fmaf(km[i], 0.0f, km[i]);
             put_mul(0, km);
             #pragma unroll
             for (int b = 0; b < NB; b++) {

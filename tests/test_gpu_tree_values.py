@@ -174,3 +174,20 @@ def test_seen_values_of_no_weight(rows, cached, p0, p1, value):
     # least normal number may be 0: (cached + 6) 2^-126 |v|, where nothing of weight has a value but 0
     v = 6.0 if rows == F32 else 127 * 0.03
     assert (np.abs(got - want) <= tol + (cached + 6) * 2.0 ** -126 * v).all()
+
+
+@pytest.mark.parametrize("value", [np.nan, np.inf, -np.inf])
+@pytest.mark.parametrize("rows", [F32, SPINOR])
+@pytest.mark.parametrize("hd", [64, 128, 256])
+def test_seen_k_values_that_are_not_finite(rows, hd, value):
+    """In K alone, one column or chunk: no finite value for the nodes that see it, whatever
+    the signs of its products sum up to; the others as without it."""
+    for cached, p in ((300, 12), (300, 298), (300, 303), (5000, 3000), (5000, 5004)):
+        t = Tree(rows, hd, 4, [cached], [6], kind="chain", seed=35)
+        spoil(t, p, 0, value, hd - 1)
+        t.ready()
+        with np.errstate(all="ignore"):
+            got, (want, tol) = t.run(), t.want()
+        sees = np.arange(6) >= p - cached
+        assert not np.isfinite(got[sees]).any(), (cached, p)
+        assert (np.abs(got[~sees] - want[~sees]) <= tol[~sees]).all()
