@@ -1277,7 +1277,7 @@ int run_batch(sp_kvdecode_handle *h, int T, int pos0, int pos_hi, BatchKind kind
                 HIPCHK(dev_malloc(&b.tbuf, need), "tree work alloc");
                 b.tbytes = need;
             }
-            tree_attention(h, a, l);
+            if (tree_attention(h, a, l)) return 1;
         } else if (prefill_attention_float(a)) launch_prefill_float(a, s);
         else for (int t = 0; t < T; t += b.TB) {                // one pass for a batched decode
             AttnArgs c = a;
@@ -1353,7 +1353,7 @@ int tree_attention(sp_kvdecode_handle *h, const AttnArgs &a, int layer, size_t *
     t.q = a.qr; t.out = a.ao; t.q_stride = t.out_stride = (int64_t)a.NH * a.HD;
     t.work = h->b.tbuf;
     if (need) return sp_hipkv_tree_attention_work(&t, need);
-    launch_tree(t, s);
+    HIPCHK(launch_tree(t, s), "tree attention launch");
     return 0;
 }
 
@@ -1816,8 +1816,7 @@ int sp_hipkv_tree_step(sp_kvdecode_handle *h, const int32_t *tokens, const int32
         std::fill(hs->given, hs->given + n * most, -1);
         for (int i = 0; i < n; i++) if (parents[i] >= 0) hs->given[parents[i] * most + nth[i]] = tokens[i];
         HIPCHK(hipMemcpyAsync(d->given, hs->given, (size_t)n * most * 4, hipMemcpyHostToDevice, s), "tree upload");
-        launch_logprob(a, s);
-        HIPCHK(hipGetLastError(), "sp_hipkv_tree_step: launch");
+        HIPCHK(launch_logprob(a, s), "sp_hipkv_tree_step: launch");
         HIPCHK(hipMemcpyAsync(hs->lp, d->lp, (size_t)n * most * 4, hipMemcpyDeviceToHost, s), "log probability download");
     }
     if (next_tokens) HIPCHK(hipMemcpyAsync(b.hnext, b.next, (size_t)n * 4, hipMemcpyDeviceToHost, s), "tree tokens download");
@@ -1858,8 +1857,7 @@ int sp_hipkv_tree_keep(sp_kvdecode_handle *h, const int32_t *nodes, int n) {
         a.max_keep = n; a.max_positions = h->dpos + pending;
         a.tables = (const void *const *const *)h->d_lists; a.ring_pages = h->d_rings;
         a.cached = &h->d_tree->cached; a.keep_start = h->d_tree->keep_start; a.keep = h->d_tree->keep;
-        launch_keep(a, h->stream);
-        HIPCHK(hipGetLastError(), "sp_hipkv_tree_keep: launch");
+        HIPCHK(launch_keep(a, h->stream), "sp_hipkv_tree_keep: launch");
         HIPCHK(hipStreamSynchronize(h->stream), "tree keep");
     }
     h->tree_n = 0;
@@ -1895,8 +1893,7 @@ int sp_hipkv_score(sp_kvdecode_handle *h, const int32_t *tokens, const int32_t *
         for (int t = 0; t < T; t++) hs->given[t] = given ? given[i + t] : i + t + 1 < n ? tokens[i + t + 1] : -1;
         HIPCHK(hipMemcpyAsync(d->given, hs->given, (size_t)T * 4, hipMemcpyHostToDevice, s), "score tokens");
         if (run_batch(h, T, h->dpos + i, h->dpos + i + T - 1, SCORE)) return 1;
-        launch_logprob(a, s);
-        HIPCHK(hipGetLastError(), "sp_hipkv_score: launch");
+        HIPCHK(launch_logprob(a, s), "sp_hipkv_score: launch");
         HIPCHK(hipMemcpyAsync(hs->lp, d->lp, sizeof(Score) - offsetof(Score, lp), hipMemcpyDeviceToHost, s), "score download");
         HIPCHK(hipStreamSynchronize(s), "score");
         if (logprob) memcpy(logprob + i, hs->lp, (size_t)T * 4);

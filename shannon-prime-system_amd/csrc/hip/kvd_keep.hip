@@ -71,10 +71,10 @@ int keep_check(const sp_hipkv_keep_args *a) {
 
 }  // namespace
 
-void launch_keep(const sp_hipkv_keep_args &a, hipStream_t s) {
+hipError_t launch_keep(const sp_hipkv_keep_args &a, hipStream_t s) {
     const int64_t threads = (int64_t)(a.row_bytes / 16) * 2 * a.n_kv_heads;
     const dim3 grid((uint32_t)((threads + 255) / 256), 1, a.n_tables < 65535 ? a.n_tables : 65535);
-    hipLaunchKernelGGL(k_keep, grid, dim3(256), 0, s, a);
+    return op_launch(k_keep, grid, dim3(256), s, a);
 }
 
 }  // namespace kvd
@@ -84,6 +84,5 @@ extern "C" int sp_hipkv_keep_rows(const sp_hipkv_keep_args *a, void *stream) {
     if (keep_check(a)) return 1;
     if (!a->n_tables || !a->max_keep) return 0;
     OpDevice dev((hipStream_t)stream);
-    if (dev.err == hipSuccess) launch_keep(*a, (hipStream_t)stream);
-    return op_done("sp_hipkv_keep_rows", dev);
+    return op_done("sp_hipkv_keep_rows", dev.err != hipSuccess ? dev.err : launch_keep(*a, (hipStream_t)stream));
 }

@@ -311,14 +311,13 @@ int logprob_check_arrays(const char *who, const sp_hipkv_logprob_args *a, size_t
 
 }  // namespace
 
-void launch_logprob(const sp_hipkv_logprob_args &a, hipStream_t s) {
+hipError_t launch_logprob(const sp_hipkv_logprob_args &a, hipStream_t s) {
     const LpPlan p = lp_plan(a);
     LpPart *part = (LpPart *)a.work;
     uint64_t *keys = (uint64_t *)((uint8_t *)a.work + lp_part_bytes(p));
     const dim3 grid(p.segs, a.n_rows), wg(LP_THREADS);
-    if (p.per == LP_LONG) hipLaunchKernelGGL(k_lp_part<LP_LONG>, grid, wg, 0, s, a, part, keys);
-    else hipLaunchKernelGGL(k_lp_part<LP_SHORT>, grid, wg, 0, s, a, part, keys);
-    hipLaunchKernelGGL(k_lp_merge, dim3(a.n_rows), wg, 0, s, a, p.segs, part, keys);
+    const hipError_t e = op_launch(p.per == LP_LONG ? k_lp_part<LP_LONG> : k_lp_part<LP_SHORT>, grid, wg, s, a, part, keys);
+    return e != hipSuccess ? e : op_launch(k_lp_merge, dim3(a.n_rows), wg, s, a, p.segs, part, keys);
 }
 
 }  // namespace kvd
@@ -341,6 +340,5 @@ extern "C" int sp_hipkv_token_logprobs(const sp_hipkv_logprob_args *a, void *str
     size_t need = 0;
     if (sp_hipkv_token_logprobs_work(a, &need) || logprob_check_arrays(who, a, need)) return 1;
     OpDevice dev((hipStream_t)stream);
-    if (dev.err == hipSuccess) launch_logprob(*a, (hipStream_t)stream);
-    return op_done(who, dev);
+    return op_done(who, dev.err != hipSuccess ? dev.err : launch_logprob(*a, (hipStream_t)stream));
 }

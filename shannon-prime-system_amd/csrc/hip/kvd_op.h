@@ -37,16 +37,27 @@ public:
     ~OpDevice() { if (moved) hipSetDevice(was); }
 };
 
-// The end of a call: its launches' error, if any.
-inline int op_done(const char *who, const OpDevice &d) {
-    const hipError_t e = d.err != hipSuccess ? d.err : hipGetLastError();
-    return e == hipSuccess ? 0 : op_fail(who, hipGetErrorString(e));
+// One launch and its own error: hipGetLastError would give, and take, an error that an
+// earlier call of the same thread left.
+template <typename T> struct op_param { typedef T type; };
+template <typename... P>
+hipError_t op_launch(void (*k)(P...), dim3 grid, dim3 wg, hipStream_t s, const typename op_param<P>::type &...p) {
+    void *args[] = {const_cast<void *>(static_cast<const void *>(&p))...};
+    return hipLaunchKernel(reinterpret_cast<const void *>(k), grid, wg, args, 0, s);
 }
 
-// The operators' launches, for arguments that their entry points accept.
-void launch_tree(const sp_hipkv_tree_args &a, hipStream_t s);
-void launch_logprob(const sp_hipkv_logprob_args &a, hipStream_t s);
-void launch_keep(const sp_hipkv_keep_args &a, hipStream_t s);
+// The end of a call, e its launches' error; an error of its own is reported here and not left behind.
+inline int op_done(const char *who, hipError_t e) {
+    if (e == hipSuccess) return 0;
+    (void)hipGetLastError();
+    return op_fail(who, hipGetErrorString(e));
+}
+
+// The operators' launches, for arguments that their entry points accept.  On an error
+// the launches behind it are left out.
+hipError_t launch_tree(const sp_hipkv_tree_args &a, hipStream_t s);
+hipError_t launch_logprob(const sp_hipkv_logprob_args &a, hipStream_t s);
+hipError_t launch_keep(const sp_hipkv_keep_args &a, hipStream_t s);
 
 __host__ __device__ constexpr int row_bytes_of(int rows, int hd) { return rows == SP_HIPKV_ROWS_SPINOR ? spn_row_bytes(hd) : 4 * hd; }
 

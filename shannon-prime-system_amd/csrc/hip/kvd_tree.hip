@@ -1287,21 +1287,20 @@ int tree_check_arrays(const char *who, const sp_hipkv_tree_args *a, size_t need)
 
 int64_t tree_grid(const sp_hipkv_tree_args &a, const TreePlan &p) { return (int64_t)a.n_kv_heads * p.groups * p.nsplit * a.n_seqs; }
 
-template <int ROWS> void tree_float(const sp_hipkv_tree_args &a, hipStream_t s) {
+template <int ROWS> hipError_t tree_float(const sp_hipkv_tree_args &a, hipStream_t s) {
     const TreePlan p = tree_plan(a);
     const dim3 grid((uint32_t)tree_grid(a, p)), wg(256);
-#define TREE_RUN(EPL, RT) hipLaunchKernelGGL((k_tree_float<ROWS, EPL, RT>), grid, dim3(64 * tree_waves(ROWS)), 0, s, a, p.groups, p.nsplit, p.pages)
+    hipError_t e = hipSuccess;
+#define TREE_RUN(EPL, RT) e = op_launch(k_tree_float<ROWS, EPL, RT>, grid, dim3(64 * tree_waves(ROWS)), s, a, p.groups, p.nsplit, p.pages)
     if (a.head_dim == 256) {
         if constexpr (ROWS == SP_HIPKV_ROWS_F32) { if (p.rt == 2) TREE_RUN(4, 2); else TREE_RUN(4, 1); }
         else TREE_RUN(4, 1);
     } else if (a.head_dim == 128) { if (p.rt == 1) TREE_RUN(2, 1); else if (p.rt == 2) TREE_RUN(2, 2); else if constexpr (ROWS == SP_HIPKV_ROWS_F32) TREE_RUN(2, 3); }
     else { if (p.rt == 1) TREE_RUN(1, 1); else if (p.rt == 2) TREE_RUN(1, 2); else if (p.rt == 3) TREE_RUN(1, 3); else if constexpr (ROWS == SP_HIPKV_ROWS_F32) TREE_RUN(1, 4); }
 #undef TREE_RUN
-    if (p.nsplit == 1) return;
+    if (e != hipSuccess || p.nsplit == 1) return e;
     const dim3 mg((uint32_t)((int64_t)a.n_nodes * a.n_heads));
-    if (a.head_dim == 256) hipLaunchKernelGGL(k_tree_merge<256>, mg, wg, 0, s, a, p.nsplit);
-    else if (a.head_dim == 128) hipLaunchKernelGGL(k_tree_merge<128>, mg, wg, 0, s, a, p.nsplit);
-    else hipLaunchKernelGGL(k_tree_merge<64>, mg, wg, 0, s, a, p.nsplit);
+    return op_launch(a.head_dim == 256 ? k_tree_merge<256> : a.head_dim == 128 ? k_tree_merge<128> : k_tree_merge<64>, mg, wg, s, a, p.nsplit);
 }
 
 // Exact rows: a workgroup's row tiles for the scores, whose q digits two workgroups' LDS
@@ -1331,31 +1330,31 @@ XPlan tree_xplan(const sp_hipkv_tree_args &a) {
     p.bytes = zb + mb + sb + up(rows * p.w.vsplit * 8);
     return p;
 }
-template <int EPL> void tree_xgo(const sp_hipkv_tree_args &a, const XPlan &p, hipStream_t s) {
+template <int EPL> hipError_t tree_xgo(const sp_hipkv_tree_args &a, const XPlan &p, hipStream_t s) {
     const int64_t base = (int64_t)a.n_kv_heads * a.n_seqs;
-#define TREE_SCORE(RT) hipLaunchKernelGGL((k_tree_xscore<EPL, RT>), dim3((uint32_t)(base * p.sgroups * p.w.nsplit)), dim3(256), 0, s, a, p.w, p.sgroups)
-#define TREE_SUM(RT) hipLaunchKernelGGL((k_tree_xsum<EPL, RT>), dim3((uint32_t)(base * p.groups * p.w.vsplit)), dim3(EPL * 128), 0, s, a, p.w, p.groups)
+    hipError_t e = hipSuccess;
+#define TREE_SCORE(RT) e = op_launch(k_tree_xscore<EPL, RT>, dim3((uint32_t)(base * p.sgroups * p.w.nsplit)), dim3(256), s, a, p.w, p.sgroups)
+#define TREE_SUM(RT) e = op_launch(k_tree_xsum<EPL, RT>, dim3((uint32_t)(base * p.groups * p.w.vsplit)), dim3(EPL * 128), s, a, p.w, p.groups)
     if (p.srt == 1) TREE_SCORE(1); else if (p.srt == 2) TREE_SCORE(2); else if (p.srt == 3) TREE_SCORE(3); else if (p.srt == 4) TREE_SCORE(4); else TREE_SCORE(6);
+    if (e != hipSuccess) return e;
     if (p.rt == 1) TREE_SUM(1);
     else if (EPL == 1 || p.rt == 2) TREE_SUM(2);
     else if constexpr (EPL > 1) TREE_SUM(3);
-    hipLaunchKernelGGL(k_tree_xdiv<EPL * 64>, dim3((uint32_t)((int64_t)a.n_nodes * a.n_heads)), dim3(512), 0, s, a, p.w);
+    if (e != hipSuccess) return e;
+    return op_launch(k_tree_xdiv<EPL * 64>, dim3((uint32_t)((int64_t)a.n_nodes * a.n_heads)), dim3(512), s, a, p.w);
 #undef TREE_SCORE
 #undef TREE_SUM
 }
-void tree_exact(const sp_hipkv_tree_args &a, hipStream_t s) {
+hipError_t tree_exact(const sp_hipkv_tree_args &a, hipStream_t s) {
     const XPlan p = tree_xplan(a);
-    if (a.head_dim == 256) tree_xgo<4>(a, p, s);
-    else if (a.head_dim == 128) tree_xgo<2>(a, p, s);
-    else tree_xgo<1>(a, p, s);
+    return a.head_dim == 256 ? tree_xgo<4>(a, p, s) : a.head_dim == 128 ? tree_xgo<2>(a, p, s) : tree_xgo<1>(a, p, s);
 }
 
 }  // namespace
 
-void launch_tree(const sp_hipkv_tree_args &a, hipStream_t s) {
-    if (a.rows == SP_HIPKV_ROWS_EXACT) tree_exact(a, s);
-    else if (a.rows == SP_HIPKV_ROWS_F32) tree_float<SP_HIPKV_ROWS_F32>(a, s);
-    else tree_float<SP_HIPKV_ROWS_SPINOR>(a, s);
+hipError_t launch_tree(const sp_hipkv_tree_args &a, hipStream_t s) {
+    if (a.rows == SP_HIPKV_ROWS_EXACT) return tree_exact(a, s);
+    return a.rows == SP_HIPKV_ROWS_F32 ? tree_float<SP_HIPKV_ROWS_F32>(a, s) : tree_float<SP_HIPKV_ROWS_SPINOR>(a, s);
 }
 
 }  // namespace kvd
@@ -1388,6 +1387,5 @@ extern "C" int sp_hipkv_tree_attention(const sp_hipkv_tree_args *a, void *stream
     size_t need = 0;
     if (sp_hipkv_tree_attention_work(a, &need) || tree_check_arrays(who, a, need)) return 1;
     OpDevice dev((hipStream_t)stream);
-    if (dev.err == hipSuccess) launch_tree(*a, (hipStream_t)stream);
-    return op_done(who, dev);
+    return op_done(who, dev.err != hipSuccess ? dev.err : launch_tree(*a, (hipStream_t)stream));
 }
