@@ -148,7 +148,8 @@ int  sp_hipkv_decode_batch(sp_kvdecode_handle *const *hs, int n, const int32_t *
  * weight matrix is read once for all nodes; each node attends the context and its
  * ancestors.  logits: n x vocab rows (may be NULL), row i the distribution after
  * node i; next_tokens: their greedy tokens (lowest on ties, may be NULL); logprob
- * (may be NULL): log p of each node's own token after its parent, NaN for roots.
+ * (may be NULL): log p of each node's own token after its parent, NaN for roots;
+ * with it no node has more than 64 children.
  * In exact mode every row is bit for bit what decode steps along the node's path
  * give; in float mode the sums' order differs.  The position stays: the nodes are
  * pending, until sp_hipkv_tree_keep takes a path of them or any other call writes

@@ -415,16 +415,17 @@ class Backend:
               "sp_hipkv_decode_batch_times")
         return nxt, ms, nl, by
 
-    def tree_step(self, tokens, parents, vocab=0):
+    def tree_step(self, tokens, parents, vocab=0, logprob=True):
         """A step over a drafted tree (node i continues node parents[i], -1: the
-        context); vocab > 0 asks for the logits.  Returns (logits [n][vocab] or
-        None, greedy next tokens [n], log p of each node's token [n])."""
+        context); vocab > 0 asks for the logits, logprob for log p of at most 64
+        children of each node.  Returns (logits [n][vocab] or None, greedy next
+        tokens [n], log p of each node's token [n] or None)."""
         import numpy as np
         t, p = (np.ascontiguousarray(x, dtype=np.int32) for x in (tokens, parents))
         assert t.shape == p.shape and t.ndim == 1
         lg = np.zeros((len(t), vocab), np.float32) if vocab else None
-        nxt, lp = np.zeros(len(t), np.int32), np.zeros(len(t), np.float32)
-        check(kv().sp_hipkv_tree_step(self.h, ptr(t), ptr(p), len(t), ptr(lg) if vocab else None, ptr(nxt), ptr(lp)),
+        nxt, lp = np.zeros(len(t), np.int32), np.zeros(len(t), np.float32) if logprob else None
+        check(kv().sp_hipkv_tree_step(self.h, ptr(t), ptr(p), len(t), ptr(lg) if vocab else None, ptr(nxt), ptr(lp) if logprob else None),
               "sp_hipkv_tree_step")
         return lg, nxt, lp
 
