@@ -316,6 +316,11 @@ int  sp_hipkv_tree_attention(const sp_hipkv_tree_args *a, void *stream);
  * the sizes in the block and the sequence's own lengths, not by other sequences'.
  * Ask again when a size changes: a smaller call may need more parts. */
 int  sp_hipkv_tree_attention_work(const sp_hipkv_tree_args *a, size_t *bytes);
+/* How a call of these sizes is cut, for tests and timing (the pointers are not looked
+ * at): plan[0] the tiles of 16 rows, a row being a node's q head, that a workgroup
+ * takes, plan[1] the most parts of a span; plan[2], plan[3] the same of exact rows' V
+ * sums (else 0). */
+int  sp_hipkv_tree_attention_plan(const sp_hipkv_tree_args *a, int32_t plan[4]);
 
 /* Of each row of logits, with y = scale x and p = softmax(y): log p of given
  * tokens, the entropy -sum p log p (nats), log sum exp y, and the n_top largest

@@ -1379,6 +1379,23 @@ extern "C" int sp_hipkv_tree_attention_work(const sp_hipkv_tree_args *a, size_t 
     return 0;
 }
 
+extern "C" int sp_hipkv_tree_attention_plan(const sp_hipkv_tree_args *a, int32_t plan[4]) {
+    using namespace kvd;
+    const char *who = "sp_hipkv_tree_attention_plan";
+    if (tree_check(who, a)) return 1;
+    OP_NEED(plan, "null plan");
+    if (a->rows == SP_HIPKV_ROWS_EXACT) {
+        sp_hipkv_tree_args b = *a;
+        b.work = nullptr;
+        const XPlan p = tree_xplan(b);
+        plan[0] = p.srt; plan[1] = p.w.nsplit; plan[2] = p.rt; plan[3] = p.w.vsplit;
+    } else {
+        const TreePlan p = tree_plan(*a);
+        plan[0] = p.rt; plan[1] = p.nsplit; plan[2] = plan[3] = 0;
+    }
+    return 0;
+}
+
 extern "C" int sp_hipkv_tree_attention(const sp_hipkv_tree_args *a, void *stream) {
     using namespace kvd;
     const char *who = "sp_hipkv_tree_attention";

@@ -168,6 +168,7 @@ def kv():
         for op, args in (("tree_attention", TreeArgs), ("token_logprobs", LogprobArgs), ("keep_rows", KeepArgs)):
             _sig(lib, "sp_hipkv_" + op, c_int, [ctypes.POINTER(args), c_void_p])
         _sig(lib, "sp_hipkv_tree_attention_work", c_int, [ctypes.POINTER(TreeArgs), ctypes.POINTER(c_size_t)])
+        _sig(lib, "sp_hipkv_tree_attention_plan", c_int, [ctypes.POINTER(TreeArgs), c_void_p])
         _sig(lib, "sp_hipkv_token_logprobs_work", c_int, [ctypes.POINTER(LogprobArgs), ctypes.POINTER(c_size_t)])
         _kv = lib
     return _kv
@@ -199,6 +200,13 @@ def tree_attention_work(args):
     n = c_size_t()
     check(kv().sp_hipkv_tree_attention_work(args, ctypes.byref(n)), "sp_hipkv_tree_attention_work")
     return n.value
+
+
+def tree_attention_plan(args):
+    """(row tiles of a workgroup, parts, the same of exact rows' V sums) a call of these sizes takes."""
+    p = (c_int32 * 4)()
+    check(kv().sp_hipkv_tree_attention_plan(args, p), "sp_hipkv_tree_attention_plan")
+    return tuple(p)
 
 
 def token_logprobs(args, stream=0):
