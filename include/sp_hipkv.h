@@ -154,7 +154,10 @@ int  sp_hipkv_decode_batch(sp_kvdecode_handle *const *hs, int n, const int32_t *
  * give; in float mode the sums' order differs.  The position stays: the nodes are
  * pending, until sp_hipkv_tree_keep takes a path of them or any other call writes
  * or rewinds.  A window ring takes what a prefill pass does; stored nodes count
- * as written positions for later rewinds.  Fails, with nothing changed, with recall
+ * as written positions for later rewinds.  The attention's work stays with the batched
+ * calls' buffers: partial outputs, at most 64 rows for each node and q head, and in exact
+ * mode 4 bytes for each node, q head and position (1.1 GB for 128 nodes of 16 heads at
+ * 131072 positions).  Fails, with nothing changed, with recall
  * on, or for model shapes without the batched path. */
 #define SP_HIPKV_TREE_MAX 128
 int  sp_hipkv_tree_step(sp_kvdecode_handle *h, const int32_t *tokens, const int32_t *parents, int n, float *logits,
@@ -269,8 +272,9 @@ int  sp_hipkv_info(const sp_kvdecode_handle *h, long long out[8]);
  * the call's own kernels, so calls in one stream order may share it, and calls
  * (or graphs) that may run at the same time need one each.  Arguments outside
  * the stated limits fail with nothing enqueued.  Limits on what the device arrays
- * hold are the caller's to keep; an array that breaks them gives wrong values,
- * and only page addresses can make a kernel read outside the memory it was given. */
+ * hold are the caller's to keep; an array that breaks them gives wrong values, and
+ * only page tables, with them a ring's size, and keep_start can make a kernel touch
+ * memory that it was not given. */
 enum { SP_HIPKV_ROWS_F32 = 0, SP_HIPKV_ROWS_EXACT = 1, SP_HIPKV_ROWS_SPINOR = 2 };
 
 /* Attention of drafted tokens (nodes) that follow a sequence's cached positions,
@@ -283,10 +287,12 @@ enum { SP_HIPKV_ROWS_F32 = 0, SP_HIPKV_ROWS_EXACT = 1, SP_HIPKV_ROWS_SPINOR = 2 
  * or, for exact rows, with the integer arithmetic of exact mode (bit for bit what
  * a decode step computes on the same rows; |q| below 2^15, |scores| below 2^17).
  * Nodes that see no position get zeros.  Rows that a node does not see do not
- * reach it whatever they hold; one that it sees with a value that is not finite
- * leaves it without a finite value (magnitudes from 2^127 on may count as that, of
- * Spinor rows a multiplier's times 127).  Rows of `out` behind the last sequence's
- * nodes stay as they are. */
+ * reach it whatever they hold.  One that it sees with a value that is not finite
+ * leaves it without a finite value, in K everywhere, in V in the value's column (of
+ * Spinor rows: chunk), however small its weight; magnitudes from 2^127 in K and 2^100
+ * in V on may count as that (of Spinor rows a multiplier's times 127), as may scores
+ * that f32 does not hold.  Rows of `out` behind the last sequence's nodes stay as they
+ * are. */
 typedef struct sp_hipkv_tree_args {
     int32_t n_heads, n_kv_heads;    /* at most 4096, and 16 q heads for each kv head */
     int32_t head_dim;               /* 64, 128 or 256 */
@@ -311,7 +317,8 @@ typedef struct sp_hipkv_tree_args {
     size_t work_bytes;
 } sp_hipkv_tree_args;
 int  sp_hipkv_tree_attention(const sp_hipkv_tree_args *a, void *stream);
-/* Bytes of `work` for these sizes (the pointers are not looked at).  The number
+/* Bytes of `work` for these sizes (the pointers are not looked at): partial sums of
+ * the parts, and of exact rows 4 bytes for each node, q head and position.  The number
  * of parts that a span is cut into, and with it the order of the f32 sums, goes by
  * the sizes in the block and the sequence's own lengths, not by other sequences'.
  * Ask again when a size changes: a smaller call may need more parts. */
@@ -324,11 +331,11 @@ int  sp_hipkv_tree_attention_plan(const sp_hipkv_tree_args *a, int32_t plan[4]);
 
 /* Of each row of logits, with y = scale x and p = softmax(y): log p of given
  * tokens, the entropy -sum p log p (nats), log sum exp y, and the n_top largest
- * logits' tokens (ties: the lowest token first) with their log p.  -inf logits
- * have p = 0.  A given token outside [0, vocab) gets NaN.  A row with a NaN or
- * +inf logit, or with nothing above -inf, has NaN for every value but lse (NaN, or
- * +inf, or -inf); its top tokens are still those of the largest logits, a NaN
- * counting as larger than any number.  f32 sums without the largest term, which is
+ * logits' tokens (ties: the lowest token first) with their log p.  y is f32: what
+ * scale takes out of its range is infinite.  A y of -inf has p = 0.  A given token
+ * outside [0, vocab) gets NaN.  A row with a NaN or a y of +inf, or with nothing above
+ * -inf, has NaN for every value but lse (NaN, or +inf, or -inf); its top tokens are still
+ * those of the largest logits, a NaN counting as larger than any number.  f32 sums without the largest term, which is
  * 1 exactly: entropies near 0 keep their relative precision. */
 typedef struct sp_hipkv_logprob_args {
     int32_t n_rows, vocab;          /* at most 65535 rows, 2^20 tokens */

@@ -74,3 +74,20 @@ def test_sure_rows_and_flat_rows():
     given = np.array([[5000, 77, 151935, 9]] * 5, np.int32)
     o, _ = logprob(x, 1.0, given, 20)
     check(x, 1.0, given, o)
+
+
+def test_logits_that_scaling_takes_out_of_range():
+    """y beyond f32 is infinite: the lowest number as a mask has p = 0 at any temperature, and a
+    row whose largest y is +inf, or that has none above -inf, has no distribution."""
+    lowest, largest = np.finfo(np.float32).min, np.finfo(np.float32).max
+    g = np.random.default_rng(6)
+    x = np.full((4, 9000), lowest, np.float32)
+    x[0, :50] = g.standard_normal(50)
+    x[1, 8999] = -3.0
+    x[3, :] = 0.0; x[3, 70] = largest
+    given = np.array([[3, 8000]] * 4, np.int32)
+    o, _ = logprob(x, 1.25, given, 3)
+    check(x[:1, :50], 1.25, given[:1, :1], {k: v[:1, :1] if k == "lp" else v[:1] for k, v in o.items()})
+    assert o["lp"][0, 1] == -np.inf and o["ent"][1] == 0 and o["lse"][1] == -3.75 and o["ids"][1, 0] == 8999 and o["top"][1, 0] == 0
+    assert np.isnan(o["lp"][2:]).all() and np.isnan(o["ent"][2:]).all() and o["lse"][2] == -np.inf and o["lse"][3] == np.inf
+    assert list(o["ids"][3]) == [70, 0, 1] and list(o["ids"][2]) == [0, 1, 2]

@@ -191,3 +191,23 @@ def test_seen_k_values_that_are_not_finite(rows, hd, value):
         sees = np.arange(6) >= p - cached
         assert not np.isfinite(got[sees]).any(), (cached, p)
         assert (np.abs(got[~sees] - want[~sees]) <= tol[~sees]).all()
+
+
+@pytest.mark.parametrize("rows", [F32, SPINOR])
+def test_seen_v_values_up_to_the_stated_magnitude(rows):
+    """Weights reach 2^8 before the running maximum moves, and their sum 2^28 over the longest
+    spans: V values below 2^100 stay within f32."""
+    for cached, nodes in ((300, 40), (5000, 9)):
+        t = Tree(rows, 128, 2, [cached], [nodes], kind="chain", seed=36)
+        if rows == F32:
+            t.cache.pool[:, 1] *= np.float32(2.0 ** 96)
+        else:
+            mul = np.ascontiguousarray(t.cache.pool[..., 128:140]).view(np.float32)
+            mul[:, 1] *= np.float32(2.0 ** 97)
+            t.cache.pool[..., 128:140] = mul.view(np.uint8)
+        t.q[:, :256] *= 4                              # scores that rise by several powers of two
+        t.dq.put(t.q)
+        t.ready()
+        with np.errstate(all="ignore"):
+            assert 2.0 ** 98 < np.nanmax(np.abs(t.cache.values(0, range(cached + nodes), 1))) < 2.0 ** 100
+        t.check()
