@@ -7,9 +7,11 @@
 // stores; since keep ascends, keep[i] >= i, and a row is read before or with the
 // batch that writes over it.  Threads share nothing, so there is no barrier.
 //
-// The floor is the rows' bytes, read and written; the rest is three dependent loads
-// (lists, page address, row).  A workgroup takes 256 pieces of a table's slices, so that rows
-// below 1 KiB leave no lanes empty: 16 sequences of 36 layers, 8 kv heads of 128 f32, 4 rows each
+// The floor is the rows' bytes, read and written.  The rest is dependent loads (lists, page
+// address, row), row after row: the compiler keeps the 8 rows of a batch in scratch memory
+// (144 bytes a lane), and a row has arrived before it is stored there and the next one's
+// load goes out.  A workgroup takes 256 pieces of a table's slices, so that rows below
+// 1 KiB leave no lanes empty: 16 sequences of 36 layers, 8 kv heads of 128 f32, 4 rows each
 // take 11.1 us (14.5 with one slice a workgroup of 64), a copy of as much 8.
 #include "kvd_op.h"
 

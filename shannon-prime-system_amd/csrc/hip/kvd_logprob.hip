@@ -20,7 +20,7 @@
 // 25 of 8192 at 20), which are ranked by counting.  More than the list holds (many equal
 // logits) are searched by rounds, from memory: keys kept for that would fill the
 // registers, and 64 of them let 8 workgroups share a unit.  64 rows of 262144, 20
-// alternatives: k_lp_part 19.6 us, k_lp_merge 6.9 (28.8 and 7.8 with a bound of
+// alternatives: k_lp_part 20.1 us, k_lp_merge 6.6 (28.8 and 7.8 with a bound of
 // each wave's own, 32 steps and 82 registers).  The rest above the bytes is the bound's and the
 // ranking's latency, once for each workgroup.
 #include "kvd_op.h"

@@ -72,7 +72,7 @@ __device__ __forceinline__ const uint8_t *uniform(const uint8_t *x) {
 // this kernel: 16x16x4 takes 32 cycles, 154 TF, 223 us of the 322 that 64 nodes of 16
 // heads at 32k took (8 kv heads of 256 dims).  A product of two f32 as six products
 // of bf16 pieces (below) costs 2.7 times fewer cycles and errs by 2^-26 of it, less than
-// f32 accumulation does: 235 us.  What bounds it now is a sum, as variants with one part
+// f32 accumulation does: 229 us.  What bounds it now is a sum, as variants with one part
 // taken out showed: forming the pieces (3 roundings and 2 subtractions for each element) a third, the
 // matrix products a third, the wait for memory and for the slowest wave the rest; in a
 // wave they hardly overlap, and the registers (O: 16 RT x HD f32 a wave) allow 2 waves
@@ -84,7 +84,7 @@ __device__ __forceinline__ const uint8_t *uniform(const uint8_t *x) {
 // position) joins outside the product: on the scores of the chunk's dims, and on the weights
 // before they are taken apart.  Dims and columns are therefore dealt to steps and tiles by
 // chunk, as windows of 64 dims of which 51 (43, 32) count.  16 nodes at 6k of 16 heads (8 kv
-// heads of 256 dims) take 25.9 us; as f32 products of codes times multipliers, which was the first form,
+// heads of 256 dims) take 26.4 us; as f32 products of codes times multipliers, which was the first form,
 // 36.5, and 30 nodes of 32 heads at 12k 50 for 82 us.  The codes' conversion bounds it now, 1.5
 // instructions a code, and below 20 us what is fixed.
 //
@@ -706,11 +706,16 @@ __global__ __launch_bounds__(256) void k_tree_merge(sp_hipkv_tree_args a, int ns
 // The weights' digits are made once for all waves and pass through LDS; half of the waves
 // make the next page's before the products, half after.
 //
-// 48 nodes of 16 heads at 32k (8 kv heads of 256 dims): scores 105 us, sums 120, division
-// 6; reading K and V once is 113 us, and variants with one part taken out name none
-// that would give more than 40 (memory's wait; the int8 products, digits, weights and
-// epilogues 10 each).  7 nodes at 4k: 9.7 + 11 + 3.4 us, where no part but the first loads (3 us)
-// shows: launches and dependent loads.
+// 48 nodes of 16 heads at 32k (8 kv heads of 256 dims): scores 100 us, sums 114, division
+// 6; reading K and V once is 113 us, z (100 MB) written and read once some 42 more, and variants
+// with one part taken out name none that would give more than 40 (memory's wait; the int8
+// products, digits, weights and epilogues 10 each).  7 nodes at 4k: 10.5 + 11.2 + 3.9 us, where no
+// part but the first loads (3 us) shows: launches and dependent loads.
+//
+// The V sums of head dim 64, and of 128 with two row tiles or more, are slower than their
+// work: from four position pairs a thread on the compiler leaves `weights` a function, and
+// what it takes by reference lies in scratch memory, 352 to 416 bytes a lane.  24 nodes of 32
+// heads at 4k (8 kv heads of 128 dims) take 90 us, of 16 heads with 256 dims 49.
 constexpr int DIG3 = 127 * (1 + 256 + 65536);                    // largest |x| of three balanced digits
 
 // x = d0 + 2^8 d1 + 2^16 d2 + 2^24 d3, d in [-128, 127]; four values' digits, one dword per
