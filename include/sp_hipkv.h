@@ -377,6 +377,133 @@ typedef struct sp_hipkv_keep_args {
 } sp_hipkv_keep_args;
 int  sp_hipkv_keep_rows(const sp_hipkv_keep_args *a, void *stream);
 
+/* ---- operators of serving from a paged cache on device memory ----
+ * Writing the cache, attention of whole prompts, and attention of new tokens over a
+ * cache in 8 bits, for programs that keep K/V in pages themselves.  No counterpart in
+ * the reference (its decode stores f32 rows, one token at a time).  What is said above
+ * of pointers, streams, work and limits holds here too.  Values that these calls take
+ * and give (q, k, v, out) are of one type:
+ *   SP_HIPKV_F32          f32
+ *   SP_HIPKV_BF16         bf16, each result rounded once, to nearest
+ * Rows of values start 16-byte aligned: strides count values and are multiples of 4
+ * (bf16: of 8).  The tokens of a call are packed: sequence s has tokens start[s] ..
+ * start[s + 1], at positions cached[s] .. behind what it holds; a sequence may have none.
+ * Rows behind the last sequence's tokens stay as they are.
+ *
+ * A page of 8-bit rows (SP_HIPKV_ROWS_BLOCK8; 16-byte aligned,
+ * sp_hipkv_block8_page_bytes of them) holds int8 codes with one f32 scale, not
+ * negative, for each block of 16 positions, of K and of V, of each kv head; a value is code x scale:
+ *   K codes  [n_kv_heads][64 positions][head_dim]
+ *   V codes  [n_kv_heads][head_dim][64]; of a column's 64 bytes, position
+ *            16 u + 4 g + i (u, g, i < 4) is at 16 g + 4 u + i
+ *   scales   [K, V][n_kv_heads][4 blocks] */
+enum { SP_HIPKV_F32 = 0, SP_HIPKV_BF16 = 1 };
+enum { SP_HIPKV_ROWS_BLOCK8 = 3 };
+/* 2 n_kv_heads (64 head_dim + 16); 0 for sizes that the operators refuse */
+size_t sp_hipkv_block8_page_bytes(int32_t n_kv_heads, int32_t head_dim);
+
+/* Append tokens to the cache, with what comes before it: of every q and k head
+ *   x <- x w / sqrt(mean x^2 + eps)                        (q_norm, k_norm; NULL: left out)
+ *   x_i, x_(i + head_dim/2) <- turned by the angle position x freq[i]   (freq NULL: left out)
+ * in 64 bits, angles too (below 2^30).  q and, where asked for, k are given back; K and V
+ * go to the pages, as f32 rows or in 8 bits from the 64-bit values.  Of a block in 8 bits
+ * the scale is the least power of two (from 2^-126 on) that holds its largest magnitude in
+ * 127 codes; a block that already holds earlier positions of the sequence keeps a larger
+ * scale, and when its scale grows the codes of those positions are rounded again: tokens
+ * appended one by one may so differ by a code from the same ones in one call.  The first
+ * position of a block starts it anew.  A block given a value that is not finite gets
+ * a scale of NaN, and every position of it reads as NaN until it is started anew.
+ * Of more tokens than a ring holds, those whose page a later one takes are not stored.
+ * No two sequences may write the same page. */
+typedef struct sp_hipkv_append_args {
+    int32_t n_heads, n_kv_heads;    /* at most 4096, and 16 q heads for each kv head */
+    int32_t head_dim;               /* 64, 128 or 256 */
+    int32_t type;                   /* SP_HIPKV_F32, SP_HIPKV_BF16: q, k, v and what is given back */
+    int32_t rows;                   /* SP_HIPKV_ROWS_F32 or SP_HIPKV_ROWS_BLOCK8 */
+    int32_t n_seqs, n_tokens;       /* sequences (at most 4096), tokens of all of them (at most 2^20) */
+    int32_t max_tokens;             /* no sequence has more */
+    int32_t max_positions;          /* cached + tokens of no sequence is more (at most 2^20) */
+    int32_t ring_pages;             /* 0: full tables */
+    float   eps;                    /* of the norms, not negative */
+    const int32_t *start;           /* [n_seqs + 1] ascending */
+    const int32_t *cached;          /* [n_seqs] */
+    const void *const *const *tables;   /* [n_seqs] page tables */
+    const double *freq;             /* [head_dim / 2] radians a position; NULL: no rotation */
+    const float *q_norm, *k_norm;   /* [head_dim]; NULL: no norm */
+    const void *q;                  /* [n_tokens][q_stride], head h at h * head_dim; NULL with q_out */
+    int64_t q_stride;
+    const void *k;                  /* [n_tokens][k_stride], kv head h at h * head_dim */
+    int64_t k_stride;
+    const void *v;                  /* as k */
+    int64_t v_stride;
+    void *q_out;                    /* as q, q itself too; NULL: q is left out */
+    int64_t q_out_stride;
+    void *k_out;                    /* as k, k itself too; NULL: not wanted */
+    int64_t k_out_stride;
+} sp_hipkv_append_args;
+int  sp_hipkv_append(const sp_hipkv_append_args *a, void *stream);
+
+/* Attention of whole prompts from packed q, k, v (after norm and rotation): token t of a
+ * sequence, counted from the sequence's first, attends tokens [max(0, t - window + 1), t]
+ * of it: out = sum_p softmax_p(scale q.k_p) v_p, sums in f32.  f32 products are made of
+ * bf16 pieces, to 2^-25; of bf16 values the weights are rounded to bf16 before they
+ * multiply v.  Tokens that a token does not attend do not reach it whatever they hold.  A
+ * value that is not finite in one that it attends leaves it without a finite value, in k
+ * everywhere (but for bf16 scores of -inf, whose weight is 0), in v in the value's column
+ * (f32 magnitudes above 3.38e38 may count as that, as may scores that f32 does not hold). */
+typedef struct sp_hipkv_prompt_args {
+    int32_t n_heads, n_kv_heads;    /* at most 4096, and 16 q heads for each kv head */
+    int32_t head_dim;               /* 64, 128 or 256 */
+    int32_t type;                   /* SP_HIPKV_F32, SP_HIPKV_BF16 */
+    int32_t n_seqs, n_tokens;       /* sequences (at most 4096), tokens of all of them (at most 2^20) */
+    int32_t max_tokens;             /* no sequence has more */
+    int32_t window;                 /* 0: every token before */
+    float   scale;                  /* 1 / sqrt(head_dim) in the models served */
+    const int32_t *start;           /* [n_seqs + 1] ascending */
+    const void *q;                  /* [n_tokens][q_stride], head h at h * head_dim */
+    int64_t q_stride;
+    const void *k;                  /* [n_tokens][k_stride], kv head h at h * head_dim */
+    int64_t k_stride;
+    const void *v;                  /* as k */
+    int64_t v_stride;
+    void *out;                      /* as q */
+    int64_t out_stride;
+} sp_hipkv_prompt_args;
+int  sp_hipkv_prompt_attention(const sp_hipkv_prompt_args *a, void *stream);
+
+/* Attention of new tokens over the 8-bit cache, which holds their rows already (a decode
+ * step's one token a sequence, or a piece of a prompt): token j of sequence s, at position
+ * p = cached[s] + j, attends positions [max(0, p - window + 1), p]:
+ * out = sum softmax(scale q.k) v.  q and the weights are taken to integers of 23 bits (of a
+ * row's largest value, of a page's largest weight), whose products with the codes are exact.
+ * Positions that a token does not attend do not reach it whatever their codes and scales.
+ * A scale that is not finite in a block that it attends, or a q value that is not, leaves
+ * it without a finite value. */
+typedef struct sp_hipkv_cache_args {
+    int32_t n_heads, n_kv_heads;    /* at most 4096, and 16 q heads for each kv head */
+    int32_t head_dim;               /* 64, 128 or 256 */
+    int32_t type;                   /* SP_HIPKV_F32, SP_HIPKV_BF16: q and out */
+    int32_t n_seqs, n_tokens;       /* sequences (at most 4096), tokens of all of them (times n_heads at most 2^22) */
+    int32_t max_tokens;             /* no sequence has more (at most 512) */
+    int32_t max_positions;          /* cached + tokens of no sequence is more (at most 2^20) */
+    int32_t window;                 /* 0: every position before */
+    int32_t ring_pages;             /* 0: full tables; a ring holds window + max_tokens positions and a page more */
+    float   scale;                  /* 1 / sqrt(head_dim) in the models served */
+    const int32_t *start;           /* [n_seqs + 1] ascending */
+    const int32_t *cached;          /* [n_seqs] positions before the tokens */
+    const void *const *const *tables;   /* [n_seqs] page tables */
+    const void *q;                  /* [n_tokens][q_stride], head h at h * head_dim */
+    int64_t q_stride;
+    void *out;                      /* as q */
+    int64_t out_stride;
+    void *work;                     /* sp_hipkv_cache_attention_work bytes, 16-byte aligned */
+    size_t work_bytes;
+} sp_hipkv_cache_args;
+int  sp_hipkv_cache_attention(const sp_hipkv_cache_args *a, void *stream);
+/* Bytes of `work` for these sizes (the pointers are not looked at).  Ask again when a
+ * size changes: a smaller call may need more parts. */
+int  sp_hipkv_cache_attention_work(const sp_hipkv_cache_args *a, size_t *bytes);
+
 #ifdef __cplusplus
 }
 #endif

@@ -58,6 +58,9 @@ inline int op_done(const char *who, hipError_t e) {
 hipError_t launch_tree(const sp_hipkv_tree_args &a, hipStream_t s);
 hipError_t launch_logprob(const sp_hipkv_logprob_args &a, hipStream_t s);
 hipError_t launch_keep(const sp_hipkv_keep_args &a, hipStream_t s);
+hipError_t launch_append(const sp_hipkv_append_args &a, hipStream_t s);
+hipError_t launch_prompt(const sp_hipkv_prompt_args &a, hipStream_t s);
+hipError_t launch_cache(const sp_hipkv_cache_args &a, hipStream_t s);
 
 __host__ __device__ constexpr int row_bytes_of(int rows, int hd) { return rows == SP_HIPKV_ROWS_SPINOR ? spn_row_bytes(hd) : 4 * hd; }
 

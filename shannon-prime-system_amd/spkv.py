@@ -44,7 +44,8 @@ class DispatchTable(ctypes.Structure):
                 ("rewind", c_void_p), ("position", c_void_p), ("close", c_void_p)]
 
 
-ROWS_F32, ROWS_EXACT, ROWS_SPINOR = 0, 1, 2     # SP_HIPKV_ROWS_* (include/sp_hipkv.h)
+ROWS_F32, ROWS_EXACT, ROWS_SPINOR, ROWS_BLOCK8 = 0, 1, 2, 3     # SP_HIPKV_ROWS_* (include/sp_hipkv.h)
+F32, BF16 = 0, 1                                # SP_HIPKV_F32, SP_HIPKV_BF16
 
 
 class TreeArgs(ctypes.Structure):
@@ -70,6 +71,32 @@ class KeepArgs(ctypes.Structure):
     _fields_ = [("n_kv_heads", c_int32), ("row_bytes", c_int32), ("n_tables", c_int32), ("n_seqs", c_int32),
                 ("max_keep", c_int32), ("max_positions", c_int32), ("tables", c_void_p), ("seq", c_void_p),
                 ("ring_pages", c_void_p), ("cached", c_void_p), ("keep_start", c_void_p), ("keep", c_void_p)]
+
+
+class AppendArgs(ctypes.Structure):
+    """sp_hipkv_append_args (include/sp_hipkv.h)."""
+    _fields_ = [("n_heads", c_int32), ("n_kv_heads", c_int32), ("head_dim", c_int32), ("type", c_int32), ("rows", c_int32),
+                ("n_seqs", c_int32), ("n_tokens", c_int32), ("max_tokens", c_int32), ("max_positions", c_int32), ("ring_pages", c_int32),
+                ("eps", c_float), ("start", c_void_p), ("cached", c_void_p), ("tables", c_void_p), ("freq", c_void_p),
+                ("q_norm", c_void_p), ("k_norm", c_void_p), ("q", c_void_p), ("q_stride", ctypes.c_int64), ("k", c_void_p),
+                ("k_stride", ctypes.c_int64), ("v", c_void_p), ("v_stride", ctypes.c_int64), ("q_out", c_void_p),
+                ("q_out_stride", ctypes.c_int64), ("k_out", c_void_p), ("k_out_stride", ctypes.c_int64)]
+
+
+class PromptArgs(ctypes.Structure):
+    """sp_hipkv_prompt_args (include/sp_hipkv.h)."""
+    _fields_ = [("n_heads", c_int32), ("n_kv_heads", c_int32), ("head_dim", c_int32), ("type", c_int32), ("n_seqs", c_int32),
+                ("n_tokens", c_int32), ("max_tokens", c_int32), ("window", c_int32), ("scale", c_float), ("start", c_void_p),
+                ("q", c_void_p), ("q_stride", ctypes.c_int64), ("k", c_void_p), ("k_stride", ctypes.c_int64), ("v", c_void_p),
+                ("v_stride", ctypes.c_int64), ("out", c_void_p), ("out_stride", ctypes.c_int64)]
+
+
+class CacheArgs(ctypes.Structure):
+    """sp_hipkv_cache_args (include/sp_hipkv.h)."""
+    _fields_ = [("n_heads", c_int32), ("n_kv_heads", c_int32), ("head_dim", c_int32), ("type", c_int32), ("n_seqs", c_int32),
+                ("n_tokens", c_int32), ("max_tokens", c_int32), ("max_positions", c_int32), ("window", c_int32), ("ring_pages", c_int32),
+                ("scale", c_float), ("start", c_void_p), ("cached", c_void_p), ("tables", c_void_p), ("q", c_void_p),
+                ("q_stride", ctypes.c_int64), ("out", c_void_p), ("out_stride", ctypes.c_int64), ("work", c_void_p), ("work_bytes", c_size_t)]
 
 
 _l1 = None
@@ -165,11 +192,14 @@ def kv():
         _sig(lib, "sp_hipkv_tree_step", c_int, [c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_void_p, c_void_p])
         _sig(lib, "sp_hipkv_tree_keep", c_int, [c_void_p, c_void_p, c_int])
         _sig(lib, "sp_hipkv_score", c_int, [c_void_p, c_void_p, c_void_p, c_int, c_int, c_void_p, c_void_p, c_void_p, c_void_p])
-        for op, args in (("tree_attention", TreeArgs), ("token_logprobs", LogprobArgs), ("keep_rows", KeepArgs)):
+        for op, args in (("tree_attention", TreeArgs), ("token_logprobs", LogprobArgs), ("keep_rows", KeepArgs), ("append", AppendArgs),
+                         ("prompt_attention", PromptArgs), ("cache_attention", CacheArgs)):
             _sig(lib, "sp_hipkv_" + op, c_int, [ctypes.POINTER(args), c_void_p])
         _sig(lib, "sp_hipkv_tree_attention_work", c_int, [ctypes.POINTER(TreeArgs), ctypes.POINTER(c_size_t)])
         _sig(lib, "sp_hipkv_tree_attention_plan", c_int, [ctypes.POINTER(TreeArgs), c_void_p])
         _sig(lib, "sp_hipkv_token_logprobs_work", c_int, [ctypes.POINTER(LogprobArgs), ctypes.POINTER(c_size_t)])
+        _sig(lib, "sp_hipkv_cache_attention_work", c_int, [ctypes.POINTER(CacheArgs), ctypes.POINTER(c_size_t)])
+        _sig(lib, "sp_hipkv_block8_page_bytes", c_size_t, [c_int32, c_int32])
         _kv = lib
     return _kv
 
@@ -223,6 +253,32 @@ def token_logprobs_work(args):
 def keep_rows(args, stream=0):
     """Move the accepted nodes' K/V rows into place (sp_hipkv_keep_rows)."""
     check(kv().sp_hipkv_keep_rows(args, stream), "sp_hipkv_keep_rows")
+
+
+def block8_page_bytes(n_kv_heads, head_dim):
+    """Bytes of a page of 8-bit rows (ROWS_BLOCK8)."""
+    return kv().sp_hipkv_block8_page_bytes(n_kv_heads, head_dim)
+
+
+def append(args, stream=0):
+    """Norm, rotation and append of new tokens to the paged cache (sp_hipkv_append)."""
+    check(kv().sp_hipkv_append(args, stream), "sp_hipkv_append")
+
+
+def prompt_attention(args, stream=0):
+    """Causal attention of packed prompts (sp_hipkv_prompt_attention)."""
+    check(kv().sp_hipkv_prompt_attention(args, stream), "sp_hipkv_prompt_attention")
+
+
+def cache_attention(args, stream=0):
+    """Attention of new tokens over the 8-bit cache (sp_hipkv_cache_attention)."""
+    check(kv().sp_hipkv_cache_attention(args, stream), "sp_hipkv_cache_attention")
+
+
+def cache_attention_work(args):
+    n = c_size_t()
+    check(kv().sp_hipkv_cache_attention_work(args, ctypes.byref(n)), "sp_hipkv_cache_attention_work")
+    return n.value
 
 
 # ---------------------------------------------------------------- synthetic inputs

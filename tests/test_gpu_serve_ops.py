@@ -1,0 +1,468 @@
+"""The operators of serving from a paged cache on device memory against plain 64-bit
+implementations (tests/serve_ref.py, where the tolerances are derived)."""
+import ctypes
+
+import numpy as np
+import pytest
+
+import spkv
+import tree_ref
+from devmem import Dev, Stream, hip, sync
+from serve_ref import BLOCK, PAGE, Append, Cache8, Cached, Packed, Prompt, cache_attention, close, packed_start, prepared, prompt_attention
+
+pytestmark = pytest.mark.gpu
+F32, BF16, BLOCK8, ROWS = spkv.F32, spkv.BF16, spkv.ROWS_BLOCK8, spkv.ROWS_F32
+TYPES = [F32, BF16]
+HEADS = [(64, 1), (64, 4), (128, 2), (128, 4), (256, 2), (256, 16), (128, 3), (64, 7)]
+
+
+def rng(*seed):
+    return np.random.default_rng(list(seed))
+
+
+def f32_cache(g, nkv, hd, lens, ring=0):
+    c = tree_ref.Cache(g, ROWS, nkv, hd, lens, ring)
+    c.pool[:] = g.standard_normal(c.pool.shape)
+    return c.upload()
+
+
+# ---------------------------------------------------------------- append
+def appended(g, rows, typ, hd, G, cached, counts, ring=0, nkv=2, room=None, **kw):
+    if rows == BLOCK8:
+        c = Cache8(g, nkv, hd, cached, ring, room or [a + b for a, b in zip(cached, counts)]).upload()
+    else:
+        c = f32_cache(g, nkv, hd, room or [a + b for a, b in zip(cached, counts)], ring)
+    return Append(g, c, rows, typ, hd, G, cached, counts, **kw)
+
+
+@pytest.mark.parametrize("typ", TYPES)
+@pytest.mark.parametrize("rows", [BLOCK8, ROWS])
+@pytest.mark.parametrize("hd,G", HEADS)
+def test_append_heads(rows, typ, hd, G):
+    appended(rng(1, hd, G), rows, typ, hd, G, [70, 0], [9, 100]).check()
+
+
+@pytest.mark.parametrize("typ", TYPES)
+@pytest.mark.parametrize("rows", [BLOCK8, ROWS])
+@pytest.mark.parametrize("cached,counts", [([0], [1]), ([0], [16]), ([15], [1]), ([15], [2]), ([63], [2]), ([64], [1]), ([17], [130]), ([1], [63]),
+                                           ([0, 5, 300, 64, 7], [3, 0, 17, 64, 0]), ([0] * 70, [1] * 70), ([100] * 3, [0, 0, 5]), ([3, 90], [200, 1])])
+def test_append_lengths(rows, typ, cached, counts):
+    appended(rng(2, len(cached)), rows, typ, 128, 2, cached, counts).check()
+
+
+@pytest.mark.parametrize("rows", [BLOCK8, ROWS])
+@pytest.mark.parametrize("kw", [dict(norm=False), dict(freq=False), dict(norm=False, freq=False), dict(q_out=False), dict(k_out=None), dict(q_out="same", k_out="same"),
+                                dict(pad=8), dict(q_out=False, k_out=None, pad=16), dict(more_tokens=5)])
+def test_append_forms(rows, kw):
+    for typ in TYPES:
+        appended(rng(3), rows, typ, 64, 2, [20, 50], [30, 5], **kw).check()
+
+
+@pytest.mark.parametrize("typ", TYPES)
+def test_append_far_positions(typ):
+    """The angle of a position near 2^20: off by 0.06 in 32 bits."""
+    g = rng(4)
+    c = Cache8(g, 1, 128, [PAGE], 1, [PAGE])                 # a ring of one page holds any position
+    c.upload()
+    Append(g, c, BLOCK8, typ, 128, 2, [(1 << 20) - 20], [20], base=1e6).check()
+
+
+def test_append_step_by_step():
+    """Tokens one by one, each against what it should leave: scales grow, earlier codes are
+    rounded again; and the values stay within a step and a half of the block's last scale."""
+    for typ in TYPES:
+        g = rng(5)
+        n, nkv, hd = 40, 2, 64
+        c = Cache8(g, nkv, hd, [0], 0, [n]).upload()
+        grow = (2.0 ** (np.arange(n) % BLOCK / 2))[:, None, None]
+        k, v = g.standard_normal((n, nkv, hd)) * grow, g.standard_normal((n, nkv, hd)) * grow[::-1]
+        for t in range(n):
+            c.lens = [t]
+            Append(g, c, BLOCK8, typ, hd, 1, [t], [1], norm=False, freq=False, k=k[t:t + 1], v=v[t:t + 1]).check()
+        for which, x in ((0, k), (1, v)):
+            codes, sc = c.values(0, range(n), which)
+            x = Packed(x, typ).values()
+            assert (np.abs(codes * sc[..., None] - x) <= 1.5 * sc[..., None]).all()
+
+
+def test_append_extremes():
+    """Zeros, the smallest and largest numbers, and values around 127 of a power of two."""
+    g = rng(6)
+    vals = [0.0, -0.0, 1e-45, 1.1754944e-38, 2.0 ** -119, 127 * 2.0 ** -126, 127.0, np.nextafter(np.float32(127), np.float32(200)), 63.5, 64.0, 3.4028235e38, -3e38]
+    n = len(vals)
+    x = np.zeros((n * BLOCK, 1, 64))
+    for i, a in enumerate(vals):
+        x[i * BLOCK:(i + 1) * BLOCK, 0] = a * (g.random((BLOCK, 64)) < 0.5)
+    c = Cache8(g, 1, 64, [0], 0, [n * BLOCK]).upload()
+    a = Append(g, c, BLOCK8, F32, 64, 1, [0], [n * BLOCK], norm=False, freq=False, k=x, v=x)
+    a.check()
+    assert np.isfinite(c.s[c.page[0]][:, 0, 0].reshape(-1)[:n]).all()
+
+
+@pytest.mark.parametrize("bad", [np.nan, np.inf, -np.inf])
+def test_append_values_that_are_not_finite(bad):
+    """Their block gets a scale of NaN, keeps it, and is started anew at its first position."""
+    g = rng(7)
+    x = g.standard_normal((40, 2, 64))
+    x[5, 0, 3], x[33, 1, 60] = bad, bad
+    for typ in TYPES:
+        c = Cache8(g, 2, 64, [0], 0, [48]).upload()
+        a = Append(g, c, BLOCK8, typ, 64, 1, [0], [40], norm=False, freq=False, k_out=None, k=x, v=x)
+        a.check()
+        assert np.isnan(c.s).sum() >= 4
+        one = g.standard_normal((1, 2, 64))
+        Append(g, c, BLOCK8, typ, 64, 1, [40], [1], norm=False, freq=False, k=one, v=one).check()
+        again = g.standard_normal((8, 2, 64))
+        Append(g, c, BLOCK8, typ, 64, 1, [32], [8], norm=False, freq=False, k=again, v=again).check()
+        pg, i = c.block(0, 2)
+        assert np.isfinite(c.s[pg, :, :, i]).all()
+
+
+@pytest.mark.parametrize("rows", [BLOCK8, ROWS])
+@pytest.mark.parametrize("cached,counts,ring", [([100, 640], [40, 3], 3), ([0], [1000], 3), ([70], [64 * 3], 3), ([5000], [200], 1), ([130], [1], 2)])
+def test_append_rings(rows, cached, counts, ring):
+    g = rng(8, ring)
+    if rows == BLOCK8:
+        c = Cache8(g, 2, 64, cached, ring).upload()
+    else:
+        c = f32_cache(g, 2, 64, [64 * ring] * len(cached), ring)
+    Append(g, c, rows, F32, 64, 2, cached, counts).check()
+
+
+def test_append_more_heads_than_a_wave():
+    appended(rng(9), BLOCK8, BF16, 64, 1, [3], [20], nkv=70).check()
+
+
+# ---------------------------------------------------------------- prompts
+@pytest.mark.parametrize("typ", TYPES)
+@pytest.mark.parametrize("hd,G", HEADS)
+def test_prompt_heads(typ, hd, G):
+    Prompt(rng(11, hd, G), typ, hd, G, [70, 9]).check()
+
+
+@pytest.mark.parametrize("typ", TYPES)
+@pytest.mark.parametrize("counts", [[1], [2], [31], [32], [33], [63], [64], [65], [129], [200], [1, 1, 1], [0, 5, 0, 0, 70, 1, 0], [40] * 20, [3] * 70])
+def test_prompt_lengths(typ, counts):
+    Prompt(rng(12, len(counts)), typ, 128, 2, counts).check()
+
+
+@pytest.mark.parametrize("typ", TYPES)
+@pytest.mark.parametrize("hd", [64, 128, 256])
+def test_prompt_long(typ, hd):
+    Prompt(rng(13, hd), typ, hd, 2, [700], nkv=1).check()
+
+
+@pytest.mark.parametrize("typ", TYPES)
+@pytest.mark.parametrize("window", [1, 2, 31, 64, 100, 1000])
+def test_prompt_windows(typ, window):
+    Prompt(rng(14, window), typ, 64, 2, [300, 17], window=window, nkv=1).check()
+    Prompt(rng(15, window), typ, 128, 3, [130], window=window, nkv=1).check()
+
+
+@pytest.mark.parametrize("typ", TYPES)
+@pytest.mark.parametrize("scale", [0.0, -0.1, 1.0, 1e-30])
+def test_prompt_scales(typ, scale):
+    Prompt(rng(16), typ, 64, 2, [100, 3], scale=scale).check()
+
+
+@pytest.mark.parametrize("typ", TYPES)
+def test_prompt_strides_and_rows_behind(typ):
+    Prompt(rng(17), typ, 128, 2, [50, 20], pad=8, more_tokens=6).check()
+
+
+@pytest.mark.parametrize("typ", TYPES)
+def test_prompt_peaked_weights(typ):
+    """Scores in the hundreds: the running maximum moves far, weights vanish."""
+    Prompt(rng(18), typ, 64, 2, [300], wide=60.0).check()
+
+
+@pytest.mark.parametrize("typ", TYPES)
+@pytest.mark.parametrize("hd", [64, 128, 256])
+@pytest.mark.parametrize("bad", [np.nan, np.inf, -np.inf])
+def test_prompt_values_that_are_not_attended(typ, hd, bad):
+    """K and V rows of later tokens, of tokens before the window and of other sequences hold
+    values that are not finite: tokens that do not attend them are as without, the others
+    are not finite (from K everywhere, from V in its column)."""
+    g = rng(19, hd)
+    counts, window, G = [90, 80], 40, 2
+    p = Prompt(g, typ, hd, G, counts, window=window, nkv=1)
+    clean, tol = p.want()
+    k, v = p.k.values().copy(), p.v.values().copy()
+    k[20, 0, 5] = bad                                       # attended by tokens 20 .. 59 of sequence 0
+    v[70, 0, 7] = bad                                       # by 70 .. 89
+    v[100, 0, :] = bad                                      # token 10 of sequence 1: 10 .. 49
+    p.k, p.v = Packed(k, typ), Packed(v, typ)
+    p.args.k, p.args.k_stride, p.args.v, p.args.v_stride = p.k.at, p.k.stride, p.v.at, p.v.stride
+    got = p.run()
+    hit = np.zeros(got.shape, bool)
+    hit[70:90, :, 7] = True
+    hit[100:140] = True
+    gone = np.zeros(got.shape, bool)
+    gone[20:60] = True
+    if np.isinf(bad) and typ == BF16:                       # scores of -inf have weight 0
+        assert 0 < np.isfinite(got[20:60]).all(-1).sum() < 40 * G
+    else:
+        assert not np.isfinite(got[gone]).any()
+    assert not np.isfinite(got[hit & ~gone]).any()
+    rest = ~(hit | gone)
+    assert (np.abs(got - clean)[rest] <= tol[rest]).all()
+
+
+@pytest.mark.parametrize("typ", TYPES)
+def test_prompt_nothing_read_behind_the_last_row(typ):
+    """k and v that end with the last sequence: what lies behind is not a row of theirs."""
+    g = rng(20)
+    p = Prompt(g, typ, 64, 1, [33], nkv=1)
+    p.k, p.v = Packed(p.k.values(), typ, 0, 0), Packed(p.v.values(), typ, 0, 0)
+    p.args.k, p.args.k_stride, p.args.v, p.args.v_stride = p.k.at, p.k.stride, p.v.at, p.v.stride
+    p.check()
+
+
+# ---------------------------------------------------------------- cache
+@pytest.mark.parametrize("typ", TYPES)
+@pytest.mark.parametrize("hd,G", HEADS)
+def test_cache_heads(typ, hd, G):
+    Cached(rng(21, hd, G), typ, hd, G, [70, 5], [9, 1]).ready().check()
+
+
+@pytest.mark.parametrize("typ", TYPES)
+@pytest.mark.parametrize("cached,counts", [([0], [1]), ([0], [5]), ([1], [1]), ([15], [1]), ([63], [2]), ([64], [1]), ([62], [67]), ([128], [64]),
+                                           ([1000], [3]), ([515], [130]), ([0, 5, 300, 64, 9], [3, 0, 17, 40, 0]), ([33] * 40, [1] * 40)])
+def test_cache_lengths(typ, cached, counts):
+    Cached(rng(22, len(cached)), typ, 128, 2, cached, counts).ready().check()
+
+
+@pytest.mark.parametrize("typ", TYPES)
+@pytest.mark.parametrize("hd", [64, 128, 256])
+def test_cache_long(typ, hd):
+    """Spans cut into parts, and every count of tokens around a tile."""
+    for n in (1, 8, 9, 33):
+        Cached(rng(23, n), typ, hd, 2, [5003], [n], nkv=1).ready().check()
+
+
+@pytest.mark.parametrize("typ", TYPES)
+def test_cache_ragged_parts(typ):
+    Cached(rng(24), typ, 64, 2, [9000, 10, 700, 0, 2500], [2, 1, 3, 1, 0], nkv=1).ready().check()
+
+
+def test_cache_longest():
+    """Positions up to 2^17: page tables of 2048 entries."""
+    Cached(rng(25), F32, 64, 1, [(1 << 17) - 1], [1], nkv=1).ready().check()
+
+
+@pytest.mark.parametrize("typ", TYPES)
+@pytest.mark.parametrize("cached,ring", [(40, 0), (200, 0), (1000, 0), (1000, 4), (127, 4), (2000, 3)])
+def test_cache_windows(typ, cached, ring):
+    Cached(rng(26, cached), typ, 128, 2, [cached, cached + 1], [24, 3], window=100, ring=ring).ready().check()
+    Cached(rng(27, cached), typ, 64, 4, [cached], [24], window=1, ring=ring).ready().check()
+
+
+@pytest.mark.parametrize("typ", TYPES)
+@pytest.mark.parametrize("scale", [0.0, -0.1, 1.0])
+def test_cache_scales(typ, scale):
+    Cached(rng(28), typ, 64, 2, [100, 3], [2, 2], scale=scale, wide=3.0).ready().check()
+
+
+@pytest.mark.parametrize("typ", TYPES)
+def test_cache_strides_and_rows_behind(typ):
+    for cached in ([70, 9], [6000, 9]):                     # one part, and several
+        Cached(rng(29), typ, 128, 2, cached, [5, 2], pad=8, more_tokens=6).ready().check()
+
+
+def test_cache_scales_far_apart():
+    """Blocks whose scales differ by 2^60, in K and in V, zero scales among them."""
+    g = rng(30)
+    t = Cached(g, F32, 64, 2, [500], [2], nkv=1)
+    for pg in t.cache.page[0]:
+        t.cache.s[pg, 1] *= 2.0 ** g.choice([-30, 0, 30], 4)
+        t.cache.s[pg, 0] *= 2.0 ** g.choice([-30, 0], 4)
+    t.cache.s[t.cache.page[0][2], :, 0, 1] = 0
+    t.ready().check()
+
+
+@pytest.mark.parametrize("bad", [np.nan, np.inf])
+def test_cache_scales_that_are_not_finite(bad):
+    """A block's scale of NaN or infinity reaches the tokens that attend one of its positions, all
+    of their values; tokens before it and those whose window is past it are as without."""
+    for which in (0, 1):
+        for typ in TYPES:
+            g = rng(31, which)
+            t = Cached(g, typ, 64, 2, [100], [40], window=30, nkv=1)
+            want, tol = t.want()
+            pg, i = t.cache.block(0, 7)                      # positions 112 .. 127, from token 12 on
+            t.cache.s[pg, which, 0, i] = bad
+            t.ready()
+            got = t.run()
+            assert not np.isfinite(got[12:]).any()
+            assert (np.abs(got - want)[:12] <= tol[:12]).all()
+            late = Cached(g, typ, 64, 2, [157], [3], window=30, nkv=1)    # windows from 128 on
+            pg, i = late.cache.block(0, 7)
+            late.cache.s[pg, which, 0, i] = bad
+            late.ready().check()
+
+
+@pytest.mark.parametrize("bad", [np.nan, np.inf])
+def test_cache_q_that_is_not_finite(bad):
+    t = Cached(rng(33), F32, 64, 2, [100], [3], nkv=1)
+    want, tol = t.want()
+    q = t.q.values().copy()
+    q[1, 0, 9] = bad
+    t.q = Packed(q, F32)
+    t.args.q = t.q.at
+    got = t.ready().run()
+    assert not np.isfinite(got[1, 0]).any()
+    rest = np.ones(got.shape, bool)
+    rest[1, 0] = False
+    assert (np.abs(got - want)[rest] <= tol[rest]).all()
+
+
+@pytest.mark.parametrize("value", [0.0, 1e-42, 3e38])
+def test_cache_extreme_q(value):
+    g = rng(34)
+    q = g.standard_normal((2, 2, 64))
+    q[1] = value
+    t = Cached(g, F32, 64, 2, [100], [2], nkv=1, q=q, scale=1e-38 if value > 1 else 0.125)
+    t.ready().check()
+
+
+# ---------------------------------------------------------------- as they would be used
+@pytest.mark.parametrize("typ", TYPES)
+@pytest.mark.parametrize("hd,G,window", [(128, 2, 0), (64, 4, 40), (256, 2, 100)])
+def test_prompts_then_tokens(typ, hd, G, window):
+    """A packed batch of prompts is appended and attended, then tokens one at a time and a piece of
+    five: the cache's values are those of append, outputs those of the cache that it left."""
+    g = rng(41, hd)
+    counts, nkv = [70, 1, 130], 2
+    ring = -(-(window + 5) // PAGE) + 1 if window else 0
+    room = [c + 20 for c in counts]
+    c = Cache8(g, nkv, hd, [0] * 3, ring, room).upload()
+    a = Append(g, c, BLOCK8, typ, hd, G, [0] * 3, counts)
+    p = Prompt(g, typ, hd, G, counts, window=window, nkv=nkv, q=a.q0, k=a.k0, v=a.v0)
+    p.args.q, p.args.q_stride, p.args.k, p.args.k_stride = a.q_out.at, a.q_out.stride, a.k_out.at, a.k_out.stride
+    s = Stream()
+    spkv.append(a.args, s.h.value)
+    spkv.prompt_attention(p.args, s.h.value)
+    s.sync()
+    a.check(run=False)
+    p.q, p.k = a.q_out, a.k_out
+    a.q_out.dev.a, a.k_out.dev.a = a.q_out.dev.get(), a.k_out.dev.get()
+    close(p.got(), *p.want())
+    at = list(counts)
+    for step in (1, 1, 5, 1):
+        n = [step] * 3
+        a = Append(g, c, BLOCK8, typ, hd, G, at, n)
+        t = Cached(g, typ, hd, G, at, n, window=window, nkv=nkv, cache=c, q=a.q0).ready()
+        t.args.q, t.args.q_stride = a.q_out.at, a.q_out.stride
+        spkv.append(a.args, s.h.value)
+        spkv.cache_attention(t.args, s.h.value)
+        s.sync()
+        a.check(run=False)
+        a.q_out.dev.a = a.q_out.dev.get()
+        t.q = a.q_out
+        close(t.got(), *t.want())
+        at = [x + step for x in at]
+
+
+def test_appended_f32_rows_are_tree_attentions():
+    """f32 rows that append writes, read by tree attention as a chain."""
+    g = rng(42)
+    cached, n, hd, G, nkv = 100, 5, 128, 2, 2
+    c = f32_cache(g, nkv, hd, [cached + n])
+    a = Append(g, c, ROWS, F32, hd, G, [cached], [n])
+    spkv.append(a.args)
+    a.check(run=False)
+    see, depth = tree_ref.masks(g, "chain", n)
+    vis, out = Dev(tree_ref.words(see, 1)), Dev(np.zeros((n, nkv * G, hd), np.float32))
+    t = spkv.TreeArgs(n_heads=nkv * G, n_kv_heads=nkv, head_dim=hd, rows=ROWS, n_seqs=1, n_nodes=n, max_nodes=n, max_positions=cached + n, window=0, ring_pages=0,
+                      mask_words=1, scale=0.1, node_start=a.hold["start"].at, cached=a.hold["cached"].at, visible=vis.at, tables=c.lists.at, q=a.q_out.at,
+                      q_stride=a.q_out.stride, out=out.at, out_stride=nkv * G * hd)
+    need = spkv.tree_attention_work(t)
+    work = Dev(np.zeros(need + 16, np.uint8))
+    t.work, t.work_bytes = work.at, need
+    spkv.tree_attention(t)
+    q = a.q_out.get()[:n]
+    c.pool = c.dev.get()
+    want, tol = tree_ref.tree_attention(c, [cached], [(see, depth)], q, 0, float(np.float32(0.1)))
+    assert (np.abs(out.get() - want) <= tol).all()
+
+
+@pytest.mark.parametrize("typ", TYPES)
+def test_calls_in_a_graph(typ):
+    """A decode step captured and replayed on new inputs, with the program's own work between the
+    replays: each replay is the call on those inputs."""
+    g = rng(43)
+    hd, G, nkv, cached = 128, 2, 2, [3000, 40]
+    c = Cache8(g, nkv, hd, cached, 0, [x + 16 for x in cached]).upload()
+    a = Append(g, c, BLOCK8, typ, hd, G, cached, [1, 1])
+    t = Cached(g, typ, hd, G, cached, [1, 1], nkv=nkv, cache=c, q=a.q0).ready()
+    p = Prompt(g, typ, hd, G, [60, 70], nkv=nkv)
+    t.args.q, t.args.q_stride = a.q_out.at, a.q_out.stride
+    s = Stream()
+
+    def record(stream):
+        spkv.append(a.args, stream)
+        spkv.cache_attention(t.args, stream)
+        spkv.prompt_attention(p.args, stream)
+
+    e = s.capture(record)
+    for k in range(4):
+        x = rng(44, k)
+        q, kk, v = (Packed(x.standard_normal(z.shape), typ) for z in (a.q, a.k, a.v))
+        for dst, src in ((a.q, q), (a.k, kk), (a.v, v)):
+            dst.dev.put(src.dev.a[:, :dst.stride] if dst.stride == src.stride else src.dev.a)
+        c.dev.put(c.pool)
+        a.q0, a.k0, a.v0 = q.values()[:2], kk.values()[:2], v.values()[:2]
+        pq = Packed(x.standard_normal(p.q.shape), typ)
+        p.q.dev.put(pq.dev.a)
+        p.q.dev.a = pq.dev.a
+        s.launch(e)
+        s.sync()
+        before = c.pool.copy()
+        a.check(run=False)
+        q_out = a.q_out.get()
+        want, tol = cache_attention(c, q_out[:2], cached, [1, 1], 0, t.scale, typ)
+        close(t.got(), want, tol)
+        close(p.got(), *p.want())
+        Dev(np.zeros(1 << 20, np.uint8)).get()
+        c.pool[:] = before
+
+
+def test_two_streams_at_once():
+    """Calls on two streams with workspaces of their own."""
+    g = rng(45)
+    a, b = Cached(g, F32, 128, 2, [4000], [3], nkv=1).ready(), Cached(g, BF16, 64, 4, [3000, 20], [1, 2], nkv=1).ready()
+    s, r = Stream(), Stream()
+    for _ in range(5):
+        spkv.cache_attention(a.args, s.h.value)
+        spkv.cache_attention(b.args, r.h.value)
+    s.sync(); r.sync()
+    a.check(a.got())
+    b.check(b.got())
+
+
+def test_same_bits_again():
+    """No order of arrival decides a sum: the same call gives the same bits."""
+    g = rng(46)
+    for typ in TYPES:
+        t, p = Cached(g, typ, 128, 2, [5000, 900], [2, 7], nkv=1).ready(), Prompt(g, typ, 128, 2, [500], nkv=1)
+        x, y = t.run().copy(), p.run().copy()
+        for _ in range(3):
+            assert np.array_equal(t.run().view(np.uint32), x.view(np.uint32)) and np.array_equal(p.run().view(np.uint32), y.view(np.uint32))
+
+
+def test_beside_a_pending_error():
+    """An error that an earlier call of the program left neither fails these calls nor is taken by them."""
+    g = rng(47)
+    t, p = Cached(g, F32, 64, 2, [5000], [3], nkv=1).ready(), Prompt(g, F32, 64, 2, [40], nkv=1)
+    a = appended(g, BLOCK8, F32, 64, 2, [20], [5])
+    hip().hipGetLastError()
+    code = hip().hipMalloc(None, ctypes.c_size_t(16))
+    assert code != 0
+    spkv.cache_attention(t.args)
+    spkv.prompt_attention(p.args)
+    spkv.append(a.args)
+    assert hip().hipGetLastError() == code
+    sync()
+    t.check(t.got())
+    p.check(p.got())
+    a.check(run=False)
