@@ -44,7 +44,7 @@ __device__ __forceinline__ const uint8_t *uniform(const uint8_t *x) {
 }
 
 template <typename T, int HD, int RT>
-__global__ __launch_bounds__(64 * CACHE_WAVES, 2) void k_cache(sp_hipkv_cache_args a, int groups, int nsplit, int pages) {
+__global__ __launch_bounds__(64 * CACHE_WAVES, HD == 256 ? 1 : 2) void k_cache(sp_hipkv_cache_args a, int groups, int nsplit, int pages) {
     constexpr int KS = HD / 64, CT = HD / 16, NW = CACHE_WAVES, NT = 64 * NW;
     __shared__ __align__(16) float s_o[NW][16][HD];
     __shared__ float s_m[NW][16], s_l[NW][16], s_M[16], s_L[16];
