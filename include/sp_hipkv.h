@@ -385,8 +385,8 @@ int  sp_hipkv_keep_rows(const sp_hipkv_keep_args *a, void *stream);
  * and give (q, k, v, out) are of one type:
  *   SP_HIPKV_F32          f32
  *   SP_HIPKV_BF16         bf16, each result rounded once, to nearest
- * Rows of values start 16-byte aligned: strides count values and are multiples of 4
- * (bf16: of 8).  The tokens of a call are packed: sequence s has tokens start[s] ..
+ * Rows of values start 16-byte aligned: strides count values, are multiples of 4 (bf16: of
+ * 8) and at most 2^24.  The tokens of a call are packed: sequence s has tokens start[s] ..
  * start[s + 1], at positions cached[s] .. behind what it holds; a sequence may have none.
  * Rows behind the last sequence's tokens stay as they are.
  *
@@ -450,7 +450,8 @@ int  sp_hipkv_append(const sp_hipkv_append_args *a, void *stream);
  * multiply v.  Tokens that a token does not attend do not reach it whatever they hold.  A
  * value that is not finite in one that it attends leaves it without a finite value, in k
  * everywhere (but for bf16 scores of -inf, whose weight is 0), in v in the value's column
- * (f32 magnitudes above 3.38e38 may count as that, as may scores that f32 does not hold). */
+ * (magnitudes from 2^90 on in v may count as that, f32 ones above 3.38e38 in k, and scores
+ * that f32 does not hold). */
 typedef struct sp_hipkv_prompt_args {
     int32_t n_heads, n_kv_heads;    /* at most 4096, and 16 q heads for each kv head */
     int32_t head_dim;               /* 64, 128 or 256 */

@@ -15,13 +15,16 @@
 // output's own rounding (sqrt 2 of it together); the sum adds them unrounded.
 // f32: K, V, q and weights as three bf16 pieces, six products each (kvd_pieces.h).
 //
-// The running maximum only moves when a score exceeds it by 2^8 in the exponent: weights
-// stay below 2^8 and nothing is lost, and most tiles leave the output unscaled.
+// The running maximum only moves when a score exceeds it by 2^16 in the exponent: weights
+// stay below 2^16, nothing is lost below sums of 2^128 (v of 2^90 over 2^20 tokens), and most tiles leave the
+// output unscaled.  With 2^8, scores of a standard deviation of 4.5 had some row of 32 move in every
+// eighth tile of 8192 tokens, 90 us of 640.
 //
 // A key that a row does not attend has weight 0, which a V value that is not finite would turn
 // into NaN: tiles that some row does not attend whole are staged with zeros in place of such
 // values, and rows that attend them get them afterwards.
 #include "kvd_serve.h"
+#include "kvd_pass.h"
 #include <algorithm>
 
 namespace kvd {
@@ -32,6 +35,8 @@ typedef float v16f __attribute__((ext_vector_type(16)));
 typedef short v4s __attribute__((ext_vector_type(4)));
 typedef __attribute__((address_space(3))) v4s lds4s;
 constexpr float LOG2E_F = 1.44269504088896341f;
+
+constexpr float SLACK = 16.0f;                                           // exponent (base 2) that a weight may reach
 
 __device__ __forceinline__ float other_half(float x) { return __shfl_xor(x, 32, 64); }
 
@@ -97,7 +102,7 @@ __global__ __launch_bounds__(256, (PromptShape<T, HD>::WPS)) void k_prompt(sp_hi
     const int first = r0 / G, last = (min(r0 + BM, R) - 1) / G, w_first = min(wr0, R - 1) / G, w_last = (min(wr0 + 32 * QT, R) - 1) / G;
     const int k0 = max(first - W + 1, 0) / BN, k1 = last / BN + 1;
     // scale <= 0 goes into q's sign (or makes q zero), so that larger scores have larger weights
-    const float sgn = a.scale > 0 ? 1.0f : a.scale < 0 ? -1.0f : 0.0f, c = a.scale == 0 ? LOG2E_F : fabsf(a.scale) * LOG2E_F, slack = 8.0f / c;
+    const float sgn = a.scale > 0 ? 1.0f : a.scale < 0 ? -1.0f : 0.0f, c = a.scale == 0 ? LOG2E_F : fabsf(a.scale) * LOG2E_F, slack = SLACK / c;
     int tok[QT];
     bf8 Q[QT][HD / 16][NP];
     #pragma unroll
@@ -295,6 +300,187 @@ __global__ __launch_bounds__(256, (PromptShape<T, HD>::WPS)) void k_prompt(sp_hi
     }
 }
 
+// ---------------------------------------------------------------- bf16
+// K and V come through LDS by direct loads, two tiles deep, with one barrier a tile.
+template <int HD>
+__global__ __launch_bounds__(256, HD == 256 ? 1 : 2) void k_prompt16(sp_hipkv_prompt_args a, int slots) {
+    constexpr int BN = HD == 256 ? 32 : 64, BM = 128, KT = BN / 32, KS = HD / 16, DT = HD / 32, C8 = HD / 8, TB = BN * HD * 2;      // bytes of a tile
+    __shared__ __align__(1024) uint8_t lds[4 * TB];                       // K of even and odd tiles, then V
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), l32 = lane & 31, half = lane >> 5;
+    const int G = a.n_heads / a.n_kv_heads, h = blockIdx.x % a.n_kv_heads;
+    // the longest spans first: a sequence's last rows before its first
+    const int slot = slots - 1 - blockIdx.x / a.n_kv_heads;
+    const int s = unit_seq(a.start, a.n_seqs, slot, G, BM, 1);
+    const int t0 = max(gmem(a.start)[s], 0), n = min(min(gmem(a.start)[s + 1], a.n_tokens) - t0, a.max_tokens);
+    const int64_t j = slot - unit_base(a.start, s, G, BM, 1);
+    if (n <= 0 || j < 0 || j * BM >= (int64_t)n * G) return;
+    const int R = n * G, r0 = (int)j * BM, wr0 = r0 + wave * 32;
+    const int W = a.window ? a.window : INT32_MAX;
+    const int first = r0 / G, last = (min(r0 + BM, R) - 1) / G, w_first = min(wr0, R - 1) / G, w_last = (min(wr0 + 32, R) - 1) / G;
+    const int k0 = max(first - W + 1, 0) / BN, k1 = last / BN + 1;
+    const float sgn = a.scale > 0 ? 1.0f : a.scale < 0 ? -1.0f : 0.0f, c = a.scale == 0 ? LOG2E_F : fabsf(a.scale) * LOG2E_F, slack = SLACK / c;
+    const Bf16 *kp = (const Bf16 *)a.k + (size_t)t0 * a.k_stride + (size_t)h * HD, *vp = (const Bf16 *)a.v + (size_t)t0 * a.v_stride + (size_t)h * HD;
+    // Direct loads fill LDS in order; a lane takes the 16-byte chunk whose place that is: chunks of a K
+    // row lie in an order that spreads a column over the banks, 64-byte runs of V that of four rows
+    constexpr int RPI = 512 / HD, NI = TB / 4096;                         // rows of one load, loads of a wave for a tile
+    auto k_swz = [](int row) { return HD == 64 ? row >> 1 & 7 : row & 15; };
+    auto v_swz = [](int row) { return HD == 64 ? (row >> 1 & 1) << 2 : (row & 3) << 2; };
+    int ko[NI], vo[NI];
+    #pragma unroll
+    for (int i = 0; i < NI; i++) {
+        const int row = (wave * NI + i) * RPI + lane / C8, ch = lane % C8;
+        ko[i] = (row * (int)a.k_stride + 8 * (ch ^ k_swz(row))) * 2;
+        vo[i] = (row * (int)a.v_stride + 8 * (ch ^ v_swz(row))) * 2;
+    }
+    const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) const uint8_t *)lds + wave * NI * 1024;
+    auto load = [&](const Bf16 *p, int64_t stride, const int (&off)[NI], int tile, int to) {
+        const int rows = min(n - tile * BN, BN);
+        const v4i rs = rsrc_of(p + (int64_t)tile * BN * stride, rows > 0 ? (uint32_t)((rows - 1) * (int)stride + HD) * 2 : 0);
+        #pragma unroll
+        for (int i = 0; i < NI; i++) dma16(lds0 + to * TB + i * 1024, off[i], rs);
+    };
+    load(kp, a.k_stride, ko, k0, 0);
+    load(vp, a.v_stride, vo, k0, 2);
+    const int row = min(wr0 + l32, R - 1), tok = row / G;
+    bf8 Q[KS];
+    {
+        const Bf16 *q = (const Bf16 *)a.q + (size_t)(t0 + tok) * a.q_stride + (size_t)(h * G + row % G) * HD + 8 * half;
+        #pragma unroll
+        for (int k = 0; k < KS; k++) {
+            float x[8];
+            load_values(q + 16 * k, x);
+            Q[k] = __builtin_bit_cast(bf8, (v4u){bf16x2(x[0] * sgn, x[1] * sgn), bf16x2(x[2] * sgn, x[3] * sgn), bf16x2(x[4] * sgn, x[5] * sgn), bf16x2(x[6] * sgn, x[7] * sgn)});
+        }
+    }
+    v16f O[DT];
+    const v16f zero = {0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0};
+    #pragma unroll
+    for (int d = 0; d < DT; d++) O[d] = zero;
+    float m = -INFINITY, l = 0.0f;
+    // this lane's places in a tile: of K by dims, of V (row (l % 16) / 4 of four, 4 columns of 16, for the
+    // transposing reads) by columns
+    int k_at[KS], v_at[DT];
+    #pragma unroll
+    for (int k = 0; k < KS; k++) k_at[k] = (l32 * C8 + ((2 * k + half) ^ k_swz(l32))) * 16;
+    #pragma unroll
+    for (int d = 0; d < DT; d++) {
+        const int r = 4 * half + (lane & 15) / 4, col = d * 32 + 16 * (lane >> 4 & 1) + 4 * (lane & 3);
+        v_at[d] = (r * C8 + ((col / 8) ^ v_swz(r))) * 16 + col % 8 * 2;
+    }
+    // V values that were left out of a tile, for the rows that attend them
+    auto add_odd = [&](int key0) __attribute__((always_inline)) {
+        #pragma unroll 1
+        for (int key = key0; key < min(key0 + BN, n); key++) {
+            const Bf16 *vrow = vp + (size_t)key * a.v_stride + 4 * half;
+            #pragma unroll
+            for (int d = 0; d < DT; d++)
+                #pragma unroll
+                for (int i = 0; i < 16; i += 4) {
+                    float x[4];
+                    load_values(vrow + d * 32 + 2 * i, x);
+                    #pragma unroll
+                    for (int y = 0; y < 4; y++) O[d][i + y] += key <= tok && key > tok - W && !pieces_hold(x[y]) ? x[y] * INFINITY : 0.0f;
+                }
+        }
+    };
+    // zeros in LDS in place of V values that are not finite; whether this thread found one
+    auto clean = [&](uint8_t *lds) __attribute__((always_inline)) {
+        bool bad = false;
+        #pragma unroll
+        for (int i = 0; i < TB / 4096; i++) {
+            Chunk<Bf16> x = {((v4u *)lds)[threadIdx.x + 256 * i]};
+            if (chunk_clean(x)) { bad = true; ((v4u *)lds)[threadIdx.x + 256 * i] = x.a; }
+        }
+        return bad;
+    };
+    auto work = [&](int tile, auto part) __attribute__((always_inline)) {
+        constexpr int BUF = part.value;
+        const bool ragged = tile * BN + BN - 1 > first || tile * BN < last - W + 1;        // some row does not attend it whole
+        asm volatile("s_waitcnt vmcnt(0)" : : : "memory");
+        __syncthreads();
+        bool odd = false;
+        if (ragged) odd = __syncthreads_or(clean(lds + (2 + BUF) * TB));
+        if (tile + 1 < k1) {
+            load(kp, a.k_stride, ko, tile + 1, 1 - BUF);
+            load(vp, a.v_stride, vo, tile + 1, 3 - BUF);
+        }
+        if (tile * BN > w_last || tile * BN + BN <= w_first - W + 1) return;               // no row of this wave attends any
+        v16f S[KT];
+        #pragma unroll
+        for (int u = 0; u < KT; u++)
+            #pragma unroll
+            for (int k = 0; k < KS; k++)
+                S[u] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(*(const bf8 *)(lds + k_at[k] + BUF * TB + u * 32 * HD * 2), Q[k], k ? S[u] : zero, 0, 0, 0);
+        if (tile * BN + BN - 1 > w_first || tile * BN < w_last - W + 1) {
+            #pragma unroll
+            for (int u = 0; u < KT; u++)
+                #pragma unroll
+                for (int i = 0; i < 16; i++) {
+                    const int key = tile * BN + u * 32 + 8 * (i / 4) + 4 * half + i % 4;
+                    S[u][i] = key <= tok && key > tok - W ? S[u][i] : -INFINITY;
+                }
+        }
+        float mx = S[0][0];
+        #pragma unroll
+        for (int u = 0; u < KT; u++)
+            #pragma unroll
+            for (int i = 0; i < 16; i++) mx = fmaxf(mx, S[u][i]);
+        if (__builtin_expect(__any(mx > m + slack), 0)) {
+            mx = fmaxf(mx, other_half(mx));
+            const float mn = fmaxf(m, mx), al = mn == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f((m - mn) * c);
+            m = mn;
+            l *= al;
+            #pragma unroll
+            for (int d = 0; d < DT; d++)
+                #pragma unroll
+                for (int i = 0; i < 16; i++) O[d][i] *= al;
+        }
+        const float nm = m == -INFINITY ? 0.0f : -m * c;
+        bf8 P[KT][2];
+        #pragma unroll
+        for (int u = 0; u < KT; u++)
+            #pragma unroll
+            for (int e = 0; e < 2; e++) {
+                float w[8];
+                #pragma unroll
+                for (int i = 0; i < 8; i++) {
+                    w[i] = __builtin_amdgcn_exp2f(fmaf(S[u][8 * e + i], c, nm));
+                    l += w[i];
+                }
+                P[u][e] = __builtin_bit_cast(bf8, (v4u){bf16x2(w[0], w[1]), bf16x2(w[2], w[3]), bf16x2(w[4], w[5]), bf16x2(w[6], w[7])});
+            }
+        #pragma unroll
+        for (int u = 0; u < KT; u++)
+            #pragma unroll
+            for (int e = 0; e < 2; e++)
+                #pragma unroll
+                for (int d = 0; d < DT; d++) {
+                    typedef short v8s __attribute__((ext_vector_type(8)));
+                    const v4s y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4s *)(lds + v_at[d] + (2 + BUF) * TB + (32 * u + 16 * e) * HD * 2));
+                    const v4s z = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4s *)(lds + v_at[d] + (2 + BUF) * TB + (32 * u + 16 * e + 8) * HD * 2));
+                    O[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf8, __builtin_shufflevector(y, z, 0, 1, 2, 3, 4, 5, 6, 7)), P[u][e], O[d], 0, 0, 0);
+                }
+        if (odd) add_odd(tile * BN);
+    };
+    for (int tile = k0; tile < k1; tile += 2) {
+        work(tile, std::integral_constant<int, 0>{});
+        if (tile + 1 < k1) work(tile + 1, std::integral_constant<int, 1>{});
+    }
+    const int r = wr0 + l32;
+    const float inv = 1.0f / (l + other_half(l));
+    if (r >= R) return;
+    Bf16 *o = (Bf16 *)a.out + (size_t)(t0 + tok) * a.out_stride + (size_t)(h * G + r % G) * HD + 4 * half;
+    #pragma unroll
+    for (int d = 0; d < DT; d++)
+        #pragma unroll
+        for (int i = 0; i < 16; i += 4) {
+            float x[4];
+            #pragma unroll
+            for (int y = 0; y < 4; y++) x[y] = O[d][i + y] * inv;
+            store_values(o + d * 32 + 2 * i, x);
+        }
+}
+
 int prompt_check(const sp_hipkv_prompt_args *a) {
     const char *who = "sp_hipkv_prompt_attention";
     if (serve_check(who, a)) return 1;
@@ -307,6 +493,10 @@ int prompt_check(const sp_hipkv_prompt_args *a) {
 }
 
 template <typename T, int HD> hipError_t prompt_go(const sp_hipkv_prompt_args &a, hipStream_t s) {
+    if constexpr (sizeof(T) == 2) {
+        const int slots = (int)((int64_t)a.n_tokens * (a.n_heads / a.n_kv_heads) / 128) + a.n_seqs;
+        return op_launch(k_prompt16<HD>, dim3((uint32_t)((int64_t)slots * a.n_kv_heads)), dim3(256), s, a, slots);
+    }
     const int slots = (int)((int64_t)a.n_tokens * (a.n_heads / a.n_kv_heads) / PromptShape<T, HD>::BM) + a.n_seqs;
     return op_launch(k_prompt<T, HD>, dim3((uint32_t)((int64_t)slots * a.n_kv_heads)), dim3(256), s, a, slots);
 }
