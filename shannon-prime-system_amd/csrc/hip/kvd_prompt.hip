@@ -302,9 +302,9 @@ __global__ __launch_bounds__(256, (PromptShape<T, HD>::WPS)) void k_prompt(sp_hi
 
 // ---------------------------------------------------------------- bf16
 // K and V come through LDS by direct loads, two tiles deep, with one barrier a tile.
-template <int HD>
-__global__ __launch_bounds__(256, HD == 256 ? 1 : 2) void k_prompt16(sp_hipkv_prompt_args a, int slots) {
-    constexpr int BN = HD == 256 ? 32 : 64, BM = 128, KT = BN / 32, KS = HD / 16, DT = HD / 32, C8 = HD / 8, TB = BN * HD * 2;      // bytes of a tile
+template <int HD, int NW>
+__global__ __launch_bounds__(64 * NW, HD == 256 ? 1 : 2) void k_prompt16(sp_hipkv_prompt_args a, int slots) {
+    constexpr int BN = HD == 256 ? 32 : 64, BM = 32 * NW, KT = BN / 32, KS = HD / 16, DT = HD / 32, C8 = HD / 8, TB = BN * HD * 2;      // bytes of a tile
     __shared__ __align__(1024) uint8_t lds[4 * TB];                       // K of even and odd tiles, then V
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), l32 = lane & 31, half = lane >> 5;
     const int G = a.n_heads / a.n_kv_heads, h = blockIdx.x % a.n_kv_heads;
@@ -322,7 +322,7 @@ __global__ __launch_bounds__(256, HD == 256 ? 1 : 2) void k_prompt16(sp_hipkv_pr
     const Bf16 *kp = (const Bf16 *)a.k + (size_t)t0 * a.k_stride + (size_t)h * HD, *vp = (const Bf16 *)a.v + (size_t)t0 * a.v_stride + (size_t)h * HD;
     // Direct loads fill LDS in order; a lane takes the 16-byte chunk whose place that is: chunks of a K
     // row lie in an order that spreads a column over the banks, 64-byte runs of V that of four rows
-    constexpr int RPI = 512 / HD, NI = TB / 4096;                         // rows of one load, loads of a wave for a tile
+    constexpr int RPI = 512 / HD, NI = TB / 1024 / NW;                         // rows of one load, loads of a wave for a tile
     auto k_swz = [](int row) { return HD == 64 ? row >> 1 & 7 : row & 15; };
     auto v_swz = [](int row) { return HD == 64 ? (row >> 1 & 1) << 2 : (row & 3) << 2; };
     int ko[NI], vo[NI];
@@ -387,9 +387,9 @@ __global__ __launch_bounds__(256, HD == 256 ? 1 : 2) void k_prompt16(sp_hipkv_pr
     auto clean = [&](uint8_t *lds) __attribute__((always_inline)) {
         bool bad = false;
         #pragma unroll
-        for (int i = 0; i < TB / 4096; i++) {
-            Chunk<Bf16> x = {((v4u *)lds)[threadIdx.x + 256 * i]};
-            if (chunk_clean(x)) { bad = true; ((v4u *)lds)[threadIdx.x + 256 * i] = x.a; }
+        for (int i = 0; i < NI; i++) {
+            Chunk<Bf16> x = {((v4u *)lds)[threadIdx.x + 64 * NW * i]};
+            if (chunk_clean(x)) { bad = true; ((v4u *)lds)[threadIdx.x + 64 * NW * i] = x.a; }
         }
         return bad;
     };
@@ -405,12 +405,27 @@ __global__ __launch_bounds__(256, HD == 256 ? 1 : 2) void k_prompt16(sp_hipkv_pr
             load(vp, a.v_stride, vo, tile + 1, 3 - BUF);
         }
         if (tile * BN > w_last || tile * BN + BN <= w_first - W + 1) return;               // no row of this wave attends any
+        // fragments are read 8 products ahead, the first of V beside the last of K
+        constexpr int NF = 8, NKF = KT * KS, NVF = KT * 2 * DT;
         v16f S[KT];
+        bf8 F[NF];
+        auto read_k = [&](int x) { return *(const bf8 *)(lds + k_at[x % KS] + BUF * TB + x / KS * 32 * HD * 2); };
+        auto read_v = [&](int x) {
+            typedef short v8s __attribute__((ext_vector_type(8)));
+            const v4s y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4s *)(lds + v_at[x % DT] + (2 + BUF) * TB + 16 * (x / DT) * HD * 2));
+            const v4s z = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4s *)(lds + v_at[x % DT] + (2 + BUF) * TB + (16 * (x / DT) + 8) * HD * 2));
+            return __builtin_bit_cast(bf8, __builtin_shufflevector(y, z, 0, 1, 2, 3, 4, 5, 6, 7));
+        };
         #pragma unroll
-        for (int u = 0; u < KT; u++)
-            #pragma unroll
-            for (int k = 0; k < KS; k++)
-                S[u] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(*(const bf8 *)(lds + k_at[k] + BUF * TB + u * 32 * HD * 2), Q[k], k ? S[u] : zero, 0, 0, 0);
+        for (int x = 0; x < NF; x++) F[x] = read_k(x);
+        __builtin_amdgcn_sched_group_barrier(0x100, NF, 0);
+        #pragma unroll
+        for (int x = 0; x < NKF; x++) {
+            S[x / KS] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(F[x % NF], Q[x % KS], x % KS ? S[x / KS] : zero, 0, 0, 0);
+            F[x % NF] = x + NF < NKF ? read_k(x + NF) : read_v(x + NF - NKF);
+            __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+            if (x + NF < NKF) __builtin_amdgcn_sched_group_barrier(0x100, 1, 0); else __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
+        }
         if (tile * BN + BN - 1 > w_first || tile * BN < w_last - W + 1) {
             #pragma unroll
             for (int u = 0; u < KT; u++)
@@ -450,16 +465,12 @@ __global__ __launch_bounds__(256, HD == 256 ? 1 : 2) void k_prompt16(sp_hipkv_pr
                 P[u][e] = __builtin_bit_cast(bf8, (v4u){bf16x2(w[0], w[1]), bf16x2(w[2], w[3]), bf16x2(w[4], w[5]), bf16x2(w[6], w[7])});
             }
         #pragma unroll
-        for (int u = 0; u < KT; u++)
-            #pragma unroll
-            for (int e = 0; e < 2; e++)
-                #pragma unroll
-                for (int d = 0; d < DT; d++) {
-                    typedef short v8s __attribute__((ext_vector_type(8)));
-                    const v4s y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4s *)(lds + v_at[d] + (2 + BUF) * TB + (32 * u + 16 * e) * HD * 2));
-                    const v4s z = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4s *)(lds + v_at[d] + (2 + BUF) * TB + (32 * u + 16 * e + 8) * HD * 2));
-                    O[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf8, __builtin_shufflevector(y, z, 0, 1, 2, 3, 4, 5, 6, 7)), P[u][e], O[d], 0, 0, 0);
-                }
+        for (int x = 0; x < NVF; x++) {
+            O[x % DT] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(F[x % NF], P[x / DT / 2][x / DT % 2], O[x % DT], 0, 0, 0);
+            if (x + NF < NVF) F[x % NF] = read_v(x + NF);
+            __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+            if (x + NF < NVF) __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
+        }
         if (odd) add_odd(tile * BN);
     };
     for (int tile = k0; tile < k1; tile += 2) {
@@ -494,8 +505,9 @@ int prompt_check(const sp_hipkv_prompt_args *a) {
 
 template <typename T, int HD> hipError_t prompt_go(const sp_hipkv_prompt_args &a, hipStream_t s) {
     if constexpr (sizeof(T) == 2) {
-        const int slots = (int)((int64_t)a.n_tokens * (a.n_heads / a.n_kv_heads) / 128) + a.n_seqs;
-        return op_launch(k_prompt16<HD>, dim3((uint32_t)((int64_t)slots * a.n_kv_heads)), dim3(256), s, a, slots);
+        constexpr int NW = 4;
+        const int slots = (int)((int64_t)a.n_tokens * (a.n_heads / a.n_kv_heads) / (32 * NW)) + a.n_seqs;
+        return op_launch(k_prompt16<HD, NW>, dim3((uint32_t)((int64_t)slots * a.n_kv_heads)), dim3(64 * NW), s, a, slots);
     }
     const int slots = (int)((int64_t)a.n_tokens * (a.n_heads / a.n_kv_heads) / PromptShape<T, HD>::BM) + a.n_seqs;
     return op_launch(k_prompt<T, HD>, dim3((uint32_t)((int64_t)slots * a.n_kv_heads)), dim3(256), s, a, slots);
