@@ -13,7 +13,7 @@
 //
 // bf16: weights are rounded to bf16 before the second product, an error of the size of the
 // output's own rounding (sqrt 2 of it together); the sum adds them unrounded.
-// f32: K, V, q and weights as three bf16 pieces, six products each (kvd_pieces.h).
+// f32: K, V, q and weights as two f16 numbers each, three products (below).
 //
 // The running maximum only moves when a score exceeds it by 2^16 in the exponent: weights
 // stay below 2^16, nothing is lost below sums of 2^128 (v of 2^90 over 2^20 tokens), and most tiles leave the
@@ -25,6 +25,7 @@
 // values, and rows that attend them get them afterwards.
 #include "kvd_serve.h"
 #include "kvd_pass.h"
+#include "kvd_vec.h"
 #include <algorithm>
 
 namespace kvd {
@@ -40,265 +41,19 @@ constexpr float SLACK = 16.0f;                                           // expo
 
 __device__ __forceinline__ float other_half(float x) { return __shfl_xor(x, 32, 64); }
 
-template <typename T, int HD> struct PromptShape {
-    static constexpr int NP = sizeof(T) == 4 ? 3 : 1, BN = NP == 3 ? 32 : 64;
-    static constexpr int QT = 1, BM = 128 * QT;
-    static constexpr int WPS = NP == 3 && HD == 256 ? 1 : HD == 256 ? 1 : 2;             // waves a SIMD
-};
-
-// eight staged values: f32 as they are, bf16 as bits
-template <typename T> struct Chunk;
-template <> struct Chunk<float> { v4f a, b; };
-template <> struct Chunk<Bf16> { v4u a; };
-__device__ __forceinline__ void chunk_load(Chunk<float> &c, const float *p) { c.a = *gmem((const v4f *)p); c.b = *gmem((const v4f *)(p + 4)); }
-__device__ __forceinline__ void chunk_load(Chunk<Bf16> &c, const Bf16 *p) { c.a = *gmem((const v4u *)p); }
-__device__ __forceinline__ void chunk_zero(Chunk<float> &c) { c.a = c.b = (v4f){0, 0, 0, 0}; }
-__device__ __forceinline__ void chunk_zero(Chunk<Bf16> &c) { c.a = (v4u){0, 0, 0, 0}; }
-// zeros in place of values that are not finite; whether there were any
-__device__ __forceinline__ bool chunk_clean(Chunk<float> &c) {
-    bool bad = false;
-    #pragma unroll
-    for (int k = 0; k < 4; k++) {
-        const bool x = !pieces_hold(c.a[k]), y = !pieces_hold(c.b[k]);
-        bad |= x | y;
-        c.a[k] = x ? 0.0f : c.a[k]; c.b[k] = y ? 0.0f : c.b[k];
-    }
-    return bad;
-}
 __device__ __forceinline__ bool bf16_finite(uint32_t u) { return (u & 0x7F80) != 0x7F80; }
-__device__ __forceinline__ bool chunk_clean(Chunk<Bf16> &c) {
+// zeros in place of values that are not finite; whether there were any
+__device__ __forceinline__ bool chunk_clean(v4u &c) {
     bool bad = false;
     #pragma unroll
     for (int k = 0; k < 4; k++) {
-        const bool x = !bf16_finite(c.a[k]), y = !bf16_finite(c.a[k] >> 16);
+        const bool x = !bf16_finite(c[k]), y = !bf16_finite(c[k] >> 16);
         bad |= x | y;
-        c.a[k] &= (x ? 0xFFFF0000u : ~0u) & (y ? 0xFFFFu : ~0u);
+        c[k] &= (x ? 0xFFFF0000u : ~0u) & (y ? 0xFFFFu : ~0u);
     }
     return bad;
 }
-__device__ __forceinline__ void chunk_pieces(const Chunk<float> &c, bf8 (&p)[3]) {
-    const Pieces x = pieces_of([&](int k) { return k < 4 ? c.a[k & 3] : c.b[k & 3]; });
-    p[0] = x.p[0]; p[1] = x.p[1]; p[2] = x.p[2];
-}
-__device__ __forceinline__ void chunk_pieces(const Chunk<Bf16> &c, bf8 (&p)[1]) { p[0] = __builtin_bit_cast(bf8, c.a); }
-
-template <typename T, int HD>
-__global__ __launch_bounds__(256, (PromptShape<T, HD>::WPS)) void k_prompt(sp_hipkv_prompt_args a, int slots) {
-    using P = PromptShape<T, HD>;
-    constexpr int NP = P::NP, BN = P::BN, QT = P::QT, BM = P::BM, KT = BN / 32, DT = HD / 32, C8 = HD / 8, NC = BN * C8 / 256;
-    constexpr int NMUL = NP == 3 ? 6 : 1;
-    __shared__ __align__(1024) bf8 s_k[NP * BN * C8], s_v[NP * BN * C8];
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), l32 = lane & 31, half = lane >> 5;
-    const int G = a.n_heads / a.n_kv_heads, h = blockIdx.x % a.n_kv_heads;
-    // the longest spans first: a sequence's last rows before its first
-    const int slot = slots - 1 - blockIdx.x / a.n_kv_heads;
-    const int s = unit_seq(a.start, a.n_seqs, slot, G, BM, 1);
-    const int t0 = max(gmem(a.start)[s], 0), n = min(min(gmem(a.start)[s + 1], a.n_tokens) - t0, a.max_tokens);
-    const int64_t j = slot - unit_base(a.start, s, G, BM, 1);
-    if (n <= 0 || j < 0 || j * BM >= (int64_t)n * G) return;
-    const int R = n * G, r0 = (int)j * BM, wr0 = r0 + wave * 32 * QT;
-    // tokens of the workgroup and of this wave, and the keys that they attend
-    const int W = a.window ? a.window : INT32_MAX;
-    const int first = r0 / G, last = (min(r0 + BM, R) - 1) / G, w_first = min(wr0, R - 1) / G, w_last = (min(wr0 + 32 * QT, R) - 1) / G;
-    const int k0 = max(first - W + 1, 0) / BN, k1 = last / BN + 1;
-    // scale <= 0 goes into q's sign (or makes q zero), so that larger scores have larger weights
-    const float sgn = a.scale > 0 ? 1.0f : a.scale < 0 ? -1.0f : 0.0f, c = a.scale == 0 ? LOG2E_F : fabsf(a.scale) * LOG2E_F, slack = SLACK / c;
-    int tok[QT];
-    bf8 Q[QT][HD / 16][NP];
-    #pragma unroll
-    for (int t = 0; t < QT; t++) {
-        const int r = min(wr0 + t * 32 + l32, R - 1);
-        tok[t] = r / G;
-        const T *q = (const T *)a.q + (size_t)(t0 + tok[t]) * a.q_stride + (size_t)(h * G + r % G) * HD + 8 * half;
-        #pragma unroll
-        for (int k = 0; k < HD / 16; k++) {
-            float x[8];
-            load_values(q + 16 * k, x);
-            Chunk<float> f = {{x[0] * sgn, x[1] * sgn, x[2] * sgn, x[3] * sgn}, {x[4] * sgn, x[5] * sgn, x[6] * sgn, x[7] * sgn}};
-            if constexpr (NP == 3) chunk_pieces(f, Q[t][k]);
-            else {
-                Chunk<Bf16> b = {{bf16x2(f.a[0], f.a[1]), bf16x2(f.a[2], f.a[3]), bf16x2(f.b[0], f.b[1]), bf16x2(f.b[2], f.b[3])}};
-                chunk_pieces(b, Q[t][k]);
-            }
-        }
-    }
-    // A row's 16-byte chunks lie in an order that spreads a column of K over the banks, and
-    // the 64-byte runs of four rows of V
-    auto k_at = [](int row, int ch) { return row * C8 + (HD == 64 ? ch ^ (row >> 1 & 7) : ch ^ (row & 15)); };
-    auto v_at = [](int row, int ch) { return row * C8 + (HD == 64 ? ch ^ (row >> 1 & 1) << 2 : ch ^ (row & 3) << 2); };
-    const T *kp = (const T *)a.k + (size_t)t0 * a.k_stride + (size_t)h * HD, *vp = (const T *)a.v + (size_t)t0 * a.v_stride + (size_t)h * HD;
-    Chunk<T> ck[NC], cv[NC];
-    auto load = [&](int tile) {
-        #pragma unroll
-        for (int k = 0; k < NC; k++) {
-            const int id = threadIdx.x + 256 * k, row = tile * BN + id / C8, ch = id % C8;
-            if (row < n) {
-                chunk_load(ck[k], kp + (size_t)row * a.k_stride + 8 * ch);
-                chunk_load(cv[k], vp + (size_t)row * a.v_stride + 8 * ch);
-            } else { chunk_zero(ck[k]); chunk_zero(cv[k]); }
-        }
-    };
-    auto put = [&](bool clean) {
-        bool bad = false;
-        #pragma unroll
-        for (int k = 0; k < NC; k++) {
-            const int id = threadIdx.x + 256 * k, row = id / C8, ch = id % C8;
-            bf8 p[NP];
-            chunk_pieces(ck[k], p);
-            #pragma unroll
-            for (int e = 0; e < NP; e++) s_k[e * BN * C8 + k_at(row, ch)] = p[e];
-            if (clean) bad |= chunk_clean(cv[k]);
-            chunk_pieces(cv[k], p);
-            #pragma unroll
-            for (int e = 0; e < NP; e++) s_v[e * BN * C8 + v_at(row, ch)] = p[e];
-        }
-        return bad;
-    };
-    v16f O[QT][DT];
-    float m[QT], l[QT];
-    #pragma unroll
-    for (int t = 0; t < QT; t++) {
-        m[t] = -INFINITY; l[t] = 0.0f;
-        #pragma unroll
-        for (int d = 0; d < DT; d++)
-            #pragma unroll
-            for (int i = 0; i < 16; i++) O[t][d][i] = 0.0f;
-    }
-    // this lane's address for the transposing reads: row (l % 16) / 4 of four, 4 columns of 16
-    const int v_row = 4 * half + (lane & 15) / 4, v_col = 16 * (lane >> 4 & 1) + 4 * (lane & 3);
-    load(k0);
-    for (int tile = k0; tile < k1; tile++) {
-        const int key0 = tile * BN;
-        const bool ragged = key0 + BN - 1 > first || key0 < last - W + 1;               // some row does not attend it whole
-        const bool flag = put(ragged);
-        bool odd = false;
-        if (ragged) odd = __syncthreads_or(flag); else __syncthreads();
-        if (tile + 1 < k1) load(tile + 1);
-        if (wr0 < R && key0 <= w_last && key0 + BN > w_first - W + 1) {
-            const bool w_ragged = key0 + BN - 1 > w_first || key0 < w_last - W + 1;
-            v16f S[QT][KT];
-            #pragma unroll
-            for (int t = 0; t < QT; t++)
-                #pragma unroll
-                for (int u = 0; u < KT; u++)
-                    #pragma unroll
-                    for (int i = 0; i < 16; i++) S[t][u][i] = 0.0f;
-            #pragma unroll
-            for (int k = 0; k < HD / 16; k++)
-                #pragma unroll
-                for (int u = 0; u < KT; u++) {
-                    bf8 A[NP];
-                    #pragma unroll
-                    for (int e = 0; e < NP; e++) A[e] = s_k[e * BN * C8 + k_at(u * 32 + l32, 2 * k + half)];
-                    #pragma unroll
-                    for (int t = 0; t < QT; t++)
-                        #pragma unroll
-                        for (int x = 6 - NMUL; x < 6; x++) S[t][u] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(A[MUL_A[x]], Q[t][k][MUL_B[x]], S[t][u], 0, 0, 0);
-                }
-            bf8 Pw[QT][KT][2][NP];
-            #pragma unroll
-            for (int t = 0; t < QT; t++) {
-                if (w_ragged) {
-                    #pragma unroll
-                    for (int u = 0; u < KT; u++)
-                        #pragma unroll
-                        for (int i = 0; i < 16; i++) {
-                            const int key = key0 + u * 32 + 8 * (i / 4) + 4 * half + i % 4;
-                            S[t][u][i] = key <= tok[t] && key > tok[t] - W ? S[t][u][i] : -INFINITY;
-                        }
-                }
-                float mx = S[t][0][0];
-                #pragma unroll
-                for (int u = 0; u < KT; u++)
-                    #pragma unroll
-                    for (int i = 0; i < 16; i++) mx = fmaxf(mx, S[t][u][i]);
-                if (__any(mx > m[t] + slack)) {
-                    mx = fmaxf(mx, other_half(mx));
-                    const float mn = fmaxf(m[t], mx), al = mn == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f((m[t] - mn) * c);
-                    m[t] = mn;
-                    l[t] *= al;
-                    #pragma unroll
-                    for (int d = 0; d < DT; d++)
-                        #pragma unroll
-                        for (int i = 0; i < 16; i++) O[t][d][i] *= al;
-                }
-                const float nm = m[t] == -INFINITY ? 0.0f : -m[t] * c;
-                #pragma unroll
-                for (int u = 0; u < KT; u++)
-                    #pragma unroll
-                    for (int e = 0; e < 2; e++) {
-                        float w[8];
-                        #pragma unroll
-                        for (int i = 0; i < 8; i++) {
-                            w[i] = __builtin_amdgcn_exp2f(fmaf(S[t][u][8 * e + i], c, nm));
-                            l[t] += w[i];
-                        }
-                        if constexpr (NP == 3) {
-                            const Pieces x = pieces_of([&](int k) { return w[k]; });
-                            Pw[t][u][e][0] = x.p[0]; Pw[t][u][e][1] = x.p[1]; Pw[t][u][e][2] = x.p[2];
-                        } else Pw[t][u][e][0] = __builtin_bit_cast(bf8, (v4u){bf16x2(w[0], w[1]), bf16x2(w[2], w[3]), bf16x2(w[4], w[5]), bf16x2(w[6], w[7])});
-                    }
-            }
-            #pragma unroll
-            for (int d = 0; d < DT; d++)
-                #pragma unroll
-                for (int u = 0; u < KT; u++)
-                    #pragma unroll
-                    for (int e = 0; e < 2; e++) {
-                        bf8 A[NP];
-                        #pragma unroll
-                        for (int x = 0; x < NP; x++) {
-                            v4s y[2];
-                            #pragma unroll
-                            for (int z = 0; z < 2; z++) {
-                                const int row = u * 32 + 16 * e + 8 * z + v_row, col = d * 32 + v_col;
-                                y[z] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4s *)((uint8_t *)(s_v + x * BN * C8 + v_at(row, col / 8)) + col % 8 * 2));
-                            }
-                            typedef short v8s __attribute__((ext_vector_type(8)));
-                            A[x] = __builtin_bit_cast(bf8, __builtin_shufflevector(y[0], y[1], 0, 1, 2, 3, 4, 5, 6, 7));
-                        }
-                        #pragma unroll
-                        for (int t = 0; t < QT; t++)
-                            #pragma unroll
-                            for (int x = 6 - NMUL; x < 6; x++) O[t][d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(A[MUL_A[x]], Pw[t][u][e][MUL_B[x]], O[t][d], 0, 0, 0);
-                    }
-            if (odd) {                                                      // V values that were left out, for the rows that attend them
-                #pragma unroll 1
-                for (int key = key0; key < min(key0 + BN, n); key++) {
-                    const T *row = vp + (size_t)key * a.v_stride + 4 * half;
-                    #pragma unroll
-                    for (int d = 0; d < DT; d++)
-                        #pragma unroll
-                        for (int i = 0; i < 16; i += 4) {
-                            float x[4];
-                            load_values(row + d * 32 + 2 * i, x);
-                            #pragma unroll
-                            for (int t = 0; t < QT; t++)
-                                #pragma unroll
-                                for (int y = 0; y < 4; y++) O[t][d][i + y] += key <= tok[t] && key > tok[t] - W && !pieces_hold(x[y]) ? x[y] * INFINITY : 0.0f;
-                        }
-                }
-            }
-        }
-        __syncthreads();
-    }
-    #pragma unroll
-    for (int t = 0; t < QT; t++) {
-        const int r = wr0 + t * 32 + l32;
-        const float inv = 1.0f / (l[t] + other_half(l[t]));
-        if (r >= R) continue;
-        T *o = (T *)a.out + (size_t)(t0 + tok[t]) * a.out_stride + (size_t)(h * G + r % G) * HD + 4 * half;
-        #pragma unroll
-        for (int d = 0; d < DT; d++)
-            #pragma unroll
-            for (int i = 0; i < 16; i += 4) {
-                float x[4];
-                #pragma unroll
-                for (int y = 0; y < 4; y++) x[y] = O[t][d][i + y] * inv;
-                store_values(o + d * 32 + 2 * i, x);
-            }
-    }
-}
+__device__ __forceinline__ bool finite32(float x) { return (__float_as_uint(x) & 0x7F800000u) != 0x7F800000u; }
 
 // ---------------------------------------------------------------- bf16
 // K and V come through LDS by direct loads, two tiles deep, with one barrier a tile.
@@ -379,7 +134,7 @@ __global__ __launch_bounds__(64 * NW, HD == 256 ? 1 : 2) void k_prompt16(sp_hipk
                     float x[4];
                     load_values(vrow + d * 32 + 2 * i, x);
                     #pragma unroll
-                    for (int y = 0; y < 4; y++) O[d][i + y] += key <= tok && key > tok - W && !pieces_hold(x[y]) ? x[y] * INFINITY : 0.0f;
+                    for (int y = 0; y < 4; y++) O[d][i + y] += key <= tok && key > tok - W && !finite32(x[y]) ? x[y] * INFINITY : 0.0f;
                 }
         }
     };
@@ -388,8 +143,8 @@ __global__ __launch_bounds__(64 * NW, HD == 256 ? 1 : 2) void k_prompt16(sp_hipk
         bool bad = false;
         #pragma unroll
         for (int i = 0; i < NI; i++) {
-            Chunk<Bf16> x = {((v4u *)lds)[threadIdx.x + 64 * NW * i]};
-            if (chunk_clean(x)) { bad = true; ((v4u *)lds)[threadIdx.x + 64 * NW * i] = x.a; }
+            v4u x = ((v4u *)lds)[threadIdx.x + 64 * NW * i];
+            if (chunk_clean(x)) { bad = true; ((v4u *)lds)[threadIdx.x + 64 * NW * i] = x; }
         }
         return bad;
     };
@@ -492,6 +247,274 @@ __global__ __launch_bounds__(64 * NW, HD == 256 ? 1 : 2) void k_prompt16(sp_hipk
         }
 }
 
+// ---------------------------------------------------------------- f32
+// An f32 as two f16: h, its rounding, and l, that of what is left, of values times the power of two
+// that brings their row's largest below 2^15: x = h + l but for 2^-22 of itself, or 2^-40 of the largest.
+typedef _Float16 h2 __attribute__((ext_vector_type(2)));
+typedef _Float16 h8 __attribute__((ext_vector_type(8)));
+struct Halves { h8 h, l; };
+template <typename X> __device__ __forceinline__ Halves halves_of(X &&x) {                 // of x(0) .. x(7)
+    v4u h, l;
+    #pragma unroll
+    for (int k = 0; k < 4; k++) {
+        const float a = x(2 * k), b = x(2 * k + 1);
+        const h2 y = __builtin_convertvector((v2f){a, b}, h2);
+        h[k] = __builtin_bit_cast(uint32_t, y);
+        l[k] = __builtin_bit_cast(uint32_t, __builtin_convertvector((v2f){fmaf((float)y[0], -1.0f, a), fmaf((float)y[1], -1.0f, b)}, h2));
+    }
+    return {__builtin_bit_cast(h8, h), __builtin_bit_cast(h8, l)};
+}
+// of a row's largest magnitude the exponent e, and of that the factor 2^(141 - e) and its inverse
+__device__ __forceinline__ uint32_t row_exp(float big) { return min(max(__float_as_uint(big) >> 23, 16u), 254u); }
+__device__ __forceinline__ float row_up(uint32_t e) { return __uint_as_float((268u - e) << 23); }
+__device__ __forceinline__ float row_down(uint32_t e) { return __uint_as_float((e - 14u) << 23); }
+// the largest over N = 8, 16 or 32 neighbouring lanes
+template <int N> __device__ __forceinline__ float lanes_max(float x) {
+    auto step = [&](auto ctrl) { x = fmaxf(x, __uint_as_float(dpp32<decltype(ctrl)::value, 0xF>(__float_as_uint(x), 0))); };
+    step(std::integral_constant<int, 0xB1>{});                            // quad_perm 1,0,3,2
+    step(std::integral_constant<int, 0x4E>{});                            // quad_perm 2,3,0,1
+    step(std::integral_constant<int, 0x141>{});                           // row_half_mirror
+    if constexpr (N > 8) step(std::integral_constant<int, 0x140>{});      // row_mirror
+    if constexpr (N > 16) x = fmaxf(x, __shfl_xor(x, 16, 64));
+    return x;
+}
+__device__ __forceinline__ float abs_max(const v4f &a, const v4f &b) {
+    return fmaxf(fmaxf(fmaxf(fabsf(a[0]), fabsf(a[1])), fmaxf(fabsf(a[2]), fabsf(a[3]))), fmaxf(fmaxf(fabsf(b[0]), fabsf(b[1])), fmaxf(fabsf(b[2]), fabsf(b[3]))));
+}
+__device__ __forceinline__ v16f mfma_halves(const Halves &a, const Halves &b, v16f c) {
+    c = __builtin_amdgcn_mfma_f32_32x32x16_f16(a.l, b.h, c, 0, 0, 0);
+    c = __builtin_amdgcn_mfma_f32_32x32x16_f16(a.h, b.l, c, 0, 0, 0);
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(a.h, b.h, c, 0, 0, 0);
+}
+
+// A tile of 32 keys comes into LDS as it is, by direct loads, while the one before is worked on, and is
+// taken apart by all threads: rows of K and of V each by a factor of their own, whose inverses join the
+// scores and, relative to the largest so far (as with the scores' maximum, the output is scaled when it
+// moves), the weights.
+template <int HD, int NW>
+__global__ __launch_bounds__(64 * NW, HD == 256 ? 1 : 2) void k_prompt32(sp_hipkv_prompt_args a, int slots) {
+    constexpr int BN = 32, BM = 32 * NW, KS = HD / 16, DT = HD / 32, C8 = HD / 8, RAW = BN * HD * 4, PIECE = BN * HD * 2, NC = BN * C8 / (64 * NW);
+    constexpr float SLACK32 = 8.0f;                                       // weights times 2^7 are f16 numbers
+    __shared__ __align__(1024) uint8_t raw[2 * RAW], lds[4 * PIECE];      // K, V; K's h and l, V's h and l
+    __shared__ __align__(16) float s_kf[BN], s_vf[NW][BN];
+    __shared__ uint32_t s_ve[BN];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), l32 = lane & 31, half = lane >> 5;
+    const int G = a.n_heads / a.n_kv_heads, h = blockIdx.x % a.n_kv_heads;
+    // the longest spans first: a sequence's last rows before its first
+    const int slot = slots - 1 - blockIdx.x / a.n_kv_heads;
+    const int s = unit_seq(a.start, a.n_seqs, slot, G, BM, 1);
+    const int t0 = max(gmem(a.start)[s], 0), n = min(min(gmem(a.start)[s + 1], a.n_tokens) - t0, a.max_tokens);
+    const int64_t j = slot - unit_base(a.start, s, G, BM, 1);
+    if (n <= 0 || j < 0 || j * BM >= (int64_t)n * G) return;
+    const int R = n * G, r0 = (int)j * BM, wr0 = r0 + wave * 32;
+    const int W = a.window ? a.window : INT32_MAX;
+    const int first = r0 / G, last = (min(r0 + BM, R) - 1) / G, w_first = min(wr0, R - 1) / G, w_last = (min(wr0 + 32, R) - 1) / G;
+    const int k0 = max(first - W + 1, 0) / BN, k1 = last / BN + 1;
+    const float *kp = (const float *)a.k + (size_t)t0 * a.k_stride + (size_t)h * HD, *vp = (const float *)a.v + (size_t)t0 * a.v_stride + (size_t)h * HD;
+    constexpr int NI = RAW / 1024 / NW;                                   // loads of a wave for a tile
+    int ko[NI], vo[NI];
+    #pragma unroll
+    for (int i = 0; i < NI; i++) {
+        const int at = (wave * NI + i) * 256 + lane * 4;
+        ko[i] = (at / HD * (int)a.k_stride + at % HD) * 4;
+        vo[i] = (at / HD * (int)a.v_stride + at % HD) * 4;
+    }
+    const uint32_t raw0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) const uint8_t *)raw + wave * NI * 1024;
+    auto load = [&](const float *p, int64_t stride, const int (&off)[NI], int tile, int to) __attribute__((always_inline)) {
+        const int rows = min(n - tile * BN, BN);
+        const v4i rs = rsrc_of(p + (int64_t)tile * BN * stride, rows > 0 ? (uint32_t)((rows - 1) * (int)stride + HD) * 4 : 0);
+        #pragma unroll
+        for (int i = 0; i < NI; i++) dma16(raw0 + to + i * 1024, off[i], rs);
+    };
+    load(kp, a.k_stride, ko, k0, 0);
+    load(vp, a.v_stride, vo, k0, RAW);
+    // q's halves; its factor joins that of the scores, c >= 0 (scale <= 0 goes into q's sign, or makes q zero)
+    const float sgn = a.scale > 0 ? 1.0f : a.scale < 0 ? -1.0f : 0.0f;
+    const int row = min(wr0 + l32, R - 1), tok = row / G;
+    Halves Q[KS];
+    float c;
+    {
+        const float *q = (const float *)a.q + (size_t)(t0 + tok) * a.q_stride + (size_t)(h * G + row % G) * HD + 8 * half;
+        float x[8];
+        float big = 0.0f;                                                  // (a NaN makes its own way into the scores)
+        #pragma unroll
+        for (int k = 0; k < KS; k++) {
+            load_values(q + 16 * k, x);
+            #pragma unroll
+            for (int i = 0; i < 8; i++) big = fmaxf(big, fabsf(x[i]));
+        }
+        asm volatile("" : : : "memory");                                  // read again, not kept: KS x 8 registers
+        big = fmaxf(big, other_half(big));
+        const uint32_t e = row_exp(big);
+        const float up = sgn * row_up(e);
+        c = (a.scale == 0 ? LOG2E_F : fabsf(a.scale) * LOG2E_F) * row_down(e);
+        #pragma unroll
+        for (int k = 0; k < KS; k++) {
+            load_values(q + 16 * k, x);
+            Q[k] = halves_of([&](int i) { return x[i] * up; });
+        }
+    }
+    const float slack = SLACK32 / c;
+    v16f O[DT];
+    const v16f zero = {0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0};
+    #pragma unroll
+    for (int d = 0; d < DT; d++) O[d] = zero;
+    float m = -INFINITY, l = 0.0f;
+    uint32_t E = 16;                                                       // the exponent that O is relative to
+    // A row's 16-byte chunks lie in an order that spreads a column of K over the banks, and
+    // the 64-byte runs of four rows of V
+    auto k_swz = [](int r) { return HD == 64 ? r >> 1 & 7 : r & 15; };
+    auto v_swz = [](int r) { return HD == 64 ? (r >> 1 & 1) << 2 : (r & 3) << 2; };
+    int k_at[KS], v_at[DT];
+    #pragma unroll
+    for (int k = 0; k < KS; k++) k_at[k] = (l32 * C8 + ((2 * k + half) ^ k_swz(l32))) * 16;
+    #pragma unroll
+    for (int d = 0; d < DT; d++) {
+        const int r = 4 * half + (lane & 15) / 4, col = d * 32 + 16 * (lane >> 4 & 1) + 4 * (lane & 3);
+        v_at[d] = (r * C8 + ((col / 8) ^ v_swz(r))) * 16 + col % 8 * 2;
+    }
+    for (int tile = k0; tile < k1; tile++) {
+        const bool ragged = tile * BN + BN - 1 > first || tile * BN < last - W + 1;        // some row does not attend it whole
+        asm volatile("s_waitcnt vmcnt(0)" : : : "memory");
+        __syncthreads();
+        bool bad = false;
+        #pragma unroll
+        for (int i = 0; i < NC; i++) {
+            const int id = threadIdx.x + 64 * NW * i, r = id / C8, ch = id % C8;
+            const v4f x0 = *(const v4f *)(raw + id * 32), x1 = *(const v4f *)(raw + id * 32 + 16);
+            v4f y0 = *(const v4f *)(raw + RAW + id * 32), y1 = *(const v4f *)(raw + RAW + id * 32 + 16);
+            float kb = abs_max(x0, x1), vb = abs_max(y0, y1);
+            if (ragged || __any(vb == INFINITY)) {                         // a row of V has the factor of its finite values
+                vb = 0.0f;
+                #pragma unroll
+                for (int k = 0; k < 4; k++) {
+                    const bool f0 = finite32(y0[k]), f1 = finite32(y1[k]);
+                    vb = fmaxf(vb, fmaxf(f0 ? fabsf(y0[k]) : 0.0f, f1 ? fabsf(y1[k]) : 0.0f));
+                    if (ragged) {
+                        bad |= !f0 | !f1;
+                        y0[k] = f0 ? y0[k] : 0.0f; y1[k] = f1 ? y1[k] : 0.0f;
+                    }
+                }
+            }
+            const uint32_t ke = row_exp(lanes_max<C8>(kb)), ve = row_exp(lanes_max<C8>(vb));
+            const float ku = row_up(ke), vu = row_up(ve);
+            if (ch == 0) { s_kf[r] = row_down(ke); s_ve[r] = ve; }
+            // (an infinity in K becomes h = inf, l = NaN)
+            const Halves K = halves_of([&](int k) { return (k < 4 ? x0[k & 3] : x1[k & 3]) * ku; });
+            const Halves V = halves_of([&](int k) { return (k < 4 ? y0[k & 3] : y1[k & 3]) * vu; });
+            h8 *kd = (h8 *)lds + r * C8 + (ch ^ k_swz(r)), *vd = (h8 *)(lds + 2 * PIECE) + r * C8 + (ch ^ v_swz(r));
+            kd[0] = K.h; kd[PIECE / 16] = K.l;
+            vd[0] = V.h; vd[PIECE / 16] = V.l;
+        }
+        bool odd = false;
+        if (ragged) odd = __syncthreads_or(bad); else __syncthreads();
+        if (tile + 1 < k1) {
+            load(kp, a.k_stride, ko, tile + 1, 0);
+            load(vp, a.v_stride, vo, tile + 1, RAW);
+        }
+        if (tile * BN > w_last || tile * BN + BN <= w_first - W + 1) continue;             // no row of this wave attends any
+        const uint32_t ve = s_ve[l32], top = (uint32_t)wave_allmax_i((int)ve);
+        v16f S = zero;
+        #pragma unroll
+        for (int k = 0; k < KS; k++) S = mfma_halves(Halves{*(const h8 *)(lds + k_at[k]), *(const h8 *)(lds + k_at[k] + PIECE)}, Q[k], S);
+        // this lane's keys: 8 (i / 4) + 4 half + i % 4
+        #pragma unroll
+        for (int i = 0; i < 16; i += 4) {
+            const v4f x = *(const v4f *)(s_kf + 2 * i + 4 * half);
+            #pragma unroll
+            for (int k = 0; k < 4; k++) S[i + k] *= x[k];
+        }
+        if (tile * BN + BN - 1 > w_first || tile * BN < w_last - W + 1) {
+            #pragma unroll
+            for (int i = 0; i < 16; i++) {
+                const int key = tile * BN + 8 * (i / 4) + 4 * half + i % 4;
+                S[i] = key <= tok && key > tok - W ? S[i] : -INFINITY;
+            }
+        }
+        float mx = S[0];
+        #pragma unroll
+        for (int i = 1; i < 16; i++) mx = fmaxf(mx, S[i]);
+        if (__builtin_expect(__any(mx > m + slack), 0)) {
+            mx = fmaxf(mx, other_half(mx));
+            const float mn = fmaxf(m, mx), al = mn == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f((m - mn) * c);
+            m = mn;
+            l *= al;
+            #pragma unroll
+            for (int d = 0; d < DT; d++)
+                #pragma unroll
+                for (int i = 0; i < 16; i++) O[d][i] *= al;
+        }
+        const float nm = m == -INFINITY ? 0.0f : -m * c;
+        #pragma unroll
+        for (int i = 0; i < 16; i++) {
+            S[i] = __builtin_amdgcn_exp2f(fmaf(S[i], c, nm));
+            l += S[i];
+        }
+        if (top > E) {
+            const float f = E + 126 < top ? 0.0f : __uint_as_float((127u + E - top) << 23);
+            E = top;
+            #pragma unroll
+            for (int d = 0; d < DT; d++)
+                #pragma unroll
+                for (int i = 0; i < 16; i++) O[d][i] *= f;
+        }
+        // the keys' factors relative to E, 2^(7 + ve - E), each formed by one lane
+        s_vf[wave][l32] = ve + 126 < E ? 0.0f : __uint_as_float((134u + ve - E) << 23);
+        __builtin_amdgcn_wave_barrier();
+        #pragma unroll
+        for (int i = 0; i < 16; i += 4) {
+            const v4f x = *(const v4f *)(s_vf[wave] + 2 * i + 4 * half);
+            #pragma unroll
+            for (int k = 0; k < 4; k++) S[i + k] *= x[k];
+        }
+        Halves P[2];
+        #pragma unroll
+        for (int e = 0; e < 2; e++) P[e] = halves_of([&](int k) { return S[8 * e + k]; });
+        #pragma unroll
+        for (int e = 0; e < 2; e++)
+            #pragma unroll
+            for (int d = 0; d < DT; d++) {
+                typedef short v8s __attribute__((ext_vector_type(8)));
+                h8 V[2];
+                #pragma unroll
+                for (int x = 0; x < 2; x++) {
+                    const uint8_t *at = lds + v_at[d] + (2 + x) * PIECE + 16 * e * HD * 2;
+                    const v4s y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4s *)at), z = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4s *)(at + 8 * HD * 2));
+                    V[x] = __builtin_bit_cast(h8, __builtin_shufflevector(y, z, 0, 1, 2, 3, 4, 5, 6, 7));
+                }
+                O[d] = mfma_halves(Halves{V[0], V[1]}, P[e], O[d]);
+            }
+        if (odd) {                                                          // V values that were left out, for the rows that attend them
+            #pragma unroll 1
+            for (int key = tile * BN; key < min(tile * BN + BN, n); key++) {
+                const float *vrow = vp + (size_t)key * a.v_stride + 4 * half;
+                #pragma unroll
+                for (int d = 0; d < DT; d++)
+                    #pragma unroll
+                    for (int i = 0; i < 16; i += 4) {
+                        float x[4];
+                        load_values(vrow + d * 32 + 2 * i, x);
+                        #pragma unroll
+                        for (int y = 0; y < 4; y++) O[d][i + y] += key <= tok && key > tok - W && !finite32(x[y]) ? x[y] * INFINITY : 0.0f;
+                    }
+            }
+        }
+    }
+    const int r = wr0 + l32;
+    const float inv = ldexpf(1.0f / (l + other_half(l)), (int)E - 148);
+    if (r >= R) return;
+    float *o = (float *)a.out + (size_t)(t0 + tok) * a.out_stride + (size_t)(h * G + r % G) * HD + 4 * half;
+    #pragma unroll
+    for (int d = 0; d < DT; d++)
+        #pragma unroll
+        for (int i = 0; i < 16; i += 4) {
+            float x[4];
+            #pragma unroll
+            for (int y = 0; y < 4; y++) x[y] = O[d][i + y] * inv;
+            store_values(o + d * 32 + 2 * i, x);
+        }
+}
+
 int prompt_check(const sp_hipkv_prompt_args *a) {
     const char *who = "sp_hipkv_prompt_attention";
     if (serve_check(who, a)) return 1;
@@ -504,13 +527,11 @@ int prompt_check(const sp_hipkv_prompt_args *a) {
 }
 
 template <typename T, int HD> hipError_t prompt_go(const sp_hipkv_prompt_args &a, hipStream_t s) {
-    if constexpr (sizeof(T) == 2) {
-        constexpr int NW = 4;
-        const int slots = (int)((int64_t)a.n_tokens * (a.n_heads / a.n_kv_heads) / (32 * NW)) + a.n_seqs;
-        return op_launch(k_prompt16<HD, NW>, dim3((uint32_t)((int64_t)slots * a.n_kv_heads)), dim3(64 * NW), s, a, slots);
-    }
-    const int slots = (int)((int64_t)a.n_tokens * (a.n_heads / a.n_kv_heads) / PromptShape<T, HD>::BM) + a.n_seqs;
-    return op_launch(k_prompt<T, HD>, dim3((uint32_t)((int64_t)slots * a.n_kv_heads)), dim3(256), s, a, slots);
+    constexpr int NW = 4;
+    const int slots = (int)((int64_t)a.n_tokens * (a.n_heads / a.n_kv_heads) / (32 * NW)) + a.n_seqs;
+    const dim3 grid((uint32_t)((int64_t)slots * a.n_kv_heads)), wg(64 * NW);
+    if constexpr (sizeof(T) == 4) return op_launch(k_prompt32<HD, NW>, grid, wg, s, a, slots);
+    else return op_launch(k_prompt16<HD, NW>, grid, wg, s, a, slots);
 }
 template <typename T> hipError_t prompt_type(const sp_hipkv_prompt_args &a, hipStream_t s) {
     return a.head_dim == 256 ? prompt_go<T, 256>(a, s) : a.head_dim == 128 ? prompt_go<T, 128>(a, s) : prompt_go<T, 64>(a, s);
