@@ -291,9 +291,14 @@ __device__ __forceinline__ v16f mfma_halves(const Halves &a, const Halves &b, v1
 // taken apart by all threads: rows of K and of V each by a factor of their own, whose inverses join the
 // scores and, relative to the largest so far (as with the scores' maximum, the output is scaled when it
 // moves), the weights.
+//
+// Dims of 256 are shared by two waves, each 128 of the scores' products and of the output's columns,
+// who hand each other their parts of the scores through LDS, where K lay as it came (the next K is
+// sent for after that): one wave with all of them needs over 256 registers, so that a SIMD has no other
+// to work while it waits (2047 tokens with a window of 1024: 200 us).
 template <int HD, int NW>
-__global__ __launch_bounds__(64 * NW, HD == 256 ? 1 : 2) void k_prompt32(sp_hipkv_prompt_args a, int slots) {
-    constexpr int BN = 32, BM = 32 * NW, KS = HD / 16, DT = HD / 32, C8 = HD / 8, RAW = BN * HD * 4, PIECE = BN * HD * 2, NC = BN * C8 / (64 * NW);
+__global__ __launch_bounds__(64 * NW, 2) void k_prompt32(sp_hipkv_prompt_args a, int slots) {
+    constexpr int BN = 32, SPLIT = HD == 256 ? 2 : 1, RG = NW / SPLIT, BM = 32 * RG, KS = HD / SPLIT / 16, DT = HD / SPLIT / 32, C8 = HD / 8, RAW = BN * HD * 4, PIECE = BN * HD * 2, NC = BN * C8 / (64 * NW);
     constexpr float SLACK32 = 8.0f;                                       // weights times 2^7 are f16 numbers
     __shared__ __align__(1024) uint8_t raw[2 * RAW], lds[4 * PIECE];      // K, V; K's h and l, V's h and l
     __shared__ __align__(16) float s_kf[BN], s_vf[NW][BN];
@@ -306,7 +311,7 @@ __global__ __launch_bounds__(64 * NW, HD == 256 ? 1 : 2) void k_prompt32(sp_hipk
     const int t0 = max(gmem(a.start)[s], 0), n = min(min(gmem(a.start)[s + 1], a.n_tokens) - t0, a.max_tokens);
     const int64_t j = slot - unit_base(a.start, s, G, BM, 1);
     if (n <= 0 || j < 0 || j * BM >= (int64_t)n * G) return;
-    const int R = n * G, r0 = (int)j * BM, wr0 = r0 + wave * 32;
+    const int R = n * G, r0 = (int)j * BM, wr0 = r0 + wave % RG * 32, dim0 = wave / RG * (HD / SPLIT);            // this wave's rows and dims
     const int W = a.window ? a.window : INT32_MAX;
     const int first = r0 / G, last = (min(r0 + BM, R) - 1) / G, w_first = min(wr0, R - 1) / G, w_last = (min(wr0 + 32, R) - 1) / G;
     const int k0 = max(first - W + 1, 0) / BN, k1 = last / BN + 1;
@@ -334,7 +339,7 @@ __global__ __launch_bounds__(64 * NW, HD == 256 ? 1 : 2) void k_prompt32(sp_hipk
     Halves Q[KS];
     float c;
     {
-        const float *q = (const float *)a.q + (size_t)(t0 + tok) * a.q_stride + (size_t)(h * G + row % G) * HD + 8 * half;
+        const float *q = (const float *)a.q + (size_t)(t0 + tok) * a.q_stride + (size_t)(h * G + row % G) * HD + dim0 + 8 * half;
         float x[8];
         float big = 0.0f;                                                  // (a NaN makes its own way into the scores)
         #pragma unroll
@@ -345,6 +350,12 @@ __global__ __launch_bounds__(64 * NW, HD == 256 ? 1 : 2) void k_prompt32(sp_hipk
         }
         asm volatile("" : : : "memory");                                  // read again, not kept: KS x 8 registers
         big = fmaxf(big, other_half(big));
+        if constexpr (SPLIT == 2) {                                        // one factor for both parts of a row
+            ((float *)lds)[wave * 32 + l32] = big;
+            __syncthreads();
+            big = fmaxf(big, ((float *)lds)[(wave ^ RG) * 32 + l32]);
+            __syncthreads();
+        }
         const uint32_t e = row_exp(big);
         const float up = sgn * row_up(e);
         c = (a.scale == 0 ? LOG2E_F : fabsf(a.scale) * LOG2E_F) * row_down(e);
@@ -367,10 +378,10 @@ __global__ __launch_bounds__(64 * NW, HD == 256 ? 1 : 2) void k_prompt32(sp_hipk
     auto v_swz = [](int r) { return HD == 64 ? (r >> 1 & 1) << 2 : (r & 3) << 2; };
     int k_at[KS], v_at[DT];
     #pragma unroll
-    for (int k = 0; k < KS; k++) k_at[k] = (l32 * C8 + ((2 * k + half) ^ k_swz(l32))) * 16;
+    for (int k = 0; k < KS; k++) k_at[k] = (l32 * C8 + ((dim0 / 8 + 2 * k + half) ^ k_swz(l32))) * 16;
     #pragma unroll
     for (int d = 0; d < DT; d++) {
-        const int r = 4 * half + (lane & 15) / 4, col = d * 32 + 16 * (lane >> 4 & 1) + 4 * (lane & 3);
+        const int r = 4 * half + (lane & 15) / 4, col = dim0 + d * 32 + 16 * (lane >> 4 & 1) + 4 * (lane & 3);
         v_at[d] = (r * C8 + ((col / 8) ^ v_swz(r))) * 16 + col % 8 * 2;
     }
     for (int tile = k0; tile < k1; tile++) {
@@ -409,14 +420,32 @@ __global__ __launch_bounds__(64 * NW, HD == 256 ? 1 : 2) void k_prompt32(sp_hipk
         bool odd = false;
         if (ragged) odd = __syncthreads_or(bad); else __syncthreads();
         if (tile + 1 < k1) {
-            load(kp, a.k_stride, ko, tile + 1, 0);
+            if (SPLIT == 1) load(kp, a.k_stride, ko, tile + 1, 0);
             load(vp, a.v_stride, vo, tile + 1, RAW);
         }
-        if (tile * BN > w_last || tile * BN + BN <= w_first - W + 1) continue;             // no row of this wave attends any
-        const uint32_t ve = s_ve[l32], top = (uint32_t)wave_allmax_i((int)ve);
+        const bool idle = tile * BN > w_last || tile * BN + BN <= w_first - W + 1;         // no row of this wave attends any
         v16f S = zero;
-        #pragma unroll
-        for (int k = 0; k < KS; k++) S = mfma_halves(Halves{*(const h8 *)(lds + k_at[k]), *(const h8 *)(lds + k_at[k] + PIECE)}, Q[k], S);
+        if (!idle) {
+            #pragma unroll
+            for (int k = 0; k < KS; k++) S = mfma_halves(Halves{*(const h8 *)(lds + k_at[k]), *(const h8 *)(lds + k_at[k] + PIECE)}, Q[k], S);
+        }
+        if constexpr (SPLIT == 2) {
+            float *x = (float *)raw + wave * 1024 + lane * 4;
+            #pragma unroll
+            for (int i = 0; i < 16; i += 4) *(v4f *)(x + i * 64) = (v4f){S[i], S[i + 1], S[i + 2], S[i + 3]};
+            __syncthreads();
+            const float *y = (const float *)raw + (wave ^ RG) * 1024 + lane * 4;
+            #pragma unroll
+            for (int i = 0; i < 16; i += 4) {
+                const v4f z = *(const v4f *)(y + i * 64);
+                #pragma unroll
+                for (int k = 0; k < 4; k++) S[i + k] += z[k];
+            }
+            __syncthreads();
+            if (tile + 1 < k1) load(kp, a.k_stride, ko, tile + 1, 0);
+        }
+        if (idle) continue;
+        const uint32_t ve = s_ve[l32], top = (uint32_t)wave_allmax_i((int)ve);
         // this lane's keys: 8 (i / 4) + 4 half + i % 4
         #pragma unroll
         for (int i = 0; i < 16; i += 4) {
@@ -487,7 +516,7 @@ __global__ __launch_bounds__(64 * NW, HD == 256 ? 1 : 2) void k_prompt32(sp_hipk
         if (odd) {                                                          // V values that were left out, for the rows that attend them
             #pragma unroll 1
             for (int key = tile * BN; key < min(tile * BN + BN, n); key++) {
-                const float *vrow = vp + (size_t)key * a.v_stride + 4 * half;
+                const float *vrow = vp + (size_t)key * a.v_stride + dim0 + 4 * half;
                 #pragma unroll
                 for (int d = 0; d < DT; d++)
                     #pragma unroll
@@ -503,7 +532,7 @@ __global__ __launch_bounds__(64 * NW, HD == 256 ? 1 : 2) void k_prompt32(sp_hipk
     const int r = wr0 + l32;
     const float inv = ldexpf(1.0f / (l + other_half(l)), (int)E - 148);
     if (r >= R) return;
-    float *o = (float *)a.out + (size_t)(t0 + tok) * a.out_stride + (size_t)(h * G + r % G) * HD + 4 * half;
+    float *o = (float *)a.out + (size_t)(t0 + tok) * a.out_stride + (size_t)(h * G + r % G) * HD + dim0 + 4 * half;
     #pragma unroll
     for (int d = 0; d < DT; d++)
         #pragma unroll
@@ -527,11 +556,11 @@ int prompt_check(const sp_hipkv_prompt_args *a) {
 }
 
 template <typename T, int HD> hipError_t prompt_go(const sp_hipkv_prompt_args &a, hipStream_t s) {
-    constexpr int NW = 4;
-    const int slots = (int)((int64_t)a.n_tokens * (a.n_heads / a.n_kv_heads) / (32 * NW)) + a.n_seqs;
-    const dim3 grid((uint32_t)((int64_t)slots * a.n_kv_heads)), wg(64 * NW);
-    if constexpr (sizeof(T) == 4) return op_launch(k_prompt32<HD, NW>, grid, wg, s, a, slots);
-    else return op_launch(k_prompt16<HD, NW>, grid, wg, s, a, slots);
+    constexpr int ROWS = 128;                                              // of a workgroup
+    const int slots = (int)((int64_t)a.n_tokens * (a.n_heads / a.n_kv_heads) / ROWS) + a.n_seqs;
+    const dim3 grid((uint32_t)((int64_t)slots * a.n_kv_heads));
+    if constexpr (sizeof(T) == 4) return op_launch(k_prompt32<HD, HD == 256 ? 8 : 4>, grid, dim3(HD == 256 ? 512 : 256), s, a, slots);
+    else return op_launch(k_prompt16<HD, 4>, grid, dim3(256), s, a, slots);
 }
 template <typename T> hipError_t prompt_type(const sp_hipkv_prompt_args &a, hipStream_t s) {
     return a.head_dim == 256 ? prompt_go<T, 256>(a, s) : a.head_dim == 128 ? prompt_go<T, 128>(a, s) : prompt_go<T, 64>(a, s);
