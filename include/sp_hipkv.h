@@ -476,7 +476,8 @@ int  sp_hipkv_prompt_attention(const sp_hipkv_prompt_args *a, void *stream);
  * step's one token a sequence, or a piece of a prompt): token j of sequence s, at position
  * p = cached[s] + j, attends positions [max(0, p - window + 1), p]:
  * out = sum softmax(scale q.k) v.  q and the weights are taken to integers of 23 bits (of a
- * row's largest value, of a page's largest weight), whose products with the codes are exact.
+ * row's largest value, of a page's largest weight; bf16: 15), whose products with the codes are
+ * exact.
  * Positions that a token does not attend do not reach it whatever their codes and scales.
  * A scale that is not finite in a block that it attends, or a q value that is not, leaves
  * it without a finite value. */

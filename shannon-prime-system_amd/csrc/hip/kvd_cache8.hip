@@ -8,7 +8,7 @@
 // Codes go to the int8 matrix cores as they lie in memory.  q is taken to integers of 23 bits and
 // a sign (127 2^16 for the row's largest value) and these to three digits to base 256, from -128
 // on, so a score is three exact integer products; so are then the weights of a page, each times
-// its V block's scale (127 2^16 for the row's largest).  With 22 bits above a power of two outputs
+// its V block's scale (127 2^16 for the row's largest).  (bf16 values: 15 bits, two digits.)  With 22 bits above a power of two outputs
 // were off by 1.4e-6 where f32 products are by 0.7e-6.  Digits joined: d2 2^16 + (d1 2^8 + d0), the bracket in int32 (256 dims of
 // 2^14 fit), the rest in f32.
 //
@@ -27,15 +27,21 @@ namespace {
 
 constexpr float LOG2E_F = 1.44269504088896341f;
 constexpr int CACHE_PAGES = 256, CACHE_WAVES = 4;                       // pages of a split at most; waves of a workgroup
-constexpr float DIGITS = 127 * 65536;                                   // the largest magnitude whose three digits lie in a byte each, with room for carries
+// Digits of q and the weights: three, and for bf16 values, which are off by 2^-9 themselves, two (15
+// bits: a third fewer products, three instructions for five to join them); the largest magnitude that
+// they hold, with room for carries.
+template <typename T> constexpr int DIG = sizeof(T) == 4 ? 3 : 2;
+template <typename T> constexpr float DIGITS = sizeof(T) == 4 ? 127 * 65536 : 127 * 256;
+// the number that products with digits 0, 1, .. make up
+__device__ __forceinline__ float joined(int a, int b) { return (float)(b * 256 + a); }
+__device__ __forceinline__ float joined(int a, int b, int c) { return fmaf((float)c, 65536.0f, (float)(b * 256 + a)); }
 
-// the bytes b of four words, b = 0, 1, 2: planes[b]
-__device__ __forceinline__ void byte_planes(const uint32_t (&t)[4], uint32_t (&p)[3]) {
+// the bytes b of four words, b = 0 .. ND - 1: p[b]
+template <int ND> __device__ __forceinline__ void byte_planes(const uint32_t (&t)[4], uint32_t (&p)[ND]) {
     const uint32_t a = __builtin_amdgcn_perm(t[1], t[0], 0x05010400), b = __builtin_amdgcn_perm(t[3], t[2], 0x05010400);
     p[0] = __builtin_amdgcn_perm(b, a, 0x05040100);
     p[1] = __builtin_amdgcn_perm(b, a, 0x07060302);
-    const uint32_t c = __builtin_amdgcn_perm(t[1], t[0], 0x0C0C0602), d = __builtin_amdgcn_perm(t[3], t[2], 0x06020C0C);
-    p[2] = c | d;
+    if constexpr (ND == 3) p[2] = __builtin_amdgcn_perm(t[1], t[0], 0x0C0C0602) | __builtin_amdgcn_perm(t[3], t[2], 0x06020C0C);
 }
 
 __device__ __forceinline__ const uint8_t *uniform(const uint8_t *x) {
@@ -43,9 +49,19 @@ __device__ __forceinline__ const uint8_t *uniform(const uint8_t *x) {
     return (const uint8_t *)((uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(p >> 32)) << 32 | (uint32_t)__builtin_amdgcn_readfirstlane((int)p));
 }
 
+// the largest of lanes l, l ^ 16, l ^ 32, l ^ 48
+__device__ __forceinline__ float rows_max(float x) {
+    const v2u a = __builtin_bit_cast(v2u, __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false));
+    x = fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
+    const v2u b = __builtin_bit_cast(v2u, __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false));
+    return fmaxf(__uint_as_float(b[0]), __uint_as_float(b[1]));
+}
+
 template <typename T, int HD, int RT>
 __global__ __launch_bounds__(64 * CACHE_WAVES, HD == 256 ? 1 : 2) void k_cache(sp_hipkv_cache_args a, int groups, int nsplit, int pages) {
-    constexpr int KS = HD / 64, CT = HD / 16, NW = CACHE_WAVES, NT = 64 * NW;
+    constexpr int ND = DIG<T>, KS = HD / 64, CT = HD / 16, NW = CACHE_WAVES, NT = 64 * NW, QE = (RT * KS + NW - 1) / NW;
+    __shared__ v4i s_q[RT * KS * ND][64];
+    __shared__ uint32_t s_big[RT * KS][16];
     __shared__ __align__(16) float s_o[NW][16][HD];
     __shared__ float s_m[NW][16], s_l[NW][16], s_M[16], s_L[16];
     __shared__ const uint8_t *s_page[CACHE_PAGES];
@@ -55,6 +71,7 @@ __global__ __launch_bounds__(64 * CACHE_WAVES, HD == 256 ? 1 : 2) void k_cache(s
     const int h = id % a.n_kv_heads; id /= a.n_kv_heads;
     const int grp = id % groups; id /= groups;
     const int split = id % nsplit, s = id / nsplit;
+    const void *const *table = gmem(a.tables)[s];                          // (here: one wait for all of a sequence's numbers)
     const int t0 = max(gmem(a.start)[s], 0), cached = min(max(gmem(a.cached)[s], 0), a.max_positions);
     const int n = min(min(gmem(a.start)[s + 1], a.n_tokens) - t0, min(a.max_tokens, a.max_positions - cached)), end = cached + n;
     const int R = n * G, r0 = grp * RT * 16;
@@ -73,55 +90,6 @@ __global__ __launch_bounds__(64 * CACHE_WAVES, HD == 256 ? 1 : 2) void k_cache(s
         if (threadIdx.x < RT * 16 && r < R) *gmem((v2f *)(pml + 2 * (row_of(r) * nsplit + split))) = (v2f){-INFINITY, 0.0f};
         return;
     }
-    for (int i = threadIdx.x; i < b1 - b0; i += NT) {
-        const int lp = b0 + i;
-        s_page[i] = (const uint8_t *)gmem(gmem(a.tables)[s])[a.ring_pages ? lp % a.ring_pages : lp];
-    }
-    // q's digits: lane (g, l) row l, dims 64 e + 16 g ..
-    v4i Q[RT][KS][3];
-    float qs[RT];
-    int at[RT];
-    #pragma unroll
-    for (int t = 0; t < RT; t++) {
-        const int r = min(r0 + t * 16 + l16, R - 1);
-        at[t] = cached + r / G;
-        const T *q = (const T *)a.q + (size_t)(t0 + r / G) * a.q_stride + (size_t)(h * G + r % G) * HD + 16 * g;
-        float x[KS][2][8];
-        uint32_t big = 0;
-        #pragma unroll
-        for (int e = 0; e < KS; e++) {
-            load_values(q + 64 * e, x[e][0]);
-            load_values(q + 64 * e + 8, x[e][1]);
-        }
-        #pragma unroll
-        for (int e = 0; e < KS; e++)
-            #pragma unroll
-            for (int k = 0; k < 16; k++) big = max(big, __float_as_uint(x[e][k / 8][k % 8]) & 0x7FFFFFFFu);
-        big = max(big, (uint32_t)__shfl_xor((int)big, 16, 64));
-        big = max(big, (uint32_t)__shfl_xor((int)big, 32, 64));
-        const float up = fminf(DIGITS / __uint_as_float(big), 3e38f);      // (of zeros and the smallest denormals the largest)
-        qs[t] = big < 0x7F800000u ? a.scale * LOG2E_F / up : NAN;
-        #pragma unroll
-        for (int e = 0; e < KS; e++)
-            #pragma unroll
-            for (int k = 0; k < 4; k++) {
-                uint32_t w[4], p[3];
-                #pragma unroll
-                for (int i = 0; i < 4; i++) w[i] = (uint32_t)(int)rintf(x[e][k / 2][4 * (k % 2) + i] * up) + 0x808080u;
-                byte_planes(w, p);
-                #pragma unroll
-                for (int d = 0; d < 3; d++) Q[t][e][d][k] = (int)(p[d] ^ 0x80808080u);
-            }
-    }
-    v4f O[RT][CT];
-    float m[RT], l[RT];
-    #pragma unroll
-    for (int t = 0; t < RT; t++) {
-        m[t] = -INFINITY; l[t] = 0.0f;
-        #pragma unroll
-        for (int c = 0; c < CT; c++) O[t][c] = (v4f){0, 0, 0, 0};
-    }
-    __syncthreads();
     const size_t kat = (size_t)h * PAGE * HD, vat = (size_t)(a.n_kv_heads + h) * PAGE * HD, sat = (size_t)a.n_kv_heads * 2 * PAGE * HD + 16 * h;
     v4i K[4][KS], V[CT];
     v4f ks, vs;
@@ -137,11 +105,79 @@ __global__ __launch_bounds__(64 * CACHE_WAVES, HD == 256 ? 1 : 2) void k_cache(s
         for (int c = 0; c < CT; c++) V[c] = *gmem((const v4i *)(pg + vat + (16 * c + l16) * PAGE + 16 * g));
         vs = *gmem((const v4f *)(pg + sat + 16 * a.n_kv_heads));
     };
-    if (b0 + wave < b1) {
-        const uint8_t *pg = uniform(s_page[wave]);
+    auto page_at = [&](int lp) { return (const uint8_t *)gmem(table)[a.ring_pages ? lp % a.ring_pages : lp]; };
+    for (int i = threadIdx.x; i < b1 - b0; i += NT) s_page[i] = page_at(b0 + i);
+    // q's digits, [row tile][64 dims][digit][lane] 16 bytes: lane (g, l) has row l, dims 64 e + 16 g ..
+    const bool any_page = b0 + wave < b1;
+    float x[QE][2][8];
+    int at[RT];
+    #pragma unroll
+    for (int i = 0; i < QE; i++) {
+        const int te = wave + NW * i, r = min(r0 + te / KS * 16 + l16, R - 1);
+        if (te < RT * KS) {
+            const T *q = (const T *)a.q + (size_t)(t0 + r / G) * a.q_stride + (size_t)(h * G + r % G) * HD + 64 * (te % KS) + 16 * g;
+            load_values(q, x[i][0]);
+            load_values(q + 8, x[i][1]);
+        }
+    }
+    __builtin_amdgcn_sched_barrier(0);
+    if (any_page) {                                                        // on their way while q is taken apart
+        const uint8_t *pg = uniform(page_at(b0 + wave));
         load_k(pg);
         load_v(pg);
     }
+    __builtin_amdgcn_sched_barrier(0);
+    #pragma unroll
+    for (int i = 0; i < QE; i++) {
+        uint32_t big = 0;                                                  // as bits: NaN is above infinity
+        #pragma unroll
+        for (int k = 0; k < 16; k++) big = max(big, __float_as_uint(x[i][k / 8][k % 8]) & 0x7FFFFFFFu);
+        big = max(big, (uint32_t)__shfl_xor((int)big, 16, 64));
+        big = max(big, (uint32_t)__shfl_xor((int)big, 32, 64));
+        if (wave + NW * i < RT * KS && lane < 16) s_big[wave + NW * i][l16] = big;
+    }
+    __syncthreads();
+    float qs[RT];
+    auto row_big = [&](int t) {
+        uint32_t big = 0;
+        #pragma unroll
+        for (int e = 0; e < KS; e++) big = max(big, s_big[t * KS + e][l16]);
+        return big;
+    };
+    auto row_up = [&](uint32_t big) { return fminf(DIGITS<T> / __uint_as_float(big), 3e38f); };    // (of zeros and the smallest denormals the largest)
+    #pragma unroll
+    for (int t = 0; t < RT; t++) {
+        at[t] = cached + min(r0 + t * 16 + l16, R - 1) / G;
+        const uint32_t big = row_big(t);
+        qs[t] = big < 0x7F800000u ? a.scale * LOG2E_F / row_up(big) : NAN;
+    }
+    #pragma unroll
+    for (int i = 0; i < QE; i++) {
+        const int te = wave + NW * i;
+        if (te >= RT * KS) break;
+        const float up = row_up(row_big(te / KS));
+        v4i q[ND];
+        #pragma unroll
+        for (int k = 0; k < 4; k++) {
+            uint32_t w[4], p[ND];
+            #pragma unroll
+            for (int j = 0; j < 4; j++) w[j] = (uint32_t)(int)rintf(x[i][k / 2][4 * (k % 2) + j] * up) + (ND == 3 ? 0x808080u : 0x8080u);
+            byte_planes(w, p);
+            #pragma unroll
+            for (int d = 0; d < ND; d++) q[d][k] = (int)(p[d] ^ 0x80808080u);
+        }
+        #pragma unroll
+        for (int d = 0; d < ND; d++) s_q[te * ND + d][lane] = q[d];
+    }
+    v4f O[RT][CT];
+    float m[RT], l[RT];
+    #pragma unroll
+    for (int t = 0; t < RT; t++) {
+        m[t] = -INFINITY; l[t] = 0.0f;
+        #pragma unroll
+        for (int c = 0; c < CT; c++) O[t][c] = (v4f){0, 0, 0, 0};
+    }
+    __syncthreads();
     for (int b = b0 + wave; b < b1; b += NW) {
         const bool more = b + NW < b1;
         const uint8_t *pn = uniform(s_page[(more ? b + NW : b) - b0]);
@@ -152,21 +188,22 @@ __global__ __launch_bounds__(64 * CACHE_WAVES, HD == 256 ? 1 : 2) void k_cache(s
         for (int t = 0; t < RT; t++)
             #pragma unroll
             for (int u = 0; u < 4; u++) {
-                v4i acc[3];
+                asm volatile("" : : : "memory");                           // q's digits are read again: 12 registers for each 64 dims
+                v4i acc[ND] = {};
                 #pragma unroll
-                for (int d = 0; d < 3; d++) {
-                    acc[d] = (v4i){0, 0, 0, 0};
+                for (int e = 0; e < KS; e++)
                     #pragma unroll
-                    for (int e = 0; e < KS; e++) acc[d] = __builtin_amdgcn_mfma_i32_16x16x64_i8(K[u][e], Q[t][e][d], acc[d], 0, 0, 0);
-                }
+                    for (int d = 0; d < ND; d++) acc[d] = __builtin_amdgcn_mfma_i32_16x16x64_i8(K[u][e], s_q[(t * KS + e) * ND + d][lane], acc[d], 0, 0, 0);
                 const float f = qs[t] * fmaf(ks[u], 0.0f, ks[u]);           // NaN of an infinite scale
                 #pragma unroll
-                for (int i = 0; i < 4; i++) S[t][u][i] = f * fmaf((float)acc[2][i], 65536.0f, (float)(acc[1][i] * 256 + acc[0][i]));
+                for (int i = 0; i < 4; i++) {
+                    if constexpr (ND == 3) S[t][u][i] = f * joined(acc[0][i], acc[1][i], acc[2][i]); else S[t][u][i] = f * joined(acc[0][i], acc[1][i]);
+                }
             }
         __builtin_amdgcn_sched_barrier(0);
         if (more) load_k(pn);
         __builtin_amdgcn_sched_barrier(0);
-        v4i Pd[RT][3];
+        v4i Pd[RT][ND];
         float back[RT];
         #pragma unroll
         for (int t = 0; t < RT; t++) {
@@ -184,9 +221,8 @@ __global__ __launch_bounds__(64 * CACHE_WAVES, HD == 256 ? 1 : 2) void k_cache(s
             float mx = -INFINITY;
             #pragma unroll
             for (int k = 0; k < 16; k++) mx = fmaxf(mx, S[t][k / 4][k % 4]);
-            if (__any(mx > m[t] + 8.0f)) {
-                mx = fmaxf(mx, __shfl_xor(mx, 16, 64));
-                mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
+            if (__any(mx > m[t] + 16.0f)) {
+                mx = rows_max(mx);
                 const float mn = fmaxf(m[t], mx), al = mn == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m[t] - mn);
                 m[t] = mn;
                 l[t] *= al;
@@ -215,19 +251,19 @@ __global__ __launch_bounds__(64 * CACHE_WAVES, HD == 256 ? 1 : 2) void k_cache(s
                 #pragma unroll
                 for (int i = 0; i < 4; i++) top = fmaxf(top, S[t][u][i]);
             }
-            top = fmaxf(top, __shfl_xor(top, 16, 64));
-            top = fmaxf(top, __shfl_xor(top, 32, 64));
-            // weights to integers up to DIGITS; 2^23 + x has x in its low bits, 0x8080 more makes digits of the lower two bytes
+            top = rows_max(top);
+            // weights to integers up to DIGITS; 2^23 + x has x in its low bits, half a digit more in each but the last byte makes digits of them
             top = fmaxf(top, 1e-30f);
-            const float up = DIGITS / top;
-            back[t] = top * (1.0f / DIGITS);
+            const float up = DIGITS<T> / top;
+            back[t] = top * (1.0f / DIGITS<T>);
             #pragma unroll
             for (int u = 0; u < 4; u++) {
-                uint32_t w[4], p[3];
+                uint32_t w[4], p[ND];
                 #pragma unroll
-                for (int i = 0; i < 4; i++) w[i] = __float_as_uint(fmaf(S[t][u][i], up, 8388608.0f)) + 0x8080u;
+                for (int i = 0; i < 4; i++) w[i] = __float_as_uint(fmaf(S[t][u][i], up, 8388608.0f)) + (ND == 3 ? 0x8080u : 0x80u);
                 byte_planes(w, p);
-                Pd[t][0][u] = (int)(p[0] ^ 0x80808080u); Pd[t][1][u] = (int)(p[1] ^ 0x80808080u); Pd[t][2][u] = (int)p[2];
+                #pragma unroll
+                for (int d = 0; d < ND; d++) Pd[t][d][u] = (int)(d < ND - 1 ? p[d] ^ 0x80808080u : p[d]);
             }
         }
         #pragma unroll
@@ -237,11 +273,14 @@ __global__ __launch_bounds__(64 * CACHE_WAVES, HD == 256 ? 1 : 2) void k_cache(s
             for (int i = 0; i < 4; i++) f[i] = __shfl(back[t], 4 * g + i, 64);
             #pragma unroll
             for (int c = 0; c < CT; c++) {
-                v4i acc[3];
+                v4i acc[ND];
                 #pragma unroll
-                for (int d = 0; d < 3; d++) acc[d] = __builtin_amdgcn_mfma_i32_16x16x64_i8(Pd[t][d], V[c], (v4i){0, 0, 0, 0}, 0, 0, 0);
+                for (int d = 0; d < ND; d++) acc[d] = __builtin_amdgcn_mfma_i32_16x16x64_i8(Pd[t][d], V[c], (v4i){0, 0, 0, 0}, 0, 0, 0);
                 #pragma unroll
-                for (int i = 0; i < 4; i++) O[t][c][i] = fmaf(f[i], fmaf((float)acc[2][i], 65536.0f, (float)(acc[1][i] * 256 + acc[0][i])), O[t][c][i]);
+                for (int i = 0; i < 4; i++) {
+                    if constexpr (ND == 3) O[t][c][i] = fmaf(f[i], joined(acc[0][i], acc[1][i], acc[2][i]), O[t][c][i]);
+                    else O[t][c][i] = fmaf(f[i], joined(acc[0][i], acc[1][i]), O[t][c][i]);
+                }
             }
         }
         __builtin_amdgcn_sched_barrier(0);
@@ -294,13 +333,12 @@ __global__ __launch_bounds__(64 * CACHE_WAVES, HD == 256 ? 1 : 2) void k_cache(s
     }
 }
 
-// Joins a row's parts: a workgroup of 256 for 1024 / HD rows' worth of column groups, each
-// thread four columns of one row's every NG-th part.
-template <typename T, int HD>
-__global__ __launch_bounds__(256) void k_cache_merge(sp_hipkv_cache_args a, int nsplit) {
-    constexpr int NG = 1024 / HD;
+// Joins a row's parts: a workgroup a row, a thread four columns of every NG-th part.
+template <typename T, int HD, int NT>
+__global__ __launch_bounds__(NT) void k_cache_merge(sp_hipkv_cache_args a, int nsplit) {
+    constexpr int NG = 4 * NT / HD;
     __shared__ float s_f[64], s_L;
-    __shared__ v4f s_x[256];
+    __shared__ v4f s_x[NT];
     const size_t row = blockIdx.x;
     const int c = threadIdx.x % (HD / 4), grp = threadIdx.x / (HD / 4), token = (int)(row / a.n_heads);
     if (token < gmem(a.start)[0] || token >= gmem(a.start)[a.n_seqs]) return;               // of no sequence: left as it was
@@ -331,19 +369,35 @@ __global__ __launch_bounds__(256) void k_cache_merge(sp_hipkv_cache_args a, int 
     store_values((T *)a.out + (size_t)token * a.out_stride + (row % a.n_heads) * HD + 4 * c, y);
 }
 
-// How a launch is cut: row tiles of a workgroup, workgroups along a sequence's rows, parts of
-// its pages.
-struct CachePlan { int rt, groups, nsplit, pages; };
+// How a launch is cut: workgroups along a sequence's rows (groups, of 16 rows), parts of its pages
+// (nsplit), for the least time estimated of
+//   a workgroup's fixed 5, 7.5, 8 us (dims of 64, 128, 256) and 1.2, 1.8, 3.75 a page and wave, a quarter
+//   more for each that shares its unit (3, 2, 1 can), as often as the units are filled;
+//   memory at 4.8 TB/s (several sequences are taken to be 0.6 of the longest), and a quarter of
+//   the lesser of the two on top;
+//   3.5 us to join parts.
+// From sweeps of nsplit: one token of 16 heads at 32703 (dims of 256) takes 37.8, 33.6, 44.1 us with
+// 24, 32, 48 parts; 30 sessions at 914 (32 heads of 128) 16.8, 19.6, 25 with 1, 2, 4; 24 tokens at 12000
+// 32.7, 29.1, 36.5 with 4, 8, 12.  Against filling 1024 workgroups: 4 x 48 tokens with a window of 1024
+// 28 us for 49.
+struct CachePlan { int groups, nsplit, pages; };
 CachePlan cache_plan(const sp_hipkv_cache_args &a) {
     CachePlan p{};
-    const int tiles = std::max(1, (int)(((int64_t)a.max_tokens * (a.n_heads / a.n_kv_heads) + 15) / 16)), most = 1;
-    p.groups = (tiles + most - 1) / most;
-    p.rt = (tiles + p.groups - 1) / p.groups;
-    const int64_t span = a.window ? std::min<int64_t>(a.max_positions, (int64_t)a.window + 16 * p.rt + PAGE) : a.max_positions;
+    p.groups = std::max(1, (int)(((int64_t)a.max_tokens * (a.n_heads / a.n_kv_heads) + 15) / 16));
+    const int64_t span = a.window ? std::min<int64_t>(a.max_positions, (int64_t)a.window + 16 + PAGE) : a.max_positions;
     p.pages = (int)std::max<int64_t>(1, (span + PAGE - 1) / PAGE);
-    const int64_t base = (int64_t)a.n_kv_heads * std::max(a.n_seqs, 1) * p.groups;
-    p.nsplit = (int)std::max<int64_t>((p.pages + CACHE_PAGES - 1) / CACHE_PAGES, std::min<int64_t>({1024 / base, (p.pages + 3) / 4, 64}));
-    p.nsplit = std::max(p.nsplit, 1);
+    const double fixed = a.head_dim == 256 ? 8 : a.head_dim == 128 ? 7.5 : 5, page = a.head_dim == 256 ? 3.75 : a.head_dim == 128 ? 1.8 : 1.2;
+    const int units = a.head_dim == 256 ? 1 : a.head_dim == 128 ? 2 : 3;
+    const double seqs = (double)a.n_kv_heads * std::max(a.n_seqs, 1);
+    const double mem = fixed / 2 + (a.n_seqs > 1 ? 0.6 : 1.0) * seqs * p.pages * 2 * PAGE * a.head_dim / 4.8e6;
+    double best = 0;
+    for (int n = (p.pages + CACHE_PAGES - 1) / CACHE_PAGES; n <= 64 && n <= p.pages; n++) {
+        const int each = (p.pages + n - 1) / n;
+        const double wgs = std::ceil(seqs * p.groups * n / 256), at_once = std::min<double>(wgs, units);
+        const double run = std::ceil(wgs / units) * (fixed + page * (0.75 + 0.25 * at_once) * ((each + CACHE_WAVES - 1) / CACHE_WAVES + 0.05 * each));
+        const double us = std::max(run, mem) + 0.25 * std::min(run, mem) + (n > 1 ? 3.5 + 1.6e-6 * a.n_tokens * a.n_heads * n * a.head_dim : 0.0);
+        if (!p.nsplit || us < best) { best = us; p.nsplit = n; }
+    }
     return p;
 }
 int64_t cache_grid(const sp_hipkv_cache_args &a, const CachePlan &p) { return (int64_t)a.n_kv_heads * p.groups * p.nsplit * a.n_seqs; }
@@ -369,7 +423,10 @@ template <typename T, int HD> hipError_t cache_go(const sp_hipkv_cache_args &a, 
     const CachePlan p = cache_plan(a);
     hipError_t e = op_launch(k_cache<T, HD, 1>, dim3((uint32_t)cache_grid(a, p)), dim3(64 * CACHE_WAVES), s, a, p.groups, p.nsplit, p.pages);
     if (e != hipSuccess || p.nsplit == 1) return e;
-    return op_launch(k_cache_merge<T, HD>, dim3((uint32_t)((int64_t)a.n_tokens * a.n_heads)), dim3(256), s, a, p.nsplit);
+    // (32 parts of 16 rows: 4.8 us with 1024 threads a row, 7.5 with 256; 2 parts of 2048 rows: 10.6, 4.8)
+    const dim3 rows((uint32_t)((int64_t)a.n_tokens * a.n_heads));
+    if (p.nsplit > 8) return op_launch(k_cache_merge<T, HD, 1024>, rows, dim3(1024), s, a, p.nsplit);
+    return op_launch(k_cache_merge<T, HD, 256>, rows, dim3(256), s, a, p.nsplit);
 }
 template <typename T> hipError_t cache_type(const sp_hipkv_cache_args &a, hipStream_t s) {
     return a.head_dim == 256 ? cache_go<T, 256>(a, s) : a.head_dim == 128 ? cache_go<T, 128>(a, s) : cache_go<T, 64>(a, s);

@@ -10,7 +10,7 @@ from devmem import Dev
 PAGE, BLOCK = 64, 16
 U, B = 2.0 ** -24, 2.0 ** -8
 MARK = 0xC6C6                                           # bf16 bits, and twice f32's, of a value that must survive
-DIGITS = 127 * 65536
+DIGITS = {spkv.F32: 127 * 65536, spkv.BF16: 127 * 256}     # the integers of q's and the weights' largest
 
 
 def to_bf16(x):
@@ -312,12 +312,12 @@ def cache_attention(cache, q, cached, counts, window, scale, typ, pool=None):
                 z = K @ x * scale
                 w = softmax_rows(z)
                 o, r = w @ V, w @ np.abs(V)
-                d = abs(scale) * (np.abs(K) @ (np.abs(x).max() / DIGITS / 2 + 8 * U * np.abs(x))).max() + 8 * U * np.abs(z - z.max()).max()
+                d = abs(scale) * (np.abs(K) @ (np.abs(x).max() / DIGITS[typ] / 2 + 8 * U * np.abs(x))).max() + 8 * U * np.abs(z - z.max()).max()
                 step = np.zeros(hd)
                 y = w * vs[:, h // G]
                 for pg in range(pos[0] // PAGE, p // PAGE + 1):
                     at = pos // PAGE == pg
-                    step += y[at].max() * (0.5 / DIGITS + 4 * U) * np.abs(vc[at, h // G]).sum(0)
+                    step += y[at].max() * (0.5 / DIGITS[typ] + 4 * U) * np.abs(vc[at, h // G]).sum(0)
                 pages = p // PAGE - pos[0] // PAGE + 1
                 out[start[s] + j, h] = o
                 tol[start[s] + j, h] = (4 * d + (8 * pages + 64) * U) * r + step + U * np.abs(o)
