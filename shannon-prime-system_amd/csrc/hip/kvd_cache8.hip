@@ -59,7 +59,7 @@ __device__ __forceinline__ float rows_max(float x) {
 
 template <typename T, int HD, int RT>
 __global__ __launch_bounds__(64 * CACHE_WAVES, HD == 256 ? 1 : 2) void k_cache(sp_hipkv_cache_args a, int groups, int nsplit, int pages) {
-    constexpr int ND = DIG<T>, KS = HD / 64, CT = HD / 16, NW = CACHE_WAVES, NT = 64 * NW, QE = (RT * KS + NW - 1) / NW;
+    constexpr int ND = DIG<T>, KS = HD / 64, CT = HD / 16, NW = CACHE_WAVES, NT = 64 * NW, QE = (RT * KS + NW - 1) / NW, UB = HD == 256 ? 2 : 4;
     __shared__ v4i s_q[RT * KS * ND][64];
     __shared__ uint32_t s_big[RT * KS][16];
     __shared__ __align__(16) float s_o[NW][16][HD];
@@ -80,9 +80,10 @@ __global__ __launch_bounds__(64 * CACHE_WAVES, HD == 256 ? 1 : 2) void k_cache(s
     const int W = a.window ? a.window : INT32_MAX;
     const int at0 = cached + r0 / G, at1 = cached + (min(r0 + RT * 16, R) - 1) / G, lo = max(at0 - W + 1, 0);
     // this split's pages (of a sequence shorter than the longest there are proportionally fewer)
-    const int pg0 = lo / PAGE, np = at1 / PAGE + 1 - pg0;
-    const int parts = max((int)(((int64_t)np * nsplit + pages - 1) / pages), (np + CACHE_PAGES - 1) / CACHE_PAGES);
-    const int b0 = pg0 + (int)((int64_t)np * min(split, parts) / parts), b1 = pg0 + (int)((int64_t)np * min(split + 1, parts) / parts);
+    const int pg0 = lo / PAGE;
+    const uint32_t np = at1 / PAGE + 1 - pg0;
+    const uint32_t parts = max((np * nsplit + pages - 1) / pages, (np + CACHE_PAGES - 1) / CACHE_PAGES);          // (2^14 x 64 at most)
+    const int b0 = pg0 + np * min((uint32_t)split, parts) / parts, b1 = pg0 + np * min((uint32_t)split + 1, parts) / parts;
     float *po = (float *)a.work, *pml = po + (size_t)a.n_tokens * a.n_heads * nsplit * HD;
     auto row_of = [&](int r) { return (size_t)(t0 + r / G) * a.n_heads + h * G + r % G; };
     if (nsplit > 1 && b0 >= b1) {
@@ -187,17 +188,27 @@ __global__ __launch_bounds__(64 * CACHE_WAVES, HD == 256 ? 1 : 2) void k_cache(s
         #pragma unroll
         for (int t = 0; t < RT; t++)
             #pragma unroll
-            for (int u = 0; u < 4; u++) {
+            for (int u0 = 0; u0 < 4; u0 += UB) {
                 asm volatile("" : : : "memory");                           // q's digits are read again: 12 registers for each 64 dims
-                v4i acc[ND] = {};
+                v4i acc[UB][ND] = {};
                 #pragma unroll
-                for (int e = 0; e < KS; e++)
+                for (int e = 0; e < KS; e++) {
+                    v4i q[ND];
                     #pragma unroll
-                    for (int d = 0; d < ND; d++) acc[d] = __builtin_amdgcn_mfma_i32_16x16x64_i8(K[u][e], s_q[(t * KS + e) * ND + d][lane], acc[d], 0, 0, 0);
-                const float f = qs[t] * fmaf(ks[u], 0.0f, ks[u]);           // NaN of an infinite scale
+                    for (int d = 0; d < ND; d++) q[d] = s_q[(t * KS + e) * ND + d][lane];
+                    #pragma unroll
+                    for (int u = 0; u < UB; u++)
+                        #pragma unroll
+                        for (int d = 0; d < ND; d++) acc[u][d] = __builtin_amdgcn_mfma_i32_16x16x64_i8(K[u0 + u][e], q[d], acc[u][d], 0, 0, 0);
+                }
                 #pragma unroll
-                for (int i = 0; i < 4; i++) {
-                    if constexpr (ND == 3) S[t][u][i] = f * joined(acc[0][i], acc[1][i], acc[2][i]); else S[t][u][i] = f * joined(acc[0][i], acc[1][i]);
+                for (int u = 0; u < UB; u++) {
+                    const float f = qs[t] * fmaf(ks[u0 + u], 0.0f, ks[u0 + u]);       // NaN of an infinite scale
+                    #pragma unroll
+                    for (int i = 0; i < 4; i++) {
+                        if constexpr (ND == 3) S[t][u0 + u][i] = f * joined(acc[u][0][i], acc[u][1][i], acc[u][2][i]);
+                        else S[t][u0 + u][i] = f * joined(acc[u][0][i], acc[u][1][i]);
+                    }
                 }
             }
         __builtin_amdgcn_sched_barrier(0);
@@ -281,6 +292,7 @@ __global__ __launch_bounds__(64 * CACHE_WAVES, HD == 256 ? 1 : 2) void k_cache(s
                     if constexpr (ND == 3) O[t][c][i] = fmaf(f[i], joined(acc[0][i], acc[1][i], acc[2][i]), O[t][c][i]);
                     else O[t][c][i] = fmaf(f[i], joined(acc[0][i], acc[1][i]), O[t][c][i]);
                 }
+                if (c % 2) asm volatile("" : "+v"(O[t][c - 1]), "+v"(O[t][c]));       // here, not behind all columns' products: their registers
             }
         }
         __builtin_amdgcn_sched_barrier(0);
@@ -371,22 +383,22 @@ __global__ __launch_bounds__(NT) void k_cache_merge(sp_hipkv_cache_args a, int n
 
 // How a launch is cut: workgroups along a sequence's rows (groups, of 16 rows), parts of its pages
 // (nsplit), for the least time estimated of
-//   a workgroup's fixed 5, 7.5, 8 us (dims of 64, 128, 256) and 1.2, 1.8, 3.75 a page and wave, a quarter
+//   a workgroup's fixed 5, 7.5, 8 us (dims of 64, 128, 256) and 1.2, 1.8, 2.7 a page and wave, a quarter
 //   more for each that shares its unit (3, 2, 1 can), as often as the units are filled;
 //   memory at 4.8 TB/s (several sequences are taken to be 0.6 of the longest), and a quarter of
 //   the lesser of the two on top;
 //   3.5 us to join parts.
-// From sweeps of nsplit: one token of 16 heads at 32703 (dims of 256) takes 37.8, 33.6, 44.1 us with
-// 24, 32, 48 parts; 30 sessions at 914 (32 heads of 128) 16.8, 19.6, 25 with 1, 2, 4; 24 tokens at 12000
-// 32.7, 29.1, 36.5 with 4, 8, 12.  Against filling 1024 workgroups: 4 x 48 tokens with a window of 1024
-// 28 us for 49.
+// From sweeps of nsplit: one token of 16 heads at 32703 (dims of 256) takes 32.1, 31.5, 39.5 us with
+// 24, 32, 48 parts; 30 sessions at 914 (32 heads of 128) 15.7, 18.4, 23.3 with 1, 2, 4; 24 tokens at 12000
+// 27.9, 28.2, 32.9 with 4, 8, 12.  Against filling 1024 workgroups: 4 x 48 tokens with a window of 1024
+// 23 us for 45.
 struct CachePlan { int groups, nsplit, pages; };
 CachePlan cache_plan(const sp_hipkv_cache_args &a) {
     CachePlan p{};
     p.groups = std::max(1, (int)(((int64_t)a.max_tokens * (a.n_heads / a.n_kv_heads) + 15) / 16));
     const int64_t span = a.window ? std::min<int64_t>(a.max_positions, (int64_t)a.window + 16 + PAGE) : a.max_positions;
     p.pages = (int)std::max<int64_t>(1, (span + PAGE - 1) / PAGE);
-    const double fixed = a.head_dim == 256 ? 8 : a.head_dim == 128 ? 7.5 : 5, page = a.head_dim == 256 ? 3.75 : a.head_dim == 128 ? 1.8 : 1.2;
+    const double fixed = a.head_dim == 256 ? 8 : a.head_dim == 128 ? 7.5 : 5, page = a.head_dim == 256 ? 2.7 : a.head_dim == 128 ? 1.8 : 1.2;
     const int units = a.head_dim == 256 ? 1 : a.head_dim == 128 ? 2 : 3;
     const double seqs = (double)a.n_kv_heads * std::max(a.n_seqs, 1);
     const double mem = fixed / 2 + (a.n_seqs > 1 ? 0.6 : 1.0) * seqs * p.pages * 2 * PAGE * a.head_dim / 4.8e6;
