@@ -1,17 +1,17 @@
 // kvd_append.hip -- appending tokens to the paged cache: norm and rotation of q and k,
 // K and V rows into their pages.
 //
-// A workgroup takes one head (of q, k or v) of the tokens that fall into one page, a wave the
-// 16 positions of a block in four rounds of four: lane (i, l) of round r has position
-// 4 r + i and the pairs l PP .. (l + 1) PP of its head, PP = head_dim / 32, so that a head's
-// row is read and written whole by 16 lanes, and a block's largest magnitude and scale stay in
-// a wave.  V codes lie by columns (their byte order is the matrix products'): they
-// pass LDS, from where a thread writes the 16 bytes of a column that it owns.
+// A wave takes the 16 positions of a block in four rounds of four, of one head of k or v or up to
+// QHEADS of q: lane (i, l) of round r has position 4 r + i and the pairs l PP .. (l + 1) PP of a
+// head, PP = head_dim / 32, so that a row is read and written whole by 16 lanes, and a block's
+// largest magnitude and scale stay in a wave.  V codes lie by columns (their byte order is the
+// matrix products'): they pass LDS, from where a thread writes the bytes of a column that it owns.
 //
 // Everything is computed in 64 bits: the angle of position p is p freq, off by 2^-53 of
 // itself (in 32 bits it would be off by 0.008 at position 131072), and a code is the rounded
-// quotient itself, not that of a rounded value.  Sine and cosine are their Taylor series
-// behind a reduction by multiples of pi / 2; f64 runs at the rate of f32 here.
+// quotient itself, not that of a rounded value.  f64 runs at the rate of f32 here.  Sine and
+// cosine are Taylor series behind a reduction by multiples of pi / 2, for a lane's first position and for a
+// step of four; the other rounds' follow by turning, and the q heads of a wave share them.
 #include "kvd_serve.h"
 #include "kvd_vec.h"
 #include <algorithm>
@@ -42,20 +42,26 @@ __device__ __forceinline__ void turn(double x, double &c, double &s) {
     c = (q + 1) & 2 ? -v : v;
 }
 
-// y as an f32 whose rounding to bf16 is that of y: to the odd of its two neighbours
-__device__ __forceinline__ float odd_float(double y) {
-    const float f = (float)y;
-    uint32_t u = __float_as_uint(f);
-    const double d = (double)f;
-    if (d != y && fabsf(f) < INFINITY) {
-        u -= fabs(d) > fabs(y);                                           // towards zero
-        u |= 1;
+// y[] as f32, or as f32 whose rounding to bf16 is that of y: only where the nearest f32 lies half way between
+// two bf16 does the second rounding need the side that y is on
+template <typename T, int N> __device__ __forceinline__ void rounded(const double (&y)[N], float (&z)[N]) {
+    bool tie = false;
+    #pragma unroll
+    for (int k = 0; k < N; k++) {
+        z[k] = (float)y[k];
+        tie |= sizeof(T) == 2 && (__float_as_uint(z[k]) & 0xFFFF) == 0x8000;
     }
-    return __uint_as_float(u);
+    if (sizeof(T) == 2 && __builtin_expect(__any(tie), 0)) {
+        #pragma unroll
+        for (int k = 0; k < N; k++) {
+            const uint32_t u = __float_as_uint(z[k]);
+            if ((u & 0xFFFF) == 0x8000) z[k] = __uint_as_float(u + (fabs(y[k]) > fabs((double)z[k])) - (fabs(y[k]) < fabs((double)z[k])));
+        }
+    }
 }
 
 // The exponent of a block's scale: the least e, from -126 on, with big <= 127 2^e; INT32_MAX if
-// f32 has none
+// f32 has none, or big is none
 __device__ __forceinline__ int scale_exp(double big) {
     const uint64_t u = __builtin_bit_cast(uint64_t, big);
     const int e = (int)(u >> 52 & 2047) - 1022;                           // big = m 2^e, m in [1/2, 1)
@@ -67,58 +73,143 @@ __device__ __forceinline__ float block_scale(int e, bool older, float was) {
     const float s = e == INT32_MAX ? NAN : __uint_as_float((uint32_t)(e + 127) << 23);
     return older && !(was < s) && s == s ? was : s;
 }
-__device__ __forceinline__ int code_of(double y, double inv) {
-    const double r = rint(y * inv);
-    return r == r ? (int)fmin(fmax(r, -127.0), 127.0) : 0;
-}
+// Codes, in the low byte: adding 3 2^51 (2^22) leaves the nearest integer in the low bits, ties to even
+__device__ __forceinline__ uint32_t code_of(double y, double inv) { return (uint32_t)__builtin_bit_cast(uint64_t, fma(y, inv, 6755399441055744.0)); }
+__device__ __forceinline__ uint32_t code_of(float y, float inv) { return __float_as_uint(fmaf(y, inv, 12582912.0f)); }
 // a stored code at another scale
-__device__ __forceinline__ uint32_t recode(uint32_t code, float ratio) {
-    const float x = (float)(int8_t)code * ratio;
-    return (uint32_t)(x == x ? (int)rintf(x) : 0) & 255;
-}
+__device__ __forceinline__ uint32_t recode(uint32_t code, float ratio) { return code_of((float)(int8_t)code, ratio) & 255; }
 
-template <typename T, int ROWS, int HD>
-__global__ __launch_bounds__(256) void k_append(sp_hipkv_append_args a, int seq_pages) {
-    constexpr int PP = HD / 32, H2 = HD / 2;
+constexpr int QHEADS = 4;
+
+// NW waves a workgroup: 4, a page, or 1, a block.  heads: of q, at most QHEADS.
+template <typename T, int ROWS, int HD, int NW>
+__global__ __launch_bounds__(64 * NW) void k_append(sp_hipkv_append_args a, int seq_units, int heads) {
+    constexpr int PP = HD / 32, H2 = HD / 2, UNIT = BLOCK8 * NW;
     constexpr bool B8 = ROWS == SP_HIPKV_ROWS_BLOCK8;
-    constexpr int COL = PAGE + 16;                                        // bytes of a column of V codes in LDS
+    constexpr int COL = 16 * NW + 16;                                     // bytes of a column of V codes in LDS
     __shared__ __align__(16) uint8_t s_code[B8 ? HD * COL : 16];
     __shared__ float s_ratio;
-    // this workgroup's sequence and page
+    // this workgroup's sequence and unit of positions
     const int slot = blockIdx.y;
     int s, j;
-    if (seq_pages) { s = slot / seq_pages; j = slot - s * seq_pages; }
-    else { s = unit_seq(a.start, a.n_seqs, slot, 1, PAGE, 2); j = slot - (int)unit_base(a.start, s, 1, PAGE, 2); }
+    if (seq_units) { s = slot / seq_units; j = slot - s * seq_units; }
+    else { s = unit_seq(a.start, a.n_seqs, slot, 1, UNIT, 2); j = slot - (int)unit_base(a.start, s, 1, UNIT, 2); }
+    const void *const *table = gmem(a.tables)[s];
     const int t0 = max(gmem(a.start)[s], 0), first = min(max(gmem(a.cached)[s], 0), a.max_positions);
     const int n = min(min(gmem(a.start)[s + 1], a.n_tokens) - t0, min(a.max_tokens, a.max_positions - first)), end = first + n;
-    const int lp = first / PAGE + j;
-    if (n <= 0 || j < 0 || lp > (end - 1) / PAGE) return;
-    // q, k or v, and its head
+    const int p0 = (first / UNIT + j) * UNIT, lp = p0 / PAGE;
+    if (n <= 0 || j < 0 || p0 >= end) return;
+    // q (heads h .. h1), k or v, and its head
+    const int gq = a.q_out ? (a.n_heads + heads - 1) / heads : 0;
     int h = blockIdx.x, kind = 0;
-    const int nq = a.q_out ? a.n_heads : 0;
-    if (h >= nq) { h -= nq; kind = 1; }
+    if (h >= gq) { h -= gq; kind = 1; }
     if (kind == 1 && h >= a.n_kv_heads) { h -= a.n_kv_heads; kind = 2; }
+    if (kind == 0) h *= heads;
+    const int h1 = min(h + heads, a.n_heads);
     const bool stored = kind && !(a.ring_pages && lp + a.ring_pages <= (end - 1) / PAGE);
     if (!stored && !(kind == 0 || (kind == 1 && a.k_out))) return;
-    const int lane = threadIdx.x & 63, u = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), i = lane >> 4, l = lane & 15;
-    const int b0 = lp * PAGE + BLOCK8 * u;
-    const bool some = b0 < end && b0 + BLOCK8 > first, cols = B8 && kind == 2;
-    if (!some && !cols) return;
-    uint8_t *page = stored ? (uint8_t *)gmem(gmem(a.tables)[s])[a.ring_pages ? lp % a.ring_pages : lp] : nullptr;
-    float *scale_at = B8 && stored ? (float *)(page + (size_t)2 * a.n_kv_heads * PAGE * HD) + ((kind - 1) * a.n_kv_heads + h) * PAGE_BLOCKS + u : nullptr;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), i = lane >> 4, l = lane & 15;
+    const int b0 = p0 + BLOCK8 * wave, u = b0 / BLOCK8 % PAGE_BLOCKS;
+    const bool some = b0 < end && b0 + BLOCK8 > first;
+    if (!some && !(B8 && kind == 2)) return;
+    uint8_t *page = stored ? (uint8_t *)gmem(table)[a.ring_pages ? lp % a.ring_pages : lp] : nullptr;
     auto live = [&](int r) { const int p = b0 + 4 * r + i; return p >= first && p < end; };
     auto round_live = [&](int r) { return b0 + 4 * r < end && b0 + 4 * r + 4 > first; };
-    const T *src = (const T *)(kind == 0 ? a.q : kind == 1 ? a.k : a.v);
-    const int64_t stride = kind == 0 ? a.q_stride : kind == 1 ? a.k_stride : a.v_stride;
+    const bool older = B8 && some && stored && first > b0;                // positions of the block from earlier calls
+    auto row_of = [&](auto *p, int64_t stride, int r, int head) __attribute__((always_inline)) {
+        return p + (size_t)(t0 + b0 + 4 * r + i - first) * stride + (size_t)head * HD + l * PP;
+    };
+    auto put = [&](auto *row, const float (&z)[2 * PP]) __attribute__((always_inline)) {
+        float z0[PP], z1[PP];
+        #pragma unroll
+        for (int k = 0; k < PP; k++) { z0[k] = z[k]; z1[k] = z[PP + k]; }
+        store_values(row, z0);
+        store_values(row + H2, z1);
+    };
+    // a round's sines and cosines, from the last round's
+    double c[PP], sn[PP], cs[PP], ss[PP];
+    auto start = [&] {
+        #pragma unroll
+        for (int k = 0; k < PP; k++) {
+            const double f = gmem(a.freq)[l * PP + k];
+            turn((double)(b0 + i) * f, c[k], sn[k]);
+            turn(4.0 * f, cs[k], ss[k]);
+        }
+    };
+    auto step = [&] {
+        #pragma unroll
+        for (int k = 0; k < PP; k++) {
+            const double x = fma(c[k], cs[k], -(sn[k] * ss[k]));
+            sn[k] = fma(c[k], ss[k], sn[k] * cs[k]);
+            c[k] = x;
+        }
+    };
+    float w[2][PP];
+    const float *nw = kind ? a.k_norm : a.q_norm;
+    auto weights = [&] {
+        #pragma unroll
+        for (int k = 0; k < PP; k++) { w[0][k] = gmem(nw)[l * PP + k]; w[1][k] = gmem(nw)[H2 + l * PP + k]; }
+    };
+    // norm and rotation of a row (every lane of the 16 comes here)
+    auto prepare = [&](const float (&x)[2][PP], double (&y)[2 * PP]) __attribute__((always_inline)) {
+        #pragma unroll
+        for (int k = 0; k < PP; k++) { y[k] = (double)x[0][k]; y[PP + k] = (double)x[1][k]; }
+        if (nw) {
+            double q = 0.0;
+            #pragma unroll
+            for (int k = 0; k < 2 * PP; k++) q = fma(y[k], y[k], q);
+            #pragma unroll
+            for (int o = 1; o < 16; o <<= 1) q += __shfl_xor(q, o, 64);
+            const double m = 1.0 / sqrt(q * (1.0 / HD) + (double)a.eps);
+            #pragma unroll
+            for (int k = 0; k < PP; k++) { y[k] *= m * (double)w[0][k]; y[PP + k] *= m * (double)w[1][k]; }
+        }
+        if (a.freq) {
+            #pragma unroll
+            for (int k = 0; k < PP; k++) {
+                const double x0 = y[k], x1 = y[PP + k];
+                y[k] = fma(x0, c[k], -(x1 * sn[k]));
+                y[PP + k] = fma(x0, sn[k], x1 * c[k]);
+            }
+        }
+    };
+    if (kind == 0) {
+        if (nw) weights();
+        if (a.freq) start();
+        #pragma unroll
+        for (int r = 0; r < 4; r++) {
+            if (r && a.freq) step();
+            if (!round_live(r)) continue;
+            float x[QHEADS][2][PP];
+            #pragma unroll
+            for (int e = 0; e < QHEADS; e++)
+                if (h + e < h1 && live(r)) {
+                    const T *row = row_of((const T *)a.q, a.q_stride, r, h + e);
+                    load_values(row, x[e][0]);
+                    load_values(row + H2, x[e][1]);
+                }
+            #pragma unroll
+            for (int e = 0; e < QHEADS; e++) {
+                if (h + e >= h1) break;
+                double y[2 * PP];
+                float z[2 * PP];
+                prepare(x[e], y);
+                rounded<T>(y, z);
+                if (live(r)) put(row_of((T *)a.q_out, a.q_out_stride, r, h + e), z);
+            }
+        }
+        return;
+    }
+    const T *src = (const T *)(kind == 1 ? a.k : a.v);
+    const int64_t stride = kind == 1 ? a.k_stride : a.v_stride;
     float x[4][2][PP];
     #pragma unroll
     for (int r = 0; r < 4; r++)
         if (live(r)) {
-            const T *row = src + (size_t)(t0 + b0 + 4 * r + i - first) * stride + (size_t)h * HD + l * PP;
+            const T *row = row_of(src, stride, r, h);
             load_values(row, x[r][0]);
             load_values(row + H2, x[r][1]);
         }
-    const bool older = B8 && some && stored && first > b0;                // positions of the block from earlier calls
     if (kind == 2) {
         if constexpr (!B8) {
             #pragma unroll
@@ -129,10 +220,11 @@ __global__ __launch_bounds__(256) void k_append(sp_hipkv_append_args a, int seq_
                     store_values(row + H2, x[r][1]);
                 }
         } else {
+            float *scale_at = (float *)(page + (size_t)2 * a.n_kv_heads * PAGE * HD) + (a.n_kv_heads + h) * PAGE_BLOCKS + u;
             if (threadIdx.x == 0) s_ratio = 1.0f;
-            __syncthreads();
+            if (NW > 1) __syncthreads();
             if (some) {
-                uint32_t big = 0;                                         // as bits: NaN is above infinity
+                uint32_t big = 0;                                     // as bits: NaN is above infinity
                 #pragma unroll
                 for (int r = 0; r < 4; r++)
                     if (live(r)) {
@@ -141,8 +233,7 @@ __global__ __launch_bounds__(256) void k_append(sp_hipkv_append_args a, int seq_
                     }
                 big = (uint32_t)wave_allmax_i((int)big);
                 const float was = older ? *scale_at : 0.0f;
-                const float sc = block_scale(scale_exp((double)__uint_as_float(big)), older, was);
-                const double inv = 1.0 / (double)sc;
+                const float sc = block_scale(scale_exp((double)__uint_as_float(big)), older, was), inv = 1.0f / sc;
                 if (lane == 0) {
                     *scale_at = sc;
                     if (older) s_ratio = was / sc;
@@ -152,152 +243,107 @@ __global__ __launch_bounds__(256) void k_append(sp_hipkv_append_args a, int seq_
                     if (live(r)) {
                         #pragma unroll
                         for (int k = 0; k < PP; k++) {
-                            uint8_t *col = s_code + (l * PP + k) * COL + 16 * r + 4 * u + i;
-                            col[0] = (uint8_t)code_of((double)x[r][0][k], inv);
-                            col[H2 * COL] = (uint8_t)code_of((double)x[r][1][k], inv);
+                            uint8_t *col = s_code + (l * PP + k) * COL + 4 * NW * r + 4 * wave + i;
+                            col[0] = (uint8_t)code_of(x[r][0][k], inv);
+                            col[H2 * COL] = (uint8_t)code_of(x[r][1][k], inv);
                         }
                     }
             }
             __syncthreads();
-            const float ratio = s_ratio;                                  // of the codes that the first block has already
-            const int p0 = lp * PAGE, old0 = first / BLOCK8 * BLOCK8;
-            for (int id = threadIdx.x; id < HD * 4; id += 256) {
+            const float ratio = s_ratio;                              // of the codes that the first block has already
+            const int old0 = first / BLOCK8 * BLOCK8;
+            // NW words of four positions each, 4 g .. of NW neighbouring blocks
+            for (int id = threadIdx.x; id < HD * 4; id += 64 * NW) {
                 const int d = id >> 2, g = id & 3;
-                v4u w = *(const v4u *)(s_code + d * COL + 16 * g);
-                KVD_GLOBAL v4u *dst = gmem((v4u *)(page + ((size_t)a.n_kv_heads + h) * PAGE * HD + (size_t)d * PAGE + 16 * g));
-                uint32_t fresh = 0, again = 0;                            // bytes to write, bytes to round again
+                uint32_t w[NW];
+                const uint32_t *from = (const uint32_t *)(s_code + d * COL + 4 * NW * g);
+                KVD_GLOBAL uint32_t *dst = gmem((uint32_t *)(page + ((size_t)a.n_kv_heads + h) * PAGE * HD + (size_t)d * PAGE + 16 * g + (NW == 1 ? 4 * u : 0)));
+                uint32_t fresh = 0, again = 0;                        // bytes to write, bytes to round again
                 #pragma unroll
-                for (int k = 0; k < 16; k++) {
+                for (int k = 0; k < 4 * NW; k++) {
                     const int p = p0 + (k >> 2) * 16 + 4 * g + (k & 3);
                     fresh |= (uint32_t)(p >= first && p < end) << k;
                     again |= (uint32_t)(p >= old0 && p < first && ratio != 1.0f) << k;
                 }
                 if (!(fresh | again)) continue;
-                if (fresh != 0xFFFF) {
-                    const v4u o = *dst;
+                #pragma unroll
+                for (int k = 0; k < NW; k++) w[k] = from[k];
+                if (fresh != (1u << 4 * NW) - 1) {
+                    uint32_t o[NW];
                     #pragma unroll
-                    for (int k = 0; k < 16; k++) {
+                    for (int k = 0; k < NW; k++) o[k] = dst[k];
+                    #pragma unroll
+                    for (int k = 0; k < 4 * NW; k++) {
                         const int sh = 8 * (k & 3);
                         uint32_t b = o[k >> 2] >> sh & 255;
                         if (again >> k & 1) b = recode(b, ratio);
                         if (!(fresh >> k & 1)) w[k >> 2] = (w[k >> 2] & ~(255u << sh)) | b << sh;
                     }
                 }
-                *dst = w;
+                if constexpr (NW == 4) *(KVD_GLOBAL v4u *)dst = (v4u){w[0], w[1], w[2], w[3]};
+                else dst[0] = w[0];
             }
         }
         return;
     }
-    // q or k: norm, rotation
-    double y[4][2][PP];
-    double f[PP];
-    float w[2][PP];
-    const float *nw = kind ? a.k_norm : a.q_norm;
-    if (a.freq) {
-        #pragma unroll
-        for (int k = 0; k < PP; k++) f[k] = gmem(a.freq)[l * PP + k];
-    }
-    if (nw) {
-        #pragma unroll
-        for (int k = 0; k < PP; k++) { w[0][k] = gmem(nw)[l * PP + k]; w[1][k] = gmem(nw)[H2 + l * PP + k]; }
-    }
-    double big = 0.0;
+    if (nw) weights();
+    if (a.freq) start();
+    double y[4][2 * PP], big = 0.0, none = 0.0;                            // none: NaN if some value is not finite
     #pragma unroll
     for (int r = 0; r < 4; r++) {
+        if (r && a.freq) step();
         if (!round_live(r)) continue;
-        #pragma unroll
-        for (int k = 0; k < PP; k++) { y[r][0][k] = (double)x[r][0][k]; y[r][1][k] = (double)x[r][1][k]; }
-        if (nw) {
-            double ss = 0.0;
-            #pragma unroll
-            for (int k = 0; k < PP; k++) ss = fma(y[r][0][k], y[r][0][k], fma(y[r][1][k], y[r][1][k], ss));
-            #pragma unroll
-            for (int o = 1; o < 16; o <<= 1) ss += __shfl_xor(ss, o, 64);
-            const double m = 1.0 / sqrt(ss * (1.0 / HD) + (double)a.eps);
-            #pragma unroll
-            for (int k = 0; k < PP; k++) { y[r][0][k] = y[r][0][k] * m * (double)w[0][k]; y[r][1][k] = y[r][1][k] * m * (double)w[1][k]; }
+        prepare(x[r], y[r]);
+        if (!live(r)) continue;
+        float z[2 * PP];
+        if (a.k_out) {
+            rounded<T>(y[r], z);
+            put(row_of((T *)a.k_out, a.k_out_stride, r, h), z);
         }
-        if (a.freq) {
-            const double p = (double)(b0 + 4 * r + i);
+        if constexpr (B8) {
             #pragma unroll
-            for (int k = 0; k < PP; k++) {
-                double c, sn;
-                turn(p * f[k], c, sn);
-                const double x0 = y[r][0][k], x1 = y[r][1][k];
-                y[r][0][k] = fma(x0, c, -(x1 * sn));
-                y[r][1][k] = fma(x0, sn, x1 * c);
-            }
-        }
-        if (B8 && live(r)) {
-            #pragma unroll
-            for (int k = 0; k < PP; k++)
-                #pragma unroll
-                for (int e = 0; e < 2; e++) {                              // NaN and infinities as infinity
-                    const double v = fabs(y[r][e][k]);
-                    big = v < INFINITY ? fmax(big, v) : INFINITY;
-                }
-        }
-        void *back = kind ? a.k_out : a.q_out;
-        if (back && live(r)) {
-            T *row = (T *)back + (size_t)(t0 + b0 + 4 * r + i - first) * (kind ? a.k_out_stride : a.q_out_stride) + (size_t)h * HD + l * PP;
-            float z[2][PP];
-            #pragma unroll
-            for (int k = 0; k < PP; k++)
-                #pragma unroll
-                for (int e = 0; e < 2; e++) z[e][k] = sizeof(T) == 4 ? (float)y[r][e][k] : odd_float(y[r][e][k]);
-            store_values(row, z[0]);
-            store_values(row + H2, z[1]);
-        }
-        if (!B8 && stored && live(r)) {
-            float *row = (float *)page + ((size_t)h * PAGE + BLOCK8 * u + 4 * r + i) * HD + l * PP;
-            float z[2][PP];
-            #pragma unroll
-            for (int k = 0; k < PP; k++) { z[0][k] = (float)y[r][0][k]; z[1][k] = (float)y[r][1][k]; }
-            store_values(row, z[0]);
-            store_values(row + H2, z[1]);
+            for (int k = 0; k < 2 * PP; k++) { big = fmax(big, fabs(y[r][k])); none = fma(y[r][k], 0.0, none); }
+        } else if (stored) {
+            rounded<float>(y[r], z);
+            put((float *)page + ((size_t)h * PAGE + BLOCK8 * u + 4 * r + i) * HD + l * PP, z);
         }
     }
-    if (!B8 || !stored) return;
-    big = bcast63(wave_to63(big, 0.0, [](double p, double q) { return fmax(p, q); }));
-    const float was = older ? *scale_at : 0.0f;
-    const float sc = block_scale(scale_exp(big), older, was), ratio = was / sc;
-    const double inv = 1.0 / (double)sc;
-    if (lane == 0) *scale_at = sc;
-    #pragma unroll
-    for (int r = 0; r < 4; r++) {
-        const int p = b0 + 4 * r + i;
-        const bool again = older && p < first && ratio != 1.0f;
-        if (!live(r) && !again) continue;
+    if constexpr (B8) {
+        if (!stored) return;
+        big = none == none ? big : INFINITY;
+        big = bcast63(wave_to63(big, 0.0, [](double p, double q) { return fmax(p, q); }));
+        float *scale_at = (float *)(page + (size_t)2 * a.n_kv_heads * PAGE * HD) + h * PAGE_BLOCKS + u;
+        const float was = older ? *scale_at : 0.0f;
+        const float sc = block_scale(scale_exp(big), older, was), ratio = was / sc;
+        const double inv = 1.0 / (double)sc;
+        if (lane == 0) *scale_at = sc;
         #pragma unroll
-        for (int e = 0; e < 2; e++) {
-            uint8_t *row = page + ((size_t)h * PAGE + BLOCK8 * u + 4 * r + i) * HD + l * PP + e * H2;
-            uint32_t c[(PP + 3) / 4];
-            if (again) {
+        for (int r = 0; r < 4; r++) {
+            const bool again = older && b0 + 4 * r + i < first && ratio != 1.0f;
+            if (!live(r) && !again) continue;
+            #pragma unroll
+            for (int e = 0; e < 2; e++) {
+                uint8_t *row = page + ((size_t)h * PAGE + BLOCK8 * u + 4 * r + i) * HD + l * PP + e * H2;
+                uint32_t b[(PP + 3) / 4];
                 #pragma unroll
                 for (int k = 0; k < PP; k++) {
-                    const uint32_t b = recode(gmem(row)[k], ratio);
-                    c[k / 4] = k % 4 ? c[k / 4] | b << 8 * (k % 4) : b;
+                    const uint32_t code = again ? recode(gmem(row)[k], ratio) : code_of(y[r][e * PP + k], inv) & 255;
+                    b[k / 4] = k % 4 ? b[k / 4] | code << 8 * (k % 4) : code;
                 }
-            } else {
-                #pragma unroll
-                for (int k = 0; k < PP; k++) {
-                    const uint32_t b = (uint32_t)code_of(y[r][e][k], inv) & 255;
-                    c[k / 4] = k % 4 ? c[k / 4] | b << 8 * (k % 4) : b;
-                }
+                if constexpr (PP == 2) *gmem((uint16_t *)row) = (uint16_t)b[0];
+                else if constexpr (PP == 4) *gmem((uint32_t *)row) = b[0];
+                else *gmem((v2u *)row) = (v2u){b[0], b[1]};
             }
-            if constexpr (PP == 2) *gmem((uint16_t *)row) = (uint16_t)c[0];
-            else if constexpr (PP == 4) *gmem((uint32_t *)row) = c[0];
-            else *gmem((v2u *)row) = (v2u){c[0], c[1]};
         }
     }
 }
 
-// Pages that a call's tokens may fall into: with few tokens a sequence every sequence's most,
-// else by the packed tokens (a page and its neighbour more for each sequence).
-struct AppendPlan { int slots, seq_pages; };
-AppendPlan append_plan(const sp_hipkv_append_args &a) {
-    const int64_t most = ((int64_t)a.max_tokens + PAGE - 2) / PAGE + 1, packed = (int64_t)a.n_tokens / PAGE + 2 * a.n_seqs;
-    return most * a.n_seqs <= packed ? AppendPlan{(int)(most * a.n_seqs), (int)most} : AppendPlan{(int)packed, 0};
+// Units of positions that a call's tokens may fall into: with few tokens a sequence every sequence's
+// most, else by the packed tokens (a unit and its neighbour more for each sequence).
+int64_t append_slots(const sp_hipkv_append_args &a, int unit, int *seq_units) {
+    const int64_t most = ((int64_t)a.max_tokens + unit - 2) / unit + 1, packed = (int64_t)a.n_tokens / unit + 2 * a.n_seqs;
+    *seq_units = most * a.n_seqs <= packed ? (int)most : 0;
+    return *seq_units ? most * a.n_seqs : packed;
 }
 
 int append_check(const sp_hipkv_append_args *a) {
@@ -320,18 +366,23 @@ int append_check(const sp_hipkv_append_args *a) {
     return 0;
 }
 
-template <typename T, int ROWS> hipError_t append_go(const sp_hipkv_append_args &a, hipStream_t s) {
-    const AppendPlan p = append_plan(a);
-    const dim3 grid((a.q_out ? a.n_heads : 0) + 2 * a.n_kv_heads, p.slots);
-    return op_launch(a.head_dim == 256 ? k_append<T, ROWS, 256> : a.head_dim == 128 ? k_append<T, ROWS, 128> : k_append<T, ROWS, 64>,
-                     grid, dim3(256), s, a, p.seq_pages);
+template <typename T, int ROWS, int NW> hipError_t append_go(const sp_hipkv_append_args &a, hipStream_t s) {
+    int seq_units = 0;
+    const int64_t slots = append_slots(a, BLOCK8 * NW, &seq_units), rows = (a.q_out ? a.n_heads : 0) + 2 * a.n_kv_heads;
+    const int heads = slots * rows * NW >= 16384 ? QHEADS : 1;
+    const int groups = (a.q_out ? (a.n_heads + heads - 1) / heads : 0) + 2 * a.n_kv_heads;
+    return op_launch(a.head_dim == 256 ? k_append<T, ROWS, 256, NW> : a.head_dim == 128 ? k_append<T, ROWS, 128, NW> : k_append<T, ROWS, 64, NW>,
+                     dim3(groups, (uint32_t)slots), dim3(64 * NW), s, a, seq_units, heads);
+}
+template <typename T, int ROWS> hipError_t append_rows(const sp_hipkv_append_args &a, hipStream_t s) {
+    return a.max_tokens <= BLOCK8 ? append_go<T, ROWS, 1>(a, s) : append_go<T, ROWS, 4>(a, s);
 }
 
 }  // namespace
 
 hipError_t launch_append(const sp_hipkv_append_args &a, hipStream_t s) {
-    if (a.rows == SP_HIPKV_ROWS_F32) return a.type == SP_HIPKV_F32 ? append_go<float, SP_HIPKV_ROWS_F32>(a, s) : append_go<Bf16, SP_HIPKV_ROWS_F32>(a, s);
-    return a.type == SP_HIPKV_F32 ? append_go<float, SP_HIPKV_ROWS_BLOCK8>(a, s) : append_go<Bf16, SP_HIPKV_ROWS_BLOCK8>(a, s);
+    if (a.rows == SP_HIPKV_ROWS_F32) return a.type == SP_HIPKV_F32 ? append_rows<float, SP_HIPKV_ROWS_F32>(a, s) : append_rows<Bf16, SP_HIPKV_ROWS_F32>(a, s);
+    return a.type == SP_HIPKV_F32 ? append_rows<float, SP_HIPKV_ROWS_BLOCK8>(a, s) : append_rows<Bf16, SP_HIPKV_ROWS_BLOCK8>(a, s);
 }
 
 }  // namespace kvd
