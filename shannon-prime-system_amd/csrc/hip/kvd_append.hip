@@ -1,8 +1,7 @@
 // kvd_append.hip -- appending tokens to the paged cache: norm and rotation of q and k,
 // K and V rows into their pages.
 //
-// A wave takes the 16 positions of a block in four rounds of four, of one head of k or v or up to
-// QHEADS of q: lane (i, l) of round r has position 4 r + i and the pairs l PP .. (l + 1) PP of a
+// A wave takes the 16 positions of a block in four rounds of four, of one head of q, k or v: lane (i, l) of round r has position 4 r + i and the pairs l PP .. (l + 1) PP of a
 // head, PP = head_dim / 32, so that a row is read and written whole by 16 lanes, and a block's
 // largest magnitude and scale stay in a wave.  V codes lie by columns (their byte order is the
 // matrix products'): they pass LDS, from where a thread writes the bytes of a column that it owns.
@@ -11,7 +10,8 @@
 // itself (in 32 bits it would be off by 0.008 at position 131072), and a code is the rounded
 // quotient itself, not that of a rounded value.  f64 runs at the rate of f32 here.  Sine and
 // cosine are Taylor series behind a reduction by multiples of pi / 2, for a lane's first position and for a
-// step of four; the other rounds' follow by turning, and the q heads of a wave share them.
+// step of four; the other rounds' follow by turning.  (Four q heads a wave with the same sines: 38.6 us
+// for 37.2 of 4096 tokens, 32 and 8 heads of 128; what counts is rows on their way.)
 #include "kvd_serve.h"
 #include "kvd_vec.h"
 #include <algorithm>
@@ -40,6 +40,23 @@ __device__ __forceinline__ void turn(double x, double &c, double &s) {
     const double u = q & 1 ? b : a, v = q & 1 ? a : b;
     s = q & 2 ? -u : u;
     c = (q + 1) & 2 ? -v : v;
+}
+
+// the sum over the 16 lanes of a row
+__device__ __forceinline__ double row_sum(double x) {
+    auto step = [&](auto ctrl) { x += __builtin_bit_cast(double, dpp64<decltype(ctrl)::value, 0xF>(__builtin_bit_cast(uint64_t, x), 0)); };
+    step(std::integral_constant<int, 0xB1>{});                            // quad_perm 1,0,3,2
+    step(std::integral_constant<int, 0x4E>{});                            // quad_perm 2,3,0,1
+    step(std::integral_constant<int, 0x141>{});                           // row_half_mirror
+    step(std::integral_constant<int, 0x140>{});                           // row_mirror
+    return x;
+}
+// 1 / sqrt(x): the instruction's estimate (2^-24 or better), then Newton's y + y (1 - x y^2) / 2 twice: 3/8 e^2 each
+__device__ __forceinline__ double inv_sqrt(double x) {
+    double y = __builtin_amdgcn_rsq(x);
+    #pragma unroll
+    for (int i = 0; i < 2; i++) y = fma(y * 0.5, fma(-(x * y), y, 1.0), y);
+    return y;
 }
 
 // y[] as f32, or as f32 whose rounding to bf16 is that of y: only where the nearest f32 lies half way between
@@ -79,11 +96,9 @@ __device__ __forceinline__ uint32_t code_of(float y, float inv) { return __float
 // a stored code at another scale
 __device__ __forceinline__ uint32_t recode(uint32_t code, float ratio) { return code_of((float)(int8_t)code, ratio) & 255; }
 
-constexpr int QHEADS = 4;
-
-// NW waves a workgroup: 4, a page, or 1, a block.  heads: of q, at most QHEADS.
+// NW waves a workgroup: 4, a page, or 1, a block.
 template <typename T, int ROWS, int HD, int NW>
-__global__ __launch_bounds__(64 * NW) void k_append(sp_hipkv_append_args a, int seq_units, int heads) {
+__global__ __launch_bounds__(64 * NW, HD == 256 ? 1 : 2) void k_append(sp_hipkv_append_args a, int seq_units) {
     constexpr int PP = HD / 32, H2 = HD / 2, UNIT = BLOCK8 * NW;
     constexpr bool B8 = ROWS == SP_HIPKV_ROWS_BLOCK8;
     constexpr int COL = 16 * NW + 16;                                     // bytes of a column of V codes in LDS
@@ -99,13 +114,11 @@ __global__ __launch_bounds__(64 * NW) void k_append(sp_hipkv_append_args a, int 
     const int n = min(min(gmem(a.start)[s + 1], a.n_tokens) - t0, min(a.max_tokens, a.max_positions - first)), end = first + n;
     const int p0 = (first / UNIT + j) * UNIT, lp = p0 / PAGE;
     if (n <= 0 || j < 0 || p0 >= end) return;
-    // q (heads h .. h1), k or v, and its head
-    const int gq = a.q_out ? (a.n_heads + heads - 1) / heads : 0;
+    // q, k or v, and its head
     int h = blockIdx.x, kind = 0;
-    if (h >= gq) { h -= gq; kind = 1; }
+    const int nq = a.q_out ? a.n_heads : 0;
+    if (h >= nq) { h -= nq; kind = 1; }
     if (kind == 1 && h >= a.n_kv_heads) { h -= a.n_kv_heads; kind = 2; }
-    if (kind == 0) h *= heads;
-    const int h1 = min(h + heads, a.n_heads);
     const bool stored = kind && !(a.ring_pages && lp + a.ring_pages <= (end - 1) / PAGE);
     if (!stored && !(kind == 0 || (kind == 1 && a.k_out))) return;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), i = lane >> 4, l = lane & 15;
@@ -126,83 +139,9 @@ __global__ __launch_bounds__(64 * NW) void k_append(sp_hipkv_append_args a, int 
         store_values(row, z0);
         store_values(row + H2, z1);
     };
-    // a round's sines and cosines, from the last round's
-    double c[PP], sn[PP], cs[PP], ss[PP];
-    auto start = [&] {
-        #pragma unroll
-        for (int k = 0; k < PP; k++) {
-            const double f = gmem(a.freq)[l * PP + k];
-            turn((double)(b0 + i) * f, c[k], sn[k]);
-            turn(4.0 * f, cs[k], ss[k]);
-        }
-    };
-    auto step = [&] {
-        #pragma unroll
-        for (int k = 0; k < PP; k++) {
-            const double x = fma(c[k], cs[k], -(sn[k] * ss[k]));
-            sn[k] = fma(c[k], ss[k], sn[k] * cs[k]);
-            c[k] = x;
-        }
-    };
-    float w[2][PP];
-    const float *nw = kind ? a.k_norm : a.q_norm;
-    auto weights = [&] {
-        #pragma unroll
-        for (int k = 0; k < PP; k++) { w[0][k] = gmem(nw)[l * PP + k]; w[1][k] = gmem(nw)[H2 + l * PP + k]; }
-    };
-    // norm and rotation of a row (every lane of the 16 comes here)
-    auto prepare = [&](const float (&x)[2][PP], double (&y)[2 * PP]) __attribute__((always_inline)) {
-        #pragma unroll
-        for (int k = 0; k < PP; k++) { y[k] = (double)x[0][k]; y[PP + k] = (double)x[1][k]; }
-        if (nw) {
-            double q = 0.0;
-            #pragma unroll
-            for (int k = 0; k < 2 * PP; k++) q = fma(y[k], y[k], q);
-            #pragma unroll
-            for (int o = 1; o < 16; o <<= 1) q += __shfl_xor(q, o, 64);
-            const double m = 1.0 / sqrt(q * (1.0 / HD) + (double)a.eps);
-            #pragma unroll
-            for (int k = 0; k < PP; k++) { y[k] *= m * (double)w[0][k]; y[PP + k] *= m * (double)w[1][k]; }
-        }
-        if (a.freq) {
-            #pragma unroll
-            for (int k = 0; k < PP; k++) {
-                const double x0 = y[k], x1 = y[PP + k];
-                y[k] = fma(x0, c[k], -(x1 * sn[k]));
-                y[PP + k] = fma(x0, sn[k], x1 * c[k]);
-            }
-        }
-    };
-    if (kind == 0) {
-        if (nw) weights();
-        if (a.freq) start();
-        #pragma unroll
-        for (int r = 0; r < 4; r++) {
-            if (r && a.freq) step();
-            if (!round_live(r)) continue;
-            float x[QHEADS][2][PP];
-            #pragma unroll
-            for (int e = 0; e < QHEADS; e++)
-                if (h + e < h1 && live(r)) {
-                    const T *row = row_of((const T *)a.q, a.q_stride, r, h + e);
-                    load_values(row, x[e][0]);
-                    load_values(row + H2, x[e][1]);
-                }
-            #pragma unroll
-            for (int e = 0; e < QHEADS; e++) {
-                if (h + e >= h1) break;
-                double y[2 * PP];
-                float z[2 * PP];
-                prepare(x[e], y);
-                rounded<T>(y, z);
-                if (live(r)) put(row_of((T *)a.q_out, a.q_out_stride, r, h + e), z);
-            }
-        }
-        return;
-    }
-    const T *src = (const T *)(kind == 1 ? a.k : a.v);
-    const int64_t stride = kind == 1 ? a.k_stride : a.v_stride;
-    float x[4][2][PP];
+    const T *src = (const T *)(kind == 0 ? a.q : kind == 1 ? a.k : a.v);
+    const int64_t stride = kind == 0 ? a.q_stride : kind == 1 ? a.k_stride : a.v_stride;
+    float x[4][2][PP] = {};
     #pragma unroll
     for (int r = 0; r < 4; r++)
         if (live(r)) {
@@ -286,25 +225,66 @@ __global__ __launch_bounds__(64 * NW) void k_append(sp_hipkv_append_args a, int 
         }
         return;
     }
-    if (nw) weights();
-    if (a.freq) start();
-    double y[4][2 * PP], big = 0.0, none = 0.0;                            // none: NaN if some value is not finite
+    // q or k: norm and rotation
+    const float *nw = kind ? a.k_norm : a.q_norm;
+    float w[2][PP];
+    double c[PP], sn[PP], cs[PP], ss[PP], y[B8 ? 4 : 1][2 * PP];         // 8-bit rows wait for their block's scale
+    if (nw) {
+        #pragma unroll
+        for (int k = 0; k < PP; k++) { w[0][k] = gmem(nw)[l * PP + k]; w[1][k] = gmem(nw)[H2 + l * PP + k]; }
+    }
+    if (a.freq) {
+        #pragma unroll
+        for (int k = 0; k < PP; k++) {
+            const double f = gmem(a.freq)[l * PP + k];
+            turn((double)(b0 + i) * f, c[k], sn[k]);
+            turn(4.0 * f, cs[k], ss[k]);
+        }
+    }
+    T *back = (T *)(kind ? a.k_out : a.q_out);
+    const int64_t back_stride = kind ? a.k_out_stride : a.q_out_stride;
+    double big = 0.0, none = 0.0;                                          // none: NaN if some value is not finite
     #pragma unroll
     for (int r = 0; r < 4; r++) {
-        if (r && a.freq) step();
-        if (!round_live(r)) continue;
-        prepare(x[r], y[r]);
+        double (&v)[2 * PP] = y[B8 ? r : 0];
+        if (r && a.freq) {
+            #pragma unroll
+            for (int k = 0; k < PP; k++) {
+                const double t = fma(c[k], cs[k], -(sn[k] * ss[k]));
+                sn[k] = fma(c[k], ss[k], sn[k] * cs[k]);
+                c[k] = t;
+            }
+        }
+        if (NW == 1 && !round_live(r)) continue;
+        #pragma unroll
+        for (int k = 0; k < PP; k++) { v[k] = (double)x[r][0][k]; v[PP + k] = (double)x[r][1][k]; }
+        if (nw) {
+            double q = 0.0;
+            #pragma unroll
+            for (int k = 0; k < 2 * PP; k++) q = fma(v[k], v[k], q);
+            const double m = inv_sqrt(row_sum(q) * (1.0 / HD) + (double)a.eps);
+            #pragma unroll
+            for (int k = 0; k < PP; k++) { v[k] *= m * (double)w[0][k]; v[PP + k] *= m * (double)w[1][k]; }
+        }
+        if (a.freq) {
+            #pragma unroll
+            for (int k = 0; k < PP; k++) {
+                const double x0 = v[k], x1 = v[PP + k];
+                v[k] = fma(x0, c[k], -(x1 * sn[k]));
+                v[PP + k] = fma(x0, sn[k], x1 * c[k]);
+            }
+        }
         if (!live(r)) continue;
         float z[2 * PP];
-        if (a.k_out) {
-            rounded<T>(y[r], z);
-            put(row_of((T *)a.k_out, a.k_out_stride, r, h), z);
+        if (back) {
+            rounded<T>(v, z);
+            put(row_of(back, back_stride, r, h), z);
         }
         if constexpr (B8) {
             #pragma unroll
-            for (int k = 0; k < 2 * PP; k++) { big = fmax(big, fabs(y[r][k])); none = fma(y[r][k], 0.0, none); }
+            for (int k = 0; k < 2 * PP; k++) { big = fmax(big, fabs(v[k])); none = fma(v[k], 0.0, none); }
         } else if (stored) {
-            rounded<float>(y[r], z);
+            rounded<float>(v, z);
             put((float *)page + ((size_t)h * PAGE + BLOCK8 * u + 4 * r + i) * HD + l * PP, z);
         }
     }
@@ -368,11 +348,9 @@ int append_check(const sp_hipkv_append_args *a) {
 
 template <typename T, int ROWS, int NW> hipError_t append_go(const sp_hipkv_append_args &a, hipStream_t s) {
     int seq_units = 0;
-    const int64_t slots = append_slots(a, BLOCK8 * NW, &seq_units), rows = (a.q_out ? a.n_heads : 0) + 2 * a.n_kv_heads;
-    const int heads = slots * rows * NW >= 16384 ? QHEADS : 1;
-    const int groups = (a.q_out ? (a.n_heads + heads - 1) / heads : 0) + 2 * a.n_kv_heads;
+    const int64_t slots = append_slots(a, BLOCK8 * NW, &seq_units);
     return op_launch(a.head_dim == 256 ? k_append<T, ROWS, 256, NW> : a.head_dim == 128 ? k_append<T, ROWS, 128, NW> : k_append<T, ROWS, 64, NW>,
-                     dim3(groups, (uint32_t)slots), dim3(64 * NW), s, a, seq_units, heads);
+                     dim3((a.q_out ? a.n_heads : 0) + 2 * a.n_kv_heads, (uint32_t)slots), dim3(64 * NW), s, a, seq_units);
 }
 template <typename T, int ROWS> hipError_t append_rows(const sp_hipkv_append_args &a, hipStream_t s) {
     return a.max_tokens <= BLOCK8 ? append_go<T, ROWS, 1>(a, s) : append_go<T, ROWS, 4>(a, s);
