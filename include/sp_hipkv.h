@@ -386,7 +386,7 @@ int  sp_hipkv_keep_rows(const sp_hipkv_keep_args *a, void *stream);
  *   SP_HIPKV_F32          f32
  *   SP_HIPKV_BF16         bf16, each result rounded once, to nearest
  * Rows of values start 16-byte aligned: strides count values, are multiples of 4 (bf16: of
- * 8) and at most 2^24.  The tokens of a call are packed: sequence s has tokens start[s] ..
+ * 8) and at most 2^22.  The tokens of a call are packed: sequence s has tokens start[s] ..
  * start[s + 1], at positions cached[s] .. behind what it holds; a sequence may have none.
  * Rows behind the last sequence's tokens stay as they are.
  *

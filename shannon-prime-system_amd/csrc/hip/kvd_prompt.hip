@@ -39,6 +39,9 @@ constexpr float LOG2E_F = 1.44269504088896341f;
 
 constexpr float SLACK = 16.0f;                                           // exponent (base 2) that a weight may reach
 
+// waves that share a row's dims
+constexpr int prompt_split(int hd) { return hd == 256 ? 2 : 1; }
+
 __device__ __forceinline__ float other_half(float x) { return __shfl_xor(x, 32, 64); }
 
 __device__ __forceinline__ bool bf16_finite(uint32_t u) { return (u & 0x7F80) != 0x7F80; }
@@ -55,12 +58,59 @@ __device__ __forceinline__ bool chunk_clean(v4u &c) {
 }
 __device__ __forceinline__ bool finite32(float x) { return (__float_as_uint(x) & 0x7F800000u) != 0x7F800000u; }
 
+// Joins the outputs of the KS parts of RG row groups (maxima m, sums l, exponents by c): the parts'
+// outputs pass LDS (RG KS 32 rows of 32 DT f32), each part's wave sums up every KS-th tile of
+// columns and hands its rows' quotients to put(column tile, index, 4 values).
+template <int RG, int KS, int DT, typename Put>
+__device__ __forceinline__ void join_parts(v16f (&O)[DT], float m, float l, float c, uint8_t *lds, v2f (*s_ml)[32], int wave, int lane, Put &&put) {
+    v4f *x = (v4f *)lds;
+    if (lane < 32) s_ml[wave][lane] = (v2f){m, l};
+    __syncthreads();                                                       // K and V are read
+    #pragma unroll
+    for (int d = 0; d < DT; d++)
+        #pragma unroll
+        for (int i = 0; i < 4; i++) x[((wave * DT + d) * 4 + i) * 64 + lane] = (v4f){O[d][4 * i], O[d][4 * i + 1], O[d][4 * i + 2], O[d][4 * i + 3]};
+    __syncthreads();
+    const int rg = wave % RG, part = wave / RG;
+    float M = -INFINITY, L = 0.0f, f[KS];
+    #pragma unroll
+    for (int k = 0; k < KS; k++) M = fmaxf(M, s_ml[k * RG + rg][lane & 31][0]);
+    #pragma unroll
+    for (int k = 0; k < KS; k++) {
+        const v2f ml = s_ml[k * RG + rg][lane & 31];
+        f[k] = ml[0] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f((ml[0] - M) * c);
+        L += ml[1] == 0.0f ? 0.0f : f[k] * ml[1];                          // NaN sums stay, empty ones add nothing
+    }
+    const float inv = 1.0f / L;
+    #pragma unroll
+    for (int d0 = 0; d0 < DT; d0 += KS) {
+        const int d = d0 + part;
+        if (d >= DT) break;
+        #pragma unroll
+        for (int i = 0; i < 4; i++) {
+            v4f y = {0, 0, 0, 0};
+            #pragma unroll
+            for (int k = 0; k < KS; k++) y += x[(((k * RG + rg) * DT + d) * 4 + i) * 64 + lane] * f[k];
+            const float z[4] = {y[0] * inv, y[1] * inv, y[2] * inv, y[3] * inv};
+            put(d, 4 * i, z);
+        }
+    }
+}
+
 // ---------------------------------------------------------------- bf16
-// K and V come through LDS by direct loads, two tiles deep, with one barrier a tile.
-template <int HD, int NW>
-__global__ __launch_bounds__(64 * NW, HD == 256 ? 1 : 2) void k_prompt16(sp_hipkv_prompt_args a, int slots) {
-    constexpr int BN = HD == 256 ? 32 : 64, BM = 32 * NW, KT = BN / 32, KS = HD / 16, DT = HD / 32, C8 = HD / 8, TB = BN * HD * 2;      // bytes of a tile
+// K and V come through LDS by direct loads, two tiles deep, with one barrier a tile.  A workgroup's waves
+// are RG row groups of 32 times KS parts of a tile's keys, 32 KT of them each; the parts are joined at the
+// end through LDS.  KS > 1 is for calls with too few rows to fill the device, where the way along the keys is what
+// takes the time.
+//
+// Dims of 256 are shared by two waves, as in f32 (below), who hand each other their parts of the scores
+// where the tile's K lay: 2000 tokens of 16 heads of 256 take @ us, 88 with one wave for all
+// dims, which leaves one wave a SIMD.
+template <int HD, int RG, int KS, int KT>
+__global__ __launch_bounds__(64 * RG * KS * prompt_split(HD), 2) void k_prompt16(sp_hipkv_prompt_args a, int slots) {
+    constexpr int SP = prompt_split(HD), NW = RG * KS * SP, BN = 32 * KT * KS, BM = 32 * RG, NS = HD / SP / 16, DT = HD / SP / 32, C8 = HD / 8, TB = BN * HD * 2;      // bytes of a tile
     __shared__ __align__(1024) uint8_t lds[4 * TB];                       // K of even and odd tiles, then V
+    __shared__ v2f s_ml[KS > 1 ? NW : 1][32];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), l32 = lane & 31, half = lane >> 5;
     const int G = a.n_heads / a.n_kv_heads, h = blockIdx.x % a.n_kv_heads;
     // the longest spans first: a sequence's last rows before its first
@@ -69,7 +119,8 @@ __global__ __launch_bounds__(64 * NW, HD == 256 ? 1 : 2) void k_prompt16(sp_hipk
     const int t0 = max(gmem(a.start)[s], 0), n = min(min(gmem(a.start)[s + 1], a.n_tokens) - t0, a.max_tokens);
     const int64_t j = slot - unit_base(a.start, s, G, BM, 1);
     if (n <= 0 || j < 0 || j * BM >= (int64_t)n * G) return;
-    const int R = n * G, r0 = (int)j * BM, wr0 = r0 + wave * 32;
+    const int R = n * G, r0 = (int)j * BM, wr0 = r0 + wave % RG * 32;
+    const int part = wave / RG % KS, dim0 = wave / (RG * KS) * (HD / SP);                 // this wave's keys of a tile, and dims
     const int W = a.window ? a.window : INT32_MAX;
     const int first = r0 / G, last = (min(r0 + BM, R) - 1) / G, w_first = min(wr0, R - 1) / G, w_last = (min(wr0 + 32, R) - 1) / G;
     const int k0 = max(first - W + 1, 0) / BN, k1 = last / BN + 1;
@@ -97,11 +148,11 @@ __global__ __launch_bounds__(64 * NW, HD == 256 ? 1 : 2) void k_prompt16(sp_hipk
     load(kp, a.k_stride, ko, k0, 0);
     load(vp, a.v_stride, vo, k0, 2);
     const int row = min(wr0 + l32, R - 1), tok = row / G;
-    bf8 Q[KS];
+    bf8 Q[NS];
     {
-        const Bf16 *q = (const Bf16 *)a.q + (size_t)(t0 + tok) * a.q_stride + (size_t)(h * G + row % G) * HD + 8 * half;
+        const Bf16 *q = (const Bf16 *)a.q + (size_t)(t0 + tok) * a.q_stride + (size_t)(h * G + row % G) * HD + dim0 + 8 * half;
         #pragma unroll
-        for (int k = 0; k < KS; k++) {
+        for (int k = 0; k < NS; k++) {
             float x[8];
             load_values(q + 16 * k, x);
             Q[k] = __builtin_bit_cast(bf8, (v4u){bf16x2(x[0] * sgn, x[1] * sgn), bf16x2(x[2] * sgn, x[3] * sgn), bf16x2(x[4] * sgn, x[5] * sgn), bf16x2(x[6] * sgn, x[7] * sgn)});
@@ -114,19 +165,19 @@ __global__ __launch_bounds__(64 * NW, HD == 256 ? 1 : 2) void k_prompt16(sp_hipk
     float m = -INFINITY, l = 0.0f;
     // this lane's places in a tile: of K by dims, of V (row (l % 16) / 4 of four, 4 columns of 16, for the
     // transposing reads) by columns
-    int k_at[KS], v_at[DT];
+    int k_at[NS], v_at[DT];
     #pragma unroll
-    for (int k = 0; k < KS; k++) k_at[k] = (l32 * C8 + ((2 * k + half) ^ k_swz(l32))) * 16;
+    for (int k = 0; k < NS; k++) k_at[k] = ((part * 32 * KT + l32) * C8 + ((dim0 / 8 + 2 * k + half) ^ k_swz(l32))) * 16;
     #pragma unroll
     for (int d = 0; d < DT; d++) {
-        const int r = 4 * half + (lane & 15) / 4, col = d * 32 + 16 * (lane >> 4 & 1) + 4 * (lane & 3);
-        v_at[d] = (r * C8 + ((col / 8) ^ v_swz(r))) * 16 + col % 8 * 2;
+        const int r = 4 * half + (lane & 15) / 4, col = dim0 + d * 32 + 16 * (lane >> 4 & 1) + 4 * (lane & 3);
+        v_at[d] = ((part * 32 * KT + r) * C8 + ((col / 8) ^ v_swz(r))) * 16 + col % 8 * 2;
     }
     // V values that were left out of a tile, for the rows that attend them
     auto add_odd = [&](int key0) __attribute__((always_inline)) {
         #pragma unroll 1
-        for (int key = key0; key < min(key0 + BN, n); key++) {
-            const Bf16 *vrow = vp + (size_t)key * a.v_stride + 4 * half;
+        for (int key = key0; key < min(key0 + 32 * KT, n); key++) {
+            const Bf16 *vrow = vp + (size_t)key * a.v_stride + dim0 + 4 * half;
             #pragma unroll
             for (int d = 0; d < DT; d++)
                 #pragma unroll
@@ -148,8 +199,8 @@ __global__ __launch_bounds__(64 * NW, HD == 256 ? 1 : 2) void k_prompt16(sp_hipk
         }
         return bad;
     };
-    auto work = [&](int tile, auto part) __attribute__((always_inline)) {
-        constexpr int BUF = part.value;
+    auto work = [&](int tile, auto buf) __attribute__((always_inline)) {
+        constexpr int BUF = buf.value;
         const bool ragged = tile * BN + BN - 1 > first || tile * BN < last - W + 1;        // some row does not attend it whole
         asm volatile("s_waitcnt vmcnt(0)" : : : "memory");
         __syncthreads();
@@ -159,12 +210,15 @@ __global__ __launch_bounds__(64 * NW, HD == 256 ? 1 : 2) void k_prompt16(sp_hipk
             load(kp, a.k_stride, ko, tile + 1, 1 - BUF);
             load(vp, a.v_stride, vo, tile + 1, 3 - BUF);
         }
-        if (tile * BN > w_last || tile * BN + BN <= w_first - W + 1) return;               // no row of this wave attends any
-        // fragments are read 8 products ahead, the first of V beside the last of K
-        constexpr int NF = 8, NKF = KT * KS, NVF = KT * 2 * DT;
+        const int key0 = tile * BN + part * 32 * KT;                                       // this wave's keys
+        const bool idle = key0 > w_last || key0 + 32 * KT <= w_first - W + 1;              // none that a row of it attends
+        if (SP == 1 && idle) return;
+        // fragments are read up to 8 products ahead, the first of V beside the last of K
+        constexpr int NKF = KT * NS, NVF = KT * 2 * DT, NF = NKF < 8 ? NKF : 8;
+        static_assert(NF <= NVF, "the first NF fragments of V");
         v16f S[KT];
         bf8 F[NF];
-        auto read_k = [&](int x) { return *(const bf8 *)(lds + k_at[x % KS] + BUF * TB + x / KS * 32 * HD * 2); };
+        auto read_k = [&](int x) { return *(const bf8 *)(lds + k_at[x % NS] + BUF * TB + x / NS * 32 * HD * 2); };
         auto read_v = [&](int x) {
             typedef short v8s __attribute__((ext_vector_type(8)));
             const v4s y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4s *)(lds + v_at[x % DT] + (2 + BUF) * TB + 16 * (x / DT) * HD * 2));
@@ -176,17 +230,32 @@ __global__ __launch_bounds__(64 * NW, HD == 256 ? 1 : 2) void k_prompt16(sp_hipk
         __builtin_amdgcn_sched_group_barrier(0x100, NF, 0);
         #pragma unroll
         for (int x = 0; x < NKF; x++) {
-            S[x / KS] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(F[x % NF], Q[x % KS], x % KS ? S[x / KS] : zero, 0, 0, 0);
+            S[x / NS] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(F[x % NF], Q[x % NS], x % NS ? S[x / NS] : zero, 0, 0, 0);
             F[x % NF] = x + NF < NKF ? read_k(x + NF) : read_v(x + NF - NKF);
             __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
             if (x + NF < NKF) __builtin_amdgcn_sched_group_barrier(0x100, 1, 0); else __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
         }
-        if (tile * BN + BN - 1 > w_first || tile * BN < w_last - W + 1) {
+        if constexpr (SP == 2) {                                           // both waves' parts of the scores, in the tile's K
+            static_assert(KT * KS == 1 && NW * 4096 <= TB, "a tile of 32 keys, whose K the waves' parts fit");
+            __syncthreads();
+            v4f *x = (v4f *)(lds + BUF * TB);
+            #pragma unroll
+            for (int i = 0; i < 4; i++) x[(wave * 4 + i) * 64 + lane] = (v4f){S[0][4 * i], S[0][4 * i + 1], S[0][4 * i + 2], S[0][4 * i + 3]};
+            __syncthreads();
+            #pragma unroll
+            for (int i = 0; i < 4; i++) {
+                const v4f y = x[((wave ^ RG) * 4 + i) * 64 + lane];
+                #pragma unroll
+                for (int e = 0; e < 4; e++) S[0][4 * i + e] += y[e];
+            }
+            if (idle) return;
+        }
+        if (key0 + 32 * KT - 1 > w_first || key0 < w_last - W + 1) {
             #pragma unroll
             for (int u = 0; u < KT; u++)
                 #pragma unroll
                 for (int i = 0; i < 16; i++) {
-                    const int key = tile * BN + u * 32 + 8 * (i / 4) + 4 * half + i % 4;
+                    const int key = key0 + u * 32 + 8 * (i / 4) + 4 * half + i % 4;
                     S[u][i] = key <= tok && key > tok - W ? S[u][i] : -INFINITY;
                 }
         }
@@ -226,25 +295,32 @@ __global__ __launch_bounds__(64 * NW, HD == 256 ? 1 : 2) void k_prompt16(sp_hipk
             __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
             if (x + NF < NVF) __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
         }
-        if (odd) add_odd(tile * BN);
+        if (odd) add_odd(key0);
     };
     for (int tile = k0; tile < k1; tile += 2) {
         work(tile, std::integral_constant<int, 0>{});
         if (tile + 1 < k1) work(tile + 1, std::integral_constant<int, 1>{});
     }
+    l += other_half(l);
     const int r = wr0 + l32;
-    const float inv = 1.0f / (l + other_half(l));
-    if (r >= R) return;
-    Bf16 *o = (Bf16 *)a.out + (size_t)(t0 + tok) * a.out_stride + (size_t)(h * G + r % G) * HD + 4 * half;
-    #pragma unroll
-    for (int d = 0; d < DT; d++)
+    Bf16 *o = (Bf16 *)a.out + (size_t)(t0 + r / G) * a.out_stride + (size_t)(h * G + r % G) * HD + dim0 + 4 * half;
+    if constexpr (KS == 1) {
+        const float inv = 1.0f / l;
+        if (r >= R) return;
         #pragma unroll
-        for (int i = 0; i < 16; i += 4) {
-            float x[4];
+        for (int d = 0; d < DT; d++)
             #pragma unroll
-            for (int y = 0; y < 4; y++) x[y] = O[d][i + y] * inv;
-            store_values(o + d * 32 + 2 * i, x);
-        }
+            for (int i = 0; i < 16; i += 4) {
+                float x[4];
+                #pragma unroll
+                for (int y = 0; y < 4; y++) x[y] = O[d][i + y] * inv;
+                store_values(o + d * 32 + 2 * i, x);
+            }
+    } else {
+        join_parts<RG, KS, DT>(O, m, l, c, lds, s_ml, wave, lane, [&](int d, int i, const float (&x)[4]) {
+            if (r < R) store_values(o + d * 32 + 2 * i, x);
+        });
+    }
 }
 
 // ---------------------------------------------------------------- f32
@@ -298,7 +374,7 @@ __device__ __forceinline__ v16f mfma_halves(const Halves &a, const Halves &b, v1
 // to work while it waits (2047 tokens with a window of 1024: 200 us).
 template <int HD, int NW>
 __global__ __launch_bounds__(64 * NW, 2) void k_prompt32(sp_hipkv_prompt_args a, int slots) {
-    constexpr int BN = 32, SPLIT = HD == 256 ? 2 : 1, RG = NW / SPLIT, BM = 32 * RG, KS = HD / SPLIT / 16, DT = HD / SPLIT / 32, C8 = HD / 8, RAW = BN * HD * 4, PIECE = BN * HD * 2, NC = BN * C8 / (64 * NW);
+    constexpr int BN = 32, SPLIT = prompt_split(HD), RG = NW / SPLIT, BM = 32 * RG, KS = HD / SPLIT / 16, DT = HD / SPLIT / 32, C8 = HD / 8, RAW = BN * HD * 4, PIECE = BN * HD * 2, NC = BN * C8 / (64 * NW);
     constexpr float SLACK32 = 8.0f;                                       // weights times 2^7 are f16 numbers
     __shared__ __align__(1024) uint8_t raw[2 * RAW], lds[4 * PIECE];      // K, V; K's h and l, V's h and l
     __shared__ __align__(16) float s_kf[BN], s_vf[NW][BN];
@@ -555,12 +631,23 @@ int prompt_check(const sp_hipkv_prompt_args *a) {
            serve_rows(who, a, a->v, a->v_stride, a->n_kv_heads) || serve_rows(who, a, a->out, a->out_stride, a->n_heads);
 }
 
+// rows of a workgroup: units that a call's rows may fall into
+int64_t prompt_slots(const sp_hipkv_prompt_args &a, int rows) { return (int64_t)a.n_tokens * (a.n_heads / a.n_kv_heads) / rows + a.n_seqs; }
+
 template <typename T, int HD> hipError_t prompt_go(const sp_hipkv_prompt_args &a, hipStream_t s) {
-    constexpr int ROWS = 128;                                              // of a workgroup
-    const int slots = (int)((int64_t)a.n_tokens * (a.n_heads / a.n_kv_heads) / ROWS) + a.n_seqs;
-    const dim3 grid((uint32_t)((int64_t)slots * a.n_kv_heads));
-    if constexpr (sizeof(T) == 4) return op_launch(k_prompt32<HD, HD == 256 ? 8 : 4>, grid, dim3(HD == 256 ? 512 : 256), s, a, slots);
-    else return op_launch(k_prompt16<HD, 4>, grid, dim3(256), s, a, slots);
+#define PROMPT_RUN(K, ROWS, THREADS) \
+    op_launch(K, dim3((uint32_t)(prompt_slots(a, ROWS) * a.n_kv_heads)), dim3(THREADS), s, a, (int)prompt_slots(a, ROWS))
+    if constexpr (sizeof(T) == 4) return PROMPT_RUN((k_prompt32<HD, 4 * prompt_split(HD)>), 128, 256 * prompt_split(HD));
+    else if constexpr (HD == 256) return PROMPT_RUN((k_prompt16<HD, 2, 1, 1>), 64, 256);
+    else {
+        // A unit holds two workgroups of four waves: with fewer rows than half of them take, the keys of 64 rows
+        // are shared by four waves each, a workgroup of eight a unit (1000 tokens of 16 and 8 heads of
+        // 128: 19.0 us for 24.4; 500 of 32: 14.0 for 16.5; 1000 of 32, too many: 28.2 for 26.9; 130 tokens, too
+        // few keys: 9.5 for 9.3).
+        if (a.max_tokens >= 192 && prompt_slots(a, 64) * a.n_kv_heads <= 256) return PROMPT_RUN((k_prompt16<HD, 2, 4, 1>), 64, 512);
+        return PROMPT_RUN((k_prompt16<HD, 4, 1, 2>), 128, 256);
+    }
+#undef PROMPT_RUN
 }
 template <typename T> hipError_t prompt_type(const sp_hipkv_prompt_args &a, hipStream_t s) {
     return a.head_dim == 256 ? prompt_go<T, 256>(a, s) : a.head_dim == 128 ? prompt_go<T, 128>(a, s) : prompt_go<T, 64>(a, s);

@@ -100,8 +100,8 @@ template <typename A> int serve_check(const char *who, const A *a) {
 // a packed array of values: heads x head_dim of them a token
 template <typename A> int serve_rows(const char *who, const A *a, const void *p, int64_t stride, int heads) {
     OP_NEED(p, "null array");
-    OP_NEED(stride >= (int64_t)heads * a->head_dim && stride % (a->type == SP_HIPKV_F32 ? 4 : 8) == 0 && stride <= 1 << 24,
-            "a stride is below heads * head_dim, above 2^24 or does not keep rows 16-byte aligned");
+    OP_NEED(stride >= (int64_t)heads * a->head_dim && stride % (a->type == SP_HIPKV_F32 ? 4 : 8) == 0 && stride <= 1 << 22,
+            "a stride is below heads * head_dim, above 2^22 or does not keep rows 16-byte aligned");
     OP_NEED(aligned(p, 16), "misaligned array");
     return 0;
 }
