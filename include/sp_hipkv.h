@@ -445,13 +445,14 @@ int  sp_hipkv_append(const sp_hipkv_append_args *a, void *stream);
 
 /* Attention of whole prompts from packed q, k, v (after norm and rotation): token t of a
  * sequence, counted from the sequence's first, attends tokens [max(0, t - window + 1), t]
- * of it: out = sum_p softmax_p(scale q.k_p) v_p, sums in f32.  f32 products are made of
- * bf16 pieces, to 2^-25; of bf16 values the weights are rounded to bf16 before they
- * multiply v.  Tokens that a token does not attend do not reach it whatever they hold.  A
- * value that is not finite in one that it attends leaves it without a finite value, in k
- * everywhere (but for bf16 scores of -inf, whose weight is 0), in v in the value's column
- * (magnitudes from 2^90 on in v may count as that, f32 ones above 3.38e38 in k, and scores
- * that f32 does not hold). */
+ * of it: out = sum_p softmax_p(scale q.k_p) v_p, sums in f32.  An f32 value takes part as two
+ * f16 numbers, exact to 2^-22 of it and 2^-39 of its head's largest; a weight of f32 values, times
+ * the largest value of its v, to 2^-22 and to 2^-32 of the largest such that the row of q attends.
+ * Of bf16 values the weights are rounded to bf16 before they multiply v.  Tokens that a token does not
+ * attend do not reach it whatever they hold.  A value that is not finite in one that it
+ * attends leaves it without a finite value, in k everywhere (but for bf16 scores of -inf,
+ * whose weight is 0), in v in the value's column (magnitudes from 2^90 on in v, and f32 ones from
+ * 2^100 on in k, may count as that, and scores that f32 does not hold). */
 typedef struct sp_hipkv_prompt_args {
     int32_t n_heads, n_kv_heads;    /* at most 4096, and 16 q heads for each kv head */
     int32_t head_dim;               /* 64, 128 or 256 */

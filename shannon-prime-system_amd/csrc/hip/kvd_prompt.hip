@@ -104,7 +104,7 @@ __device__ __forceinline__ void join_parts(v16f (&O)[DT], float m, float l, floa
 // takes the time.
 //
 // Dims of 256 are shared by two waves, as in f32 (below), who hand each other their parts of the scores
-// where the tile's K lay: 2000 tokens of 16 heads of 256 take @ us, 88 with one wave for all
+// where the tile's K lay: 2000 tokens of 16 heads of 256 take 79 us, 88 with one wave for all
 // dims, which leaves one wave a SIMD.
 template <int HD, int RG, int KS, int KT>
 __global__ __launch_bounds__(64 * RG * KS * prompt_split(HD), 2) void k_prompt16(sp_hipkv_prompt_args a, int slots) {
@@ -325,7 +325,7 @@ __global__ __launch_bounds__(64 * RG * KS * prompt_split(HD), 2) void k_prompt16
 
 // ---------------------------------------------------------------- f32
 // An f32 as two f16: h, its rounding, and l, that of what is left, of values times the power of two
-// that brings their row's largest below 2^15: x = h + l but for 2^-22 of itself, or 2^-40 of the largest.
+// that brings their row's largest to 2^14 .. 2^15: x = h + l but for 2^-22 of itself, or 2^-39 of the largest.
 typedef _Float16 h2 __attribute__((ext_vector_type(2)));
 typedef _Float16 h8 __attribute__((ext_vector_type(8)));
 struct Halves { h8 h, l; };
@@ -336,7 +336,11 @@ template <typename X> __device__ __forceinline__ Halves halves_of(X &&x) {      
         const float a = x(2 * k), b = x(2 * k + 1);
         const h2 y = __builtin_convertvector((v2f){a, b}, h2);
         h[k] = __builtin_bit_cast(uint32_t, y);
-        l[k] = __builtin_bit_cast(uint32_t, __builtin_convertvector((v2f){fmaf((float)y[0], -1.0f, a), fmaf((float)y[1], -1.0f, b)}, h2));
+        // a - h as one instruction each (the compiler takes two)
+        float c, d;
+        asm("v_fma_mix_f32 %0, %1, -1.0, %2 op_sel_hi:[1,0,0]" : "=v"(c) : "v"(h[k]), "v"(a));
+        asm("v_fma_mix_f32 %0, %1, -1.0, %2 op_sel:[1,0,0] op_sel_hi:[1,0,0]" : "=v"(d) : "v"(h[k]), "v"(b));
+        l[k] = __builtin_bit_cast(uint32_t, __builtin_convertvector((v2f){c, d}, h2));
     }
     return {__builtin_bit_cast(h8, h), __builtin_bit_cast(h8, l)};
 }
@@ -344,15 +348,19 @@ template <typename X> __device__ __forceinline__ Halves halves_of(X &&x) {      
 __device__ __forceinline__ uint32_t row_exp(float big) { return min(max(__float_as_uint(big) >> 23, 16u), 254u); }
 __device__ __forceinline__ float row_up(uint32_t e) { return __uint_as_float((268u - e) << 23); }
 __device__ __forceinline__ float row_down(uint32_t e) { return __uint_as_float((e - 14u) << 23); }
-// the largest over N = 8, 16 or 32 neighbouring lanes
-template <int N> __device__ __forceinline__ float lanes_max(float x) {
-    auto step = [&](auto ctrl) { x = fmaxf(x, __uint_as_float(dpp32<decltype(ctrl)::value, 0xF>(__float_as_uint(x), 0))); };
+// the largest over N = 8, 16 or 32 neighbouring lanes, of numbers that are not negative (as bits: one instruction a step)
+template <int N> __device__ __forceinline__ float lanes_max(float y) {
+    uint32_t x = __float_as_uint(y);
+    auto step = [&](auto ctrl) { x = max(x, dpp32<decltype(ctrl)::value, 0xF>(x, 0)); };
     step(std::integral_constant<int, 0xB1>{});                            // quad_perm 1,0,3,2
     step(std::integral_constant<int, 0x4E>{});                            // quad_perm 2,3,0,1
     step(std::integral_constant<int, 0x141>{});                           // row_half_mirror
     if constexpr (N > 8) step(std::integral_constant<int, 0x140>{});      // row_mirror
-    if constexpr (N > 16) x = fmaxf(x, __shfl_xor(x, 16, 64));
-    return x;
+    if constexpr (N > 16) {
+        const v2u z = __builtin_bit_cast(v2u, __builtin_amdgcn_permlane16_swap(x, x, false, false));
+        x = max(z[0], z[1]);
+    }
+    return __uint_as_float(x);
 }
 __device__ __forceinline__ float abs_max(const v4f &a, const v4f &b) {
     return fmaxf(fmaxf(fmaxf(fabsf(a[0]), fabsf(a[1])), fmaxf(fabsf(a[2]), fabsf(a[3]))), fmaxf(fmaxf(fabsf(b[0]), fabsf(b[1])), fmaxf(fabsf(b[2]), fabsf(b[3]))));
@@ -363,22 +371,26 @@ __device__ __forceinline__ v16f mfma_halves(const Halves &a, const Halves &b, v1
     return __builtin_amdgcn_mfma_f32_32x32x16_f16(a.h, b.h, c, 0, 0, 0);
 }
 
-// A tile of 32 keys comes into LDS as it is, by direct loads, while the one before is worked on, and is
+// A tile of 32 KS keys comes into LDS as it is, by direct loads, while the one before is worked on, and is
 // taken apart by all threads: rows of K and of V each by a factor of their own, whose inverses join the
-// scores and, relative to the largest so far (as with the scores' maximum, the output is scaled when it
-// moves), the weights.
+// scores and the weights.  The weights so become numbers of V's range, of which f16 pairs hold 2^-32 of the
+// largest that a row of q has met: each has a factor 2^ge of its own for them, which (as the scores'
+// maximum does) moves when they leave the range that it leaves them, with the output.  One factor for
+// all rows would let a large V that one row attends, or none, take the others' bits.
 //
 // Dims of 256 are shared by two waves, each 128 of the scores' products and of the output's columns,
 // who hand each other their parts of the scores through LDS, where K lay as it came (the next K is
 // sent for after that): one wave with all of them needs over 256 registers, so that a SIMD has no other
-// to work while it waits (2047 tokens with a window of 1024: 200 us).
-template <int HD, int NW>
-__global__ __launch_bounds__(64 * NW, 2) void k_prompt32(sp_hipkv_prompt_args a, int slots) {
-    constexpr int BN = 32, SPLIT = prompt_split(HD), RG = NW / SPLIT, BM = 32 * RG, KS = HD / SPLIT / 16, DT = HD / SPLIT / 32, C8 = HD / 8, RAW = BN * HD * 4, PIECE = BN * HD * 2, NC = BN * C8 / (64 * NW);
+// to work while it waits (2047 tokens of 16 and 8 heads with a window of 1024: 200 us; so 184, 167
+// at the rate of a library's f32 product, 62 at a third of the f16 one's).
+template <int HD, int RG, int KS>
+__global__ __launch_bounds__(64 * RG * KS * prompt_split(HD), 2) void k_prompt32(sp_hipkv_prompt_args a, int slots) {
+    constexpr int SPLIT = prompt_split(HD), NW = RG * KS * SPLIT, BN = 32 * KS, BM = 32 * RG, NS = HD / SPLIT / 16, DT = HD / SPLIT / 32, C8 = HD / 8, RAW = BN * HD * 4, PIECE = BN * HD * 2, NC = BN * C8 / (64 * NW);
     constexpr float SLACK32 = 8.0f;                                       // weights times 2^7 are f16 numbers
-    __shared__ __align__(1024) uint8_t raw[2 * RAW], lds[4 * PIECE];      // K, V; K's h and l, V's h and l
-    __shared__ __align__(16) float s_kf[BN], s_vf[NW][BN];
-    __shared__ uint32_t s_ve[BN];
+    __shared__ __align__(1024) uint8_t raw[2 * RAW + 4 * PIECE];          // K, V; K's h and l, V's h and l
+    __shared__ __align__(16) float s_kf[BN], s_vf[BN];
+    __shared__ v2f s_ml[KS > 1 ? NW : 1][32];
+    uint8_t *lds = raw + 2 * RAW;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), l32 = lane & 31, half = lane >> 5;
     const int G = a.n_heads / a.n_kv_heads, h = blockIdx.x % a.n_kv_heads;
     // the longest spans first: a sequence's last rows before its first
@@ -387,7 +399,8 @@ __global__ __launch_bounds__(64 * NW, 2) void k_prompt32(sp_hipkv_prompt_args a,
     const int t0 = max(gmem(a.start)[s], 0), n = min(min(gmem(a.start)[s + 1], a.n_tokens) - t0, a.max_tokens);
     const int64_t j = slot - unit_base(a.start, s, G, BM, 1);
     if (n <= 0 || j < 0 || j * BM >= (int64_t)n * G) return;
-    const int R = n * G, r0 = (int)j * BM, wr0 = r0 + wave % RG * 32, dim0 = wave / RG * (HD / SPLIT);            // this wave's rows and dims
+    const int R = n * G, r0 = (int)j * BM, wr0 = r0 + wave % RG * 32;
+    const int part = wave / RG % KS, dim0 = wave / (RG * KS) * (HD / SPLIT);              // this wave's keys of a tile, and dims
     const int W = a.window ? a.window : INT32_MAX;
     const int first = r0 / G, last = (min(r0 + BM, R) - 1) / G, w_first = min(wr0, R - 1) / G, w_last = (min(wr0 + 32, R) - 1) / G;
     const int k0 = max(first - W + 1, 0) / BN, k1 = last / BN + 1;
@@ -396,9 +409,10 @@ __global__ __launch_bounds__(64 * NW, 2) void k_prompt32(sp_hipkv_prompt_args a,
     int ko[NI], vo[NI];
     #pragma unroll
     for (int i = 0; i < NI; i++) {
-        const int at = (wave * NI + i) * 256 + lane * 4;
-        ko[i] = (at / HD * (int)a.k_stride + at % HD) * 4;
-        vo[i] = (at / HD * (int)a.v_stride + at % HD) * 4;
+        // of a row first the even 16 bytes, then the odd: a thread's 32 bytes are then read without bank conflicts
+        const int at = (wave * NI + i) * 64 + lane, r = at / (2 * C8), p = at % (2 * C8), unit = p < C8 ? 2 * p : 2 * (p - C8) + 1;
+        ko[i] = (r * (int)a.k_stride + 4 * unit) * 4;
+        vo[i] = (r * (int)a.v_stride + 4 * unit) * 4;
     }
     const uint32_t raw0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) const uint8_t *)raw + wave * NI * 1024;
     auto load = [&](const float *p, int64_t stride, const int (&off)[NI], int tile, int to) __attribute__((always_inline)) {
@@ -412,31 +426,31 @@ __global__ __launch_bounds__(64 * NW, 2) void k_prompt32(sp_hipkv_prompt_args a,
     // q's halves; its factor joins that of the scores, c >= 0 (scale <= 0 goes into q's sign, or makes q zero)
     const float sgn = a.scale > 0 ? 1.0f : a.scale < 0 ? -1.0f : 0.0f;
     const int row = min(wr0 + l32, R - 1), tok = row / G;
-    Halves Q[KS];
+    Halves Q[NS];
     float c;
     {
         const float *q = (const float *)a.q + (size_t)(t0 + tok) * a.q_stride + (size_t)(h * G + row % G) * HD + dim0 + 8 * half;
         float x[8];
         float big = 0.0f;                                                  // (a NaN makes its own way into the scores)
         #pragma unroll
-        for (int k = 0; k < KS; k++) {
+        for (int k = 0; k < NS; k++) {
             load_values(q + 16 * k, x);
             #pragma unroll
             for (int i = 0; i < 8; i++) big = fmaxf(big, fabsf(x[i]));
         }
-        asm volatile("" : : : "memory");                                  // read again, not kept: KS x 8 registers
+        asm volatile("" : : : "memory");                                  // read again, not kept: NS x 8 registers
         big = fmaxf(big, other_half(big));
         if constexpr (SPLIT == 2) {                                        // one factor for both parts of a row
             ((float *)lds)[wave * 32 + l32] = big;
             __syncthreads();
-            big = fmaxf(big, ((float *)lds)[(wave ^ RG) * 32 + l32]);
+            big = fmaxf(big, ((float *)lds)[(wave ^ RG * KS) * 32 + l32]);
             __syncthreads();
         }
         const uint32_t e = row_exp(big);
         const float up = sgn * row_up(e);
         c = (a.scale == 0 ? LOG2E_F : fabsf(a.scale) * LOG2E_F) * row_down(e);
         #pragma unroll
-        for (int k = 0; k < KS; k++) {
+        for (int k = 0; k < NS; k++) {
             load_values(q + 16 * k, x);
             Q[k] = halves_of([&](int i) { return x[i] * up; });
         }
@@ -447,18 +461,19 @@ __global__ __launch_bounds__(64 * NW, 2) void k_prompt32(sp_hipkv_prompt_args a,
     #pragma unroll
     for (int d = 0; d < DT; d++) O[d] = zero;
     float m = -INFINITY, l = 0.0f;
-    uint32_t E = 16;                                                       // the exponent that O is relative to
+    float tm = 0.0f;                                                       // the largest weight times factor of V so far
+    int ge = 126;                                                          // O is relative to 2^-ge
     // A row's 16-byte chunks lie in an order that spreads a column of K over the banks, and
     // the 64-byte runs of four rows of V
     auto k_swz = [](int r) { return HD == 64 ? r >> 1 & 7 : r & 15; };
     auto v_swz = [](int r) { return HD == 64 ? (r >> 1 & 1) << 2 : (r & 3) << 2; };
-    int k_at[KS], v_at[DT];
+    int k_at[NS], v_at[DT];
     #pragma unroll
-    for (int k = 0; k < KS; k++) k_at[k] = (l32 * C8 + ((dim0 / 8 + 2 * k + half) ^ k_swz(l32))) * 16;
+    for (int k = 0; k < NS; k++) k_at[k] = ((part * 32 + l32) * C8 + ((dim0 / 8 + 2 * k + half) ^ k_swz(l32))) * 16;
     #pragma unroll
     for (int d = 0; d < DT; d++) {
         const int r = 4 * half + (lane & 15) / 4, col = dim0 + d * 32 + 16 * (lane >> 4 & 1) + 4 * (lane & 3);
-        v_at[d] = (r * C8 + ((col / 8) ^ v_swz(r))) * 16 + col % 8 * 2;
+        v_at[d] = ((part * 32 + r) * C8 + ((col / 8) ^ v_swz(r))) * 16 + col % 8 * 2;
     }
     for (int tile = k0; tile < k1; tile++) {
         const bool ragged = tile * BN + BN - 1 > first || tile * BN < last - W + 1;        // some row does not attend it whole
@@ -468,10 +483,11 @@ __global__ __launch_bounds__(64 * NW, 2) void k_prompt32(sp_hipkv_prompt_args a,
         #pragma unroll
         for (int i = 0; i < NC; i++) {
             const int id = threadIdx.x + 64 * NW * i, r = id / C8, ch = id % C8;
-            const v4f x0 = *(const v4f *)(raw + id * 32), x1 = *(const v4f *)(raw + id * 32 + 16);
-            v4f y0 = *(const v4f *)(raw + RAW + id * 32), y1 = *(const v4f *)(raw + RAW + id * 32 + 16);
+            const v4f *at = (const v4f *)raw + r * 2 * C8 + ch;
+            const v4f x0 = at[0], x1 = at[C8];
+            v4f y0 = at[RAW / 16], y1 = at[RAW / 16 + C8];
             float kb = abs_max(x0, x1), vb = abs_max(y0, y1);
-            if (ragged || __any(vb == INFINITY)) {                         // a row of V has the factor of its finite values
+            if (ragged || __any(!(vb < INFINITY))) {                         // a row of V has the factor of its finite values
                 vb = 0.0f;
                 #pragma unroll
                 for (int k = 0; k < 4; k++) {
@@ -485,7 +501,7 @@ __global__ __launch_bounds__(64 * NW, 2) void k_prompt32(sp_hipkv_prompt_args a,
             }
             const uint32_t ke = row_exp(lanes_max<C8>(kb)), ve = row_exp(lanes_max<C8>(vb));
             const float ku = row_up(ke), vu = row_up(ve);
-            if (ch == 0) { s_kf[r] = row_down(ke); s_ve[r] = ve; }
+            if (ch == 0) { s_kf[r] = row_down(ke); s_vf[r] = __uint_as_float((ve - 15) << 23); }       // (2^(ve - 142), half of what V was divided by)
             // (an infinity in K becomes h = inf, l = NaN)
             const Halves K = halves_of([&](int k) { return (k < 4 ? x0[k & 3] : x1[k & 3]) * ku; });
             const Halves V = halves_of([&](int k) { return (k < 4 ? y0[k & 3] : y1[k & 3]) * vu; });
@@ -499,18 +515,43 @@ __global__ __launch_bounds__(64 * NW, 2) void k_prompt32(sp_hipkv_prompt_args a,
             if (SPLIT == 1) load(kp, a.k_stride, ko, tile + 1, 0);
             load(vp, a.v_stride, vo, tile + 1, RAW);
         }
-        const bool idle = tile * BN > w_last || tile * BN + BN <= w_first - W + 1;         // no row of this wave attends any
+        const int key0 = tile * BN + part * 32;                            // this wave's keys
+        const bool idle = key0 > w_last || key0 + 32 <= w_first - W + 1;   // none that a row of it attends
+        // fragments are read NF products ahead, the first of V beside the last of K
+        constexpr int NF = 4, NVF = 2 * DT;
+        constexpr bool AHEAD = SPLIT == 1;                                 // (no registers for V's first fragments beside two waves' sums)
+        Halves F[NF];
+        auto read_k = [&](int x) { return Halves{*(const h8 *)(lds + k_at[x]), *(const h8 *)(lds + k_at[x] + PIECE)}; };
+        auto read_v = [&](int x) {
+            typedef short v8s __attribute__((ext_vector_type(8)));
+            h8 V[2];
+            #pragma unroll
+            for (int z = 0; z < 2; z++) {
+                const uint8_t *at = lds + v_at[x % DT] + (2 + z) * PIECE + 16 * (x / DT) * HD * 2;
+                const v4s p = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4s *)at), q = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4s *)(at + 8 * HD * 2));
+                V[z] = __builtin_bit_cast(h8, __builtin_shufflevector(p, q, 0, 1, 2, 3, 4, 5, 6, 7));
+            }
+            return Halves{V[0], V[1]};
+        };
         v16f S = zero;
         if (!idle) {
             #pragma unroll
-            for (int k = 0; k < KS; k++) S = mfma_halves(Halves{*(const h8 *)(lds + k_at[k]), *(const h8 *)(lds + k_at[k] + PIECE)}, Q[k], S);
+            for (int x = 0; x < NF; x++) F[x] = read_k(x);
+            __builtin_amdgcn_sched_group_barrier(0x100, 2 * NF, 0);
+            #pragma unroll
+            for (int x = 0; x < NS; x++) {
+                S = mfma_halves(F[x % NF], Q[x], S);
+                if (x + NF < NS) F[x % NF] = read_k(x + NF); else if (AHEAD) F[x % NF] = read_v(x + NF - NS);
+                __builtin_amdgcn_sched_group_barrier(0x008, 3, 0);
+                if (x + NF < NS) __builtin_amdgcn_sched_group_barrier(0x100, 2, 0); else if (AHEAD) __builtin_amdgcn_sched_group_barrier(0x100, 4, 0);
+            }
         }
         if constexpr (SPLIT == 2) {
             float *x = (float *)raw + wave * 1024 + lane * 4;
             #pragma unroll
             for (int i = 0; i < 16; i += 4) *(v4f *)(x + i * 64) = (v4f){S[i], S[i + 1], S[i + 2], S[i + 3]};
             __syncthreads();
-            const float *y = (const float *)raw + (wave ^ RG) * 1024 + lane * 4;
+            const float *y = (const float *)raw + (wave ^ RG * KS) * 1024 + lane * 4;
             #pragma unroll
             for (int i = 0; i < 16; i += 4) {
                 const v4f z = *(const v4f *)(y + i * 64);
@@ -521,77 +562,75 @@ __global__ __launch_bounds__(64 * NW, 2) void k_prompt32(sp_hipkv_prompt_args a,
             if (tile + 1 < k1) load(kp, a.k_stride, ko, tile + 1, 0);
         }
         if (idle) continue;
-        const uint32_t ve = s_ve[l32], top = (uint32_t)wave_allmax_i((int)ve);
         // this lane's keys: 8 (i / 4) + 4 half + i % 4
         #pragma unroll
         for (int i = 0; i < 16; i += 4) {
-            const v4f x = *(const v4f *)(s_kf + 2 * i + 4 * half);
+            const v4f x = *(const v4f *)(s_kf + part * 32 + 2 * i + 4 * half);
             #pragma unroll
             for (int k = 0; k < 4; k++) S[i + k] *= x[k];
         }
-        if (tile * BN + BN - 1 > w_first || tile * BN < w_last - W + 1) {
+        if (key0 + 31 > w_first || key0 < w_last - W + 1) {
+            asm volatile("");                                              // a branch: whole tiles do without this
             #pragma unroll
             for (int i = 0; i < 16; i++) {
-                const int key = tile * BN + 8 * (i / 4) + 4 * half + i % 4;
+                const int key = key0 + 8 * (i / 4) + 4 * half + i % 4;
                 S[i] = key <= tok && key > tok - W ? S[i] : -INFINITY;
             }
         }
         float mx = S[0];
         #pragma unroll
         for (int i = 1; i < 16; i++) mx = fmaxf(mx, S[i]);
-        if (__builtin_expect(__any(mx > m + slack), 0)) {
+        float al = 1.0f, mt = 0.0f;
+        const bool moved = __any(mx > m + slack);
+        if (__builtin_expect(moved, 0)) {
             mx = fmaxf(mx, other_half(mx));
-            const float mn = fmaxf(m, mx), al = mn == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f((m - mn) * c);
+            const float mn = fmaxf(m, mx);
+            al = mn == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f((m - mn) * c);
             m = mn;
             l *= al;
-            #pragma unroll
-            for (int d = 0; d < DT; d++)
-                #pragma unroll
-                for (int i = 0; i < 16; i++) O[d][i] *= al;
         }
         const float nm = m == -INFINITY ? 0.0f : -m * c;
         #pragma unroll
-        for (int i = 0; i < 16; i++) {
-            S[i] = __builtin_amdgcn_exp2f(fmaf(S[i], c, nm));
-            l += S[i];
+        for (int i = 0; i < 16; i += 4) {
+            const v4f x = *(const v4f *)(s_vf + part * 32 + 2 * i + 4 * half);
+            #pragma unroll
+            for (int k = 0; k < 4; k++) {
+                const float w = __builtin_amdgcn_exp2f(fmaf(S[i + k], c, nm));
+                l += w;
+                S[i + k] = w * x[k];
+                mt = fmaxf(mt, S[i + k]);
+            }
         }
-        if (top > E) {
-            const float f = E + 126 < top ? 0.0f : __uint_as_float((127u + E - top) << 23);
-            E = top;
+        if (__builtin_expect(moved || __any(ldexpf(mt, ge) > 32768.0f), 0)) {
+            tm = fmaxf(tm * al, mt);
+            tm = fmaxf(tm, other_half(tm));
+            const int to = 134 - min(max((int)(__float_as_uint(tm) >> 23), 8), 254);
+            const float f = ldexpf(al, to - ge);
+            ge = to;
             #pragma unroll
             for (int d = 0; d < DT; d++)
                 #pragma unroll
                 for (int i = 0; i < 16; i++) O[d][i] *= f;
         }
-        // the keys' factors relative to E, 2^(7 + ve - E), each formed by one lane
-        s_vf[wave][l32] = ve + 126 < E ? 0.0f : __uint_as_float((134u + ve - E) << 23);
-        __builtin_amdgcn_wave_barrier();
         #pragma unroll
-        for (int i = 0; i < 16; i += 4) {
-            const v4f x = *(const v4f *)(s_vf[wave] + 2 * i + 4 * half);
-            #pragma unroll
-            for (int k = 0; k < 4; k++) S[i + k] *= x[k];
-        }
+        for (int i = 0; i < 16; i++) S[i] = ldexpf(S[i], ge);
         Halves P[2];
         #pragma unroll
         for (int e = 0; e < 2; e++) P[e] = halves_of([&](int k) { return S[8 * e + k]; });
-        #pragma unroll
-        for (int e = 0; e < 2; e++)
+        if (!AHEAD) {
             #pragma unroll
-            for (int d = 0; d < DT; d++) {
-                typedef short v8s __attribute__((ext_vector_type(8)));
-                h8 V[2];
-                #pragma unroll
-                for (int x = 0; x < 2; x++) {
-                    const uint8_t *at = lds + v_at[d] + (2 + x) * PIECE + 16 * e * HD * 2;
-                    const v4s y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4s *)at), z = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4s *)(at + 8 * HD * 2));
-                    V[x] = __builtin_bit_cast(h8, __builtin_shufflevector(y, z, 0, 1, 2, 3, 4, 5, 6, 7));
-                }
-                O[d] = mfma_halves(Halves{V[0], V[1]}, P[e], O[d]);
-            }
+            for (int x = 0; x < NF; x++) F[x] = read_v(x);
+        }
+        #pragma unroll
+        for (int x = 0; x < NVF; x++) {
+            O[x % DT] = mfma_halves(F[x % NF], P[x / DT], O[x % DT]);
+            if (x + NF < NVF) F[x % NF] = read_v(x + NF);
+            __builtin_amdgcn_sched_group_barrier(0x008, 3, 0);
+            if (x + NF < NVF) __builtin_amdgcn_sched_group_barrier(0x100, 4, 0);
+        }
         if (odd) {                                                          // V values that were left out, for the rows that attend them
             #pragma unroll 1
-            for (int key = tile * BN; key < min(tile * BN + BN, n); key++) {
+            for (int key = key0; key < min(key0 + 32, n); key++) {
                 const float *vrow = vp + (size_t)key * a.v_stride + dim0 + 4 * half;
                 #pragma unroll
                 for (int d = 0; d < DT; d++)
@@ -605,19 +644,30 @@ __global__ __launch_bounds__(64 * NW, 2) void k_prompt32(sp_hipkv_prompt_args a,
             }
         }
     }
+    l += other_half(l);
     const int r = wr0 + l32;
-    const float inv = ldexpf(1.0f / (l + other_half(l)), (int)E - 148);
-    if (r >= R) return;
-    float *o = (float *)a.out + (size_t)(t0 + tok) * a.out_stride + (size_t)(h * G + r % G) * HD + dim0 + 4 * half;
-    #pragma unroll
-    for (int d = 0; d < DT; d++)
+    float *o = (float *)a.out + (size_t)(t0 + r / G) * a.out_stride + (size_t)(h * G + r % G) * HD + dim0 + 4 * half;
+    if constexpr (KS == 1) {
+        const float inv = 1.0f / l;
+        if (r >= R) return;
         #pragma unroll
-        for (int i = 0; i < 16; i += 4) {
-            float x[4];
+        for (int d = 0; d < DT; d++)
             #pragma unroll
-            for (int y = 0; y < 4; y++) x[y] = O[d][i + y] * inv;
-            store_values(o + d * 32 + 2 * i, x);
-        }
+            for (int i = 0; i < 16; i += 4) {
+                float x[4];
+                #pragma unroll
+                for (int y = 0; y < 4; y++) x[y] = ldexpf(O[d][i + y] * inv, 1 - ge);
+                store_values(o + d * 32 + 2 * i, x);
+            }
+    } else {
+        #pragma unroll
+        for (int d = 0; d < DT; d++)
+            #pragma unroll
+            for (int i = 0; i < 16; i++) O[d][i] = ldexpf(O[d][i], 1 - ge);                 // each part has its own
+        join_parts<RG, KS, DT>(O, m, l, c, raw, s_ml, wave, lane, [&](int d, int i, const float (&x)[4]) {
+            if (r < R) store_values(o + d * 32 + 2 * i, x);
+        });
+    }
 }
 
 int prompt_check(const sp_hipkv_prompt_args *a) {
@@ -637,7 +687,20 @@ int64_t prompt_slots(const sp_hipkv_prompt_args &a, int rows) { return (int64_t)
 template <typename T, int HD> hipError_t prompt_go(const sp_hipkv_prompt_args &a, hipStream_t s) {
 #define PROMPT_RUN(K, ROWS, THREADS) \
     op_launch(K, dim3((uint32_t)(prompt_slots(a, ROWS) * a.n_kv_heads)), dim3(THREADS), s, a, (int)prompt_slots(a, ROWS))
-    if constexpr (sizeof(T) == 4) return PROMPT_RUN((k_prompt32<HD, 4 * prompt_split(HD)>), 128, 256 * prompt_split(HD));
+    if constexpr (sizeof(T) == 4) {
+        // Up to some workgroups a unit it is the way along the keys that takes the time, and a workgroup of eight
+        // waves walks 64 keys (dims of 64: 128) in the time that four take for 32.  One sequence of n tokens,
+        // 16 and 8 heads of 128: 28 us for 30 at n = 250, 68 for 89 at 1000, 123 for 168 at 2000, but 21.3 for
+        // 20.3 at 130; 32 and 8 heads: 148 for 174 at 2000 (504 workgroups), 767 for 701 at 5000.  Dims of 64,
+        // 32 and 8 heads: 45 for 53 at 1000 (504), 129 for 101 at 2000.  Of short sequences the longer
+        // last tiles cost more: six of 50 to 400 tokens take 36 us for 41 (216) and 52.5 for 47.9 (384).
+        if constexpr (HD < 256) {
+            constexpr int KS = HD == 128 ? 2 : 4, RG = 8 / KS;
+            const int64_t units = prompt_slots(a, 32 * RG) * a.n_kv_heads;
+            if (a.max_tokens >= 192 && units <= (a.n_tokens >= (int64_t)256 * a.n_seqs ? 512 : 256)) return PROMPT_RUN((k_prompt32<HD, RG, KS>), 32 * RG, 512);
+        }
+        return PROMPT_RUN((k_prompt32<HD, 4, 1>), 128, 256 * prompt_split(HD));
+    }
     else if constexpr (HD == 256) return PROMPT_RUN((k_prompt16<HD, 2, 1, 1>), 64, 256);
     else {
         // A unit holds two workgroups of four waves: with fewer rows than half of them take, the keys of 64 rows

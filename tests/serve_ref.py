@@ -264,12 +264,15 @@ def softmax_rows(z):
 def prompt_attention(q, k, v, counts, window, scale, typ):
     """[tokens][heads][hd] in 64 bits and a bound on the kernel's error.
 
-    Scores: six products a term (one of bf16 values), each exact to 2^-25 of itself, 6 hd
-    additions in f32: off by (6 hd + 8) u scale sum |q||k| (factor and subtraction of the
-    maximum among the 8), and by 4 u of the largest |score difference| for the exponential's
-    argument: d.  Weights are so off by 4 d (e^(2 d) - 1 for small d, above and below), sums over
-    n positions by (12 n + 64) u.  bf16 weights are rounded before they multiply v: b; the output
-    once: half a step of it."""
+    Scores: f32 values are two f16 numbers each, off by 2^-22 = 4 u and by 2^-39 of their
+    row's largest; of four products the smallest, 4 u of the term, is left out: 12 u; 3 hd additions
+    in f32 (bf16: hd) of at most 2 u: off by (6 hd + 20) u scale sum |q||k| (factor and subtraction of
+    the maximum among the 20), by what the rows' largest bring, and by 4 u of the largest |score
+    difference| for the exponential's argument: d.  Weights are so off by 4 d (e^(2 d) - 1 for small d,
+    above and below), sums over n positions by (12 n + 64) u.  f32 weights times their V rows' powers of two,
+    which the rows' largest are below the double of, are off by 2^-32 of the largest such, each
+    times less than 2: n 2^-31 of the largest weight times |v|.  bf16 weights are rounded
+    before they multiply v: b; the output once: half a step of it."""
     out, tol = np.zeros(q.shape), np.zeros(q.shape)
     NH, hd = q.shape[1:]
     G, start = NH // k.shape[1], packed_start(counts)
@@ -281,9 +284,14 @@ def prompt_attention(q, k, v, counts, window, scale, typ):
                 z = K @ x * scale
                 w = softmax_rows(z)
                 o, r = w @ V, w @ np.abs(V)
-                d = (6 * hd + 8) * U * abs(scale) * (np.abs(K) @ np.abs(x)).max() + 4 * U * np.abs(z - z.max()).max()
+                d = (6 * hd + 20) * U * abs(scale) * (np.abs(K) @ np.abs(x)).max() + 4 * U * np.abs(z - z.max()).max()
+                if typ == spkv.F32:
+                    d += 2.0 ** -39 * abs(scale) * (np.abs(x).max() * np.abs(K).sum(1) + np.abs(K).max(1) * np.abs(x).sum()).max()
                 out[a + t, h] = o
                 tol[a + t, h] = (4 * d + (12 * len(z) + 64) * U) * r + U * np.abs(o)
+                if typ == spkv.F32:
+                    big = w * np.abs(V).max(1)
+                    tol[a + t, h] += 2.0 ** -31 * len(z) * big.max() + 2.0 ** -39 * big.sum()
                 if typ == spkv.BF16:
                     tol[a + t, h] = (tol[a + t, h] + B * r) * (1 + B) + B * np.abs(o)
     return out, tol

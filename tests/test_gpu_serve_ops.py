@@ -209,6 +209,49 @@ def test_prompt_values_that_are_not_attended(typ, hd, bad):
 
 
 @pytest.mark.parametrize("typ", TYPES)
+@pytest.mark.parametrize("hd,counts", [(64, [90, 40]), (128, [90, 40]), (256, [90, 40]), (64, [300]), (128, [300])])
+@pytest.mark.parametrize("big", [1e10, 1e25, 3e38])
+def test_prompt_large_values_that_are_not_attended(typ, hd, counts, big):
+    """Finite, and far above what the tokens before them, behind their window and of other
+    sequences attend, whose bounds do not know of them."""
+    g = rng(23, hd)
+    T = sum(counts)
+    k, v = g.standard_normal((T, 2, hd)), g.standard_normal((T, 2, hd))
+    v[33, 0] *= big / 10
+    v[60, 1, 3] = -big
+    k[75, 1] = big * 0.9
+    p = Prompt(g, typ, hd, 2, counts, window=20, k=k, v=v)
+    got, (want, tol) = p.run(), p.want()
+    fine = np.ones(T, bool)
+    fine[33:min(53, counts[0])] = fine[60:80] = fine[75:95] = False    # those that attend them (some of 1e25 and more are not finite)
+    assert fine.sum() > 60 and (np.abs(got - want)[fine] <= tol[fine]).all()
+    if big == 1e10:
+        few = ~fine
+        few[75:95] = False
+        assert (np.abs(got - want)[few] <= tol[few]).all()
+
+
+@pytest.mark.parametrize("typ", TYPES)
+@pytest.mark.parametrize("hd", [64, 128, 256])
+@pytest.mark.parametrize("low", [1, 40, 200])
+def test_prompt_large_values_of_small_weight(typ, hd, low):
+    """V of 1e20 where the weights are e^-80, first or for long the only ones: what is left of them
+    is 1e-15 beside the others' 1."""
+    g = rng(24, hd, low)
+    q, k, v = g.standard_normal((300, 2, hd)), g.standard_normal((300, 1, hd)), g.standard_normal((300, 1, hd))
+    q[..., 0], k[..., 0], k[:low, 0, 0] = 30, 0, -80 / 30 * hd ** 0.5
+    v[:low] *= 1e20
+    Prompt(g, typ, hd, 2, [300], nkv=1, q=q, k=k, v=v).check()
+
+
+@pytest.mark.parametrize("typ", TYPES)
+@pytest.mark.parametrize("hd,n,nkv", [(64, 400, 48), (128, 300, 64), (128, 250, 160)])
+def test_prompt_long_with_many_heads(typ, hd, n, nkv):
+    """Too many rows for a workgroup a unit."""
+    Prompt(rng(25, hd), typ, hd, 1, [n], nkv=nkv).check()
+
+
+@pytest.mark.parametrize("typ", TYPES)
 def test_prompt_nothing_read_behind_the_last_row(typ):
     """k and v that end with the last sequence: what lies behind is not a row of theirs."""
     g = rng(20)
