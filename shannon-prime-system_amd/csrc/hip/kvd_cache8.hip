@@ -1,7 +1,7 @@
 // kvd_cache8.hip -- attention of new tokens over the 8-bit paged cache.
 //
 // The q heads of a kv head share its K and V: the rows of one kv head are r = token G + q
-// head of the group, 16 to a matrix tile, RT tiles to a workgroup.  Its waves take the pages of a
+// head of the group, 16 of them, a matrix tile, to a workgroup.  Its waves take the pages of a
 // range (a split) in turn, each with a running maximum, sum and output of its own; they meet
 // in LDS at the end, the splits in k_cache_merge.
 //
@@ -57,11 +57,12 @@ __device__ __forceinline__ float rows_max(float x) {
     return fmaxf(__uint_as_float(b[0]), __uint_as_float(b[1]));
 }
 
-template <typename T, int HD, int RT>
+template <typename T, int HD>
 __global__ __launch_bounds__(64 * CACHE_WAVES, HD == 256 ? 1 : 2) void k_cache(sp_hipkv_cache_args a, int groups, int nsplit, int pages) {
-    constexpr int ND = DIG<T>, KS = HD / 64, CT = HD / 16, NW = CACHE_WAVES, NT = 64 * NW, QE = (RT * KS + NW - 1) / NW, UB = HD == 256 ? 2 : 4;
-    __shared__ v4i s_q[RT * KS * ND][64];
-    __shared__ uint32_t s_big[RT * KS][16];
+    static_assert(HD / 64 <= CACHE_WAVES, "a wave for every 64 dims of q");
+    constexpr int ND = DIG<T>, KS = HD / 64, CT = HD / 16, NW = CACHE_WAVES, NT = 64 * NW, UB = HD == 256 ? 2 : 4;
+    __shared__ v4i s_q[KS * ND][64];
+    __shared__ uint32_t s_big[KS][16];
     __shared__ __align__(16) float s_o[NW][16][HD];
     __shared__ float s_m[NW][16], s_l[NW][16], s_M[16], s_L[16];
     __shared__ const uint8_t *s_page[CACHE_PAGES];
@@ -74,11 +75,11 @@ __global__ __launch_bounds__(64 * CACHE_WAVES, HD == 256 ? 1 : 2) void k_cache(s
     const void *const *table = gmem(a.tables)[s];                          // (here: one wait for all of a sequence's numbers)
     const int t0 = max(gmem(a.start)[s], 0), cached = min(max(gmem(a.cached)[s], 0), a.max_positions);
     const int n = min(min(gmem(a.start)[s + 1], a.n_tokens) - t0, min(a.max_tokens, a.max_positions - cached)), end = cached + n;
-    const int R = n * G, r0 = grp * RT * 16;
+    const int R = n * G, r0 = grp * 16;
     if (r0 >= R) return;
     // the positions that this workgroup's rows see: first row's window start to the last row's own
     const int W = a.window ? a.window : INT32_MAX;
-    const int at0 = cached + r0 / G, at1 = cached + (min(r0 + RT * 16, R) - 1) / G, lo = max(at0 - W + 1, 0);
+    const int at0 = cached + r0 / G, at1 = cached + (min(r0 + 16, R) - 1) / G, lo = max(at0 - W + 1, 0);
     // this split's pages (of a sequence shorter than the longest there are proportionally fewer)
     const int pg0 = lo / PAGE;
     const uint32_t np = at1 / PAGE + 1 - pg0;
@@ -88,7 +89,7 @@ __global__ __launch_bounds__(64 * CACHE_WAVES, HD == 256 ? 1 : 2) void k_cache(s
     auto row_of = [&](int r) { return (size_t)(t0 + r / G) * a.n_heads + h * G + r % G; };
     if (nsplit > 1 && b0 >= b1) {
         const int r = r0 + threadIdx.x;
-        if (threadIdx.x < RT * 16 && r < R) *gmem((v2f *)(pml + 2 * (row_of(r) * nsplit + split))) = (v2f){-INFINITY, 0.0f};
+        if (threadIdx.x < 16 && r < R) *gmem((v2f *)(pml + 2 * (row_of(r) * nsplit + split))) = (v2f){-INFINITY, 0.0f};
         return;
     }
     const size_t kat = (size_t)h * PAGE * HD, vat = (size_t)(a.n_kv_heads + h) * PAGE * HD, sat = (size_t)a.n_kv_heads * 2 * PAGE * HD + 16 * h;
@@ -108,18 +109,14 @@ __global__ __launch_bounds__(64 * CACHE_WAVES, HD == 256 ? 1 : 2) void k_cache(s
     };
     auto page_at = [&](int lp) { return (const uint8_t *)gmem(table)[a.ring_pages ? lp % a.ring_pages : lp]; };
     for (int i = threadIdx.x; i < b1 - b0; i += NT) s_page[i] = page_at(b0 + i);
-    // q's digits, [row tile][64 dims][digit][lane] 16 bytes: lane (g, l) has row l, dims 64 e + 16 g ..
+    // q's digits, [64 dims][digit][lane] 16 bytes: lane (g, l) has row l, dims 64 e + 16 g ..
     const bool any_page = b0 + wave < b1;
-    float x[QE][2][8];
-    int at[RT];
-    #pragma unroll
-    for (int i = 0; i < QE; i++) {
-        const int te = wave + NW * i, r = min(r0 + te / KS * 16 + l16, R - 1);
-        if (te < RT * KS) {
-            const T *q = (const T *)a.q + (size_t)(t0 + r / G) * a.q_stride + (size_t)(h * G + r % G) * HD + 64 * (te % KS) + 16 * g;
-            load_values(q, x[i][0]);
-            load_values(q + 8, x[i][1]);
-        }
+    float x[2][8];
+    if (wave < KS) {
+        const int r = min(r0 + l16, R - 1);
+        const T *q = (const T *)a.q + (size_t)(t0 + r / G) * a.q_stride + (size_t)(h * G + r % G) * HD + 64 * wave + 16 * g;
+        load_values(q, x[0]);
+        load_values(q + 8, x[1]);
     }
     __builtin_amdgcn_sched_barrier(0);
     if (any_page) {                                                        // on their way while q is taken apart
@@ -128,219 +125,189 @@ __global__ __launch_bounds__(64 * CACHE_WAVES, HD == 256 ? 1 : 2) void k_cache(s
         load_v(pg);
     }
     __builtin_amdgcn_sched_barrier(0);
-    #pragma unroll
-    for (int i = 0; i < QE; i++) {
+    if (wave < KS) {
         uint32_t big = 0;                                                  // as bits: NaN is above infinity
         #pragma unroll
-        for (int k = 0; k < 16; k++) big = max(big, __float_as_uint(x[i][k / 8][k % 8]) & 0x7FFFFFFFu);
+        for (int k = 0; k < 16; k++) big = max(big, __float_as_uint(x[k / 8][k % 8]) & 0x7FFFFFFFu);
         big = max(big, (uint32_t)__shfl_xor((int)big, 16, 64));
         big = max(big, (uint32_t)__shfl_xor((int)big, 32, 64));
-        if (wave + NW * i < RT * KS && lane < 16) s_big[wave + NW * i][l16] = big;
+        if (lane < 16) s_big[wave][l16] = big;
     }
     __syncthreads();
-    float qs[RT];
-    auto row_big = [&](int t) {
-        uint32_t big = 0;
-        #pragma unroll
-        for (int e = 0; e < KS; e++) big = max(big, s_big[t * KS + e][l16]);
-        return big;
-    };
-    auto row_up = [&](uint32_t big) { return fminf(DIGITS<T> / __uint_as_float(big), 3e38f); };    // (of zeros and the smallest denormals the largest)
+    uint32_t big = 0;
     #pragma unroll
-    for (int t = 0; t < RT; t++) {
-        at[t] = cached + min(r0 + t * 16 + l16, R - 1) / G;
-        const uint32_t big = row_big(t);
-        qs[t] = big < 0x7F800000u ? a.scale * LOG2E_F / row_up(big) : NAN;
-    }
-    #pragma unroll
-    for (int i = 0; i < QE; i++) {
-        const int te = wave + NW * i;
-        if (te >= RT * KS) break;
-        const float up = row_up(row_big(te / KS));
+    for (int e = 0; e < KS; e++) big = max(big, s_big[e][l16]);
+    const float up = fminf(DIGITS<T> / __uint_as_float(big), 3e38f);       // (of zeros and the smallest denormals the largest)
+    const float qs = big < 0x7F800000u ? a.scale * LOG2E_F / up : NAN;
+    const int at = cached + min(r0 + l16, R - 1) / G;
+    if (wave < KS) {
         v4i q[ND];
         #pragma unroll
         for (int k = 0; k < 4; k++) {
             uint32_t w[4], p[ND];
             #pragma unroll
-            for (int j = 0; j < 4; j++) w[j] = (uint32_t)(int)rintf(x[i][k / 2][4 * (k % 2) + j] * up) + (ND == 3 ? 0x808080u : 0x8080u);
+            for (int j = 0; j < 4; j++) w[j] = (uint32_t)(int)rintf(x[k / 2][4 * (k % 2) + j] * up) + (ND == 3 ? 0x808080u : 0x8080u);
             byte_planes(w, p);
             #pragma unroll
             for (int d = 0; d < ND; d++) q[d][k] = (int)(p[d] ^ 0x80808080u);
         }
         #pragma unroll
-        for (int d = 0; d < ND; d++) s_q[te * ND + d][lane] = q[d];
+        for (int d = 0; d < ND; d++) s_q[wave * ND + d][lane] = q[d];
     }
-    v4f O[RT][CT];
-    float m[RT], l[RT];
+    v4f O[CT];
+    float m = -INFINITY, l = 0.0f;
     #pragma unroll
-    for (int t = 0; t < RT; t++) {
-        m[t] = -INFINITY; l[t] = 0.0f;
-        #pragma unroll
-        for (int c = 0; c < CT; c++) O[t][c] = (v4f){0, 0, 0, 0};
-    }
+    for (int c = 0; c < CT; c++) O[c] = (v4f){0, 0, 0, 0};
     __syncthreads();
     for (int b = b0 + wave; b < b1; b += NW) {
         const bool more = b + NW < b1;
         const uint8_t *pn = uniform(s_page[(more ? b + NW : b) - b0]);
         // some row of the workgroup does not see the page whole
         const bool ragged = b * PAGE + PAGE - 1 > at0 || b * PAGE < at1 - W + 1;
-        float S[RT][4][4];
+        float S[4][4];
         #pragma unroll
-        for (int t = 0; t < RT; t++)
+        for (int u0 = 0; u0 < 4; u0 += UB) {
+            asm volatile("" : : : "memory");                           // q's digits are read again: 12 registers for each 64 dims
+            v4i acc[UB][ND] = {};
             #pragma unroll
-            for (int u0 = 0; u0 < 4; u0 += UB) {
-                asm volatile("" : : : "memory");                           // q's digits are read again: 12 registers for each 64 dims
-                v4i acc[UB][ND] = {};
+            for (int e = 0; e < KS; e++) {
+                v4i q[ND];
                 #pragma unroll
-                for (int e = 0; e < KS; e++) {
-                    v4i q[ND];
-                    #pragma unroll
-                    for (int d = 0; d < ND; d++) q[d] = s_q[(t * KS + e) * ND + d][lane];
-                    #pragma unroll
-                    for (int u = 0; u < UB; u++)
-                        #pragma unroll
-                        for (int d = 0; d < ND; d++) acc[u][d] = __builtin_amdgcn_mfma_i32_16x16x64_i8(K[u0 + u][e], q[d], acc[u][d], 0, 0, 0);
-                }
+                for (int d = 0; d < ND; d++) q[d] = s_q[e * ND + d][lane];
                 #pragma unroll
-                for (int u = 0; u < UB; u++) {
-                    const float f = qs[t] * fmaf(ks[u0 + u], 0.0f, ks[u0 + u]);       // NaN of an infinite scale
+                for (int u = 0; u < UB; u++)
                     #pragma unroll
-                    for (int i = 0; i < 4; i++) {
-                        if constexpr (ND == 3) S[t][u0 + u][i] = f * joined(acc[u][0][i], acc[u][1][i], acc[u][2][i]);
-                        else S[t][u0 + u][i] = f * joined(acc[u][0][i], acc[u][1][i]);
-                    }
+                    for (int d = 0; d < ND; d++) acc[u][d] = __builtin_amdgcn_mfma_i32_16x16x64_i8(K[u0 + u][e], q[d], acc[u][d], 0, 0, 0);
+            }
+            #pragma unroll
+            for (int u = 0; u < UB; u++) {
+                const float f = qs * fmaf(ks[u0 + u], 0.0f, ks[u0 + u]);       // NaN of an infinite scale
+                #pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    if constexpr (ND == 3) S[u0 + u][i] = f * joined(acc[u][0][i], acc[u][1][i], acc[u][2][i]);
+                    else S[u0 + u][i] = f * joined(acc[u][0][i], acc[u][1][i]);
                 }
             }
+        }
         __builtin_amdgcn_sched_barrier(0);
         if (more) load_k(pn);
         __builtin_amdgcn_sched_barrier(0);
-        v4i Pd[RT][ND];
-        float back[RT];
-        #pragma unroll
-        for (int t = 0; t < RT; t++) {
-            uint32_t seen = 0xFFFF;
-            if (ragged) {
-                seen = 0;
-                #pragma unroll
-                for (int k = 0; k < 16; k++) {
-                    const int p = b * PAGE + 16 * (k / 4) + 4 * g + k % 4;
-                    const bool on = p <= at[t] && p > at[t] - W;
-                    seen |= (uint32_t)on << k;
-                    S[t][k / 4][k % 4] = on ? S[t][k / 4][k % 4] : -INFINITY;
-                }
-            }
-            float mx = -INFINITY;
+        v4i Pd[ND];
+        uint32_t seen = 0xFFFF;
+        if (ragged) {
+            seen = 0;
             #pragma unroll
-            for (int k = 0; k < 16; k++) mx = fmaxf(mx, S[t][k / 4][k % 4]);
-            if (__any(mx > m[t] + 16.0f)) {
-                mx = rows_max(mx);
-                const float mn = fmaxf(m[t], mx), al = mn == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m[t] - mn);
-                m[t] = mn;
-                l[t] *= al;
-                #pragma unroll
-                for (int i = 0; i < 4; i++) {                              // O's rows are 4 g + i
-                    const float f = __shfl(al, 4 * g + i, 64);
-                    #pragma unroll
-                    for (int c = 0; c < CT; c++) O[t][c][i] *= f;
-                }
-            }
-            const float ms = m[t] == -INFINITY ? 0.0f : m[t];
-            float top = 0.0f;
-            #pragma unroll
-            for (int u = 0; u < 4; u++) {
-                #pragma unroll
-                for (int i = 0; i < 4; i++) {
-                    const float w = __builtin_amdgcn_exp2f(S[t][u][i] - ms);
-                    l[t] += w;
-                    S[t][u][i] = w * vs[u];
-                }
-                if ((__float_as_uint(vs[u]) & 0x7F800000u) == 0x7F800000u) {  // uniform: a scale that is not finite
-                    if (seen >> 4 * u & 15) l[t] = NAN;
-                    #pragma unroll
-                    for (int i = 0; i < 4; i++) S[t][u][i] = 0.0f;
-                }
-                #pragma unroll
-                for (int i = 0; i < 4; i++) top = fmaxf(top, S[t][u][i]);
-            }
-            top = rows_max(top);
-            // weights to integers up to DIGITS; 2^23 + x has x in its low bits, half a digit more in each but the last byte makes digits of them
-            top = fmaxf(top, 1e-30f);
-            const float up = DIGITS<T> / top;
-            back[t] = top * (1.0f / DIGITS<T>);
-            #pragma unroll
-            for (int u = 0; u < 4; u++) {
-                uint32_t w[4], p[ND];
-                #pragma unroll
-                for (int i = 0; i < 4; i++) w[i] = __float_as_uint(fmaf(S[t][u][i], up, 8388608.0f)) + (ND == 3 ? 0x8080u : 0x80u);
-                byte_planes(w, p);
-                #pragma unroll
-                for (int d = 0; d < ND; d++) Pd[t][d][u] = (int)(d < ND - 1 ? p[d] ^ 0x80808080u : p[d]);
+            for (int k = 0; k < 16; k++) {
+                const int p = b * PAGE + 16 * (k / 4) + 4 * g + k % 4;
+                const bool on = p <= at && p > at - W;
+                seen |= (uint32_t)on << k;
+                S[k / 4][k % 4] = on ? S[k / 4][k % 4] : -INFINITY;
             }
         }
+        float mx = -INFINITY;
         #pragma unroll
-        for (int t = 0; t < RT; t++) {
-            float f[4];
+        for (int k = 0; k < 16; k++) mx = fmaxf(mx, S[k / 4][k % 4]);
+        if (__any(mx > m + 16.0f)) {
+            mx = rows_max(mx);
+            const float mn = fmaxf(m, mx), al = mn == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m - mn);
+            m = mn;
+            l *= al;
             #pragma unroll
-            for (int i = 0; i < 4; i++) f[i] = __shfl(back[t], 4 * g + i, 64);
-            #pragma unroll
-            for (int c = 0; c < CT; c++) {
-                v4i acc[ND];
+            for (int i = 0; i < 4; i++) {                              // O's rows are 4 g + i
+                const float f = __shfl(al, 4 * g + i, 64);
                 #pragma unroll
-                for (int d = 0; d < ND; d++) acc[d] = __builtin_amdgcn_mfma_i32_16x16x64_i8(Pd[t][d], V[c], (v4i){0, 0, 0, 0}, 0, 0, 0);
-                #pragma unroll
-                for (int i = 0; i < 4; i++) {
-                    if constexpr (ND == 3) O[t][c][i] = fmaf(f[i], joined(acc[0][i], acc[1][i], acc[2][i]), O[t][c][i]);
-                    else O[t][c][i] = fmaf(f[i], joined(acc[0][i], acc[1][i]), O[t][c][i]);
-                }
-                if (c % 2) asm volatile("" : "+v"(O[t][c - 1]), "+v"(O[t][c]));       // here, not behind all columns' products: their registers
+                for (int c = 0; c < CT; c++) O[c][i] *= f;
             }
+        }
+        const float ms = m == -INFINITY ? 0.0f : m;
+        float top = 0.0f;
+        #pragma unroll
+        for (int u = 0; u < 4; u++) {
+            #pragma unroll
+            for (int i = 0; i < 4; i++) {
+                const float w = __builtin_amdgcn_exp2f(S[u][i] - ms);
+                l += w;
+                S[u][i] = w * vs[u];
+            }
+            if ((__float_as_uint(vs[u]) & 0x7F800000u) == 0x7F800000u) {  // uniform: a scale that is not finite
+                if (seen >> 4 * u & 15) l = NAN;
+                #pragma unroll
+                for (int i = 0; i < 4; i++) S[u][i] = 0.0f;
+            }
+            #pragma unroll
+            for (int i = 0; i < 4; i++) top = fmaxf(top, S[u][i]);
+        }
+        top = rows_max(top);
+        // weights to integers up to DIGITS; 2^23 + x has x in its low bits, half a digit more in each but the last byte makes digits of them
+        top = fmaxf(top, 1e-30f);
+        const float up = DIGITS<T> / top;
+        const float back = top * (1.0f / DIGITS<T>);
+        #pragma unroll
+        for (int u = 0; u < 4; u++) {
+            uint32_t w[4], p[ND];
+            #pragma unroll
+            for (int i = 0; i < 4; i++) w[i] = __float_as_uint(fmaf(S[u][i], up, 8388608.0f)) + (ND == 3 ? 0x8080u : 0x80u);
+            byte_planes(w, p);
+            #pragma unroll
+            for (int d = 0; d < ND; d++) Pd[d][u] = (int)(d < ND - 1 ? p[d] ^ 0x80808080u : p[d]);
+        }
+        float f[4];
+        #pragma unroll
+        for (int i = 0; i < 4; i++) f[i] = __shfl(back, 4 * g + i, 64);
+        #pragma unroll
+        for (int c = 0; c < CT; c++) {
+            v4i acc[ND];
+            #pragma unroll
+            for (int d = 0; d < ND; d++) acc[d] = __builtin_amdgcn_mfma_i32_16x16x64_i8(Pd[d], V[c], (v4i){0, 0, 0, 0}, 0, 0, 0);
+            #pragma unroll
+            for (int i = 0; i < 4; i++) {
+                if constexpr (ND == 3) O[c][i] = fmaf(f[i], joined(acc[0][i], acc[1][i], acc[2][i]), O[c][i]);
+                else O[c][i] = fmaf(f[i], joined(acc[0][i], acc[1][i]), O[c][i]);
+            }
+            if (c % 2) asm volatile("" : "+v"(O[c - 1]), "+v"(O[c]));       // here, not behind all columns' products: their registers
         }
         __builtin_amdgcn_sched_barrier(0);
         if (more) load_v(pn);
         __builtin_amdgcn_sched_barrier(0);
     }
-    // join the waves, a row tile at a time
+    // join the waves
+    l += __shfl_xor(l, 16, 64);
+    l += __shfl_xor(l, 32, 64);
+    if (lane < 16) { s_m[wave][l16] = m; s_l[wave][l16] = l; }
     #pragma unroll
-    for (int t = 0; t < RT; t++) {
-        l[t] += __shfl_xor(l[t], 16, 64);
-        l[t] += __shfl_xor(l[t], 32, 64);
-        if (t) __syncthreads();
-        if (lane < 16) { s_m[wave][l16] = m[t]; s_l[wave][l16] = l[t]; }
+    for (int c = 0; c < CT; c++)
         #pragma unroll
-        for (int c = 0; c < CT; c++)
-            #pragma unroll
-            for (int i = 0; i < 4; i++) s_o[wave][4 * g + i][16 * c + l16] = O[t][c][i];
-        __syncthreads();
-        if (threadIdx.x < 16) {
-            float M = s_m[0][l16], L = 0.0f;
-            #pragma unroll
-            for (int w = 1; w < NW; w++) M = fmaxf(M, s_m[w][l16]);
-            const float Ms = M == -INFINITY ? 0.0f : M;
-            #pragma unroll
-            for (int w = 0; w < NW; w++) {
-                const float f = __builtin_amdgcn_exp2f(s_m[w][l16] - Ms);
-                L += s_l[w][l16] != 0.0f ? f * s_l[w][l16] : 0.0f;          // NaN sums stay, empty ones add nothing
-                s_m[w][l16] = f;
-            }
-            s_M[l16] = M; s_L[l16] = L;
+        for (int i = 0; i < 4; i++) s_o[wave][4 * g + i][16 * c + l16] = O[c][i];
+    __syncthreads();
+    if (threadIdx.x < 16) {
+        float M = s_m[0][l16], L = 0.0f;
+        #pragma unroll
+        for (int w = 1; w < NW; w++) M = fmaxf(M, s_m[w][l16]);
+        const float Ms = M == -INFINITY ? 0.0f : M;
+        #pragma unroll
+        for (int w = 0; w < NW; w++) {
+            const float f = __builtin_amdgcn_exp2f(s_m[w][l16] - Ms);
+            L += s_l[w][l16] != 0.0f ? f * s_l[w][l16] : 0.0f;          // NaN sums stay, empty ones add nothing
+            s_m[w][l16] = f;
         }
-        __syncthreads();
-        for (int i = threadIdx.x; i < 16 * HD / 4; i += NT) {
-            const int k = i / (HD / 4), c = i % (HD / 4) * 4, r = r0 + t * 16 + k;
-            if (r >= R) continue;
-            v4f x = {0, 0, 0, 0};
-            #pragma unroll
-            for (int w = 0; w < NW; w++) x += *(const v4f *)&s_o[w][k][c] * s_m[w][k];
-            const float L = s_L[k];
-            if (nsplit == 1) {
-                const float inv = L != 0.0f ? 1.0f / L : 0.0f;
-                float y[4] = {x[0] * inv, x[1] * inv, x[2] * inv, x[3] * inv};
-                store_values((T *)a.out + (size_t)(t0 + r / G) * a.out_stride + (size_t)(h * G + r % G) * HD + c, y);
-            } else {
-                const size_t at = row_of(r) * nsplit + split;
-                *gmem((v4f *)(po + at * HD + c)) = x;
-                if (c == 0) *gmem((v2f *)(pml + 2 * at)) = (v2f){s_M[k], L};
-            }
+        s_M[l16] = M; s_L[l16] = L;
+    }
+    __syncthreads();
+    for (int i = threadIdx.x; i < 16 * HD / 4; i += NT) {
+        const int k = i / (HD / 4), c = i % (HD / 4) * 4, r = r0 + k;
+        if (r >= R) continue;
+        v4f x = {0, 0, 0, 0};
+        #pragma unroll
+        for (int w = 0; w < NW; w++) x += *(const v4f *)&s_o[w][k][c] * s_m[w][k];
+        const float L = s_L[k];
+        if (nsplit == 1) {
+            const float inv = L != 0.0f ? 1.0f / L : 0.0f;
+            float y[4] = {x[0] * inv, x[1] * inv, x[2] * inv, x[3] * inv};
+            store_values((T *)a.out + (size_t)(t0 + r / G) * a.out_stride + (size_t)(h * G + r % G) * HD + c, y);
+        } else {
+            const size_t at = row_of(r) * nsplit + split;
+            *gmem((v4f *)(po + at * HD + c)) = x;
+            if (c == 0) *gmem((v2f *)(pml + 2 * at)) = (v2f){s_M[k], L};
         }
     }
 }
@@ -433,7 +400,7 @@ int cache_check_arrays(const char *who, const sp_hipkv_cache_args *a, size_t nee
 
 template <typename T, int HD> hipError_t cache_go(const sp_hipkv_cache_args &a, hipStream_t s) {
     const CachePlan p = cache_plan(a);
-    hipError_t e = op_launch(k_cache<T, HD, 1>, dim3((uint32_t)cache_grid(a, p)), dim3(64 * CACHE_WAVES), s, a, p.groups, p.nsplit, p.pages);
+    hipError_t e = op_launch(k_cache<T, HD>, dim3((uint32_t)cache_grid(a, p)), dim3(64 * CACHE_WAVES), s, a, p.groups, p.nsplit, p.pages);
     if (e != hipSuccess || p.nsplit == 1) return e;
     // (32 parts of 16 rows: 4.8 us with 1024 threads a row, 7.5 with 256; 2 parts of 2048 rows: 10.6, 4.8)
     const dim3 rows((uint32_t)((int64_t)a.n_tokens * a.n_heads));
