@@ -457,7 +457,8 @@ typedef struct sp_hipkv_prompt_args {
     int32_t n_heads, n_kv_heads;    /* at most 4096, and 16 q heads for each kv head */
     int32_t head_dim;               /* 64, 128 or 256 */
     int32_t type;                   /* SP_HIPKV_F32, SP_HIPKV_BF16 */
-    int32_t n_seqs, n_tokens;       /* sequences (at most 4096), tokens of all of them (at most 2^20) */
+    int32_t n_seqs, n_tokens;       /* sequences (at most 4096), tokens of all of them (at most 2^20, and n_tokens n_heads / 64 +
+                                       n_seqs n_kv_heads below 2^23) */
     int32_t max_tokens;             /* no sequence has more */
     int32_t window;                 /* 0: every token before */
     float   scale;                  /* 1 / sqrt(head_dim) in the models served */
@@ -476,9 +477,9 @@ int  sp_hipkv_prompt_attention(const sp_hipkv_prompt_args *a, void *stream);
 /* Attention of new tokens over the 8-bit cache, which holds their rows already (a decode
  * step's one token a sequence, or a piece of a prompt): token j of sequence s, at position
  * p = cached[s] + j, attends positions [max(0, p - window + 1), p]:
- * out = sum softmax(scale q.k) v.  q and the weights are taken to integers of 23 bits (of a
- * row's largest value, of a page's largest weight; bf16: 15), whose products with the codes are
- * exact.
+ * out = sum softmax(scale q.k) v.  q and the weights, times their v's scales, are taken to integers
+ * of 23 bits (of a row's largest value, of a page's largest such weight or of 1e-30; bf16: 15), whose
+ * products with the codes are exact.
  * Positions that a token does not attend do not reach it whatever their codes and scales.
  * A scale that is not finite in a block that it attends, or a q value that is not, leaves
  * it without a finite value. */

@@ -402,9 +402,10 @@ template <typename T, int HD> hipError_t cache_go(const sp_hipkv_cache_args &a, 
     const CachePlan p = cache_plan(a);
     hipError_t e = op_launch(k_cache<T, HD>, dim3((uint32_t)cache_grid(a, p)), dim3(64 * CACHE_WAVES), s, a, p.groups, p.nsplit, p.pages);
     if (e != hipSuccess || p.nsplit == 1) return e;
-    // (32 parts of 16 rows: 4.8 us with 1024 threads a row, 7.5 with 256; 2 parts of 2048 rows: 10.6, 4.8)
+    // (32 parts of 16 rows: 4.8 us with 1024 threads a row, 7.5 with 256; 2 parts of 2048 rows: 10.6, 4.8.  A
+    // launch has fewer than 2^32 threads.)
     const dim3 rows((uint32_t)((int64_t)a.n_tokens * a.n_heads));
-    if (p.nsplit > 8) return op_launch(k_cache_merge<T, HD, 1024>, rows, dim3(1024), s, a, p.nsplit);
+    if (p.nsplit > 8 && rows.x <= 1 << 20) return op_launch(k_cache_merge<T, HD, 1024>, rows, dim3(1024), s, a, p.nsplit);
     return op_launch(k_cache_merge<T, HD, 256>, rows, dim3(256), s, a, p.nsplit);
 }
 template <typename T> hipError_t cache_type(const sp_hipkv_cache_args &a, hipStream_t s) {

@@ -678,19 +678,20 @@ __global__ __launch_bounds__(64 * RG * KS * prompt_split(HD), 2) void k_prompt32
     }
 }
 
+// Units of `rows` rows that a call's rows may fall into, each a workgroup for every kv head
+int64_t prompt_slots(const sp_hipkv_prompt_args &a, int rows) { return (int64_t)a.n_tokens * (a.n_heads / a.n_kv_heads) / rows + a.n_seqs; }
+
 int prompt_check(const sp_hipkv_prompt_args *a) {
     const char *who = "sp_hipkv_prompt_attention";
     if (serve_check(who, a)) return 1;
     OP_NEED(a->window >= 0, "negative window");
     OP_NEED(std::isfinite(a->scale), "scale is not finite");
     if (!a->n_tokens) return 0;
+    OP_NEED(prompt_slots(*a, 64) * a->n_kv_heads < 1 << 23, "too many sequences, heads and tokens for one launch");      // (of 512 threads, 2^32 in all)
     OP_NEED(a->start, "null array");
     return serve_rows(who, a, a->q, a->q_stride, a->n_heads) || serve_rows(who, a, a->k, a->k_stride, a->n_kv_heads) ||
            serve_rows(who, a, a->v, a->v_stride, a->n_kv_heads) || serve_rows(who, a, a->out, a->out_stride, a->n_heads);
 }
-
-// rows of a workgroup: units that a call's rows may fall into
-int64_t prompt_slots(const sp_hipkv_prompt_args &a, int rows) { return (int64_t)a.n_tokens * (a.n_heads / a.n_kv_heads) / rows + a.n_seqs; }
 
 template <typename T, int HD> hipError_t prompt_go(const sp_hipkv_prompt_args &a, hipStream_t s) {
 #define PROMPT_RUN(K, ROWS, THREADS) \

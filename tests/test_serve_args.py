@@ -11,7 +11,7 @@ HEADS = dict(n_heads=16, n_kv_heads=8, head_dim=128, type=spkv.F32, n_seqs=2, n_
 BAD_HEADS = [dict(head_dim=96), dict(head_dim=0), dict(n_kv_heads=0), dict(n_heads=12), dict(n_heads=0), dict(n_heads=136), dict(n_heads=4104, n_kv_heads=1026),
              dict(type=2), dict(type=-1), dict(n_seqs=-1), dict(n_seqs=4097), dict(n_tokens=-1), dict(n_tokens=33), dict(max_tokens=-1),
              dict(n_seqs=4096, max_tokens=512, n_tokens=(1 << 20) + 1), dict(start=None), dict(q_stride=2047), dict(q_stride=2050), dict(q_stride=1024),
-             dict(q=P + 4), dict(q=P + 8), dict(type=spkv.BF16, q_stride=2052)]
+             dict(q=P + 4), dict(q=P + 8), dict(type=spkv.BF16, q_stride=2052), dict(q_stride=(1 << 22) + 8)]
 
 
 def append(**kw):
@@ -32,7 +32,8 @@ def cached(**kw):
     dict(rows=spkv.ROWS_EXACT), dict(rows=spkv.ROWS_SPINOR), dict(rows=4), dict(max_positions=-1), dict(max_positions=(1 << 20) + 1), dict(ring_pages=-1),
     dict(max_tokens=(1 << 20) + 1), dict(eps=-1e-6), dict(eps=float("nan")), dict(eps=float("inf")), dict(cached=None), dict(tables=None), dict(tables=P + 4),
     dict(freq=P + 4), dict(q=None), dict(k=None), dict(v=None), dict(k=P + 8), dict(v=P + 4), dict(k_stride=1020), dict(v_stride=1025), dict(q_out=P + 8),
-    dict(q_out_stride=2044), dict(k_out=P + 8), dict(k_out_stride=1000), dict(q_out_stride=2052), dict(k_out_stride=1028)])
+    dict(q_out_stride=2044), dict(k_out=P + 8), dict(k_out_stride=1000), dict(q_out_stride=2052), dict(k_out_stride=1028),
+    dict(v_stride=(1 << 22) + 8), dict(k_out_stride=(1 << 22) + 8)])
 def test_append_refusals(bad):
     with pytest.raises(RuntimeError, match="sp_hipkv_append"):
         spkv.append(append(**bad))
@@ -40,7 +41,8 @@ def test_append_refusals(bad):
 
 @pytest.mark.parametrize("bad", BAD_HEADS + [
     dict(window=-1), dict(scale=float("nan")), dict(scale=float("inf")), dict(q=None), dict(k=None), dict(v=None), dict(out=None), dict(k=P + 4), dict(v=P + 8),
-    dict(out=P + 4), dict(k_stride=1020), dict(v_stride=1026), dict(out_stride=2044)])
+    dict(out=P + 4), dict(k_stride=1020), dict(v_stride=1026), dict(out_stride=2044), dict(k_stride=(1 << 22) + 8), dict(out_stride=1 << 23),
+    dict(n_seqs=4096, n_tokens=4096, n_heads=4096, n_kv_heads=4096, head_dim=64, **{x + "_stride": 1 << 18 for x in ("q", "k", "v", "out")})])
 def test_prompt_refusals(bad):
     with pytest.raises(RuntimeError, match="sp_hipkv_prompt_attention"):
         spkv.prompt_attention(prompt(**bad))
@@ -48,7 +50,7 @@ def test_prompt_refusals(bad):
 
 @pytest.mark.parametrize("bad", BAD_HEADS + [
     dict(max_positions=-1), dict(max_positions=(1 << 20) + 1), dict(max_tokens=513), dict(window=-1), dict(ring_pages=-1), dict(scale=float("nan")),
-    dict(scale=float("-inf")), dict(cached=None), dict(tables=None), dict(tables=P + 4), dict(q=None), dict(out=None), dict(out=P + 8), dict(out_stride=2046),
+    dict(scale=float("-inf")), dict(cached=None), dict(tables=None), dict(tables=P + 4), dict(q=None), dict(out=None), dict(out=P + 8), dict(out_stride=2046), dict(out_stride=(1 << 22) + 8),
     dict(n_seqs=4096, max_tokens=512, n_tokens=(1 << 18) + 1)])
 def test_cache_refusals(bad):
     with pytest.raises(RuntimeError, match="sp_hipkv_cache_attention"):
