@@ -1,17 +1,22 @@
 // kvd_append.hip -- appending tokens to the paged cache: norm and rotation of q and k,
 // K and V rows into their pages.
 //
-// A wave takes the 16 positions of a block in four rounds of four, of one head of q, k or v: lane (i, l) of round r has position 4 r + i and the pairs l PP .. (l + 1) PP of a
-// head, PP = head_dim / 32, so that a row is read and written whole by 16 lanes, and a block's
-// largest magnitude and scale stay in a wave.  V codes lie by columns (their byte order is the
+// A wave takes the 16 positions of a block, or half of them, in rounds of four, of one head of q, k
+// or v: lane (i, l) of round r has position 4 r + i and the pairs l PP .. (l + 1) PP of a head, PP =
+// head_dim / 32, so that a row is read and written whole by 16 lanes, and a block's largest
+// magnitude and scale stay in a wave.  V codes lie by columns (their byte order is the
 // matrix products'): they pass LDS, from where a thread writes the bytes of a column that it owns.
 //
 // Everything is computed in 64 bits: the angle of position p is p freq, off by 2^-53 of
 // itself (in 32 bits it would be off by 0.008 at position 131072), and a code is the rounded
 // quotient itself, not that of a rounded value.  f64 runs at the rate of f32 here.  Sine and
 // cosine are Taylor series behind a reduction by multiples of pi / 2, for a lane's first position and for a
-// step of four; the other rounds' follow by turning.  (Four q heads a wave with the same sines: 38.6 us
-// for 37.2 of 4096 tokens, 32 and 8 heads of 128; what counts is rows on their way.)
+// step of four; the other rounds' follow by turning.
+//
+// 4096 tokens of 32 and 8 heads of 128 in bf16 take 36.5 us, 20.8 at the rate of a large copy: 7.5 of it
+// are sines, about as much the other arithmetic, and a wave's loads wait for no other's. (Four q heads a
+// wave with the same sines: 38.6 us; what counts is rows on their way.)  2 x 8 heads of 256 in f32 to f32
+// rows, which need no scale first, run at 90 % of that rate.
 #include "kvd_serve.h"
 #include "kvd_vec.h"
 #include <algorithm>
@@ -96,14 +101,20 @@ __device__ __forceinline__ uint32_t code_of(float y, float inv) { return __float
 // a stored code at another scale
 __device__ __forceinline__ uint32_t recode(uint32_t code, float ratio) { return code_of((float)(int8_t)code, ratio) & 255; }
 
-// NW waves a workgroup: 4, a page, or 1, a block.
-template <typename T, int ROWS, int HD, int NW>
-__global__ __launch_bounds__(64 * NW, HD == 256 ? 1 : 2) void k_append(sp_hipkv_append_args a, int seq_units) {
-    constexpr int PP = HD / 32, H2 = HD / 2, UNIT = BLOCK8 * NW;
+// Waves that share a block, two rounds each: of 8-bit rows of 256 dims one alone holds 64 values of 64 bits a lane
+// until the block's scale is known (3900 tokens of 16 and 8 heads 76 us for 71, 20 of 40 tokens 30.3 for 27.9; of
+// 128 dims the sines formed twice cost more: 36.5 us for 44 of 4096 tokens of 32 and 8 heads)
+constexpr int block_waves(int rows, int hd) { return rows == SP_HIPKV_ROWS_BLOCK8 && hd == 256 ? 2 : 1; }
+
+// NB blocks a workgroup: 4, a page, or 1.
+template <typename T, int ROWS, int HD, int NB>
+__global__ __launch_bounds__(64 * NB * block_waves(ROWS, HD), 2) void k_append(sp_hipkv_append_args a, int seq_units) {
+    constexpr int PP = HD / 32, H2 = HD / 2, UNIT = BLOCK8 * NB, WB = block_waves(ROWS, HD), NR = 4 / WB, NT = 64 * NB * WB;
     constexpr bool B8 = ROWS == SP_HIPKV_ROWS_BLOCK8;
-    constexpr int COL = 16 * NW + 16;                                     // bytes of a column of V codes in LDS
+    constexpr int COL = 16 * NB + 16;                                     // bytes of a column of V codes in LDS
     __shared__ __align__(16) uint8_t s_code[B8 ? HD * COL : 16];
     __shared__ float s_ratio;
+    __shared__ double s_big[NB * WB];
     // this workgroup's sequence and unit of positions
     const int slot = blockIdx.y;
     int s, j;
@@ -122,15 +133,15 @@ __global__ __launch_bounds__(64 * NW, HD == 256 ? 1 : 2) void k_append(sp_hipkv_
     const bool stored = kind && !(a.ring_pages && lp + a.ring_pages <= (end - 1) / PAGE);
     if (!stored && !(kind == 0 || (kind == 1 && a.k_out))) return;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), i = lane >> 4, l = lane & 15;
-    const int b0 = p0 + BLOCK8 * wave, u = b0 / BLOCK8 % PAGE_BLOCKS;
+    const int b0 = p0 + BLOCK8 * (wave / WB), r0 = wave % WB * NR, u = b0 / BLOCK8 % PAGE_BLOCKS;
     const bool some = b0 < end && b0 + BLOCK8 > first;
-    if (!some && !(B8 && kind == 2)) return;
+    if (!some && !(B8 && kind == 2) && !(WB > 1 && stored)) return;
     uint8_t *page = stored ? (uint8_t *)gmem(table)[a.ring_pages ? lp % a.ring_pages : lp] : nullptr;
-    auto live = [&](int r) { const int p = b0 + 4 * r + i; return p >= first && p < end; };
-    auto round_live = [&](int r) { return b0 + 4 * r < end && b0 + 4 * r + 4 > first; };
+    auto live = [&](int r) { const int p = b0 + 4 * (r0 + r) + i; return p >= first && p < end; };
+    auto round_live = [&](int r) { return b0 + 4 * (r0 + r) < end && b0 + 4 * (r0 + r) + 4 > first; };
     const bool older = B8 && some && stored && first > b0;                // positions of the block from earlier calls
     auto row_of = [&](auto *p, int64_t stride, int r, int head) __attribute__((always_inline)) {
-        return p + (size_t)(t0 + b0 + 4 * r + i - first) * stride + (size_t)head * HD + l * PP;
+        return p + (size_t)(t0 + b0 + 4 * (r0 + r) + i - first) * stride + (size_t)head * HD + l * PP;
     };
     auto put = [&](auto *row, const float (&z)[2 * PP]) __attribute__((always_inline)) {
         float z0[PP], z1[PP];
@@ -141,9 +152,9 @@ __global__ __launch_bounds__(64 * NW, HD == 256 ? 1 : 2) void k_append(sp_hipkv_
     };
     const T *src = (const T *)(kind == 0 ? a.q : kind == 1 ? a.k : a.v);
     const int64_t stride = kind == 0 ? a.q_stride : kind == 1 ? a.k_stride : a.v_stride;
-    float x[4][2][PP] = {};
+    float x[NR][2][PP] = {};
     #pragma unroll
-    for (int r = 0; r < 4; r++)
+    for (int r = 0; r < NR; r++)
         if (live(r)) {
             const T *row = row_of(src, stride, r, h);
             load_values(row, x[r][0]);
@@ -152,37 +163,42 @@ __global__ __launch_bounds__(64 * NW, HD == 256 ? 1 : 2) void k_append(sp_hipkv_
     if (kind == 2) {
         if constexpr (!B8) {
             #pragma unroll
-            for (int r = 0; r < 4; r++)
+            for (int r = 0; r < NR; r++)
                 if (live(r)) {
-                    float *row = (float *)page + ((size_t)(a.n_kv_heads + h) * PAGE + BLOCK8 * u + 4 * r + i) * HD + l * PP;
+                    float *row = (float *)page + ((size_t)(a.n_kv_heads + h) * PAGE + BLOCK8 * u + 4 * (r0 + r) + i) * HD + l * PP;
                     store_values(row, x[r][0]);
                     store_values(row + H2, x[r][1]);
                 }
         } else {
             float *scale_at = (float *)(page + (size_t)2 * a.n_kv_heads * PAGE * HD) + (a.n_kv_heads + h) * PAGE_BLOCKS + u;
             if (threadIdx.x == 0) s_ratio = 1.0f;
-            if (NW > 1) __syncthreads();
+            if (NT > 64) __syncthreads();
+            uint32_t big = 0;                                         // as bits: NaN is above infinity
+            #pragma unroll
+            for (int r = 0; r < NR; r++)
+                if (live(r)) {
+                    #pragma unroll
+                    for (int k = 0; k < PP; k++) big = max(big, max(__float_as_uint(x[r][0][k]) & 0x7FFFFFFFu, __float_as_uint(x[r][1][k]) & 0x7FFFFFFFu));
+                }
+            big = (uint32_t)wave_allmax_i((int)big);
+            const float was = older ? *scale_at : 0.0f;
+            if constexpr (WB > 1) {
+                if (lane == 0) ((uint32_t *)s_big)[wave] = big;
+                __syncthreads();
+                big = max(big, ((uint32_t *)s_big)[wave ^ 1]);
+            }
             if (some) {
-                uint32_t big = 0;                                     // as bits: NaN is above infinity
-                #pragma unroll
-                for (int r = 0; r < 4; r++)
-                    if (live(r)) {
-                        #pragma unroll
-                        for (int k = 0; k < PP; k++) big = max(big, max(__float_as_uint(x[r][0][k]) & 0x7FFFFFFFu, __float_as_uint(x[r][1][k]) & 0x7FFFFFFFu));
-                    }
-                big = (uint32_t)wave_allmax_i((int)big);
-                const float was = older ? *scale_at : 0.0f;
                 const float sc = block_scale(scale_exp((double)__uint_as_float(big)), older, was), inv = 1.0f / sc;
-                if (lane == 0) {
+                if (lane == 0 && r0 == 0) {
                     *scale_at = sc;
                     if (older) s_ratio = was / sc;
                 }
                 #pragma unroll
-                for (int r = 0; r < 4; r++)
+                for (int r = 0; r < NR; r++)
                     if (live(r)) {
                         #pragma unroll
                         for (int k = 0; k < PP; k++) {
-                            uint8_t *col = s_code + (l * PP + k) * COL + 4 * NW * r + 4 * wave + i;
+                            uint8_t *col = s_code + (l * PP + k) * COL + 4 * NB * (r0 + r) + 4 * (wave / WB) + i;
                             col[0] = (uint8_t)code_of(x[r][0][k], inv);
                             col[H2 * COL] = (uint8_t)code_of(x[r][1][k], inv);
                         }
@@ -191,35 +207,35 @@ __global__ __launch_bounds__(64 * NW, HD == 256 ? 1 : 2) void k_append(sp_hipkv_
             __syncthreads();
             const float ratio = s_ratio;                              // of the codes that the first block has already
             const int old0 = first / BLOCK8 * BLOCK8;
-            // NW words of four positions each, 4 g .. of NW neighbouring blocks
-            for (int id = threadIdx.x; id < HD * 4; id += 64 * NW) {
+            // NB words of four positions each, 4 g .. of NB neighbouring blocks
+            for (int id = threadIdx.x; id < HD * 4; id += NT) {
                 const int d = id >> 2, g = id & 3;
-                uint32_t w[NW];
-                const uint32_t *from = (const uint32_t *)(s_code + d * COL + 4 * NW * g);
-                KVD_GLOBAL uint32_t *dst = gmem((uint32_t *)(page + ((size_t)a.n_kv_heads + h) * PAGE * HD + (size_t)d * PAGE + 16 * g + (NW == 1 ? 4 * u : 0)));
+                uint32_t w[NB];
+                const uint32_t *from = (const uint32_t *)(s_code + d * COL + 4 * NB * g);
+                KVD_GLOBAL uint32_t *dst = gmem((uint32_t *)(page + ((size_t)a.n_kv_heads + h) * PAGE * HD + (size_t)d * PAGE + 16 * g + (NB == 1 ? 4 * u : 0)));
                 uint32_t fresh = 0, again = 0;                        // bytes to write, bytes to round again
                 #pragma unroll
-                for (int k = 0; k < 4 * NW; k++) {
+                for (int k = 0; k < 4 * NB; k++) {
                     const int p = p0 + (k >> 2) * 16 + 4 * g + (k & 3);
                     fresh |= (uint32_t)(p >= first && p < end) << k;
                     again |= (uint32_t)(p >= old0 && p < first && ratio != 1.0f) << k;
                 }
                 if (!(fresh | again)) continue;
                 #pragma unroll
-                for (int k = 0; k < NW; k++) w[k] = from[k];
-                if (fresh != (1u << 4 * NW) - 1) {
-                    uint32_t o[NW];
+                for (int k = 0; k < NB; k++) w[k] = from[k];
+                if (fresh != (1u << 4 * NB) - 1) {
+                    uint32_t o[NB];
                     #pragma unroll
-                    for (int k = 0; k < NW; k++) o[k] = dst[k];
+                    for (int k = 0; k < NB; k++) o[k] = dst[k];
                     #pragma unroll
-                    for (int k = 0; k < 4 * NW; k++) {
+                    for (int k = 0; k < 4 * NB; k++) {
                         const int sh = 8 * (k & 3);
                         uint32_t b = o[k >> 2] >> sh & 255;
                         if (again >> k & 1) b = recode(b, ratio);
                         if (!(fresh >> k & 1)) w[k >> 2] = (w[k >> 2] & ~(255u << sh)) | b << sh;
                     }
                 }
-                if constexpr (NW == 4) *(KVD_GLOBAL v4u *)dst = (v4u){w[0], w[1], w[2], w[3]};
+                if constexpr (NB == 4) *(KVD_GLOBAL v4u *)dst = (v4u){w[0], w[1], w[2], w[3]};
                 else dst[0] = w[0];
             }
         }
@@ -228,7 +244,7 @@ __global__ __launch_bounds__(64 * NW, HD == 256 ? 1 : 2) void k_append(sp_hipkv_
     // q or k: norm and rotation
     const float *nw = kind ? a.k_norm : a.q_norm;
     float w[2][PP];
-    double c[PP], sn[PP], cs[PP], ss[PP], y[B8 ? 4 : 1][2 * PP];         // 8-bit rows wait for their block's scale
+    double c[PP], sn[PP], cs[PP], ss[PP], y[B8 ? NR : 1][2 * PP];         // 8-bit rows wait for their block's scale
     if (nw) {
         #pragma unroll
         for (int k = 0; k < PP; k++) { w[0][k] = gmem(nw)[l * PP + k]; w[1][k] = gmem(nw)[H2 + l * PP + k]; }
@@ -237,7 +253,7 @@ __global__ __launch_bounds__(64 * NW, HD == 256 ? 1 : 2) void k_append(sp_hipkv_
         #pragma unroll
         for (int k = 0; k < PP; k++) {
             const double f = gmem(a.freq)[l * PP + k];
-            turn((double)(b0 + i) * f, c[k], sn[k]);
+            turn((double)(b0 + 4 * r0 + i) * f, c[k], sn[k]);
             turn(4.0 * f, cs[k], ss[k]);
         }
     }
@@ -245,7 +261,7 @@ __global__ __launch_bounds__(64 * NW, HD == 256 ? 1 : 2) void k_append(sp_hipkv_
     const int64_t back_stride = kind ? a.k_out_stride : a.q_out_stride;
     double big = 0.0, none = 0.0;                                          // none: NaN if some value is not finite
     #pragma unroll
-    for (int r = 0; r < 4; r++) {
+    for (int r = 0; r < NR; r++) {
         double (&v)[2 * PP] = y[B8 ? r : 0];
         if (r && a.freq) {
             #pragma unroll
@@ -255,7 +271,7 @@ __global__ __launch_bounds__(64 * NW, HD == 256 ? 1 : 2) void k_append(sp_hipkv_
                 c[k] = t;
             }
         }
-        if (NW == 1 && !round_live(r)) continue;
+        if ((NB == 1 || WB > 1) && !round_live(r)) continue;
         #pragma unroll
         for (int k = 0; k < PP; k++) { v[k] = (double)x[r][0][k]; v[PP + k] = (double)x[r][1][k]; }
         if (nw) {
@@ -285,7 +301,7 @@ __global__ __launch_bounds__(64 * NW, HD == 256 ? 1 : 2) void k_append(sp_hipkv_
             for (int k = 0; k < 2 * PP; k++) { big = fmax(big, fabs(v[k])); none = fma(v[k], 0.0, none); }
         } else if (stored) {
             rounded<float>(v, z);
-            put((float *)page + ((size_t)h * PAGE + BLOCK8 * u + 4 * r + i) * HD + l * PP, z);
+            put((float *)page + ((size_t)h * PAGE + BLOCK8 * u + 4 * (r0 + r) + i) * HD + l * PP, z);
         }
     }
     if constexpr (B8) {
@@ -294,16 +310,22 @@ __global__ __launch_bounds__(64 * NW, HD == 256 ? 1 : 2) void k_append(sp_hipkv_
         big = bcast63(wave_to63(big, 0.0, [](double p, double q) { return fmax(p, q); }));
         float *scale_at = (float *)(page + (size_t)2 * a.n_kv_heads * PAGE * HD) + h * PAGE_BLOCKS + u;
         const float was = older ? *scale_at : 0.0f;
+        if constexpr (WB > 1) {
+            if (lane == 0) s_big[wave] = big;
+            __syncthreads();
+            big = fmax(big, s_big[wave ^ 1]);
+            if (!some) return;
+        }
         const float sc = block_scale(scale_exp(big), older, was), ratio = was / sc;
         const double inv = 1.0 / (double)sc;
-        if (lane == 0) *scale_at = sc;
+        if (lane == 0 && r0 == 0) *scale_at = sc;
         #pragma unroll
-        for (int r = 0; r < 4; r++) {
-            const bool again = older && b0 + 4 * r + i < first && ratio != 1.0f;
+        for (int r = 0; r < NR; r++) {
+            const bool again = older && b0 + 4 * (r0 + r) + i < first && ratio != 1.0f;
             if (!live(r) && !again) continue;
             #pragma unroll
             for (int e = 0; e < 2; e++) {
-                uint8_t *row = page + ((size_t)h * PAGE + BLOCK8 * u + 4 * r + i) * HD + l * PP + e * H2;
+                uint8_t *row = page + ((size_t)h * PAGE + BLOCK8 * u + 4 * (r0 + r) + i) * HD + l * PP + e * H2;
                 uint32_t b[(PP + 3) / 4];
                 #pragma unroll
                 for (int k = 0; k < PP; k++) {
@@ -346,11 +368,11 @@ int append_check(const sp_hipkv_append_args *a) {
     return 0;
 }
 
-template <typename T, int ROWS, int NW> hipError_t append_go(const sp_hipkv_append_args &a, hipStream_t s) {
+template <typename T, int ROWS, int NB> hipError_t append_go(const sp_hipkv_append_args &a, hipStream_t s) {
     int seq_units = 0;
-    const int64_t slots = append_slots(a, BLOCK8 * NW, &seq_units);
-    return op_launch(a.head_dim == 256 ? k_append<T, ROWS, 256, NW> : a.head_dim == 128 ? k_append<T, ROWS, 128, NW> : k_append<T, ROWS, 64, NW>,
-                     dim3((a.q_out ? a.n_heads : 0) + 2 * a.n_kv_heads, (uint32_t)slots), dim3(64 * NW), s, a, seq_units);
+    const int64_t slots = append_slots(a, BLOCK8 * NB, &seq_units);
+    return op_launch(a.head_dim == 256 ? k_append<T, ROWS, 256, NB> : a.head_dim == 128 ? k_append<T, ROWS, 128, NB> : k_append<T, ROWS, 64, NB>,
+                     dim3((a.q_out ? a.n_heads : 0) + 2 * a.n_kv_heads, (uint32_t)slots), dim3(64 * NB * block_waves(ROWS, a.head_dim)), s, a, seq_units);
 }
 template <typename T, int ROWS> hipError_t append_rows(const sp_hipkv_append_args &a, hipStream_t s) {
     return a.max_tokens <= BLOCK8 ? append_go<T, ROWS, 1>(a, s) : append_go<T, ROWS, 4>(a, s);
