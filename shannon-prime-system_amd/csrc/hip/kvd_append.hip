@@ -11,11 +11,12 @@
 // itself (in 32 bits it would be off by 0.008 at position 131072), and a code is the rounded
 // quotient itself, not that of a rounded value.  f64 runs at the rate of f32 here.  Sine and
 // cosine are Taylor series behind a reduction by multiples of pi / 2, for a lane's first position and for a
-// step of four; the other rounds' follow by turning.
+// step of four (a quarter of its pairs in each of the four rows of lanes); the other rounds' follow by
+// turning.
 //
-// 4096 tokens of 32 and 8 heads of 128 in bf16 take 36.5 us, 20.8 at the rate of a large copy: 7.5 of it
-// are sines, about as much the other arithmetic, and a wave's loads wait for no other's. (Four q heads a
-// wave with the same sines: 38.6 us; what counts is rows on their way.)  2 x 8 heads of 256 in f32 to f32
+// 4096 tokens of 32 and 8 heads of 128 in bf16 take 36.0 us, 20.8 at the rate of a large copy: about 5 of it
+// are sines (37 with all of them formed in every lane), as much is the other arithmetic, which a wave's loads
+// wait for.  (Four q heads a wave with the same sines: 38.6 us; what counts is rows on their way.)  16 and 8 heads of 256 in f32 to f32
 // rows, which need no scale first, run at 90 % of that rate.
 #include "kvd_serve.h"
 #include "kvd_vec.h"
@@ -102,8 +103,8 @@ __device__ __forceinline__ uint32_t code_of(float y, float inv) { return __float
 __device__ __forceinline__ uint32_t recode(uint32_t code, float ratio) { return code_of((float)(int8_t)code, ratio) & 255; }
 
 // Waves that share a block, two rounds each: of 8-bit rows of 256 dims one alone holds 64 values of 64 bits a lane
-// until the block's scale is known (3900 tokens of 16 and 8 heads 76 us for 71, 20 of 40 tokens 30.3 for 27.9; of
-// 128 dims the sines formed twice cost more: 36.5 us for 44 of 4096 tokens of 32 and 8 heads)
+// until the block's scale is known (3900 tokens of 16 and 8 heads 76 us for 71, 20 prompts of 40 30.3 for 27.9; of
+// 128 dims the sines formed twice cost more: 36.5 us for 44, 4096 tokens of 32 and 8 heads)
 constexpr int block_waves(int rows, int hd) { return rows == SP_HIPKV_ROWS_BLOCK8 && hd == 256 ? 2 : 1; }
 
 // NB blocks a workgroup: 4, a page, or 1.
@@ -249,12 +250,21 @@ __global__ __launch_bounds__(64 * NB * block_waves(ROWS, HD), 2) void k_append(s
         #pragma unroll
         for (int k = 0; k < PP; k++) { w[0][k] = gmem(nw)[l * PP + k]; w[1][k] = gmem(nw)[H2 + l * PP + k]; }
     }
+    // the first round with tokens, from whose sines the others' are turned
+    const int rounds0 = max((first - b0) / 4 - r0, 0);
     if (a.freq) {
         #pragma unroll
-        for (int k = 0; k < PP; k++) {
-            const double f = gmem(a.freq)[l * PP + k];
-            turn((double)(b0 + 4 * r0 + i) * f, c[k], sn[k]);
-            turn(4.0 * f, cs[k], ss[k]);
+        for (int k = 0; k < PP; k++) turn((double)(b0 + 4 * (r0 + rounds0) + i) * gmem(a.freq)[l * PP + k], c[k], sn[k]);
+        if (rounds0 + 1 < NR && round_live(rounds0 + 1)) {                // the step's are the same in all four rows: each forms a part
+            constexpr int PART = PP > 4 ? PP / 4 : 1, ROWS_OF = PP / PART;
+            double cp[PART], sp[PART];
+            #pragma unroll
+            for (int k = 0; k < PART; k++) turn(4.0 * gmem(a.freq)[l * PP + i % ROWS_OF * PART + k], cp[k], sp[k]);
+            #pragma unroll
+            for (int k = 0; k < PP; k++) {
+                cs[k] = __shfl(cp[k % PART], k / PART * 16 + l, 64);
+                ss[k] = __shfl(sp[k % PART], k / PART * 16 + l, 64);
+            }
         }
     }
     T *back = (T *)(kind ? a.k_out : a.q_out);
@@ -263,7 +273,7 @@ __global__ __launch_bounds__(64 * NB * block_waves(ROWS, HD), 2) void k_append(s
     #pragma unroll
     for (int r = 0; r < NR; r++) {
         double (&v)[2 * PP] = y[B8 ? r : 0];
-        if (r && a.freq) {
+        if (r > rounds0 && a.freq) {
             #pragma unroll
             for (int k = 0; k < PP; k++) {
                 const double t = fma(c[k], cs[k], -(sn[k] * ss[k]));
