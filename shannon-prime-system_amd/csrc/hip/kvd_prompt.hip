@@ -708,6 +708,14 @@ template <typename T, int HD> hipError_t prompt_go(const sp_hipkv_prompt_args &a
             const int64_t units = prompt_slots(a, 32 * RG) * a.n_kv_heads;
             if (a.max_tokens >= 192 && units <= (a.n_tokens >= (int64_t)256 * a.n_seqs ? 512 : 256)) return PROMPT_RUN((k_prompt32<HD, RG, KS>), 32 * RG, 512);
         }
+        // Dims of 256: a unit holds one workgroup, and with no more than one for each the longest span is what counts,
+        // which 64 rows walk faster than 128: 16 and 8 heads 129 us for 156 at 1000 tokens, 280 for 303 at 2047 (256
+        // units of 128 rows), 485 for 388 at 2600.  With a window all spans are much the same, and it is their sum that
+        // counts from half as many on: 1024 of 1400 tokens 139 for 171, of 1788 219 for 174.
+        if constexpr (HD == 256) {
+            const bool even = a.window && 3 * (int64_t)a.window < 2 * (int64_t)a.max_tokens;
+            if ((int64_t)a.n_tokens * a.n_heads / 128 <= (even ? 128 : 256)) return PROMPT_RUN((k_prompt32<HD, 2, 1>), 64, 256);
+        }
         return PROMPT_RUN((k_prompt32<HD, 4, 1>), 128, 256 * prompt_split(HD));
     }
     else if constexpr (HD == 256) return PROMPT_RUN((k_prompt16<HD, 2, 1, 1>), 64, 256);

@@ -245,10 +245,16 @@ def test_prompt_large_values_of_small_weight(typ, hd, low):
 
 
 @pytest.mark.parametrize("typ", TYPES)
-@pytest.mark.parametrize("hd,n,nkv", [(64, 400, 48), (128, 300, 64), (128, 250, 160)])
+@pytest.mark.parametrize("hd,n,nkv", [(64, 400, 48), (128, 300, 64), (128, 250, 160), (256, 230, 150)])
 def test_prompt_long_with_many_heads(typ, hd, n, nkv):
     """Too many rows for a workgroup a unit."""
     Prompt(rng(25, hd), typ, hd, 1, [n], nkv=nkv).check()
+
+
+@pytest.mark.parametrize("typ", TYPES)
+@pytest.mark.parametrize("n,nkv", [(200, 40), (200, 100)])
+def test_prompt_wide_heads_in_a_window(typ, n, nkv):
+    Prompt(rng(26, nkv), typ, 256, 1, [n, 3], window=70, nkv=nkv).check()
 
 
 @pytest.mark.parametrize("typ", TYPES)
