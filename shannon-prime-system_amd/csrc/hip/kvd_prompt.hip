@@ -1,8 +1,8 @@
 // kvd_prompt.hip -- attention of whole prompts: packed sequences, causal, grouped heads.
 //
 // The q heads of a kv head share its K and V: the rows of one kv head are r = token G + q
-// head of the group, 32 to a matrix tile, QT tiles to a wave, 4 waves to a workgroup, which walk the
-// K and V tiles of their rows' span in step, with a running maximum and sum.
+// head of the group, 32 to a wave, a matrix tile.  The waves of a workgroup walk the K and V tiles of their
+// rows' span in step, with a running maximum and sum.
 //
 // Both products are made transposed: S^T = K Q^T (K the A operand, from LDS; Q the B
 // operand, in registers), then O^T += V^T P^T.  A lane then holds scores, weights,
@@ -15,8 +15,8 @@
 // output's own rounding (sqrt 2 of it together); the sum adds them unrounded.
 // f32: K, V, q and weights as two f16 numbers each, three products (below).
 //
-// The running maximum only moves when a score exceeds it by 2^16 in the exponent: weights
-// stay below 2^16, nothing is lost below sums of 2^128 (v of 2^90 over 2^20 tokens), and most tiles leave the
+// The running maximum only moves when a score exceeds it by 2^16 (f32: 2^8, f16 numbers end
+// sooner) in the exponent: weights stay below 2^16, nothing is lost below sums of 2^128 (v of 2^90 over 2^20 tokens), and most tiles leave the
 // output unscaled.  With 2^8, scores of a standard deviation of 4.5 had some row of 32 move in every
 // eighth tile of 8192 tokens, 90 us of 640.
 //

@@ -3,19 +3,21 @@
 // the layout of 8-bit pages, checks.
 #pragma once
 #include "kvd_op.h"
-#include "kvd_pieces.h"
 
 namespace kvd {
 
 constexpr int BLOCK8 = 16, PAGE_BLOCKS = PAGE / BLOCK8;                // positions with one scale; scales of a page's head
 __host__ __device__ constexpr size_t block8_bytes(int nkv, int hd) { return (size_t)nkv * 2 * (PAGE * hd + PAGE_BLOCKS * 4); }
 
+typedef float v2f __attribute__((ext_vector_type(2)));
+typedef float v4f __attribute__((ext_vector_type(4)));
 typedef uint32_t v2u __attribute__((ext_vector_type(2)));
-typedef v4u32 v4u;
+typedef uint32_t v4u __attribute__((ext_vector_type(4)));
+typedef __bf16 bf2 __attribute__((ext_vector_type(2)));
+typedef __bf16 bf8 __attribute__((ext_vector_type(8)));
 
 // ---------------------------------------------------------------- values
 struct Bf16 { uint16_t u; };
-template <typename T> constexpr int type_of = sizeof(T) == 4 ? SP_HIPKV_F32 : SP_HIPKV_BF16;
 // N neighbouring values as f32, from an address aligned to as many
 template <int N> __device__ __forceinline__ void load_values(const float *p, float (&x)[N]) {
     if constexpr (N == 2) { const v2f a = *gmem((const v2f *)p); x[0] = a[0]; x[1] = a[1]; }
