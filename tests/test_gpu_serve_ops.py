@@ -67,12 +67,13 @@ def test_append_far_positions(typ):
     Append(g, c, BLOCK8, typ, 128, 2, [(1 << 20) - 20], [20], base=1e6).check()
 
 
-def test_append_step_by_step():
+@pytest.mark.parametrize("hd", [64, 128, 256])
+def test_append_step_by_step(hd):
     """Tokens one by one, each against what it should leave: scales grow, earlier codes are
     rounded again; and the values stay within a step and a half of the block's last scale."""
     for typ in TYPES:
         g = rng(5)
-        n, nkv, hd = 40, 2, 64
+        n, nkv = 40, 2
         c = Cache8(g, nkv, hd, [0], 0, [n]).upload()
         grow = (2.0 ** (np.arange(n) % BLOCK / 2))[:, None, None]
         k, v = g.standard_normal((n, nkv, hd)) * grow, g.standard_normal((n, nkv, hd)) * grow[::-1]
@@ -100,33 +101,41 @@ def test_append_extremes():
 
 
 @pytest.mark.parametrize("bad", [np.nan, np.inf, -np.inf])
-def test_append_values_that_are_not_finite(bad):
+@pytest.mark.parametrize("hd", [64, 256])
+def test_append_values_that_are_not_finite(hd, bad):
     """Their block gets a scale of NaN, keeps it, and is started anew at its first position."""
     g = rng(7)
-    x = g.standard_normal((40, 2, 64))
+    x = g.standard_normal((40, 2, hd))
     x[5, 0, 3], x[33, 1, 60] = bad, bad
     for typ in TYPES:
-        c = Cache8(g, 2, 64, [0], 0, [48]).upload()
-        a = Append(g, c, BLOCK8, typ, 64, 1, [0], [40], norm=False, freq=False, k_out=None, k=x, v=x)
+        c = Cache8(g, 2, hd, [0], 0, [48]).upload()
+        a = Append(g, c, BLOCK8, typ, hd, 1, [0], [40], norm=False, freq=False, k_out=None, k=x, v=x)
         a.check()
         assert np.isnan(c.s).sum() >= 4
-        one = g.standard_normal((1, 2, 64))
-        Append(g, c, BLOCK8, typ, 64, 1, [40], [1], norm=False, freq=False, k=one, v=one).check()
-        again = g.standard_normal((8, 2, 64))
-        Append(g, c, BLOCK8, typ, 64, 1, [32], [8], norm=False, freq=False, k=again, v=again).check()
+        one = g.standard_normal((1, 2, hd))
+        Append(g, c, BLOCK8, typ, hd, 1, [40], [1], norm=False, freq=False, k=one, v=one).check()
+        again = g.standard_normal((8, 2, hd))
+        Append(g, c, BLOCK8, typ, hd, 1, [32], [8], norm=False, freq=False, k=again, v=again).check()
         pg, i = c.block(0, 2)
         assert np.isfinite(c.s[pg, :, :, i]).all()
 
 
 @pytest.mark.parametrize("rows", [BLOCK8, ROWS])
 @pytest.mark.parametrize("cached,counts,ring", [([100, 640], [40, 3], 3), ([0], [1000], 3), ([70], [64 * 3], 3), ([5000], [200], 1), ([130], [1], 2)])
-def test_append_rings(rows, cached, counts, ring):
+@pytest.mark.parametrize("hd", [64, 256])
+def test_append_rings(hd, rows, cached, counts, ring):
     g = rng(8, ring)
     if rows == BLOCK8:
-        c = Cache8(g, 2, 64, cached, ring).upload()
+        c = Cache8(g, 2, hd, cached, ring).upload()
     else:
-        c = f32_cache(g, 2, 64, [64 * ring] * len(cached), ring)
-    Append(g, c, rows, F32, 64, 2, cached, counts).check()
+        c = f32_cache(g, 2, hd, [64 * ring] * len(cached), ring)
+    Append(g, c, rows, F32, hd, 2, cached, counts).check()
+
+
+@pytest.mark.parametrize("typ", TYPES)
+@pytest.mark.parametrize("cached,counts", [([0], [1]), ([15], [2]), ([7], [3]), ([8], [8]), ([62], [3]), ([17], [130]), ([0, 5, 300, 9, 7], [3, 0, 17, 64, 0]), ([100] * 3, [0, 0, 5])])
+def test_append_wide_heads(typ, cached, counts):
+    appended(rng(10, len(cached)), BLOCK8, typ, 256, 2, cached, counts).check()
 
 
 def test_append_more_heads_than_a_wave():
@@ -474,6 +483,54 @@ def test_calls_in_a_graph(typ):
         close(p.got(), *p.want())
         Dev(np.zeros(1 << 20, np.uint8)).get()
         c.pool[:] = before
+
+
+def test_graph_of_other_lengths():
+    """What a graph was captured with bounds the lengths; where sequences lie and end, the device
+    memory says at each replay."""
+    g = rng(48)
+    hd, G, nkv = 128, 2, 2
+    most = [5000, 300, 2000]
+    c = Cache8(g, nkv, hd, [x + 8 for x in most]).upload()
+    t = Cached(g, F32, hd, G, most, [8, 8, 8], nkv=nkv, cache=c).ready()
+    p = Prompt(g, BF16, hd, G, [90, 300, 10], nkv=nkv)
+    s = Stream()
+
+    def record(stream):
+        spkv.cache_attention(t.args, stream)
+        spkv.prompt_attention(p.args, stream)
+
+    e = s.capture(record)
+    for cached, counts, prompts in ((most, [8, 8, 8], [90, 300, 10]), ([0, 299, 64], [1, 8, 0], [300, 0, 100]), ([4999, 1, 130], [1, 1, 1], [1, 1, 1]), ([64, 63, 1999], [3, 1, 5], [150, 100, 150])):
+        t.cached, t.counts, p.counts = cached, counts, prompts
+        t.dcached.put(np.array(cached, np.int32)); t.dstart.put(packed_start(counts)); p.dstart.put(packed_start(prompts))
+        for out in (t.out, p.out):
+            out.dev.put(np.full(out.dev.a.shape, out.one, out.dev.a.dtype))
+        s.launch(e)
+        s.sync()
+        close(t.got(), *t.want())
+        close(p.got(), *p.want())
+
+
+@pytest.mark.parametrize("typ", TYPES)
+@pytest.mark.parametrize("cached", [[100, 30], [9000, 30]])
+def test_rows_before_the_first_sequence(typ, cached):
+    """start need not begin with 0: rows before it stay as they are, too."""
+    g = rng(49)
+    n, off = [40, 21], 7
+    p = Prompt(g, typ, 64, 2, n, more_tokens=off)
+    t = Cached(g, typ, 64, 2, cached, n, more_tokens=off).ready()
+    for x, run in ((p, spkv.prompt_attention), (t, spkv.cache_attention)):
+        x.dstart.put(packed_start(n) + off)
+        run(x.args)
+        raw = x.out.dev.get()
+        assert (raw[:off] == x.out.one).all() and (raw[sum(n) + off:] == x.out.one).all()
+        got = x.out.values(raw)[off:off + sum(n)]
+        q = x.q.values()[off:]
+        if x is p:
+            close(got, *prompt_attention(q, p.k.values()[off:], p.v.values()[off:], n, 0, p.scale, typ))
+        else:
+            close(got, *cache_attention(t.cache, q, cached, n, 0, t.scale, typ))
 
 
 def test_two_streams_at_once():
