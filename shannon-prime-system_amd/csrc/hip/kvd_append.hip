@@ -118,12 +118,20 @@ __global__ __launch_bounds__(64 * NB * block_waves(ROWS, HD), 2) void k_append(s
     __shared__ double s_big[NB * WB];
     // this workgroup's sequence and unit of positions
     const int slot = blockIdx.y;
-    int s, j;
-    if (seq_units) { s = slot / seq_units; j = slot - s * seq_units; }
-    else { s = unit_seq(a.start, a.n_seqs, slot, 1, UNIT, 2); j = slot - (int)unit_base(a.start, s, 1, UNIT, 2); }
+    UnitSeq seq;
+    int j;
+    if (seq_units) {
+        seq.s = slot / seq_units;
+        j = slot - seq.s * seq_units;
+        seq.start = gmem(a.start)[seq.s]; seq.end = gmem(a.start)[seq.s + 1];
+    } else {
+        seq = unit_seq(a.start, a.n_seqs, slot, 1, UNIT, 2);
+        j = slot - (int)unit_base(seq.start, seq.s, 1, UNIT, 2);
+    }
+    const int s = seq.s;
     const void *const *table = gmem(a.tables)[s];
-    const int t0 = max(gmem(a.start)[s], 0), first = min(max(gmem(a.cached)[s], 0), a.max_positions);
-    const int n = min(min(gmem(a.start)[s + 1], a.n_tokens) - t0, min(a.max_tokens, a.max_positions - first)), end = first + n;
+    const int t0 = max(seq.start, 0), first = min(max(gmem(a.cached)[s], 0), a.max_positions);
+    const int n = min(min(seq.end, a.n_tokens) - t0, min(a.max_tokens, a.max_positions - first)), end = first + n;
     const int p0 = (first / UNIT + j) * UNIT, lp = p0 / PAGE;
     if (n <= 0 || j < 0 || p0 >= end) return;
     // q, k or v, and its head

@@ -115,9 +115,9 @@ __global__ __launch_bounds__(64 * RG * KS * prompt_split(HD), 2) void k_prompt16
     const int G = a.n_heads / a.n_kv_heads, h = blockIdx.x % a.n_kv_heads;
     // the longest spans first: a sequence's last rows before its first
     const int slot = slots - 1 - blockIdx.x / a.n_kv_heads;
-    const int s = unit_seq(a.start, a.n_seqs, slot, G, BM, 1);
-    const int t0 = max(gmem(a.start)[s], 0), n = min(min(gmem(a.start)[s + 1], a.n_tokens) - t0, a.max_tokens);
-    const int64_t j = slot - unit_base(a.start, s, G, BM, 1);
+    const UnitSeq seq = unit_seq(a.start, a.n_seqs, slot, G, BM, 1);
+    const int t0 = max(seq.start, 0), n = min(min(seq.end, a.n_tokens) - t0, a.max_tokens);
+    const int64_t j = slot - unit_base(seq.start, seq.s, G, BM, 1);
     if (n <= 0 || j < 0 || j * BM >= (int64_t)n * G) return;
     const int R = n * G, r0 = (int)j * BM, wr0 = r0 + wave % RG * 32;
     const int part = wave / RG % KS, dim0 = wave / (RG * KS) * (HD / SP);                 // this wave's keys of a tile, and dims
@@ -403,9 +403,9 @@ __global__ __launch_bounds__(64 * RG * KS * prompt_split(HD), 2) void k_prompt32
     const int G = a.n_heads / a.n_kv_heads, h = blockIdx.x % a.n_kv_heads;
     // the longest spans first: a sequence's last rows before its first
     const int slot = slots - 1 - blockIdx.x / a.n_kv_heads;
-    const int s = unit_seq(a.start, a.n_seqs, slot, G, BM, 1);
-    const int t0 = max(gmem(a.start)[s], 0), n = min(min(gmem(a.start)[s + 1], a.n_tokens) - t0, a.max_tokens);
-    const int64_t j = slot - unit_base(a.start, s, G, BM, 1);
+    const UnitSeq seq = unit_seq(a.start, a.n_seqs, slot, G, BM, 1);
+    const int t0 = max(seq.start, 0), n = min(min(seq.end, a.n_tokens) - t0, a.max_tokens);
+    const int64_t j = slot - unit_base(seq.start, seq.s, G, BM, 1);
     if (n <= 0 || j < 0 || j * BM >= (int64_t)n * G) return;
     const int R = n * G, r0 = (int)j * BM, wr0 = r0 + wave % RG * 32;
     const int part = wave / RG % KS, dim0 = wave / (RG * KS) * (HD / SPLIT);              // this wave's keys of a tile, and dims

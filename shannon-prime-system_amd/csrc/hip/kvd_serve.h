@@ -70,21 +70,23 @@ template <int N> __device__ __forceinline__ void store_values(Bf16 *p, const flo
 // each sequence.  Without a list of units, sequence s gets those from
 // floor(mul start[s] / UNIT) + spare s on: a sequence with n of them has at most floor(n / UNIT) +
 // spare where spare covers its cut ends, so ranges do not overlap, and `spare` units a sequence stay empty.
-__device__ __forceinline__ int64_t unit_base(const int32_t *start, int s, int mul, int unit, int spare) {
-    return (int64_t)gmem(start)[s] * mul / unit + (int64_t)spare * s;
+__device__ __forceinline__ int64_t unit_base(int start, int s, int mul, int unit, int spare) {
+    return (int64_t)start * mul / unit + (int64_t)spare * s;
 }
-// The last sequence whose units start at or before u: each lane of a wave tries one, up to 64
-// sequences with one load, 4096 with two (a search by halves waits for one load after another,
-// 1.5 us for 9 sequences).
-__device__ __forceinline__ int unit_seq(const int32_t *start, int n_seqs, int64_t u, int mul, int unit, int spare) {
+// The last sequence whose units start at or before u, and its start and end: each lane of a wave tries one, up
+// to 64 sequences with one wait for memory, 4096 with two (a search by halves waits for one load after
+// another, 1.5 us for 9 sequences).
+struct UnitSeq { int s, start, end; };
+__device__ __forceinline__ UnitSeq unit_seq(const int32_t *start, int n_seqs, int64_t u, int mul, int unit, int spare) {
     const int lane = threadIdx.x & 63;
-    int s = 0;
+    UnitSeq q{};
     for (int step = n_seqs > 64 ? 64 : 1; step; step /= 64) {
-        const int t = s + lane * step;
-        const uint64_t before = __ballot(t < n_seqs && unit_base(start, t, mul, unit, spare) <= u);
-        s += (before ? 63 - __builtin_clzll(before) : 0) * step;
+        const int t = min(q.s + lane * step, n_seqs - 1), from = gmem(start)[t], to = gmem(start)[t + 1];
+        const uint64_t before = __ballot(q.s + lane * step < n_seqs && unit_base(from, t, mul, unit, spare) <= u);
+        const int at = before ? 63 - __builtin_clzll(before) : 0;
+        q = {q.s + at * step, __builtin_amdgcn_readlane(from, at), __builtin_amdgcn_readlane(to, at)};
     }
-    return s;
+    return q;
 }
 
 // ---------------------------------------------------------------- checks (one block of arguments or another)
