@@ -389,8 +389,8 @@ __device__ __forceinline__ v16f mfma_halves(const Halves &a, const Halves &b, v1
 // Dims of 256 are shared by two waves, each 128 of the scores' products and of the output's columns,
 // who hand each other their parts of the scores through LDS, where K lay as it came (the next K is
 // sent for after that): one wave with all of them needs over 256 registers, so that a SIMD has no other
-// to work while it waits (2047 tokens of 16 and 8 heads with a window of 1024: 200 us; so 184, 167
-// at the rate of a library's f32 product, 62 at a third of the f16 one's).
+// to work while it waits (2047 tokens of 16 and 8 heads with a window of 1024: 200 us; so 165, 167
+// at the rate of a library's f32 product, 62 at a third of the bf16 one's).
 template <int HD, int RG, int KS>
 __global__ __launch_bounds__(64 * RG * KS * prompt_split(HD), 2) void k_prompt32(sp_hipkv_prompt_args a, int slots) {
     constexpr int SPLIT = prompt_split(HD), NW = RG * KS * SPLIT, BN = 32 * KS, BM = 32 * RG, NS = HD / SPLIT / 16, DT = HD / SPLIT / 32, C8 = HD / 8, RAW = BN * HD * 4, PIECE = BN * HD * 2, NC = BN * C8 / (64 * NW);
@@ -438,15 +438,14 @@ __global__ __launch_bounds__(64 * RG * KS * prompt_split(HD), 2) void k_prompt32
     float c;
     {
         const float *q = (const float *)a.q + (size_t)(t0 + tok) * a.q_stride + (size_t)(h * G + row % G) * HD + dim0 + 8 * half;
-        float x[8];
+        float x[NS][8];
         float big = 0.0f;                                                  // (a NaN makes its own way into the scores)
         #pragma unroll
-        for (int k = 0; k < NS; k++) {
-            load_values(q + 16 * k, x);
+        for (int k = 0; k < NS; k++) load_values(q + 16 * k, x[k]);
+        #pragma unroll
+        for (int k = 0; k < NS; k++)
             #pragma unroll
-            for (int i = 0; i < 8; i++) big = fmaxf(big, fabsf(x[i]));
-        }
-        asm volatile("" : : : "memory");                                  // read again, not kept: NS x 8 registers
+            for (int i = 0; i < 8; i++) big = fmaxf(big, fabsf(x[k][i]));
         big = fmaxf(big, other_half(big));
         if constexpr (SPLIT == 2) {                                        // one factor for both parts of a row
             ((float *)lds)[wave * 32 + l32] = big;
@@ -458,10 +457,7 @@ __global__ __launch_bounds__(64 * RG * KS * prompt_split(HD), 2) void k_prompt32
         const float up = sgn * row_up(e);
         c = (a.scale == 0 ? LOG2E_F : fabsf(a.scale) * LOG2E_F) * row_down(e);
         #pragma unroll
-        for (int k = 0; k < NS; k++) {
-            load_values(q + 16 * k, x);
-            Q[k] = halves_of([&](int i) { return x[i] * up; });
-        }
+        for (int k = 0; k < NS; k++) Q[k] = halves_of([&](int i) { return x[k][i] * up; });
     }
     const float slack = SLACK32 / c;
     v16f O[DT];
@@ -526,8 +522,8 @@ __global__ __launch_bounds__(64 * RG * KS * prompt_split(HD), 2) void k_prompt32
         const int key0 = tile * BN + part * 32;                            // this wave's keys
         const bool idle = key0 > w_last || key0 + 32 <= w_first - W + 1;   // none that a row of it attends
         // fragments are read NF products ahead, the first of V beside the last of K
-        constexpr int NF = 4, NVF = 2 * DT;
-        constexpr bool AHEAD = SPLIT == 1;                                 // (no registers for V's first fragments beside two waves' sums)
+        constexpr int NF = SPLIT == 2 && NW == 4 ? 6 : 4, NVF = 2 * DT;
+        constexpr bool AHEAD = SPLIT == 1 || NW == 4;                      // (two waves a SIMD, each with sums of 128 dims, have no registers for V's first)
         Halves F[NF];
         auto read_k = [&](int x) { return Halves{*(const h8 *)(lds + k_at[x]), *(const h8 *)(lds + k_at[x] + PIECE)}; };
         auto read_v = [&](int x) {
@@ -627,12 +623,12 @@ __global__ __launch_bounds__(64 * RG * KS * prompt_split(HD), 2) void k_prompt32
         for (int e = 0; e < 2; e++) P[e] = halves_of([&](int k) { return S[8 * e + k]; });
         if (!AHEAD) {
             #pragma unroll
-            for (int x = 0; x < NF; x++) F[x] = read_v(x);
+            for (int x = 0; x < NF; x++) F[(NS + x) % NF] = read_v(x);
         }
         #pragma unroll
         for (int x = 0; x < NVF; x++) {
-            O[x % DT] = mfma_halves(F[x % NF], P[x / DT], O[x % DT]);
-            if (x + NF < NVF) F[x % NF] = read_v(x + NF);
+            O[x % DT] = mfma_halves(F[(NS + x) % NF], P[x / DT], O[x % DT]);
+            if (x + NF < NVF) F[(NS + x) % NF] = read_v(x + NF);
             __builtin_amdgcn_sched_group_barrier(0x008, 3, 0);
             if (x + NF < NVF) __builtin_amdgcn_sched_group_barrier(0x100, 4, 0);
         }
@@ -699,19 +695,19 @@ template <typename T, int HD> hipError_t prompt_go(const sp_hipkv_prompt_args &a
     if constexpr (sizeof(T) == 4) {
         // Up to some workgroups a unit it is the way along the keys that takes the time, and a workgroup of eight
         // waves walks 64 keys (dims of 64: 128) in the time that four take for 32.  One sequence of n tokens,
-        // 16 and 8 heads of 128: 28 us for 30 at n = 250, 68 for 89 at 1000, 123 for 168 at 2000, but 21.3 for
-        // 20.3 at 130; 32 and 8 heads: 148 for 174 at 2000 (504 workgroups), 767 for 701 at 5000.  Dims of 64,
-        // 32 and 8 heads: 45 for 53 at 1000 (504), 129 for 101 at 2000.  Of short sequences the longer
-        // last tiles cost more: six of 50 to 400 tokens take 36 us for 41 (216) and 52.5 for 47.9 (384).
+        // 16 and 8 heads of 128: 18.1 us for 18.9 at n = 130, 65 for 88 at 1000, 118 for 163 at 2000; 32 and 8
+        // heads: 151 for 176 at 2000 (504 workgroups), 772 for 726 at 5000.  Dims of 64: 32 and 8 heads 11.9 for 11.9 at 130, 42 for 52 at 1000 (504), 123 for 99 at 2000.  Six of 50 to 400 tokens: 33 for 39.5
+        // (216), 46.6 for 45.9 (384).
         if constexpr (HD < 256) {
             constexpr int KS = HD == 128 ? 2 : 4, RG = 8 / KS;
             const int64_t units = prompt_slots(a, 32 * RG) * a.n_kv_heads;
-            if (a.max_tokens >= 192 && units <= (a.n_tokens >= (int64_t)256 * a.n_seqs ? 512 : 256)) return PROMPT_RUN((k_prompt32<HD, RG, KS>), 32 * RG, 512);
+            if (a.max_tokens >= 128 && units <= 512) return PROMPT_RUN((k_prompt32<HD, RG, KS>), 32 * RG, 512);
         }
         // Dims of 256: a unit holds one workgroup, and with no more than one for each the longest span is what counts,
-        // which 64 rows walk faster than 128: 16 and 8 heads 129 us for 156 at 1000 tokens, 280 for 303 at 2047 (256
-        // units of 128 rows), 485 for 388 at 2600.  With a window all spans are much the same, and it is their sum that
-        // counts from half as many on: 1024 of 1400 tokens 139 for 171, of 1788 219 for 174.
+        // which 64 rows walk faster than 128 (one wave a SIMD has registers for more fragments ahead): 16 and 8 heads
+        // 121 us for 146 at 1000 tokens, 260 for 283 at 2047 (256 units of 128 rows), 455 for 365 at 2600.  With a window
+        // all spans are much the same, and it is their sum that counts from half as many on: 1024 of 1400 tokens
+        // 130 for 160, of 1788 204 for 163.
         if constexpr (HD == 256) {
             const bool even = a.window && 3 * (int64_t)a.window < 2 * (int64_t)a.max_tokens;
             if ((int64_t)a.n_tokens * a.n_heads / 128 <= (even ? 128 : 256)) return PROMPT_RUN((k_prompt32<HD, 2, 1>), 64, 256);
