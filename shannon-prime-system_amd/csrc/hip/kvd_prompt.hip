@@ -717,10 +717,15 @@ template <typename T, int HD> hipError_t prompt_go(const sp_hipkv_prompt_args &a
     else if constexpr (HD == 256) return PROMPT_RUN((k_prompt16<HD, 2, 1, 1>), 64, 256);
     else {
         // A unit holds two workgroups of four waves: with fewer rows than half of them take, the keys of 64 rows
-        // are shared by four waves each, a workgroup of eight a unit (1000 tokens of 16 and 8 heads of
-        // 128: 19.0 us for 24.4; 500 of 32: 14.0 for 16.5; 1000 of 32, too many: 28.2 for 26.9; 130 tokens, too
-        // few keys: 9.5 for 9.3).
-        if (a.max_tokens >= 192 && prompt_slots(a, 64) * a.n_kv_heads <= 256) return PROMPT_RUN((k_prompt16<HD, 2, 4, 1>), 64, 512);
+        // are shared by four waves each, a workgroup of eight a unit.  One sequence of 16 and 8 heads of 128: 13.0
+        // us for 15.3 at 500 tokens, 21.7 for 27.4 at 1200; 32 and 8 heads: 13.5 for 15.8 at 500, 22.8, too many,
+        // for 21.9 at 800; 130 tokens, too few keys: 9.2 for 8.6.
+        if (a.max_tokens >= 192 && prompt_slots(a, 64) * a.n_kv_heads <= 304) return PROMPT_RUN((k_prompt16<HD, 2, 4, 1>), 64, 512);
+        // With fewer than all take, the keys of 128 rows by two: 16 and 8 heads 50.9 for 58.7 at 2800 tokens, 63.9 for 74.1 at
+        // 3300, 107.7 for 104.5 at 4500; 32 and 8 27.8 for 30.4 at 1200, 51.8 for 51.1 at 2000.  Short sequences' last tiles
+        // cost more (six of 50 to 400 tokens 22.5 for 18.7), and dims of 64 gain nothing (20.8 for 20.8, 36.1 for 32.7).
+        if constexpr (HD == 128)
+            if (a.n_tokens >= (int64_t)800 * a.n_seqs && prompt_slots(a, 128) * a.n_kv_heads <= 432) return PROMPT_RUN((k_prompt16<HD, 4, 2, 1>), 128, 512);
         return PROMPT_RUN((k_prompt16<HD, 4, 1, 2>), 128, 256);
     }
 #undef PROMPT_RUN

@@ -254,7 +254,7 @@ def test_prompt_large_values_of_small_weight(typ, hd, low):
 
 
 @pytest.mark.parametrize("typ", TYPES)
-@pytest.mark.parametrize("hd,n,nkv", [(64, 400, 48), (128, 300, 64), (128, 250, 160), (256, 230, 150)])
+@pytest.mark.parametrize("hd,n,nkv", [(64, 400, 48), (128, 300, 64), (128, 250, 160), (128, 900, 12), (256, 230, 150)])
 def test_prompt_long_with_many_heads(typ, hd, n, nkv):
     """Too many rows for a workgroup a unit."""
     Prompt(rng(25, hd), typ, hd, 1, [n], nkv=nkv).check()
