@@ -10,14 +10,16 @@
 // Everything is computed in 64 bits: the angle of position p is p freq, off by 2^-53 of
 // itself (in 32 bits it would be off by 0.008 at position 131072), and a code is the rounded
 // quotient itself, not that of a rounded value.  f64 runs at the rate of f32 here.  Sine and
-// cosine are Taylor series behind a reduction by multiples of pi / 2, for a lane's first position and for a
-// step of four (a quarter of its pairs in each of the four rows of lanes); the other rounds' follow by
-// turning.
+// cosine are Taylor series behind a reduction by multiples of pi / 2, for four positions and for a
+// step of four; the others' follow by turning.  Of long appends a workgroup takes one block of four q or k heads,
+// whose sines it forms once, in LDS; of short ones each wave forms its own (the step's by parts in its four rows of
+// lanes, none for single tokens).
 //
-// 4096 tokens of 32 and 8 heads of 128 in bf16 take 36.0 us, 20.8 at the rate of a large copy: about 5 of it
-// are sines (37 with all of them formed in every lane), as much is the other arithmetic, which a wave's loads
-// wait for.  (Four q heads a wave with the same sines: 38.6 us; what counts is rows on their way.)  16 and 8 heads of 256 in f32 to f32
-// rows, which need no scale first, run at 90 % of that rate.
+// 4096 tokens of 32 and 8 heads of 128 in bf16 take 34.7 us (36.4 with sines a head), 20.8 at the rate of a
+// large copy.  Without norm and rotation they take 30 to 32: waves load, compute and store by turns, and what
+// counts is how many rows are on their way.  (K's values formed again behind the scale, for fewer registers: 58 us for
+// 64, 3900 tokens of 16 and 8 heads of 256, but 36 here and 14.5 for 11.8, four prompts of 200.)  16
+// and 8 heads of 256 in f32 to f32 rows, which need no scale first, run at 88 % of a copy's rate.
 #include "kvd_serve.h"
 #include "kvd_vec.h"
 #include <algorithm>
@@ -25,6 +27,8 @@
 namespace kvd {
 
 namespace {
+
+typedef double v2d __attribute__((ext_vector_type(2)));
 
 // sin and cos of x, |x| below 2^30: x = n pi / 2 + r, |r| <= pi / 4 (a little more where n rounds),
 // series to r^15 / 15! and r^16 / 16!, whose next terms are below 2^-54
@@ -104,16 +108,23 @@ __device__ __forceinline__ uint32_t recode(uint32_t code, float ratio) { return 
 
 // Waves that share a block, two rounds each: of 8-bit rows of 256 dims one alone holds 64 values of 64 bits a lane
 // until the block's scale is known (3900 tokens of 16 and 8 heads 76 us for 71, 20 prompts of 40 30.3 for 27.9; of
-// 128 dims the sines formed twice cost more: 36.5 us for 44, 4096 tokens of 32 and 8 heads)
+// 128 dims, each wave with sines of its own, 36.5 us for 44, 4096 tokens of 32 and 8 heads)
 constexpr int block_waves(int rows, int hd) { return rows == SP_HIPKV_ROWS_BLOCK8 && hd == 256 ? 2 : 1; }
 
-// NB blocks a workgroup: 4, a page, or 1.
+// q and k heads by workgroups of HG
+template <int HG> __host__ __device__ constexpr int append_qk(const sp_hipkv_append_args &a) {
+    return ((a.q_out ? a.n_heads : 0) + a.n_kv_heads + HG - 1) / HG * HG;
+}
+
+// NB: 4, a page, or 1.
 template <typename T, int ROWS, int HD, int NB>
 __global__ __launch_bounds__(64 * NB * block_waves(ROWS, HD), 2) void k_append(sp_hipkv_append_args a, int seq_units) {
     constexpr int PP = HD / 32, H2 = HD / 2, UNIT = BLOCK8 * NB, WB = block_waves(ROWS, HD), NR = 4 / WB, NT = 64 * NB * WB;
     constexpr bool B8 = ROWS == SP_HIPKV_ROWS_BLOCK8;
     constexpr int COL = 16 * NB + 16;                                     // bytes of a column of V codes in LDS
-    __shared__ __align__(16) uint8_t s_code[B8 ? HD * COL : 16];
+    constexpr int HG = NB > 1 ? 4 : 1;                                    // heads of q and k of a workgroup
+    constexpr int CODES = B8 ? HD * COL : 16, SINES = NB > 1 ? 16 * H2 * 16 : 16;
+    __shared__ __align__(16) uint8_t s_code[CODES > SINES ? CODES : SINES];
     __shared__ float s_ratio;
     __shared__ double s_big[NB * WB];
     // this workgroup's sequence and unit of positions
@@ -134,19 +145,24 @@ __global__ __launch_bounds__(64 * NB * block_waves(ROWS, HD), 2) void k_append(s
     const int n = min(min(seq.end, a.n_tokens) - t0, min(a.max_tokens, a.max_positions - first)), end = first + n;
     const int p0 = (first / UNIT + j) * UNIT, lp = p0 / PAGE;
     if (n <= 0 || j < 0 || p0 >= end) return;
-    // q, k or v, and its head
-    int h = blockIdx.x, kind = 0;
-    const int nq = a.q_out ? a.n_heads : 0;
-    if (h >= nq) { h -= nq; kind = 1; }
-    if (kind == 1 && h >= a.n_kv_heads) { h -= a.n_kv_heads; kind = 2; }
-    const bool stored = kind && !(a.ring_pages && lp + a.ring_pages <= (end - 1) / PAGE);
-    if (!stored && !(kind == 0 || (kind == 1 && a.k_out))) return;
+    // q, k or v, and its head: of V a head's NB blocks, of q and k one block of HG heads, which share its sines
+    const int nq = a.q_out ? a.n_heads : 0, qk = append_qk<HG>(a), x0 = blockIdx.x;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), i = lane >> 4, l = lane & 15;
-    const int b0 = p0 + BLOCK8 * (wave / WB), r0 = wave % WB * NR, u = b0 / BLOCK8 % PAGE_BLOCKS;
+    int h = x0 - qk, kind = 2, blk = wave / WB;
+    if (x0 < qk) {
+        if constexpr (HG > 1) { h = x0 / HG * HG + blk; blk = x0 % HG; }
+        else h = x0;
+        kind = h >= nq;
+        if (kind) h -= nq;
+    }
+    const bool stored = kind && h < a.n_kv_heads && !(a.ring_pages && lp + a.ring_pages <= (end - 1) / PAGE);
+    if (kind == 2 && !stored) return;
+    const int b0 = p0 + BLOCK8 * blk, r0 = wave % WB * NR, u = b0 / BLOCK8 % PAGE_BLOCKS;
     const bool some = b0 < end && b0 + BLOCK8 > first;
-    if (!some && !(B8 && kind == 2) && !(WB > 1 && stored)) return;
+    if (!some && !(B8 && kind == 2)) return;                              // (of q and k all waves, of f32 rows of V without more barriers)
+    const bool mine = kind == 0 || stored || (a.k_out && h < a.n_kv_heads);
     uint8_t *page = stored ? (uint8_t *)gmem(table)[a.ring_pages ? lp % a.ring_pages : lp] : nullptr;
-    auto live = [&](int r) { const int p = b0 + 4 * (r0 + r) + i; return p >= first && p < end; };
+    auto live = [&](int r) { const int p = b0 + 4 * (r0 + r) + i; return mine && p >= first && p < end; };
     auto round_live = [&](int r) { return b0 + 4 * (r0 + r) < end && b0 + 4 * (r0 + r) + 4 > first; };
     const bool older = B8 && some && stored && first > b0;                // positions of the block from earlier calls
     auto row_of = [&](auto *p, int64_t stride, int r, int head) __attribute__((always_inline)) {
@@ -260,18 +276,37 @@ __global__ __launch_bounds__(64 * NB * block_waves(ROWS, HD), 2) void k_append(s
     }
     // the first round with tokens, from whose sines the others' are turned
     const int rounds0 = max((first - b0) / 4 - r0, 0);
+    v2d *s_sin = (v2d *)s_code;                                            // [position][pair % PP][pair / PP]: a row of lanes reads 256 bytes
     if (a.freq) {
-        #pragma unroll
-        for (int k = 0; k < PP; k++) turn((double)(b0 + 4 * (r0 + rounds0) + i) * gmem(a.freq)[l * PP + k], c[k], sn[k]);
-        if (rounds0 + 1 < NR && round_live(rounds0 + 1)) {                // the step's are the same in all four rows: each forms a part
-            constexpr int PART = PP > 4 ? PP / 4 : 1, ROWS_OF = PP / PART;
-            double cp[PART], sp[PART];
+        if constexpr (HG > 1) {
+            for (int id = threadIdx.x; id < 4 * H2; id += NT) {
+                const int pair = id % H2, at = id / H2 * H2 + pair % PP * 16 + pair / PP;
+                const double f = gmem(a.freq)[pair];
+                double c0, s0, c4, s4;
+                turn((double)(b0 + id / H2) * f, c0, s0);
+                turn(4.0 * f, c4, s4);
+                #pragma unroll
+                for (int r = 0; r < 4; r++) {
+                    s_sin[at + 4 * r * H2] = (v2d){c0, s0};
+                    const double t = fma(c0, c4, -(s0 * s4));
+                    s0 = fma(c0, s4, s0 * c4);
+                    c0 = t;
+                }
+            }
+            __syncthreads();
+        } else {
             #pragma unroll
-            for (int k = 0; k < PART; k++) turn(4.0 * gmem(a.freq)[l * PP + i % ROWS_OF * PART + k], cp[k], sp[k]);
-            #pragma unroll
-            for (int k = 0; k < PP; k++) {
-                cs[k] = __shfl(cp[k % PART], k / PART * 16 + l, 64);
-                ss[k] = __shfl(sp[k % PART], k / PART * 16 + l, 64);
+            for (int k = 0; k < PP; k++) turn((double)(b0 + 4 * (r0 + rounds0) + i) * gmem(a.freq)[l * PP + k], c[k], sn[k]);
+            if (rounds0 + 1 < NR && round_live(rounds0 + 1)) {            // the step's are the same in all four rows: each forms a part
+                constexpr int PART = PP > 4 ? PP / 4 : 1, ROWS_OF = PP / PART;
+                double cp[PART], sp[PART];
+                #pragma unroll
+                for (int k = 0; k < PART; k++) turn(4.0 * gmem(a.freq)[l * PP + i % ROWS_OF * PART + k], cp[k], sp[k]);
+                #pragma unroll
+                for (int k = 0; k < PP; k++) {
+                    cs[k] = __shfl(cp[k % PART], k / PART * 16 + l, 64);
+                    ss[k] = __shfl(sp[k % PART], k / PART * 16 + l, 64);
+                }
             }
         }
     }
@@ -281,7 +316,7 @@ __global__ __launch_bounds__(64 * NB * block_waves(ROWS, HD), 2) void k_append(s
     #pragma unroll
     for (int r = 0; r < NR; r++) {
         double (&v)[2 * PP] = y[B8 ? r : 0];
-        if (r > rounds0 && a.freq) {
+        if (HG == 1 && r > rounds0 && a.freq) {
             #pragma unroll
             for (int k = 0; k < PP; k++) {
                 const double t = fma(c[k], cs[k], -(sn[k] * ss[k]));
@@ -290,6 +325,13 @@ __global__ __launch_bounds__(64 * NB * block_waves(ROWS, HD), 2) void k_append(s
             }
         }
         if ((NB == 1 || WB > 1) && !round_live(r)) continue;
+        if (HG > 1 && a.freq) {
+            #pragma unroll
+            for (int k = 0; k < PP; k++) {
+                const v2d z = s_sin[(4 * (r0 + r) + i) * H2 + k * 16 + l];
+                c[k] = z[0]; sn[k] = z[1];
+            }
+        }
         #pragma unroll
         for (int k = 0; k < PP; k++) { v[k] = (double)x[r][0][k]; v[PP + k] = (double)x[r][1][k]; }
         if (nw) {
@@ -323,17 +365,16 @@ __global__ __launch_bounds__(64 * NB * block_waves(ROWS, HD), 2) void k_append(s
         }
     }
     if constexpr (B8) {
-        if (!stored) return;
         big = none == none ? big : INFINITY;
         big = bcast63(wave_to63(big, 0.0, [](double p, double q) { return fmax(p, q); }));
         float *scale_at = (float *)(page + (size_t)2 * a.n_kv_heads * PAGE * HD) + h * PAGE_BLOCKS + u;
-        const float was = older ? *scale_at : 0.0f;
-        if constexpr (WB > 1) {
+        const float was = stored && older ? *scale_at : 0.0f;
+        if constexpr (WB > 1) {                                            // (all waves, those of q too)
             if (lane == 0) s_big[wave] = big;
             __syncthreads();
             big = fmax(big, s_big[wave ^ 1]);
-            if (!some) return;
         }
+        if (!stored) return;
         const float sc = block_scale(scale_exp(big), older, was), ratio = was / sc;
         const double inv = 1.0 / (double)sc;
         if (lane == 0 && r0 == 0) *scale_at = sc;
@@ -390,7 +431,7 @@ template <typename T, int ROWS, int NB> hipError_t append_go(const sp_hipkv_appe
     int seq_units = 0;
     const int64_t slots = append_slots(a, BLOCK8 * NB, &seq_units);
     return op_launch(a.head_dim == 256 ? k_append<T, ROWS, 256, NB> : a.head_dim == 128 ? k_append<T, ROWS, 128, NB> : k_append<T, ROWS, 64, NB>,
-                     dim3((a.q_out ? a.n_heads : 0) + 2 * a.n_kv_heads, (uint32_t)slots), dim3(64 * NB * block_waves(ROWS, a.head_dim)), s, a, seq_units);
+                     dim3(append_qk<NB>(a) + a.n_kv_heads, (uint32_t)slots), dim3(64 * NB * block_waves(ROWS, a.head_dim)), s, a, seq_units);
 }
 template <typename T, int ROWS> hipError_t append_rows(const sp_hipkv_append_args &a, hipStream_t s) {
     return a.max_tokens <= BLOCK8 ? append_go<T, ROWS, 1>(a, s) : append_go<T, ROWS, 4>(a, s);
