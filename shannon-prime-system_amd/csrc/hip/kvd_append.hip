@@ -161,8 +161,9 @@ __global__ __launch_bounds__(64 * NB * block_waves(ROWS, HD), 2) void k_append(s
     const bool some = b0 < end && b0 + BLOCK8 > first;
     if (!some && !(B8 && kind == 2)) return;                              // (of q and k all waves, of f32 rows of V without more barriers)
     const bool mine = kind == 0 || stored || (a.k_out && h < a.n_kv_heads);
+    if (HG == 1 && !mine) return;
     uint8_t *page = stored ? (uint8_t *)gmem(table)[a.ring_pages ? lp % a.ring_pages : lp] : nullptr;
-    auto live = [&](int r) { const int p = b0 + 4 * (r0 + r) + i; return mine && p >= first && p < end; };
+    auto live = [&](int r) { const int p = b0 + 4 * (r0 + r) + i; return (HG == 1 || mine) && p >= first && p < end; };
     auto round_live = [&](int r) { return b0 + 4 * (r0 + r) < end && b0 + 4 * (r0 + r) + 4 > first; };
     const bool older = B8 && some && stored && first > b0;                // positions of the block from earlier calls
     auto row_of = [&](auto *p, int64_t stride, int r, int head) __attribute__((always_inline)) {
