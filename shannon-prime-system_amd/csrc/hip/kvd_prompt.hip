@@ -726,6 +726,13 @@ template <typename T, int HD> hipError_t prompt_go(const sp_hipkv_prompt_args &a
         // cost more (six of 50 to 400 tokens 22.5 for 18.7), and dims of 64 gain nothing (20.8 for 20.8, 36.1 for 32.7).
         if constexpr (HD == 128)
             if (a.n_tokens >= (int64_t)800 * a.n_seqs && prompt_slots(a, 128) * a.n_kv_heads <= 432) return PROMPT_RUN((k_prompt16<HD, 4, 2, 1>), 128, 512);
+        // Two rounds of workgroups of 256 rows, or many: K and V are fetched half as often.  32 and 8 heads 143 us for 151
+        // at 4000 tokens (504 of them), 505 for 520 at 8192 (1032), but 256 for 253 at 5500 (696); 16 and 8 257 for
+        // 281 at 8192 (520), 148 for 137 at 5500 (352).
+        if constexpr (HD == 128) {
+            const int64_t units = prompt_slots(a, 256) * a.n_kv_heads;
+            if (a.n_tokens >= (int64_t)2000 * a.n_seqs && units >= 432 && (units <= 528 || units >= 864)) return PROMPT_RUN((k_prompt16<HD, 8, 1, 2>), 256, 512);
+        }
         return PROMPT_RUN((k_prompt16<HD, 4, 1, 2>), 128, 256);
     }
 #undef PROMPT_RUN

@@ -8,7 +8,7 @@ import pytest
 import spkv
 import tree_ref
 from devmem import Dev, Stream, hip, sync
-from serve_ref import BLOCK, PAGE, Append, Cache8, Cached, Packed, Prompt, cache_attention, close, packed_start, prepared, prompt_attention
+from serve_ref import B, BLOCK, PAGE, U, Append, Cache8, Cached, Packed, Prompt, cache_attention, close, packed_start, prepared, prompt_attention
 
 pytestmark = pytest.mark.gpu
 F32, BF16, BLOCK8, ROWS = spkv.F32, spkv.BF16, spkv.ROWS_BLOCK8, spkv.ROWS_F32
@@ -258,6 +258,31 @@ def test_prompt_large_values_of_small_weight(typ, hd, low):
 def test_prompt_long_with_many_heads(typ, hd, n, nkv):
     """Too many rows for a workgroup a unit."""
     Prompt(rng(25, hd), typ, hd, 1, [n], nkv=nkv).check()
+
+
+@pytest.mark.parametrize("hd,window", [(128, 0), (128, 300)])
+def test_prompt_of_many_workgroups(hd, window):
+    """One sequence whose rows fill the device more than once; a few of its heads and tokens are compared."""
+    g = rng(27, window)
+    n, nkv = 2000, 60
+    p = Prompt(g, BF16, hd, 1, [n], nkv=nkv, window=window)
+    got, few = p.run(), [0, 7, nkv - 1]
+    q, k, v = (x.values()[:, few] for x in (p.q, p.k, p.v))
+    for t in (0, 1, 63, 64, 255, 256, 257, 300, 1023, 1500, n - 1):
+        lo = max(0, t - window + 1) if window else 0
+        want, tol = prompt_attention(q[lo:t + 1], k[lo:t + 1], v[lo:t + 1], [t + 1 - lo], 0, p.scale, BF16) if t < 300 else (None, None)
+        if want is None:                                    # the last token alone: the others' rows cost most of the time
+            for h in range(len(few)):
+                K, V, x = (a.astype(np.float64) for a in (k[lo:t + 1, h], v[lo:t + 1, h], q[t, h]))
+                z = K @ x * p.scale
+                w = np.exp(z - z.max())
+                w /= w.sum()
+                o, r = w @ V, w @ np.abs(V)
+                d = (6 * hd + 20) * U * p.scale * (np.abs(K) @ np.abs(x)).max() + 4 * U * np.abs(z - z.max()).max()
+                bound = ((4 * d + (12 * len(z) + 64) * U) * r + U * np.abs(o) + B * r) * (1 + B) + B * np.abs(o)
+                assert (np.abs(got[t, few[h]] - o) <= bound).all()
+        else:
+            assert (np.abs(got[t, few] - want[-1]) <= tol[-1]).all()
 
 
 @pytest.mark.parametrize("typ", TYPES)
