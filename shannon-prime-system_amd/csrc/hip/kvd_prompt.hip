@@ -58,20 +58,25 @@ __device__ __forceinline__ bool chunk_clean(v4u &c) {
 }
 __device__ __forceinline__ bool finite32(float x) { return (__float_as_uint(x) & 0x7F800000u) != 0x7F800000u; }
 
-// Joins the outputs of the KS parts of RG row groups (maxima m, sums l, exponents by c): the parts'
-// outputs pass LDS (RG KS 32 rows of 32 DT f32), each part's wave sums up every KS-th tile of
-// columns and hands its rows' quotients to put(column tile, index, 4 values).
+// Joins the outputs of the KS parts of RG row groups (maxima m, sums l, exponents by c): of the tiles of 32
+// columns each part's wave sums up every KS-th and hands its rows' quotients to put(column tile, index, 4
+// values).  Its own share of them stays in registers, the other parts' pass LDS, 4 KiB a tile and wave.
+constexpr int join_bytes(int rg, int ks, int dt) { return rg * (ks - 1) * dt * 4096; }
 template <int RG, int KS, int DT, typename Put>
 __device__ __forceinline__ void join_parts(v16f (&O)[DT], float m, float l, float c, uint8_t *lds, v2f (*s_ml)[32], int wave, int lane, Put &&put) {
     v4f *x = (v4f *)lds;
+    const int rg = wave % RG, part = wave / RG;
+    auto at = [&](int d, int k, int i) { return (((d * (KS - 1) + k - (k > d % KS)) * RG + rg) * 4 + i) * 64 + lane; };
+    auto own = [&](int d, int i) { return (v4f){O[d][4 * i], O[d][4 * i + 1], O[d][4 * i + 2], O[d][4 * i + 3]}; };
     if (lane < 32) s_ml[wave][lane] = (v2f){m, l};
     __syncthreads();                                                       // K and V are read
     #pragma unroll
     for (int d = 0; d < DT; d++)
-        #pragma unroll
-        for (int i = 0; i < 4; i++) x[((wave * DT + d) * 4 + i) * 64 + lane] = (v4f){O[d][4 * i], O[d][4 * i + 1], O[d][4 * i + 2], O[d][4 * i + 3]};
+        if (d % KS != part) {
+            #pragma unroll
+            for (int i = 0; i < 4; i++) x[at(d, part, i)] = own(d, i);
+        }
     __syncthreads();
-    const int rg = wave % RG, part = wave / RG;
     float M = -INFINITY, L = 0.0f, f[KS];
     #pragma unroll
     for (int k = 0; k < KS; k++) M = fmaxf(M, s_ml[k * RG + rg][lane & 31][0]);
@@ -83,18 +88,17 @@ __device__ __forceinline__ void join_parts(v16f (&O)[DT], float m, float l, floa
     }
     const float inv = 1.0f / L;
     #pragma unroll
-    for (int d0 = 0; d0 < DT; d0 += KS) {
-        const int d = d0 + part;
-        if (d >= DT) break;
-        #pragma unroll
-        for (int i = 0; i < 4; i++) {
-            v4f y = {0, 0, 0, 0};
+    for (int d = 0; d < DT; d++)
+        if (d % KS == part) {
             #pragma unroll
-            for (int k = 0; k < KS; k++) y += x[(((k * RG + rg) * DT + d) * 4 + i) * 64 + lane] * f[k];
-            const float z[4] = {y[0] * inv, y[1] * inv, y[2] * inv, y[3] * inv};
-            put(d, 4 * i, z);
+            for (int i = 0; i < 4; i++) {
+                v4f y = {0, 0, 0, 0};
+                #pragma unroll
+                for (int k = 0; k < KS; k++) y += (k == d % KS ? own(d, i) : x[at(d, k, i)]) * f[k];
+                const float z[4] = {y[0] * inv, y[1] * inv, y[2] * inv, y[3] * inv};
+                put(d, 4 * i, z);
+            }
         }
-    }
 }
 
 // ---------------------------------------------------------------- bf16
@@ -325,6 +329,7 @@ __global__ __launch_bounds__(64 * RG * KS * prompt_split(HD), 2) void k_prompt16
             if (to < R) *gmem((v4u *)((Bf16 *)a.out + (size_t)(t0 + to / G) * a.out_stride + (size_t)(h * G + to % G) * HD + dim0 + 8 * ch)) = x;
         }
     } else {
+        static_assert(join_bytes(RG, KS, DT) <= 4 * TB, "the parts' outputs");
         join_parts<RG, KS, DT>(O, m, l, c, lds, s_ml, wave, lane, [&](int d, int i, const float (&x)[4]) {
             if (r < R) store_values(o + d * 32 + 2 * i, x);
         });
@@ -668,6 +673,7 @@ __global__ __launch_bounds__(64 * RG * KS * prompt_split(HD), 2) void k_prompt32
         for (int d = 0; d < DT; d++)
             #pragma unroll
             for (int i = 0; i < 16; i++) O[d][i] = ldexpf(O[d][i], 1 - ge);                 // each part has its own
+        static_assert(join_bytes(RG, KS, DT) <= 2 * RAW + 4 * PIECE, "the parts' outputs");
         join_parts<RG, KS, DT>(O, m, l, c, raw, s_ml, wave, lane, [&](int d, int i, const float (&x)[4]) {
             if (r < R) store_values(o + d * 32 + 2 * i, x);
         });
@@ -721,9 +727,9 @@ template <typename T, int HD> hipError_t prompt_go(const sp_hipkv_prompt_args &a
         // us for 15.3 at 500 tokens, 21.7 for 27.4 at 1200; 32 and 8 heads: 13.5 for 15.8 at 500, 22.8, too many,
         // for 21.9 at 800; 130 tokens, too few keys: 9.2 for 8.6.
         if (a.max_tokens >= 192 && prompt_slots(a, 64) * a.n_kv_heads <= 304) return PROMPT_RUN((k_prompt16<HD, 2, 4, 1>), 64, 512);
-        // With fewer than all take, the keys of 128 rows by two: 16 and 8 heads 50.9 for 58.7 at 2800 tokens, 63.9 for 74.1 at
-        // 3300, 107.7 for 104.5 at 4500; 32 and 8 27.8 for 30.4 at 1200, 51.8 for 51.1 at 2000.  Short sequences' last tiles
-        // cost more (six of 50 to 400 tokens 22.5 for 18.7), and dims of 64 gain nothing (20.8 for 20.8, 36.1 for 32.7).
+        // With fewer than all take, the keys of 128 rows by two: 16 and 8 heads 50.5 for 58.1 at 2800 tokens, 60.0 for 68.4 at
+        // 3300, 103 for 100.9 at 4500; 32 and 8 26.1 for 29.2 at 1200, 48.6 for 48.0 at 2000.  Short sequences' last tiles
+        // cost more (six of 50 to 400 tokens 13.7 for 13.2), and dims of 64 gain nothing (19.8 for 19.7 at 1200).
         if constexpr (HD == 128)
             if (a.n_tokens >= (int64_t)800 * a.n_seqs && prompt_slots(a, 128) * a.n_kv_heads <= 432) return PROMPT_RUN((k_prompt16<HD, 4, 2, 1>), 128, 512);
         // Two rounds of workgroups of 256 rows, or many: K and V are fetched half as often.  32 and 8 heads 143 us for 151

@@ -1,0 +1,61 @@
+"""Attention of packed prompts in the forms that longer calls take, against whole matrices
+in 64 bits; bounds as serve_ref.prompt_attention derives them."""
+import numpy as np
+import pytest
+
+import spkv
+from serve_ref import B, U, Prompt, packed_start
+
+pytestmark = pytest.mark.gpu
+F32, BF16 = spkv.F32, spkv.BF16
+
+
+def reference(p, heads=None):
+    """[tokens][the given q heads][hd] and the bound.  Values that are not finite are taken as 0: rows that
+    attend them are not compared."""
+    q, k, v = (np.where(np.isfinite(x), x, 0).astype(np.float64) for x in (p.q.values(), p.k.values(), p.v.values()))
+    NH, hd = q.shape[1:]
+    G, heads, scale = NH // k.shape[1], list(range(NH)) if heads is None else heads, p.scale
+    out, tol = np.zeros((sum(p.counts), len(heads), hd)), np.zeros((sum(p.counts), len(heads), hd))
+    for a, n in zip(packed_start(p.counts), p.counts):
+        t = np.arange(n)
+        seen = t <= t[:, None]
+        if p.window:
+            seen &= t > t[:, None] - p.window
+        for i, h in enumerate(heads):
+            x, K, V = q[a:a + n, h], k[a:a + n, h // G], v[a:a + n, h // G]
+            if not n:
+                continue
+            z = np.where(seen, x @ K.T * scale, -np.inf)
+            off = z.max(1, keepdims=True) - z
+            w = np.exp(-off)
+            w /= w.sum(1, keepdims=True)
+            d = (6 * hd + 20) * U * abs(scale) * np.where(seen, np.abs(x) @ np.abs(K).T, 0).max(1) + 4 * U * np.where(seen, off, 0).max(1)
+            if p.typ == F32:
+                d += 2.0 ** -39 * abs(scale) * np.where(seen, np.abs(x).max(1)[:, None] * np.abs(K).sum(1) + np.abs(x).sum(1)[:, None] * np.abs(K).max(1), 0).max(1)
+            o, r, m = w @ V, w @ np.abs(V), seen.sum(1)
+            e = (4 * d + (12 * m + 64) * U)[:, None] * r + U * np.abs(o)
+            if p.typ == F32:
+                big = w * np.abs(V).max(1)
+                e += (2.0 ** -31 * m * big.max(1) + 2.0 ** -39 * big.sum(1))[:, None]
+            else:
+                e = (e + B * r) * (1 + B) + B * np.abs(o)
+            out[a:a + n, i], tol[a:a + n, i] = o, e
+    return out, tol
+
+
+def check(p, heads=None, rows=None):
+    """The given rows [token][head] (all) are within the bound."""
+    got, (want, tol) = p.run(), reference(p, heads)
+    got = got if heads is None else got[:, heads]
+    ok = np.isfinite(got) & (np.abs(got - want) <= tol)
+    assert (ok if rows is None else ok[rows]).all()
+    return got
+
+
+# Keys of 128 rows shared by two waves each: the parts' outputs are joined in LDS
+@pytest.mark.parametrize("G,nkv,counts,window", [(1, 24, [900], 0), (1, 24, [900], 333), (2, 8, [1300], 0), (2, 8, [1300], 64), (4, 8, [1000], 0), (2, 8, [901, 0, 1700], 0),
+                                                 (2, 8, [3000], 0)])
+def test_two_parts(G, nkv, counts, window):
+    p = Prompt(np.random.default_rng([61, G, sum(counts)]), BF16, 128, G, counts, window=window, nkv=nkv)
+    check(p, None if sum(counts) < 1500 else [0, 5, G * nkv - 1])
