@@ -38,6 +38,8 @@ typedef __attribute__((address_space(3))) v4s lds4s;
 constexpr float LOG2E_F = 1.44269504088896341f;
 
 constexpr float SLACK = 16.0f;                                           // exponent (base 2) that a weight may reach
+// ... as a difference of scores; finite, so that the first score of a row moves its maximum whatever c
+__device__ __forceinline__ float slack_of(float exponent, float c) { return fminf(exponent / c, 3e38f); }
 
 // waves that share a row's dims
 constexpr int prompt_split(int hd) { return hd == 256 ? 2 : 1; }
@@ -128,7 +130,7 @@ __global__ __launch_bounds__(64 * RG * KS * prompt_split(HD), 2) void k_prompt16
     const int W = a.window ? a.window : INT32_MAX;
     const int first = r0 / G, last = (min(r0 + BM, R) - 1) / G, w_first = min(wr0, R - 1) / G, w_last = (min(wr0 + 32, R) - 1) / G;
     const int k0 = max(first - W + 1, 0) / BN, k1 = last / BN + 1;
-    const float sgn = a.scale > 0 ? 1.0f : a.scale < 0 ? -1.0f : 0.0f, c = a.scale == 0 ? LOG2E_F : fabsf(a.scale) * LOG2E_F, slack = SLACK / c;
+    const float sgn = a.scale > 0 ? 1.0f : a.scale < 0 ? -1.0f : 0.0f, c = a.scale == 0 ? LOG2E_F : fabsf(a.scale) * LOG2E_F, slack = slack_of(SLACK, c);
     const Bf16 *kp = (const Bf16 *)a.k + (size_t)t0 * a.k_stride + (size_t)h * HD, *vp = (const Bf16 *)a.v + (size_t)t0 * a.v_stride + (size_t)h * HD;
     // Direct loads fill LDS in order; a lane takes the 16-byte chunk whose place that is: chunks of a K
     // row lie in an order that spreads a column over the banks, 64-byte runs of V that of four rows
@@ -464,7 +466,7 @@ __global__ __launch_bounds__(64 * RG * KS * prompt_split(HD), 2) void k_prompt32
         #pragma unroll
         for (int k = 0; k < NS; k++) Q[k] = halves_of([&](int i) { return x[k][i] * up; });
     }
-    const float slack = SLACK32 / c;
+    const float slack = slack_of(SLACK32, c);
     v16f O[DT];
     const v16f zero = {0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0};
     #pragma unroll

@@ -59,3 +59,24 @@ def check(p, heads=None, rows=None):
 def test_two_parts(G, nkv, counts, window):
     p = Prompt(np.random.default_rng([61, G, sum(counts)]), BF16, 128, G, counts, window=window, nkv=nkv)
     check(p, None if sum(counts) < 1500 else [0, 5, G * nkv - 1])
+
+
+@pytest.mark.parametrize("typ", [F32, BF16])
+@pytest.mark.parametrize("hd", [64, 128, 256])
+@pytest.mark.parametrize("n", [100, 300])
+def test_zero_q(typ, hd, n):
+    """A head whose q is zero, padding tokens with zeros, and rows of the smallest numbers: the mean of the V that they attend."""
+    g = np.random.default_rng([62, hd, n])
+    q = g.standard_normal((n, 4, hd))
+    q[:, 1], q[40:90], q[:, 3] = 0, 0, q[:, 3] * 1e-38
+    check(Prompt(g, typ, hd, 1, [n], nkv=4, q=q))
+    check(Prompt(g, typ, hd, 4, [n - 20, 20], nkv=1, q=q, window=70))
+
+
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("scale", [1e-38, -1e-39, 2e-45])
+def test_tiny_scales(hd, scale):
+    """Keys shared by the waves of a workgroup, and a difference of scores that weighs anything beyond f32."""
+    for counts, nkv in ([300], 4), ([1300], 16):
+        p = Prompt(np.random.default_rng([63, hd]), BF16, hd, 1, counts, nkv=nkv, scale=scale)
+        check(p, None if nkv == 4 else [0, 15])
