@@ -462,7 +462,8 @@ __global__ __launch_bounds__(64 * RG * KS * prompt_split(HD), 2) void k_prompt32
         }
         const uint32_t e = row_exp(big);
         const float up = sgn * row_up(e);
-        c = (a.scale == 0 ? LOG2E_F : fabsf(a.scale) * LOG2E_F) * row_down(e);
+        // (at least f32's smallest number, which moves no weight: 0 times a masked score, -inf, would be NaN)
+        c = fmaxf((a.scale == 0 ? LOG2E_F : fabsf(a.scale) * LOG2E_F) * row_down(e), 1.4e-45f);
         #pragma unroll
         for (int k = 0; k < NS; k++) Q[k] = halves_of([&](int i) { return x[k][i] * up; });
     }

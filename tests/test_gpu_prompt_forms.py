@@ -80,3 +80,14 @@ def test_tiny_scales(hd, scale):
     for counts, nkv in ([300], 4), ([1300], 16):
         p = Prompt(np.random.default_rng([63, hd]), BF16, hd, 1, counts, nkv=nkv, scale=scale)
         check(p, None if nkv == 4 else [0, 15])
+
+
+@pytest.mark.parametrize("hd,n", [(64, 100), (64, 300), (128, 100), (128, 300), (256, 100), (256, 700)])
+@pytest.mark.parametrize("scale", [1e-8, -1e-20, 1e-38, 2e-45])
+def test_zero_q_and_tiny_scales(hd, n, scale):
+    """f32: what a difference of scores weighs, beside a q of zeros, is below f32's smallest number."""
+    g = np.random.default_rng([64, hd, n])
+    q = g.standard_normal((n, 2, hd))
+    q[:, 1], q[30:80], q[80:90] = 0, 0, q[80:90] * 1e-38
+    check(Prompt(g, F32, hd, 1, [n], nkv=2, q=q, scale=scale))
+    check(Prompt(g, F32, hd, 2, [n], nkv=1, q=q, scale=scale, window=50))
