@@ -491,7 +491,7 @@ typedef struct sp_hipkv_cache_args {
     int32_t max_tokens;             /* no sequence has more (at most 512) */
     int32_t max_positions;          /* cached + tokens of no sequence is more (at most 2^20) */
     int32_t window;                 /* 0: every position before */
-    int32_t ring_pages;             /* 0: full tables; a ring holds window + max_tokens positions and a page more */
+    int32_t ring_pages;             /* 0: full tables; a ring holds window + max_tokens positions and a page more, or max_positions */
     float   scale;                  /* 1 / sqrt(head_dim) in the models served */
     const int32_t *start;           /* [n_seqs + 1] ascending */
     const int32_t *cached;          /* [n_seqs] positions before the tokens */

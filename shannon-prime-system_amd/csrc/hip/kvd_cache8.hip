@@ -387,6 +387,10 @@ int cache_check(const char *who, const sp_hipkv_cache_args *a) {
     OP_NEED(a->max_positions >= 0 && a->max_positions <= 1 << 20, "max_positions outside [0, 2^20]");
     OP_NEED((int64_t)a->n_tokens * a->n_heads <= 1 << 22, "more than 2^22 rows (n_tokens x n_heads)");
     OP_NEED(a->window >= 0 && a->ring_pages >= 0, "negative window or ring_pages");
+    // positions from the first token's window to the last token, wherever in a page they begin
+    OP_NEED(!a->ring_pages || a->max_positions <= (int64_t)a->ring_pages * PAGE ||
+            (a->window && (int64_t)a->window + a->max_tokens - 1 + PAGE - 1 <= (int64_t)a->ring_pages * PAGE),
+            "ring_pages hold less than window + max_tokens positions and a page more");
     return 0;
 }
 int cache_check_arrays(const char *who, const sp_hipkv_cache_args *a, size_t need) {
