@@ -482,7 +482,8 @@ int  sp_hipkv_prompt_attention(const sp_hipkv_prompt_args *a, void *stream);
  * products with the codes are exact.
  * Positions that a token does not attend do not reach it whatever their codes and scales.
  * A scale that is not finite in a block that it attends, or a q value that is not, leaves
- * it without a finite value. */
+ * it without a finite value (magnitudes from 2^90 on in V may count as that, and scores that
+ * f32 does not hold). */
 typedef struct sp_hipkv_cache_args {
     int32_t n_heads, n_kv_heads;    /* at most 4096, and 16 q heads for each kv head */
     int32_t head_dim;               /* 64, 128 or 256 */

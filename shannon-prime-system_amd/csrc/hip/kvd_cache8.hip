@@ -220,7 +220,7 @@ __global__ __launch_bounds__(64 * CACHE_WAVES, HD == 256 ? 1 : 2) void k_cache(s
             }
         }
         const float ms = m == -INFINITY ? 0.0f : m;
-        float top = 0.0f;
+        float top = 0.0f;                                                 // (weights up to 2^16, V of 2^90, 2^20 positions: sums below 2^126)
         #pragma unroll
         for (int u = 0; u < 4; u++) {
             #pragma unroll
