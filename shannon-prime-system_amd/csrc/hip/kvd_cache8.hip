@@ -301,7 +301,7 @@ __global__ __launch_bounds__(64 * CACHE_WAVES, HD == 256 ? 1 : 2) void k_cache(s
         for (int w = 0; w < NW; w++) x += *(const v4f *)&s_o[w][k][c] * s_m[w][k];
         const float L = s_L[k];
         if (nsplit == 1) {
-            const float inv = L != 0.0f ? 1.0f / L : 0.0f;
+            const float inv = 1.0f / L;                                    // (0: no score is above -inf; 0 x inf is NaN)
             float y[4] = {x[0] * inv, x[1] * inv, x[2] * inv, x[3] * inv};
             store_values((T *)a.out + (size_t)(t0 + r / G) * a.out_stride + (size_t)(h * G + r % G) * HD + c, y);
         } else {
@@ -343,7 +343,7 @@ __global__ __launch_bounds__(NT) void k_cache_merge(sp_hipkv_cache_args a, int n
     if (grp) return;
     #pragma unroll
     for (int k = 1; k < NG; k++) x += s_x[k * (HD / 4) + c];
-    const float inv = s_L != 0.0f ? 1.0f / s_L : 0.0f;
+    const float inv = 1.0f / s_L;
     float y[4] = {x[0] * inv, x[1] * inv, x[2] * inv, x[3] * inv};
     store_values((T *)a.out + (size_t)token * a.out_stride + (row % a.n_heads) * HD + 4 * c, y);
 }

@@ -42,3 +42,20 @@ def test_values_above_the_limit(typ, n, e):
         got, (want, tol) = t.run(), t.want()
     fine = np.isfinite(got)
     assert (np.abs(got - want) <= tol)[fine].all()
+
+
+@pytest.mark.parametrize("typ", TYPES)
+@pytest.mark.parametrize("n", [1, 60, 9000])
+def test_scores_below_every_number(typ, n):
+    """A token all of whose scores are below f32's range has no finite value; its neighbours do."""
+    g = np.random.default_rng([72, n])
+    q = g.standard_normal((2, 2, 64))
+    q[0, 1] = -3e38
+    t = Cached(g, typ, 64, 2, [n - 1], [2], nkv=1, q=q, scale=1.0)
+    t.cache.k[:] = np.abs(t.cache.k.astype(np.int16)).clip(1, 127)
+    t.cache.s[:, 0] = 8
+    t.ready()
+    got, (want, tol) = t.run(), t.want()
+    assert not np.isfinite(got[0, 1]).any()
+    got[0, 1], want[0, 1], tol[0, 1] = 0, 0, 0
+    close(got, want, tol)
