@@ -473,6 +473,10 @@ typedef struct sp_hipkv_prompt_args {
     int64_t out_stride;
 } sp_hipkv_prompt_args;
 int  sp_hipkv_prompt_attention(const sp_hipkv_prompt_args *a, void *stream);
+/* How a call of these sizes is cut, for tests and timing (the pointers are not looked
+ * at): plan[0] the rows, a row being a token's q head, that a workgroup takes, plan[1]
+ * the keys of a tile, plan[2] the parts that they are shared by, plan[3] the waves. */
+int  sp_hipkv_prompt_attention_plan(const sp_hipkv_prompt_args *a, int32_t plan[4]);
 
 /* Attention of new tokens over the 8-bit cache, which holds their rows already (a decode
  * step's one token a sequence, or a piece of a prompt): token j of sequence s, at position

@@ -686,21 +686,23 @@ __global__ __launch_bounds__(64 * RG * KS * prompt_split(HD), 2) void k_prompt32
 // Units of `rows` rows that a call's rows may fall into, each a workgroup for every kv head
 int64_t prompt_slots(const sp_hipkv_prompt_args &a, int rows) { return (int64_t)a.n_tokens * (a.n_heads / a.n_kv_heads) / rows + a.n_seqs; }
 
-int prompt_check(const sp_hipkv_prompt_args *a) {
-    const char *who = "sp_hipkv_prompt_attention";
+// sizes; the pointers are not looked at
+int prompt_check(const char *who, const sp_hipkv_prompt_args *a) {
     if (serve_check(who, a)) return 1;
     OP_NEED(a->window >= 0, "negative window");
     OP_NEED(std::isfinite(a->scale), "scale is not finite");
-    if (!a->n_tokens) return 0;
-    OP_NEED(prompt_slots(*a, 64) * a->n_kv_heads < 1 << 23, "too many sequences, heads and tokens for one launch");      // (of 512 threads, 2^32 in all)
+    OP_NEED(!a->n_tokens || prompt_slots(*a, 64) * a->n_kv_heads < 1 << 23, "too many sequences, heads and tokens for one launch");      // (of 512 threads, 2^32 in all)
+    return 0;
+}
+int prompt_check_arrays(const char *who, const sp_hipkv_prompt_args *a) {
     OP_NEED(a->start, "null array");
     return serve_rows(who, a, a->q, a->q_stride, a->n_heads) || serve_rows(who, a, a->k, a->k_stride, a->n_kv_heads) ||
            serve_rows(who, a, a->v, a->v_stride, a->n_kv_heads) || serve_rows(who, a, a->out, a->out_stride, a->n_heads);
 }
 
-template <typename T, int HD> hipError_t prompt_go(const sp_hipkv_prompt_args &a, hipStream_t s) {
-#define PROMPT_RUN(K, ROWS, THREADS) \
-    op_launch(K, dim3((uint32_t)(prompt_slots(a, ROWS) * a.n_kv_heads)), dim3(THREADS), s, a, (int)prompt_slots(a, ROWS))
+// The form that a call takes: row groups of 32, parts of a tile's keys, tiles of 32 keys a part (f32: 1)
+struct PromptForm { int rg, ks, kt; };
+template <typename T, int HD> PromptForm prompt_form(const sp_hipkv_prompt_args &a) {
     if constexpr (sizeof(T) == 4) {
         // Up to some workgroups a unit it is the way along the keys that takes the time, and a workgroup of eight
         // waves walks 64 keys (dims of 64: 128) in the time that four take for 32.  One sequence of n tokens,
@@ -710,7 +712,7 @@ template <typename T, int HD> hipError_t prompt_go(const sp_hipkv_prompt_args &a
         if constexpr (HD < 256) {
             constexpr int KS = HD == 128 ? 2 : 4, RG = 8 / KS;
             const int64_t units = prompt_slots(a, 32 * RG) * a.n_kv_heads;
-            if (a.max_tokens >= 128 && units <= 512) return PROMPT_RUN((k_prompt32<HD, RG, KS>), 32 * RG, 512);
+            if (a.max_tokens >= 128 && units <= 512) return {RG, KS, 1};
         }
         // Dims of 256: a unit holds one workgroup, and with no more than one for each the longest span is what counts,
         // which 64 rows walk faster than 128 (one wave a SIMD has registers for more fragments ahead): 16 and 8 heads
@@ -719,49 +721,86 @@ template <typename T, int HD> hipError_t prompt_go(const sp_hipkv_prompt_args &a
         // 130 for 160, of 1788 204 for 163.
         if constexpr (HD == 256) {
             const bool even = a.window && 3 * (int64_t)a.window < 2 * (int64_t)a.max_tokens;
-            if ((int64_t)a.n_tokens * a.n_heads / 128 <= (even ? 128 : 256)) return PROMPT_RUN((k_prompt32<HD, 2, 1>), 64, 256);
+            if ((int64_t)a.n_tokens * a.n_heads / 128 <= (even ? 128 : 256)) return {2, 1, 1};
         }
-        return PROMPT_RUN((k_prompt32<HD, 4, 1>), 128, 256 * prompt_split(HD));
+        return {4, 1, 1};
     }
-    else if constexpr (HD == 256) return PROMPT_RUN((k_prompt16<HD, 2, 1, 1>), 64, 256);
+    else if constexpr (HD == 256) return {2, 1, 1};
     else {
         // A unit holds two workgroups of four waves: with fewer rows than half of them take, the keys of 64 rows
         // are shared by four waves each, a workgroup of eight a unit.  One sequence of 16 and 8 heads of 128: 13.0
         // us for 15.3 at 500 tokens, 21.7 for 27.4 at 1200; 32 and 8 heads: 13.5 for 15.8 at 500, 22.8, too many,
         // for 21.9 at 800; 130 tokens, too few keys: 9.2 for 8.6.
-        if (a.max_tokens >= 192 && prompt_slots(a, 64) * a.n_kv_heads <= 304) return PROMPT_RUN((k_prompt16<HD, 2, 4, 1>), 64, 512);
+        if (a.max_tokens >= 192 && prompt_slots(a, 64) * a.n_kv_heads <= 304) return {2, 4, 1};
         // With fewer than all take, the keys of 128 rows by two: 16 and 8 heads 50.5 for 58.1 at 2800 tokens, 60.0 for 68.4 at
         // 3300, 103 for 100.9 at 4500; 32 and 8 26.1 for 29.2 at 1200, 48.6 for 48.0 at 2000.  Short sequences' last tiles
         // cost more (six of 50 to 400 tokens 13.7 for 13.2), and dims of 64 gain nothing (19.8 for 19.7 at 1200).
         if constexpr (HD == 128)
-            if (a.n_tokens >= (int64_t)800 * a.n_seqs && prompt_slots(a, 128) * a.n_kv_heads <= 432) return PROMPT_RUN((k_prompt16<HD, 4, 2, 1>), 128, 512);
+            if (a.n_tokens >= (int64_t)800 * a.n_seqs && prompt_slots(a, 128) * a.n_kv_heads <= 432) return {4, 2, 1};
         // Two rounds of workgroups of 256 rows, or many: K and V are fetched half as often.  32 and 8 heads 143 us for 151
         // at 4000 tokens (504 of them), 505 for 520 at 8192 (1032), but 256 for 253 at 5500 (696); 16 and 8 257 for
         // 281 at 8192 (520), 148 for 137 at 5500 (352).
         if constexpr (HD == 128) {
             const int64_t units = prompt_slots(a, 256) * a.n_kv_heads;
-            if (a.n_tokens >= (int64_t)2000 * a.n_seqs && units >= 432 && (units <= 528 || units >= 864)) return PROMPT_RUN((k_prompt16<HD, 8, 1, 2>), 256, 512);
+            if (a.n_tokens >= (int64_t)2000 * a.n_seqs && units >= 432 && (units <= 528 || units >= 864)) return {8, 1, 2};
         }
-        return PROMPT_RUN((k_prompt16<HD, 4, 1, 2>), 128, 256);
+        return {4, 1, 2};
     }
-#undef PROMPT_RUN
 }
-template <typename T> hipError_t prompt_type(const sp_hipkv_prompt_args &a, hipStream_t s) {
-    return a.head_dim == 256 ? prompt_go<T, 256>(a, s) : a.head_dim == 128 ? prompt_go<T, 128>(a, s) : prompt_go<T, 64>(a, s);
+template <typename T, int HD> hipError_t prompt_go(const sp_hipkv_prompt_args &a, hipStream_t s) {
+    const PromptForm f = prompt_form<T, HD>(a);
+    const int64_t slots = prompt_slots(a, 32 * f.rg);
+    const dim3 grid((uint32_t)(slots * a.n_kv_heads)), wg(64 * f.rg * f.ks * prompt_split(HD));
+    auto run = [&](auto k) { return op_launch(k, grid, wg, s, a, (int)slots); };
+    if constexpr (sizeof(T) == 4) {
+        if constexpr (HD == 256) return f.rg == 2 ? run(k_prompt32<HD, 2, 1>) : run(k_prompt32<HD, 4, 1>);
+        else return f.ks > 1 ? run(k_prompt32<HD, HD == 128 ? 4 : 2, HD == 128 ? 2 : 4>) : run(k_prompt32<HD, 4, 1>);
+    }
+    else if constexpr (HD == 256) return run(k_prompt16<HD, 2, 1, 1>);
+    else {
+        if (f.ks == 4) return run(k_prompt16<HD, 2, 4, 1>);
+        if constexpr (HD == 128) {
+            if (f.ks == 2) return run(k_prompt16<HD, 4, 2, 1>);
+            if (f.rg == 8) return run(k_prompt16<HD, 8, 1, 2>);
+        }
+        return run(k_prompt16<HD, 4, 1, 2>);
+    }
+}
+// f(value type, std::integral_constant of the head dim) for the call's
+template <typename F> auto prompt_pick(const sp_hipkv_prompt_args &a, F &&f) {
+    auto dim = [&](auto t) {
+        return a.head_dim == 256 ? f(t, std::integral_constant<int, 256>{}) : a.head_dim == 128 ? f(t, std::integral_constant<int, 128>{}) : f(t, std::integral_constant<int, 64>{});
+    };
+    return a.type == SP_HIPKV_F32 ? dim(float{}) : dim(Bf16{});
 }
 
 }  // namespace
 
 hipError_t launch_prompt(const sp_hipkv_prompt_args &a, hipStream_t s) {
-    return a.type == SP_HIPKV_F32 ? prompt_type<float>(a, s) : prompt_type<Bf16>(a, s);
+    return prompt_pick(a, [&](auto t, auto hd) { return prompt_go<decltype(t), hd.value>(a, s); });
 }
 
 }  // namespace kvd
 
+extern "C" int sp_hipkv_prompt_attention_plan(const sp_hipkv_prompt_args *a, int32_t plan[4]) {
+    using namespace kvd;
+    const char *who = "sp_hipkv_prompt_attention_plan";
+    if (prompt_check(who, a)) return 1;
+    OP_NEED(plan, "null plan");
+    prompt_pick(*a, [&](auto t, auto hd) {
+        const PromptForm f = prompt_form<decltype(t), hd.value>(*a);
+        plan[0] = 32 * f.rg; plan[1] = 32 * f.ks * f.kt; plan[2] = f.ks; plan[3] = f.rg * f.ks * prompt_split(hd.value);
+        return 0;
+    });
+    return 0;
+}
+
 extern "C" int sp_hipkv_prompt_attention(const sp_hipkv_prompt_args *a, void *stream) {
     using namespace kvd;
-    if (prompt_check(a)) return 1;
+    const char *who = "sp_hipkv_prompt_attention";
+    if (prompt_check(who, a)) return 1;
     if (!a->n_tokens) return 0;
+    if (prompt_check_arrays(who, a)) return 1;
     OpDevice dev((hipStream_t)stream);
-    return op_done("sp_hipkv_prompt_attention", dev.err != hipSuccess ? dev.err : launch_prompt(*a, (hipStream_t)stream));
+    return op_done(who, dev.err != hipSuccess ? dev.err : launch_prompt(*a, (hipStream_t)stream));
 }

@@ -198,6 +198,7 @@ def kv():
         _sig(lib, "sp_hipkv_tree_attention_work", c_int, [ctypes.POINTER(TreeArgs), ctypes.POINTER(c_size_t)])
         _sig(lib, "sp_hipkv_tree_attention_plan", c_int, [ctypes.POINTER(TreeArgs), c_void_p])
         _sig(lib, "sp_hipkv_token_logprobs_work", c_int, [ctypes.POINTER(LogprobArgs), ctypes.POINTER(c_size_t)])
+        _sig(lib, "sp_hipkv_prompt_attention_plan", c_int, [ctypes.POINTER(PromptArgs), c_void_p])
         _sig(lib, "sp_hipkv_cache_attention_work", c_int, [ctypes.POINTER(CacheArgs), ctypes.POINTER(c_size_t)])
         _sig(lib, "sp_hipkv_block8_page_bytes", c_size_t, [c_int32, c_int32])
         _kv = lib
@@ -268,6 +269,13 @@ def append(args, stream=0):
 def prompt_attention(args, stream=0):
     """Causal attention of packed prompts (sp_hipkv_prompt_attention)."""
     check(kv().sp_hipkv_prompt_attention(args, stream), "sp_hipkv_prompt_attention")
+
+
+def prompt_attention_plan(args):
+    """(rows of a workgroup, keys of a tile, parts that they are shared by, waves) a call of these sizes takes."""
+    p = (c_int32 * 4)()
+    check(kv().sp_hipkv_prompt_attention_plan(args, p), "sp_hipkv_prompt_attention_plan")
+    return tuple(p)
 
 
 def cache_attention(args, stream=0):

@@ -54,8 +54,10 @@ def check(p, heads=None, rows=None):
 
 
 # Keys of 128 rows shared by two waves each: the parts' outputs are joined in LDS
-@pytest.mark.parametrize("G,nkv,counts,window", [(1, 24, [900], 0), (1, 24, [900], 333), (2, 8, [1300], 0), (2, 8, [1300], 64), (4, 8, [1000], 0), (2, 8, [901, 0, 1700], 0),
-                                                 (2, 8, [3000], 0)])
+TWO_PARTS = [(1, 24, [900], 0), (1, 24, [900], 333), (2, 8, [1300], 0), (2, 8, [1300], 64), (4, 8, [1000], 0), (2, 8, [901, 0, 1700], 0), (2, 8, [3000], 0)]
+
+
+@pytest.mark.parametrize("G,nkv,counts,window", TWO_PARTS)
 def test_two_parts(G, nkv, counts, window):
     p = Prompt(np.random.default_rng([61, G, sum(counts)]), BF16, 128, G, counts, window=window, nkv=nkv)
     check(p, None if sum(counts) < 1500 else [0, 5, G * nkv - 1])
@@ -91,3 +93,57 @@ def test_zero_q_and_tiny_scales(hd, n, scale):
     q[:, 1], q[30:80], q[80:90] = 0, 0, q[80:90] * 1e-38
     check(Prompt(g, F32, hd, 1, [n], nkv=2, q=q, scale=scale))
     check(Prompt(g, F32, hd, 2, [n], nkv=1, q=q, scale=scale, window=50))
+
+
+# type, head_dim, q heads for each kv head, kv heads, tokens, window: every form that is built (test_prompt_plans.py)
+FORMS = [
+    (F32, 64, 2, 2, [100, 27], 0), (F32, 64, 8, 16, [300], 0), (F32, 64, 8, 16, [300], 70), (F32, 64, 2, 2, [300, 9, 150], 0), (F32, 64, 3, 2, [700], 0),
+    (F32, 64, 2, 2, [500], 130), (F32, 128, 2, 2, [100, 27], 0), (F32, 128, 16, 16, [300], 0), (F32, 128, 16, 16, [300], 70), (F32, 128, 2, 2, [300, 9, 150], 0),
+    (F32, 128, 3, 2, [700], 0), (F32, 128, 2, 2, [500], 130), (F32, 256, 2, 2, [300, 9], 0), (F32, 256, 2, 2, [300, 9], 70), (F32, 256, 16, 7, [300], 0),
+    (F32, 256, 16, 4, [300], 70),
+    (BF16, 64, 2, 2, [100, 27], 0), (BF16, 64, 4, 8, [700], 0), (BF16, 64, 4, 8, [700], 130), (BF16, 64, 2, 2, [300, 9, 250], 0), (BF16, 64, 3, 2, [900], 200),
+    (BF16, 128, 2, 2, [100, 27], 0), (BF16, 128, 4, 8, [700], 0), (BF16, 128, 4, 8, [700], 130), (BF16, 128, 2, 2, [300, 9, 250], 0), (BF16, 128, 3, 2, [900], 200),
+    (BF16, 128, 1, 24, [900], 0), (BF16, 128, 4, 8, [1000], 900), (BF16, 128, 16, 4, [2000], 0), (BF16, 128, 16, 4, [2000], 300),
+    (BF16, 256, 2, 2, [300, 9], 0), (BF16, 256, 3, 2, [500], 70),
+]
+
+
+def form(case, **kw):
+    typ, hd, G, nkv, counts, window = case
+    return Prompt(np.random.default_rng([65, hd, G, nkv, sum(counts)]), typ, hd, G, counts, window=window, nkv=nkv, **kw)
+
+
+def few(p):
+    NH, G = p.q.shape[1], p.q.shape[1] // p.k.shape[1]
+    return sorted({0, G - 1, G % NH, NH // 2, NH - 1})
+
+
+@pytest.mark.parametrize("case", FORMS, ids=str)
+def test_forms(case):
+    p = form(case, pad=8, more_tokens=3)
+    check(p, few(p))
+
+
+@pytest.mark.parametrize("bad", [np.nan, np.inf, -np.inf])
+@pytest.mark.parametrize("case", FORMS, ids=str)
+def test_forms_beside_values_that_are_not_finite(case, bad):
+    """In V at one column of a token of the first kv head, in K at another token, in all of V at a third: rows that do
+    not attend them are as without, those that do are not finite (from K everywhere)."""
+    p = form(case)
+    n, W = p.counts[0], p.window or 1 << 30
+    k, v = p.k.values().copy(), p.v.values().copy()
+    one, key, all_of = n // 2 + 3, 3 * n // 4, 7 * n // 8
+    v[one, 0, 7], k[key, 0, 5], v[all_of, -1] = bad, np.nan, bad
+    p.k, p.v = type(p.k)(k, p.typ), type(p.v)(v, p.typ)
+    p.args.k, p.args.k_stride, p.args.v, p.args.v_stride = p.k.at, p.k.stride, p.v.at, p.v.stride
+    heads = few(p)
+    G, t = p.q.shape[1] // p.k.shape[1], np.arange(sum(p.counts))
+
+    def attends(token, kv):
+        return ((t >= token) & (t < min(token + W, n)))[:, None] & (np.array(heads) // G == kv)
+
+    gone = np.repeat(attends(key, 0)[..., None], p.q.shape[2], 2) | attends(all_of, p.k.shape[1] - 1)[..., None]
+    gone[..., 7] |= attends(one, 0)
+    got, (want, tol) = p.run()[:, heads], reference(p, heads)
+    assert not np.isfinite(got[gone]).any()
+    assert np.isfinite(got[~gone]).all() and (np.abs(got - want) <= tol)[~gone].all()
