@@ -703,24 +703,29 @@ int prompt_check_arrays(const char *who, const sp_hipkv_prompt_args *a) {
 // The form that a call takes: row groups of 32, parts of a tile's keys, tiles of 32 keys a part (f32: 1)
 struct PromptForm { int rg, ks, kt; };
 template <typename T, int HD> PromptForm prompt_form(const sp_hipkv_prompt_args &a) {
+    // A window well below the longest prompt: all spans are much the same, and what counts is how often the
+    // units are filled.  Waves that share keys, one workgroup of eight a unit, then pay in one round only, and for
+    // spans that are worth sharing; `span` is the longest.
+    const bool even = a.window && 3 * (int64_t)a.window < 2 * (int64_t)a.max_tokens;
+    const int span = even ? a.window : a.max_tokens;
     if constexpr (sizeof(T) == 4) {
         // Up to some workgroups a unit it is the way along the keys that takes the time, and a workgroup of eight
         // waves walks 64 keys (dims of 64: 128) in the time that four take for 32.  One sequence of n tokens,
         // 16 and 8 heads of 128: 18.1 us for 18.9 at n = 130, 65 for 88 at 1000, 118 for 163 at 2000; 32 and 8
         // heads: 151 for 176 at 2000 (504 workgroups), 772 for 726 at 5000.  Dims of 64: 32 and 8 heads 11.9 for 11.9 at 130, 42 for 52 at 1000 (504), 123 for 99 at 2000.  Six of 50 to 400 tokens: 33 for 39.5
-        // (216), 46.6 for 45.9 (384).
+        // (216), 46.6 for 45.9 (384).  In windows of 64, 128, 256 of 500 tokens of 16 and 8 heads 19.0, 22.4, 29.5 for 20.6, 25.8, 36.1 (64),
+        // of 1500 of 32 and 8 38.8, 46.3, 59.3 for 27.8, 34.6, 47.2 (376), dims of 64, of 500 13.5, 14.0, 17.1 for 11.3, 14.2, 20.0 (256), of
+        // 1000 25.3, 26.4, 31.9 for 12.1, 15.2, 20.9 (504).
         if constexpr (HD < 256) {
             constexpr int KS = HD == 128 ? 2 : 4, RG = 8 / KS;
             const int64_t units = prompt_slots(a, 32 * RG) * a.n_kv_heads;
-            if (a.max_tokens >= 128 && units <= 512) return {RG, KS, 1};
+            if (a.max_tokens >= 128 && span >= 32 * KS && units <= (even ? 256 : 512)) return {RG, KS, 1};
         }
         // Dims of 256: a unit holds one workgroup, and with no more than one for each the longest span is what counts,
         // which 64 rows walk faster than 128 (one wave a SIMD has registers for more fragments ahead): 16 and 8 heads
-        // 121 us for 146 at 1000 tokens, 260 for 283 at 2047 (256 units of 128 rows), 455 for 365 at 2600.  With a window
-        // all spans are much the same, and it is their sum that counts from half as many on: 1024 of 1400 tokens
-        // 130 for 160, of 1788 204 for 163.
+        // 121 us for 146 at 1000 tokens, 260 for 283 at 2047 (256 units of 128 rows), 455 for 365 at 2600.  Of even spans
+        // it is the sum that counts from half as many on: a window of 1024 of 1400 tokens 130 for 160, of 1788 204 for 163.
         if constexpr (HD == 256) {
-            const bool even = a.window && 3 * (int64_t)a.window < 2 * (int64_t)a.max_tokens;
             if ((int64_t)a.n_tokens * a.n_heads / 128 <= (even ? 128 : 256)) return {2, 1, 1};
         }
         return {4, 1, 1};
@@ -730,19 +735,22 @@ template <typename T, int HD> PromptForm prompt_form(const sp_hipkv_prompt_args 
         // A unit holds two workgroups of four waves: with fewer rows than half of them take, the keys of 64 rows
         // are shared by four waves each, a workgroup of eight a unit.  One sequence of 16 and 8 heads of 128: 13.0
         // us for 15.3 at 500 tokens, 21.7 for 27.4 at 1200; 32 and 8 heads: 13.5 for 15.8 at 500, 22.8, too many,
-        // for 21.9 at 800; 130 tokens, too few keys: 9.2 for 8.6.
-        if (a.max_tokens >= 192 && prompt_slots(a, 64) * a.n_kv_heads <= 304) return {2, 4, 1};
+        // for 21.9 at 800; 130 tokens, too few keys: 9.2 for 8.6.  Windows of 128, 256 of 500 tokens of 32 and 8 heads 12.1, 13.4 for
+        // 11.7, 13.9 (256 workgroups); 256, 512 of 1200 of 16 and 8 21.6, 21.0 for 14.1, 18.6 (304).
+        if (span >= 192 && prompt_slots(a, 64) * a.n_kv_heads <= (even ? 256 : 304)) return {2, 4, 1};
         // With fewer than all take, the keys of 128 rows by two: 16 and 8 heads 50.5 for 58.1 at 2800 tokens, 60.0 for 68.4 at
         // 3300, 103 for 100.9 at 4500; 32 and 8 26.1 for 29.2 at 1200, 48.6 for 48.0 at 2000.  Short sequences' last tiles
         // cost more (six of 50 to 400 tokens 13.7 for 13.2), and dims of 64 gain nothing (19.8 for 19.7 at 1200).
+        // Windows of 256, 512, 1024 of 2000 tokens of 16 and 8 heads 15.8, 19.3, 26.3 for 14.9, 19.5, 27.6 (256 workgroups), of 2800
+        // 28.0, 34.9, 42.1 for 19.6, 26.0, 31.0 (352).
         if constexpr (HD == 128)
-            if (a.n_tokens >= (int64_t)800 * a.n_seqs && prompt_slots(a, 128) * a.n_kv_heads <= 432) return {4, 2, 1};
+            if (a.n_tokens >= (int64_t)800 * a.n_seqs && span >= 512 && prompt_slots(a, 128) * a.n_kv_heads <= (even ? 256 : 432)) return {4, 2, 1};
         // Two rounds of workgroups of 256 rows, or many: K and V are fetched half as often.  32 and 8 heads 143 us for 151
         // at 4000 tokens (504 of them), 505 for 520 at 8192 (1032), but 256 for 253 at 5500 (696); 16 and 8 257 for
-        // 281 at 8192 (520), 148 for 137 at 5500 (352).
+        // 281 at 8192 (520), 148 for 137 at 5500 (352).  Not of even spans: a window of 1024 78.6 for 76.7 at 4000, 159.7 for 153.4 at 8192.
         if constexpr (HD == 128) {
             const int64_t units = prompt_slots(a, 256) * a.n_kv_heads;
-            if (a.n_tokens >= (int64_t)2000 * a.n_seqs && units >= 432 && (units <= 528 || units >= 864)) return {8, 1, 2};
+            if (!even && a.n_tokens >= (int64_t)2000 * a.n_seqs && units >= 432 && (units <= 528 || units >= 864)) return {8, 1, 2};
         }
         return {4, 1, 2};
     }

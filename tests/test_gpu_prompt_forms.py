@@ -54,7 +54,7 @@ def check(p, heads=None, rows=None):
 
 
 # Keys of 128 rows shared by two waves each: the parts' outputs are joined in LDS
-TWO_PARTS = [(1, 24, [900], 0), (1, 24, [900], 333), (2, 8, [1300], 0), (2, 8, [1300], 64), (4, 8, [1000], 0), (2, 8, [901, 0, 1700], 0), (2, 8, [3000], 0)]
+TWO_PARTS = [(1, 24, [900], 0), (1, 24, [900], 700), (2, 8, [1300], 0), (2, 8, [1700], 555), (4, 8, [1000], 0), (2, 8, [901, 0, 1700], 0), (2, 8, [3000], 0)]
 
 
 @pytest.mark.parametrize("G,nkv,counts,window", TWO_PARTS)
@@ -103,7 +103,8 @@ FORMS = [
     (F32, 256, 16, 4, [300], 70),
     (BF16, 64, 2, 2, [100, 27], 0), (BF16, 64, 4, 8, [700], 0), (BF16, 64, 4, 8, [700], 130), (BF16, 64, 2, 2, [300, 9, 250], 0), (BF16, 64, 3, 2, [900], 200),
     (BF16, 128, 2, 2, [100, 27], 0), (BF16, 128, 4, 8, [700], 0), (BF16, 128, 4, 8, [700], 130), (BF16, 128, 2, 2, [300, 9, 250], 0), (BF16, 128, 3, 2, [900], 200),
-    (BF16, 128, 1, 24, [900], 0), (BF16, 128, 4, 8, [1000], 900), (BF16, 128, 16, 4, [2000], 0), (BF16, 128, 16, 4, [2000], 300),
+    (BF16, 128, 1, 24, [900], 0), (BF16, 128, 4, 8, [1000], 900), (BF16, 128, 16, 4, [2000], 0), (BF16, 128, 16, 4, [2000], 300), (BF16, 128, 16, 4, [2000], 1400),
+    (BF16, 128, 1, 24, [900], 333), (BF16, 128, 2, 8, [1300], 64), (F32, 64, 4, 8, [700], 130),
     (BF16, 256, 2, 2, [300, 9], 0), (BF16, 256, 3, 2, [500], 70),
 ]
 

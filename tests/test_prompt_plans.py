@@ -37,3 +37,13 @@ def test_plan_refusals():
     assert spkv.kv().sp_hipkv_prompt_attention_plan(None, None) != 0
     a = spkv.PromptArgs(**GOOD)
     assert spkv.prompt_attention_plan(a)[0] and spkv.kv().sp_hipkv_prompt_attention_plan(a, None) != 0
+
+
+@pytest.mark.parametrize("typ,hd,G,nkv,n", [(BF16, 128, 2, 8, 1200), (BF16, 128, 2, 8, 2800), (BF16, 128, 4, 8, 4000), (BF16, 64, 2, 8, 1200), (F32, 64, 4, 8, 1000),
+                                            (F32, 128, 4, 8, 1900)])
+def test_keys_are_not_shared_in_short_windows_of_many_rows(typ, hd, G, nkv, n):
+    """Forms for few rows and long spans, and for very many rows: a window makes spans short, and workgroups are
+    more than the device runs at once."""
+    assert plan(typ, hd, G, nkv, [n], 0) != plan(typ, hd, G, nkv, [n], 128)
+    assert plan(typ, hd, G, nkv, [n], 128)[2] == 1 and plan(typ, hd, G, nkv, [n], 128)[0] == 128
+    assert plan(typ, hd, G, nkv, [n], n) == plan(typ, hd, G, nkv, [n], 0)
