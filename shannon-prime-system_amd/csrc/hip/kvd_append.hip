@@ -61,12 +61,13 @@ __device__ __forceinline__ double row_sum(double x) {
     step(std::integral_constant<int, 0x140>{});                           // row_mirror
     return x;
 }
-// 1 / sqrt(x): the instruction's estimate (2^-24 or better), then Newton's y + y (1 - x y^2) / 2 twice: 3/8 e^2 each
+// 1 / sqrt(x): the instruction's estimate (2^-24 or better), then Newton's y + y (1 - x y^2) / 2 twice: 3/8 e^2 each; 0 of
+// infinity, where Newton's step is 0 x inf
 __device__ __forceinline__ double inv_sqrt(double x) {
     double y = __builtin_amdgcn_rsq(x);
     #pragma unroll
     for (int i = 0; i < 2; i++) y = fma(y * 0.5, fma(-(x * y), y, 1.0), y);
-    return y;
+    return x == INFINITY ? 0.0 : y;
 }
 
 // y[] as f32, or as f32 whose rounding to bf16 is that of y: only where the nearest f32 lies half way between
