@@ -38,8 +38,9 @@ typedef __attribute__((address_space(3))) v4s lds4s;
 constexpr float LOG2E_F = 1.44269504088896341f;
 
 constexpr float SLACK = 16.0f;                                           // exponent (base 2) that a weight may reach
-// ... as a difference of scores; finite, so that the first score of a row moves its maximum whatever c
-__device__ __forceinline__ float slack_of(float exponent, float c) { return fminf(exponent / c, 3e38f); }
+// Whether the largest score of a tile moves a row's maximum m.  The slack is infinite where scores weigh next to
+// nothing; the first score moves a maximum of -inf then too, as -inf + inf is no number.
+__device__ __forceinline__ bool moves(float mx, float m, float slack) { return !(mx <= m + slack); }
 
 // waves that share a row's dims
 constexpr int prompt_split(int hd) { return hd == 256 ? 2 : 1; }
@@ -130,7 +131,7 @@ __global__ __launch_bounds__(64 * RG * KS * prompt_split(HD), 2) void k_prompt16
     const int W = a.window ? a.window : INT32_MAX;
     const int first = r0 / G, last = (min(r0 + BM, R) - 1) / G, w_first = min(wr0, R - 1) / G, w_last = (min(wr0 + 32, R) - 1) / G;
     const int k0 = max(first - W + 1, 0) / BN, k1 = last / BN + 1;
-    const float sgn = a.scale > 0 ? 1.0f : a.scale < 0 ? -1.0f : 0.0f, c = a.scale == 0 ? LOG2E_F : fabsf(a.scale) * LOG2E_F, slack = slack_of(SLACK, c);
+    const float sgn = a.scale > 0 ? 1.0f : a.scale < 0 ? -1.0f : 0.0f, c = a.scale == 0 ? LOG2E_F : fabsf(a.scale) * LOG2E_F, slack = SLACK / c;
     const Bf16 *kp = (const Bf16 *)a.k + (size_t)t0 * a.k_stride + (size_t)h * HD, *vp = (const Bf16 *)a.v + (size_t)t0 * a.v_stride + (size_t)h * HD;
     // Direct loads fill LDS in order; a lane takes the 16-byte chunk whose place that is: chunks of a K
     // row lie in an order that spreads a column over the banks, 64-byte runs of V that of four rows
@@ -270,7 +271,7 @@ __global__ __launch_bounds__(64 * RG * KS * prompt_split(HD), 2) void k_prompt16
         for (int u = 0; u < KT; u++)
             #pragma unroll
             for (int i = 0; i < 16; i++) mx = fmaxf(mx, S[u][i]);
-        if (__builtin_expect(__any(mx > m + slack), 0)) {
+        if (__builtin_expect(__any(moves(mx, m, slack)), 0)) {
             mx = fmaxf(mx, other_half(mx));
             const float mn = fmaxf(m, mx), al = mn == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f((m - mn) * c);
             m = mn;
@@ -359,8 +360,8 @@ template <typename X> __device__ __forceinline__ Halves halves_of(X &&x) {      
     }
     return {__builtin_bit_cast(h8, h), __builtin_bit_cast(h8, l)};
 }
-// of a row's largest magnitude the exponent e, and of that the factor 2^(141 - e) and its inverse
-__device__ __forceinline__ uint32_t row_exp(float big) { return min(max(__float_as_uint(big) >> 23, 16u), 254u); }
+// of a row's largest magnitude the exponent e (`least` at least), and of that the factor 2^(141 - e) and its inverse
+__device__ __forceinline__ uint32_t row_exp(float big, uint32_t least = 16) { return min(max(__float_as_uint(big) >> 23, least), 254u); }
 __device__ __forceinline__ float row_up(uint32_t e) { return __uint_as_float((268u - e) << 23); }
 __device__ __forceinline__ float row_down(uint32_t e) { return __uint_as_float((e - 14u) << 23); }
 // the largest over N = 8, 16 or 32 neighbouring lanes, of numbers that are not negative (as bits: one instruction a step)
@@ -460,14 +461,15 @@ __global__ __launch_bounds__(64 * RG * KS * prompt_split(HD), 2) void k_prompt32
             big = fmaxf(big, ((float *)lds)[(wave ^ RG * KS) * 32 + l32]);
             __syncthreads();
         }
-        const uint32_t e = row_exp(big);
+        // (the least exponent keeps c from vanishing, which would make NaN of a masked score, -inf x 0: c is 2^-126 or more, of a
+        // scale that is no normal number 2^-148; what a row of q so loses is below 2^-142 |k| in a score)
+        const uint32_t e = row_exp(big, max(142 - (int)(__float_as_uint(a.scale) >> 23 & 255), 16));
         const float up = sgn * row_up(e);
-        // (at least f32's smallest number, which moves no weight: 0 times a masked score, -inf, would be NaN)
-        c = fmaxf((a.scale == 0 ? LOG2E_F : fabsf(a.scale) * LOG2E_F) * row_down(e), 1.4e-45f);
+        c = (a.scale == 0 ? LOG2E_F : fabsf(a.scale) * LOG2E_F) * row_down(e);
         #pragma unroll
         for (int k = 0; k < NS; k++) Q[k] = halves_of([&](int i) { return x[k][i] * up; });
     }
-    const float slack = slack_of(SLACK32, c);
+    const float slack = SLACK32 / c;
     v16f O[DT];
     const v16f zero = {0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0};
     #pragma unroll
@@ -593,7 +595,7 @@ __global__ __launch_bounds__(64 * RG * KS * prompt_split(HD), 2) void k_prompt32
         #pragma unroll
         for (int i = 1; i < 16; i++) mx = fmaxf(mx, S[i]);
         float al = 1.0f, mt = 0.0f;
-        const bool moved = __any(mx > m + slack);
+        const bool moved = __any(moves(mx, m, slack));
         if (__builtin_expect(moved, 0)) {
             mx = fmaxf(mx, other_half(mx));
             const float mn = fmaxf(m, mx);
