@@ -493,7 +493,8 @@ typedef struct sp_hipkv_cache_args {
     int32_t head_dim;               /* 64, 128 or 256 */
     int32_t type;                   /* SP_HIPKV_F32, SP_HIPKV_BF16: q and out */
     int32_t n_seqs, n_tokens;       /* sequences (at most 4096), tokens of all of them (times n_heads at most 2^22) */
-    int32_t max_tokens;             /* no sequence has more (at most 512) */
+    int32_t max_tokens;             /* no sequence has more (at most 512; 2^22 workgroups in all: n_seqs n_kv_heads for every 16 rows of
+                                       max_tokens n_heads / n_kv_heads and every part of the span, one for 2^14 positions at least) */
     int32_t max_positions;          /* cached + tokens of no sequence is more (at most 2^20) */
     int32_t window;                 /* 0: every position before */
     int32_t ring_pages;             /* 0: full tables; a ring holds window + max_tokens positions and a page more, or max_positions */

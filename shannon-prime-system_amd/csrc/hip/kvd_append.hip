@@ -18,7 +18,8 @@
 // 4096 tokens of 32 and 8 heads of 128 in bf16 take 34.7 us (36.4 with sines a head), 20.8 at the rate of a
 // large copy.  Without norm and rotation they take 30 to 32: waves load, compute and store by turns, and what
 // counts is how many rows are on their way.  (K's values formed again behind the scale, for fewer registers: 58 us for
-// 64, 3900 tokens of 16 and 8 heads of 256, but 36 here and 14.5 for 11.8, four prompts of 200.)  16
+// 64, 3900 tokens of 16 and 8 heads of 256, but 36 here and 14.5 for 11.8, four prompts of 200; for 256 dims and long
+// appends alone it is left.)  16
 // and 8 heads of 256 in f32 to f32 rows, which need no scale first, run at 88 % of a copy's rate.
 #include "kvd_serve.h"
 #include "kvd_vec.h"

@@ -28,8 +28,8 @@ namespace {
 constexpr float LOG2E_F = 1.44269504088896341f;
 constexpr int CACHE_PAGES = 256, CACHE_WAVES = 4;                       // pages of a split at most; waves of a workgroup
 // Digits of q and the weights: three, and for bf16 values, which are off by 2^-9 themselves, two (15
-// bits: a third fewer products, three instructions for five to join them); the largest magnitude that
-// they hold, with room for carries.
+// bits: a third fewer products, three instructions for five to join them; a q value below 2^-7 of its row's
+// largest so loses bits that it has, 2^-16 of the largest); the largest magnitude that they hold, with room for carries.
 template <typename T> constexpr int DIG = sizeof(T) == 4 ? 3 : 2;
 template <typename T> constexpr float DIGITS = sizeof(T) == 4 ? 127 * 65536 : 127 * 256;
 // the number that products with digits 0, 1, .. make up

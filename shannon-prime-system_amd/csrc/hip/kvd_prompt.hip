@@ -227,7 +227,6 @@ __global__ __launch_bounds__(64 * RG * KS * prompt_split(HD), 2) void k_prompt16
         bf8 F[NF];
         auto read_k = [&](int x) { return *(const bf8 *)(lds + k_at[x % NS] + BUF * TB + x / NS * 32 * HD * 2); };
         auto read_v = [&](int x) {
-            typedef short v8s __attribute__((ext_vector_type(8)));
             const v4s y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4s *)(lds + v_at[x % DT] + (2 + BUF) * TB + 16 * (x / DT) * HD * 2));
             const v4s z = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4s *)(lds + v_at[x % DT] + (2 + BUF) * TB + (16 * (x / DT) + 8) * HD * 2));
             return __builtin_bit_cast(bf8, __builtin_shufflevector(y, z, 0, 1, 2, 3, 4, 5, 6, 7));
@@ -397,8 +396,9 @@ __device__ __forceinline__ v16f mfma_halves(const Halves &a, const Halves &b, v1
 // Dims of 256 are shared by two waves, each 128 of the scores' products and of the output's columns,
 // who hand each other their parts of the scores through LDS, where K lay as it came (the next K is
 // sent for after that): one wave with all of them needs over 256 registers, so that a SIMD has no other
-// to work while it waits (2047 tokens of 16 and 8 heads with a window of 1024: 200 us; so 165, 167
-// at the rate of a library's f32 product, 62 at a third of the bf16 one's).
+// to work while it waits (2047 tokens of 16 and 8 heads with a window of 1024: 200 us; so 178, 167
+// at the rate of a library's f32 product, 62 at a third of the bf16 one's).  Two waves a SIMD leave 256 registers: nine are
+// spilled here and where 128 dims are in two parts, seven where they are in one.
 template <int HD, int RG, int KS>
 __global__ __launch_bounds__(64 * RG * KS * prompt_split(HD), 2) void k_prompt32(sp_hipkv_prompt_args a, int slots) {
     constexpr int SPLIT = prompt_split(HD), NW = RG * KS * SPLIT, BN = 32 * KS, BM = 32 * RG, NS = HD / SPLIT / 16, DT = HD / SPLIT / 32, C8 = HD / 8, RAW = BN * HD * 4, PIECE = BN * HD * 2, NC = BN * C8 / (64 * NW);
@@ -537,7 +537,6 @@ __global__ __launch_bounds__(64 * RG * KS * prompt_split(HD), 2) void k_prompt32
         Halves F[NF];
         auto read_k = [&](int x) { return Halves{*(const h8 *)(lds + k_at[x]), *(const h8 *)(lds + k_at[x] + PIECE)}; };
         auto read_v = [&](int x) {
-            typedef short v8s __attribute__((ext_vector_type(8)));
             h8 V[2];
             #pragma unroll
             for (int z = 0; z < 2; z++) {

@@ -35,3 +35,16 @@ def ok(ring, span):
     except RuntimeError:
         return False
     return True
+
+
+@pytest.mark.parametrize("seqs,G,max_tokens,positions,fits", [(2048, 8, 512, 2000, True), (4096, 8, 512, 2000, False), (4096, 4, 512, 2000, True), (2049, 8, 512, 2000, False),
+                                                              (4096, 16, 1, 1 << 20, True), (4096, 16, 2, 1 << 20, True), (4096, 16, 3, 1 << 20, False)])
+def test_workgroups_of_a_call(seqs, G, max_tokens, positions, fits):
+    """n_seqs n_kv_heads for every 16 rows of a sequence and every part of its span: 2^22 of them at most."""
+    kw = dict(n_seqs=seqs, n_tokens=seqs, n_kv_heads=8, n_heads=8 * G, head_dim=64, max_tokens=max_tokens, max_positions=positions, q_stride=512 * G, out_stride=512 * G)
+    if fits:
+        spkv.cache_attention_work(cached(**kw))
+    else:
+        for call in (spkv.cache_attention, spkv.cache_attention_work):
+            with pytest.raises(RuntimeError, match="too many"):
+                call(cached(**kw))
